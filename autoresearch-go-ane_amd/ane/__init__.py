@@ -9,3 +9,4 @@ from .config import (Config, stories110m, tiny, decode_gqa, tiny_decode, is_ve_l
                      views, init_params, make_tokens, VE_GATE_CHANNELS)
 from .engine import Options, Open, Engine, EngineError  # noqa: F401
 from .decode import Decoder  # noqa: F401
+from .serve import KVBatch, KVCache8, LogitControls, NO_TOKEN  # noqa: F401

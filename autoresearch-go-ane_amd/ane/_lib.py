@@ -77,6 +77,41 @@ class LayerCache(C.Structure):
                                                                   ("ffn_taps_ready", C.c_int32)]
 
 
+class Kv8Cache(C.Structure):
+    """ane_kv8_cache (include/ane_serve.h)."""
+    _fields_ = [(n, C.c_void_p) for n in ("k", "v", "k_exp", "v_exp")] + [
+        (n, C.c_int32) for n in ("pages", "page_tokens", "kv_heads", "head_dim", "device")]
+
+
+class Kv8Batch(C.Structure):
+    """ane_kv8_batch (include/ane_serve.h)."""
+    _fields_ = [(n, C.c_void_p) for n in ("table", "start", "offsets")] + [
+        (n, C.c_int32) for n in ("table_stride", "table_pages", "nseq", "rows", "max_len", "max_new")]
+
+
+class Kv8AppendArgs(C.Structure):
+    """ane_kv8_append_args (include/ane_serve.h)."""
+    _fields_ = [(n, C.c_void_p) for n in ("q", "k", "v", "q_out", "cos", "sin")] + [
+        (n, C.c_int64) for n in ("q_row", "q_head", "k_row", "k_head", "v_row", "v_head", "q_out_row",
+                                 "q_out_head")] + [("heads", C.c_int32), ("positions", C.c_int32)]
+
+
+class Kv8AttendArgs(C.Structure):
+    """ane_kv8_attend_args (include/ane_serve.h)."""
+    _fields_ = [("q", C.c_void_p), ("out", C.c_void_p)] + [
+        (n, C.c_int64) for n in ("q_row", "q_head", "out_row", "out_head")] + [
+        ("heads", C.c_int32), ("scale", C.c_float), ("ws", C.c_void_p), ("ws_bytes", C.c_int64)]
+
+
+class LogitsArgs(C.Structure):
+    """ane_logits_args (include/ane_serve.h)."""
+    _fields_ = [(n, C.c_void_p) for n in ("logits", "out", "history", "lengths", "prompts", "repetition", "frequency",
+                                          "presence", "bias", "mask", "tokens")] + [
+        (n, C.c_int64) for n in ("logits_row", "out_row", "history_row", "bias_row", "mask_row")] + [
+        (n, C.c_int32) for n in ("rows", "vocab", "history_max", "device")] + [
+        ("ws", C.c_void_p), ("ws_bytes", C.c_int64)]
+
+
 class ProfEntry(C.Structure):
     _fields_ = [("launches", C.c_int64), ("ms", C.c_double), ("flops", C.c_double), ("bytes", C.c_double)]
 
@@ -156,6 +191,14 @@ SIGNATURES = {
     "ane_moe_run": (C.c_int, [_eng]),
     "ane_moe_read_output": (C.c_int, [_eng, _fp, C.POINTER(C.c_int32), _fp]),
     "ane_moe_last_ms": (C.c_double, [_eng]),
+    # the serving operators (include/ane_serve.h)
+    "ane_kv8_append": (C.c_int, [C.POINTER(Kv8Cache), C.POINTER(Kv8Batch), C.POINTER(Kv8AppendArgs), C.c_void_p]),
+    "ane_kv8_attend_workspace": (C.c_int64, [C.POINTER(Kv8Cache), C.POINTER(Kv8Batch), C.c_int32]),
+    "ane_kv8_attend": (C.c_int, [C.POINTER(Kv8Cache), C.POINTER(Kv8Batch), C.POINTER(Kv8AttendArgs), C.c_void_p]),
+    "ane_control_logits_workspace": (C.c_int64, [C.c_int32, C.c_int32]),
+    "ane_control_logits": (C.c_int, [C.POINTER(LogitsArgs), C.c_void_p]),
+    "ane_debug_kv8_item": (C.c_int, [C.POINTER(Kv8Cache), C.POINTER(Kv8Batch), C.c_int32, C.c_int32, C.c_int64,
+                                     C.POINTER(C.c_int32)]),
     # the per-object seam (include/ane_objects.h)
     "ane_seam_last_error": (C.c_char_p, []),
     "ane_layer_forward_open": (C.c_int, [C.c_int32] * 4 + [C.POINTER(LayerWeights), C.POINTER(C.c_void_p)]),

@@ -20,15 +20,16 @@
 
 #include "../../include/ane_hip.h"
 #include "gemm.h"
+#include "op_error.h"
 #include "rowops.h"
 
 using namespace ane;
 
 namespace {
-
 thread_local std::string g_op_err;
+}
 
-int op_fail(int code, const char* fmt, ...) {
+int ane::op_fail(int code, const char* fmt, ...) {
   char buf[512];
   va_list ap;
   va_start(ap, fmt);
@@ -37,6 +38,8 @@ int op_fail(int code, const char* fmt, ...) {
   g_op_err = buf;
   return code;
 }
+
+namespace {
 
 constexpr size_t kAlign = 256;
 size_t up(size_t n) { return (n + kAlign - 1) & ~(kAlign - 1); }

@@ -1,0 +1,322 @@
+// Append to the paged 8-bit cache, with the rotation on the way
+// (ane_kv8_append), and the checks both cache operators share.
+//
+// Mathematics: include/ane_serve.h.  One block per (page that gets rows, kv
+// head) reads its keys and values, rotates the keys, takes the largest
+// magnitude of each side over the block, and writes codes; no other block
+// touches that page and head, so a page's rows from before can be rounded
+// again in place when its exponent rises.  Blocks behind the kv heads rotate
+// the queries of the same rows.
+#include <algorithm>
+
+#include "kv8.h"
+#include "op_error.h"
+
+namespace ane {
+
+namespace {
+
+constexpr int kThreads = 256;
+
+struct AppendArgs {
+  Kv8Batch b;
+  uint8_t *k, *v;
+  int8_t *k_exp, *v_exp;
+  const half_t *xq, *xk, *xv;
+  half_t* q_out;
+  const float *cos, *sin;
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head, qo_row, qo_head;
+};
+
+struct F8 {
+  float x[8];
+};
+
+__device__ __forceinline__ F8 load8(const half_t* p) {
+  const half8 h = ld_h8(p);
+  F8 f;
+#pragma unroll
+  for (int j = 0; j < 8; j++) f.x[j] = (float)h[j];
+  return f;
+}
+
+// the four pairs of 8 dimensions from d0 on, at position pos
+template <int DH>
+__device__ __forceinline__ F8 rotate8(const F8& f, const float* cs, const float* sn, int pos, int d0) {
+  const float4 c = *reinterpret_cast<const float4*>(cs + (size_t)pos * (DH / 2) + d0 / 2);
+  const float4 s = *reinterpret_cast<const float4*>(sn + (size_t)pos * (DH / 2) + d0 / 2);
+  const float cc[4] = {c.x, c.y, c.z, c.w}, ss[4] = {s.x, s.y, s.z, s.w};
+  F8 r;
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    r.x[2 * j] = f.x[2 * j] * cc[j] - f.x[2 * j + 1] * ss[j];
+    r.x[2 * j + 1] = f.x[2 * j + 1] * cc[j] + f.x[2 * j] * ss[j];
+  }
+  return r;
+}
+
+// into +-65504, by comparisons: NaN stays
+__device__ __forceinline__ void limit8(F8& f) {
+#pragma unroll
+  for (int j = 0; j < 8; j++) f.x[j] = f.x[j] > 65504.f ? 65504.f : f.x[j] < -65504.f ? -65504.f : f.x[j];
+}
+
+// largest magnitude as float bits, NaN counted as 0
+__device__ __forceinline__ uint32_t amax8(const F8& f, uint32_t m) {
+#pragma unroll
+  for (int j = 0; j < 8; j++) {
+    const uint32_t u = __float_as_uint(f.x[j]) & 0x7fffffffu;
+    m = max(m, u > 0x7f800000u ? 0u : u);
+  }
+  return m;
+}
+
+// 4 codes of x * inv, inv a power of two; top: 240 at exponent 8, else 448
+// (at which the exponent already holds every number)
+__device__ __forceinline__ uint32_t codes4(const float* x, float inv, float top) {
+  float y[4];
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    y[j] = x[j] * inv;
+    y[j] = y[j] > top ? top : y[j] < -top ? -top : y[j];
+  }
+  int c = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], c, true);
+}
+
+// 4 codes rounded again at a larger exponent
+__device__ __forceinline__ uint32_t again4(uint32_t c, float down) {
+  const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, false);
+  const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, true);
+  int r = __builtin_amdgcn_cvt_pk_fp8_f32(lo[0] * down, lo[1] * down, 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(hi[0] * down, hi[1] * down, r, true);
+}
+
+template <int DH>
+__global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs a) {
+  constexpr int CPR = DH / 8;  // chunks of 8 dimensions per row
+  constexpr int T = DH / 16;
+  extern __shared__ __attribute__((aligned(16))) uint8_t vbuf[];  // the page's V codes
+  __shared__ uint32_t top[2][kThreads / 64];
+  const Kv8Batch& b = a.b;
+  const int tid = threadIdx.x;
+  const int P = 1 << b.pshift;
+  const Kv8Span span = kv8_page_span(b, blockIdx.x);
+  if (span.n == 0) return;
+  const int nr = span.n, row0 = span.row, t0 = span.pos;
+
+  if ((int)blockIdx.y >= b.NKV) {  // a query head
+    const int h = blockIdx.y - b.NKV;
+    for (int c = tid; c < nr * CPR; c += kThreads) {
+      const int r = c / CPR, d0 = c % CPR * 8;
+      const F8 f = rotate8<DH>(load8(a.xq + (row0 + r) * a.q_row + h * a.q_head + d0), a.cos, a.sin, t0 + r, d0);
+      half8 o;
+#pragma unroll
+      for (int j = 0; j < 8; j++) o[j] = (half_t)f.x[j];
+      st_h8(a.q_out + (row0 + r) * a.qo_row + h * a.qo_head + d0, o);
+    }
+    return;
+  }
+
+  const int h = blockIdx.y;
+  const int id = kv8_page(b, span.seq, t0 >> b.pshift);
+  if (id < 0) return;
+  const half_t* xk = a.xk + row0 * a.k_row + h * a.k_head;
+  const half_t* xv = a.xv + row0 * a.v_row + h * a.v_head;
+  const size_t ph = (size_t)id * b.NKV + h;
+  uint8_t* kp = a.k + ph * P * DH;
+  uint8_t* vp = a.v + ph * P * DH;
+  const int r0 = t0 & (P - 1);
+  uint32_t mk = 0, mv = 0;
+  for (int c = tid; c < nr * CPR; c += kThreads) {
+    const int r = c / CPR, d0 = c % CPR * 8;
+    F8 fk = rotate8<DH>(load8(xk + r * a.k_row + d0), a.cos, a.sin, t0 + r, d0);
+    F8 fv = load8(xv + r * a.v_row + d0);
+    limit8(fk);
+    limit8(fv);
+    mk = amax8(fk, mk);
+    mv = amax8(fv, mv);
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    mk = max(mk, (uint32_t)__shfl_xor((int)mk, o, 64));
+    mv = max(mv, (uint32_t)__shfl_xor((int)mv, o, 64));
+  }
+  if ((tid & 63) == 0) {
+    top[0][tid >> 6] = mk;
+    top[1][tid >> 6] = mv;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kThreads / 64; w++) {
+    mk = max(mk, top[0][w]);
+    mv = max(mv, top[1][w]);
+  }
+  int ek = kv8_exponent(mk), ev = kv8_exponent(mv), ok = ek, ov = ev;
+  if (r0 > 0) {
+    ok = a.k_exp[ph];
+    ov = a.v_exp[ph];
+    ek = max(ek, ok);
+    ev = max(ev, ov);
+  }
+  __syncthreads();  // every thread has read the exponents before they change
+  if (tid == 0) {
+    a.k_exp[ph] = (int8_t)ek;
+    a.v_exp[ph] = (int8_t)ev;
+  }
+  const float ik = kv8_scale(-ek), iv = kv8_scale(-ev);
+  const float tk = ek == kKvExpMax ? 240.f : 448.f, tv = ev == kKvExpMax ? 240.f : 448.f;
+
+  if (ek > ok) {
+    const float down = kv8_scale(ok - ek);
+    uint32_t* w = reinterpret_cast<uint32_t*>(kp);
+    for (int c = tid; c < r0 * DH / 4; c += kThreads) w[c] = again4(w[c], down);
+  }
+  // V's units of 16 tokens from the first that changes to the last
+  const int u0 = ev > ov ? 0 : r0 >> 4, u1 = (r0 + nr - 1) >> 4;
+  if (ev > ov || (r0 & 15) || ((r0 + nr) & 15)) {
+    const uint32_t* src = reinterpret_cast<const uint32_t*>(vp);
+    uint32_t* dst = reinterpret_cast<uint32_t*>(vbuf);
+    const float down = kv8_scale(ov - ev);
+    for (int c = u0 * 4 * DH + tid; c < (u1 + 1) * 4 * DH; c += kThreads) {
+      uint32_t w = src[c];
+      // tokens tok .. tok + 3 of one dimension
+      const int tok = c / (4 * DH) * 16 + c % (4 * DH) / (16 * T) * 4;
+      if (ev > ov && tok < r0) {
+        const uint32_t z = again4(w, down);
+        const int n = min(r0 - tok, 4);
+        const uint32_t mine = n == 4 ? 0xffffffffu : (1u << (8 * n)) - 1;
+        w = (z & mine) | (w & ~mine);
+      }
+      dst[c] = w;
+    }
+    __syncthreads();
+  }
+  for (int c = tid; c < nr * CPR; c += kThreads) {
+    const int r = c / CPR, d0 = c % CPR * 8;
+    F8 fk = rotate8<DH>(load8(xk + r * a.k_row + d0), a.cos, a.sin, t0 + r, d0);
+    F8 fv = load8(xv + r * a.v_row + d0);
+    limit8(fk);
+    limit8(fv);
+    const uint2 ck = make_uint2(codes4(fk.x, ik, tk), codes4(fk.x + 4, ik, tk));
+    *reinterpret_cast<uint2*>(kp + (r0 + r) * DH + d0) = ck;
+    const int s16 = r0 + r;
+    uint8_t* vd = vbuf + (s16 >> 4) * 16 * DH + (s16 & 15) / 4 * 4 * DH + (s16 & 3);
+    const uint32_t cv[2] = {codes4(fv.x, iv, tv), codes4(fv.x + 4, iv, tv)};
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const int d = d0 + j;
+      vd[((d & 15) * T + (d >> 4)) * 4] = (uint8_t)(cv[j / 4] >> (8 * (j & 3)));
+    }
+  }
+  __syncthreads();
+  const uint4* src = reinterpret_cast<const uint4*>(vbuf);
+  uint4* dst = reinterpret_cast<uint4*>(vp);
+  for (int c = u0 * DH + tid; c < (u1 + 1) * DH; c += kThreads) dst[c] = src[c];
+}
+
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+}  // namespace
+
+int kv8_check(const char* op, const ane_kv8_cache* c, const ane_kv8_batch* b, Kv8Batch* out) {
+  if (!c || !b) return op_fail(ANE_ERR_ARG, "storiesane %s: no cache or batch", op);
+  if (!c->k || !c->v || !c->k_exp || !c->v_exp) return op_fail(ANE_ERR_ARG, "storiesane %s: null cache buffer", op);
+  if (!aligned16(c->k) || !aligned16(c->v))
+    return op_fail(ANE_ERR_ARG, "storiesane %s: k and v must be 16-byte aligned", op);
+  const int P = c->page_tokens;
+  if (P < 16 || P > 256 || (P & (P - 1)))
+    return op_fail(ANE_ERR_ARG, "storiesane %s: page_tokens=%d must be 16, 32, 64, 128 or 256", op, P);
+  if (c->head_dim != 64 && c->head_dim != 128)
+    return op_fail(ANE_ERR_ARG, "storiesane %s: head_dim=%d must be 64 or 128", op, c->head_dim);
+  if (c->pages < 1 || c->kv_heads < 1 || c->kv_heads > 1024)
+    return op_fail(ANE_ERR_ARG, "storiesane %s: pages=%d kv_heads=%d (pages at least 1, kv_heads 1..1024)", op,
+                   c->pages, c->kv_heads);
+  if (b->nseq < 0 || b->nseq > 65536 || b->rows < 0 || b->rows > (1 << 30))
+    return op_fail(ANE_ERR_ARG, "storiesane %s: nseq=%d want 0..65536, rows=%d want 0..%d", op, b->nseq, b->rows,
+                   1 << 30);
+  if (b->nseq > 0 && (!b->table || !b->start || !b->offsets))
+    return op_fail(ANE_ERR_ARG, "storiesane %s: null batch buffer", op);
+  if (b->table_pages < 1 || b->table_stride < b->table_pages || (int64_t)b->table_pages * P > (1 << 30))
+    return op_fail(ANE_ERR_ARG, "storiesane %s: table_pages=%d (at least 1, at most its stride %d and %d tokens)", op,
+                   b->table_pages, b->table_stride, 1 << 30);
+  if (b->max_len < 0 || b->max_new < 0)
+    return op_fail(ANE_ERR_ARG, "storiesane %s: max_len=%d max_new=%d", op, b->max_len, b->max_new);
+  int n = 0;
+  while ((1 << n) < P) n++;
+  *out = Kv8Batch{b->table, b->start, b->offsets, b->table_stride, b->table_pages, b->nseq, b->rows,
+                  c->pages, n, c->kv_heads};
+  return ANE_OK;
+}
+
+}  // namespace ane
+
+using namespace ane;
+
+extern "C" int ane_kv8_append(const ane_kv8_cache* cache, const ane_kv8_batch* batch, const ane_kv8_append_args* args,
+                              void* stream) {
+  const char* op = "kv8 append";
+  AppendArgs a;
+  int rc = kv8_check(op, cache, batch, &a.b);
+  if (rc) return rc;
+  if (!args) return op_fail(ANE_ERR_ARG, "storiesane %s: null arguments", op);
+  if (a.b.nseq == 0 || a.b.rows == 0) return ANE_OK;  // an empty tensor may have no address
+  if (!args->k || !args->v || !args->cos || !args->sin || args->heads < 0 ||
+      (args->heads > 0 && (!args->q || !args->q_out)))
+    return op_fail(ANE_ERR_ARG, "storiesane %s: null buffer", op);
+  const ane_kv8_append_args& g = *args;
+  const int64_t strides[] = {g.k_row, g.k_head, g.v_row, g.v_head, g.q_row, g.q_head, g.q_out_row, g.q_out_head};
+  for (int j = 0; j < (g.heads > 0 ? 8 : 4); j++)
+    if (strides[j] < 0 || strides[j] % 8)
+      return op_fail(ANE_ERR_ARG, "storiesane %s: stride %lld must be a multiple of 8", op, (long long)strides[j]);
+  if (!aligned16(g.k) || !aligned16(g.v) || !aligned16(g.cos) || !aligned16(g.sin) ||
+      (g.heads > 0 && (!aligned16(g.q) || !aligned16(g.q_out))))
+    return op_fail(ANE_ERR_ARG, "storiesane %s: buffers must be 16-byte aligned", op);
+  if (g.heads > 32768) return op_fail(ANE_ERR_ARG, "storiesane %s: heads=%d", op, g.heads);
+  if (g.positions < a.b.table_pages << a.b.pshift)
+    return op_fail(ANE_ERR_ARG, "storiesane %s: positions=%d must cover the table's %d", op, g.positions,
+                   a.b.table_pages << a.b.pshift);
+  if (g.heads > 0 && !kv8_apart(a.b.rows, g.q_out_row, g.heads, g.q_out_head, cache->head_dim))
+    return op_fail(ANE_ERR_ARG, "storiesane %s: rows of q_out overlap", op);
+  if (g.heads > 0 && g.q == g.q_out && (g.q_row != g.q_out_row || g.q_head != g.q_out_head))
+    return op_fail(ANE_ERR_ARG, "storiesane %s: q_out is q with other strides", op);
+  DeviceScope dev(cache->device);
+  if (dev.status() != hipSuccess)
+    return op_fail(ANE_ERR_HIP, "storiesane %s: device %d: %s", op, cache->device, hipGetErrorString(dev.status()));
+  a.k = (uint8_t*)cache->k; a.v = (uint8_t*)cache->v; a.k_exp = cache->k_exp; a.v_exp = cache->v_exp;
+  a.xq = (const half_t*)g.q; a.xk = (const half_t*)g.k; a.xv = (const half_t*)g.v; a.q_out = (half_t*)g.q_out;
+  a.cos = g.cos; a.sin = g.sin;
+  a.q_row = g.q_row; a.q_head = g.q_head; a.k_row = g.k_row; a.k_head = g.k_head; a.v_row = g.v_row;
+  a.v_head = g.v_head; a.qo_row = g.q_out_row; a.qo_head = g.q_out_head;
+  const int P = 1 << a.b.pshift;
+  const dim3 grid(kv8_count(a.b.nseq, a.b.rows, kv8_pages(P)), a.b.NKV + g.heads);
+  const size_t lds = (size_t)P * cache->head_dim;
+  if (cache->head_dim == 64)
+    hipLaunchKernelGGL(append_kernel<64>, grid, dim3(kThreads), lds, (hipStream_t)stream, a);
+  else
+    hipLaunchKernelGGL(append_kernel<128>, grid, dim3(kThreads), lds, (hipStream_t)stream, a);
+  const hipError_t h = hipGetLastError();
+  if (h != hipSuccess) return op_fail(ANE_ERR_HIP, "storiesane %s: %s", op, hipGetErrorString(h));
+  return ANE_OK;
+}
+
+extern "C" int ane_debug_kv8_item(const ane_kv8_cache* cache, const ane_kv8_batch* batch, int32_t tile_tokens,
+                                  int32_t pages, int64_t item, int32_t* out) {
+  const char* op = "debug kv8 item";
+  Kv8Batch b;
+  int rc = kv8_check(op, cache, batch, &b);
+  if (rc) return rc;
+  if (!out || tile_tokens < 1 || tile_tokens > 64 || b.nseq < 1)
+    return op_fail(ANE_ERR_ARG, "storiesane %s: tile_tokens=%d nseq=%d", op, tile_tokens, b.nseq);
+  const uint32_t n = kv8_count(b.nseq, b.rows, pages ? kv8_pages(1 << b.pshift) : kv8_tiles(tile_tokens));
+  if (item < 0 || item >= (int64_t)n)
+    return op_fail(ANE_ERR_ARG, "storiesane %s: item=%lld want below %u", op, (long long)item, n);
+  const Kv8Span s = pages ? kv8_page_span(b, (uint32_t)item) : kv8_tile_span(b, tile_tokens, (uint32_t)item);
+  out[0] = s.seq;
+  out[1] = s.row;
+  out[2] = s.n;
+  out[3] = s.pos;
+  out[4] = pages && s.n > 0 ? kv8_page(b, s.seq, s.pos >> b.pshift) : -1;
+  out[5] = (int)n;
+  return ANE_OK;
+}

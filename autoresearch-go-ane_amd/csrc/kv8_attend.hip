@@ -1,0 +1,484 @@
+// Attention over the paged 8-bit cache (ane_kv8_attend): prompts, chunks of
+// prompts and single tokens.
+//
+// Mathematics: out = softmax(scale Q K^T) V per key/value head, in one pass
+// over the keys with a running maximum and sum per row.  The rows of a tile
+// are (token, query head of the group), so one reading of K and V serves the
+// whole group.  Scores come transposed, S^T = K Q^T (MFMA 16x16x32, fp32
+// sums): a lane then holds, for one row, keys 4 g + j of every 16, and that is
+// what the second product's operand P^T takes, with V stored so that the same
+// lane finds the same four keys of its dimensions side by side: neither P nor
+// V moves between lanes or through LDS.  Codes become fp16 (exactly, page
+// exponent applied) in the registers.
+//
+// A block is one tile and one key/value head (and one part of the keys where
+// tiles are few); its four waves take steps of 64 keys in turn and meet once
+// at the end, in LDS.  There is no barrier in the loop.
+#include <algorithm>
+#include <type_traits>
+
+#include "kv8.h"
+#include "op_error.h"
+
+namespace ane {
+
+namespace {
+
+constexpr int kThreads = 256, kWaves = 4;
+constexpr int kStep = 64;                  // keys a wave takes at a time
+constexpr int kRound = kStep * kWaves;     // keys the block takes at a time
+
+struct AttendArgs {
+  Kv8Batch b;
+  const uint8_t *k, *v;
+  const int8_t *k_exp, *v_exp;
+  const half_t* q;
+  half_t* out;
+  int64_t q_row, q_head, out_row, out_head;
+  int G;        // query heads per key/value head
+  int tt;       // tokens per tile: tt * G <= rows of the tile
+  int tiles;    // items
+  int nsplit;   // parts that the keys of a tile are cut into, at most
+  float c;      // scale * log2(e)
+  float* part;  // [tiles][NKV][nsplit][tt * G][DH + 2]: sums, maximum, sum of exponentials
+};
+
+// The keys of a tile are cut into equal parts of whole rounds, at most nsplit.
+__device__ __forceinline__ int part_keys(int keys, int nsplit) {
+  const int n = (keys + nsplit - 1) / nsplit;
+  return (n + kRound - 1) / kRound * kRound;
+}
+
+__device__ __forceinline__ float xor16_max(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float xor32_max(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float xor16_sum(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float xor32_sum(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+__device__ __forceinline__ half8 join(half2v a, half2v b, half2v c, half2v d) {
+  half8 r;
+  r[0] = a[0]; r[1] = a[1]; r[2] = b[0]; r[3] = b[1]; r[4] = c[0]; r[5] = c[1]; r[6] = d[0]; r[7] = d[1];
+  return r;
+}
+
+// whether any of the four codes is NaN
+__device__ __forceinline__ bool has_nan(uint32_t w) {
+  const uint32_t x = (w & 0x7f7f7f7fu) ^ 0x7f7f7f7fu;  // a zero byte where NaN (bit 7 is clear)
+  return ((x - 0x01010101u) & 0x80808080u) != 0;
+}
+
+// One step's K and V, 16 keys (a unit) at a time: raw codes and the page's
+// exponents.  A unit that does not take part (past the end, page not there)
+// reads the pool's first page, which exists; its scores are masked and its
+// values cleared.
+template <int DH>
+struct Step {
+  u32x4 k[4][DH / 64], v[4][DH / 64];
+  float ks[4], vs[4];
+  bool there[4];
+};
+
+template <int DH, int NT>
+__global__ __launch_bounds__(kThreads, 2) void attend_kernel(AttendArgs a) {
+  constexpr int R = 16 * NT;    // rows of the tile
+  constexpr int NM = DH / 32;   // MFMAs along the head dimension
+  constexpr int ND = DH / 16;   // 16-dimension groups of the output
+  constexpr int LD = DH + 4;
+  __shared__ __attribute__((aligned(16))) float lds_o[kWaves][R][LD];
+  __shared__ float lds_m[kWaves][R], lds_l[kWaves][R];
+  const Kv8Batch& b = a.b;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 15, g = lane >> 4;
+  const int h = blockIdx.x % b.NKV;
+  const int rest = blockIdx.x / b.NKV;
+  const int sp = rest % a.nsplit;
+  const int tile = a.tiles - 1 - rest / a.nsplit;  // the longest rows of a prompt first
+  const Kv8Span span = kv8_tile_span(b, a.tt, tile);
+  if (span.n == 0) return;
+  const int rows = span.n * a.G;
+  const int kend = span.pos + span.n;  // keys of the tile's last token
+  const int pk = part_keys(kend, a.nsplit);
+  const int k0 = sp * pk;
+  if (k0 >= kend) return;
+  const int k1 = min(kend, k0 + pk);
+
+  // Q: row r = 16 t + col, dimensions 64 (m / 2) + 16 g + 8 (m % 2) + j
+  half8 q[NT][NM];
+  int lim[NT];  // the last key of the lane's row
+#pragma unroll
+  for (int t = 0; t < NT; t++) {
+    const int r = min(16 * t + col, rows - 1);
+    const int tok = r / a.G, hg = r - tok * a.G;
+    lim[t] = span.pos + tok;
+    const half_t* p = a.q + (span.row + tok) * a.q_row + (h * a.G + hg) * a.q_head + 16 * g;
+#pragma unroll
+    for (int m = 0; m < NM; m++) q[t][m] = ld_h8(p + 64 * (m >> 1) + 8 * (m & 1));
+  }
+
+  // Page ids and exponents of 64 pages from wbase on, one per lane.
+  const int* trow = b.table + (size_t)span.seq * b.table_stride;
+  int wbase = -(1 << 30), wid = -1, wexp = 0;
+  auto window = [&](int pg) {
+    wbase = pg;
+    const int p = pg + lane;
+    wid = -1;
+    if (p < b.table_pages && ((int64_t)p << b.pshift) < k1) {
+      wid = trow[p];
+      if ((unsigned)wid >= (unsigned)b.pages) wid = -1;
+    }
+    wexp = 0;
+    if (wid >= 0) {
+      const size_t e = (size_t)wid * b.NKV + h;
+      wexp = ((int)a.k_exp[e] & 0xff) | ((int)a.v_exp[e] & 0xff) << 8;
+    }
+  };
+  const size_t head_bytes = (size_t)DH << b.pshift;
+  const int kl = col * DH + 16 * g, vl = lane * (DH / 4);
+  auto fetch = [&](Step<DH>& s, int kb) {
+    if ((kb >> b.pshift) < wbase || ((kb + kStep - 1) >> b.pshift) >= wbase + 64) window(kb >> b.pshift);
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+      const int ku = kb + 16 * u;
+      const int w = (ku >> b.pshift) - wbase;
+      const int id = __builtin_amdgcn_readlane(wid, w), ex = __builtin_amdgcn_readlane(wexp, w);
+      s.there[u] = id >= 0 && ku < k1;
+      const size_t page = ((size_t)(s.there[u] ? id : 0) * b.NKV + h) * head_bytes;
+      const int slot = ku & ((1 << b.pshift) - 1);
+      const uint8_t* kp = a.k + page + slot * DH;
+      const uint8_t* vp = a.v + page + slot * DH;
+#pragma unroll
+      for (int x = 0; x < DH / 64; x++) {
+        s.k[u][x] = *reinterpret_cast<const u32x4*>(kp + kl + 64 * x);
+        s.v[u][x] = *reinterpret_cast<const u32x4*>(vp + vl + 16 * x);
+      }
+      s.ks[u] = kv8_scale((int8_t)(ex & 0xff));
+      s.vs[u] = kv8_scale((int8_t)(ex >> 8 & 0xff));
+    }
+  };
+
+  float m[NT], l[NT];
+  floatx4 o[ND][NT];
+#pragma unroll
+  for (int t = 0; t < NT; t++) {
+    m[t] = -INFINITY;
+    l[t] = 0.f;
+#pragma unroll
+    for (int d = 0; d < ND; d++) o[d][t] = floatx4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  auto step = [&](Step<DH>& s, int kb, auto edge_) {
+    constexpr bool EDGE = decltype(edge_)::value;
+    floatx4 sc[4][NT];
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+      half8 kf[NM];
+#pragma unroll
+      for (int x = 0; x < NM; x++) {
+        const uint32_t w0 = s.k[u][x >> 1][2 * (x & 1)], w1 = s.k[u][x >> 1][2 * (x & 1) + 1];
+        kf[x] = join(kv8_up<false>(w0, s.ks[u]), kv8_up<true>(w0, s.ks[u]), kv8_up<false>(w1, s.ks[u]),
+                     kv8_up<true>(w1, s.ks[u]));
+      }
+#pragma unroll
+      for (int t = 0; t < NT; t++) {
+        floatx4 c = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int x = 0; x < NM; x++) c = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[x], q[t][x], c, 0, 0, 0);
+        if (EDGE) {
+#pragma unroll
+          for (int j = 0; j < 4; j++)
+            if (!s.there[u] || kb + 16 * u + 4 * g + j > lim[t]) c[j] = -INFINITY;
+        }
+        sc[u][t] = c;
+      }
+    }
+    half8 pf[2][NT];
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+      float mx = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < 4; u++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) mx = fmaxf(mx, sc[u][t][j]);
+      mx = xor32_max(xor16_max(mx));
+      const float mn = fmaxf(m[t], mx * a.c);
+      const float mu = mn == -INFINITY ? 0.f : mn;  // no key yet: exp2(-inf) below, not exp2(nan)
+      const float al = __builtin_amdgcn_exp2f(m[t] - mu);
+      m[t] = mn;
+      float sum = 0.f;
+#pragma unroll
+      for (int u = 0; u < 4; u++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u][t][j], a.c, -mu));
+          sum += p;
+          pf[u >> 1][t][4 * (u & 1) + j] = (half_t)p;
+        }
+      l[t] = l[t] * al + sum;
+#pragma unroll
+      for (int d = 0; d < ND; d++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) o[d][t][j] *= al;
+    }
+    // values that no row of the tile attends to may be anything (rows not yet
+    // written): cleared.  NaN among those that some row attends to and some
+    // does not is taken out of the product and put back into the rows that
+    // attend to it.
+    bool nan = false;
+    if (EDGE) {
+#pragma unroll
+      for (int u = 0; u < 4; u++) {
+        const int first = kb + 16 * u + 4 * g;  // the lane's four keys
+        const int n = s.there[u] ? clampi(k1 - first, 0, 4) : 0;
+        const uint32_t mine = n == 4 ? 0xffffffffu : (1u << (8 * n)) - 1;
+#pragma unroll
+        for (int x = 0; x < DH / 64; x++)
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            s.v[u][x][j] &= mine;
+            nan |= has_nan(s.v[u][x][j]);
+          }
+      }
+      nan = __any(nan);
+    }
+#pragma unroll
+    for (int y = 0; y < 2; y++)
+#pragma unroll
+      for (int d = 0; d < ND; d++) {
+        const uint32_t w0 = s.v[2 * y][d >> 2][d & 3], w1 = s.v[2 * y + 1][d >> 2][d & 3];
+        half8 vf = join(kv8_up<false>(w0, s.vs[2 * y]), kv8_up<true>(w0, s.vs[2 * y]),
+                        kv8_up<false>(w1, s.vs[2 * y + 1]), kv8_up<true>(w1, s.vs[2 * y + 1]));
+        if (EDGE && nan) {
+          half8 isnan;
+#pragma unroll
+          for (int j = 0; j < 8; j++) {
+            const bool bad = vf[j] != vf[j];
+            isnan[j] = bad ? (half_t)1.f : (half_t)0.f;
+            if (bad) vf[j] = (half_t)0.f;
+          }
+#pragma unroll
+          for (int t = 0; t < NT; t++) {
+            half8 sees;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+              const int u = 2 * y + (j >> 2);
+              sees[j] = s.there[u] && kb + 16 * u + 4 * g + (j & 3) <= lim[t] ? (half_t)1.f : (half_t)0.f;
+            }
+            floatx4 n = {0.f, 0.f, 0.f, 0.f};
+            n = __builtin_amdgcn_mfma_f32_16x16x32_f16(isnan, sees, n, 0, 0, 0);
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+              if (n[j] > 0.f) o[d][t][j] = NAN;
+          }
+        }
+#pragma unroll
+        for (int t = 0; t < NT; t++) o[d][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[y][t], o[d][t], 0, 0, 0);
+      }
+  };
+
+  Step<DH> cur;
+  int kb = k0 + wave * kStep;
+  if (kb < k1) fetch(cur, kb);
+  while (kb < k1) {
+    Step<DH> nxt;
+    const int kn = kb + kRound;
+    if (kn < k1) fetch(nxt, kn);
+    const bool inner = kb + kStep - 1 <= span.pos && cur.there[0] && cur.there[1] && cur.there[2] && cur.there[3];
+    if (inner) step(cur, kb, std::false_type{});
+    else step(cur, kb, std::true_type{});
+    if (kn < k1) cur = nxt;
+    kb = kn;
+  }
+
+  // The waves meet: maximum over the waves, every wave's sums brought to it.
+#pragma unroll
+  for (int t = 0; t < NT; t++) {
+    l[t] = xor32_sum(xor16_sum(l[t]));
+    if (g == 0) lds_m[wave][16 * t + col] = m[t];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int t = 0; t < NT; t++) {
+    const int r = 16 * t + col;
+    const float mm = fmaxf(fmaxf(lds_m[0][r], lds_m[1][r]), fmaxf(lds_m[2][r], lds_m[3][r]));
+    const float al = __builtin_amdgcn_exp2f(m[t] - (mm == -INFINITY ? 0.f : mm));
+    if (g == 0) lds_l[wave][r] = l[t] * al;
+#pragma unroll
+    for (int d = 0; d < ND; d++)
+      *reinterpret_cast<floatx4*>(&lds_o[wave][r][16 * d + 4 * g]) = o[d][t] * al;
+  }
+  __syncthreads();
+  const bool whole = pk >= kend;
+  float* part = a.part + (((size_t)tile * b.NKV + h) * a.nsplit + sp) * ((size_t)a.tt * a.G * (DH + 2));
+  for (int c = tid; c < rows * (DH / 8); c += kThreads) {
+    const int r = c / (DH / 8), d0 = c % (DH / 8) * 8;
+    float x[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++)
+      x[j] = (lds_o[0][r][d0 + j] + lds_o[1][r][d0 + j]) + (lds_o[2][r][d0 + j] + lds_o[3][r][d0 + j]);
+    const float ls = (lds_l[0][r] + lds_l[1][r]) + (lds_l[2][r] + lds_l[3][r]);
+    if (whole) {
+      const float inv = ls == 0.f ? 0.f : 1.f / ls;
+      const int tok = r / a.G, hg = r - tok * a.G;
+      half8 y;
+#pragma unroll
+      for (int j = 0; j < 8; j++) y[j] = (half_t)(x[j] * inv);
+      st_h8(a.out + (span.row + tok) * a.out_row + (h * a.G + hg) * a.out_head + d0, y);
+    } else {
+      float* p = part + (size_t)r * (DH + 2);
+#pragma unroll
+      for (int j = 0; j < 8; j++) p[d0 + j] = x[j];
+      if (d0 == 0) {
+        p[DH] = fmaxf(fmaxf(lds_m[0][r], lds_m[1][r]), fmaxf(lds_m[2][r], lds_m[3][r]));
+        p[DH + 1] = ls;
+      }
+    }
+  }
+}
+
+// Joins the parts of a tile's keys; one block per tile and key/value head.
+template <int DH>
+__global__ __launch_bounds__(kThreads) void join_kernel(AttendArgs a) {
+  const Kv8Batch& b = a.b;
+  const int h = blockIdx.x % b.NKV, tile = blockIdx.x / b.NKV;
+  const Kv8Span span = kv8_tile_span(b, a.tt, tile);
+  if (span.n == 0) return;
+  const int kend = span.pos + span.n;
+  const int pk = part_keys(kend, a.nsplit);
+  if (pk >= kend) return;  // one part: the output is written
+  const int np = (kend + pk - 1) / pk;
+  const int rows = span.n * a.G;
+  const size_t stride = (size_t)a.tt * a.G * (DH + 2);
+  const float* part = a.part + ((size_t)tile * b.NKV + h) * a.nsplit * stride;
+  for (int c = threadIdx.x; c < rows * (DH / 8); c += kThreads) {
+    const int r = c / (DH / 8), d0 = c % (DH / 8) * 8;
+    const float* p = part + (size_t)r * (DH + 2);
+    float mm = -INFINITY;
+    for (int s = 0; s < np; s++) mm = fmaxf(mm, p[s * stride + DH]);
+    const float mu = mm == -INFINITY ? 0.f : mm;
+    float l = 0.f, x[8] = {};
+    for (int s = 0; s < np; s++) {
+      const float al = __builtin_amdgcn_exp2f(p[s * stride + DH] - mu);
+      l += p[s * stride + DH + 1] * al;
+#pragma unroll
+      for (int j = 0; j < 8; j++) x[j] += p[s * stride + d0 + j] * al;
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int tok = r / a.G, hg = r - tok * a.G;
+    half8 y;
+#pragma unroll
+    for (int j = 0; j < 8; j++) y[j] = (half_t)(x[j] * inv);
+    st_h8(a.out + (span.row + tok) * a.out_row + (h * a.G + hg) * a.out_head + d0, y);
+  }
+}
+
+struct Plan {
+  int nt = 0, tt = 0, nsplit = 0;
+  uint32_t tiles = 0;
+  int64_t bytes = 0;
+};
+
+int plan(const char* op, const Kv8Batch& b, const ane_kv8_batch& given, int DH, int heads, Plan* p) {
+  if (heads < 1 || heads % b.NKV || heads / b.NKV > kKvMaxGroup)
+    return op_fail(ANE_ERR_ARG, "storiesane %s: heads=%d must be 1..%d times kv_heads=%d", op, heads, kKvMaxGroup,
+                   b.NKV);
+  const int G = heads / b.NKV;
+  if (b.nseq == 0 || b.rows == 0) return ANE_OK;
+  // rows of the longest sequence, or of the mean one where that is not known
+  const int64_t most = (int64_t)G * (given.max_new ? std::min(given.max_new, b.rows) : (b.rows + b.nseq - 1) / b.nseq);
+  p->nt = most <= 16 ? 1 : most <= 32 || DH == 128 ? 2 : 4;
+  while (16 * p->nt < G) p->nt *= 2;
+  p->tt = 16 * p->nt / G;
+  p->tiles = kv8_count(b.nseq, b.rows, kv8_tiles(p->tt));
+  const int64_t blocks = (int64_t)p->tiles * b.NKV;
+  const int cap = b.table_pages << b.pshift;
+  const int len = given.max_len ? std::min(given.max_len, cap) : cap;
+  int64_t ns = std::max<int64_t>((1024 + blocks - 1) / blocks, p->nt == 1 ? (len + 2047) / 2048 : 1);
+  ns = std::min<int64_t>(ns, (len + kRound - 1) / kRound);
+  ns = std::max<int64_t>(1, std::min<int64_t>(ns, 64));
+  p->nsplit = (int)ns;
+  if (blocks * ns > 0x7fffffff)
+    return op_fail(ANE_ERR_ARG, "storiesane %s: rows=%d nseq=%d are too many for one launch", op, b.rows, b.nseq);
+  p->bytes = ns > 1 ? blocks * ns * p->tt * G * (DH + 2) * 4 : 0;
+  return ANE_OK;
+}
+
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+template <int DH>
+void launch(const AttendArgs& a, int nt, hipStream_t st) {
+  const dim3 grid((uint32_t)a.tiles * a.b.NKV * a.nsplit);
+  if (nt == 1) hipLaunchKernelGGL((attend_kernel<DH, 1>), grid, dim3(kThreads), 0, st, a);
+  else if (nt == 2) hipLaunchKernelGGL((attend_kernel<DH, 2>), grid, dim3(kThreads), 0, st, a);
+  else if constexpr (DH == 64) hipLaunchKernelGGL((attend_kernel<DH, 4>), grid, dim3(kThreads), 0, st, a);
+  if (a.nsplit > 1)
+    hipLaunchKernelGGL(join_kernel<DH>, dim3((uint32_t)a.tiles * a.b.NKV), dim3(kThreads), 0, st, a);
+}
+
+}  // namespace
+
+}  // namespace ane
+
+using namespace ane;
+
+extern "C" int64_t ane_kv8_attend_workspace(const ane_kv8_cache* cache, const ane_kv8_batch* batch, int32_t heads) {
+  const char* op = "kv8 attend workspace";
+  Kv8Batch b;
+  int rc = kv8_check(op, cache, batch, &b);
+  if (rc) return rc;
+  Plan p;
+  rc = plan(op, b, *batch, cache->head_dim, heads, &p);
+  return rc ? rc : p.bytes;
+}
+
+extern "C" int ane_kv8_attend(const ane_kv8_cache* cache, const ane_kv8_batch* batch, const ane_kv8_attend_args* args,
+                              void* stream) {
+  const char* op = "kv8 attend";
+  AttendArgs a;
+  int rc = kv8_check(op, cache, batch, &a.b);
+  if (rc) return rc;
+  if (!args) return op_fail(ANE_ERR_ARG, "storiesane %s: null arguments", op);
+  if (a.b.nseq == 0 || a.b.rows == 0) return ANE_OK;  // an empty tensor may have no address
+  if (!args->q || !args->out) return op_fail(ANE_ERR_ARG, "storiesane %s: null buffer", op);
+  const ane_kv8_attend_args& g = *args;
+  for (const int64_t s : {g.q_row, g.q_head, g.out_row, g.out_head})
+    if (s < 0 || s % 8)
+      return op_fail(ANE_ERR_ARG, "storiesane %s: stride %lld must be a multiple of 8", op, (long long)s);
+  if (!aligned16(g.q) || !aligned16(g.out) || !aligned16(g.ws))
+    return op_fail(ANE_ERR_ARG, "storiesane %s: buffers must be 16-byte aligned", op);
+  if (!(g.scale > 0.f) || !std::isfinite(g.scale))
+    return op_fail(ANE_ERR_ARG, "storiesane %s: scale=%g must be positive and finite", op, (double)g.scale);
+  Plan p;
+  rc = plan(op, a.b, *batch, cache->head_dim, g.heads, &p);
+  if (rc) return rc;
+  if (!kv8_apart(a.b.rows, g.out_row, g.heads, g.out_head, cache->head_dim))
+    return op_fail(ANE_ERR_ARG, "storiesane %s: rows of out overlap", op);
+  if (p.bytes > 0 && (!g.ws || g.ws_bytes < p.bytes))
+    return op_fail(ANE_ERR_ARG, "storiesane %s: workspace of %lld bytes, want %lld", op,
+                   (long long)(g.ws ? g.ws_bytes : 0), (long long)p.bytes);
+  DeviceScope dev(cache->device);
+  if (dev.status() != hipSuccess)
+    return op_fail(ANE_ERR_HIP, "storiesane %s: device %d: %s", op, cache->device, hipGetErrorString(dev.status()));
+  a.k = (const uint8_t*)cache->k; a.v = (const uint8_t*)cache->v; a.k_exp = cache->k_exp; a.v_exp = cache->v_exp;
+  a.q = (const half_t*)g.q; a.out = (half_t*)g.out;
+  a.q_row = g.q_row; a.q_head = g.q_head; a.out_row = g.out_row; a.out_head = g.out_head;
+  a.G = g.heads / a.b.NKV; a.tt = p.tt; a.tiles = (int)p.tiles; a.nsplit = p.nsplit;
+  a.c = g.scale * 1.44269504088896340736f;
+  a.part = (float*)g.ws;
+  if (cache->head_dim == 64) launch<64>(a, p.nt, (hipStream_t)stream);
+  else launch<128>(a, p.nt, (hipStream_t)stream);
+  const hipError_t h = hipGetLastError();
+  if (h != hipSuccess) return op_fail(ANE_ERR_HIP, "storiesane %s: %s", op, hipGetErrorString(h));
+  return ANE_OK;
+}
