@@ -12,10 +12,9 @@
 // exponent applied) in the registers.
 //
 // A block is one tile and one key/value head (and one part of the keys where
-// tiles are few); its four waves take steps of 64 keys in turn and meet once
+// tiles are few); its four waves take steps of 32 or 64 keys in turn and meet once
 // at the end, in LDS.  There is no barrier in the loop.
 #include <algorithm>
-#include <type_traits>
 
 #include "kv8.h"
 #include "op_error.h"
@@ -25,8 +24,9 @@ namespace ane {
 namespace {
 
 constexpr int kThreads = 256, kWaves = 4;
-constexpr int kStep = 64;                  // keys a wave takes at a time
-constexpr int kRound = kStep * kWaves;     // keys the block takes at a time
+// keys that a block takes at a time are a divisor of this; parts of the keys
+// are multiples of it
+constexpr int kRound = 256;
 
 struct AttendArgs {
   Kv8Batch b;
@@ -72,29 +72,29 @@ __device__ __forceinline__ half8 join(half2v a, half2v b, half2v c, half2v d) {
   return r;
 }
 
-// whether any of the four codes is NaN
-__device__ __forceinline__ bool has_nan(uint32_t w) {
-  const uint32_t x = (w & 0x7f7f7f7fu) ^ 0x7f7f7f7fu;  // a zero byte where NaN (bit 7 is clear)
-  return ((x - 0x01010101u) & 0x80808080u) != 0;
+// 0xff in every byte of w that is a NaN code
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
+  return ((((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7) * 0xffu;
 }
 
-// One step's K and V, 16 keys (a unit) at a time: raw codes and the page's
-// exponents.  A unit that does not take part (past the end, page not there)
-// reads the pool's first page, which exists; its scores are masked and its
-// values cleared.
-template <int DH>
+// One step's K and V, NU units of 16 keys: raw codes and where they come from.
+// A unit that does not take part (past the end, page not there) reads the
+// pool's first page, which exists; its scores are masked and its values
+// cleared.
+template <int DH, int NU>
 struct Step {
-  u32x4 k[4][DH / 64], v[4][DH / 64];
-  float ks[4], vs[4];
-  bool there[4];
+  u32x4 k[NU][DH / 64], v[NU][DH / 64];
+  bool there[NU];
 };
 
-template <int DH, int NT>
+// NU: units of 16 keys in a wave's step.
+template <int DH, int NT, int NU>
 __global__ __launch_bounds__(kThreads, 2) void attend_kernel(AttendArgs a) {
   constexpr int R = 16 * NT;    // rows of the tile
   constexpr int NM = DH / 32;   // MFMAs along the head dimension
   constexpr int ND = DH / 16;   // 16-dimension groups of the output
   constexpr int LD = DH + 4;
+  constexpr int KS = 16 * NU;   // keys of a step
   __shared__ __attribute__((aligned(16))) float lds_o[kWaves][R][LD];
   __shared__ float lds_m[kWaves][R], lds_l[kWaves][R];
   const Kv8Batch& b = a.b;
@@ -114,6 +114,48 @@ __global__ __launch_bounds__(kThreads, 2) void attend_kernel(AttendArgs a) {
   if (k0 >= kend) return;
   const int k1 = min(kend, k0 + pk);
 
+  // Page ids and exponents of 64 pages from wbase on, one per lane.
+  const int* trow = b.table + (size_t)span.seq * b.table_stride;
+  int wbase = -(1 << 30), wid = -1, wexp = 0;
+  auto window = [&](int pg) {
+    wbase = pg;
+    const int p = pg + lane;
+    wid = -1;
+    if (p < b.table_pages && ((int64_t)p << b.pshift) < k1) {
+      wid = trow[p];
+      if ((unsigned)wid >= (unsigned)b.pages) wid = -1;
+    }
+    const size_t e = (size_t)(wid >= 0 ? wid : 0) * b.NKV + h;
+    wexp = ((int)a.k_exp[e] & 0xff) | ((int)a.v_exp[e] & 0xff) << 8;
+  };
+  const size_t head_bytes = (size_t)DH << b.pshift;
+  const int kl = col * DH + 16 * g, vl = lane * (DH / 4);
+  auto within = [&](int kb) {
+    if ((kb >> b.pshift) < wbase || ((kb + KS - 1) >> b.pshift) >= wbase + 64) window(kb >> b.pshift);
+  };
+  auto fetch = [&](Step<DH, NU>& s, int kb) {
+    within(kb);
+#pragma unroll
+    for (int u = 0; u < NU; u++) {
+      const int ku = kb + 16 * u;
+      const int id = __builtin_amdgcn_readlane(wid, (ku >> b.pshift) - wbase);
+      s.there[u] = id >= 0 && ku < k1;
+      const size_t page = ((size_t)(s.there[u] ? id : 0) * b.NKV + h) * head_bytes;
+      const int slot = ku & ((1 << b.pshift) - 1);
+      const uint8_t* kp = a.k + page + slot * DH;
+      const uint8_t* vp = a.v + page + slot * DH;
+#pragma unroll
+      for (int x = 0; x < DH / 64; x++) {
+        s.k[u][x] = *reinterpret_cast<const u32x4*>(kp + kl + 64 * x);
+        s.v[u][x] = *reinterpret_cast<const u32x4*>(vp + vl + 16 * x);
+      }
+    }
+  };
+
+  Step<DH, NU> cur;
+  int kb = k0 + wave * KS;
+  if (kb < k1) fetch(cur, kb);
+
   // Q: row r = 16 t + col, dimensions 64 (m / 2) + 16 g + 8 (m % 2) + j
   half8 q[NT][NM];
   int lim[NT];  // the last key of the lane's row
@@ -127,47 +169,11 @@ __global__ __launch_bounds__(kThreads, 2) void attend_kernel(AttendArgs a) {
     for (int m = 0; m < NM; m++) q[t][m] = ld_h8(p + 64 * (m >> 1) + 8 * (m & 1));
   }
 
-  // Page ids and exponents of 64 pages from wbase on, one per lane.
-  const int* trow = b.table + (size_t)span.seq * b.table_stride;
-  int wbase = -(1 << 30), wid = -1, wexp = 0;
-  auto window = [&](int pg) {
-    wbase = pg;
-    const int p = pg + lane;
-    wid = -1;
-    if (p < b.table_pages && ((int64_t)p << b.pshift) < k1) {
-      wid = trow[p];
-      if ((unsigned)wid >= (unsigned)b.pages) wid = -1;
-    }
-    wexp = 0;
-    if (wid >= 0) {
-      const size_t e = (size_t)wid * b.NKV + h;
-      wexp = ((int)a.k_exp[e] & 0xff) | ((int)a.v_exp[e] & 0xff) << 8;
-    }
-  };
-  const size_t head_bytes = (size_t)DH << b.pshift;
-  const int kl = col * DH + 16 * g, vl = lane * (DH / 4);
-  auto fetch = [&](Step<DH>& s, int kb) {
-    if ((kb >> b.pshift) < wbase || ((kb + kStep - 1) >> b.pshift) >= wbase + 64) window(kb >> b.pshift);
-#pragma unroll
-    for (int u = 0; u < 4; u++) {
-      const int ku = kb + 16 * u;
-      const int w = (ku >> b.pshift) - wbase;
-      const int id = __builtin_amdgcn_readlane(wid, w), ex = __builtin_amdgcn_readlane(wexp, w);
-      s.there[u] = id >= 0 && ku < k1;
-      const size_t page = ((size_t)(s.there[u] ? id : 0) * b.NKV + h) * head_bytes;
-      const int slot = ku & ((1 << b.pshift) - 1);
-      const uint8_t* kp = a.k + page + slot * DH;
-      const uint8_t* vp = a.v + page + slot * DH;
-#pragma unroll
-      for (int x = 0; x < DH / 64; x++) {
-        s.k[u][x] = *reinterpret_cast<const u32x4*>(kp + kl + 64 * x);
-        s.v[u][x] = *reinterpret_cast<const u32x4*>(vp + vl + 16 * x);
-      }
-      s.ks[u] = kv8_scale((int8_t)(ex & 0xff));
-      s.vs[u] = kv8_scale((int8_t)(ex >> 8 & 0xff));
-    }
-  };
-
+  // m: what the exponentials are relative to, the same in the four lanes of a
+  // row: at least the row's maximum less kSlack so far.  It moves only when a
+  // score passes it by more, so that most steps neither join the lanes'
+  // maxima nor touch the sums; weights stay below 2^kSlack.
+  constexpr float kSlack = 8.f;
   float m[NT], l[NT];
   floatx4 o[ND][NT];
 #pragma unroll
@@ -178,67 +184,90 @@ __global__ __launch_bounds__(kThreads, 2) void attend_kernel(AttendArgs a) {
     for (int d = 0; d < ND; d++) o[d][t] = floatx4{0.f, 0.f, 0.f, 0.f};
   }
 
-  auto step = [&](Step<DH>& s, int kb, auto edge_) {
-    constexpr bool EDGE = decltype(edge_)::value;
-    floatx4 sc[4][NT];
+  // whether a step holds keys that some row does not attend to
+  auto at_edge = [&](const Step<DH, NU>& s, int kb) {
+    bool inner = kb + KS - 1 <= span.pos;
 #pragma unroll
-    for (int u = 0; u < 4; u++) {
+    for (int u = 0; u < NU; u++) inner = inner && s.there[u];
+    return !inner;
+  };
+
+  uint32_t nan = 0;
+  auto step = [&](Step<DH, NU>& s, int kb, const float (&ks)[NU], const float (&vs)[NU], bool edge) {
+    floatx4 sc[NU][NT];
+#pragma unroll
+    for (int u = 0; u < NU; u++) {
       half8 kf[NM];
 #pragma unroll
       for (int x = 0; x < NM; x++) {
         const uint32_t w0 = s.k[u][x >> 1][2 * (x & 1)], w1 = s.k[u][x >> 1][2 * (x & 1) + 1];
-        kf[x] = join(kv8_up<false>(w0, s.ks[u]), kv8_up<true>(w0, s.ks[u]), kv8_up<false>(w1, s.ks[u]),
-                     kv8_up<true>(w1, s.ks[u]));
+        kf[x] = join(kv8_up<false>(w0, ks[u]), kv8_up<true>(w0, ks[u]), kv8_up<false>(w1, ks[u]),
+                     kv8_up<true>(w1, ks[u]));
       }
 #pragma unroll
       for (int t = 0; t < NT; t++) {
         floatx4 c = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int x = 0; x < NM; x++) c = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[x], q[t][x], c, 0, 0, 0);
-        if (EDGE) {
-#pragma unroll
-          for (int j = 0; j < 4; j++)
-            if (!s.there[u] || kb + 16 * u + 4 * g + j > lim[t]) c[j] = -INFINITY;
-        }
         sc[u][t] = c;
       }
     }
-    half8 pf[2][NT];
+    if (edge) {
+#pragma unroll
+      for (int u = 0; u < NU; u++)
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+          for (int j = 0; j < 4; j++)
+            if (!s.there[u] || kb + 16 * u + 4 * g + j > lim[t]) sc[u][t][j] = -INFINITY;
+    }
+    float mx[NT];
+    bool up = false;
 #pragma unroll
     for (int t = 0; t < NT; t++) {
-      float mx = -INFINITY;
+      mx[t] = sc[0][t][0];
 #pragma unroll
-      for (int u = 0; u < 4; u++)
+      for (int u = 0; u < NU; u++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) mx = fmaxf(mx, sc[u][t][j]);
-      mx = xor32_max(xor16_max(mx));
-      const float mn = fmaxf(m[t], mx * a.c);
-      const float mu = mn == -INFINITY ? 0.f : mn;  // no key yet: exp2(-inf) below, not exp2(nan)
-      const float al = __builtin_amdgcn_exp2f(m[t] - mu);
-      m[t] = mn;
+        for (int j = 0; j < 4; j++) mx[t] = fmaxf(mx[t], sc[u][t][j]);
+      mx[t] *= a.c;
+      up |= mx[t] > m[t] + kSlack;
+    }
+    if (__any(up)) {
+#pragma unroll
+      for (int t = 0; t < NT; t++) {
+        const float mn = fmaxf(m[t], xor32_max(xor16_max(mx[t])));
+        const float al = __builtin_amdgcn_exp2f(m[t] - (mn == -INFINITY ? 0.f : mn));
+        m[t] = mn;
+        l[t] *= al;
+#pragma unroll
+        for (int d = 0; d < ND; d++)
+#pragma unroll
+          for (int j = 0; j < 4; j++) o[d][t][j] *= al;
+      }
+    }
+    half8 pf[NU / 2][NT];
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+      const float mu = m[t] == -INFINITY ? 0.f : m[t];  // no key yet: exp2(-inf), not exp2(nan)
       float sum = 0.f;
 #pragma unroll
-      for (int u = 0; u < 4; u++)
+      for (int u = 0; u < NU; u++)
 #pragma unroll
         for (int j = 0; j < 4; j++) {
           const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u][t][j], a.c, -mu));
           sum += p;
           pf[u >> 1][t][4 * (u & 1) + j] = (half_t)p;
         }
-      l[t] = l[t] * al + sum;
-#pragma unroll
-      for (int d = 0; d < ND; d++)
-#pragma unroll
-        for (int j = 0; j < 4; j++) o[d][t][j] *= al;
+      l[t] += sum;
     }
-    // values that no row of the tile attends to may be anything (rows not yet
+    // Values that no row of the tile attends to may be anything (rows not yet
     // written): cleared.  NaN among those that some row attends to and some
-    // does not is taken out of the product and put back into the rows that
-    // attend to it.
-    bool nan = false;
-    if (EDGE) {
+    // does not is taken out of the product, and put back behind the loop into
+    // the rows that attend to it.
+    if (edge) {
 #pragma unroll
-      for (int u = 0; u < 4; u++) {
+      for (int u = 0; u < NU; u++) {
         const int first = kb + 16 * u + 4 * g;  // the lane's four keys
         const int n = s.there[u] ? clampi(k1 - first, 0, 4) : 0;
         const uint32_t mine = n == 4 ? 0xffffffffu : (1u << (8 * n)) - 1;
@@ -246,59 +275,74 @@ __global__ __launch_bounds__(kThreads, 2) void attend_kernel(AttendArgs a) {
         for (int x = 0; x < DH / 64; x++)
 #pragma unroll
           for (int j = 0; j < 4; j++) {
-            s.v[u][x][j] &= mine;
-            nan |= has_nan(s.v[u][x][j]);
+            const uint32_t w = s.v[u][x][j] & mine, bad = nan_bytes(w);
+            nan |= bad;
+            s.v[u][x][j] = w & ~bad;
           }
       }
-      nan = __any(nan);
     }
 #pragma unroll
-    for (int y = 0; y < 2; y++)
+    for (int y = 0; y < NU / 2; y++)
 #pragma unroll
       for (int d = 0; d < ND; d++) {
         const uint32_t w0 = s.v[2 * y][d >> 2][d & 3], w1 = s.v[2 * y + 1][d >> 2][d & 3];
-        half8 vf = join(kv8_up<false>(w0, s.vs[2 * y]), kv8_up<true>(w0, s.vs[2 * y]),
-                        kv8_up<false>(w1, s.vs[2 * y + 1]), kv8_up<true>(w1, s.vs[2 * y + 1]));
-        if (EDGE && nan) {
-          half8 isnan;
-#pragma unroll
-          for (int j = 0; j < 8; j++) {
-            const bool bad = vf[j] != vf[j];
-            isnan[j] = bad ? (half_t)1.f : (half_t)0.f;
-            if (bad) vf[j] = (half_t)0.f;
-          }
-#pragma unroll
-          for (int t = 0; t < NT; t++) {
-            half8 sees;
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-              const int u = 2 * y + (j >> 2);
-              sees[j] = s.there[u] && kb + 16 * u + 4 * g + (j & 3) <= lim[t] ? (half_t)1.f : (half_t)0.f;
-            }
-            floatx4 n = {0.f, 0.f, 0.f, 0.f};
-            n = __builtin_amdgcn_mfma_f32_16x16x32_f16(isnan, sees, n, 0, 0, 0);
-#pragma unroll
-            for (int j = 0; j < 4; j++)
-              if (n[j] > 0.f) o[d][t][j] = NAN;
-          }
-        }
+        const half8 vf = join(kv8_up<false>(w0, vs[2 * y]), kv8_up<true>(w0, vs[2 * y]),
+                              kv8_up<false>(w1, vs[2 * y + 1]), kv8_up<true>(w1, vs[2 * y + 1]));
 #pragma unroll
         for (int t = 0; t < NT; t++) o[d][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[y][t], o[d][t], 0, 0, 0);
       }
   };
 
-  Step<DH> cur;
-  int kb = k0 + wave * kStep;
-  if (kb < k1) fetch(cur, kb);
   while (kb < k1) {
-    Step<DH> nxt;
-    const int kn = kb + kRound;
+    // the exponents, before the window may move on
+    float ks[NU], vs[NU];
+#pragma unroll
+    for (int u = 0; u < NU; u++) {
+      const int ex = __builtin_amdgcn_readlane(wexp, ((kb + 16 * u) >> b.pshift) - wbase);
+      ks[u] = kv8_scale((int8_t)(ex & 0xff));
+      vs[u] = kv8_scale((int8_t)(ex >> 8 & 0xff));
+    }
+    Step<DH, NU> nxt;
+    const int kn = kb + KS * kWaves;
     if (kn < k1) fetch(nxt, kn);
-    const bool inner = kb + kStep - 1 <= span.pos && cur.there[0] && cur.there[1] && cur.there[2] && cur.there[3];
-    if (inner) step(cur, kb, std::false_type{});
-    else step(cur, kb, std::true_type{});
+    step(cur, kb, ks, vs, at_edge(cur, kb));
     if (kn < k1) cur = nxt;
     kb = kn;
+  }
+  if (__any(nan != 0)) {
+    // rare: how many NaN of each dimension a row attends to, as a product of
+    // zeros and ones, over the steps that had them taken out
+    for (kb = k0 + wave * KS; kb < k1; kb += KS * kWaves) {
+      fetch(cur, kb);
+      if (!at_edge(cur, kb)) continue;
+#pragma unroll
+      for (int y = 0; y < NU / 2; y++) {
+        half8 sees[NT];
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+          for (int j = 0; j < 8; j++) {
+            const int u = 2 * y + (j >> 2);
+            sees[t][j] = cur.there[u] && kb + 16 * u + 4 * g + (j & 3) <= lim[t] ? (half_t)1.f : (half_t)0.f;
+          }
+#pragma unroll
+        for (int d = 0; d < ND; d++) {
+          half8 isnan;
+#pragma unroll
+          for (int j = 0; j < 8; j++)
+            isnan[j] = nan_bytes(cur.v[2 * y + (j >> 2)][d >> 2][d & 3]) >> (8 * (j & 3)) & 1 ? (half_t)1.f
+                                                                                             : (half_t)0.f;
+#pragma unroll
+          for (int t = 0; t < NT; t++) {
+            floatx4 n = {0.f, 0.f, 0.f, 0.f};
+            n = __builtin_amdgcn_mfma_f32_16x16x32_f16(isnan, sees[t], n, 0, 0, 0);
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+              if (n[j] > 0.f) o[d][t][j] = NAN;
+          }
+        }
+      }
+    }
   }
 
   // The waves meet: maximum over the waves, every wave's sums brought to it.
@@ -419,9 +463,9 @@ bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 template <int DH>
 void launch(const AttendArgs& a, int nt, hipStream_t st) {
   const dim3 grid((uint32_t)a.tiles * a.b.NKV * a.nsplit);
-  if (nt == 1) hipLaunchKernelGGL((attend_kernel<DH, 1>), grid, dim3(kThreads), 0, st, a);
-  else if (nt == 2) hipLaunchKernelGGL((attend_kernel<DH, 2>), grid, dim3(kThreads), 0, st, a);
-  else if constexpr (DH == 64) hipLaunchKernelGGL((attend_kernel<DH, 4>), grid, dim3(kThreads), 0, st, a);
+  if (nt == 1) hipLaunchKernelGGL((attend_kernel<DH, 1, DH == 64 ? 4 : 2>), grid, dim3(kThreads), 0, st, a);
+  else if (nt == 2) hipLaunchKernelGGL((attend_kernel<DH, 2, 2>), grid, dim3(kThreads), 0, st, a);
+  else if constexpr (DH == 64) hipLaunchKernelGGL((attend_kernel<DH, 4, 2>), grid, dim3(kThreads), 0, st, a);
   if (a.nsplit > 1)
     hipLaunchKernelGGL(join_kernel<DH>, dim3((uint32_t)a.tiles * a.b.NKV), dim3(kThreads), 0, st, a);
 }
