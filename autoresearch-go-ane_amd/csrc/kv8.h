@@ -66,12 +66,19 @@ __host__ __device__ __forceinline__ uint32_t kv8_first(const Kv8Batch& b, Kv8Ite
 }
 inline uint32_t kv8_count(int nseq, int rows, Kv8Items t) { return ((uint32_t)rows + (uint32_t)nseq * t.slack) / t.width; }
 
-// The largest i with f(i) <= item: 64 candidates a round, so up to 4096
-// sequences take two dependent loads.  Offsets that do not rise lead to some
-// i in [0, nseq), never outside.
-__host__ __device__ __forceinline__ int kv8_find(const Kv8Batch& b, Kv8Items t, uint32_t item) {
+// The sequence of an item -- the largest i with f(i) <= item -- and its rows:
+// 64 candidates a round, so up to 64 sequences take one load's latency, up to
+// 4096 two.  In the last round each lane holds its own sequence's numbers, and
+// the chosen lane's become scalars, without another load.  Offsets that do
+// not rise lead to some i in [0, nseq), never outside.
+struct Kv8Found {
+  int i;
+  Kv8Seq s;
+  uint32_t first;  // f(i)
+};
+__host__ __device__ __forceinline__ Kv8Found kv8_find(const Kv8Batch& b, Kv8Items t, uint32_t item) {
   int lo = 0, span = b.nseq;
-  while (span > 1) {
+  while (span > 64) {
     const int step = (span + 63) >> 6;
     int below = 0;
 #ifdef __HIP_DEVICE_COMPILE__
@@ -87,9 +94,21 @@ __host__ __device__ __forceinline__ int kv8_find(const Kv8Batch& b, Kv8Items t, 
     span = step < rest ? step : rest;
   }
 #ifdef __HIP_DEVICE_COMPILE__
-  lo = __builtin_amdgcn_readfirstlane(lo);  // the same in every lane; in a scalar register from here on
+  const int lane = threadIdx.x & 63;
+  const int mine = lo + min(lane, span - 1);
+  const Kv8Seq s = kv8_seq(b, mine);
+  const uint32_t first = ((uint32_t)s.row0 + (uint32_t)mine * t.slack) / t.width;
+  const int below = __popcll(__ballot(lane < span && first <= item));
+  const int c = below > 0 ? below - 1 : 0;
+  return {__builtin_amdgcn_readfirstlane(lo + c),
+          {__builtin_amdgcn_readlane(s.row0, c), __builtin_amdgcn_readlane(s.n, c), __builtin_amdgcn_readlane(s.st, c)},
+          (uint32_t)__builtin_amdgcn_readlane((int)first, c)};
+#else
+  int below = 0;
+  for (int lane = 0; lane < span; lane++) below += kv8_first(b, t, lo + lane) <= item;
+  const int i = lo + (below > 0 ? below - 1 : 0);
+  return {i, kv8_seq(b, i), kv8_first(b, t, i)};
 #endif
-  return lo;
 }
 
 // What an item takes: tokens of sequence `seq` at positions pos .. pos + n - 1,
@@ -105,22 +124,18 @@ __host__ __device__ __forceinline__ Kv8Span kv8_cut(const Kv8Seq& s, int i, int6
 }
 // the item-th tile of `w` tokens
 __host__ __device__ __forceinline__ Kv8Span kv8_tile_span(const Kv8Batch& b, int w, uint32_t item) {
-  const Kv8Items t = kv8_tiles(w);
-  const int i = kv8_find(b, t, item);
-  const Kv8Seq s = kv8_seq(b, i);
-  const int64_t k = (int64_t)item - kv8_first(b, t, i);
-  if (k < 0) return {i, 0, 0, 0};
-  return kv8_cut(s, i, s.st + k * w, s.st + (k + 1) * w);
+  const Kv8Found f = kv8_find(b, kv8_tiles(w), item);
+  const int64_t k = (int64_t)item - f.first;
+  if (k < 0) return {f.i, 0, 0, 0};
+  return kv8_cut(f.s, f.i, f.s.st + k * w, f.s.st + (k + 1) * w);
 }
 // the rows of the item-th page that gets any (page pos >> pshift of the table)
 __host__ __device__ __forceinline__ Kv8Span kv8_page_span(const Kv8Batch& b, uint32_t item) {
-  const Kv8Items t = kv8_pages(1 << b.pshift);
-  const int i = kv8_find(b, t, item);
-  const Kv8Seq s = kv8_seq(b, i);
-  const int64_t k = (int64_t)item - kv8_first(b, t, i);
-  if (k < 0) return {i, 0, 0, 0};
-  const int64_t pg = (s.st >> b.pshift) + k;
-  return kv8_cut(s, i, pg << b.pshift, (pg + 1) << b.pshift);
+  const Kv8Found f = kv8_find(b, kv8_pages(1 << b.pshift), item);
+  const int64_t k = (int64_t)item - f.first;
+  if (k < 0) return {f.i, 0, 0, 0};
+  const int64_t pg = (f.s.st >> b.pshift) + k;
+  return kv8_cut(f.s, f.i, pg << b.pshift, (pg + 1) << b.pshift);
 }
 
 // e4m3 -> fp16 with the exponent applied, two codes of a dword at a time;

@@ -12,7 +12,7 @@
 // exponent applied) in the registers.
 //
 // A block is one tile and one key/value head (and one part of the keys where
-// tiles are few); its four waves take steps of 32 or 64 keys in turn and meet once
+// tiles are few); its waves take steps of 32 or 64 keys in turn and meet once
 // at the end, in LDS.  There is no barrier in the loop.
 #include <algorithm>
 
@@ -22,11 +22,6 @@
 namespace ane {
 
 namespace {
-
-constexpr int kThreads = 256, kWaves = 4;
-// keys that a block takes at a time are a divisor of this; parts of the keys
-// are multiples of it
-constexpr int kRound = 256;
 
 struct AttendArgs {
   Kv8Batch b;
@@ -39,14 +34,15 @@ struct AttendArgs {
   int tt;       // tokens per tile: tt * G <= rows of the tile
   int tiles;    // items
   int nsplit;   // parts that the keys of a tile are cut into, at most
+  int round;    // keys that a block takes at a time: parts are multiples of it
   float c;      // scale * log2(e)
   float* part;  // [tiles][NKV][nsplit][tt * G][DH + 2]: sums, maximum, sum of exponentials
 };
 
 // The keys of a tile are cut into equal parts of whole rounds, at most nsplit.
-__device__ __forceinline__ int part_keys(int keys, int nsplit) {
+__device__ __forceinline__ int part_keys(int keys, int nsplit, int round) {
   const int n = (keys + nsplit - 1) / nsplit;
-  return (n + kRound - 1) / kRound * kRound;
+  return (n + round - 1) / round * round;
 }
 
 __device__ __forceinline__ float xor16_max(float x) {
@@ -87,16 +83,16 @@ struct Step {
   bool there[NU];
 };
 
-// NU: units of 16 keys in a wave's step.
-template <int DH, int NT, int NU>
-__global__ __launch_bounds__(kThreads, 2) void attend_kernel(AttendArgs a) {
+// NT: tiles of 16 rows; NU: units of 16 keys in a wave's step; KW: waves.
+template <int DH, int NT, int NU, int KW>
+__global__ __launch_bounds__(64 * KW, KW == 16 ? 1 : 2) void attend_kernel(AttendArgs a) {
   constexpr int R = 16 * NT;    // rows of the tile
   constexpr int NM = DH / 32;   // MFMAs along the head dimension
   constexpr int ND = DH / 16;   // 16-dimension groups of the output
   constexpr int LD = DH + 4;
   constexpr int KS = 16 * NU;   // keys of a step
-  __shared__ __attribute__((aligned(16))) float lds_o[kWaves][R][LD];
-  __shared__ float lds_m[kWaves][R], lds_l[kWaves][R];
+  __shared__ __attribute__((aligned(16))) float lds_o[KW][R][LD];
+  __shared__ float lds_m[KW][R], lds_l[KW][R];
   const Kv8Batch& b = a.b;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -109,7 +105,7 @@ __global__ __launch_bounds__(kThreads, 2) void attend_kernel(AttendArgs a) {
   if (span.n == 0) return;
   const int rows = span.n * a.G;
   const int kend = span.pos + span.n;  // keys of the tile's last token
-  const int pk = part_keys(kend, a.nsplit);
+  const int pk = part_keys(kend, a.nsplit, a.round);
   const int k0 = sp * pk;
   if (k0 >= kend) return;
   const int k1 = min(kend, k0 + pk);
@@ -303,7 +299,7 @@ __global__ __launch_bounds__(kThreads, 2) void attend_kernel(AttendArgs a) {
       vs[u] = kv8_scale((int8_t)(ex >> 8 & 0xff));
     }
     Step<DH, NU> nxt;
-    const int kn = kb + KS * kWaves;
+    const int kn = kb + KS * KW;
     if (kn < k1) fetch(nxt, kn);
     step(cur, kb, ks, vs, at_edge(cur, kb));
     if (kn < k1) cur = nxt;
@@ -312,7 +308,7 @@ __global__ __launch_bounds__(kThreads, 2) void attend_kernel(AttendArgs a) {
   if (__any(nan != 0)) {
     // rare: how many NaN of each dimension a row attends to, as a product of
     // zeros and ones, over the steps that had them taken out
-    for (kb = k0 + wave * KS; kb < k1; kb += KS * kWaves) {
+    for (kb = k0 + wave * KS; kb < k1; kb += KS * KW) {
       fetch(cur, kb);
       if (!at_edge(cur, kb)) continue;
 #pragma unroll
@@ -355,80 +351,102 @@ __global__ __launch_bounds__(kThreads, 2) void attend_kernel(AttendArgs a) {
 #pragma unroll
   for (int t = 0; t < NT; t++) {
     const int r = 16 * t + col;
-    const float mm = fmaxf(fmaxf(lds_m[0][r], lds_m[1][r]), fmaxf(lds_m[2][r], lds_m[3][r]));
+    float mm = lds_m[0][r];
+#pragma unroll
+    for (int w = 1; w < KW; w++) mm = fmaxf(mm, lds_m[w][r]);
     const float al = __builtin_amdgcn_exp2f(m[t] - (mm == -INFINITY ? 0.f : mm));
     if (g == 0) lds_l[wave][r] = l[t] * al;
+    if (r < rows) {
 #pragma unroll
-    for (int d = 0; d < ND; d++)
-      *reinterpret_cast<floatx4*>(&lds_o[wave][r][16 * d + 4 * g]) = o[d][t] * al;
+      for (int d = 0; d < ND; d++) *reinterpret_cast<floatx4*>(&lds_o[wave][r][16 * d + 4 * g]) = o[d][t] * al;
+    }
   }
   __syncthreads();
   const bool whole = pk >= kend;
   float* part = a.part + (((size_t)tile * b.NKV + h) * a.nsplit + sp) * ((size_t)a.tt * a.G * (DH + 2));
-  for (int c = tid; c < rows * (DH / 8); c += kThreads) {
-    const int r = c / (DH / 8), d0 = c % (DH / 8) * 8;
-    float x[8];
+  for (int c = tid; c < rows * (DH / 4); c += 64 * KW) {
+    const int r = c / (DH / 4), d0 = c % (DH / 4) * 4;
+    floatx4 x = *reinterpret_cast<const floatx4*>(&lds_o[0][r][d0]);
+    float ls = lds_l[0][r];
 #pragma unroll
-    for (int j = 0; j < 8; j++)
-      x[j] = (lds_o[0][r][d0 + j] + lds_o[1][r][d0 + j]) + (lds_o[2][r][d0 + j] + lds_o[3][r][d0 + j]);
-    const float ls = (lds_l[0][r] + lds_l[1][r]) + (lds_l[2][r] + lds_l[3][r]);
+    for (int w = 1; w < KW; w++) {
+      x += *reinterpret_cast<const floatx4*>(&lds_o[w][r][d0]);
+      ls += lds_l[w][r];
+    }
     if (whole) {
       const float inv = ls == 0.f ? 0.f : 1.f / ls;
       const int tok = r / a.G, hg = r - tok * a.G;
-      half8 y;
+      half4 y;
 #pragma unroll
-      for (int j = 0; j < 8; j++) y[j] = (half_t)(x[j] * inv);
-      st_h8(a.out + (span.row + tok) * a.out_row + (h * a.G + hg) * a.out_head + d0, y);
+      for (int j = 0; j < 4; j++) y[j] = (half_t)(x[j] * inv);
+      *reinterpret_cast<half4*>(a.out + (span.row + tok) * a.out_row + (h * a.G + hg) * a.out_head + d0) = y;
     } else {
       float* p = part + (size_t)r * (DH + 2);
 #pragma unroll
-      for (int j = 0; j < 8; j++) p[d0 + j] = x[j];
+      for (int j = 0; j < 4; j++) p[d0 + j] = x[j];
       if (d0 == 0) {
-        p[DH] = fmaxf(fmaxf(lds_m[0][r], lds_m[1][r]), fmaxf(lds_m[2][r], lds_m[3][r]));
+        float mm = lds_m[0][r];
+#pragma unroll
+        for (int w = 1; w < KW; w++) mm = fmaxf(mm, lds_m[w][r]);
+        p[DH] = mm;
         p[DH + 1] = ls;
       }
     }
   }
 }
 
-// Joins the parts of a tile's keys; one block per tile and key/value head.
+// Joins the parts of a tile's keys: a wave per row, lane s first taking part
+// s's maximum and sum (at most kMaxSplit parts), then every lane DH / 64
+// dimensions of all parts.
+constexpr int kMaxSplit = 64;
 template <int DH>
-__global__ __launch_bounds__(kThreads) void join_kernel(AttendArgs a) {
+__global__ __launch_bounds__(256) void join_kernel(AttendArgs a) {
+  constexpr int W = DH / 64;
   const Kv8Batch& b = a.b;
+  const int lane = threadIdx.x & 63;
   const int h = blockIdx.x % b.NKV, tile = blockIdx.x / b.NKV;
   const Kv8Span span = kv8_tile_span(b, a.tt, tile);
-  if (span.n == 0) return;
+  const int r = blockIdx.y * 4 + (threadIdx.x >> 6);
+  if (r >= span.n * a.G) return;
   const int kend = span.pos + span.n;
-  const int pk = part_keys(kend, a.nsplit);
+  const int pk = part_keys(kend, a.nsplit, a.round);
   if (pk >= kend) return;  // one part: the output is written
   const int np = (kend + pk - 1) / pk;
-  const int rows = span.n * a.G;
   const size_t stride = (size_t)a.tt * a.G * (DH + 2);
-  const float* part = a.part + ((size_t)tile * b.NKV + h) * a.nsplit * stride;
-  for (int c = threadIdx.x; c < rows * (DH / 8); c += kThreads) {
-    const int r = c / (DH / 8), d0 = c % (DH / 8) * 8;
-    const float* p = part + (size_t)r * (DH + 2);
-    float mm = -INFINITY;
-    for (int s = 0; s < np; s++) mm = fmaxf(mm, p[s * stride + DH]);
-    const float mu = mm == -INFINITY ? 0.f : mm;
-    float l = 0.f, x[8] = {};
-    for (int s = 0; s < np; s++) {
-      const float al = __builtin_amdgcn_exp2f(p[s * stride + DH] - mu);
-      l += p[s * stride + DH + 1] * al;
-#pragma unroll
-      for (int j = 0; j < 8; j++) x[j] += p[s * stride + d0 + j] * al;
-    }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    const int tok = r / a.G, hg = r - tok * a.G;
-    half8 y;
-#pragma unroll
-    for (int j = 0; j < 8; j++) y[j] = (half_t)(x[j] * inv);
-    st_h8(a.out + (span.row + tok) * a.out_row + (h * a.G + hg) * a.out_head + d0, y);
+  const float* part = a.part + ((size_t)tile * b.NKV + h) * a.nsplit * stride + (size_t)r * (DH + 2);
+  float m = -INFINITY, l = 0.f;
+  if (lane < np) {
+    m = part[lane * stride + DH];
+    l = part[lane * stride + DH + 1];
   }
+  const float mm = wave_max(m);
+  const float al = __builtin_amdgcn_exp2f(m - (mm == -INFINITY ? 0.f : mm));
+  l = wave_sum(l * al);
+  float x[W] = {};
+  constexpr int B = 8;  // parts whose loads are under way at once
+  for (int s = 0; s < np; s += B) {
+    float v[B][W];
+#pragma unroll
+    for (int u = 0; u < B; u++)
+#pragma unroll
+      for (int j = 0; j < W; j++) v[u][j] = part[min(s + u, np - 1) * stride + lane + 64 * j];
+#pragma unroll
+    for (int u = 0; u < B; u++) {
+      const float w = s + u < np ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(al), s + u)) : 0.f;
+#pragma unroll
+      for (int j = 0; j < W; j++)
+        if (s + u < np) x[j] += v[u][j] * w;
+    }
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const int tok = r / a.G, hg = r - tok * a.G;
+  half_t* y = a.out + (span.row + tok) * a.out_row + (h * a.G + hg) * a.out_head + lane;
+#pragma unroll
+  for (int j = 0; j < W; j++) y[64 * j] = (half_t)(x[j] * inv);
 }
 
 struct Plan {
-  int nt = 0, tt = 0, nsplit = 0;
+  int nt = 0, tt = 0, nsplit = 0, kw = 4, round = 0;
   uint32_t tiles = 0;
   int64_t bytes = 0;
 };
@@ -448,9 +466,18 @@ int plan(const char* op, const Kv8Batch& b, const ane_kv8_batch& given, int DH, 
   const int64_t blocks = (int64_t)p->tiles * b.NKV;
   const int cap = b.table_pages << b.pshift;
   const int len = given.max_len ? std::min(given.max_len, cap) : cap;
-  int64_t ns = std::max<int64_t>((1024 + blocks - 1) / blocks, p->nt == 1 ? (len + 2047) / 2048 : 1);
-  ns = std::min<int64_t>(ns, (len + kRound - 1) / kRound);
-  ns = std::max<int64_t>(1, std::min<int64_t>(ns, 64));
+  if (p->nt == 1) {
+    const int r16 = 16 * (DH == 64 ? 64 : 32);
+    p->kw = blocks >= 128 || len <= 2 * r16 ? 16 : 4;
+    if (const char* f = getenv("ZZ_KW")) p->kw = atoi(f);
+    p->round = p->kw * (DH == 64 ? 64 : 32);
+  } else p->round = 128;
+  int64_t want = p->kw == 16 ? 256 : p->nt == 1 ? 1024 : 512;
+  if (const char* f = getenv("ZZ_WANT")) want = atoi(f);
+  int64_t ns = std::max<int64_t>((want + blocks - 1) / blocks, p->nt == 1 ? (len + 4095) / 4096 : 1);
+  if (p->kw == 16 && len <= 2 * p->round) ns = 1;
+  ns = std::min<int64_t>(ns, (len + p->round - 1) / p->round);
+  ns = std::max<int64_t>(1, std::min<int64_t>(ns, kMaxSplit));
   p->nsplit = (int)ns;
   if (blocks * ns > 0x7fffffff)
     return op_fail(ANE_ERR_ARG, "storiesane %s: rows=%d nseq=%d are too many for one launch", op, b.rows, b.nseq);
@@ -460,14 +487,21 @@ int plan(const char* op, const Kv8Batch& b, const ane_kv8_batch& given, int DH, 
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
-template <int DH>
-void launch(const AttendArgs& a, int nt, hipStream_t st) {
+template <int DH, int NT, int NU, int KW>
+void launch_form(const AttendArgs& a, hipStream_t st) {
   const dim3 grid((uint32_t)a.tiles * a.b.NKV * a.nsplit);
-  if (nt == 1) hipLaunchKernelGGL((attend_kernel<DH, 1, DH == 64 ? 4 : 2>), grid, dim3(kThreads), 0, st, a);
-  else if (nt == 2) hipLaunchKernelGGL((attend_kernel<DH, 2, 2>), grid, dim3(kThreads), 0, st, a);
-  else if constexpr (DH == 64) hipLaunchKernelGGL((attend_kernel<DH, 4, 2>), grid, dim3(kThreads), 0, st, a);
+  hipLaunchKernelGGL((attend_kernel<DH, NT, NU, KW>), grid, dim3(64 * KW), 0, st, a);
+}
+
+template <int DH>
+void launch(const AttendArgs& a, const Plan& p, hipStream_t st) {
+  constexpr int NU1 = DH == 64 ? 4 : 2;
+  if (p.nt == 1 && p.kw == 16) launch_form<DH, 1, NU1, 16>(a, st);
+  else if (p.nt == 1) launch_form<DH, 1, NU1, 4>(a, st);
+  else if (p.nt == 2) launch_form<DH, 2, 2, 4>(a, st);
+  else if constexpr (DH == 64) launch_form<DH, 4, 2, 4>(a, st);
   if (a.nsplit > 1)
-    hipLaunchKernelGGL(join_kernel<DH>, dim3((uint32_t)a.tiles * a.b.NKV), dim3(kThreads), 0, st, a);
+    hipLaunchKernelGGL(join_kernel<DH>, dim3((uint32_t)a.tiles * a.b.NKV, (a.tt * a.G + 3) / 4), dim3(256), 0, st, a);
 }
 
 }  // namespace
@@ -517,11 +551,11 @@ extern "C" int ane_kv8_attend(const ane_kv8_cache* cache, const ane_kv8_batch* b
   a.k = (const uint8_t*)cache->k; a.v = (const uint8_t*)cache->v; a.k_exp = cache->k_exp; a.v_exp = cache->v_exp;
   a.q = (const half_t*)g.q; a.out = (half_t*)g.out;
   a.q_row = g.q_row; a.q_head = g.q_head; a.out_row = g.out_row; a.out_head = g.out_head;
-  a.G = g.heads / a.b.NKV; a.tt = p.tt; a.tiles = (int)p.tiles; a.nsplit = p.nsplit;
+  a.G = g.heads / a.b.NKV; a.tt = p.tt; a.tiles = (int)p.tiles; a.nsplit = p.nsplit; a.round = p.round;
   a.c = g.scale * 1.44269504088896340736f;
   a.part = (float*)g.ws;
-  if (cache->head_dim == 64) launch<64>(a, p.nt, (hipStream_t)stream);
-  else launch<128>(a, p.nt, (hipStream_t)stream);
+  if (cache->head_dim == 64) launch<64>(a, p, (hipStream_t)stream);
+  else launch<128>(a, p, (hipStream_t)stream);
   const hipError_t h = hipGetLastError();
   if (h != hipSuccess) return op_fail(ANE_ERR_HIP, "storiesane %s: %s", op, hipGetErrorString(h));
   return ANE_OK;
