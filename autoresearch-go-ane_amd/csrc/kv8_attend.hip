@@ -53,15 +53,6 @@ __device__ __forceinline__ float xor32_max(float x) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
-__device__ __forceinline__ float xor16_sum(float x) {
-  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
-__device__ __forceinline__ float xor32_sum(float x) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
-
 __device__ __forceinline__ half8 join(half2v a, half2v b, half2v c, half2v d) {
   half8 r;
   r[0] = a[0]; r[1] = a[1]; r[2] = b[0]; r[3] = b[1]; r[4] = c[0]; r[5] = c[1]; r[6] = d[0]; r[7] = d[1];
@@ -73,34 +64,43 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
   return ((((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7) * 0xffu;
 }
 
-// One step's K and V, NU units of 16 keys: raw codes and where they come from.
-// A unit that does not take part (past the end, page not there) reads the
-// pool's first page, which exists; its scores are masked and its values
-// cleared.
+// One step's K and V, NU units of 16 keys: raw codes, and of each unit's page
+// the exponents (K in bits 0..7, V in 8..15) and whether it is there (bit 16).
+// A page that is not there reads the pool's first, which exists; its scores
+// are masked and its values cleared.
 template <int DH, int NU>
 struct Step {
   u32x4 k[NU][DH / 64], v[NU][DH / 64];
-  bool there[NU];
+  int ex[NU];
 };
+constexpr int kThere = 1 << 16;
+__device__ __forceinline__ float k_scale(int ex) { return kv8_scale((int8_t)(ex & 0xff)); }
+__device__ __forceinline__ float v_scale(int ex) { return kv8_scale((int8_t)(ex >> 8 & 0xff)); }
 
-// NT: tiles of 16 rows; NU: units of 16 keys in a wave's step; KW: waves.
-template <int DH, int NT, int NU, int KW>
-__global__ __launch_bounds__(64 * KW, KW == 16 ? 1 : 2) void attend_kernel(AttendArgs a) {
+// NT: tiles of 16 rows; NU: units of 16 keys in a wave's step; KW: waves that
+// share a tile's keys; RW: tiles a block takes, each by waves of its own (KW =
+// 1: the waves have nothing to do with each other); ONE: a step's keys are of
+// one page (pages of at least 16 NU tokens).
+template <int DH, int NT, int NU, int KW, int RW, bool ONE>
+__global__ __launch_bounds__(64 * KW * RW, KW == 16 ? 1 : NT == 1 ? (DH == 64 ? 4 : 3) : NT == 2 && DH == 64 ? 4 : 2) void attend_kernel(AttendArgs a) {
+  static_assert(KW == 1 || RW == 1, "the waves of a block meet over one tile");
   constexpr int R = 16 * NT;    // rows of the tile
   constexpr int NM = DH / 32;   // MFMAs along the head dimension
   constexpr int ND = DH / 16;   // 16-dimension groups of the output
   constexpr int LD = DH + 4;
   constexpr int KS = 16 * NU;   // keys of a step
-  __shared__ __attribute__((aligned(16))) float lds_o[KW][R][LD];
+  __shared__ __attribute__((aligned(16))) float lds_o[KW == 1 ? 1 : KW][KW == 1 ? 1 : R][LD];
   __shared__ float lds_m[KW][R], lds_l[KW][R];
   const Kv8Batch& b = a.b;
   const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wave = KW == 1 ? 0 : __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, g = lane >> 4;
   const int h = blockIdx.x % b.NKV;
   const int rest = blockIdx.x / b.NKV;
   const int sp = rest % a.nsplit;
-  const int tile = a.tiles - 1 - rest / a.nsplit;  // the longest rows of a prompt first
+  // the longest rows of a prompt first
+  const int tile = a.tiles - 1 - rest / a.nsplit * RW - (RW > 1 ? __builtin_amdgcn_readfirstlane(tid >> 6) : 0);
+  if (RW > 1 && tile < 0) return;
   const Kv8Span span = kv8_tile_span(b, a.tt, tile);
   if (span.n == 0) return;
   const int rows = span.n * a.G;
@@ -110,47 +110,55 @@ __global__ __launch_bounds__(64 * KW, KW == 16 ? 1 : 2) void attend_kernel(Atten
   if (k0 >= kend) return;
   const int k1 = min(kend, k0 + pk);
 
-  // Page ids and exponents of 64 pages from wbase on, one per lane.
+  // 64 pages from wbase on, one per lane: where the head's rows begin, and
+  // what Step says of the page.  wend: the first position behind them.
   const int* trow = b.table + (size_t)span.seq * b.table_stride;
-  int wbase = -(1 << 30), wid = -1, wexp = 0;
+  int wbase = 0, wexp = 0;
+  int64_t wend = 0;
+  uint32_t wlo = 0, whi = 0;
   auto window = [&](int pg) {
     wbase = pg;
+    wend = (int64_t)(pg + 64) << b.pshift;
     const int p = pg + lane;
-    wid = -1;
+    int id = -1;
     if (p < b.table_pages && ((int64_t)p << b.pshift) < k1) {
-      wid = trow[p];
-      if ((unsigned)wid >= (unsigned)b.pages) wid = -1;
+      id = trow[p];
+      if ((unsigned)id >= (unsigned)b.pages) id = -1;
     }
-    const size_t e = (size_t)(wid >= 0 ? wid : 0) * b.NKV + h;
-    wexp = ((int)a.k_exp[e] & 0xff) | ((int)a.v_exp[e] & 0xff) << 8;
+    const size_t e = (size_t)(id >= 0 ? id : 0) * b.NKV + h;
+    const size_t at = e * ((size_t)DH << b.pshift);
+    wlo = (uint32_t)at;
+    whi = (uint32_t)(at >> 32);
+    wexp = ((int)a.k_exp[e] & 0xff) | ((int)a.v_exp[e] & 0xff) << 8 | (id >= 0 ? kThere : 0);
   };
-  const size_t head_bytes = (size_t)DH << b.pshift;
-  const int kl = col * DH + 16 * g, vl = lane * (DH / 4);
-  auto within = [&](int kb) {
-    if ((kb >> b.pshift) < wbase || ((kb + KS - 1) >> b.pshift) >= wbase + 64) window(kb >> b.pshift);
-  };
-  auto fetch = [&](Step<DH, NU>& s, int kb) {
-    within(kb);
+  // The codes of the step at kb; `on` false: nothing is wanted of them (one
+  // line is read).
+  const uint32_t kl = col * DH + 16 * g, vl = lane * (DH / 4);
+  auto fetch = [&](Step<DH, NU>& s, int kb, bool on) {
+    if (kb + KS > wend) window(kb >> b.pshift);
+    const uint32_t ko = on ? kl : 0, vo = on ? vl : 0;
+    size_t at = 0;
 #pragma unroll
     for (int u = 0; u < NU; u++) {
       const int ku = kb + 16 * u;
-      const int id = __builtin_amdgcn_readlane(wid, (ku >> b.pshift) - wbase);
-      s.there[u] = id >= 0 && ku < k1;
-      const size_t page = ((size_t)(s.there[u] ? id : 0) * b.NKV + h) * head_bytes;
-      const int slot = ku & ((1 << b.pshift) - 1);
-      const uint8_t* kp = a.k + page + slot * DH;
-      const uint8_t* vp = a.v + page + slot * DH;
+      if (u == 0 || !ONE) {
+        const int w = (ku >> b.pshift) - wbase;
+        at = (uint32_t)__builtin_amdgcn_readlane((int)wlo, w) |
+             (size_t)(uint32_t)__builtin_amdgcn_readlane((int)whi, w) << 32;
+        s.ex[u] = __builtin_amdgcn_readlane(wexp, w);
+        at += (ku & ((1 << b.pshift) - 1)) * DH;
+      } else {
+        s.ex[u] = s.ex[0];
+        at += 16 * DH;
+      }
+      const uint8_t *kp = a.k + at, *vp = a.v + at;
 #pragma unroll
       for (int x = 0; x < DH / 64; x++) {
-        s.k[u][x] = *reinterpret_cast<const u32x4*>(kp + kl + 64 * x);
-        s.v[u][x] = *reinterpret_cast<const u32x4*>(vp + vl + 16 * x);
+        s.k[u][x] = *reinterpret_cast<const u32x4*>(kp + ko + 64 * x);
+        s.v[u][x] = *reinterpret_cast<const u32x4*>(vp + vo + 16 * x);
       }
     }
   };
-
-  Step<DH, NU> cur;
-  int kb = k0 + wave * KS;
-  if (kb < k1) fetch(cur, kb);
 
   // Q: row r = 16 t + col, dimensions 64 (m / 2) + 16 g + 8 (m % 2) + j
   half8 q[NT][NM];
@@ -164,41 +172,56 @@ __global__ __launch_bounds__(64 * KW, KW == 16 ? 1 : 2) void attend_kernel(Atten
 #pragma unroll
     for (int m = 0; m < NM; m++) q[t][m] = ld_h8(p + 64 * (m >> 1) + 8 * (m & 1));
   }
+  Step<DH, NU> cur;
+  int kb = k0 + wave * KS;
+  fetch(cur, kb, kb < k1);
+  // waited for here, once (they were issued first), and not in every step
+#pragma unroll
+  for (int t = 0; t < NT; t++)
+#pragma unroll
+    for (int m = 0; m < NM; m++) asm volatile("" : "+v"(q[t][m]));
 
   // m: what the exponentials are relative to, the same in the four lanes of a
   // row: at least the row's maximum less kSlack so far.  It moves only when a
   // score passes it by more, so that most steps neither join the lanes'
-  // maxima nor touch the sums; weights stay below 2^kSlack.
+  // maxima nor touch the sums; weights stay below 2^kSlack.  bar: how far a
+  // score may pass it; -inf while the row has seen no key (m is then 0).
   constexpr float kSlack = 8.f;
-  float m[NT], l[NT];
-  floatx4 o[ND][NT];
+  float m[NT], bar[NT];
+  floatx4 o[ND][NT], l[NT];  // l: the sum of the row's weights, four times
 #pragma unroll
   for (int t = 0; t < NT; t++) {
-    m[t] = -INFINITY;
-    l[t] = 0.f;
+    m[t] = 0.f;
+    bar[t] = -INFINITY;
+    l[t] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int d = 0; d < ND; d++) o[d][t] = floatx4{0.f, 0.f, 0.f, 0.f};
   }
 
   // whether a step holds keys that some row does not attend to
   auto at_edge = [&](const Step<DH, NU>& s, int kb) {
-    bool inner = kb + KS - 1 <= span.pos;
+    int all = s.ex[0];
 #pragma unroll
-    for (int u = 0; u < NU; u++) inner = inner && s.there[u];
-    return !inner;
+    for (int u = 1; u < (ONE ? 1 : NU); u++) all &= s.ex[u];
+    return kb + KS - 1 > span.pos || !(all & kThere);
   };
 
+  half8 ones;
+#pragma unroll
+  for (int j = 0; j < 8; j++) ones[j] = (half_t)1.f;
+  asm volatile("" : "+v"(ones));  // in vector registers: scalar ones are spilled and read back in every step
   uint32_t nan = 0;
-  auto step = [&](Step<DH, NU>& s, int kb, const float (&ks)[NU], const float (&vs)[NU], bool edge) {
+  auto step = [&](Step<DH, NU>& s, int kb) {
+    const bool edge = at_edge(s, kb);
     floatx4 sc[NU][NT];
 #pragma unroll
     for (int u = 0; u < NU; u++) {
       half8 kf[NM];
+      const float ks = k_scale(s.ex[u]);
 #pragma unroll
       for (int x = 0; x < NM; x++) {
         const uint32_t w0 = s.k[u][x >> 1][2 * (x & 1)], w1 = s.k[u][x >> 1][2 * (x & 1) + 1];
-        kf[x] = join(kv8_up<false>(w0, ks[u]), kv8_up<true>(w0, ks[u]), kv8_up<false>(w1, ks[u]),
-                     kv8_up<true>(w1, ks[u]));
+        kf[x] = join(kv8_up<false>(w0, ks), kv8_up<true>(w0, ks), kv8_up<false>(w1, ks), kv8_up<true>(w1, ks));
       }
 #pragma unroll
       for (int t = 0; t < NT; t++) {
@@ -215,47 +238,53 @@ __global__ __launch_bounds__(64 * KW, KW == 16 ? 1 : 2) void attend_kernel(Atten
         for (int t = 0; t < NT; t++)
 #pragma unroll
           for (int j = 0; j < 4; j++)
-            if (!s.there[u] || kb + 16 * u + 4 * g + j > lim[t]) sc[u][t][j] = -INFINITY;
+            if (!(s.ex[u] & kThere) || kb + 16 * u + 4 * g + j > lim[t]) sc[u][t][j] = -INFINITY;
     }
     float mx[NT];
     bool up = false;
 #pragma unroll
     for (int t = 0; t < NT; t++) {
-      mx[t] = sc[0][t][0];
+      mx[t] = -INFINITY;
 #pragma unroll
       for (int u = 0; u < NU; u++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) mx[t] = fmaxf(mx[t], sc[u][t][j]);
-      mx[t] *= a.c;
-      up |= mx[t] > m[t] + kSlack;
+        for (int j = 0; j < 4; j++) {
+          sc[u][t][j] = __builtin_fmaf(sc[u][t][j], a.c, -m[t]);
+          mx[t] = fmaxf(mx[t], sc[u][t][j]);
+        }
+      up |= mx[t] > bar[t];
     }
     if (__any(up)) {
 #pragma unroll
       for (int t = 0; t < NT; t++) {
-        const float mn = fmaxf(m[t], xor32_max(xor16_max(mx[t])));
-        const float al = __builtin_amdgcn_exp2f(m[t] - (mn == -INFINITY ? 0.f : mn));
-        m[t] = mn;
-        l[t] *= al;
+        const float top = xor32_max(xor16_max(mx[t]));
+        if (top > bar[t]) {  // the same in the row's four lanes
+          const float al = bar[t] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(-top);
+          m[t] += top;
+          bar[t] = kSlack;
 #pragma unroll
-        for (int d = 0; d < ND; d++)
+          for (int u = 0; u < NU; u++)
 #pragma unroll
-          for (int j = 0; j < 4; j++) o[d][t][j] *= al;
+            for (int j = 0; j < 4; j++) sc[u][t][j] -= top;
+#pragma unroll
+          for (int j = 0; j < 4; j++) l[t][j] *= al;
+#pragma unroll
+          for (int d = 0; d < ND; d++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) o[d][t][j] *= al;
+        }
       }
     }
     half8 pf[NU / 2][NT];
 #pragma unroll
     for (int t = 0; t < NT; t++) {
-      const float mu = m[t] == -INFINITY ? 0.f : m[t];  // no key yet: exp2(-inf), not exp2(nan)
-      float sum = 0.f;
 #pragma unroll
       for (int u = 0; u < NU; u++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u][t][j], a.c, -mu));
-          sum += p;
-          pf[u >> 1][t][4 * (u & 1) + j] = (half_t)p;
-        }
-      l[t] += sum;
+        for (int j = 0; j < 4; j++) pf[u >> 1][t][4 * (u & 1) + j] = (half_t)__builtin_amdgcn_exp2f(sc[u][t][j]);
+      // the weights' sums on the matrix cores, of the weights as rounded
+#pragma unroll
+      for (int y = 0; y < NU / 2; y++) l[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pf[y][t], l[t], 0, 0, 0);
     }
     // Values that no row of the tile attends to may be anything (rows not yet
     // written): cleared.  NaN among those that some row attends to and some
@@ -265,7 +294,7 @@ __global__ __launch_bounds__(64 * KW, KW == 16 ? 1 : 2) void attend_kernel(Atten
 #pragma unroll
       for (int u = 0; u < NU; u++) {
         const int first = kb + 16 * u + 4 * g;  // the lane's four keys
-        const int n = s.there[u] ? clampi(k1 - first, 0, 4) : 0;
+        const int n = s.ex[u] & kThere ? clampi(k1 - first, 0, 4) : 0;
         const uint32_t mine = n == 4 ? 0xffffffffu : (1u << (8 * n)) - 1;
 #pragma unroll
         for (int x = 0; x < DH / 64; x++)
@@ -281,35 +310,36 @@ __global__ __launch_bounds__(64 * KW, KW == 16 ? 1 : 2) void attend_kernel(Atten
     for (int y = 0; y < NU / 2; y++)
 #pragma unroll
       for (int d = 0; d < ND; d++) {
+        const float v0 = v_scale(s.ex[2 * y]), v1 = v_scale(s.ex[2 * y + 1]);
         const uint32_t w0 = s.v[2 * y][d >> 2][d & 3], w1 = s.v[2 * y + 1][d >> 2][d & 3];
-        const half8 vf = join(kv8_up<false>(w0, vs[2 * y]), kv8_up<true>(w0, vs[2 * y]),
-                              kv8_up<false>(w1, vs[2 * y + 1]), kv8_up<true>(w1, vs[2 * y + 1]));
+        const half8 vf = join(kv8_up<false>(w0, v0), kv8_up<true>(w0, v0), kv8_up<false>(w1, v1), kv8_up<true>(w1, v1));
 #pragma unroll
         for (int t = 0; t < NT; t++) o[d][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[y][t], o[d][t], 0, 0, 0);
       }
   };
 
-  while (kb < k1) {
-    // the exponents, before the window may move on
-    float ks[NU], vs[NU];
-#pragma unroll
-    for (int u = 0; u < NU; u++) {
-      const int ex = __builtin_amdgcn_readlane(wexp, ((kb + 16 * u) >> b.pshift) - wbase);
-      ks[u] = kv8_scale((int8_t)(ex & 0xff));
-      vs[u] = kv8_scale((int8_t)(ex >> 8 & 0xff));
-    }
-    Step<DH, NU> nxt;
+  // One step on `now`, with the loads of the one behind it under way into
+  // `then`; whether there is one.  Behind the last step they are of one line,
+  // so that every path has the same loads outstanding and waits for no more
+  // than it needs.
+  auto turn = [&](Step<DH, NU>& now, Step<DH, NU>& then) {
     const int kn = kb + KS * KW;
-    if (kn < k1) fetch(nxt, kn);
-    step(cur, kb, ks, vs, at_edge(cur, kb));
-    if (kn < k1) cur = nxt;
+    fetch(then, kn < k1 ? kn : kb, kn < k1);
+    step(now, kb);
     kb = kn;
+    return kn < k1;
+  };
+  if (kb < k1) {
+    Step<DH, NU> nxt;
+    while (turn(cur, nxt) && turn(nxt, cur)) {
+    }
   }
   if (__any(nan != 0)) {
     // rare: how many NaN of each dimension a row attends to, as a product of
     // zeros and ones, over the steps that had them taken out
+    wend = 0;
     for (kb = k0 + wave * KS; kb < k1; kb += KS * KW) {
-      fetch(cur, kb);
+      fetch(cur, kb, true);
       if (!at_edge(cur, kb)) continue;
 #pragma unroll
       for (int y = 0; y < NU / 2; y++) {
@@ -319,7 +349,7 @@ __global__ __launch_bounds__(64 * KW, KW == 16 ? 1 : 2) void attend_kernel(Atten
 #pragma unroll
           for (int j = 0; j < 8; j++) {
             const int u = 2 * y + (j >> 2);
-            sees[t][j] = cur.there[u] && kb + 16 * u + 4 * g + (j & 3) <= lim[t] ? (half_t)1.f : (half_t)0.f;
+            sees[t][j] = (cur.ex[u] & kThere) && kb + 16 * u + 4 * g + (j & 3) <= lim[t] ? (half_t)1.f : (half_t)0.f;
           }
 #pragma unroll
         for (int d = 0; d < ND; d++) {
@@ -341,10 +371,29 @@ __global__ __launch_bounds__(64 * KW, KW == 16 ? 1 : 2) void attend_kernel(Atten
     }
   }
 
+  if constexpr (KW == 1) {  // the tile's only wave: lane (col, g) has 4 dimensions of 16 in row col
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+      const int r = 16 * t + col;
+      const float inv = l[t][0] == 0.f ? 0.f : 1.f / l[t][0];
+      const int tok = r / a.G, hg = r - tok * a.G;
+      half_t* y = a.out + (span.row + tok) * a.out_row + (h * a.G + hg) * a.out_head + 4 * g;
+      if (r < rows) {
+#pragma unroll
+        for (int d = 0; d < ND; d++) {
+          half4 z;
+#pragma unroll
+          for (int j = 0; j < 4; j++) z[j] = (half_t)(o[d][t][j] * inv);
+          *reinterpret_cast<half4*>(y + 16 * d) = z;
+        }
+      }
+    }
+    return;
+  }
   // The waves meet: maximum over the waves, every wave's sums brought to it.
 #pragma unroll
   for (int t = 0; t < NT; t++) {
-    l[t] = xor32_sum(xor16_sum(l[t]));
+    if (bar[t] == -INFINITY) m[t] = -INFINITY;  // no key
     if (g == 0) lds_m[wave][16 * t + col] = m[t];
   }
   __syncthreads();
@@ -355,7 +404,7 @@ __global__ __launch_bounds__(64 * KW, KW == 16 ? 1 : 2) void attend_kernel(Atten
 #pragma unroll
     for (int w = 1; w < KW; w++) mm = fmaxf(mm, lds_m[w][r]);
     const float al = __builtin_amdgcn_exp2f(m[t] - (mm == -INFINITY ? 0.f : mm));
-    if (g == 0) lds_l[wave][r] = l[t] * al;
+    if (g == 0) lds_l[wave][r] = l[t][0] * al;
     if (r < rows) {
 #pragma unroll
       for (int d = 0; d < ND; d++) *reinterpret_cast<floatx4*>(&lds_o[wave][r][16 * d + 4 * g]) = o[d][t] * al;
@@ -459,7 +508,7 @@ int plan(const char* op, const Kv8Batch& b, const ane_kv8_batch& given, int DH, 
   if (b.nseq == 0 || b.rows == 0) return ANE_OK;
   // rows of the longest sequence, or of the mean one where that is not known
   const int64_t most = (int64_t)G * (given.max_new ? std::min(given.max_new, b.rows) : (b.rows + b.nseq - 1) / b.nseq);
-  p->nt = most <= 16 ? 1 : most <= 32 || DH == 128 ? 2 : 4;
+  p->nt = most <= 16 ? 1 : most <= 32 || DH == 128 || (given.max_len && given.max_len <= 512) ? 2 : 4;
   while (16 * p->nt < G) p->nt *= 2;
   p->tt = 16 * p->nt / G;
   p->tiles = kv8_count(b.nseq, b.rows, kv8_tiles(p->tt));
@@ -467,15 +516,15 @@ int plan(const char* op, const Kv8Batch& b, const ane_kv8_batch& given, int DH, 
   const int cap = b.table_pages << b.pshift;
   const int len = given.max_len ? std::min(given.max_len, cap) : cap;
   if (p->nt == 1) {
-    const int r16 = 16 * (DH == 64 ? 64 : 32);
-    p->kw = blocks >= 128 || len <= 2 * r16 ? 16 : 4;
-    if (const char* f = getenv("ZZ_KW")) p->kw = atoi(f);
+    p->kw = DH == 64 && (len <= 1152 || (blocks >= 128 && len <= 2048)) ? 16 : 4;
     p->round = p->kw * (DH == 64 ? 64 : 32);
-  } else p->round = 128;
+  } else {
+    p->round = 128;
+    if (len <= 512) p->kw = 1;
+  }
   int64_t want = p->kw == 16 ? 256 : p->nt == 1 ? 1024 : 512;
-  if (const char* f = getenv("ZZ_WANT")) want = atoi(f);
-  int64_t ns = std::max<int64_t>((want + blocks - 1) / blocks, p->nt == 1 ? (len + 4095) / 4096 : 1);
-  if (p->kw == 16 && len <= 2 * p->round) ns = 1;
+  int64_t ns = std::max<int64_t>(blocks >= 512 ? 1 : (want + blocks - 1) / blocks, p->nt == 1 ? (len + 4095) / 4096 : 1);
+  if ((p->kw == 16 && len <= 2 * p->round) || p->kw == 1) ns = 1;
   ns = std::min<int64_t>(ns, (len + p->round - 1) / p->round);
   ns = std::max<int64_t>(1, std::min<int64_t>(ns, kMaxSplit));
   p->nsplit = (int)ns;
@@ -487,19 +536,26 @@ int plan(const char* op, const Kv8Batch& b, const ane_kv8_batch& given, int DH, 
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
-template <int DH, int NT, int NU, int KW>
+template <int DH, int NT, int NU, int KW, int RW>
 void launch_form(const AttendArgs& a, hipStream_t st) {
-  const dim3 grid((uint32_t)a.tiles * a.b.NKV * a.nsplit);
-  hipLaunchKernelGGL((attend_kernel<DH, NT, NU, KW>), grid, dim3(64 * KW), 0, st, a);
+  const dim3 grid(((uint32_t)a.tiles + RW - 1) / RW * a.b.NKV * a.nsplit), block(64 * KW * RW);
+  if (16 * NU <= 1 << a.b.pshift)
+    hipLaunchKernelGGL((attend_kernel<DH, NT, NU, KW, RW, true>), grid, block, 0, st, a);
+  else
+    hipLaunchKernelGGL((attend_kernel<DH, NT, NU, KW, RW, false>), grid, block, 0, st, a);
 }
 
 template <int DH>
 void launch(const AttendArgs& a, const Plan& p, hipStream_t st) {
   constexpr int NU1 = DH == 64 ? 4 : 2;
-  if (p.nt == 1 && p.kw == 16) launch_form<DH, 1, NU1, 16>(a, st);
-  else if (p.nt == 1) launch_form<DH, 1, NU1, 4>(a, st);
-  else if (p.nt == 2) launch_form<DH, 2, 2, 4>(a, st);
-  else if constexpr (DH == 64) launch_form<DH, 4, 2, 4>(a, st);
+  if (DH == 64 && p.nt == 1 && p.kw == 16) launch_form<64, 1, 4, 16, 1>(a, st);
+  else if (p.nt == 1) launch_form<DH, 1, NU1, 4, 1>(a, st);
+  else if (p.nt == 2 && p.kw == 4) launch_form<DH, 2, 2, 4, 1>(a, st);
+  else if (p.nt == 2) launch_form<DH, 2, 2, 1, 4>(a, st);
+  else if constexpr (DH == 64) {
+    if (p.kw == 4) launch_form<DH, 4, 2, 4, 1>(a, st);
+    else launch_form<DH, 4, 2, 1, 4>(a, st);
+  }
   if (a.nsplit > 1)
     hipLaunchKernelGGL(join_kernel<DH>, dim3((uint32_t)a.tiles * a.b.NKV, (a.tt * a.G + 3) / 4), dim3(256), 0, st, a);
 }
