@@ -82,12 +82,16 @@ __device__ __forceinline__ float v_scale(int ex) { return kv8_scale((int8_t)(ex 
 // 1: the waves have nothing to do with each other); ONE: a step's keys are of
 // one page (pages of at least 16 NU tokens).
 template <int DH, int NT, int NU, int KW, int RW, bool ONE>
-__global__ __launch_bounds__(64 * KW * RW, KW == 16 ? 1 : NT == 1 ? (DH == 64 ? 4 : 3) : NT == 2 && DH == 64 ? 4 : 2) void attend_kernel(AttendArgs a) {
+__global__ __launch_bounds__(64 * KW * RW, KW == 16 ? 1 : NT == 1 ? (DH == 64 ? 4 : 3) : DH == 64 ? (NT == 2 ? 4 : 3) : 2) void attend_kernel(AttendArgs a) {
   static_assert(KW == 1 || RW == 1, "the waves of a block meet over one tile");
   constexpr int R = 16 * NT;    // rows of the tile
   constexpr int NM = DH / 32;   // MFMAs along the head dimension
   constexpr int ND = DH / 16;   // 16-dimension groups of the output
-  constexpr int LD = DH + 4;
+  // the waves meet over the output's dimensions in parts that leave LDS for
+  // as many blocks as there are registers for
+  constexpr int PASS = KW == 4 && R * DH > 2048 ? 2 : 1;
+  constexpr int DP = DH / PASS;
+  constexpr int LD = DP + 4;
   constexpr int KS = 16 * NU;   // keys of a step
   __shared__ __attribute__((aligned(16))) float lds_o[KW == 1 ? 1 : KW][KW == 1 ? 1 : R][LD];
   __shared__ float lds_m[KW][R], lds_l[KW][R];
@@ -403,42 +407,51 @@ __global__ __launch_bounds__(64 * KW * RW, KW == 16 ? 1 : NT == 1 ? (DH == 64 ? 
     float mm = lds_m[0][r];
 #pragma unroll
     for (int w = 1; w < KW; w++) mm = fmaxf(mm, lds_m[w][r]);
-    const float al = __builtin_amdgcn_exp2f(m[t] - (mm == -INFINITY ? 0.f : mm));
-    if (g == 0) lds_l[wave][r] = l[t][0] * al;
-    if (r < rows) {
-#pragma unroll
-      for (int d = 0; d < ND; d++) *reinterpret_cast<floatx4*>(&lds_o[wave][r][16 * d + 4 * g]) = o[d][t] * al;
-    }
+    m[t] = __builtin_amdgcn_exp2f(m[t] - (mm == -INFINITY ? 0.f : mm));  // the wave's factor from here on
+    if (g == 0) lds_l[wave][r] = l[t][0] * m[t];
   }
-  __syncthreads();
   const bool whole = pk >= kend;
   float* part = a.part + (((size_t)tile * b.NKV + h) * a.nsplit + sp) * ((size_t)a.tt * a.G * (DH + 2));
-  for (int c = tid; c < rows * (DH / 4); c += 64 * KW) {
-    const int r = c / (DH / 4), d0 = c % (DH / 4) * 4;
-    floatx4 x = *reinterpret_cast<const floatx4*>(&lds_o[0][r][d0]);
-    float ls = lds_l[0][r];
 #pragma unroll
-    for (int w = 1; w < KW; w++) {
-      x += *reinterpret_cast<const floatx4*>(&lds_o[w][r][d0]);
-      ls += lds_l[w][r];
+  for (int z = 0; z < PASS; z++) {
+    if (z > 0) __syncthreads();
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+      const int r = 16 * t + col;
+      if (r < rows) {
+#pragma unroll
+        for (int d = 0; d < ND / PASS; d++)
+          *reinterpret_cast<floatx4*>(&lds_o[wave][r][16 * d + 4 * g]) = o[z * (ND / PASS) + d][t] * m[t];
+      }
     }
-    if (whole) {
-      const float inv = ls == 0.f ? 0.f : 1.f / ls;
-      const int tok = r / a.G, hg = r - tok * a.G;
-      half4 y;
+    __syncthreads();
+    for (int c = tid; c < rows * (DP / 4); c += 64 * KW) {
+      const int r = c / (DP / 4), d0 = c % (DP / 4) * 4, d = z * DP + d0;
+      floatx4 x = *reinterpret_cast<const floatx4*>(&lds_o[0][r][d0]);
+      float ls = lds_l[0][r];
 #pragma unroll
-      for (int j = 0; j < 4; j++) y[j] = (half_t)(x[j] * inv);
-      *reinterpret_cast<half4*>(a.out + (span.row + tok) * a.out_row + (h * a.G + hg) * a.out_head + d0) = y;
-    } else {
-      float* p = part + (size_t)r * (DH + 2);
+      for (int w = 1; w < KW; w++) {
+        x += *reinterpret_cast<const floatx4*>(&lds_o[w][r][d0]);
+        ls += lds_l[w][r];
+      }
+      if (whole) {
+        const float inv = ls == 0.f ? 0.f : 1.f / ls;
+        const int tok = r / a.G, hg = r - tok * a.G;
+        half4 y;
 #pragma unroll
-      for (int j = 0; j < 4; j++) p[d0 + j] = x[j];
-      if (d0 == 0) {
-        float mm = lds_m[0][r];
+        for (int j = 0; j < 4; j++) y[j] = (half_t)(x[j] * inv);
+        *reinterpret_cast<half4*>(a.out + (span.row + tok) * a.out_row + (h * a.G + hg) * a.out_head + d) = y;
+      } else {
+        float* p = part + (size_t)r * (DH + 2);
 #pragma unroll
-        for (int w = 1; w < KW; w++) mm = fmaxf(mm, lds_m[w][r]);
-        p[DH] = mm;
-        p[DH + 1] = ls;
+        for (int j = 0; j < 4; j++) p[d + j] = x[j];
+        if (d == 0) {
+          float mm = lds_m[0][r];
+#pragma unroll
+          for (int w = 1; w < KW; w++) mm = fmaxf(mm, lds_m[w][r]);
+          p[DH] = mm;
+          p[DH + 1] = ls;
+        }
       }
     }
   }
@@ -508,7 +521,8 @@ int plan(const char* op, const Kv8Batch& b, const ane_kv8_batch& given, int DH, 
   if (b.nseq == 0 || b.rows == 0) return ANE_OK;
   // rows of the longest sequence, or of the mean one where that is not known
   const int64_t most = (int64_t)G * (given.max_new ? std::min(given.max_new, b.rows) : (b.rows + b.nseq - 1) / b.nseq);
-  p->nt = most <= 16 ? 1 : most <= 32 || DH == 128 || (given.max_len && given.max_len <= 512) ? 2 : 4;
+  p->nt = most <= 16 ? 1 : most <= 32 || DH == 128 ? 2 : 3;
+  if (p->nt == 3 && 32 / G * 48 > 48 / G * 38) p->nt = 2;  // where 48 rows would stay a fifth emptier than 32
   while (16 * p->nt < G) p->nt *= 2;
   p->tt = 16 * p->nt / G;
   p->tiles = kv8_count(b.nseq, b.rows, kv8_tiles(p->tt));
@@ -553,8 +567,8 @@ void launch(const AttendArgs& a, const Plan& p, hipStream_t st) {
   else if (p.nt == 2 && p.kw == 4) launch_form<DH, 2, 2, 4, 1>(a, st);
   else if (p.nt == 2) launch_form<DH, 2, 2, 1, 4>(a, st);
   else if constexpr (DH == 64) {
-    if (p.kw == 4) launch_form<DH, 4, 2, 4, 1>(a, st);
-    else launch_form<DH, 4, 2, 1, 4>(a, st);
+    if (p.kw == 4) launch_form<DH, 3, 2, 4, 1>(a, st);
+    else launch_form<DH, 3, 2, 1, 4>(a, st);
   }
   if (a.nsplit > 1)
     hipLaunchKernelGGL(join_kernel<DH>, dim3((uint32_t)a.tiles * a.b.NKV, (a.tt * a.G + 3) / 4), dim3(256), 0, st, a);
