@@ -2,11 +2,12 @@
 // (ane_kv8_append), and the checks both cache operators share.
 //
 // Mathematics: include/ane_serve.h.  One block per (page that gets rows, kv
-// head) reads its keys and values, rotates the keys, takes the largest
-// magnitude of each side over the block, and writes codes; no other block
-// touches that page and head, so a page's rows from before can be rounded
-// again in place when its exponent rises.  Blocks behind the kv heads rotate
-// the queries of the same rows.
+// head) holds its new keys and values in registers, rotates the keys, takes
+// the largest magnitude of each side over the block, and writes codes; no
+// other block touches that page and head, so a page's rows from before can be
+// rounded again in place when its exponent rises.  V's codes go through LDS
+// into the order of the cache.  Blocks behind the kv heads rotate the queries
+// of the same rows, kQHeads heads each.
 #include <algorithm>
 
 #include "kv8.h"
@@ -16,7 +17,7 @@ namespace ane {
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kQHeads = 4;
 
 struct AppendArgs {
   Kv8Batch b;
@@ -26,26 +27,32 @@ struct AppendArgs {
   half_t* q_out;
   const float *cos, *sin;
   int64_t q_row, q_head, k_row, k_head, v_row, v_head, qo_row, qo_head;
+  int heads;
 };
 
 struct F8 {
   float x[8];
 };
 
-__device__ __forceinline__ F8 load8(const half_t* p) {
-  const half8 h = ld_h8(p);
+__device__ __forceinline__ F8 wide8(half8 h) {
   F8 f;
 #pragma unroll
   for (int j = 0; j < 8; j++) f.x[j] = (float)h[j];
   return f;
 }
 
-// the four pairs of 8 dimensions from d0 on, at position pos
+// the cosines and sines of the four pairs of dimensions from d0 on
+struct Turn {
+  float4 c, s;
+};
 template <int DH>
-__device__ __forceinline__ F8 rotate8(const F8& f, const float* cs, const float* sn, int pos, int d0) {
-  const float4 c = *reinterpret_cast<const float4*>(cs + (size_t)pos * (DH / 2) + d0 / 2);
-  const float4 s = *reinterpret_cast<const float4*>(sn + (size_t)pos * (DH / 2) + d0 / 2);
-  const float cc[4] = {c.x, c.y, c.z, c.w}, ss[4] = {s.x, s.y, s.z, s.w};
+__device__ __forceinline__ Turn turn_of(const float* cs, const float* sn, int pos, int d0) {
+  return {*reinterpret_cast<const float4*>(cs + (size_t)pos * (DH / 2) + d0 / 2),
+          *reinterpret_cast<const float4*>(sn + (size_t)pos * (DH / 2) + d0 / 2)};
+}
+__device__ __forceinline__ F8 rotate8(half8 h, const Turn& w) {
+  const F8 f = wide8(h);
+  const float cc[4] = {w.c.x, w.c.y, w.c.z, w.c.w}, ss[4] = {w.s.x, w.s.y, w.s.z, w.s.w};
   F8 r;
 #pragma unroll
   for (int j = 0; j < 4; j++) {
@@ -92,12 +99,13 @@ __device__ __forceinline__ uint32_t again4(uint32_t c, float down) {
   return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(hi[0] * down, hi[1] * down, r, true);
 }
 
-template <int DH>
-__global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs a) {
-  constexpr int CPR = DH / 8;  // chunks of 8 dimensions per row
+// NC * TH chunks of 8 dimensions are a page's.
+template <int DH, int NC, int TH>
+__global__ __launch_bounds__(TH) void append_kernel(AppendArgs a) {
+  constexpr int CPR = DH / 8;  // chunks per row
   constexpr int T = DH / 16;
-  extern __shared__ __attribute__((aligned(16))) uint8_t vbuf[];  // the page's V codes
-  __shared__ uint32_t top[2][kThreads / 64];
+  __shared__ __attribute__((aligned(16))) uint8_t vbuf[NC * TH * 8];  // the page's V codes
+  __shared__ uint32_t top[2][TH / 64];
   const Kv8Batch& b = a.b;
   const int tid = threadIdx.x;
   const int P = 1 << b.pshift;
@@ -105,37 +113,74 @@ __global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs a) {
   if (span.n == 0) return;
   const int nr = span.n, row0 = span.row, t0 = span.pos;
 
-  if ((int)blockIdx.y >= b.NKV) {  // a query head
-    const int h = blockIdx.y - b.NKV;
-    for (int c = tid; c < nr * CPR; c += kThreads) {
+  if ((int)blockIdx.y >= b.NKV) {  // query heads
+    const int h0 = (blockIdx.y - b.NKV) * kQHeads;
+    for (int c = tid; c < nr * CPR; c += TH) {
       const int r = c / CPR, d0 = c % CPR * 8;
-      const F8 f = rotate8<DH>(load8(a.xq + (row0 + r) * a.q_row + h * a.q_head + d0), a.cos, a.sin, t0 + r, d0);
-      half8 o;
+      const Turn w = turn_of<DH>(a.cos, a.sin, t0 + r, d0);
+      const half_t* x = a.xq + (row0 + r) * a.q_row + d0;
+      half_t* y = a.q_out + (row0 + r) * a.qo_row + d0;
+      half8 in[kQHeads];
 #pragma unroll
-      for (int j = 0; j < 8; j++) o[j] = (half_t)f.x[j];
-      st_h8(a.q_out + (row0 + r) * a.qo_row + h * a.qo_head + d0, o);
+      for (int k = 0; k < kQHeads; k++)
+        if (h0 + k < a.heads) in[k] = ld_h8(x + (h0 + k) * a.q_head);
+#pragma unroll
+      for (int k = 0; k < kQHeads; k++)
+        if (h0 + k < a.heads) {
+          const F8 f = rotate8(in[k], w);
+          half8 o;
+#pragma unroll
+          for (int j = 0; j < 8; j++) o[j] = (half_t)f.x[j];
+          st_h8(y + (h0 + k) * a.qo_head, o);
+        }
     }
     return;
   }
 
   const int h = blockIdx.y;
-  const int id = kv8_page(b, span.seq, t0 >> b.pshift);
-  if (id < 0) return;
   const half_t* xk = a.xk + row0 * a.k_row + h * a.k_head;
   const half_t* xv = a.xv + row0 * a.v_row + h * a.v_head;
+  const int id = kv8_page(b, span.seq, t0 >> b.pshift);
+  half8 hk[NC], hv[NC];
+  Turn w[NC];
+#pragma unroll
+  for (int i = 0; i < NC; i++) {
+    const int c = min(i * TH + tid, nr * CPR - 1), r = c / CPR, d0 = c % CPR * 8;
+    hk[i] = ld_h8(xk + r * a.k_row + d0);
+    hv[i] = ld_h8(xv + r * a.v_row + d0);
+    w[i] = turn_of<DH>(a.cos, a.sin, t0 + r, d0);
+  }
+  if (id < 0) return;  // the same in the whole block
   const size_t ph = (size_t)id * b.NKV + h;
   uint8_t* kp = a.k + ph * P * DH;
   uint8_t* vp = a.v + ph * P * DH;
-  const int r0 = t0 & (P - 1);
+  const int r0 = t0 & (P - 1), r1 = r0 + nr;
+  int ok = kKvExpMin, ov = kKvExpMin;
+  if (r0 > 0) {
+    ok = a.k_exp[ph];
+    ov = a.v_exp[ph];
+  }
+  // V's units of 16 tokens that the new rows fill in part: their codes first
+  const int u0 = r0 >> 4, u1 = (r1 - 1) >> 4;
+  {
+    const uint4* src = reinterpret_cast<const uint4*>(vp);
+    uint4* dst = reinterpret_cast<uint4*>(vbuf);
+    for (int c = tid; c < 2 * DH; c += TH) {
+      const int u = c < DH ? u0 : u1, at = u * DH + (c & (DH - 1));
+      const bool part = c < DH ? (r0 & 15) || (u0 == u1 && (r1 & 15)) : u1 > u0 && (r1 & 15);
+      if (part) dst[at] = src[at];
+    }
+  }
+  F8 fk[NC];
   uint32_t mk = 0, mv = 0;
-  for (int c = tid; c < nr * CPR; c += kThreads) {
-    const int r = c / CPR, d0 = c % CPR * 8;
-    F8 fk = rotate8<DH>(load8(xk + r * a.k_row + d0), a.cos, a.sin, t0 + r, d0);
-    F8 fv = load8(xv + r * a.v_row + d0);
-    limit8(fk);
-    limit8(fv);
-    mk = amax8(fk, mk);
-    mv = amax8(fv, mv);
+#pragma unroll
+  for (int i = 0; i < NC; i++) {
+    fk[i] = rotate8(hk[i], w[i]);
+    limit8(fk[i]);
+    mk = amax8(fk[i], mk);  // chunks past the last row repeat it
+    F8 f = wide8(hv[i]);
+    limit8(f);
+    mv = amax8(f, mv);
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) {
@@ -146,20 +191,13 @@ __global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs a) {
     top[0][tid >> 6] = mk;
     top[1][tid >> 6] = mv;
   }
-  __syncthreads();
+  __syncthreads();  // every thread has read the old exponents too
 #pragma unroll
-  for (int w = 0; w < kThreads / 64; w++) {
-    mk = max(mk, top[0][w]);
-    mv = max(mv, top[1][w]);
+  for (int k = 0; k < TH / 64; k++) {
+    mk = max(mk, top[0][k]);
+    mv = max(mv, top[1][k]);
   }
-  int ek = kv8_exponent(mk), ev = kv8_exponent(mv), ok = ek, ov = ev;
-  if (r0 > 0) {
-    ok = a.k_exp[ph];
-    ov = a.v_exp[ph];
-    ek = max(ek, ok);
-    ev = max(ev, ov);
-  }
-  __syncthreads();  // every thread has read the exponents before they change
+  const int ek = max(kv8_exponent(mk), ok), ev = max(kv8_exponent(mv), ov);
   if (tid == 0) {
     a.k_exp[ph] = (int8_t)ek;
     a.v_exp[ph] = (int8_t)ev;
@@ -167,52 +205,55 @@ __global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs a) {
   const float ik = kv8_scale(-ek), iv = kv8_scale(-ev);
   const float tk = ek == kKvExpMax ? 240.f : 448.f, tv = ev == kKvExpMax ? 240.f : 448.f;
 
-  if (ek > ok) {
+  // rows from before, rounded again where the exponent rose
+  if (r0 > 0 && ek > ok) {
     const float down = kv8_scale(ok - ek);
-    uint32_t* w = reinterpret_cast<uint32_t*>(kp);
-    for (int c = tid; c < r0 * DH / 4; c += kThreads) w[c] = again4(w[c], down);
+    uint32_t* x = reinterpret_cast<uint32_t*>(kp);
+    for (int c = tid; c < r0 * DH / 4; c += TH) x[c] = again4(x[c], down);
   }
-  // V's units of 16 tokens from the first that changes to the last
-  const int u0 = ev > ov ? 0 : r0 >> 4, u1 = (r0 + nr - 1) >> 4;
-  if (ev > ov || (r0 & 15) || ((r0 + nr) & 15)) {
-    const uint32_t* src = reinterpret_cast<const uint32_t*>(vp);
-    uint32_t* dst = reinterpret_cast<uint32_t*>(vbuf);
+  if (r0 > 0 && ev > ov) {
     const float down = kv8_scale(ov - ev);
-    for (int c = u0 * 4 * DH + tid; c < (u1 + 1) * 4 * DH; c += kThreads) {
-      uint32_t w = src[c];
-      // tokens tok .. tok + 3 of one dimension
-      const int tok = c / (4 * DH) * 16 + c % (4 * DH) / (16 * T) * 4;
-      if (ev > ov && tok < r0) {
-        const uint32_t z = again4(w, down);
-        const int n = min(r0 - tok, 4);
-        const uint32_t mine = n == 4 ? 0xffffffffu : (1u << (8 * n)) - 1;
-        w = (z & mine) | (w & ~mine);
-      }
-      dst[c] = w;
+    uint32_t* x = reinterpret_cast<uint32_t*>(vp);
+    for (int c = tid; c < u0 * 4 * DH; c += TH) x[c] = again4(x[c], down);  // whole units of them
+    x = reinterpret_cast<uint32_t*>(vbuf);
+    for (int c = u0 * 4 * DH + tid; c < (u0 + 1) * 4 * DH && (r0 & 15); c += TH) {
+      const int n = clampi(r0 - (u0 * 16 + c % (4 * DH) / (16 * T) * 4), 0, 4);  // of the dword's four tokens
+      const uint32_t mine = n == 4 ? 0xffffffffu : (1u << (8 * n)) - 1;
+      x[c] = (again4(x[c], down) & mine) | (x[c] & ~mine);
     }
     __syncthreads();
   }
-  for (int c = tid; c < nr * CPR; c += kThreads) {
-    const int r = c / CPR, d0 = c % CPR * 8;
-    F8 fk = rotate8<DH>(load8(xk + r * a.k_row + d0), a.cos, a.sin, t0 + r, d0);
-    F8 fv = load8(xv + r * a.v_row + d0);
-    limit8(fk);
-    limit8(fv);
-    const uint2 ck = make_uint2(codes4(fk.x, ik, tk), codes4(fk.x + 4, ik, tk));
-    *reinterpret_cast<uint2*>(kp + (r0 + r) * DH + d0) = ck;
-    const int s16 = r0 + r;
-    uint8_t* vd = vbuf + (s16 >> 4) * 16 * DH + (s16 & 15) / 4 * 4 * DH + (s16 & 3);
-    const uint32_t cv[2] = {codes4(fv.x, iv, tv), codes4(fv.x + 4, iv, tv)};
+#pragma unroll
+  for (int i = 0; i < NC; i++) {
+    const int c = i * TH + tid;
+    if (c >= nr * CPR) break;
+    const int s = r0 + c / CPR, d0 = c % CPR * 8;
+    *reinterpret_cast<uint2*>(kp + s * DH + d0) = make_uint2(codes4(fk[i].x, ik, tk), codes4(fk[i].x + 4, ik, tk));
+    const F8 f = wide8(hv[i]);
+    const uint32_t cv[2] = {codes4(f.x, iv, tv), codes4(f.x + 4, iv, tv)};
+    uint8_t* y = vbuf + (s >> 4) * 16 * DH + (s & 15) / 4 * 4 * DH + (s & 3);
 #pragma unroll
     for (int j = 0; j < 8; j++) {
       const int d = d0 + j;
-      vd[((d & 15) * T + (d >> 4)) * 4] = (uint8_t)(cv[j / 4] >> (8 * (j & 3)));
+      y[((d & 15) * T + (d >> 4)) * 4] = (uint8_t)(cv[j / 4] >> (8 * (j & 3)));
     }
   }
   __syncthreads();
   const uint4* src = reinterpret_cast<const uint4*>(vbuf);
   uint4* dst = reinterpret_cast<uint4*>(vp);
-  for (int c = u0 * DH + tid; c < (u1 + 1) * DH; c += kThreads) dst[c] = src[c];
+  for (int c = u0 * DH + tid; c < (u1 + 1) * DH; c += TH) dst[c] = src[c];
+}
+
+template <int DH>
+void launch(const AppendArgs& a, dim3 grid, hipStream_t st) {
+  switch ((DH / 8) << a.b.pshift) {
+    case 128: hipLaunchKernelGGL((append_kernel<DH, 1, 128>), grid, dim3(128), 0, st, a); break;
+    case 256: hipLaunchKernelGGL((append_kernel<DH, 1, 256>), grid, dim3(256), 0, st, a); break;
+    case 512: hipLaunchKernelGGL((append_kernel<DH, 2, 256>), grid, dim3(256), 0, st, a); break;
+    case 1024: hipLaunchKernelGGL((append_kernel<DH, 4, 256>), grid, dim3(256), 0, st, a); break;
+    case 2048: hipLaunchKernelGGL((append_kernel<DH, 4, 512>), grid, dim3(512), 0, st, a); break;
+    default: hipLaunchKernelGGL((append_kernel<DH, 4, 1024>), grid, dim3(1024), 0, st, a); break;
+  }
 }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
@@ -289,12 +330,10 @@ extern "C" int ane_kv8_append(const ane_kv8_cache* cache, const ane_kv8_batch* b
   a.q_row = g.q_row; a.q_head = g.q_head; a.k_row = g.k_row; a.k_head = g.k_head; a.v_row = g.v_row;
   a.v_head = g.v_head; a.qo_row = g.q_out_row; a.qo_head = g.q_out_head;
   const int P = 1 << a.b.pshift;
-  const dim3 grid(kv8_count(a.b.nseq, a.b.rows, kv8_pages(P)), a.b.NKV + g.heads);
-  const size_t lds = (size_t)P * cache->head_dim;
-  if (cache->head_dim == 64)
-    hipLaunchKernelGGL(append_kernel<64>, grid, dim3(kThreads), lds, (hipStream_t)stream, a);
-  else
-    hipLaunchKernelGGL(append_kernel<128>, grid, dim3(kThreads), lds, (hipStream_t)stream, a);
+  a.heads = g.heads;
+  const dim3 grid(kv8_count(a.b.nseq, a.b.rows, kv8_pages(P)), a.b.NKV + (g.heads + kQHeads - 1) / kQHeads);
+  if (cache->head_dim == 64) launch<64>(a, grid, (hipStream_t)stream);
+  else launch<128>(a, grid, (hipStream_t)stream);
   const hipError_t h = hipGetLastError();
   if (h != hipSuccess) return op_fail(ANE_ERR_HIP, "storiesane %s: %s", op, hipGetErrorString(h));
   return ANE_OK;
