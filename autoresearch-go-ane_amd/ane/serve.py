@@ -36,8 +36,8 @@ def _fail(op, msg):
 
 
 def _tensor(op, name, t, dtypes, device, dims=None, shape=None):
-    """A tensor of one of ``dtypes`` on ``device``, its last dimension (if it
-    has more than one element) contiguous."""
+    """The address of a tensor of one of ``dtypes`` on ``device``, its last
+    dimension (if it has more than one element) contiguous."""
     if not hasattr(t, "data_ptr"):
         _fail(op, f"{name} is not a tensor")
     if t.dtype not in dtypes:
@@ -60,20 +60,19 @@ def _whole(op, name, t, dtypes, device, dims=None, shape=None):
     return p
 
 
-def _strides(t):
-    """Of rows and heads; a dimension of one element has none that matters."""
-    (r, h, _), (sr, sh, _) = t.shape, t.stride()
-    return sr if r > 1 else 0, sh if h > 1 else 0
-
-
 def _on_gpu(op, t):
     if not hasattr(t, "device") or t.device.type != "cuda":
         _fail(op, "tensors must be on a GPU")
     return t.device
 
 
-def _stream(device):
-    return _torch().cuda.current_stream(device).cuda_stream
+def _stream_getter():
+    """device index -> its current stream's handle.  torch's own getter of the
+    bare handle where it has one: 0.2 us against 3 for the Stream object, in
+    calls that take 10."""
+    torch = _torch()
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return raw if raw is not None else lambda index: torch.cuda.current_stream(index).cuda_stream
 
 
 def _check(lib, rc):
@@ -108,6 +107,8 @@ class KVBatch:
         self._keep = (table, start, offsets)
         self.device, self.nseq, self.rows = dev, nseq, int(rows)
         self._c = _lib.Kv8Batch(t, s, o, stride, int(table.shape[1]), nseq, int(rows), int(max_len), int(max_new))
+        self._ref = C.byref(self._c)
+        self._ws = {}  # workspace bytes by (kv_heads, page_tokens, head_dim, heads)
 
 
 class KVCache8:
@@ -133,9 +134,11 @@ class KVCache8:
         self.k, self.v, self.k_exp, self.v_exp = k, v, k_exp, v_exp
         self.device, self.kv_heads, self.head_dim = dev, kvh, dh
         self.pages, self.page_tokens = pages, page
-        self._half = (torch.float16,)
-        self._f32 = (torch.float32,)
-        self._c = _lib.Kv8Cache(kp, vp, ke, ve, pages, page, kvh, dh, dev.index or 0)
+        self._half, self._f32 = torch.float16, (torch.float32,)
+        self._index = dev.index
+        self._empty, self._u8, self._stream = torch.empty, torch.uint8, _stream_getter()
+        self._c = _lib.Kv8Cache(kp, vp, ke, ve, pages, page, kvh, dh, dev.index)
+        self._ref = C.byref(self._c)
 
     @classmethod
     def Empty(cls, pages, kv_heads, head_dim=64, page_tokens=64, device="cuda"):
@@ -148,14 +151,32 @@ class KVCache8:
         return cls(k.view(torch.float8_e4m3fn), v.view(torch.float8_e4m3fn), e[0], e[1])
 
     def _rows(self, op, name, t, batch, heads=None):
-        p = _tensor(op, name, t, self._half, self.device, dims=3)
-        if t.shape[0] != batch.rows or t.shape[2] != self.head_dim or (heads is not None and t.shape[1] != heads):
-            _fail(op, f"{name} has shape {tuple(t.shape)}, want ({batch.rows}, {heads or 'heads'}, {self.head_dim})")
-        return p
+        """(address, stride of rows, stride of heads) of fp16 [rows, heads,
+        head_dim]; a dimension of one element has no stride that matters."""
+        try:
+            r, h, d = t.shape
+            sr, sh, sd = t.stride()
+            if (t.dtype is self._half and t.get_device() == self._index and r == batch.rows and d == self.head_dim
+                    and sd == 1 and (heads is None or h == heads)):
+                return t.data_ptr(), sr if r > 1 else 0, sh if h > 1 else 0
+        except (AttributeError, ValueError):
+            pass
+        _tensor(op, name, t, (self._half,), self.device, dims=3)  # says what is wrong with it
+        _fail(op, f"{name} has shape {tuple(t.shape)}, want ({batch.rows}, {heads or 'heads'}, {self.head_dim})")
+
+    def _new(self, batch, heads):
+        return self._empty((batch.rows, heads, self.head_dim), dtype=self._half, device=self.device)
 
     def _batch(self, op, batch):
         if batch.device != self.device:
             _fail(op, f"batch is on {batch.device}, the cache on {self.device}")
+
+    def _angles(self, op, name, t):
+        if not (t.dtype is self._f32[0] and t.get_device() == self._index and t.dim() == 2 and t.is_contiguous()
+                and t.shape[1] * 2 == self.head_dim):
+            _whole(op, name, t, self._f32, self.device, dims=2)
+            _fail(op, f"{name} has shape {tuple(t.shape)}, want (positions, {self.head_dim // 2})")
+        return t.data_ptr()
 
     def Append(self, batch, q, k, v, cos, sin, q_out=None):
         """Rotates q and k (fp16 [rows, heads or kv_heads, head_dim], any
@@ -165,28 +186,25 @@ class KVCache8:
         Returns q_out."""
         op = "kv8 append"
         self._batch(op, batch)
-        a = _lib.Kv8AppendArgs()
-        a.k = self._rows(op, "k", k, batch, self.kv_heads)
-        a.v = self._rows(op, "v", v, batch, self.kv_heads)
-        a.k_row, a.k_head = _strides(k)
-        a.v_row, a.v_head = _strides(v)
+        kp, kr, kh = self._rows(op, "k", k, batch, self.kv_heads)
+        vp, vr, vh = self._rows(op, "v", v, batch, self.kv_heads)
+        heads, qp, qr, qh, op_, or_, oh = 0, None, 0, 0, None, 0, 0
         if q is not None:
-            a.q = self._rows(op, "q", q, batch)
+            qp, qr, qh = self._rows(op, "q", q, batch)
+            heads = q.shape[1]
             if q_out is None:
-                q_out = _torch().empty((batch.rows, q.shape[1], self.head_dim), dtype=q.dtype, device=self.device)
-            a.q_out = self._rows(op, "q_out", q_out, batch, q.shape[1])
-            a.heads = q.shape[1]
-            a.q_row, a.q_head = _strides(q)
-            a.q_out_row, a.q_out_head = _strides(q_out)
+                q_out = self._new(batch, heads)
+            op_, or_, oh = self._rows(op, "q_out", q_out, batch, heads)
         elif q_out is not None:
             _fail(op, "q_out without q")
-        a.cos = _whole(op, "cos", cos, self._f32, self.device, dims=2)
-        a.sin = _whole(op, "sin", sin, self._f32, self.device, dims=2)
-        if cos.shape != sin.shape or cos.shape[1] * 2 != self.head_dim:
-            _fail(op, f"cos {tuple(cos.shape)} and sin {tuple(sin.shape)} must be [positions, {self.head_dim // 2}]")
-        a.positions = cos.shape[0]
-        _check(self._lib, self._lib.ane_kv8_append(C.byref(self._c), C.byref(batch._c), C.byref(a),
-                                                   _stream(self.device)))
+        cp, sp = self._angles(op, "cos", cos), self._angles(op, "sin", sin)
+        n = cos.shape[0]
+        if sin.shape[0] != n:
+            _fail(op, f"cos has {n} positions, sin {sin.shape[0]}")
+        a = _lib.Kv8AppendArgs(qp, kp, vp, op_, cp, sp, qr, qh, kr, kh, vr, vh, or_, oh, heads, n)
+        rc = self._lib.ane_kv8_append(self._ref, batch._ref, C.byref(a), self._stream(self._index))
+        if rc:
+            _check(self._lib, rc)
         return q_out
 
     def Attend(self, batch, q, out=None, scale=None):
@@ -196,22 +214,21 @@ class KVCache8:
         then undefined)."""
         op = "kv8 attend"
         self._batch(op, batch)
-        a = _lib.Kv8AttendArgs()
-        a.q = self._rows(op, "q", q, batch)
+        qp, qr, qh = self._rows(op, "q", q, batch)
         heads = q.shape[1]
         if out is None:
-            out = _torch().empty((batch.rows, heads, self.head_dim), dtype=q.dtype, device=self.device)
-        a.out = self._rows(op, "out", out, batch, heads)
-        a.q_row, a.q_head = _strides(q)
-        a.out_row, a.out_head = _strides(out)
-        a.heads = heads
-        a.scale = self.head_dim ** -0.5 if scale is None else scale
-        n = _check(self._lib, self._lib.ane_kv8_attend_workspace(C.byref(self._c), C.byref(batch._c), heads))
-        if n:
-            ws = _torch().empty(n, dtype=_torch().uint8, device=self.device)
-            a.ws, a.ws_bytes = ws.data_ptr(), n
-        _check(self._lib, self._lib.ane_kv8_attend(C.byref(self._c), C.byref(batch._c), C.byref(a),
-                                                   _stream(self.device)))
+            out = self._new(batch, heads)
+        yp, yr, yh = self._rows(op, "out", out, batch, heads)
+        key = (self.kv_heads, self.page_tokens, self.head_dim, heads)
+        n = batch._ws.get(key)
+        if n is None:
+            n = batch._ws[key] = _check(self._lib, self._lib.ane_kv8_attend_workspace(self._ref, batch._ref, heads))
+        ws = self._empty(n, dtype=self._u8, device=self.device) if n else None
+        a = _lib.Kv8AttendArgs(qp, yp, qr, qh, yr, yh, heads, self.head_dim ** -0.5 if scale is None else scale,
+                               None if ws is None else ws.data_ptr(), n)
+        rc = self._lib.ane_kv8_attend(self._ref, batch._ref, C.byref(a), self._stream(self._index))
+        if rc:
+            _check(self._lib, rc)
         return out
 
 
@@ -230,7 +247,7 @@ class LogitControls:
         self._keep = given = [t for t in (repetition, frequency, presence, bias, mask) if t is not None]
         self.device = _on_gpu(op, given[0]) if given else None
         self.rows = None
-        self._a = a = _lib.LogitsArgs()
+        a = _lib.LogitsArgs()
         f32 = (torch.float32,)
         for name, t in (("repetition", repetition), ("frequency", frequency), ("presence", presence)):
             if t is not None:
@@ -249,6 +266,10 @@ class LogitControls:
         self.penalties = any(t is not None for t in (repetition, frequency, presence))
         self._f32, self._i32 = f32, (torch.int32,)
         self._u16 = (torch.uint16, torch.int16)
+        self._empty, self._u8, self._stream = torch.empty, torch.uint8, _stream_getter()
+        self._index = self.device.index if self.device is not None else None
+        self._params = (a.repetition, a.frequency, a.presence, a.bias, a.mask, a.bias_row, a.mask_row)
+        self._bytes = {}  # of the workspace, by rows
         self._lib = _lib.load()
 
     def _same_rows(self, name, n):
@@ -268,40 +289,62 @@ class LogitControls:
         bits [rows, n], of which lengths int32 [rows] are tokens, the first
         prompts int32 [rows] (None: 0) of them the prompt's."""
         op = self._op
-        dev = _on_gpu(op, logits)
-        if self.device is not None and dev != self.device:
-            _fail(op, f"logits are on {dev}, the controls on {self.device}")
-        a = _lib.LogitsArgs.from_buffer_copy(self._a)
-        a.logits = _tensor(op, "logits", logits, self._f32, dev, dims=2)
-        rows, vocab = logits.shape
+        index = logits.get_device() if hasattr(logits, "get_device") else -1
+        if index < 0:
+            _on_gpu(op, logits)
+        if self._index is not None and index != self._index:
+            _fail(op, f"logits are on {logits.device}, the controls on {self.device}")
+        lp, lr, rows, vocab = self._matrix("logits", logits, self._f32, index)
         if vocab != self.vocab or (self.rows is not None and rows != self.rows):
             _fail(op, f"logits have shape {tuple(logits.shape)}, want ({self.rows or 'rows'}, {self.vocab})")
-        torch = _torch()
         if out is None:
-            out = torch.empty((rows, vocab), dtype=logits.dtype, device=dev)
+            out = self._empty((rows, vocab), dtype=logits.dtype, device=logits.device)
+        yp, yr, yn, yv = self._matrix("out", out, self._f32, index)
+        if yn != rows or yv != vocab:
+            _fail(op, f"out has shape {tuple(out.shape)}, want ({rows}, {vocab})")
         if tokens is None:
-            tokens = torch.empty(rows, dtype=torch.int32, device=dev)
-        a.out = _tensor(op, "out", out, self._f32, dev, shape=(rows, vocab))
-        a.tokens = _whole(op, "tokens", tokens, self._i32, dev, shape=(rows,))
-        a.logits_row, a.out_row = self._row(logits), self._row(out)
+            tokens = self._empty(rows, dtype=self._i32[0], device=logits.device)
+        tp = self._vector("tokens", tokens, index, rows)
+        hp = hr = np_ = pp = None
+        most = 0
         if history is not None:
-            a.history = _tensor(op, "history", history, self._u16, dev, dims=2)
-            if history.shape[0] != rows:
-                _fail(op, f"history has {history.shape[0]} rows, want {rows}")
-            a.history_row, a.history_max = self._row(history), history.shape[1]
+            hp, hr, hn, most = self._matrix("history", history, self._u16, index)
+            if hn != rows:
+                _fail(op, f"history has {hn} rows, want {rows}")
             if lengths is None:
                 _fail(op, "history without lengths")
-            a.lengths = _whole(op, "lengths", lengths, self._i32, dev, shape=(rows,))
+            np_ = self._vector("lengths", lengths, index, rows)
             if prompts is not None:
-                a.prompts = _whole(op, "prompts", prompts, self._i32, dev, shape=(rows,))
+                pp = self._vector("prompts", prompts, index, rows)
         elif self.penalties:
             _fail(op, "penalties without a history")
         elif lengths is not None or prompts is not None:
             _fail(op, "lengths without a history")
-        a.rows, a.vocab, a.device = rows, vocab, dev.index or 0
-        n = _check(self._lib, self._lib.ane_control_logits_workspace(rows, vocab))
-        if n:
-            ws = torch.empty(n, dtype=torch.uint8, device=dev)
-            a.ws, a.ws_bytes = ws.data_ptr(), n
-        _check(self._lib, self._lib.ane_control_logits(C.byref(a), _stream(dev)))
+        n = self._bytes.get(rows)
+        if n is None:
+            n = self._bytes[rows] = _check(self._lib, self._lib.ane_control_logits_workspace(rows, vocab))
+        ws = self._empty(n, dtype=self._u8, device=logits.device) if n else None
+        rep, freq, pres, bias, mask, bias_row, mask_row = self._params
+        a = _lib.LogitsArgs(lp, yp, hp, np_, pp, rep, freq, pres, bias, mask, tp, lr, yr, hr or 0, bias_row, mask_row,
+                            rows, vocab, most, index, None if ws is None else ws.data_ptr(), n)
+        rc = self._lib.ane_control_logits(C.byref(a), self._stream(index))
+        if rc:
+            _check(self._lib, rc)
         return out, tokens
+
+    def _matrix(self, name, t, dtypes, index):
+        """(address, stride of rows, rows, columns)."""
+        try:
+            n, w = t.shape
+            sn, sw = t.stride()
+            if t.dtype in dtypes and t.get_device() == index and (sw == 1 or w <= 1 or n == 0):
+                return t.data_ptr(), sn if n > 1 else max(sn, w), n, w
+        except (AttributeError, ValueError):
+            pass
+        _tensor(self._op, name, t, dtypes, _torch().device("cuda", index), dims=2)  # says what is wrong with it
+        _fail(self._op, f"{name} is not a matrix of rows")
+
+    def _vector(self, name, t, index, rows):
+        if t.dtype is self._i32[0] and t.get_device() == index and t.shape == (rows,) and t.is_contiguous():
+            return t.data_ptr()
+        return _whole(self._op, name, t, self._i32, _torch().device("cuda", index), shape=(rows,))
