@@ -58,6 +58,12 @@ class DecodeCfg(C.Structure):
                 ("rope_theta", C.c_double), ("device", C.c_int32)]
 
 
+class DecodeControls(C.Structure):
+    """ane_decode_controls (include/ane_hip.h)."""
+    _fields_ = [(n, C.POINTER(C.c_float)) for n in ("repetition", "frequency", "presence", "bias")] + [
+        ("mask", C.POINTER(C.c_uint32)), ("mask_rows", C.c_int32)]
+
+
 class MoeCfg(C.Structure):
     _fields_ = [("dim", C.c_int32), ("hidden", C.c_int32), ("experts", C.c_int32), ("top_k", C.c_int32),
                 ("max_tokens", C.c_int32), ("device", C.c_int32)]
@@ -181,6 +187,8 @@ SIGNATURES = {
     "ane_decode_position": (C.c_int32, [_eng]),
     "ane_decode_last_ms": (C.c_double, [_eng]),
     "ane_decode_fused_chain": (C.c_int32, [_eng]),
+    "ane_decode_set_cache": (C.c_int, [_eng, C.c_int32]),
+    "ane_decode_set_controls": (C.c_int, [_eng, C.POINTER(DecodeControls)]),
     "ane_decode_debug_fill_cache": (C.c_int, [_eng, C.c_int]),
     "ane_moe_open": (C.c_int, [C.POINTER(MoeCfg), C.POINTER(C.c_void_p)]),
     "ane_moe_destroy": (None, [_eng]),

@@ -26,9 +26,12 @@ def _f(a):
 
 
 class Decoder:
-    """Open(cfg, params, max_batch, max_ctx) -> Prefill -> Step / Generate."""
+    """Open(cfg, params, max_batch, max_ctx) -> Prefill -> Step / Generate.
 
-    def __init__(self, cfg: Config, params, max_batch: int = 64, max_ctx: int = 1152, device: int = 0):
+    page_tokens: 0 keeps the fp16 cache, 16..256 the paged 8-bit one (SetCache)."""
+
+    def __init__(self, cfg: Config, params, max_batch: int = 64, max_ctx: int = 1152, device: int = 0,
+                 page_tokens: int = 0):
         if cfg.arch != "llama2":
             raise EngineError(_lib.ANE_ERR_ARG, "storiesane decode open: arch must be llama2")
         self._lib = _lib.load()
@@ -45,6 +48,8 @@ class Decoder:
         self._h = h
         self.nseq = 0
         try:
+            if page_tokens:
+                self.SetCache(page_tokens)
             self.SetParams(params)
         except Exception:
             self.Close()
@@ -94,6 +99,53 @@ class Decoder:
         out = np.zeros((nsteps, max(self.nseq, 1)), np.uint16)
         self._check(self._lib.ane_decode_generate(self._h, int(nsteps), _u16(out)))
         return np.ascontiguousarray(out[:, :self.nseq].T)
+
+    def SetCache(self, page_tokens: int = 64):
+        """The cache to keep from here on: 0 fp16, 16..256 (a power of two)
+        the paged 8-bit one, half the memory and half the bytes an attention
+        reads.  Drops the active batch: Prefill comes next."""
+        self._live()
+        self._check(self._lib.ane_decode_set_cache(self._h, int(page_tokens)))
+        self.nseq = 0
+
+    def SetControls(self, repetition=None, frequency=None, presence=None, bias=None, mask=None):
+        """Controls on the logits before each next token is chosen, until they
+        are changed: penalties [max_batch] (repetition divides or multiplies,
+        1 changes nothing; frequency and presence are subtracted) that count
+        prompt and output, or output; bias [vocab]; mask uint32 words
+        [ceil(vocab/32)] or [rows, ceil(vocab/32)], bit v % 32 of word v // 32
+        set: token v allowed.  The first come before Prefill; then they may
+        change between any two calls.  Returned logits are the changed ones; a
+        sequence that nothing is allowed for gets NO_TOKEN."""
+        self._live()
+        B, V = self._c.max_batch, self.cfg.vocab
+
+        def arr(name, x, shape):
+            if x is None:
+                return None
+            a = np.ascontiguousarray(x, dtype=np.float32)
+            if a.shape != shape:
+                raise EngineError(_lib.ANE_ERR_ARG, f"storiesane decode set controls: {name} has shape {a.shape}, "
+                                                    f"want {shape}")
+            return a
+        rows = [arr(n, x, (B,)) for n, x in (("repetition", repetition), ("frequency", frequency),
+                                             ("presence", presence))]
+        b = arr("bias", bias, (V,))
+        m, n = None, 0
+        if mask is not None:
+            m = np.ascontiguousarray(mask)
+            if m.dtype not in (np.uint32, np.int32) or m.ndim not in (1, 2) or m.shape[-1] != (V + 31) // 32:
+                raise EngineError(_lib.ANE_ERR_ARG, f"storiesane decode set controls: mask is {m.dtype} {m.shape}, "
+                                                    f"want 32-bit words ([rows,] {(V + 31) // 32})")
+            n = 1 if m.ndim == 1 else m.shape[0]
+        c = _lib.DecodeControls(*[None if x is None else _f(x) for x in (*rows, b)],
+                                None if m is None else m.ctypes.data_as(C.POINTER(C.c_uint32)), n)
+        self._check(self._lib.ane_decode_set_controls(self._h, C.byref(c)))
+
+    def ClearControls(self):
+        """The plain argmax again."""
+        self._live()
+        self._check(self._lib.ane_decode_set_controls(self._h, None))
 
     def Position(self) -> int:
         self._live()

@@ -110,6 +110,26 @@ struct DecAttnArgs {
 };
 hipError_t dec_attention(const DecAttnArgs& a, hipStream_t s);
 
+// ---- steps over the paged 8-bit cache, and controlled logits --------------------
+// qkv [nb][N1] fp16 = the QKV GEMM's partials summed in split order (times
+// rr[row], where given); start[b] = ctr[0] and offsets[b] = b for the append
+// and attention that follow.  With *err set (a failed chain wait: the partials
+// are not to be used) the offsets say that no sequence has a new token, so
+// that nothing of them reaches the cache.
+hipError_t dec_qkv_rows(const float* part, int ks, const float* rr, half_t* qkv, int N1, int nb, const int* ctr,
+                        const int* err, int* start, int* offsets, hipStream_t s);
+// start[i] = 0, offsets[i] = i * plen for i <= nseq (prefill of nseq prompts)
+hipError_t dec_prompt_plan(int* start, int* offsets, int nseq, int plen, hipStream_t s);
+// The history that penalties count, uint16 [..][ld]: the prompts (and the
+// row lengths), and at each step the token that is fed, at position ctr[0].
+hipError_t dec_history_prompt(uint16_t* hist, int ld, const uint16_t* prefix, int plen, int* lengths, int* prompts,
+                              int nseq, hipStream_t s);
+hipError_t dec_history_feed(uint16_t* hist, int ld, const uint16_t* tok, const int* ctr, int* lengths, int nb,
+                            hipStream_t s);
+// tok_out[b] (and row *step of hist, where given) = the chosen tokens
+hipError_t dec_take_tokens(uint16_t* tok_out, uint16_t* hist, const int* step, const int* chosen, int nb,
+                           hipStream_t s);
+
 // ---- the per-layer GEMM chain in one launch (decode_tail.hip) ---------------
 // Wo + residual, W1|W3 + SwiGLU, W2 + residual, the next layer's QKV
 // projection and its 1 / rms: one 16-wave block per 32-column group (per

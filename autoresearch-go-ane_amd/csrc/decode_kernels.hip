@@ -752,7 +752,99 @@ __global__ __launch_bounds__(256) void gather_last_kernel(float* dst, const floa
   for (int c = threadIdx.x; c < D; c += 256) dst[(size_t)i * D + c] = s[c];
 }
 
+// A block per row; a thread two neighbouring columns at a time.
+__global__ __launch_bounds__(256) void qkv_rows_kernel(const float* part, int ks, const float* rr, half_t* qkv, int N1,
+                                                       int nb, const int* ctr, const int* err, int* start,
+                                                       int* offsets) {
+  const int t = blockIdx.x;
+  const bool ok = !err || *err == 0;
+  if (threadIdx.x == 0) {
+    start[t] = ctr[0];
+    offsets[t] = ok ? t : 0;
+    if (t == nb - 1) offsets[nb] = ok ? nb : 0;
+  }
+  const float r = rr ? rr[t] : 1.f;
+  for (int c = threadIdx.x * 2; c < N1; c += 512) {
+    float x = 0.f, y = 0.f;
+    for (int s = 0; s < ks; s++) {
+      const float2 p = *reinterpret_cast<const float2*>(part + ((size_t)s * kDecRows + t) * N1 + c);
+      x += p.x;
+      y += p.y;
+    }
+    half2v h;
+    h[0] = (half_t)(x * r);
+    h[1] = (half_t)(y * r);
+    *reinterpret_cast<half2v*>(qkv + (size_t)t * N1 + c) = h;
+  }
+}
+
+__global__ __launch_bounds__(64) void prompt_plan_kernel(int* start, int* offsets, int nseq, int plen) {
+  const int i = blockIdx.x * 64 + threadIdx.x;
+  if (i < nseq) start[i] = 0;
+  if (i <= nseq) offsets[i] = i * plen;
+}
+
+__global__ __launch_bounds__(256) void history_prompt_kernel(uint16_t* hist, int ld, const uint16_t* prefix, int plen,
+                                                             int* lengths, int* prompts) {
+  const int b = blockIdx.x;
+  for (int j = threadIdx.x; j < plen; j += 256) hist[(size_t)b * ld + j] = prefix[(size_t)b * plen + j];
+  if (threadIdx.x == 0) {
+    lengths[b] = plen;
+    prompts[b] = plen;
+  }
+}
+
+__global__ __launch_bounds__(64) void history_feed_kernel(uint16_t* hist, int ld, const uint16_t* tok, const int* ctr,
+                                                          int* lengths, int nb) {
+  const int b = threadIdx.x, pos = ctr[0];
+  if (b >= nb || pos >= ld) return;
+  hist[(size_t)b * ld + pos] = tok[b];
+  lengths[b] = pos + 1;
+}
+
+__global__ __launch_bounds__(64) void take_tokens_kernel(uint16_t* tok_out, uint16_t* hist, const int* step,
+                                                         const int* chosen, int nb) {
+  const int b = threadIdx.x;
+  if (b >= nb) return;
+  const uint16_t t = (uint16_t)chosen[b];
+  tok_out[b] = t;
+  if (hist) hist[(size_t)(*step) * nb + b] = t;
+}
+
 }  // namespace
+
+hipError_t dec_qkv_rows(const float* part, int ks, const float* rr, half_t* qkv, int N1, int nb, const int* ctr,
+                        const int* err, int* start, int* offsets, hipStream_t s) {
+  if (nb < 1 || nb > kDecRows || ks < 1 || N1 % 2) return hipErrorInvalidValue;
+  hipLaunchKernelGGL(qkv_rows_kernel, dim3(nb), dim3(256), 0, s, part, ks, rr, qkv, N1, nb, ctr, err, start, offsets);
+  return hipGetLastError();
+}
+
+hipError_t dec_prompt_plan(int* start, int* offsets, int nseq, int plen, hipStream_t s) {
+  hipLaunchKernelGGL(prompt_plan_kernel, dim3(nseq / 64 + 1), dim3(64), 0, s, start, offsets, nseq, plen);
+  return hipGetLastError();
+}
+
+hipError_t dec_history_prompt(uint16_t* hist, int ld, const uint16_t* prefix, int plen, int* lengths, int* prompts,
+                              int nseq, hipStream_t s) {
+  if (plen > ld) return hipErrorInvalidValue;
+  hipLaunchKernelGGL(history_prompt_kernel, dim3(nseq), dim3(256), 0, s, hist, ld, prefix, plen, lengths, prompts);
+  return hipGetLastError();
+}
+
+hipError_t dec_history_feed(uint16_t* hist, int ld, const uint16_t* tok, const int* ctr, int* lengths, int nb,
+                            hipStream_t s) {
+  if (nb < 1 || nb > kDecRows) return hipErrorInvalidValue;
+  hipLaunchKernelGGL(history_feed_kernel, dim3(1), dim3(64), 0, s, hist, ld, tok, ctr, lengths, nb);
+  return hipGetLastError();
+}
+
+hipError_t dec_take_tokens(uint16_t* tok_out, uint16_t* hist, const int* step, const int* chosen, int nb,
+                           hipStream_t s) {
+  if (nb < 1 || nb > kDecRows) return hipErrorInvalidValue;
+  hipLaunchKernelGGL(take_tokens_kernel, dim3(1), dim3(64), 0, s, tok_out, hist, step, chosen, nb);
+  return hipGetLastError();
+}
 
 // Waves per block splitting K (K <= 1024, the decoder's dim limit: at most
 // 16 windows): exactly two k-windows each when the window count allows one

@@ -11,6 +11,8 @@
 //   embed_h  fp16 [V][D]              tied classifier
 //   f*       the same five in MFMA-fragment-major order (decode.h)
 //   kc, vc   fp16 [L][max_batch][kv_heads][max_ctx][64]
+//            (or k8, v8, ke8, ve8: the paged 8-bit cache of ane_serve.h, one pool
+//            per layer, each sequence's pages one after the other)
 //   decode rows (64 each): x fp32 [64][D], xn/q/att fp16 [64][D],
 //   gate fp16 [64][H], split-K partials, attention partials, argmax partials
 //   prefill chunk (<= 8192 tokens): px fp32, pxn/pqkv/patt/pgate fp16
@@ -28,6 +30,7 @@
 #include "decode.h"
 #include "gemm.h"
 #include "host_copy.h"
+#include "kv8.h"
 #include "rowops.h"
 
 using namespace ane;
@@ -80,7 +83,26 @@ struct ane_decoder {
   // the same weights in MFMA-fragment-major order for the 64-row decode GEMMs
   half_t *fwqkv = nullptr, *fwo = nullptr, *fw13 = nullptr, *fw2 = nullptr, *fembed = nullptr;
   half_t *kc = nullptr, *vc = nullptr;
-  float *rope_cos = nullptr, *rope_sin = nullptr;
+  float *rope_cos = nullptr, *rope_sin = nullptr;  // [rope_rows][32]
+  int rope_rows = 0;
+  // the paged 8-bit cache, when chosen (page8 > 0)
+  int page8 = 0, seq_pages = 0;  // tokens per page, pages per sequence
+  uint8_t *k8 = nullptr, *v8 = nullptr;
+  int8_t *ke8 = nullptr, *ve8 = nullptr;
+  int *table8 = nullptr, *start8 = nullptr, *off8 = nullptr;
+  half_t* qkv8 = nullptr;  // [64][N1] rows of a step
+  void* ws8 = nullptr;     // attention workspace
+  size_t ws8_cap = 0;
+  // controls on the logits, when set
+  bool controls = false;
+  ane_logits_args ctl{};      // what is given (device pointers; NULL: not used)
+  float* ctl_rows = nullptr;  // repetition | frequency | presence, [3][64]
+  float* ctl_bias = nullptr;
+  uint32_t* ctl_mask = nullptr;
+  uint16_t* ctl_hist = nullptr;  // [B][max_ctx]
+  int *ctl_len = nullptr, *ctl_prompt = nullptr, *ctl_tok = nullptr;
+  void* ctl_ws = nullptr;
+  int ctl_mask_rows = 0;
   float* x = nullptr;
   half_t *xn = nullptr, *att = nullptr, *gate = nullptr;
   half_t* att2 = nullptr;  // the fused chain's odd layers' attention output (the next chain reads the other)
@@ -158,6 +180,8 @@ void free_all(ane_decoder* d) {
   d->graph = nullptr;
   for (void* p : d->allocs) (void)hipFree(p);
   d->allocs.clear();
+  if (d->ws8) (void)hipFree(d->ws8);
+  d->ws8 = nullptr;
   if (d->ev0) (void)hipEventDestroy(d->ev0);
   if (d->ev1) (void)hipEventDestroy(d->ev1);
   d->ev0 = d->ev1 = nullptr;
@@ -218,8 +242,10 @@ int open_impl(ane_decoder* d) {
   DCHK(op, dalloc(d, &d->vc, cache));
   // RoPE tables (buildRoPETables, ane/train_util.go:183-202: f64 angle, fp32 cos/sin)
   {
-    std::vector<float> cs((size_t)C * 32), sn((size_t)C * 32);
-    for (int p = 0; p < C; p++)
+    // to a whole page of any size: the paged cache's positions
+    const int R = d->rope_rows = (C + 255) / 256 * 256;
+    std::vector<float> cs((size_t)R * 32), sn((size_t)R * 32);
+    for (int p = 0; p < R; p++)
       for (int i = 0; i < 32; i++) {
         const double f = (double)p / std::pow(c.rope_theta, (double)(2 * i) / 64.0);
         cs[(size_t)p * 32 + i] = (float)std::cos(f);
@@ -325,11 +351,101 @@ hipError_t gemm(ane_decoder* d, const half_t* A, const half_t* Bw, int M, int N,
 int enqueue_step_tail(ane_decoder* d, float* logits, uint16_t* hist);
 int generate_run(ane_decoder* d, const char* op, int nsteps, uint16_t* out_tok);
 
+// A serving operator's failure (its message is the thread's).
+#define SCHK(op, expr)                                                                              \
+  do {                                                                                              \
+    const int _r = (int)(expr);                                                                     \
+    if (_r < 0) return dfail(d, _r, "storiesane decode %s: %s", op, ane_op_last_error());           \
+  } while (0)
+
+void drop_graph(ane_decoder* d) {
+  if (d->gexec) (void)hipGraphExecDestroy(d->gexec);
+  if (d->graph) (void)hipGraphDestroy(d->graph);
+  d->gexec = nullptr;
+  d->graph = nullptr;
+}
+
+// Layer l of the 8-bit cache, and a batch over its first `nseq` sequences from
+// seq0 on.
+ane_kv8_cache cache8(const ane_decoder* d, int l) {
+  const size_t pages = (size_t)d->B * d->seq_pages, page = (size_t)d->NKV * d->page8 * 64;
+  return {d->k8 + l * pages * page, d->v8 + l * pages * page, d->ke8 + l * pages * d->NKV, d->ve8 + l * pages * d->NKV,
+          (int32_t)pages, d->page8, d->NKV, 64, d->cfg.device};
+}
+ane_kv8_batch batch8(const ane_decoder* d, int seq0, int nseq, int rows, int max_len, int max_new) {
+  return {d->table8 + (size_t)seq0 * d->seq_pages, d->start8, d->off8, d->seq_pages, d->seq_pages, nseq, rows, max_len,
+          max_new};
+}
+
+// Room for the attention's workspace (not during a capture).
+int room8(ane_decoder* d, const char* op, const ane_kv8_batch& b) {
+  const ane_kv8_cache c = cache8(d, 0);
+  const int64_t n = ane_kv8_attend_workspace(&c, &b, d->NH);
+  SCHK(op, n);
+  if ((size_t)n <= d->ws8_cap) return ANE_OK;
+  DCHK(op, hipStreamSynchronize(d->stream));
+  drop_graph(d);  // it holds the old address
+  if (d->ws8) (void)hipFree(d->ws8);
+  d->ws8 = nullptr;
+  d->ws8_cap = 0;
+  DCHK(op, hipMalloc(&d->ws8, (size_t)n));
+  d->ws8_cap = (size_t)n;
+  return ANE_OK;
+}
+
+// q | k | v rows (N1 apart) of the batch: rotate, append, attend; q in place.
+int attention8(ane_decoder* d, const char* op, int l, const ane_kv8_batch& b, half_t* qkv, half_t* out, bool frag) {
+  const int D = d->D, N1 = d->N1;
+  const ane_kv8_cache c = cache8(d, l);
+  ane_kv8_append_args a{};
+  a.q = a.q_out = (uint16_t*)qkv;
+  a.k = (const uint16_t*)(qkv + D);
+  a.v = (const uint16_t*)(qkv + D + d->KVD);
+  a.cos = d->rope_cos; a.sin = d->rope_sin;
+  a.q_row = a.k_row = a.v_row = a.q_out_row = N1;
+  a.q_head = a.k_head = a.v_head = a.q_out_head = 64;
+  a.heads = d->NH; a.positions = d->rope_rows;
+  SCHK(op, ane_kv8_append(&c, &b, &a, d->stream));
+  ane_kv8_attend_args t{};
+  t.q = (const uint16_t*)qkv; t.out = (uint16_t*)out;
+  t.q_row = N1; t.q_head = 64; t.out_row = D; t.out_head = 64;
+  t.heads = d->NH; t.scale = 0.125f; t.ws = d->ws8; t.ws_bytes = (int64_t)d->ws8_cap;
+  SCHK(op, kv8_attend(&c, &b, &t, frag, d->stream));
+  return ANE_OK;
+}
+
+// The same for a step, from the QKV GEMM's partials.
+int step_attention8(ane_decoder* d, const char* op, int l, int ks, const float* rr, const int* err, half_t* att) {
+  DCHK(op, dec_qkv_rows(d->kpart, ks, rr, d->qkv8, d->N1, d->nseq, d->ctr_d, err, d->start8, d->off8, d->stream));
+  return attention8(d, op, l, batch8(d, 0, d->nseq, d->nseq, d->C, 1), d->qkv8, att, true);
+}
+
+// The next tokens of the current logits: the argmax, or the controls' choice
+// (then logits_d holds the changed logits).
+int choose(ane_decoder* d, const char* op, uint16_t* hist) {
+  const hipStream_t st = d->stream;
+  if (!d->controls) {
+    DCHK(op, argmax_reduce(d->tok_d, hist, hist ? d->ctr_d + 1 : nullptr, d->amax, d->V / 32, d->nseq, st));
+    return ANE_OK;
+  }
+  ane_logits_args a = d->ctl;
+  a.rows = d->nseq;
+  SCHK(op, ane_control_logits(&a, st));
+  DCHK(op, dec_take_tokens(d->tok_d, hist, d->ctr_d + 1, d->ctl_tok, d->nseq, st));
+  return ANE_OK;
+}
+int feed_history(ane_decoder* d, const char* op) {
+  if (d->controls)
+    DCHK(op, dec_history_feed(d->ctl_hist, d->C, d->tok_d, d->ctr_d, d->ctl_len, d->nseq, d->stream));
+  return ANE_OK;
+}
+
 int enqueue_step(ane_decoder* d, float* logits, uint16_t* hist) {
   if (d->use_tail) return enqueue_step_tail(d, logits, hist);
   const char* op = "step";
   const int D = d->D, H = d->H, N1 = d->N1, nb = d->nseq;
   const hipStream_t st = d->stream;
+  if (int rc = feed_history(d, op)) return rc;
   DCHK(op, dec_embed_norm(d->x, d->xn, d->P + d->off_embed, d->tok_d, d->P + d->off[0].g_att, nb, D, d->V, st));
   for (int l = 0; l < d->L; l++) {
     const DecLayerOff& o = d->off[l];
@@ -339,12 +455,16 @@ int enqueue_step(ane_decoder* d, float* logits, uint16_t* hist) {
     // per-row finish that sums the splits and applies the epilogue (the QKV
     // partials are finished by the attention kernel)
     DCHK(op, skinny_partials(d->xn, d->fwqkv + (size_t)l * N1 * D, d->kpart, d->kpart_cap, N1, D, st));
-    DecAttnArgs aa;
-    aa.qkv_part = d->kpart; aa.qkv_ks = skinny_splits(N1, D); aa.rope_cos = d->rope_cos; aa.rope_sin = d->rope_sin;
-    aa.kc = kcl; aa.vc = vcl; aa.ctr = d->ctr_d; aa.part = d->apart; aa.att = d->att; aa.nb = nb;
-    aa.NH = d->NH; aa.NKV = d->NKV; aa.max_ctx = d->C; aa.nsplit = d->nsplit; aa.scale = 0.125f;
-    aa.form = d->attn_form;
-    DCHK(op, dec_attention(aa, st));
+    if (d->page8) {
+      if (int rc = step_attention8(d, op, l, skinny_splits(N1, D), nullptr, nullptr, d->att)) return rc;
+    } else {
+      DecAttnArgs aa;
+      aa.qkv_part = d->kpart; aa.qkv_ks = skinny_splits(N1, D); aa.rope_cos = d->rope_cos; aa.rope_sin = d->rope_sin;
+      aa.kc = kcl; aa.vc = vcl; aa.ctr = d->ctr_d; aa.part = d->apart; aa.att = d->att; aa.nb = nb;
+      aa.NH = d->NH; aa.NKV = d->NKV; aa.max_ctx = d->C; aa.nsplit = d->nsplit; aa.scale = 0.125f;
+      aa.form = d->attn_form;
+      DCHK(op, dec_attention(aa, st));
+    }
     DCHK(op, skinny_partials(d->att, d->fwo + (size_t)l * D * D, d->kpart, d->kpart_cap, D, D, st));
     DCHK(op, skinny_finish_resid_norm(d->kpart, D, D, d->x, d->xn, d->P + o.g_ffn, nb, st));
     DCHK(op, skinny_partials(d->xn, d->fw13 + (size_t)l * 2 * H * D, d->kpart, d->kpart_cap, 2 * H, D, st));
@@ -357,9 +477,9 @@ int enqueue_step(ane_decoder* d, float* logits, uint16_t* hist) {
   memset(&s, 0, sizeof s);
   s.nb = nb;
   s.X = d->xn; s.W = d->fembed; s.N = d->V; s.K = D; s.amax = d->amax;
-  s.logits = logits; s.nvalid = d->V;
+  s.logits = d->controls ? d->logits_d : logits; s.nvalid = d->V;
   DCHK(op, classifier_argmax(s, st));
-  DCHK(op, argmax_reduce(d->tok_d, hist, d->ctr_d + 1, d->amax, d->V / 32, nb, st));
+  if (int rc = choose(d, op, hist)) return rc;
   DCHK(op, dec_advance(d->ctr_d, st));
   return ANE_OK;
 }
@@ -372,6 +492,7 @@ int enqueue_step_tail(ane_decoder* d, float* logits, uint16_t* hist) {
   const char* op = "step";
   const int D = d->D, H = d->H, N1 = d->N1, nb = d->nseq, L = d->L;
   const hipStream_t st = d->stream;
+  if (int rc = feed_history(d, op)) return rc;
   DCHK(op, dec_row_xg(d->x, d->xg_att, d->rr_d, d->P + d->off_embed, d->tok_d, d->P + d->off[0].g_att, nb, D, d->V,
                       st));
   DCHK(op, skinny_partials(d->xg_att, d->fwqkv, d->kpart, d->kpart_cap, N1, D, st));
@@ -389,9 +510,14 @@ int enqueue_step_tail(ane_decoder* d, float* logits, uint16_t* hist) {
   // With the data-polling chain, the next layer's attention (wide form, one
   // split) runs inside each chain launch; its output alternates between att
   // and att2 so that a launch never writes what its own Wo blocks read.
-  const bool fuse = d->tail_poll && d->fuse_att && d->att2 && dec_attention_fusable(attn_args(1 < L ? 1 : 0, d->att));
+  const bool fuse = !d->page8 && d->tail_poll && d->fuse_att && d->att2 && dec_attention_fusable(attn_args(1 < L ? 1 : 0, d->att));
   auto att_of = [&](int l) { return fuse && (l & 1) ? d->att2 : d->att; };
-  DCHK(op, dec_attention(attn_args(0, att_of(0)), st));
+  auto attend = [&](int l) {
+    if (d->page8) return step_attention8(d, op, l, l == 0 ? skinny_splits(N1, D) : 1, d->rr_d, d->err_d, d->att);
+    DCHK(op, dec_attention(attn_args(l, att_of(l)), st));
+    return (int)ANE_OK;
+  };
+  if (int rc = attend(0)) return rc;
   for (int l = 0; l < L; l++) {
     const DecLayerOff& o = d->off[l];
     const bool last = l + 1 == L;
@@ -416,15 +542,16 @@ int enqueue_step_tail(ane_decoder* d, float* logits, uint16_t* hist) {
       t.b_att = nb * d->NKV;
     }
     DCHK(op, dec_tail(t, st));
-    if (!fuse && !last) DCHK(op, dec_attention(attn_args(l + 1, d->att), st));
+    if (!fuse && !last)
+      if (int rc = attend(l + 1)) return rc;
   }
   SkinnyArgs s;
   memset(&s, 0, sizeof s);
   s.nb = nb;
   s.X = d->xg_att; s.W = d->fembed; s.N = d->V; s.K = D; s.amax = d->amax;
-  s.logits = logits; s.nvalid = d->V; s.rr = d->rr_d;
+  s.logits = d->controls ? d->logits_d : logits; s.nvalid = d->V; s.rr = d->rr_d;
   DCHK(op, classifier_argmax(s, st));
-  DCHK(op, argmax_reduce(d->tok_d, hist, d->ctr_d + 1, d->amax, d->V / 32, nb, st));
+  if (int rc = choose(d, op, hist)) return rc;
   DCHK(op, dec_advance(d->ctr_d, st));
   return ANE_OK;
 }
@@ -459,10 +586,7 @@ int tail_failed(ane_decoder* d, const char* op, bool* failed) {
 void latch_per_gemm(ane_decoder* d) {
   d->use_tail = false;
   d->chain_latched = 1;
-  if (d->gexec) (void)hipGraphExecDestroy(d->gexec);
-  if (d->graph) (void)hipGraphDestroy(d->graph);
-  d->gexec = nullptr;
-  d->graph = nullptr;
+  drop_graph(d);
 }
 
 // The start of a step / generate call, kept so that the call can be redone:
@@ -569,11 +693,22 @@ extern "C" int ane_decode_prefill(ane_decoder* d, const uint16_t* prefix, int32_
   if (plen < 64 || plen % 64 || plen >= d->C)
     return dfail(d, ANE_ERR_ARG, "storiesane decode prefill: plen=%d must be a multiple of 64 below max_ctx=%d",
                  plen, d->C);
+  if (d->controls && d->ctl_mask_rows > 1 && d->ctl_mask_rows < nseq)
+    return dfail(d, ANE_ERR_ARG, "storiesane decode prefill: nseq=%d, but the controls' mask has %d rows", nseq,
+                 d->ctl_mask_rows);
   const int D = d->D, H = d->H, N1 = d->N1;
   const hipStream_t st = d->stream;
   DCHK(op, hipSetDevice(d->cfg.device));
   DCHK(op, hipMemcpyAsync(d->prefix_d, prefix, (size_t)nseq * plen * 2, hipMemcpyHostToDevice, st));
   const int per = std::max(1, d->TC / plen);
+  if (d->page8) {
+    const int most = std::min(per, nseq);
+    for (int n : {most, nseq % most ? nseq % most : most})
+      if (int rc = room8(d, op, batch8(d, 0, n, n * plen, plen, plen))) return rc;
+    DCHK(op, dec_prompt_plan(d->start8, d->off8, most, plen, st));
+  }
+  if (d->controls)
+    DCHK(op, dec_history_prompt(d->ctl_hist, d->C, d->prefix_d, plen, d->ctl_len, d->ctl_prompt, nseq, st));
   for (int s0 = 0; s0 < nseq; s0 += per) {
     const int n = std::min(per, nseq - s0), T = n * plen;
     DCHK(op, embed_lookup(d->px, d->P + d->off_embed, d->prefix_d + (size_t)s0 * plen, T, D, d->V, st));
@@ -587,8 +722,10 @@ extern "C" int ane_decode_prefill(ane_decoder* d, const uint16_t* prefix, int32_
         p.C = d->pqkv; p.ldc = N1;
         DCHK(op, gemm(d, d->pxn, d->wqkv + (size_t)l * N1 * D, T, N1, D, EPI_STORE_H, p));
       }
-      DCHK(op, prefill_kv_write(d->pqkv, kcl, vcl, d->rope_cos, d->rope_sin, s0, n, plen, d->NH, d->NKV, d->C, st));
-      {
+      if (d->page8) {
+        if (int rc = attention8(d, op, l, batch8(d, s0, n, T, plen, plen), d->pqkv, d->patt, false)) return rc;
+      } else {
+        DCHK(op, prefill_kv_write(d->pqkv, kcl, vcl, d->rope_cos, d->rope_sin, s0, n, plen, d->NH, d->NKV, d->C, st));
         PrefillAttnArgs a;
         a.qkv = d->pqkv; a.ldq = N1; a.kc = kcl; a.vc = vcl; a.out = d->patt; a.seq0 = s0; a.nseq = n; a.S = plen;
         a.NH = d->NH; a.NKV = d->NKV; a.max_ctx = d->C; a.scale = 0.125f;
@@ -619,9 +756,9 @@ extern "C" int ane_decode_prefill(ane_decoder* d, const uint16_t* prefix, int32_
   memset(&s, 0, sizeof s);
   s.nb = nseq;
   s.X = d->xn; s.W = d->fembed; s.N = d->V; s.K = D; s.amax = d->amax;
-  s.logits = logits ? d->logits_d : nullptr; s.nvalid = d->V;
+  s.logits = logits || d->controls ? d->logits_d : nullptr; s.nvalid = d->V;
   DCHK(op, classifier_argmax(s, st));
-  DCHK(op, argmax_reduce(d->tok_d, nullptr, nullptr, d->amax, d->V / 32, nseq, st));
+  if (int rc = choose(d, op, nullptr)) return rc;
   DCHK(op, dec_set_ctr(d->ctr_d, plen, 0, st));
   d->pos = plen;
   return copy_out(d, next_tok, logits);  // prefill launches no chain kernel: nothing to check
@@ -633,6 +770,8 @@ extern "C" int ane_decode_step(ane_decoder* d, const uint16_t* in_tok, uint16_t*
   if (d->nseq == 0) return dfail(d, ANE_ERR_STATE, "storiesane decode step: no prefill");
   if (d->pos >= d->C) return dfail(d, ANE_ERR_ARG, "storiesane decode step: cache full (max_ctx=%d)", d->C);
   DCHK(op, hipSetDevice(d->cfg.device));
+  if (d->page8)
+    if (int rc = room8(d, op, batch8(d, 0, d->nseq, d->nseq, d->C, 1))) return rc;
   if (in_tok) DCHK(op, hipMemcpyAsync(d->tok_d, in_tok, (size_t)d->nseq * 2, hipMemcpyHostToDevice, d->stream));
   const int pos0 = d->pos;
   int rc = d->use_tail ? save_start(d, op) : ANE_OK;
@@ -660,6 +799,8 @@ extern "C" int ane_decode_generate(ane_decoder* d, int32_t nsteps, uint16_t* out
                  d->pos, d->C);
   if (nsteps == 0) return ANE_OK;
   DCHK(op, hipSetDevice(d->cfg.device));
+  if (d->page8)
+    if (int rc = room8(d, op, batch8(d, 0, d->nseq, d->nseq, d->C, 1))) return rc;
   const int pos0 = d->pos;
   int rc = d->use_tail ? save_start(d, op) : ANE_OK;
   if (rc == ANE_OK) rc = generate_run(d, op, nsteps, out_tok);
@@ -682,10 +823,7 @@ namespace {
 int generate_run(ane_decoder* d, const char* op, int nsteps, uint16_t* out_tok) {
   const hipStream_t st = d->stream;
   if (!d->gexec || d->graph_nseq != d->nseq) {
-    if (d->gexec) (void)hipGraphExecDestroy(d->gexec);
-    if (d->graph) (void)hipGraphDestroy(d->graph);
-    d->gexec = nullptr;
-    d->graph = nullptr;
+    drop_graph(d);
     DCHK(op, hipStreamBeginCapture(st, hipStreamCaptureModeThreadLocal));
     int rc = enqueue_step(d, nullptr, d->hist_d);
     hipGraph_t g = nullptr;
@@ -723,11 +861,168 @@ extern "C" int32_t ane_decode_position(ane_decoder* d) { return d ? d->pos : -1;
 
 extern "C" double ane_decode_last_ms(ane_decoder* d) { return d ? d->last_ms : 0.0; }
 
+namespace {
+
+void dfree(ane_decoder* d, void* p) {
+  d->allocs.erase(std::remove(d->allocs.begin(), d->allocs.end(), p), d->allocs.end());
+  if (p) (void)hipFree(p);
+}
+template <typename T>
+void drop(ane_decoder* d, T** p) {
+  dfree(d, *p);
+  *p = nullptr;
+}
+
+int alloc8(ane_decoder* d, const char* op, int page) {
+  const int per = (d->C + page - 1) / page;
+  const size_t pages = (size_t)d->L * d->B * per, codes = pages * d->NKV * page * 64;
+  DCHK(op, dalloc(d, &d->k8, codes));
+  DCHK(op, dalloc(d, &d->v8, codes));
+  DCHK(op, dalloc(d, &d->ke8, pages * d->NKV));
+  DCHK(op, dalloc(d, &d->ve8, pages * d->NKV));
+  DCHK(op, dalloc(d, &d->table8, (size_t)d->B * per));
+  DCHK(op, dalloc(d, &d->start8, (size_t)d->B + 1));
+  DCHK(op, dalloc(d, &d->off8, (size_t)d->B + 1));
+  DCHK(op, dalloc(d, &d->qkv8, (size_t)kDecRows * d->N1));
+  std::vector<int> t((size_t)d->B * per);
+  for (size_t i = 0; i < t.size(); i++) t[i] = (int)i;
+  DCHK(op, hipMemcpy(d->table8, t.data(), t.size() * 4, hipMemcpyHostToDevice));
+  d->seq_pages = per;
+  d->page8 = page;
+  return ANE_OK;
+}
+void free8(ane_decoder* d) {
+  drop(d, &d->k8); drop(d, &d->v8); drop(d, &d->ke8); drop(d, &d->ve8);
+  drop(d, &d->table8); drop(d, &d->start8); drop(d, &d->off8); drop(d, &d->qkv8);
+  d->page8 = d->seq_pages = 0;
+}
+int alloc16(ane_decoder* d, const char* op) {
+  const size_t cache = (size_t)d->L * d->B * d->NKV * d->C * 64;
+  DCHK(op, dalloc(d, &d->kc, cache));
+  DCHK(op, dalloc(d, &d->vc, cache));
+  return ANE_OK;
+}
+
+}  // namespace
+
+extern "C" int ane_decode_set_cache(ane_decoder* d, int32_t page_tokens) {
+  const char* op = "set cache";
+  if (!d || !d->stream) return ANE_ERR_STATE;
+  if (page_tokens != 0 && (page_tokens < 16 || page_tokens > 256 || (page_tokens & (page_tokens - 1))))
+    return dfail(d, ANE_ERR_ARG, "storiesane decode set cache: page_tokens=%d must be 0, 16, 32, 64, 128 or 256",
+                 page_tokens);
+  DCHK(op, hipSetDevice(d->cfg.device));
+  DCHK(op, hipStreamSynchronize(d->stream));
+  drop_graph(d);
+  d->nseq = 0;  // what the old cache held is gone
+  if (page_tokens == d->page8) return ANE_OK;
+  const int before = d->page8;
+  // the old cache goes first: there may not be room for both
+  free8(d);
+  drop(d, &d->kc);
+  drop(d, &d->vc);
+  int rc = page_tokens ? alloc8(d, op, page_tokens) : alloc16(d, op);
+  if (rc != ANE_OK) {  // back to what was there
+    free8(d);
+    drop(d, &d->kc);
+    drop(d, &d->vc);
+    const std::string why = d->err;
+    const int back = before ? alloc8(d, op, before) : alloc16(d, op);
+    if (back != ANE_OK) {
+      free_all(d);  // the decoder is closed
+      return dfail(d, back, "storiesane decode set cache: no memory for either cache");
+    }
+    d->err = why;
+  }
+  return rc;
+}
+
+extern "C" int ane_decode_set_controls(ane_decoder* d, const ane_decode_controls* c) {
+  const char* op = "set controls";
+  if (!d || !d->stream) return ANE_ERR_STATE;
+  if (!c) {
+    if (d->controls) drop_graph(d);
+    d->controls = false;
+    return ANE_OK;
+  }
+  if (!d->controls && d->nseq > 0)
+    return dfail(d, ANE_ERR_STATE, "storiesane decode set controls: a batch is active (set them before Prefill)");
+  const int B = d->B, W = (d->V + 31) / 32;
+  if (c->mask_rows < 0 || c->mask_rows > B || (c->mask == nullptr) != (c->mask_rows == 0) ||
+      (c->mask_rows > 1 && c->mask_rows < d->nseq))
+    return dfail(d, ANE_ERR_ARG, "storiesane decode set controls: mask_rows=%d must be 1 or cover the batch (%d), at "
+                                 "most %d", c->mask_rows, d->nseq, B);
+  if (d->V > 65535)
+    return dfail(d, ANE_ERR_ARG, "storiesane decode set controls: vocab=%d exceeds 65535", d->V);
+  DCHK(op, hipSetDevice(d->cfg.device));
+  if (!d->ctl_rows) {
+    float* rows = nullptr;
+    DCHK(op, dalloc(d, &d->ctl_bias, (size_t)d->V));
+    DCHK(op, dalloc(d, &d->ctl_mask, (size_t)B * W));
+    DCHK(op, dalloc(d, &d->ctl_hist, (size_t)B * d->C));
+    DCHK(op, dalloc(d, &d->ctl_len, (size_t)B));
+    DCHK(op, dalloc(d, &d->ctl_prompt, (size_t)B));
+    DCHK(op, dalloc(d, &d->ctl_tok, (size_t)B));
+    uint8_t* ws = nullptr;
+    const int64_t n = ane_control_logits_workspace(B, d->V);
+    SCHK(op, n);
+    DCHK(op, dalloc(d, &ws, (size_t)n));
+    d->ctl_ws = ws;
+    DCHK(op, dalloc(d, &rows, (size_t)3 * kDecRows));
+    d->ctl_rows = rows;  // last: all of them are there
+  }
+  ane_logits_args a{};
+  a.logits = a.out = d->logits_d;
+  a.logits_row = a.out_row = a.vocab = d->V;
+  a.device = d->cfg.device;
+  a.tokens = d->ctl_tok;
+  a.ws = d->ctl_ws;
+  a.ws_bytes = ane_control_logits_workspace(B, d->V);
+  // copies behind whatever the stream still runs, done before the call returns
+  HostCopy hc(&d->host_pool, d->cfg.device, d->stream);
+  const float* given[3] = {c->repetition, c->frequency, c->presence};
+  const float** into[3] = {&a.repetition, &a.frequency, &a.presence};
+  for (int i = 0; i < 3; i++)
+    if (given[i]) {
+      DCHK(op, hc.up(d->ctl_rows + i * kDecRows, given[i], (size_t)B * 4));
+      *into[i] = d->ctl_rows + i * kDecRows;
+    }
+  if (a.repetition || a.frequency || a.presence) {
+    a.history = d->ctl_hist;
+    a.history_row = a.history_max = d->C;
+    a.lengths = d->ctl_len;
+    a.prompts = d->ctl_prompt;
+  }
+  if (c->bias) {
+    DCHK(op, hc.up(d->ctl_bias, c->bias, (size_t)d->V * 4));
+    a.bias = d->ctl_bias;
+  }
+  if (c->mask) {
+    DCHK(op, hc.up(d->ctl_mask, c->mask, (size_t)c->mask_rows * W * 4));
+    a.mask = d->ctl_mask;
+    a.mask_row = c->mask_rows == 1 ? 0 : W;
+  }
+  DCHK(op, hc.finish());
+  // a captured step holds these arguments, not the arrays' contents
+  if (!d->controls || memcmp(&a, &d->ctl, sizeof a) != 0) drop_graph(d);
+  d->ctl = a;
+  d->ctl_mask_rows = c->mask_rows;
+  d->controls = true;
+  return ANE_OK;
+}
+
 extern "C" int ane_decode_debug_fill_cache(ane_decoder* d, int byte) {
   const char* op = "debug fill cache";
   if (!d || !d->stream) return ANE_ERR_STATE;
   const size_t bytes = (size_t)d->L * d->B * d->NKV * d->C * 64 * sizeof(half_t);
   DCHK(op, hipSetDevice(d->cfg.device));
+  if (d->page8) {
+    const size_t pages = (size_t)d->L * d->B * d->seq_pages, codes = pages * d->NKV * d->page8 * 64;
+    DCHK(op, hipMemsetAsync(d->k8, byte & 0xff, codes, d->stream));
+    DCHK(op, hipMemsetAsync(d->v8, byte & 0xff, codes, d->stream));
+    DCHK(op, hipStreamSynchronize(d->stream));
+    return ANE_OK;
+  }
   DCHK(op, hipMemsetAsync(d->kc, byte & 0xff, bytes, d->stream));
   DCHK(op, hipMemsetAsync(d->vc, byte & 0xff, bytes, d->stream));
   DCHK(op, hipStreamSynchronize(d->stream));

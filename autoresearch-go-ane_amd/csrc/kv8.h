@@ -158,6 +158,11 @@ __device__ __forceinline__ int kv8_exponent(uint32_t amax_bits) {
 // kernels' form; ANE_OK or ANE_ERR_ARG with the message set.
 int kv8_check(const char* op, const ane_kv8_cache* c, const ane_kv8_batch* b, Kv8Batch* out);
 
+// ane_kv8_attend; frag: out is the decoder's 64-row activation fragments
+// (decode.h), its strides unused.
+int kv8_attend(const ane_kv8_cache* cache, const ane_kv8_batch* batch, const ane_kv8_attend_args* args, bool frag,
+               void* stream);
+
 // Whether fp16 rows of [rows][heads][dh] with these strides do not overlap
 // (outputs; either order of the two outer dimensions).
 inline bool kv8_apart(int64_t rows, int64_t row, int64_t heads, int64_t head, int64_t dh) {

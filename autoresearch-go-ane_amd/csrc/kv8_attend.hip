@@ -16,6 +16,7 @@
 // at the end, in LDS.  There is no barrier in the loop.
 #include <algorithm>
 
+#include "decode.h"
 #include "kv8.h"
 #include "op_error.h"
 
@@ -30,6 +31,7 @@ struct AttendArgs {
   const half_t* q;
   half_t* out;
   int64_t q_row, q_head, out_row, out_head;
+  int frag;     // out is the decoder's activation fragments (decode.h) instead
   int G;        // query heads per key/value head
   int tt;       // tokens per tile: tt * G <= rows of the tile
   int tiles;    // items
@@ -38,6 +40,12 @@ struct AttendArgs {
   float c;      // scale * log2(e)
   float* part;  // [tiles][NKV][nsplit][tt * G][DH + 2]: sums, maximum, sum of exponentials
 };
+
+// where dimension d of a row's query head goes
+template <int DH>
+__device__ __forceinline__ half_t* out_at(const AttendArgs& a, int row, int head, int d) {
+  return a.out + (a.frag ? (int64_t)act_frag_off(row, head * DH + d) : row * a.out_row + head * a.out_head + d);
+}
 
 // The keys of a tile are cut into equal parts of whole rounds, at most nsplit.
 __device__ __forceinline__ int part_keys(int keys, int nsplit, int round) {
@@ -381,14 +389,13 @@ __global__ __launch_bounds__(64 * KW * RW, KW == 16 ? 1 : NT == 1 ? (DH == 64 ? 
       const int r = 16 * t + col;
       const float inv = l[t][0] == 0.f ? 0.f : 1.f / l[t][0];
       const int tok = r / a.G, hg = r - tok * a.G;
-      half_t* y = a.out + (span.row + tok) * a.out_row + (h * a.G + hg) * a.out_head + 4 * g;
       if (r < rows) {
 #pragma unroll
         for (int d = 0; d < ND; d++) {
           half4 z;
 #pragma unroll
           for (int j = 0; j < 4; j++) z[j] = (half_t)(o[d][t][j] * inv);
-          *reinterpret_cast<half4*>(y + 16 * d) = z;
+          *reinterpret_cast<half4*>(out_at<DH>(a, span.row + tok, h * a.G + hg, 16 * d + 4 * g)) = z;
         }
       }
     }
@@ -440,7 +447,7 @@ __global__ __launch_bounds__(64 * KW * RW, KW == 16 ? 1 : NT == 1 ? (DH == 64 ? 
         half4 y;
 #pragma unroll
         for (int j = 0; j < 4; j++) y[j] = (half_t)(x[j] * inv);
-        *reinterpret_cast<half4*>(a.out + (span.row + tok) * a.out_row + (h * a.G + hg) * a.out_head + d) = y;
+        *reinterpret_cast<half4*>(out_at<DH>(a, span.row + tok, h * a.G + hg, d)) = y;
       } else {
         float* p = part + (size_t)r * (DH + 2);
 #pragma unroll
@@ -502,9 +509,8 @@ __global__ __launch_bounds__(256) void join_kernel(AttendArgs a) {
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   const int tok = r / a.G, hg = r - tok * a.G;
-  half_t* y = a.out + (span.row + tok) * a.out_row + (h * a.G + hg) * a.out_head + lane;
 #pragma unroll
-  for (int j = 0; j < W; j++) y[64 * j] = (half_t)(x[j] * inv);
+  for (int j = 0; j < W; j++) *out_at<DH>(a, span.row + tok, h * a.G + hg, lane + 64 * j) = (half_t)(x[j] * inv);
 }
 
 struct Plan {
@@ -592,6 +598,11 @@ extern "C" int64_t ane_kv8_attend_workspace(const ane_kv8_cache* cache, const an
 
 extern "C" int ane_kv8_attend(const ane_kv8_cache* cache, const ane_kv8_batch* batch, const ane_kv8_attend_args* args,
                               void* stream) {
+  return kv8_attend(cache, batch, args, false, stream);
+}
+
+int ane::kv8_attend(const ane_kv8_cache* cache, const ane_kv8_batch* batch, const ane_kv8_attend_args* args, bool frag,
+                    void* stream) {
   const char* op = "kv8 attend";
   AttendArgs a;
   int rc = kv8_check(op, cache, batch, &a.b);
@@ -610,7 +621,9 @@ extern "C" int ane_kv8_attend(const ane_kv8_cache* cache, const ane_kv8_batch* b
   Plan p;
   rc = plan(op, a.b, *batch, cache->head_dim, g.heads, &p);
   if (rc) return rc;
-  if (!kv8_apart(a.b.rows, g.out_row, g.heads, g.out_head, cache->head_dim))
+  if (frag && a.b.rows > kDecRows)
+    return op_fail(ANE_ERR_ARG, "storiesane %s: rows=%d of fragments, want at most %d", op, a.b.rows, kDecRows);
+  if (!frag && !kv8_apart(a.b.rows, g.out_row, g.heads, g.out_head, cache->head_dim))
     return op_fail(ANE_ERR_ARG, "storiesane %s: rows of out overlap", op);
   if (p.bytes > 0 && (!g.ws || g.ws_bytes < p.bytes))
     return op_fail(ANE_ERR_ARG, "storiesane %s: workspace of %lld bytes, want %lld", op,
@@ -624,6 +637,7 @@ extern "C" int ane_kv8_attend(const ane_kv8_cache* cache, const ane_kv8_batch* b
   a.G = g.heads / a.b.NKV; a.tt = p.tt; a.tiles = (int)p.tiles; a.nsplit = p.nsplit; a.round = p.round;
   a.c = g.scale * 1.44269504088896340736f;
   a.part = (float*)g.ws;
+  a.frag = frag;
   if (cache->head_dim == 64) launch<64>(a, p, (hipStream_t)stream);
   else launch<128>(a, p, (hipStream_t)stream);
   const hipError_t h = hipGetLastError();

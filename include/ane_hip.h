@@ -401,6 +401,31 @@ double ane_decode_last_ms(ane_decoder *d);
  * ane/train_full.go:356-368).  If the redo itself fails, the active batch is
  * dropped: Step / Generate then refuse until the next Prefill. */
 int32_t ane_decode_fused_chain(ane_decoder *d);
+/* Which cache a decoder keeps (no reference counterpart): page_tokens = 0 the
+ * fp16 one (as opened), 16..256 (a power of two) the paged 8-bit one of
+ * ane_serve.h, half the memory and half the bytes an attention reads; codes of
+ * e4m3 with an exponent for each page and head.  Frees the one cache and
+ * allocates the other (on failure the old one is allocated again) and drops
+ * the active batch: Prefill comes next. */
+int ane_decode_set_cache(ane_decoder *d, int32_t page_tokens);
+/* Controls on the logits before each next token is chosen (no reference
+ * counterpart; formulas at ane_control_logits, ane_serve.h), for all later
+ * Prefill, Step and Generate calls; NULL: none, the plain argmax.  Penalties
+ * count the tokens since Prefill (prompt) and those fed by steps (output), so
+ * the first controls come before Prefill (ANE_ERR_STATE while a batch is
+ * active); once set they may be changed between any two calls, a grammar's
+ * mask before each Step for instance.  Logits returned are the changed ones;
+ * a sequence that nothing is allowed for gets ANE_NO_TOKEN (65535, the zero
+ * embedding when fed).  The arrays are copied.
+ *   repetition, frequency, presence [max_batch], bias [vocab], mask
+ *   [mask_rows][ceil(vocab/32)] with mask_rows 1 (for all) or at least the
+ *   batch's size; any may be NULL (mask_rows 0). */
+typedef struct ane_decode_controls {
+  const float *repetition, *frequency, *presence, *bias;
+  const uint32_t *mask;
+  int32_t mask_rows;
+} ane_decode_controls;
+int ane_decode_set_controls(ane_decoder *d, const ane_decode_controls *c);
 /* Test-only (no reference counterpart): fills every byte of the KV cache
  * with `byte` (0xFF: fp16 NaN everywhere), so a test can show that no
  * position is read before it is written. */
