@@ -12,7 +12,7 @@
 // exponent applied) in the registers.
 //
 // A block is one tile and one key/value head (and one part of the keys where
-// tiles are few); its waves take steps of 32 or 64 keys in turn and meet once
+// tiles are few); its waves take steps of 32 keys in turn and meet once
 // at the end, in LDS.  There is no barrier in the loop.
 #include <algorithm>
 
@@ -23,6 +23,11 @@
 namespace ane {
 
 namespace {
+
+// Units of 16 keys in a wave's step.  Two: with four, single tokens were slower
+// (64 of 1100 tokens 11.1 us, not 10.7) and larger tiles do not fit.
+constexpr int NU = 2;
+constexpr int kStep = 16 * NU;
 
 struct AttendArgs {
   Kv8Batch b;
@@ -38,7 +43,8 @@ struct AttendArgs {
   int nsplit;   // parts that the keys of a tile are cut into, at most
   int round;    // keys that a block takes at a time: parts are multiples of it
   float c;      // scale * log2(e)
-  float* part;  // [tiles][NKV][nsplit][tt * G][DH + 2]: sums, maximum, sum of exponentials
+  float* part;  // [tiles][NKV][nsplit][tt * G][DH]: a row's sums
+  float2* ml;   // [tiles][NKV][nsplit][tt * G]: their maximum and sum of exponentials
 };
 
 // where dimension d of a row's query head goes
@@ -48,9 +54,9 @@ __device__ __forceinline__ half_t* out_at(const AttendArgs& a, int row, int head
 }
 
 // The keys of a tile are cut into equal parts of whole rounds, at most nsplit.
-__device__ __forceinline__ int part_keys(int keys, int nsplit, int round) {
-  const int n = (keys + nsplit - 1) / nsplit;
-  return (n + round - 1) / round * round;
+__device__ __forceinline__ int part_keys(const AttendArgs& a, int keys) {
+  const int n = (keys + a.nsplit - 1) / a.nsplit;
+  return (n + a.round - 1) / a.round * a.round;
 }
 
 __device__ __forceinline__ float xor16_max(float x) {
@@ -76,7 +82,7 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
 // the exponents (K in bits 0..7, V in 8..15) and whether it is there (bit 16).
 // A page that is not there reads the pool's first, which exists; its scores
 // are masked and its values cleared.
-template <int DH, int NU>
+template <int DH>
 struct Step {
   u32x4 k[NU][DH / 64], v[NU][DH / 64];
   int ex[NU];
@@ -85,12 +91,17 @@ constexpr int kThere = 1 << 16;
 __device__ __forceinline__ float k_scale(int ex) { return kv8_scale((int8_t)(ex & 0xff)); }
 __device__ __forceinline__ float v_scale(int ex) { return kv8_scale((int8_t)(ex >> 8 & 0xff)); }
 
-// NT: tiles of 16 rows; NU: units of 16 keys in a wave's step; KW: waves that
-// share a tile's keys; RW: tiles a block takes, each by waves of its own (KW =
-// 1: the waves have nothing to do with each other); ONE: a step's keys are of
-// one page (pages of at least 16 NU tokens).
-template <int DH, int NT, int NU, int KW, int RW, bool ONE>
-__global__ __launch_bounds__(64 * KW * RW, KW == 16 ? 1 : NT == 1 ? (DH == 64 ? 4 : 3) : DH == 64 ? (NT == 2 ? 4 : 3) : 2) void attend_kernel(AttendArgs a) {
+// Waves a SIMD is to hold: what the registers of a form leave.
+constexpr int waves_per_simd(int DH, int NT) {
+  return NT == 1 ? (DH == 64 ? 4 : 3) : DH == 64 ? (NT == 2 ? 4 : 3) : 2;
+}
+
+// NT: tiles of 16 rows; KW: waves that share a tile's keys; RW: tiles a block
+// takes, each by a wave of its own (KW = 1: the waves have nothing to do with
+// each other); ONE: a step's keys are of one page (pages of at least kStep
+// tokens).
+template <int DH, int NT, int KW, int RW, bool ONE>
+__global__ __launch_bounds__(64 * KW * RW, waves_per_simd(DH, NT)) void attend_kernel(AttendArgs a) {
   static_assert(KW == 1 || RW == 1, "the waves of a block meet over one tile");
   constexpr int R = 16 * NT;    // rows of the tile
   constexpr int NM = DH / 32;   // MFMAs along the head dimension
@@ -100,7 +111,6 @@ __global__ __launch_bounds__(64 * KW * RW, KW == 16 ? 1 : NT == 1 ? (DH == 64 ? 
   constexpr int PASS = KW == 4 && R * DH > 2048 ? 2 : 1;
   constexpr int DP = DH / PASS;
   constexpr int LD = DP + 4;
-  constexpr int KS = 16 * NU;   // keys of a step
   __shared__ __attribute__((aligned(16))) float lds_o[KW == 1 ? 1 : KW][KW == 1 ? 1 : R][LD];
   __shared__ float lds_m[KW][R], lds_l[KW][R];
   const Kv8Batch& b = a.b;
@@ -117,7 +127,7 @@ __global__ __launch_bounds__(64 * KW * RW, KW == 16 ? 1 : NT == 1 ? (DH == 64 ? 
   if (span.n == 0) return;
   const int rows = span.n * a.G;
   const int kend = span.pos + span.n;  // keys of the tile's last token
-  const int pk = part_keys(kend, a.nsplit, a.round);
+  const int pk = part_keys(a, kend);
   const int k0 = sp * pk;
   if (k0 >= kend) return;
   const int k1 = min(kend, k0 + pk);
@@ -146,8 +156,8 @@ __global__ __launch_bounds__(64 * KW * RW, KW == 16 ? 1 : NT == 1 ? (DH == 64 ? 
   // The codes of the step at kb; `on` false: nothing is wanted of them (one
   // line is read).
   const uint32_t kl = col * DH + 16 * g, vl = lane * (DH / 4);
-  auto fetch = [&](Step<DH, NU>& s, int kb, bool on) {
-    if (kb + KS > wend) window(kb >> b.pshift);
+  auto fetch = [&](Step<DH>& s, int kb, bool on) {
+    if (kb + kStep > wend) window(kb >> b.pshift);
     const uint32_t ko = on ? kl : 0, vo = on ? vl : 0;
     size_t at = 0;
 #pragma unroll
@@ -184,8 +194,8 @@ __global__ __launch_bounds__(64 * KW * RW, KW == 16 ? 1 : NT == 1 ? (DH == 64 ? 
 #pragma unroll
     for (int m = 0; m < NM; m++) q[t][m] = ld_h8(p + 64 * (m >> 1) + 8 * (m & 1));
   }
-  Step<DH, NU> cur;
-  int kb = k0 + wave * KS;
+  Step<DH> cur;
+  int kb = k0 + wave * kStep;
   fetch(cur, kb, kb < k1);
   // waited for here, once (they were issued first), and not in every step
 #pragma unroll
@@ -211,11 +221,11 @@ __global__ __launch_bounds__(64 * KW * RW, KW == 16 ? 1 : NT == 1 ? (DH == 64 ? 
   }
 
   // whether a step holds keys that some row does not attend to
-  auto at_edge = [&](const Step<DH, NU>& s, int kb) {
+  auto at_edge = [&](const Step<DH>& s, int kb) {
     int all = s.ex[0];
 #pragma unroll
     for (int u = 1; u < (ONE ? 1 : NU); u++) all &= s.ex[u];
-    return kb + KS - 1 > span.pos || !(all & kThere);
+    return kb + kStep - 1 > span.pos || !(all & kThere);
   };
 
   half8 ones;
@@ -223,7 +233,7 @@ __global__ __launch_bounds__(64 * KW * RW, KW == 16 ? 1 : NT == 1 ? (DH == 64 ? 
   for (int j = 0; j < 8; j++) ones[j] = (half_t)1.f;
   asm volatile("" : "+v"(ones));  // in vector registers: scalar ones are spilled and read back in every step
   uint32_t nan = 0;
-  auto step = [&](Step<DH, NU>& s, int kb) {
+  auto step = [&](Step<DH>& s, int kb) {
     const bool edge = at_edge(s, kb);
     floatx4 sc[NU][NT];
 #pragma unroll
@@ -334,15 +344,15 @@ __global__ __launch_bounds__(64 * KW * RW, KW == 16 ? 1 : NT == 1 ? (DH == 64 ? 
   // `then`; whether there is one.  Behind the last step they are of one line,
   // so that every path has the same loads outstanding and waits for no more
   // than it needs.
-  auto turn = [&](Step<DH, NU>& now, Step<DH, NU>& then) {
-    const int kn = kb + KS * KW;
+  auto turn = [&](Step<DH>& now, Step<DH>& then) {
+    const int kn = kb + kStep * KW;
     fetch(then, kn < k1 ? kn : kb, kn < k1);
     step(now, kb);
     kb = kn;
     return kn < k1;
   };
   if (kb < k1) {
-    Step<DH, NU> nxt;
+    Step<DH> nxt;
     while (turn(cur, nxt) && turn(nxt, cur)) {
     }
   }
@@ -350,7 +360,7 @@ __global__ __launch_bounds__(64 * KW * RW, KW == 16 ? 1 : NT == 1 ? (DH == 64 ? 
     // rare: how many NaN of each dimension a row attends to, as a product of
     // zeros and ones, over the steps that had them taken out
     wend = 0;
-    for (kb = k0 + wave * KS; kb < k1; kb += KS * KW) {
+    for (kb = k0 + wave * kStep; kb < k1; kb += kStep * KW) {
       fetch(cur, kb, true);
       if (!at_edge(cur, kb)) continue;
 #pragma unroll
@@ -418,7 +428,7 @@ __global__ __launch_bounds__(64 * KW * RW, KW == 16 ? 1 : NT == 1 ? (DH == 64 ? 
     if (g == 0) lds_l[wave][r] = l[t][0] * m[t];
   }
   const bool whole = pk >= kend;
-  float* part = a.part + (((size_t)tile * b.NKV + h) * a.nsplit + sp) * ((size_t)a.tt * a.G * (DH + 2));
+  const size_t part = (((size_t)tile * b.NKV + h) * a.nsplit + sp) * ((size_t)a.tt * a.G);  // its first row
 #pragma unroll
   for (int z = 0; z < PASS; z++) {
     if (z > 0) __syncthreads();
@@ -449,15 +459,12 @@ __global__ __launch_bounds__(64 * KW * RW, KW == 16 ? 1 : NT == 1 ? (DH == 64 ? 
         for (int j = 0; j < 4; j++) y[j] = (half_t)(x[j] * inv);
         *reinterpret_cast<half4*>(out_at<DH>(a, span.row + tok, h * a.G + hg, d)) = y;
       } else {
-        float* p = part + (size_t)r * (DH + 2);
-#pragma unroll
-        for (int j = 0; j < 4; j++) p[d + j] = x[j];
+        *reinterpret_cast<floatx4*>(a.part + (part + r) * DH + d) = x;
         if (d == 0) {
           float mm = lds_m[0][r];
 #pragma unroll
           for (int w = 1; w < KW; w++) mm = fmaxf(mm, lds_m[w][r]);
-          p[DH] = mm;
-          p[DH + 1] = ls;
+          a.ml[part + r] = make_float2(mm, ls);
         }
       }
     }
@@ -478,15 +485,17 @@ __global__ __launch_bounds__(256) void join_kernel(AttendArgs a) {
   const int r = blockIdx.y * 4 + (threadIdx.x >> 6);
   if (r >= span.n * a.G) return;
   const int kend = span.pos + span.n;
-  const int pk = part_keys(kend, a.nsplit, a.round);
+  const int pk = part_keys(a, kend);
   if (pk >= kend) return;  // one part: the output is written
   const int np = (kend + pk - 1) / pk;
-  const size_t stride = (size_t)a.tt * a.G * (DH + 2);
-  const float* part = a.part + ((size_t)tile * b.NKV + h) * a.nsplit * stride + (size_t)r * (DH + 2);
+  const size_t stride = (size_t)a.tt * a.G;  // rows of a part
+  const size_t row = ((size_t)tile * b.NKV + h) * a.nsplit * stride + r;
+  const float* part = a.part + row * DH;
   float m = -INFINITY, l = 0.f;
   if (lane < np) {
-    m = part[lane * stride + DH];
-    l = part[lane * stride + DH + 1];
+    const float2 p = a.ml[row + lane * stride];
+    m = p.x;
+    l = p.y;
   }
   const float mm = wave_max(m);
   const float al = __builtin_amdgcn_exp2f(m - (mm == -INFINITY ? 0.f : mm));
@@ -498,7 +507,7 @@ __global__ __launch_bounds__(256) void join_kernel(AttendArgs a) {
 #pragma unroll
     for (int u = 0; u < B; u++)
 #pragma unroll
-      for (int j = 0; j < W; j++) v[u][j] = part[min(s + u, np - 1) * stride + lane + 64 * j];
+      for (int j = 0; j < W; j++) v[u][j] = part[min(s + u, np - 1) * stride * DH + lane + 64 * j];
 #pragma unroll
     for (int u = 0; u < B; u++) {
       const float w = s + u < np ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(al), s + u)) : 0.f;
@@ -525,7 +534,9 @@ int plan(const char* op, const Kv8Batch& b, const ane_kv8_batch& given, int DH, 
                    b.NKV);
   const int G = heads / b.NKV;
   if (b.nseq == 0 || b.rows == 0) return ANE_OK;
-  // rows of the longest sequence, or of the mean one where that is not known
+  // Tiles of 16, 32 or 48 rows: the smallest that takes the longest sequence's
+  // rows (the mean one's where that is not known).  At head dimension 128 the
+  // registers end at 32 (48 spill: two prompts of 2000 tokens 109 us, not 49).
   const int64_t most = (int64_t)G * (given.max_new ? std::min(given.max_new, b.rows) : (b.rows + b.nseq - 1) / b.nseq);
   p->nt = most <= 16 ? 1 : most <= 32 || DH == 128 ? 2 : 3;
   if (p->nt == 3 && 32 / G * 48 > 48 / G * 38) p->nt = 2;  // where 48 rows would stay a fifth emptier than 32
@@ -535,16 +546,28 @@ int plan(const char* op, const Kv8Batch& b, const ane_kv8_batch& given, int DH, 
   const int64_t blocks = (int64_t)p->tiles * b.NKV;
   const int cap = b.table_pages << b.pshift;
   const int len = given.max_len ? std::min(given.max_len, cap) : cap;
-  if (p->nt == 1) {
-    p->kw = DH == 64 && (len <= 1152 || (blocks >= 128 && len <= 2048)) ? 16 : 4;
-    p->round = p->kw * (DH == 64 ? 64 : 32);
-  } else {
-    p->round = 128;
-    if (len <= 512) p->kw = 1;
+  // Waves that share a tile's keys.  Single tokens over short contexts: 16 and
+  // no parts to join (one sequence of 777 tokens 6.9 us against 7.9 with four
+  // waves and parts, 64 of 1100 10.7 against 14.4; but one of 2000 9.1 against
+  // 8.0, and 64 of up to 5000 29 against 22).  Short prompts: each wave a tile
+  // of its own, nothing to meet over (64 prompts of 256 24 us against 40; but
+  // 8 of 512 equal, and one of 8192 160 against 125).
+  if (p->nt == 1) p->kw = DH == 64 && (len <= 1152 || (blocks >= 128 && len <= 2048)) ? 16 : 4;
+  else p->kw = len <= 512 ? 1 : 4;
+  p->round = p->kw * kStep;
+  // Parts of the keys, where there are fewer blocks than the GPU holds: four a
+  // CU for single tokens (40 long contexts, 80 blocks: 1024 blocks 106 us, 512
+  // 118; 64 sequences of 8 heads, 512 blocks: whole 33 us, in halves 38) and
+  // two else (chunks on contexts of up to 6000, 940 blocks: whole 63 us, halves
+  // 83).  Parts of ragged
+  // single tokens end at 4096 keys, so that one long context does not outlast
+  // the rest.
+  int64_t ns = 1;
+  if (p->kw == 4) {
+    const int64_t want = p->nt == 1 ? 1024 : 512;
+    if (blocks < 512) ns = (want + blocks - 1) / blocks;
+    if (p->nt == 1) ns = std::max<int64_t>(ns, (len + 4095) / 4096);
   }
-  int64_t want = p->kw == 16 ? 256 : p->nt == 1 ? 1024 : 512;
-  int64_t ns = std::max<int64_t>(blocks >= 512 ? 1 : (want + blocks - 1) / blocks, p->nt == 1 ? (len + 4095) / 4096 : 1);
-  if ((p->kw == 16 && len <= 2 * p->round) || p->kw == 1) ns = 1;
   ns = std::min<int64_t>(ns, (len + p->round - 1) / p->round);
   ns = std::max<int64_t>(1, std::min<int64_t>(ns, kMaxSplit));
   p->nsplit = (int)ns;
@@ -556,25 +579,24 @@ int plan(const char* op, const Kv8Batch& b, const ane_kv8_batch& given, int DH, 
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
-template <int DH, int NT, int NU, int KW, int RW>
+template <int DH, int NT, int KW, int RW>
 void launch_form(const AttendArgs& a, hipStream_t st) {
   const dim3 grid(((uint32_t)a.tiles + RW - 1) / RW * a.b.NKV * a.nsplit), block(64 * KW * RW);
-  if (16 * NU <= 1 << a.b.pshift)
-    hipLaunchKernelGGL((attend_kernel<DH, NT, NU, KW, RW, true>), grid, block, 0, st, a);
+  if (kStep <= 1 << a.b.pshift)
+    hipLaunchKernelGGL((attend_kernel<DH, NT, KW, RW, true>), grid, block, 0, st, a);
   else
-    hipLaunchKernelGGL((attend_kernel<DH, NT, NU, KW, RW, false>), grid, block, 0, st, a);
+    hipLaunchKernelGGL((attend_kernel<DH, NT, KW, RW, false>), grid, block, 0, st, a);
 }
 
 template <int DH>
 void launch(const AttendArgs& a, const Plan& p, hipStream_t st) {
-  constexpr int NU1 = DH == 64 ? 4 : 2;
-  if (DH == 64 && p.nt == 1 && p.kw == 16) launch_form<64, 1, 4, 16, 1>(a, st);
-  else if (p.nt == 1) launch_form<DH, 1, NU1, 4, 1>(a, st);
-  else if (p.nt == 2 && p.kw == 4) launch_form<DH, 2, 2, 4, 1>(a, st);
-  else if (p.nt == 2) launch_form<DH, 2, 2, 1, 4>(a, st);
+  if (DH == 64 && p.nt == 1 && p.kw == 16) launch_form<64, 1, 16, 1>(a, st);
+  else if (p.nt == 1) launch_form<DH, 1, 4, 1>(a, st);
+  else if (p.nt == 2 && p.kw == 4) launch_form<DH, 2, 4, 1>(a, st);
+  else if (p.nt == 2) launch_form<DH, 2, 1, 4>(a, st);
   else if constexpr (DH == 64) {
-    if (p.kw == 4) launch_form<DH, 3, 2, 4, 1>(a, st);
-    else launch_form<DH, 3, 2, 1, 4>(a, st);
+    if (p.kw == 4) launch_form<DH, 3, 4, 1>(a, st);
+    else launch_form<DH, 3, 1, 4>(a, st);
   }
   if (a.nsplit > 1)
     hipLaunchKernelGGL(join_kernel<DH>, dim3((uint32_t)a.tiles * a.b.NKV, (a.tt * a.G + 3) / 4), dim3(256), 0, st, a);
@@ -637,6 +659,7 @@ int ane::kv8_attend(const ane_kv8_cache* cache, const ane_kv8_batch* batch, cons
   a.G = g.heads / a.b.NKV; a.tt = p.tt; a.tiles = (int)p.tiles; a.nsplit = p.nsplit; a.round = p.round;
   a.c = g.scale * 1.44269504088896340736f;
   a.part = (float*)g.ws;
+  a.ml = (float2*)(a.part + (size_t)p.tiles * a.b.NKV * p.nsplit * p.tt * a.G * cache->head_dim);
   a.frag = frag;
   if (cache->head_dim == 64) launch<64>(a, p, (hipStream_t)stream);
   else launch<128>(a, p, (hipStream_t)stream);
