@@ -120,6 +120,8 @@ hipError_t dec_qkv_rows(const float* part, int ks, const float* rr, half_t* qkv,
                         const int* err, int* start, int* offsets, hipStream_t s);
 // start[i] = 0, offsets[i] = i * plen for i <= nseq (prefill of nseq prompts)
 hipError_t dec_prompt_plan(int* start, int* offsets, int nseq, int plen, hipStream_t s);
+// p[i] = i for i < n
+hipError_t dec_count_up(int* p, int n, hipStream_t s);
 // The history that penalties count, uint16 [..][ld]: the prompts (and the
 // row lengths), and at each step the token that is fed, at position ctr[0].
 hipError_t dec_history_prompt(uint16_t* hist, int ld, const uint16_t* prefix, int plen, int* lengths, int* prompts,

@@ -784,6 +784,11 @@ __global__ __launch_bounds__(64) void prompt_plan_kernel(int* start, int* offset
   if (i <= nseq) offsets[i] = i * plen;
 }
 
+__global__ __launch_bounds__(256) void count_up_kernel(int* p, int n) {
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i < n) p[i] = i;
+}
+
 __global__ __launch_bounds__(256) void history_prompt_kernel(uint16_t* hist, int ld, const uint16_t* prefix, int plen,
                                                              int* lengths, int* prompts) {
   const int b = blockIdx.x;
@@ -822,6 +827,11 @@ hipError_t dec_qkv_rows(const float* part, int ks, const float* rr, half_t* qkv,
 
 hipError_t dec_prompt_plan(int* start, int* offsets, int nseq, int plen, hipStream_t s) {
   hipLaunchKernelGGL(prompt_plan_kernel, dim3(nseq / 64 + 1), dim3(64), 0, s, start, offsets, nseq, plen);
+  return hipGetLastError();
+}
+
+hipError_t dec_count_up(int* p, int n, hipStream_t s) {
+  hipLaunchKernelGGL(count_up_kernel, dim3((n + 255) / 256), dim3(256), 0, s, p, n);
   return hipGetLastError();
 }
 

@@ -884,9 +884,8 @@ int alloc8(ane_decoder* d, const char* op, int page) {
   DCHK(op, dalloc(d, &d->start8, (size_t)d->B + 1));
   DCHK(op, dalloc(d, &d->off8, (size_t)d->B + 1));
   DCHK(op, dalloc(d, &d->qkv8, (size_t)kDecRows * d->N1));
-  std::vector<int> t((size_t)d->B * per);
-  for (size_t i = 0; i < t.size(); i++) t[i] = (int)i;
-  DCHK(op, hipMemcpy(d->table8, t.data(), t.size() * 4, hipMemcpyHostToDevice));
+  // each sequence's pages one after the other
+  DCHK(op, dec_count_up(d->table8, d->B * per, d->stream));
   d->seq_pages = per;
   d->page8 = page;
   return ANE_OK;

@@ -608,6 +608,48 @@ def test_two_streams_at_once():
             assert all(torch.equal(a, c) for a, c in zip(trio, alone[k]))
 
 
+@pytest.mark.parametrize("nseq", [65, 700, 4200])
+def test_many_sequences(nseq):
+    """More sequences than one round of the search takes (64 and 4096), a few
+    without new rows."""
+    r = np.random.default_rng(nseq)
+    lens = [(int(r.integers(0, 20)), int(r.choice([0, 1, 1, 1, 3]))) for _ in range(nseq)]
+    run_append(np.random.default_rng(1), lens, 2, 1, 64, 16)
+    run_attend(np.random.default_rng(2), lens, 2, 1, 64, 16, max_new=3, max_len=23)
+
+
+def test_nonsense_offsets_and_starts_stay_inside():
+    """What lies outside is not followed: no fault, and memory before and
+    behind the tensors is as it was."""
+    r = np.random.default_rng(50)
+    P, kvh, heads, dh, pages, rows = 16, 2, 4, 64, 6, 40
+    wild = np.array([-2**31, -7, 0, 3, 2**30, 2**31 - 1])
+    cos, sin = (dev(x) for x in rope_tables(3 * P, dh))
+    for seed in range(6):
+        r = np.random.default_rng(seed)
+        nseq = int(r.integers(1, 90))
+        pool = Pool(r, pages + 2, kvh, P, dh)
+        c = pool.cache
+        # a cache and rows inside larger ones, whose ends must not change
+        inner = ane.KVCache8(c.k[1:-1], c.v[1:-1], c.k_exp[1:-1], c.v_exp[1:-1])
+        table = np.where(r.random((nseq, 3)) < 0.3, r.choice(wild, (nseq, 3)), r.integers(0, pages, (nseq, 3)))
+        start = np.where(r.random(nseq) < 0.3, r.choice(wild, nseq), r.integers(0, 60, nseq))
+        offsets = np.where(r.random(nseq + 1) < 0.3, r.choice(wild, nseq + 1), r.integers(0, rows, nseq + 1))
+        x = torch.zeros((rows + 2, heads + 2 * kvh, dh), dtype=torch.float16, device=DEV)
+        q_out = torch.full((rows + 2, heads, dh), 7.0, dtype=torch.float16, device=DEV)
+        out = torch.full((rows + 2, heads, dh), 7.0, dtype=torch.float16, device=DEV)
+        before = pool.held()
+        b = batch_of(table, start, offsets, rows)
+        y = x[1:-1]
+        inner.Append(b, y[:, :heads], y[:, heads:heads + kvh], y[:, heads + kvh:], cos, sin, q_out[1:-1])
+        inner.Attend(b, q_out[1:-1], out[1:-1])
+        torch.cuda.synchronize()
+        for t in (q_out, out):
+            assert (t[[0, -1]] == 7.0).all()
+        for p, a in zip(before, pool.held()):
+            np.testing.assert_array_equal(p[[0, -1]], a[[0, -1]])
+
+
 def test_refusals():
     r = np.random.default_rng(40)
     pool = Pool(r, 4, 2, 16, 64)
