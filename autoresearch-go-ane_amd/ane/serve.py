@@ -107,7 +107,7 @@ class KVBatch:
         self._keep = (table, start, offsets)
         self.device, self.nseq, self.rows = dev, nseq, int(rows)
         self._c = _lib.Kv8Batch(t, s, o, stride, int(table.shape[1]), nseq, int(rows), int(max_len), int(max_new))
-        self._ref = C.byref(self._c)
+        self._at = C.addressof(self._c)
         self._ws = {}  # workspace bytes by (kv_heads, page_tokens, head_dim, heads)
 
 
@@ -138,7 +138,8 @@ class KVCache8:
         self._index = dev.index
         self._empty, self._u8, self._stream = torch.empty, torch.uint8, _stream_getter()
         self._c = _lib.Kv8Cache(kp, vp, ke, ve, pages, page, kvh, dh, dev.index)
-        self._ref = C.byref(self._c)
+        self._at = C.addressof(self._c)
+        self._append, self._attend = (_lib.plain(self._lib, "ane_kv8_" + n) for n in ("append", "attend"))
 
     @classmethod
     def Empty(cls, pages, kv_heads, head_dim=64, page_tokens=64, device="cuda"):
@@ -188,7 +189,7 @@ class KVCache8:
         self._batch(op, batch)
         kp, kr, kh = self._rows(op, "k", k, batch, self.kv_heads)
         vp, vr, vh = self._rows(op, "v", v, batch, self.kv_heads)
-        heads, qp, qr, qh, op_, or_, oh = 0, None, 0, 0, None, 0, 0
+        heads = qp = qr = qh = op_ = or_ = oh = 0
         if q is not None:
             qp, qr, qh = self._rows(op, "q", q, batch)
             heads = q.shape[1]
@@ -201,8 +202,8 @@ class KVCache8:
         n = cos.shape[0]
         if sin.shape[0] != n:
             _fail(op, f"cos has {n} positions, sin {sin.shape[0]}")
-        a = _lib.Kv8AppendArgs(qp, kp, vp, op_, cp, sp, qr, qh, kr, kh, vr, vh, or_, oh, heads, n)
-        rc = self._lib.ane_kv8_append(self._ref, batch._ref, C.byref(a), self._stream(self._index))
+        a = _lib.pack_append(qp, kp, vp, op_, cp, sp, qr, qh, kr, kh, vr, vh, or_, oh, heads, n)
+        rc = self._append(self._at, batch._at, a, self._stream(self._index))
         if rc:
             _check(self._lib, rc)
         return q_out
@@ -222,11 +223,11 @@ class KVCache8:
         key = (self.kv_heads, self.page_tokens, self.head_dim, heads)
         n = batch._ws.get(key)
         if n is None:
-            n = batch._ws[key] = _check(self._lib, self._lib.ane_kv8_attend_workspace(self._ref, batch._ref, heads))
+            n = batch._ws[key] = _check(self._lib, self._lib.ane_kv8_attend_workspace(self._c, batch._c, heads))
         ws = self._empty(n, dtype=self._u8, device=self.device) if n else None
-        a = _lib.Kv8AttendArgs(qp, yp, qr, qh, yr, yh, heads, self.head_dim ** -0.5 if scale is None else scale,
-                               None if ws is None else ws.data_ptr(), n)
-        rc = self._lib.ane_kv8_attend(self._ref, batch._ref, C.byref(a), self._stream(self._index))
+        a = _lib.pack_attend(qp, yp, qr, qh, yr, yh, heads, self.head_dim ** -0.5 if scale is None else scale,
+                             0 if ws is None else ws.data_ptr(), n)
+        rc = self._attend(self._at, batch._at, a, self._stream(self._index))
         if rc:
             _check(self._lib, rc)
         return out
@@ -268,9 +269,11 @@ class LogitControls:
         self._u16 = (torch.uint16, torch.int16)
         self._empty, self._u8, self._stream = torch.empty, torch.uint8, _stream_getter()
         self._index = self.device.index if self.device is not None else None
-        self._params = (a.repetition, a.frequency, a.presence, a.bias, a.mask, a.bias_row, a.mask_row)
+        self._params = (a.repetition or 0, a.frequency or 0, a.presence or 0, a.bias or 0, a.mask or 0, a.bias_row,
+                        a.mask_row)
         self._bytes = {}  # of the workspace, by rows
         self._lib = _lib.load()
+        self._control = _lib.plain(self._lib, "ane_control_logits")
 
     def _same_rows(self, name, n):
         if self.rows is not None and self.rows != n:
@@ -305,8 +308,7 @@ class LogitControls:
         if tokens is None:
             tokens = self._empty(rows, dtype=self._i32[0], device=logits.device)
         tp = self._vector("tokens", tokens, index, rows)
-        hp = hr = np_ = pp = None
-        most = 0
+        hp = hr = np_ = pp = most = 0
         if history is not None:
             hp, hr, hn, most = self._matrix("history", history, self._u16, index)
             if hn != rows:
@@ -325,9 +327,9 @@ class LogitControls:
             n = self._bytes[rows] = _check(self._lib, self._lib.ane_control_logits_workspace(rows, vocab))
         ws = self._empty(n, dtype=self._u8, device=logits.device) if n else None
         rep, freq, pres, bias, mask, bias_row, mask_row = self._params
-        a = _lib.LogitsArgs(lp, yp, hp, np_, pp, rep, freq, pres, bias, mask, tp, lr, yr, hr or 0, bias_row, mask_row,
-                            rows, vocab, most, index, None if ws is None else ws.data_ptr(), n)
-        rc = self._lib.ane_control_logits(C.byref(a), self._stream(index))
+        a = _lib.pack_logits(lp, yp, hp, np_, pp, rep, freq, pres, bias, mask, tp, lr, yr, hr, bias_row, mask_row,
+                             rows, vocab, most, index, 0 if ws is None else ws.data_ptr(), n)
+        rc = self._control(a, self._stream(index))
         if rc:
             _check(self._lib, rc)
         return out, tokens

@@ -132,6 +132,16 @@ def test_calls_without_rows_do_nothing():
     refused(lib.ane_kv8_attend(cache(), batch(), None, None), "null")
 
 
+@pytest.mark.parametrize("cls,pack", [(_lib.Kv8AppendArgs, _lib.pack_append), (_lib.Kv8AttendArgs, _lib.pack_attend),
+                                      (_lib.LogitsArgs, _lib.pack_logits)])
+def test_packed_arguments_are_the_structs(cls, pack):
+    values = [7 * i + 1 for i in range(len(cls._fields_))]
+    data = pack(*values)
+    assert len(data) == C.sizeof(cls)
+    a = cls.from_buffer_copy(data)
+    assert [getattr(a, n) for n, _ in cls._fields_] == values
+
+
 class Host:
     """A batch whose arrays are host memory, for the index walk."""
 
