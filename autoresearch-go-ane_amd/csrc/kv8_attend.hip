@@ -14,6 +14,15 @@
 // A block is one tile and one key/value head (and one part of the keys where
 // tiles are few); its waves take steps of 32 keys in turn and meet once
 // at the end, in LDS.  There is no barrier in the loop.
+//
+// What bounds it.  Single tokens over long contexts: the cache's bytes (40
+// sequences of up to 40,000 tokens, 2 heads of 128: 494 MB in 108 us, 4.6 TB/s,
+// where a large copy has 5.1).  Single tokens over short contexts: the chain
+// launch, offsets, page table, first loads, meeting (one sequence of 777 tokens
+// 6.5 us, 64 of 1100 10.1).  Prompts: the vector instructions around the
+// products, about 150 for 32 keys and 48 rows where the products are 24 MFMAs,
+// with the vector units 78 % busy (one of 8192 tokens, 12 heads of 64: 121 us,
+// 850 TFLOP/s).
 #include <algorithm>
 
 #include "decode.h"
@@ -24,8 +33,9 @@ namespace ane {
 
 namespace {
 
-// Units of 16 keys in a wave's step.  Two: with four, single tokens were slower
-// (64 of 1100 tokens 11.1 us, not 10.7) and larger tiles do not fit.
+// Units of 16 keys in a wave's step.  Two: with four, single tokens are slower
+// (64 of 1100 tokens 10.8 us, not 10.1) and larger tiles and head dimension 128
+// do not fit (64 of 1500 81 us, not 34).
 constexpr int NU = 2;
 constexpr int kStep = 16 * NU;
 
@@ -546,27 +556,27 @@ int plan(const char* op, const Kv8Batch& b, const ane_kv8_batch& given, int DH, 
   const int64_t blocks = (int64_t)p->tiles * b.NKV;
   const int cap = b.table_pages << b.pshift;
   const int len = given.max_len ? std::min(given.max_len, cap) : cap;
-  // Waves that share a tile's keys.  Single tokens over short contexts: 16 and
-  // no parts to join (one sequence of 777 tokens 6.9 us against 7.9 with four
-  // waves and parts, 64 of 1100 10.7 against 14.4; but one of 2000 9.1 against
-  // 8.0, and 64 of up to 5000 29 against 22).  Short prompts: each wave a tile
-  // of its own, nothing to meet over (64 prompts of 256 24 us against 40; but
-  // 8 of 512 equal, and one of 8192 160 against 125).
-  if (p->nt == 1) p->kw = DH == 64 && (len <= 1152 || (blocks >= 128 && len <= 2048)) ? 16 : 4;
-  else p->kw = len <= 512 ? 1 : 4;
+  // Waves that share a tile's keys: four, and for short prompts each wave a
+  // tile of its own with nothing to meet over (64 prompts of 256 24 us against
+  // 40; but 8 of 512 equal, and one of 8192 160 against 125).
+  p->kw = p->nt > 1 && len <= 512 ? 1 : 4;
   p->round = p->kw * kStep;
-  // Parts of the keys, where there are fewer blocks than the GPU holds: four a
-  // CU for single tokens (40 long contexts, 80 blocks: 1024 blocks 106 us, 512
-  // 118; 64 sequences of 8 heads, 512 blocks: whole 33 us, in halves 38) and
-  // two else (chunks on contexts of up to 6000, 940 blocks: whole 63 us, halves
-  // 83).  Parts of ragged
-  // single tokens end at 4096 keys, so that one long context does not outlast
-  // the rest.
+  // Parts of the keys, where there are fewer blocks than the GPU holds: 512
+  // blocks in all (chunks on contexts of up to 6000, 940 blocks: whole 63 us,
+  // halves 83).  Single tokens have a join to pay for, 3 us: contexts stay whole
+  // up to 1024 keys, 768 of head dimension 128 (4 blocks of 512 keys 5.3 us,
+  // in parts 7.3; of 1024 6.6 and 7.3; of 2048 9.7 and 7.6), and up to 4096
+  // where there are 128 blocks (64 sequences of 4 heads and 2048 keys 13.8 and
+  // 18.3).  Their parts are 256 keys at least (4 blocks of 4096: 16 parts 8.0
+  // us, 32 8.6) and, ragged as they are, 2048 at most, so that one long
+  // context does not outlast the rest (64 of 8 heads and up to 30,000 keys 206
+  // us, whole 232; 80 blocks of up to 40,000 108 us, of 4096 keys 113).
   int64_t ns = 1;
-  if (p->kw == 4) {
-    const int64_t want = p->nt == 1 ? 1024 : 512;
-    if (blocks < 512) ns = (want + blocks - 1) / blocks;
-    if (p->nt == 1) ns = std::max<int64_t>(ns, (len + 4095) / 4096);
+  if (p->nt == 1) {
+    if (len > (blocks >= 128 ? 4096 : DH == 64 ? 1024 : 768))
+      ns = std::max<int64_t>(std::min<int64_t>((511 + blocks) / blocks, (len + 255) / 256), (len + 2047) / 2048);
+  } else if (p->kw == 4 && blocks < 512) {
+    ns = (511 + blocks) / blocks;
   }
   ns = std::min<int64_t>(ns, (len + p->round - 1) / p->round);
   ns = std::max<int64_t>(1, std::min<int64_t>(ns, kMaxSplit));
@@ -590,8 +600,7 @@ void launch_form(const AttendArgs& a, hipStream_t st) {
 
 template <int DH>
 void launch(const AttendArgs& a, const Plan& p, hipStream_t st) {
-  if (DH == 64 && p.nt == 1 && p.kw == 16) launch_form<64, 1, 16, 1>(a, st);
-  else if (p.nt == 1) launch_form<DH, 1, 4, 1>(a, st);
+  if (p.nt == 1) launch_form<DH, 1, 4, 1>(a, st);
   else if (p.nt == 2 && p.kw == 4) launch_form<DH, 2, 4, 1>(a, st);
   else if (p.nt == 2) launch_form<DH, 2, 1, 4>(a, st);
   else if constexpr (DH == 64) {
