@@ -111,15 +111,9 @@ struct DecAttnArgs {
 hipError_t dec_attention(const DecAttnArgs& a, hipStream_t s);
 
 // ---- steps over the paged 8-bit cache, and controlled logits --------------------
-// qkv [nb][N1] fp16 = the QKV GEMM's partials summed in split order (times
-// rr[row], where given); start[b] = ctr[0] and offsets[b] = b for the append
-// and attention that follow.  With *err set (a failed chain wait: the partials
-// are not to be used) the offsets say that no sequence has a new token, so
-// that nothing of them reaches the cache.
-hipError_t dec_qkv_rows(const float* part, int ks, const float* rr, half_t* qkv, int N1, int nb, const int* ctr,
-                        const int* err, int* start, int* offsets, hipStream_t s);
-// start[i] = 0, offsets[i] = i * plen for i <= nseq (prefill of nseq prompts)
-hipError_t dec_prompt_plan(int* start, int* offsets, int nseq, int plen, hipStream_t s);
+// start[i] = ctr[0] (no ctr: 0) and offsets[i] = i * each for i <= nseq: a step
+// (each = 1) or the prefill of nseq prompts
+hipError_t dec_batch_plan(int* start, int* offsets, const int* ctr, int nseq, int each, hipStream_t s);
 // p[i] = i for i < n
 hipError_t dec_count_up(int* p, int n, hipStream_t s);
 // The history that penalties count, uint16 [..][ld]: the prompts (and the

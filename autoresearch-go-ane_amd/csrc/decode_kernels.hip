@@ -752,36 +752,10 @@ __global__ __launch_bounds__(256) void gather_last_kernel(float* dst, const floa
   for (int c = threadIdx.x; c < D; c += 256) dst[(size_t)i * D + c] = s[c];
 }
 
-// A block per row; a thread two neighbouring columns at a time.
-__global__ __launch_bounds__(256) void qkv_rows_kernel(const float* part, int ks, const float* rr, half_t* qkv, int N1,
-                                                       int nb, const int* ctr, const int* err, int* start,
-                                                       int* offsets) {
-  const int t = blockIdx.x;
-  const bool ok = !err || *err == 0;
-  if (threadIdx.x == 0) {
-    start[t] = ctr[0];
-    offsets[t] = ok ? t : 0;
-    if (t == nb - 1) offsets[nb] = ok ? nb : 0;
-  }
-  const float r = rr ? rr[t] : 1.f;
-  for (int c = threadIdx.x * 2; c < N1; c += 512) {
-    float x = 0.f, y = 0.f;
-    for (int s = 0; s < ks; s++) {
-      const float2 p = *reinterpret_cast<const float2*>(part + ((size_t)s * kDecRows + t) * N1 + c);
-      x += p.x;
-      y += p.y;
-    }
-    half2v h;
-    h[0] = (half_t)(x * r);
-    h[1] = (half_t)(y * r);
-    *reinterpret_cast<half2v*>(qkv + (size_t)t * N1 + c) = h;
-  }
-}
-
-__global__ __launch_bounds__(64) void prompt_plan_kernel(int* start, int* offsets, int nseq, int plen) {
+__global__ __launch_bounds__(64) void batch_plan_kernel(int* start, int* offsets, const int* ctr, int nseq, int each) {
   const int i = blockIdx.x * 64 + threadIdx.x;
-  if (i < nseq) start[i] = 0;
-  if (i <= nseq) offsets[i] = i * plen;
+  if (i < nseq) start[i] = ctr ? ctr[0] : 0;
+  if (i <= nseq) offsets[i] = i * each;
 }
 
 __global__ __launch_bounds__(256) void count_up_kernel(int* p, int n) {
@@ -818,15 +792,8 @@ __global__ __launch_bounds__(64) void take_tokens_kernel(uint16_t* tok_out, uint
 
 }  // namespace
 
-hipError_t dec_qkv_rows(const float* part, int ks, const float* rr, half_t* qkv, int N1, int nb, const int* ctr,
-                        const int* err, int* start, int* offsets, hipStream_t s) {
-  if (nb < 1 || nb > kDecRows || ks < 1 || N1 % 2) return hipErrorInvalidValue;
-  hipLaunchKernelGGL(qkv_rows_kernel, dim3(nb), dim3(256), 0, s, part, ks, rr, qkv, N1, nb, ctr, err, start, offsets);
-  return hipGetLastError();
-}
-
-hipError_t dec_prompt_plan(int* start, int* offsets, int nseq, int plen, hipStream_t s) {
-  hipLaunchKernelGGL(prompt_plan_kernel, dim3(nseq / 64 + 1), dim3(64), 0, s, start, offsets, nseq, plen);
+hipError_t dec_batch_plan(int* start, int* offsets, const int* ctr, int nseq, int each, hipStream_t s) {
+  hipLaunchKernelGGL(batch_plan_kernel, dim3(nseq / 64 + 1), dim3(64), 0, s, start, offsets, ctr, nseq, each);
   return hipGetLastError();
 }
 

@@ -393,8 +393,10 @@ int room8(ane_decoder* d, const char* op, const ane_kv8_batch& b) {
   return ANE_OK;
 }
 
-// q | k | v rows (N1 apart) of the batch: rotate, append, attend; q in place.
-int attention8(ane_decoder* d, const char* op, int l, const ane_kv8_batch& b, half_t* qkv, half_t* out, bool frag) {
+// q | k | v rows (N1 apart; or, for a step, the product's sums): rotate,
+// append, attend; the rotated q to qkv.
+int attention8(ane_decoder* d, const char* op, int l, const ane_kv8_batch& b, half_t* qkv, const Kv8Sums* from,
+               half_t* out, bool frag) {
   const int D = d->D, N1 = d->N1;
   const ane_kv8_cache c = cache8(d, l);
   ane_kv8_append_args a{};
@@ -405,7 +407,7 @@ int attention8(ane_decoder* d, const char* op, int l, const ane_kv8_batch& b, ha
   a.q_row = a.k_row = a.v_row = a.q_out_row = N1;
   a.q_head = a.k_head = a.v_head = a.q_out_head = 64;
   a.heads = d->NH; a.positions = d->rope_rows;
-  SCHK(op, ane_kv8_append(&c, &b, &a, d->stream));
+  SCHK(op, kv8_append(&c, &b, &a, from, d->stream));
   ane_kv8_attend_args t{};
   t.q = (const uint16_t*)qkv; t.out = (uint16_t*)out;
   t.q_row = N1; t.q_head = 64; t.out_row = D; t.out_head = 64;
@@ -416,8 +418,8 @@ int attention8(ane_decoder* d, const char* op, int l, const ane_kv8_batch& b, ha
 
 // The same for a step, from the QKV GEMM's partials.
 int step_attention8(ane_decoder* d, const char* op, int l, int ks, const float* rr, const int* err, half_t* att) {
-  DCHK(op, dec_qkv_rows(d->kpart, ks, rr, d->qkv8, d->N1, d->nseq, d->ctr_d, err, d->start8, d->off8, d->stream));
-  return attention8(d, op, l, batch8(d, 0, d->nseq, d->nseq, d->C, 1), d->qkv8, att, true);
+  const Kv8Sums from{d->kpart, ks, d->N1, rr, err};
+  return attention8(d, op, l, batch8(d, 0, d->nseq, d->nseq, d->C, 1), d->qkv8, &from, att, true);
 }
 
 // The next tokens of the current logits: the argmax, or the controls' choice
@@ -434,7 +436,9 @@ int choose(ane_decoder* d, const char* op, uint16_t* hist) {
   DCHK(op, dec_take_tokens(d->tok_d, hist, d->ctr_d + 1, d->ctl_tok, d->nseq, st));
   return ANE_OK;
 }
-int feed_history(ane_decoder* d, const char* op) {
+// what a step's options have to do first
+int before_step(ane_decoder* d, const char* op) {
+  if (d->page8) DCHK(op, dec_batch_plan(d->start8, d->off8, d->ctr_d, d->nseq, 1, d->stream));
   if (d->controls)
     DCHK(op, dec_history_feed(d->ctl_hist, d->C, d->tok_d, d->ctr_d, d->ctl_len, d->nseq, d->stream));
   return ANE_OK;
@@ -445,7 +449,7 @@ int enqueue_step(ane_decoder* d, float* logits, uint16_t* hist) {
   const char* op = "step";
   const int D = d->D, H = d->H, N1 = d->N1, nb = d->nseq;
   const hipStream_t st = d->stream;
-  if (int rc = feed_history(d, op)) return rc;
+  if (int rc = before_step(d, op)) return rc;
   DCHK(op, dec_embed_norm(d->x, d->xn, d->P + d->off_embed, d->tok_d, d->P + d->off[0].g_att, nb, D, d->V, st));
   for (int l = 0; l < d->L; l++) {
     const DecLayerOff& o = d->off[l];
@@ -492,7 +496,7 @@ int enqueue_step_tail(ane_decoder* d, float* logits, uint16_t* hist) {
   const char* op = "step";
   const int D = d->D, H = d->H, N1 = d->N1, nb = d->nseq, L = d->L;
   const hipStream_t st = d->stream;
-  if (int rc = feed_history(d, op)) return rc;
+  if (int rc = before_step(d, op)) return rc;
   DCHK(op, dec_row_xg(d->x, d->xg_att, d->rr_d, d->P + d->off_embed, d->tok_d, d->P + d->off[0].g_att, nb, D, d->V,
                       st));
   DCHK(op, skinny_partials(d->xg_att, d->fwqkv, d->kpart, d->kpart_cap, N1, D, st));
@@ -705,7 +709,7 @@ extern "C" int ane_decode_prefill(ane_decoder* d, const uint16_t* prefix, int32_
     const int most = std::min(per, nseq);
     for (int n : {most, nseq % most ? nseq % most : most})
       if (int rc = room8(d, op, batch8(d, 0, n, n * plen, plen, plen))) return rc;
-    DCHK(op, dec_prompt_plan(d->start8, d->off8, most, plen, st));
+    DCHK(op, dec_batch_plan(d->start8, d->off8, nullptr, most, plen, st));
   }
   if (d->controls)
     DCHK(op, dec_history_prompt(d->ctl_hist, d->C, d->prefix_d, plen, d->ctl_len, d->ctl_prompt, nseq, st));
@@ -723,7 +727,7 @@ extern "C" int ane_decode_prefill(ane_decoder* d, const uint16_t* prefix, int32_
         DCHK(op, gemm(d, d->pxn, d->wqkv + (size_t)l * N1 * D, T, N1, D, EPI_STORE_H, p));
       }
       if (d->page8) {
-        if (int rc = attention8(d, op, l, batch8(d, s0, n, T, plen, plen), d->pqkv, d->patt, false)) return rc;
+        if (int rc = attention8(d, op, l, batch8(d, s0, n, T, plen, plen), d->pqkv, nullptr, d->patt, false)) return rc;
       } else {
         DCHK(op, prefill_kv_write(d->pqkv, kcl, vcl, d->rope_cos, d->rope_sin, s0, n, plen, d->NH, d->NKV, d->C, st));
         PrefillAttnArgs a;

@@ -158,6 +158,19 @@ __device__ __forceinline__ int kv8_exponent(uint32_t amax_bits) {
 // kernels' form; ANE_OK or ANE_ERR_ARG with the message set.
 int kv8_check(const char* op, const ane_kv8_cache* c, const ane_kv8_batch* b, Kv8Batch* out);
 
+// Rows q | k | v of the decoder's product as its fp32 sums [splits][kDecRows][n]
+// (added, times row_scale if there is one); a set *err: nothing is done.
+struct Kv8Sums {
+  const float* part = nullptr;
+  int splits = 0, n = 0;
+  const float* row_scale = nullptr;
+  const int* err = nullptr;
+};
+// ane_kv8_append; from: the rows come from there and not from q, k and v
+// (head dimension 64).
+int kv8_append(const ane_kv8_cache* cache, const ane_kv8_batch* batch, const ane_kv8_append_args* args,
+               const Kv8Sums* from, void* stream);
+
 // ane_kv8_attend; frag: out is the decoder's 64-row activation fragments
 // (decode.h), its strides unused.
 int kv8_attend(const ane_kv8_cache* cache, const ane_kv8_batch* batch, const ane_kv8_attend_args* args, bool frag,

@@ -10,6 +10,7 @@
 // of the same rows, kQHeads heads each.
 #include <algorithm>
 
+#include "decode.h"
 #include "kv8.h"
 #include "op_error.h"
 
@@ -28,6 +29,7 @@ struct AppendArgs {
   const float *cos, *sin;
   int64_t q_row, q_head, k_row, k_head, v_row, v_head, qo_row, qo_head;
   int heads;
+  Kv8Sums from;  // where the rows come from in the SUMS form, instead of xq, xk, xv
 };
 
 struct F8 {
@@ -39,6 +41,23 @@ __device__ __forceinline__ F8 wide8(half8 h) {
 #pragma unroll
   for (int j = 0; j < 8; j++) f.x[j] = (float)h[j];
   return f;
+}
+
+// dimensions d0 .. d0 + 7 of row r, columns from `col` on, of a product's sums
+// over its splits, rounded to fp16 as the rows are elsewhere
+__device__ __forceinline__ half8 sums8(const Kv8Sums& p, int r, int col) {
+  float4 lo = {0.f, 0.f, 0.f, 0.f}, hi = lo;
+  const float* x = p.part + (size_t)r * p.n + col;
+  for (int s = 0; s < p.splits; s++, x += (size_t)kDecRows * p.n) {
+    const float4 u = *reinterpret_cast<const float4*>(x), v = *reinterpret_cast<const float4*>(x + 4);
+    lo.x += u.x; lo.y += u.y; lo.z += u.z; lo.w += u.w;
+    hi.x += v.x; hi.y += v.y; hi.z += v.z; hi.w += v.w;
+  }
+  const float w = p.row_scale ? p.row_scale[r] : 1.f;
+  half8 h;
+  h[0] = (half_t)(lo.x * w); h[1] = (half_t)(lo.y * w); h[2] = (half_t)(lo.z * w); h[3] = (half_t)(lo.w * w);
+  h[4] = (half_t)(hi.x * w); h[5] = (half_t)(hi.y * w); h[6] = (half_t)(hi.z * w); h[7] = (half_t)(hi.w * w);
+  return h;
 }
 
 // the cosines and sines of the four pairs of dimensions from d0 on
@@ -99,8 +118,9 @@ __device__ __forceinline__ uint32_t again4(uint32_t c, float down) {
   return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(hi[0] * down, hi[1] * down, r, true);
 }
 
-// NC * TH chunks of 8 dimensions are a page's.
-template <int DH, int NC, int TH>
+// NC * TH chunks of 8 dimensions are a page's.  SUMS: the rows come from a
+// product's sums (kv8.h).
+template <int DH, int NC, int TH, bool SUMS>
 __global__ __launch_bounds__(TH) void append_kernel(AppendArgs a) {
   constexpr int CPR = DH / 8;  // chunks per row
   constexpr int T = DH / 16;
@@ -111,6 +131,7 @@ __global__ __launch_bounds__(TH) void append_kernel(AppendArgs a) {
   const int P = 1 << b.pshift;
   const Kv8Span span = kv8_page_span(b, blockIdx.x);
   if (span.n == 0) return;
+  if (SUMS && a.from.err && *a.from.err) return;
   const int nr = span.n, row0 = span.row, t0 = span.pos;
 
   if ((int)blockIdx.y >= b.NKV) {  // query heads
@@ -123,7 +144,8 @@ __global__ __launch_bounds__(TH) void append_kernel(AppendArgs a) {
       half8 in[kQHeads];
 #pragma unroll
       for (int k = 0; k < kQHeads; k++)
-        if (h0 + k < a.heads) in[k] = ld_h8(x + (h0 + k) * a.q_head);
+        if (h0 + k < a.heads)
+          in[k] = SUMS ? sums8(a.from, row0 + r, (h0 + k) * DH + d0) : ld_h8(x + (h0 + k) * a.q_head);
 #pragma unroll
       for (int k = 0; k < kQHeads; k++)
         if (h0 + k < a.heads) {
@@ -146,8 +168,8 @@ __global__ __launch_bounds__(TH) void append_kernel(AppendArgs a) {
 #pragma unroll
   for (int i = 0; i < NC; i++) {
     const int c = min(i * TH + tid, nr * CPR - 1), r = c / CPR, d0 = c % CPR * 8;
-    hk[i] = ld_h8(xk + r * a.k_row + d0);
-    hv[i] = ld_h8(xv + r * a.v_row + d0);
+    hk[i] = SUMS ? sums8(a.from, row0 + r, (a.heads + h) * DH + d0) : ld_h8(xk + r * a.k_row + d0);
+    hv[i] = SUMS ? sums8(a.from, row0 + r, (a.heads + b.NKV + h) * DH + d0) : ld_h8(xv + r * a.v_row + d0);
     w[i] = turn_of<DH>(a.cos, a.sin, t0 + r, d0);
   }
   if (id < 0) return;  // the same in the whole block
@@ -244,15 +266,15 @@ __global__ __launch_bounds__(TH) void append_kernel(AppendArgs a) {
   for (int c = u0 * DH + tid; c < (u1 + 1) * DH; c += TH) dst[c] = src[c];
 }
 
-template <int DH>
+template <int DH, bool SUMS>
 void launch(const AppendArgs& a, dim3 grid, hipStream_t st) {
   switch ((DH / 8) << a.b.pshift) {
-    case 128: hipLaunchKernelGGL((append_kernel<DH, 1, 128>), grid, dim3(128), 0, st, a); break;
-    case 256: hipLaunchKernelGGL((append_kernel<DH, 1, 256>), grid, dim3(256), 0, st, a); break;
-    case 512: hipLaunchKernelGGL((append_kernel<DH, 2, 256>), grid, dim3(256), 0, st, a); break;
-    case 1024: hipLaunchKernelGGL((append_kernel<DH, 4, 256>), grid, dim3(256), 0, st, a); break;
-    case 2048: hipLaunchKernelGGL((append_kernel<DH, 4, 512>), grid, dim3(512), 0, st, a); break;
-    default: hipLaunchKernelGGL((append_kernel<DH, 4, 1024>), grid, dim3(1024), 0, st, a); break;
+    case 128: hipLaunchKernelGGL((append_kernel<DH, 1, 128, SUMS>), grid, dim3(128), 0, st, a); break;
+    case 256: hipLaunchKernelGGL((append_kernel<DH, 1, 256, SUMS>), grid, dim3(256), 0, st, a); break;
+    case 512: hipLaunchKernelGGL((append_kernel<DH, 2, 256, SUMS>), grid, dim3(256), 0, st, a); break;
+    case 1024: hipLaunchKernelGGL((append_kernel<DH, 4, 256, SUMS>), grid, dim3(256), 0, st, a); break;
+    case 2048: hipLaunchKernelGGL((append_kernel<DH, 4, 512, SUMS>), grid, dim3(512), 0, st, a); break;
+    default: hipLaunchKernelGGL((append_kernel<DH, 4, 1024, SUMS>), grid, dim3(1024), 0, st, a); break;
   }
 }
 
@@ -296,14 +318,23 @@ using namespace ane;
 
 extern "C" int ane_kv8_append(const ane_kv8_cache* cache, const ane_kv8_batch* batch, const ane_kv8_append_args* args,
                               void* stream) {
+  return kv8_append(cache, batch, args, nullptr, stream);
+}
+
+int ane::kv8_append(const ane_kv8_cache* cache, const ane_kv8_batch* batch, const ane_kv8_append_args* args,
+                    const Kv8Sums* from, void* stream) {
   const char* op = "kv8 append";
   AppendArgs a;
   int rc = kv8_check(op, cache, batch, &a.b);
   if (rc) return rc;
   if (!args) return op_fail(ANE_ERR_ARG, "storiesane %s: null arguments", op);
   if (a.b.nseq == 0 || a.b.rows == 0) return ANE_OK;  // an empty tensor may have no address
-  if (!args->k || !args->v || !args->cos || !args->sin || args->heads < 0 ||
-      (args->heads > 0 && (!args->q || !args->q_out)))
+  if (from && (cache->head_dim != 64 || a.b.rows > kDecRows || from->splits < 1 || from->n % 8 ||
+               from->n < (args->heads + 2 * a.b.NKV) * 64))
+    return op_fail(ANE_ERR_ARG, "storiesane %s: head_dim=%d rows=%d splits=%d n=%d of sums", op, cache->head_dim,
+                   a.b.rows, from->splits, from->n);
+  if ((!from && (!args->k || !args->v)) || !args->cos || !args->sin || args->heads < 0 ||
+      (args->heads > 0 && ((!from && !args->q) || !args->q_out)))
     return op_fail(ANE_ERR_ARG, "storiesane %s: null buffer", op);
   const ane_kv8_append_args& g = *args;
   const int64_t strides[] = {g.k_row, g.k_head, g.v_row, g.v_head, g.q_row, g.q_head, g.q_out_row, g.q_out_head};
@@ -332,8 +363,10 @@ extern "C" int ane_kv8_append(const ane_kv8_cache* cache, const ane_kv8_batch* b
   const int P = 1 << a.b.pshift;
   a.heads = g.heads;
   const dim3 grid(kv8_count(a.b.nseq, a.b.rows, kv8_pages(P)), a.b.NKV + (g.heads + kQHeads - 1) / kQHeads);
-  if (cache->head_dim == 64) launch<64>(a, grid, (hipStream_t)stream);
-  else launch<128>(a, grid, (hipStream_t)stream);
+  a.from = from ? *from : Kv8Sums{};
+  if (from) launch<64, true>(a, grid, (hipStream_t)stream);
+  else if (cache->head_dim == 64) launch<64, false>(a, grid, (hipStream_t)stream);
+  else launch<128, false>(a, grid, (hipStream_t)stream);
   const hipError_t h = hipGetLastError();
   if (h != hipSuccess) return op_fail(ANE_ERR_HIP, "storiesane %s: %s", op, hipGetErrorString(h));
   return ANE_OK;
