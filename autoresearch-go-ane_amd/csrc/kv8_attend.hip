@@ -544,39 +544,58 @@ int plan(const char* op, const Kv8Batch& b, const ane_kv8_batch& given, int DH, 
                    b.NKV);
   const int G = heads / b.NKV;
   if (b.nseq == 0 || b.rows == 0) return ANE_OK;
-  // Tiles of 16, 32 or 48 rows: the smallest that takes the longest sequence's
-  // rows (the mean one's where that is not known).  At head dimension 128 the
-  // registers end at 32 (48 spill: two prompts of 2000 tokens 109 us, not 49).
+  const int cap = b.table_pages << b.pshift;
+  const int len = given.max_len ? std::min(given.max_len, cap) : cap;
+  // Tiles of 16 or 32 rows: the smallest that takes the longest sequence's rows
+  // (the mean one's where that is not known), and at least a token's.  48 rows
+  // use what a step converts a third better, in fewer and longer blocks: for
+  // one sequence of 4096 keys or more (a prompt of 8192 tokens 123 us, in
+  // tiles of 32 136; but one of 3000 29.5 and 27.9), and where they are 1536
+  // blocks all the same (8 chunks of 2000 on 4,000 to 8,000 219 and 236; but
+  // 20 of 50 to 150 on up to 9000 66 and 60, 32 of 10 to 128 on up to 4000 43
+  // and 37); not where they would stay a fifth emptier, and not at head
+  // dimension 128, whose registers end at 32 (two prompts of 2000 tokens 109
+  // us, not 49).
   const int64_t most = (int64_t)G * (given.max_new ? std::min(given.max_new, b.rows) : (b.rows + b.nseq - 1) / b.nseq);
-  p->nt = most <= 16 ? 1 : most <= 32 || DH == 128 ? 2 : 3;
-  if (p->nt == 3 && 32 / G * 48 > 48 / G * 38) p->nt = 2;  // where 48 rows would stay a fifth emptier than 32
-  while (16 * p->nt < G) p->nt *= 2;
+  p->nt = most <= 16 && G <= 16 ? 1 : 2;
+  if (DH == 64 && most > 32 && 32 / G * 48 <= 48 / G * 38 &&
+      ((b.nseq == 1 && len >= 4096) || (int64_t)kv8_count(b.nseq, b.rows, kv8_tiles(48 / G)) * b.NKV >= 1536))
+    p->nt = 3;
   p->tt = 16 * p->nt / G;
   p->tiles = kv8_count(b.nseq, b.rows, kv8_tiles(p->tt));
   const int64_t blocks = (int64_t)p->tiles * b.NKV;
-  const int cap = b.table_pages << b.pshift;
-  const int len = given.max_len ? std::min(given.max_len, cap) : cap;
-  // Waves that share a tile's keys: four, and for short prompts each wave a
-  // tile of its own with nothing to meet over (64 prompts of 256 24 us against
-  // 40; but 8 of 512 equal, and one of 8192 160 against 125).
-  p->kw = p->nt > 1 && len <= 512 ? 1 : 4;
+  // Waves that share a tile's keys: four, and in larger tiles each wave a tile
+  // of its own, with nothing to meet over, where that leaves the GPU full long
+  // enough to hide the longest (head dimension 64: 64 prompts of 256 23 us
+  // against 41, 16 of 1024 42 against 50; but 4 of 512 11.9 against 9.8, one of
+  // 2048 36 against 18; head dimension 128: 8 of 2048 206 against 248; but one
+  // of 2048 46 against 37).
+  const int wps = waves_per_simd(DH, p->nt);
+  p->kw = p->nt > 1 && 2 * blocks >= (int64_t)wps * len ? 1 : 4;
   p->round = p->kw * kStep;
-  // Parts of the keys, where there are fewer blocks than the GPU holds: 512
-  // blocks in all (chunks on contexts of up to 6000, 940 blocks: whole 63 us,
-  // halves 83).  Single tokens have a join to pay for, 3 us: contexts stay whole
-  // up to 1024 keys, 768 of head dimension 128 (4 blocks of 512 keys 5.3 us,
-  // in parts 7.3; of 1024 6.6 and 7.3; of 2048 9.7 and 7.6), and up to 4096
-  // where there are 128 blocks (64 sequences of 4 heads and 2048 keys 13.8 and
-  // 18.3).  Their parts are 256 keys at least (4 blocks of 4096: 16 parts 8.0
-  // us, 32 8.6) and, ragged as they are, 2048 at most, so that one long
-  // context does not outlast the rest (64 of 8 heads and up to 30,000 keys 206
-  // us, whole 232; 80 blocks of up to 40,000 108 us, of 4096 keys 113).
+  // Parts of the keys, where there are few blocks.  What parts cost is the
+  // join's launch, 3 us, and their sums in fp32: for tiles of 32 and 48 rows a
+  // block has to save more than it writes (1500 tokens of a prompt, 600 blocks:
+  // whole 13 us, halves 28).  So those are cut up to a block a CU, in parts of
+  // 512 keys at least (28 blocks of 2064 keys: whole 13.2 us, four parts 11.0;
+  // of 664: 8.2, two 10.1), and further, as many as the CUs hold at once, only
+  // into parts of 4096 (128 blocks of 16,500 keys: whole 87 us, halves 55,
+  // four 45; 250 of 17,000 90, 78, 77).
+  // Single tokens stay whole up to 1024 keys, 768 of head dimension 128 (4
+  // blocks of 512 keys 5.3 us, in parts 7.3; of 1024 6.6 and 7.3; of 2048 9.7
+  // and 7.6), and up to 4096 where there are 128 blocks (64 sequences of 4
+  // heads and 2048 keys 13.8 and 18.3).  Beyond, up to 512 blocks, in parts of
+  // 256 keys at least (4 blocks of 4096: 16 parts 8.0 us, 32 8.6) and, ragged
+  // as they are, 2048 at most, so that one long context does not outlast the
+  // rest (64 of 8 heads and up to 30,000 keys 206 us, whole 232; 80 blocks of
+  // up to 40,000 108 us, of 4096 keys 113).
   int64_t ns = 1;
   if (p->nt == 1) {
     if (len > (blocks >= 128 ? 4096 : DH == 64 ? 1024 : 768))
       ns = std::max<int64_t>(std::min<int64_t>((511 + blocks) / blocks, (len + 255) / 256), (len + 2047) / 2048);
-  } else if (p->kw == 4 && blocks < 512) {
-    ns = (511 + blocks) / blocks;
+  } else if (p->kw == 4) {
+    ns = std::max<int64_t>(std::min<int64_t>(256 / blocks, len / 512),
+                           std::min<int64_t>(256 * wps / blocks, len / 4096));
   }
   ns = std::min<int64_t>(ns, (len + p->round - 1) / p->round);
   ns = std::max<int64_t>(1, std::min<int64_t>(ns, kMaxSplit));
