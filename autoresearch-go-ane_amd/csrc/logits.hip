@@ -5,6 +5,12 @@
 // logits, mask words and biases are under way while it counts the row's
 // history over them in LDS (whole-number atomics: the order does not matter).
 // Where a row is several blocks', a second launch picks among their choices.
+//
+// What bounds it.  Many rows: bytes (400 rows of 60,011 with masks and up to
+// 8000 ids: 199 MB in 53 us, 3.7 TB/s; without histories 45: each block of a
+// row reads the row's history again.  A block per row, which reads it once,
+// took 64).  Few rows: the chain of length, history, counts, choice and the
+// second launch (one row of 32,000 7.1 us).
 #include <algorithm>
 
 #include "kv8.h"

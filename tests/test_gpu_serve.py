@@ -278,6 +278,30 @@ def test_attend_long_context_in_parts(nseq, new):
     run_attend(r, [(5000 - 37 * i, new) for i in range(nseq)], 6, 2, 64, 64, max_new=new, max_len=5009)
 
 
+LARGE = {
+    # one long sequence: its keys in parts, then whole
+    "chunk": ([(4100, 40)], 12, 4, dict(max_new=40, max_len=4140)),
+    "long-chunk": ([(4090, 530)], 12, 4, dict(max_new=530, max_len=4620)),
+    # many blocks: each wave a tile of its own
+    "many": ([(i % 7 * 9, 1 + i * 37 % 90) for i in range(60)], 16, 16, dict(max_new=90, max_len=144)),
+}
+
+
+@pytest.mark.parametrize("P", [16, 64])
+@pytest.mark.parametrize("case", LARGE)
+def test_attend_large_tiles(case, P):
+    """Tiles of 48 rows, with pages that are not there and NaN values."""
+    lens, heads, kvh, hints = LARGE[case]
+    r = np.random.default_rng(P)
+    table, start, offsets, pages = layout(r, lens, P)
+    pool = Pool(r, pages, kvh, P, 64)
+    last = lens[-1][0] + lens[-1][1] - 5
+    for p in (3, last):
+        pool.vb[table[-1, p // P], 0, p % P // 16, p % 16 // 4, 37 % 16, 37 // 16, p % 4] = 0x7f
+    pool.load()
+    run_attend(np.random.default_rng(P), lens, heads, kvh, 64, P, pool=pool, holes=[(0, 0), (len(lens) - 1, 2)], **hints)
+
+
 @pytest.mark.parametrize("dh,heads", [(64, 4), (128, 8)])
 def test_attend_missing_pages(dh, heads):
     """Keys of pages that are not there take no part; a row with none gives
