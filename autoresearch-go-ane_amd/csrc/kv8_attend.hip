@@ -581,8 +581,8 @@ int plan(const char* op, const Kv8Batch& b, const ane_kv8_batch& given, int DH, 
   // of 664: 8.2, two 10.1), and further, as many as the CUs hold at once, only
   // into parts of 4096 (128 blocks of 16,500 keys: whole 87 us, halves 55,
   // four 45; 250 of 17,000 90, 78, 77).
-  // Single tokens stay whole up to 1024 keys, 768 of head dimension 128 (4
-  // blocks of 512 keys 5.3 us, in parts 7.3; of 1024 6.6 and 7.3; of 2048 9.7
+  // Single tokens stay whole up to 1280 keys, 768 of head dimension 128 (4
+  // blocks of 512 keys 5.3 us, in parts 7.3; of 1280 7.6 and 8.1; of 2048 9.7
   // and 7.6), and up to 4096 where there are 128 blocks (64 sequences of 4
   // heads and 2048 keys 13.8 and 18.3).  Beyond, up to 512 blocks, in parts of
   // 256 keys at least (4 blocks of 4096: 16 parts 8.0 us, 32 8.6) and, ragged
@@ -591,7 +591,7 @@ int plan(const char* op, const Kv8Batch& b, const ane_kv8_batch& given, int DH, 
   // up to 40,000 108 us, of 4096 keys 113).
   int64_t ns = 1;
   if (p->nt == 1) {
-    if (len > (blocks >= 128 ? 4096 : DH == 64 ? 1024 : 768))
+    if (len > (blocks >= 128 ? 4096 : DH == 64 ? 1280 : 768))
       ns = std::max<int64_t>(std::min<int64_t>((511 + blocks) / blocks, (len + 255) / 256), (len + 2047) / 2048);
   } else if (p->kw == 4) {
     ns = std::max<int64_t>(std::min<int64_t>(256 / blocks, len / 512),
