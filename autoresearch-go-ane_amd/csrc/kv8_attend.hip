@@ -146,11 +146,11 @@ __global__ __launch_bounds__(64 * KW * RW, waves_per_simd(DH, NT)) void attend_k
   // what Step says of the page.  wend: the first position behind them.
   const int* trow = b.table + (size_t)span.seq * b.table_stride;
   int wbase = 0, wexp = 0;
-  int64_t wend = 0;
+  int wend = 0;
   uint32_t wlo = 0, whi = 0;
   auto window = [&](int pg) {
     wbase = pg;
-    wend = (int64_t)(pg + 64) << b.pshift;
+    wend = (pg + 64) << b.pshift;  // a table covers at most 2^30 tokens
     const int p = pg + lane;
     int id = -1;
     if (p < b.table_pages && ((int64_t)p << b.pshift) < k1) {
@@ -230,12 +230,12 @@ __global__ __launch_bounds__(64 * KW * RW, waves_per_simd(DH, NT)) void attend_k
     for (int d = 0; d < ND; d++) o[d][t] = floatx4{0.f, 0.f, 0.f, 0.f};
   }
 
-  // whether a step holds keys that some row does not attend to
+  // not 0: the step holds keys that some row does not attend to
   auto at_edge = [&](const Step<DH>& s, int kb) {
     int all = s.ex[0];
 #pragma unroll
     for (int u = 1; u < (ONE ? 1 : NU); u++) all &= s.ex[u];
-    return kb + kStep - 1 > span.pos || !(all & kThere);
+    return max(kb + kStep - 1 - span.pos, 0) | (~all & kThere);
   };
 
   half8 ones;
@@ -244,7 +244,7 @@ __global__ __launch_bounds__(64 * KW * RW, waves_per_simd(DH, NT)) void attend_k
   asm volatile("" : "+v"(ones));  // in vector registers: scalar ones are spilled and read back in every step
   uint32_t nan = 0;
   auto step = [&](Step<DH>& s, int kb) {
-    const bool edge = at_edge(s, kb);
+    const int edge = at_edge(s, kb);
     floatx4 sc[NU][NT];
 #pragma unroll
     for (int u = 0; u < NU; u++) {
