@@ -414,7 +414,7 @@ CONTROL = [dict(), dict(rep=True), dict(freq=True, prompts=False), dict(rep=True
 
 @pytest.mark.parametrize("kw", CONTROL, ids=lambda k: "-".join(k) or "plain")
 @pytest.mark.parametrize("rows,vocab,hist", [(1, 1, 1), (3, 33, 5), (2, 4096, 700), (5, 4097, 0), (4, 32000, 1100),
-                                             (3, 65535, 9000)])
+                                             (3, 65535, 9000), (131, 9001, 250), (128, 8192, 40)])
 def test_control(rows, vocab, hist, kw):
     r = np.random.default_rng(rows * vocab + hist)
     lg = (r.standard_normal((rows, vocab)) * 3).astype(np.float32)
