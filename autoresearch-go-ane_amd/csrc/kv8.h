@@ -129,6 +129,47 @@ __host__ __device__ __forceinline__ Kv8Span kv8_tile_span(const Kv8Batch& b, int
   if (k < 0) return {f.i, 0, 0, 0};
   return kv8_cut(f.s, f.i, f.s.st + k * w, f.s.st + (k + 1) * w);
 }
+// The same tiles with the longest contexts first, for at most 64 sequences:
+// those of the sequence that ends last, its own last tile first, and so on.
+// A lane holds a sequence and adds up the tiles of those before it.
+__host__ __device__ __forceinline__ Kv8Span kv8_tile_longest(const Kv8Batch& b, int w, uint32_t item) {
+#ifdef __HIP_DEVICE_COMPILE__
+  const int lane = threadIdx.x & 63;
+  Kv8Seq s = kv8_seq(b, min(lane, b.nseq - 1));
+  if (lane >= b.nseq) s.n = 0;
+  const int end = s.st + s.n;
+  const uint32_t tiles = ((uint32_t)s.n + w - 1) / w;
+  uint32_t first = 0;
+#pragma unroll 4
+  for (int j = 0; j < b.nseq; j++) {
+    const int e = __builtin_amdgcn_readlane(end, j);
+    first += e > end || (e == end && j < lane) ? (uint32_t)__builtin_amdgcn_readlane((int)tiles, j) : 0;
+  }
+  const uint64_t mine = __ballot(first <= item && item - first < tiles);
+  if (mine == 0) return {0, 0, 0, 0};
+  const int i = __ffsll((unsigned long long)mine) - 1;
+  s = {__builtin_amdgcn_readlane(s.row0, i), __builtin_amdgcn_readlane(s.n, i), __builtin_amdgcn_readlane(s.st, i)};
+  const uint32_t last = (uint32_t)__builtin_amdgcn_readlane((int)(first + tiles), i) - 1;
+#else
+  int i = 0;
+  Kv8Seq s;
+  uint32_t last = 0;
+  for (;; i++) {
+    if (i == b.nseq) return {0, 0, 0, 0};
+    s = kv8_seq(b, i);
+    const uint32_t tiles = ((uint32_t)s.n + w - 1) / w;
+    uint32_t first = 0;
+    for (int j = 0; j < b.nseq; j++) {
+      const Kv8Seq o = kv8_seq(b, j);
+      if (o.st + o.n > s.st + s.n || (o.st + o.n == s.st + s.n && j < i)) first += ((uint32_t)o.n + w - 1) / w;
+    }
+    last = first + tiles - 1;
+    if (first <= item && item - first < tiles) break;
+  }
+#endif
+  const int64_t k = last - item;
+  return kv8_cut(s, i, s.st + k * w, s.st + (k + 1) * w);
+}
 // the rows of the item-th page that gets any (page pos >> pshift of the table)
 __host__ __device__ __forceinline__ Kv8Span kv8_page_span(const Kv8Batch& b, uint32_t item) {
   const Kv8Found f = kv8_find(b, kv8_pages(1 << b.pshift), item);

@@ -387,15 +387,20 @@ extern "C" int ane_debug_kv8_item(const ane_kv8_cache* cache, const ane_kv8_batc
   if (rc) return rc;
   if (!out || tile_tokens < 1 || tile_tokens > 64 || b.nseq < 1)
     return op_fail(ANE_ERR_ARG, "storiesane %s: tile_tokens=%d nseq=%d", op, tile_tokens, b.nseq);
-  const uint32_t n = kv8_count(b.nseq, b.rows, pages ? kv8_pages(1 << b.pshift) : kv8_tiles(tile_tokens));
+  if (pages == 2 && b.nseq > 64)
+    return op_fail(ANE_ERR_ARG, "storiesane %s: nseq=%d want at most 64", op, b.nseq);
+  const bool tiles = pages != 1;
+  const uint32_t n = kv8_count(b.nseq, b.rows, !tiles ? kv8_pages(1 << b.pshift) : kv8_tiles(tile_tokens));
   if (item < 0 || item >= (int64_t)n)
     return op_fail(ANE_ERR_ARG, "storiesane %s: item=%lld want below %u", op, (long long)item, n);
-  const Kv8Span s = pages ? kv8_page_span(b, (uint32_t)item) : kv8_tile_span(b, tile_tokens, (uint32_t)item);
+  const Kv8Span s = !tiles ? kv8_page_span(b, (uint32_t)item)
+                    : pages ? kv8_tile_longest(b, tile_tokens, (uint32_t)item)
+                            : kv8_tile_span(b, tile_tokens, (uint32_t)item);
   out[0] = s.seq;
   out[1] = s.row;
   out[2] = s.n;
   out[3] = s.pos;
-  out[4] = pages && s.n > 0 ? kv8_page(b, s.seq, s.pos >> b.pshift) : -1;
+  out[4] = !tiles && s.n > 0 ? kv8_page(b, s.seq, s.pos >> b.pshift) : -1;
   out[5] = (int)n;
   return ANE_OK;
 }

@@ -50,6 +50,7 @@ struct AttendArgs {
   int G;        // query heads per key/value head
   int tt;       // tokens per tile: tt * G <= rows of the tile
   int tiles;    // items
+  int longest;  // tiles are numbered with the longest contexts first
   int nsplit;   // parts that the keys of a tile are cut into, at most
   int round;    // keys that a block takes at a time: parts are multiples of it
   float c;      // scale * log2(e)
@@ -61,6 +62,11 @@ struct AttendArgs {
 template <int DH>
 __device__ __forceinline__ half_t* out_at(const AttendArgs& a, int row, int head, int d) {
   return a.out + (a.frag ? (int64_t)act_frag_off(row, head * DH + d) : row * a.out_row + head * a.out_head + d);
+}
+
+// the rows of a tile; the grid counts tiles down
+__device__ __forceinline__ Kv8Span tile_span(const AttendArgs& a, int tile) {
+  return a.longest ? kv8_tile_longest(a.b, a.tt, a.tiles - 1 - tile) : kv8_tile_span(a.b, a.tt, tile);
 }
 
 // The keys of a tile are cut into equal parts of whole rounds, at most nsplit.
@@ -133,7 +139,7 @@ __global__ __launch_bounds__(64 * KW * RW, waves_per_simd(DH, NT)) void attend_k
   // the longest rows of a prompt first
   const int tile = a.tiles - 1 - rest / a.nsplit * RW - (RW > 1 ? __builtin_amdgcn_readfirstlane(tid >> 6) : 0);
   if (RW > 1 && tile < 0) return;
-  const Kv8Span span = kv8_tile_span(b, a.tt, tile);
+  const Kv8Span span = NT > 1 && KW > 1 ? tile_span(a, tile) : kv8_tile_span(b, a.tt, tile);
   if (span.n == 0) return;
   const int rows = span.n * a.G;
   const int kend = span.pos + span.n;  // keys of the tile's last token
@@ -491,7 +497,7 @@ __global__ __launch_bounds__(256) void join_kernel(AttendArgs a) {
   const Kv8Batch& b = a.b;
   const int lane = threadIdx.x & 63;
   const int h = blockIdx.x % b.NKV, tile = blockIdx.x / b.NKV;
-  const Kv8Span span = kv8_tile_span(b, a.tt, tile);
+  const Kv8Span span = tile_span(a, tile);
   const int r = blockIdx.y * 4 + (threadIdx.x >> 6);
   if (r >= span.n * a.G) return;
   const int kend = span.pos + span.n;
@@ -533,7 +539,7 @@ __global__ __launch_bounds__(256) void join_kernel(AttendArgs a) {
 }
 
 struct Plan {
-  int nt = 0, tt = 0, nsplit = 0, kw = 4, round = 0;
+  int nt = 0, tt = 0, nsplit = 0, kw = 4, round = 0, longest = 0;
   uint32_t tiles = 0;
   int64_t bytes = 0;
 };
@@ -573,6 +579,13 @@ int plan(const char* op, const Kv8Batch& b, const ane_kv8_batch& given, int DH, 
   const int wps = waves_per_simd(DH, p->nt);
   p->kw = p->nt > 1 && 2 * blocks >= (int64_t)wps * len ? 1 : 4;
   p->round = p->kw * kStep;
+  // The longest contexts first, so that the last blocks to end are short ones:
+  // chunks of prompts at the lengths they come in (8 of 100 to 400 on up to
+  // 8000, three draws: 73, 101, 57 us against 100, 105, 60; 32 of 10 to 128 on
+  // up to 4000 33 against 38).  Finding them costs each block 1.5 us at 64
+  // sequences (64 of 16 to 100, head dimension 128: 145 against 129), so up to
+  // 32, and not where a CU has no second block.
+  p->longest = p->nt > 1 && p->kw == 4 && b.nseq > 1 && b.nseq <= 32 && blocks > 256;
   // Parts of the keys, where there are few blocks.  What parts cost is the
   // join's launch, 3 us, and their sums in fp32: for tiles of 32 and 48 rows a
   // block has to save more than it writes (1500 tokens of a prompt, 600 blocks:
@@ -685,6 +698,7 @@ int ane::kv8_attend(const ane_kv8_cache* cache, const ane_kv8_batch* batch, cons
   a.q = (const half_t*)g.q; a.out = (half_t*)g.out;
   a.q_row = g.q_row; a.q_head = g.q_head; a.out_row = g.out_row; a.out_head = g.out_head;
   a.G = g.heads / a.b.NKV; a.tt = p.tt; a.tiles = (int)p.tiles; a.nsplit = p.nsplit; a.round = p.round;
+  a.longest = p.longest;
   a.c = g.scale * 1.44269504088896340736f;
   a.part = (float*)g.ws;
   a.ml = (float2*)(a.part + (size_t)p.tiles * a.b.NKV * p.nsplit * p.tt * a.G * cache->head_dim);

@@ -302,6 +302,17 @@ def test_attend_large_tiles(case, P):
     run_attend(np.random.default_rng(P), lens, heads, kvh, 64, P, pool=pool, holes=[(0, 0), (len(lens) - 1, 2)], **hints)
 
 
+@pytest.mark.parametrize("dh", [64, 128])
+@pytest.mark.parametrize("lens", [[(300, 40), (2, 90), (0, 0), (1500, 33), (700, 1), (300, 40)],
+                                  [(8200, 30), (100, 230)]])
+def test_attend_ragged_chunks(lens, dh):
+    """Enough blocks that the longest contexts are taken first: whole, and (at
+    head dimension 64 and 8230 keys) in parts."""
+    r = np.random.default_rng(dh + len(lens))
+    run_attend(r, lens, 32, 32, dh, 32, holes=[(1, 0)], max_new=max(n for _, n in lens),
+               max_len=max(s + n for s, n in lens))
+
+
 @pytest.mark.parametrize("dh,heads", [(64, 4), (128, 8)])
 def test_attend_missing_pages(dh, heads):
     """Keys of pages that are not there take no part; a row with none gives

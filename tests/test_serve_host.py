@@ -202,6 +202,39 @@ def test_every_row_is_in_one_item(nseq, page, tile):
         assert (seen[:offsets[-1]] == 1).all() and (seen[offsets[-1]:] == 0).all()
 
 
+@pytest.mark.parametrize("nseq", [1, 2, 9, 33, 64])
+@pytest.mark.parametrize("tile", [1, 5, 16])
+def test_longest_contexts_come_first(nseq, tile):
+    """The tiles of every sequence, those of the one that ends last first (of
+    two that end alike, the first), each one's own from its last on; empty
+    items behind them."""
+    r = np.random.default_rng(nseq * 100 + tile)
+    page, width = 32, 12
+    n = r.integers(0, 90, nseq)
+    n[r.random(nseq) < 0.2] = 0
+    n[0] = 7
+    start = r.integers(0, width * page - n + 1)
+    if nseq > 2:
+        start[2] = start[1] + n[1] - n[2] if start[1] + n[1] >= n[2] else start[2]
+    offsets = np.concatenate([[0], np.cumsum(n)])
+    table = r.permutation(nseq * width).reshape(nseq, width)
+    h = Host(table, start, offsets, int(offsets[-1]) + 3, page, nseq * width)
+    items = h.items(tile, 2)
+    h.within(items)
+    want = []
+    for i in sorted(range(nseq), key=lambda i: (-(start[i] + n[i]), i)):
+        for t in reversed(range(0, int(n[i]), tile)):
+            want.append((i, offsets[i] + t, min(tile, n[i] - t), start[i] + t))
+    assert [i[:4] for i in items[:len(want)]] == want
+    assert all(i[2] == 0 for i in items[len(want):])
+
+
+def test_longest_contexts_of_many_sequences_refused():
+    h = Host(np.zeros((65, 2), int), np.zeros(65, int), np.arange(66), 65, 16, 2)
+    out = (C.c_int32 * 6)()
+    refused(lib.ane_debug_kv8_item(h.c, h.b, 4, 2, 0, out), "nseq=65")
+
+
 @pytest.mark.parametrize("seed", range(40))
 def test_nonsense_stays_in_range(seed):
     r = np.random.default_rng(seed)
@@ -217,6 +250,8 @@ def test_nonsense_stays_in_range(seed):
     h = Host(some((nseq, 4), 12), some(nseq, 5 * page), some(nseq + 1, rows + 50), rows, page, 10)
     for tile in (1, 5, 64):
         h.within(h.items(tile, 0))
+        if nseq <= 64:
+            h.within(h.items(tile, 2))
     h.within(h.items(1, 1))
 
 
