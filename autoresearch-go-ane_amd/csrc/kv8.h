@@ -140,11 +140,12 @@ __host__ __device__ __forceinline__ Kv8Span kv8_tile_longest(const Kv8Batch& b, 
   const int end = s.st + s.n;
   const uint32_t tiles = ((uint32_t)s.n + w - 1) / w;
   uint32_t first = 0;
-#pragma unroll 4
-  for (int j = 0; j < b.nseq; j++) {
-    const int e = __builtin_amdgcn_readlane(end, j);
-    first += e > end || (e == end && j < lane) ? (uint32_t)__builtin_amdgcn_readlane((int)tiles, j) : 0;
-  }
+  for (int j0 = 0; j0 < b.nseq; j0 += 4)  // four at a time: lanes past the last have no tiles
+#pragma unroll
+    for (int j = j0; j < j0 + 4; j++) {
+      const int e = __builtin_amdgcn_readlane(end, j);
+      first += e > end || (e == end && j < lane) ? (uint32_t)__builtin_amdgcn_readlane((int)tiles, j) : 0;
+    }
   const uint64_t mine = __ballot(first <= item && item - first < tiles);
   if (mine == 0) return {0, 0, 0, 0};
   const int i = __ffsll((unsigned long long)mine) - 1;

@@ -582,8 +582,8 @@ int plan(const char* op, const Kv8Batch& b, const ane_kv8_batch& given, int DH, 
   // The longest contexts first, so that the last blocks to end are short ones:
   // chunks of prompts at the lengths they come in (8 of 100 to 400 on up to
   // 8000, three draws: 73, 101, 57 us against 100, 105, 60; 32 of 10 to 128 on
-  // up to 4000 33 against 38).  Finding them costs each block 1.5 us at 64
-  // sequences (64 of 16 to 100, head dimension 128: 145 against 129), so up to
+  // up to 4000 33 against 38).  Finding them costs each block 1.2 us at 64
+  // sequences (64 of 16 to 100, head dimension 128: 138 against 129), so up to
   // 32, and not where a CU has no second block.
   p->longest = p->nt > 1 && p->kw == 4 && b.nseq > 1 && b.nseq <= 32 && blocks > 256;
   // Parts of the keys, where there are few blocks.  What parts cost is the
