@@ -180,6 +180,15 @@ __host__ __device__ __forceinline__ Kv8Span kv8_page_span(const Kv8Batch& b, uin
   return kv8_cut(f.s, f.i, pg << b.pshift, (pg + 1) << b.pshift);
 }
 
+// The same with an item for every row: a page belongs to its first one, the
+// others are empty.  Fewer items where sequences have a token each.
+__host__ __device__ __forceinline__ Kv8Span kv8_row_page_span(const Kv8Batch& b, uint32_t item) {
+  const Kv8Found f = kv8_find(b, kv8_tiles(1), item);
+  const int64_t k = (int64_t)item - f.first, t = f.s.st + k, page = 1 << b.pshift;
+  if (k < 0 || (k > 0 && (t & (page - 1)))) return {f.i, 0, 0, 0};
+  return kv8_cut(f.s, f.i, t, (t | (page - 1)) + 1);
+}
+
 // e4m3 -> fp16 with the exponent applied, two codes of a dword at a time;
 // exact, since every code * 2^e is an fp16 number.
 typedef __fp16 fp16x2_t __attribute__((ext_vector_type(2)));

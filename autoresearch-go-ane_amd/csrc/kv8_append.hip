@@ -11,10 +11,10 @@
 //
 // What bounds it.  Prompts: bytes, each read and written once (24 ragged
 // prompts, 18,000 tokens, 12 / 4 heads of 64: 100 MB in 22.8 us, 4.4 TB/s).
-// Single tokens: a chain of loads, offsets, page id, rows, old exponent and
-// codes, each waiting for the one before (one token 4.8 us, 64 of them 5.7 in
-// a graph); the rows and their angles are asked for while the page id is under
-// way.
+// Single tokens, which a wave per page and head takes: a chain of loads,
+// offsets, page id, rows, old exponent and codes, each waiting for the one
+// before (one token 4.6 us, 64 of them 4.8 in a graph); the rows and their
+// angles are asked for while the page id is under way.
 #include <algorithm>
 
 #include "decode.h"
@@ -36,6 +36,7 @@ struct AppendArgs {
   const float *cos, *sin;
   int64_t q_row, q_head, k_row, k_head, v_row, v_head, qo_row, qo_head;
   int heads;
+  int by_row;    // append_few_kernel: items are rows, not pages
   Kv8Sums from;  // where the rows come from in the SUMS form, instead of xq, xk, xv
 };
 
@@ -125,9 +126,8 @@ __device__ __forceinline__ uint32_t again4(uint32_t c, float down) {
   return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(hi[0] * down, hi[1] * down, r, true);
 }
 
-// NC * TH chunks of 8 dimensions are a page's.  SUMS: the rows come from a
-// product's sums (kv8.h).
-template <int DH, int NC, int TH, bool SUMS>
+// NC * TH chunks of 8 dimensions are a page's.
+template <int DH, int NC, int TH>
 __global__ __launch_bounds__(TH) void append_kernel(AppendArgs a) {
   constexpr int CPR = DH / 8;  // chunks per row
   constexpr int T = DH / 16;
@@ -138,7 +138,6 @@ __global__ __launch_bounds__(TH) void append_kernel(AppendArgs a) {
   const int P = 1 << b.pshift;
   const Kv8Span span = kv8_page_span(b, blockIdx.x);
   if (span.n == 0) return;
-  if (SUMS && a.from.err && *a.from.err) return;
   const int nr = span.n, row0 = span.row, t0 = span.pos;
 
   if ((int)blockIdx.y >= b.NKV) {  // query heads
@@ -151,8 +150,7 @@ __global__ __launch_bounds__(TH) void append_kernel(AppendArgs a) {
       half8 in[kQHeads];
 #pragma unroll
       for (int k = 0; k < kQHeads; k++)
-        if (h0 + k < a.heads)
-          in[k] = SUMS ? sums8(a.from, row0 + r, (h0 + k) * DH + d0) : ld_h8(x + (h0 + k) * a.q_head);
+        if (h0 + k < a.heads) in[k] = ld_h8(x + (h0 + k) * a.q_head);
 #pragma unroll
       for (int k = 0; k < kQHeads; k++)
         if (h0 + k < a.heads) {
@@ -175,8 +173,8 @@ __global__ __launch_bounds__(TH) void append_kernel(AppendArgs a) {
 #pragma unroll
   for (int i = 0; i < NC; i++) {
     const int c = min(i * TH + tid, nr * CPR - 1), r = c / CPR, d0 = c % CPR * 8;
-    hk[i] = SUMS ? sums8(a.from, row0 + r, (a.heads + h) * DH + d0) : ld_h8(xk + r * a.k_row + d0);
-    hv[i] = SUMS ? sums8(a.from, row0 + r, (a.heads + b.NKV + h) * DH + d0) : ld_h8(xv + r * a.v_row + d0);
+    hk[i] = ld_h8(xk + r * a.k_row + d0);
+    hv[i] = ld_h8(xv + r * a.v_row + d0);
     w[i] = turn_of<DH>(a.cos, a.sin, t0 + r, d0);
   }
   if (id < 0) return;  // the same in the whole block
@@ -273,15 +271,142 @@ __global__ __launch_bounds__(TH) void append_kernel(AppendArgs a) {
   for (int c = u0 * DH + tid; c < (u1 + 1) * DH; c += TH) dst[c] = src[c];
 }
 
+// The same for few new rows: a wave per page and head, 64 / CPR rows (or query
+// heads) at a time, V a unit of 16 tokens at a time.  Rows past the first pass
+// are read again for their codes.  SUMS: the rows come from a product's sums.
 template <int DH, bool SUMS>
+__global__ __launch_bounds__(64) void append_few_kernel(AppendArgs a) {
+  constexpr int CPR = DH / 8, G = 64 / CPR, T = DH / 16;
+  __shared__ uint4 unit[DH];  // 16 tokens' V codes
+  const Kv8Batch& b = a.b;
+  const int lane = threadIdx.x, sub = lane / CPR, d0 = lane % CPR * 8;
+  const int P = 1 << b.pshift;
+  const Kv8Span span = a.by_row ? kv8_row_page_span(b, blockIdx.x) : kv8_page_span(b, blockIdx.x);
+  if (span.n == 0) return;
+  if (SUMS && a.from.err && *a.from.err) return;
+  const int nr = span.n, row0 = span.row, t0 = span.pos;
+
+  if ((int)blockIdx.y >= b.NKV) {  // query heads
+    const int h = (blockIdx.y - b.NKV) * G + sub;
+    if (h >= a.heads) return;
+    for (int r = 0; r < nr; r++) {
+      const Turn w = turn_of<DH>(a.cos, a.sin, t0 + r, d0);
+      const F8 f = rotate8(SUMS ? sums8(a.from, row0 + r, h * DH + d0)
+                                : ld_h8(a.xq + (row0 + r) * a.q_row + h * a.q_head + d0), w);
+      half8 o;
+#pragma unroll
+      for (int j = 0; j < 8; j++) o[j] = (half_t)f.x[j];
+      st_h8(a.q_out + (row0 + r) * a.qo_row + h * a.qo_head + d0, o);
+    }
+    return;
+  }
+
+  const int h = blockIdx.y;
+  const int id = kv8_page(b, span.seq, t0 >> b.pshift);
+  F8 fk, fv;
+  auto rows = [&](int r) {  // the lane's part of row r
+    r = min(r, nr - 1);     // rows past the last repeat it
+    const half8 k = SUMS ? sums8(a.from, row0 + r, (a.heads + h) * DH + d0)
+                         : ld_h8(a.xk + (row0 + r) * a.k_row + h * a.k_head + d0);
+    const half8 v = SUMS ? sums8(a.from, row0 + r, (a.heads + b.NKV + h) * DH + d0)
+                         : ld_h8(a.xv + (row0 + r) * a.v_row + h * a.v_head + d0);
+    fk = rotate8(k, turn_of<DH>(a.cos, a.sin, t0 + r, d0));
+    fv = wide8(v);
+    limit8(fk);
+    limit8(fv);
+  };
+  uint32_t mk = 0, mv = 0;
+  for (int g = 0; g < nr; g += G) {
+    rows(g + sub);
+    mk = amax8(fk, mk);
+    mv = amax8(fv, mv);
+  }
+  if (id < 0) return;
+  const size_t ph = (size_t)id * b.NKV + h;
+  uint8_t* kp = a.k + ph * P * DH;
+  uint8_t* vp = a.v + ph * P * DH;
+  const int r0 = t0 & (P - 1), r1 = r0 + nr;
+  int ok = kKvExpMin, ov = kKvExpMin;
+  if (r0 > 0) {
+    ok = a.k_exp[ph];
+    ov = a.v_exp[ph];
+  }
+  const int u0 = r0 >> 4, u1 = (r1 - 1) >> 4;
+  uint4 was[DH / 64];  // the first unit
+#pragma unroll
+  for (int i = 0; i < DH / 64; i++) was[i] = reinterpret_cast<const uint4*>(vp)[u0 * DH + i * 64 + lane];
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    mk = max(mk, (uint32_t)__shfl_xor((int)mk, o, 64));
+    mv = max(mv, (uint32_t)__shfl_xor((int)mv, o, 64));
+  }
+  const int ek = max(kv8_exponent(mk), ok), ev = max(kv8_exponent(mv), ov);
+  if (lane == 0) {
+    a.k_exp[ph] = (int8_t)ek;
+    a.v_exp[ph] = (int8_t)ev;
+  }
+  const float ik = kv8_scale(-ek), iv = kv8_scale(-ev);
+  const float tk = ek == kKvExpMax ? 240.f : 448.f, tv = ev == kKvExpMax ? 240.f : 448.f;
+
+  // rows from before, rounded again where the exponent rose
+  if (r0 > 0 && ek > ok) {
+    const float down = kv8_scale(ok - ek);
+    uint32_t* x = reinterpret_cast<uint32_t*>(kp);
+    for (int c = lane; c < r0 * DH / 4; c += 64) x[c] = again4(x[c], down);
+  }
+  const bool up = r0 > 0 && ev > ov;
+  const float down = kv8_scale(ov - ev);
+  if (up) {  // whole units of them
+    uint32_t* x = reinterpret_cast<uint32_t*>(vp);
+    for (int c = lane; c < u0 * 4 * DH; c += 64) x[c] = again4(x[c], down);
+  }
+  for (int u = u0; u <= u1; u++) {
+    const int s0 = max(r0, 16 * u), s1 = min(r1, 16 * u + 16);  // the new rows of this unit
+#pragma unroll
+    for (int i = 0; i < DH / 64; i++) {
+      const int c = i * 64 + lane;
+      uint4 x = was[i];
+      if (up && u == u0) {
+        const int n = clampi(r0 - (16 * u + 4 * c / DH * 4), 0, 4);  // of its four tokens, those from before
+        const uint32_t mine = n == 4 ? 0xffffffffu : (1u << (8 * n)) - 1;
+        x.x = (again4(x.x, down) & mine) | (x.x & ~mine);
+        x.y = (again4(x.y, down) & mine) | (x.y & ~mine);
+        x.z = (again4(x.z, down) & mine) | (x.z & ~mine);
+        x.w = (again4(x.w, down) & mine) | (x.w & ~mine);
+      }
+      unit[c] = x;
+      if (u < u1) was[i] = reinterpret_cast<const uint4*>(vp)[(u + 1) * DH + c];
+    }
+    __syncthreads();
+    for (int g = (s0 - r0) / G * G; g < s1 - r0; g += G) {
+      if (nr > G) rows(g + sub);
+      const int s = r0 + g + sub;
+      if (s < s0 || s >= s1) continue;
+      *reinterpret_cast<uint2*>(kp + s * DH + d0) = make_uint2(codes4(fk.x, ik, tk), codes4(fk.x + 4, ik, tk));
+      const uint32_t cv[2] = {codes4(fv.x, iv, tv), codes4(fv.x + 4, iv, tv)};
+      uint8_t* y = reinterpret_cast<uint8_t*>(unit) + (s & 15) / 4 * 4 * DH + (s & 3);
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const int d = d0 + j;
+        y[((d & 15) * T + (d >> 4)) * 4] = (uint8_t)(cv[j / 4] >> (8 * (j & 3)));
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < DH / 64; i++) reinterpret_cast<uint4*>(vp)[u * DH + i * 64 + lane] = unit[i * 64 + lane];
+    __syncthreads();
+  }
+}
+
+template <int DH>
 void launch(const AppendArgs& a, dim3 grid, hipStream_t st) {
   switch ((DH / 8) << a.b.pshift) {
-    case 128: hipLaunchKernelGGL((append_kernel<DH, 1, 128, SUMS>), grid, dim3(128), 0, st, a); break;
-    case 256: hipLaunchKernelGGL((append_kernel<DH, 1, 256, SUMS>), grid, dim3(256), 0, st, a); break;
-    case 512: hipLaunchKernelGGL((append_kernel<DH, 2, 256, SUMS>), grid, dim3(256), 0, st, a); break;
-    case 1024: hipLaunchKernelGGL((append_kernel<DH, 4, 256, SUMS>), grid, dim3(256), 0, st, a); break;
-    case 2048: hipLaunchKernelGGL((append_kernel<DH, 4, 512, SUMS>), grid, dim3(512), 0, st, a); break;
-    default: hipLaunchKernelGGL((append_kernel<DH, 4, 1024, SUMS>), grid, dim3(1024), 0, st, a); break;
+    case 128: hipLaunchKernelGGL((append_kernel<DH, 1, 128>), grid, dim3(128), 0, st, a); break;
+    case 256: hipLaunchKernelGGL((append_kernel<DH, 1, 256>), grid, dim3(256), 0, st, a); break;
+    case 512: hipLaunchKernelGGL((append_kernel<DH, 2, 256>), grid, dim3(256), 0, st, a); break;
+    case 1024: hipLaunchKernelGGL((append_kernel<DH, 4, 256>), grid, dim3(256), 0, st, a); break;
+    case 2048: hipLaunchKernelGGL((append_kernel<DH, 4, 512>), grid, dim3(512), 0, st, a); break;
+    default: hipLaunchKernelGGL((append_kernel<DH, 4, 1024>), grid, dim3(1024), 0, st, a); break;
   }
 }
 
@@ -369,11 +494,27 @@ int ane::kv8_append(const ane_kv8_cache* cache, const ane_kv8_batch* batch, cons
   a.v_head = g.v_head; a.qo_row = g.q_out_row; a.qo_head = g.q_out_head;
   const int P = 1 << a.b.pshift;
   a.heads = g.heads;
-  const dim3 grid(kv8_count(a.b.nseq, a.b.rows, kv8_pages(P)), a.b.NKV + (g.heads + kQHeads - 1) / kQHeads);
   a.from = from ? *from : Kv8Sums{};
-  if (from) launch<64, true>(a, grid, (hipStream_t)stream);
-  else if (cache->head_dim == 64) launch<64, false>(a, grid, (hipStream_t)stream);
-  else launch<128, false>(a, grid, (hipStream_t)stream);
+  const uint32_t pages = kv8_count(a.b.nseq, a.b.rows, kv8_pages(P));
+  const int each = batch->max_new ? std::min(batch->max_new, a.b.rows) : (a.b.rows + a.b.nseq - 1) / a.b.nseq;
+  const hipStream_t st = (hipStream_t)stream;
+  // A wave takes a page's new rows where they fit a pass of it (the longest
+  // sequence's, or where that is not known the mean one's): 64 single tokens
+  // 4.8 us against 5.9, 64 of 32 heads of 128 6.0 against 18, in pages of 256
+  // 5.1 against 23; 64 sequences of 8 rows at head dimension 64 5.6 against
+  // 6.1, but of 16 8.9 against 6.5, and of 8 at 128 9.4 against 7.7.
+  const int per = 512 / cache->head_dim;  // rows of a pass, or query heads of a block
+  if (from || each <= per) {
+    a.by_row = (uint32_t)a.b.rows < pages;
+    const dim3 grid(a.by_row ? a.b.rows : pages, a.b.NKV + (g.heads + per - 1) / per);
+    if (from) hipLaunchKernelGGL((append_few_kernel<64, true>), grid, dim3(64), 0, st, a);
+    else if (cache->head_dim == 64) hipLaunchKernelGGL((append_few_kernel<64, false>), grid, dim3(64), 0, st, a);
+    else hipLaunchKernelGGL((append_few_kernel<128, false>), grid, dim3(64), 0, st, a);
+  } else {
+    const dim3 grid(pages, a.b.NKV + (g.heads + kQHeads - 1) / kQHeads);
+    if (cache->head_dim == 64) launch<64>(a, grid, st);
+    else launch<128>(a, grid, st);
+  }
   const hipError_t h = hipGetLastError();
   if (h != hipSuccess) return op_fail(ANE_ERR_HIP, "storiesane %s: %s", op, hipGetErrorString(h));
   return ANE_OK;
@@ -389,13 +530,14 @@ extern "C" int ane_debug_kv8_item(const ane_kv8_cache* cache, const ane_kv8_batc
     return op_fail(ANE_ERR_ARG, "storiesane %s: tile_tokens=%d nseq=%d", op, tile_tokens, b.nseq);
   if (pages == 2 && b.nseq > 64)
     return op_fail(ANE_ERR_ARG, "storiesane %s: nseq=%d want at most 64", op, b.nseq);
-  const bool tiles = pages != 1;
-  const uint32_t n = kv8_count(b.nseq, b.rows, !tiles ? kv8_pages(1 << b.pshift) : kv8_tiles(tile_tokens));
+  const bool tiles = pages == 0 || pages == 2;
+  const uint32_t n = kv8_count(b.nseq, b.rows, tiles ? kv8_tiles(tile_tokens) : pages == 1 ? kv8_pages(1 << b.pshift) : kv8_tiles(1));
   if (item < 0 || item >= (int64_t)n)
     return op_fail(ANE_ERR_ARG, "storiesane %s: item=%lld want below %u", op, (long long)item, n);
-  const Kv8Span s = !tiles ? kv8_page_span(b, (uint32_t)item)
-                    : pages ? kv8_tile_longest(b, tile_tokens, (uint32_t)item)
-                            : kv8_tile_span(b, tile_tokens, (uint32_t)item);
+  const Kv8Span s = pages == 0   ? kv8_tile_span(b, tile_tokens, (uint32_t)item)
+                    : pages == 1 ? kv8_page_span(b, (uint32_t)item)
+                    : pages == 2 ? kv8_tile_longest(b, tile_tokens, (uint32_t)item)
+                                 : kv8_row_page_span(b, (uint32_t)item);
   out[0] = s.seq;
   out[1] = s.row;
   out[2] = s.n;

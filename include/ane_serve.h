@@ -165,11 +165,12 @@ int ane_control_logits(const ane_logits_args *args, void *stream);
 /* ---- for tests -----------------------------------------------------------------
  * The rows, positions and pages that a work item of the cache kernels takes,
  * by the kernels' own index arithmetic on host arrays: item `item` of tiles of
- * `tile_tokens` tokens (pages = 1: of the pages that rows go to; 2: of tiles
- * with the longest contexts first, at most 64 sequences).  out receives
- * {sequence, first row, rows taken, first position, page (-1: not there;
- * pages = 1 only), items of the batch}; rows taken = 0: the item is empty.
- * Returns ANE_OK.  No GPU is used. */
+ * `tile_tokens` tokens (pages = 0), of such tiles with the longest contexts
+ * first, at most 64 sequences (2), or of the pages that rows go to (1: as
+ * many items as pages may be, 3: an item a row).  out receives {sequence,
+ * first row, rows taken, first position, page (-1: not there; 1 and 3 only),
+ * items of the batch}; rows taken = 0: the item is empty.  Returns ANE_OK.
+ * No GPU is used. */
 int ane_debug_kv8_item(const ane_kv8_cache *cache, const ane_kv8_batch *batch, int32_t tile_tokens, int32_t pages,
                        int64_t item, int32_t *out);
 

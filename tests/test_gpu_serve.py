@@ -97,7 +97,7 @@ def check_append(before, after, exp, xk, table, start, offsets, P, cos, sin):
     assert off.mean() < 1e-3
 
 
-def run_append(r, lens, heads, kvh, dh, P, scale=1.0, packed=True, poke=None, pool=None, spread=0.7):
+def run_append(r, lens, heads, kvh, dh, P, scale=1.0, packed=True, poke=None, pool=None, spread=0.7, **hints):
     table, start, offsets, pages = layout(r, lens, P)
     rows = int(offsets[-1]) + 2   # two rows of no sequence
     pool = pool or Pool(r, pages, kvh, P, dh)
@@ -112,7 +112,7 @@ def run_append(r, lens, heads, kvh, dh, P, scale=1.0, packed=True, poke=None, po
         dev(x[:, a:b].transpose(1, 0, 2)).transpose(0, 1) for a, b in
         ((0, heads), (heads, heads + kvh), (heads + kvh, heads + 2 * kvh))]   # [heads][rows][dh] in memory
     q_out = torch.full((rows, heads, dh), 7.0, dtype=torch.float16, device=DEV)
-    b = batch_of(table, start, offsets, rows)
+    b = batch_of(table, start, offsets, rows, **hints)
     got = pool.cache.Append(b, *parts, dev(cos), dev(sin), q_out)
     torch.cuda.synchronize()
     assert got is q_out
@@ -128,7 +128,7 @@ def run_append(r, lens, heads, kvh, dh, P, scale=1.0, packed=True, poke=None, po
             continue
         pos = np.arange(start[i], start[i] + n)
         want = ref.rope(x64[a:a + n, :heads], cos[pos].astype(np.float64), sin[pos].astype(np.float64))
-        pair = np.abs(x64[a:a + n, :heads]).reshape(n, heads, -1, 2).sum(-1).repeat(2, -1)
+        pair = np.abs(x64[a:a + n, :heads]).reshape(n, heads, dh // 2, 2).sum(-1).repeat(2, -1)
         fine = np.abs(want) < 65000
         err = np.abs(q[a:a + n] - want)
         lim = np.abs(want) * 2.0 ** -11 + 2.0 ** -25 + 3 * 2.0 ** -24 * pair
@@ -143,6 +143,24 @@ def test_append(P, heads, kvh, dh):
     r = np.random.default_rng(P + heads)
     lens = [(0, 1), (P - 1, 2), (P, 1), (3, 0), (0, P), (5, 2 * P + 3), (P // 2, P // 2), (2 * P + 7, 1), (17, 40)]
     run_append(r, lens, heads, kvh, dh, P)
+
+
+FEW = {
+    # more sequences than rows fill pages of, some rows on both sides of a page's end; then whole pages and more,
+    # with a hint that promises one row each
+    "tokens": ([(n, 1) for n in (0, 1, 15, 16, 31, 63, 64, 200, 255)] + [(15, 2), (63, 3), (0, 2), (9, 0), (255, 2)], {}),
+    "wrong": ([(30, 1), (0, 300), (15, 2), (10, 0), (63, 9), (0, 16), (250, 45)], dict(max_new=1)),
+}
+
+
+@pytest.mark.parametrize("P", [16, 64, 256])
+@pytest.mark.parametrize("heads,kvh,dh", [(12, 4, 64), (5, 5, 128), (0, 2, 64)])
+@pytest.mark.parametrize("case", FEW)
+@pytest.mark.parametrize("scale", [1.0, 3000.0])
+def test_append_few_rows(case, heads, kvh, dh, P, scale):
+    """A wave per page; old rows of all sizes, so that some exponents rise."""
+    lens, hints = FEW[case]
+    run_append(np.random.default_rng(P + dh), lens, heads, kvh, dh, P, scale=scale, packed=P != 64, **hints)
 
 
 @pytest.mark.parametrize("scale", [1e-7, 3e-4, 30.0, 2000.0, 60000.0])

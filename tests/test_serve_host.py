@@ -187,7 +187,7 @@ def test_every_row_is_in_one_item(nseq, page, tile):
     offsets = np.concatenate([[0], np.cumsum(n)])
     table = r.permutation(nseq * width).reshape(nseq, width)
     h = Host(table, start, offsets, int(offsets[-1]) + 3, page, nseq * width)
-    for of_pages in (0, 1):
+    for of_pages in (0, 1, 3):
         items = [i for i in h.items(tile, of_pages) if i[2]]
         h.within(items)
         seen = np.zeros(h.rows, int)
@@ -253,6 +253,7 @@ def test_nonsense_stays_in_range(seed):
         if nseq <= 64:
             h.within(h.items(tile, 2))
     h.within(h.items(1, 1))
+    h.within(h.items(1, 3))
 
 
 def test_positions_past_the_table_are_not_taken():
