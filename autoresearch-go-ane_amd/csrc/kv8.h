@@ -64,7 +64,9 @@ __host__ __device__ __forceinline__ Kv8Items kv8_pages(int page) { return {(uint
 __host__ __device__ __forceinline__ uint32_t kv8_first(const Kv8Batch& b, Kv8Items t, int i) {
   return ((uint32_t)clampi(b.offsets[i], 0, b.rows) + (uint32_t)i * t.slack) / t.width;
 }
-inline uint32_t kv8_count(int nseq, int rows, Kv8Items t) { return ((uint32_t)rows + (uint32_t)nseq * t.slack) / t.width; }
+inline uint32_t kv8_count(int nseq, int rows, Kv8Items t) {
+  return ((uint32_t)rows + (uint32_t)nseq * t.slack) / t.width;
+}
 
 // The sequence of an item -- the largest i with f(i) <= item -- and its rows:
 // 64 candidates a round, so up to 64 sequences take one load's latency, up to

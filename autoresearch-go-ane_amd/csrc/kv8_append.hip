@@ -531,7 +531,8 @@ extern "C" int ane_debug_kv8_item(const ane_kv8_cache* cache, const ane_kv8_batc
   if (pages == 2 && b.nseq > 64)
     return op_fail(ANE_ERR_ARG, "storiesane %s: nseq=%d want at most 64", op, b.nseq);
   const bool tiles = pages == 0 || pages == 2;
-  const uint32_t n = kv8_count(b.nseq, b.rows, tiles ? kv8_tiles(tile_tokens) : pages == 1 ? kv8_pages(1 << b.pshift) : kv8_tiles(1));
+  const Kv8Items items = tiles ? kv8_tiles(tile_tokens) : pages == 1 ? kv8_pages(1 << b.pshift) : kv8_tiles(1);
+  const uint32_t n = kv8_count(b.nseq, b.rows, items);
   if (item < 0 || item >= (int64_t)n)
     return op_fail(ANE_ERR_ARG, "storiesane %s: item=%lld want below %u", op, (long long)item, n);
   const Kv8Span s = pages == 0   ? kv8_tile_span(b, tile_tokens, (uint32_t)item)

@@ -148,7 +148,8 @@ def test_append(P, heads, kvh, dh):
 FEW = {
     # more sequences than rows fill pages of, some rows on both sides of a page's end; then whole pages and more,
     # with a hint that promises one row each
-    "tokens": ([(n, 1) for n in (0, 1, 15, 16, 31, 63, 64, 200, 255)] + [(15, 2), (63, 3), (0, 2), (9, 0), (255, 2)], {}),
+    "tokens": ([(n, 1) for n in (0, 1, 15, 16, 31, 63, 64, 200, 255)] + [(15, 2), (63, 3), (0, 2), (9, 0), (255, 2)],
+               {}),
     "wrong": ([(30, 1), (0, 300), (15, 2), (10, 0), (63, 9), (0, 16), (250, 45)], dict(max_new=1)),
 }
 
@@ -317,7 +318,8 @@ def test_attend_large_tiles(case, P):
     for p in (3, last):
         pool.vb[table[-1, p // P], 0, p % P // 16, p % 16 // 4, 37 % 16, 37 // 16, p % 4] = 0x7f
     pool.load()
-    run_attend(np.random.default_rng(P), lens, heads, kvh, 64, P, pool=pool, holes=[(0, 0), (len(lens) - 1, 2)], **hints)
+    run_attend(np.random.default_rng(P), lens, heads, kvh, 64, P, pool=pool, holes=[(0, 0), (len(lens) - 1, 2)],
+               **hints)
 
 
 @pytest.mark.parametrize("dh", [64, 128])
