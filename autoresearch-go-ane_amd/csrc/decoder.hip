@@ -407,11 +407,15 @@ int attention8(ane_decoder* d, const char* op, int l, const ane_kv8_batch& b, ha
   a.q_row = a.k_row = a.v_row = a.q_out_row = N1;
   a.q_head = a.k_head = a.v_head = a.q_out_head = 64;
   a.heads = d->NH; a.positions = d->rope_rows;
-  SCHK(op, kv8_append(&c, &b, &a, from, d->stream));
   ane_kv8_attend_args t{};
   t.q = (const uint16_t*)qkv; t.out = (uint16_t*)out;
   t.q_row = N1; t.q_head = 64; t.out_row = D; t.out_head = 64;
   t.heads = d->NH; t.scale = 0.125f; t.ws = d->ws8; t.ws_bytes = (int64_t)d->ws8_cap;
+  if (from) {
+    SCHK(op, kv8_step(&c, &b, &a, from, &t, frag, d->stream));
+    return ANE_OK;
+  }
+  SCHK(op, kv8_append(&c, &b, &a, from, d->stream));
   SCHK(op, kv8_attend(&c, &b, &t, frag, d->stream));
   return ANE_OK;
 }

@@ -229,6 +229,11 @@ int kv8_append(const ane_kv8_cache* cache, const ane_kv8_batch* batch, const ane
 int kv8_attend(const ane_kv8_cache* cache, const ane_kv8_batch* batch, const ane_kv8_attend_args* args, bool frag,
                void* stream);
 
+// Both for a step of at most one new token a sequence, in one launch where the
+// contexts stay whole (q_out is then not written); the same bits.
+int kv8_step(const ane_kv8_cache* cache, const ane_kv8_batch* batch, const ane_kv8_append_args* append,
+             const Kv8Sums* from, const ane_kv8_attend_args* args, bool frag, void* stream);
+
 // Whether fp16 rows of [rows][heads][dh] with these strides do not overlap
 // (outputs; either order of the two outer dimensions).
 inline bool kv8_apart(int64_t rows, int64_t row, int64_t heads, int64_t head, int64_t dh) {

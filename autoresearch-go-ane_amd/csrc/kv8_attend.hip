@@ -13,7 +13,8 @@
 //
 // A block is one tile and one key/value head (and one part of the keys where
 // tiles are few); its waves take steps of 32 keys in turn and meet once
-// at the end, in LDS.  There is no barrier in the loop.
+// at the end, in LDS.  There is no barrier in the loop.  A decoder's step has
+// its append in the same launch (kv8_step).
 //
 // What bounds it.  Single tokens over long contexts: the cache's bytes (40
 // sequences of up to 40,000 tokens, 2 heads of 128: 494 MB in 108 us, 4.6 TB/s,
@@ -24,9 +25,9 @@
 // with the vector units 78 % busy (one of 8192 tokens, 12 heads of 64: 121 us,
 // 850 TFLOP/s).
 #include <algorithm>
+#include <type_traits>
 
-#include "decode.h"
-#include "kv8.h"
+#include "kv8_rows.h"
 #include "op_error.h"
 
 namespace ane {
@@ -56,6 +57,11 @@ struct AttendArgs {
   float c;      // scale * log2(e)
   float* part;  // [tiles][NKV][nsplit][tt * G][DH]: a row's sums
   float2* ml;   // [tiles][NKV][nsplit][tt * G]: their maximum and sum of exponentials
+};
+
+// with the append of the rows' own keys and values, from a product's sums
+struct StepArgs : AttendArgs {
+  Kv8AppendArgs in;
 };
 
 // where dimension d of a row's query head goes
@@ -115,9 +121,12 @@ constexpr int waves_per_simd(int DH, int NT) {
 // NT: tiles of 16 rows; KW: waves that share a tile's keys; RW: tiles a block
 // takes, each by a wave of its own (KW = 1: the waves have nothing to do with
 // each other); ONE: a step's keys are of one page (pages of at least kStep
-// tokens).
-template <int DH, int NT, int KW, int RW, bool ONE>
-__global__ __launch_bounds__(64 * KW * RW, waves_per_simd(DH, NT)) void attend_kernel(AttendArgs a) {
+// tokens).  Args is StepArgs: the sequences have a token each, and the block
+// first appends its key and value and rotates its queries.
+template <int DH, int NT, int KW, int RW, bool ONE, typename Args>
+__global__ __launch_bounds__(64 * KW * RW, waves_per_simd(DH, NT)) void attend_kernel(Args a) {
+  constexpr bool STEP = std::is_same_v<Args, StepArgs>;
+  static_assert(!STEP || (NT == 1 && KW == 4));
   static_assert(KW == 1 || RW == 1, "the waves of a block meet over one tile");
   constexpr int R = 16 * NT;    // rows of the tile
   constexpr int NM = DH / 32;   // MFMAs along the head dimension
@@ -147,6 +156,22 @@ __global__ __launch_bounds__(64 * KW * RW, waves_per_simd(DH, NT)) void attend_k
   const int k0 = sp * pk;
   if (k0 >= kend) return;
   const int k1 = min(kend, k0 + pk);
+
+  constexpr int CPR = DH / 8;
+  __shared__ half8 qs[STEP ? 16 * CPR : 1];  // the rotated queries
+  if constexpr (STEP) {
+    // one wave appends, three rotate; no other block touches the page and head,
+    // and behind the barrier the block's waves see what was written
+    __shared__ uint4 unit[DH];
+    if (wave == 0) {
+      if (!a.in.from.err || !*a.in.from.err) kv8_append_rows<DH, true>(a.in, span, h, unit);
+    } else if (const int c = tid - 64; c < a.G * CPR) {
+      const int d0 = c % CPR * 8;
+      qs[c] = narrow8(rotate8(sums8(a.in.from, span.row, (h * a.G + c / CPR) * DH + d0),
+                              turn_of<DH>(a.in.cos, a.in.sin, span.pos, d0)));
+    }
+    __syncthreads();
+  }
 
   // 64 pages from wbase on, one per lane: where the head's rows begin, and
   // what Step says of the page.  wend: the first position behind them.
@@ -208,7 +233,8 @@ __global__ __launch_bounds__(64 * KW * RW, waves_per_simd(DH, NT)) void attend_k
     lim[t] = span.pos + tok;
     const half_t* p = a.q + (span.row + tok) * a.q_row + (h * a.G + hg) * a.q_head + 16 * g;
 #pragma unroll
-    for (int m = 0; m < NM; m++) q[t][m] = ld_h8(p + 64 * (m >> 1) + 8 * (m & 1));
+    for (int m = 0; m < NM; m++)
+      q[t][m] = STEP ? qs[r * CPR + 8 * (m >> 1) + 2 * g + (m & 1)] : ld_h8(p + 64 * (m >> 1) + 8 * (m & 1));
   }
   Step<DH> cur;
   int kb = k0 + wave * kStep;
@@ -621,13 +647,13 @@ int plan(const char* op, const Kv8Batch& b, const ane_kv8_batch& given, int DH, 
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
-template <int DH, int NT, int KW, int RW>
-void launch_form(const AttendArgs& a, hipStream_t st) {
+template <int DH, int NT, int KW, int RW, typename Args>
+void launch_form(const Args& a, hipStream_t st) {
   const dim3 grid(((uint32_t)a.tiles + RW - 1) / RW * a.b.NKV * a.nsplit), block(64 * KW * RW);
   if (kStep <= 1 << a.b.pshift)
-    hipLaunchKernelGGL((attend_kernel<DH, NT, KW, RW, true>), grid, block, 0, st, a);
+    hipLaunchKernelGGL((attend_kernel<DH, NT, KW, RW, true, Args>), grid, block, 0, st, a);
   else
-    hipLaunchKernelGGL((attend_kernel<DH, NT, KW, RW, false>), grid, block, 0, st, a);
+    hipLaunchKernelGGL((attend_kernel<DH, NT, KW, RW, false, Args>), grid, block, 0, st, a);
 }
 
 template <int DH>
@@ -664,10 +690,14 @@ extern "C" int ane_kv8_attend(const ane_kv8_cache* cache, const ane_kv8_batch* b
   return kv8_attend(cache, batch, args, false, stream);
 }
 
-int ane::kv8_attend(const ane_kv8_cache* cache, const ane_kv8_batch* batch, const ane_kv8_attend_args* args, bool frag,
-                    void* stream) {
+namespace {
+
+// in: the append that the launch takes with it, where the plan lets it
+int attend(const ane_kv8_cache* cache, const ane_kv8_batch* batch, const ane_kv8_attend_args* args, bool frag,
+           const Kv8AppendArgs* in, void* stream) {
   const char* op = "kv8 attend";
-  AttendArgs a;
+  StepArgs step;
+  AttendArgs& a = step;
   int rc = kv8_check(op, cache, batch, &a.b);
   if (rc) return rc;
   if (!args) return op_fail(ANE_ERR_ARG, "storiesane %s: null arguments", op);
@@ -703,9 +733,35 @@ int ane::kv8_attend(const ane_kv8_cache* cache, const ane_kv8_batch* batch, cons
   a.part = (float*)g.ws;
   a.ml = (float2*)(a.part + (size_t)p.tiles * a.b.NKV * p.nsplit * p.tt * a.G * cache->head_dim);
   a.frag = frag;
-  if (cache->head_dim == 64) launch<64>(a, p, (hipStream_t)stream);
+  if (in) {
+    step.in = *in;
+    launch_form<64, 1, 4, 1>(step, (hipStream_t)stream);
+  } else if (cache->head_dim == 64) launch<64>(a, p, (hipStream_t)stream);
   else launch<128>(a, p, (hipStream_t)stream);
   const hipError_t h = hipGetLastError();
   if (h != hipSuccess) return op_fail(ANE_ERR_HIP, "storiesane %s: %s", op, hipGetErrorString(h));
   return ANE_OK;
+}
+
+}  // namespace
+
+int ane::kv8_attend(const ane_kv8_cache* cache, const ane_kv8_batch* batch, const ane_kv8_attend_args* args, bool frag,
+                    void* stream) {
+  return attend(cache, batch, args, frag, nullptr, stream);
+}
+
+int ane::kv8_step(const ane_kv8_cache* cache, const ane_kv8_batch* batch, const ane_kv8_append_args* append,
+                  const Kv8Sums* from, const ane_kv8_attend_args* args, bool frag, void* stream) {
+  Kv8AppendArgs in;
+  int rc = kv8_append_check("kv8 append", cache, batch, append, from, &in);
+  if (rc || in.b.nseq == 0 || in.b.rows == 0) return rc;
+  Plan p;
+  rc = plan("kv8 attend", in.b, *batch, cache->head_dim, append->heads, &p);
+  if (rc) return rc;
+  // The decoder's step of 64 sequences and 1024 tokens, 12 layers: 0.504 ms in
+  // one launch a layer, 0.534 in two; of 3 sequences 0.330 and 0.346.
+  const bool one = from && batch->max_new == 1 && in.b.rows <= in.b.nseq && p.nt == 1 && p.nsplit == 1;
+  if (one) return attend(cache, batch, args, frag, &in, stream);
+  rc = kv8_append(cache, batch, append, from, stream);
+  return rc ? rc : attend(cache, batch, args, frag, nullptr, stream);
 }

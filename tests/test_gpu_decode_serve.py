@@ -132,6 +132,24 @@ def test_many_sequences_and_a_long_context():
         assert d.max() <= 0.3 and np.sqrt((d ** 2).mean()) <= 0.08 * got[0].std()
 
 
+@pytest.mark.parametrize("nseq,page,heads,kv_heads", [(1, 16, 4, 2), (3, 64, 6, 2), (20, 32, 4, 4), (5, 256, 8, 2)])
+def test_steps_in_one_launch_a_layer_and_in_two_are_the_same_bits(nseq, page, heads, kv_heads):
+    """Contexts of up to 1280 tokens have the append in the attention's launch;
+    room for more does not, and up to 128 tokens its keys are one part all the
+    same."""
+    cfg = ane.tiny_decode(heads=heads, kv_heads=kv_heads, dim=64 * heads)
+    p, prefix, forced = setup(cfg, nseq, 64, 60, 61)
+    got = []
+    for ctx in (192, 1344):
+        dec = ane.Decoder(cfg, p, max_batch=nseq, max_ctx=ctx, page_tokens=page)
+        try:
+            dec.DebugFillCache(0xFF)
+            got.append(run(dec, prefix, forced))
+        finally:
+            dec.Close()
+    np.testing.assert_array_equal(got[0].view(np.uint32), got[1].view(np.uint32))
+
+
 def test_switching_the_cache():
     """8 bit and back: as if never switched; the batch is dropped."""
     cfg = ane.tiny_decode()

@@ -164,6 +164,24 @@ def test_append_few_rows(case, heads, kvh, dh, P, scale):
     run_append(np.random.default_rng(P + dh), lens, heads, kvh, dh, P, scale=scale, packed=P != 64, **hints)
 
 
+@pytest.mark.parametrize("dh", [64, 128])
+def test_append_does_not_depend_on_hints(dh):
+    """The same bits whichever kernel the hints choose."""
+    lens = [(30, 1), (0, 40), (15, 2), (63, 9), (5, 16)]
+    table, start, offsets, pages = layout(np.random.default_rng(1), lens, 32)
+    x = dev((np.random.default_rng(2).standard_normal((68, 14, dh)) * 2).astype(np.float16))
+    cos, sin = (dev(t) for t in rope_tables(table.shape[1] * 32, dh))
+    got = []
+    for hints in (dict(max_new=1), dict(max_new=40), {}):
+        pool = Pool(np.random.default_rng(3), pages, 3, 32, dh)
+        q = torch.zeros((68, 8, dh), dtype=torch.float16, device=DEV)
+        pool.cache.Append(batch_of(table, start, offsets, 68, **hints), x[:, :8], x[:, 8:11], x[:, 11:], cos, sin, q)
+        got.append([q.cpu().numpy().view(np.uint16)] + [z.copy() for z in pool.held()])
+    for other in got[1:]:
+        for a, b in zip(got[0], other):
+            np.testing.assert_array_equal(a, b)
+
+
 @pytest.mark.parametrize("scale", [1e-7, 3e-4, 30.0, 2000.0, 60000.0])
 def test_append_magnitudes(scale):
     """Exponents from the bottom (codes that are subnormal, all zeros) to the
