@@ -88,8 +88,9 @@ class KVBatch:
     offsets int32 [nseq + 1] (rows of each sequence in the step's tensors),
     rows (rows of those tensors).  The tensors are read when the kernels run:
     a captured step is replayed with what they then hold.  max_len and
-    max_new, where known on the host, choose the launch sizes; results do not
-    depend on them."""
+    max_new, where known on the host, choose the launch sizes; wrong ones cost
+    time.  An append's bits do not depend on them; attention adds its sums up
+    in as many parts as they make, so that last bits may."""
 
     def __init__(self, table, start, offsets, rows, max_len=0, max_new=0):
         op = "kv8 batch"

@@ -57,8 +57,9 @@ typedef struct ane_kv8_cache {
  * there: nothing is written to it and its keys do not take part.  Rows of no
  * sequence are left as they are.
  * max_len (tokens of the longest sequence, new ones included) and max_new (its
- * new tokens) size the launches; wrong values cost time, not correctness.  0:
- * not known. */
+ * new tokens) size the launches; wrong values cost time, not correctness (an
+ * attention's sums are added in as many parts as they make: last bits may
+ * differ).  0: not known. */
 typedef struct ane_kv8_batch {
   const int32_t *table;   /* [nseq][table_stride], table_pages of each row used */
   const int32_t *start;   /* [nseq] */
