@@ -622,15 +622,16 @@ int plan(const char* op, const Kv8Batch& b, const ane_kv8_batch& given, int DH, 
   // four 45; 250 of 17,000 90, 78, 77).
   // Single tokens stay whole up to 1280 keys, 768 of head dimension 128 (4
   // blocks of 512 keys 5.3 us, in parts 7.3; of 1280 7.6 and 8.1; of 2048 9.7
-  // and 7.6), and up to 4096 where there are 128 blocks (64 sequences of 4
-  // heads and 2048 keys 13.8 and 18.3).  Beyond, up to 512 blocks, in parts of
-  // 256 keys at least (4 blocks of 4096: 16 parts 8.0 us, 32 8.6) and, ragged
-  // as they are, 2048 at most, so that one long context does not outlast the
-  // rest (64 of 8 heads and up to 30,000 keys 206 us, whole 232; 80 blocks of
-  // up to 40,000 108 us, of 4096 keys 113).
+  // and 7.6), and up to 32 for each block, 8192 at most, where there are 128
+  // blocks (64 sequences of 4 heads and 4224 keys 25 us, in parts 30; of up to
+  // 5000 21 and 23; 128 blocks of 10,000 36 and 23).  Beyond, up to 512 blocks,
+  // in parts of 256 keys at least (4 blocks of 4096: 16 parts 8.0 us, 32 8.6)
+  // and, ragged as they are, 2048 at most, so that one long context does not
+  // outlast the rest (64 of 8 heads and up to 30,000 keys 206 us, whole 232;
+  // 80 blocks of up to 40,000 108 us, of 4096 keys 113).
   int64_t ns = 1;
   if (p->nt == 1) {
-    if (len > (blocks >= 128 ? 4096 : DH == 64 ? 1280 : 768))
+    if (len > (blocks >= 128 ? std::min<int64_t>(32 * blocks, 8192) : DH == 64 ? 1280 : 768))
       ns = std::max<int64_t>(std::min<int64_t>((511 + blocks) / blocks, (len + 255) / 256), (len + 2047) / 2048);
   } else if (p->kw == 4) {
     ns = std::max<int64_t>(std::min<int64_t>(256 / blocks, len / 512),
