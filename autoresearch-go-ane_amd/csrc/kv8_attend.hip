@@ -102,8 +102,9 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
 
 // One step's K and V, NU units of 16 keys: raw codes, and of each unit's page
 // the exponents (K in bits 0..7, V in 8..15) and whether it is there (bit 16).
-// A page that is not there reads the pool's first, which exists; its scores
-// are masked and its values cleared.
+// A page that is not there reads the pool's first, which exists but may hold
+// anything; its scores are masked, its values cleared, and its exponents 0 (a
+// scale made of a stray one, -128, is NaN and makes NaN of cleared values too).
 template <int DH>
 struct Step {
   u32x4 k[NU][DH / 64], v[NU][DH / 64];
@@ -192,7 +193,7 @@ __global__ __launch_bounds__(64 * KW * RW, waves_per_simd(DH, NT)) void attend_k
     const size_t at = e * ((size_t)DH << b.pshift);
     wlo = (uint32_t)at;
     whi = (uint32_t)(at >> 32);
-    wexp = ((int)a.k_exp[e] & 0xff) | ((int)a.v_exp[e] & 0xff) << 8 | (id >= 0 ? kThere : 0);
+    wexp = id >= 0 ? ((int)a.k_exp[e] & 0xff) | ((int)a.v_exp[e] & 0xff) << 8 | kThere : 0;
   };
   // The codes of the step at kb; `on` false: nothing is wanted of them (one
   // line is read).
