@@ -56,7 +56,7 @@ struct AttendArgs {
   int round;    // keys that a block takes at a time: parts are multiples of it
   float c;      // scale * log2(e)
   float* part;  // [tiles][NKV][nsplit][tt * G][DH]: a row's sums
-  float2* ml;   // [tiles][NKV][nsplit][tt * G]: their maximum and sum of exponentials
+  float2* ml;   // [tiles][NKV][nsplit][tt * G]: what they are relative to, and the sum of exponentials
 };
 
 // with the append of the rows' own keys and values, from a product's sums
@@ -247,11 +247,18 @@ __global__ __launch_bounds__(64 * KW * RW, waves_per_simd(DH, NT)) void attend_k
     for (int m = 0; m < NM; m++) asm volatile("" : "+v"(q[t][m]));
 
   // m: what the exponentials are relative to, the same in the four lanes of a
-  // row: at least the row's maximum less kSlack so far.  It moves only when a
-  // score passes it by more, so that most steps neither join the lanes'
-  // maxima nor touch the sums; weights stay below 2^kSlack.  bar: how far a
-  // score may pass it; -inf while the row has seen no key (m is then 0).
-  constexpr float kSlack = 8.f;
+  // row: kBase below the row's largest score when it last moved.  It moves only
+  // when a score passes it by kBase + kSlack, so that most steps neither join
+  // the lanes' maxima nor touch the sums.  bar: how far a score may pass it;
+  // -inf while the row has seen no key (m is then 0).
+  // The weights are rounded to fp16 for the second product, the largest between
+  // 2^kBase and 2^(kBase + kSlack), half of fp16's range: those down to 2^-21 of
+  // it are normal numbers, off by at most 2^-11 of themselves (and divided by
+  // the sum of the weights as rounded), smaller ones by 2^-32 of the largest, so
+  // that a million keys behind one that takes most of the weight stay below the
+  // output's own rounding.  A larger base would hold more of them, but moves
+  // more often (prompt of 8192 tokens, base 7: 121 us, 8: 123, 9: 125, 11: 126).
+  constexpr float kBase = 7.f, kSlack = 8.f;
   float m[NT], bar[NT];
   floatx4 o[ND][NT], l[NT];  // l: the sum of the row's weights, four times
 #pragma unroll
@@ -324,13 +331,14 @@ __global__ __launch_bounds__(64 * KW * RW, waves_per_simd(DH, NT)) void attend_k
       for (int t = 0; t < NT; t++) {
         const float top = xor32_max(xor16_max(mx[t]));
         if (top > bar[t]) {  // the same in the row's four lanes
-          const float al = bar[t] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(-top);
-          m[t] += top;
-          bar[t] = kSlack;
+          const float by = top - kBase;
+          const float al = bar[t] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(-by);
+          m[t] += by;
+          bar[t] = kBase + kSlack;
 #pragma unroll
           for (int u = 0; u < NU; u++)
 #pragma unroll
-            for (int j = 0; j < 4; j++) sc[u][t][j] -= top;
+            for (int j = 0; j < 4; j++) sc[u][t][j] -= by;
 #pragma unroll
           for (int j = 0; j < 4; j++) l[t][j] *= al;
 #pragma unroll
