@@ -163,6 +163,12 @@ class Decoder:
         self._live()
         self._check(self._lib.ane_decode_debug_fill_cache(self._h, int(byte)))
 
+    def DebugFailChain(self, step: int = 0):
+        """Test-only: the fused chain counts as failed from this step on of the
+        next Generate (0: or Step) call."""
+        self._live()
+        self._check(self._lib.ane_decode_debug_fail_chain(self._h, int(step)))
+
     def LastMs(self) -> float:
         self._live()
         return float(self._lib.ane_decode_last_ms(self._h))

@@ -114,6 +114,18 @@ hipError_t dec_attention(const DecAttnArgs& a, hipStream_t s);
 // start[i] = ctr[0] (no ctr: 0) and offsets[i] = i * each for i <= nseq: a step
 // (each = 1) or the prefill of nseq prompts
 hipError_t dec_batch_plan(int* start, int* offsets, const int* ctr, int nseq, int each, hipStream_t s);
+// What a redone call must find as it was: of each sequence's page `pg` of the
+// 8-bit cache, the first `rows` rows (to whole units of 16) and the exponents,
+// copied to `kept` (layers * nseq * kv_heads pages of K, then as many of V) and
+// `kept_exp`, or back from there.
+struct DecPages {
+  uint8_t *k, *v;        // [layers][seqs * per][kv_heads][page * 64]
+  int8_t *k_exp, *v_exp; // [layers][seqs * per][kv_heads]
+  uint8_t* kept;
+  int8_t* kept_exp;
+  int layers, seqs, nseq, per, kv_heads, page, pg, rows;
+};
+hipError_t dec_copy_pages(const DecPages& a, bool back, hipStream_t s);
 // p[i] = i for i < n
 hipError_t dec_count_up(int* p, int n, hipStream_t s);
 // The history that penalties count, uint16 [..][ld]: the prompts (and the

@@ -758,6 +758,35 @@ __global__ __launch_bounds__(64) void batch_plan_kernel(int* start, int* offsets
   if (i <= nseq) offsets[i] = i * each;
 }
 
+// a block per layer, sequence and kv head
+__global__ __launch_bounds__(256) void copy_pages_kernel(DecPages a, bool back) {
+  const int j = blockIdx.x, h = j % a.kv_heads, i = j / a.kv_heads % a.nseq, l = j / (a.kv_heads * a.nseq);
+  const size_t n = gridDim.x, bytes = (size_t)a.page * 64;
+  const size_t ph = (((size_t)l * a.seqs + i) * a.per + a.pg) * a.kv_heads + h;
+  uint4* k = reinterpret_cast<uint4*>(a.k + ph * bytes);
+  uint4* v = reinterpret_cast<uint4*>(a.v + ph * bytes);
+  uint4* kk = reinterpret_cast<uint4*>(a.kept + j * bytes);
+  uint4* kv = reinterpret_cast<uint4*>(a.kept + (n + j) * bytes);
+  for (int c = threadIdx.x; c < (a.rows + 15) / 16 * 64; c += 256) {
+    if (back) {
+      k[c] = kk[c];
+      v[c] = kv[c];
+    } else {
+      kk[c] = k[c];
+      kv[c] = v[c];
+    }
+  }
+  if (threadIdx.x == 0) {
+    if (back) {
+      a.k_exp[ph] = a.kept_exp[j];
+      a.v_exp[ph] = a.kept_exp[n + j];
+    } else {
+      a.kept_exp[j] = a.k_exp[ph];
+      a.kept_exp[n + j] = a.v_exp[ph];
+    }
+  }
+}
+
 __global__ __launch_bounds__(256) void count_up_kernel(int* p, int n) {
   const int i = blockIdx.x * 256 + threadIdx.x;
   if (i < n) p[i] = i;
@@ -794,6 +823,13 @@ __global__ __launch_bounds__(64) void take_tokens_kernel(uint16_t* tok_out, uint
 
 hipError_t dec_batch_plan(int* start, int* offsets, const int* ctr, int nseq, int each, hipStream_t s) {
   hipLaunchKernelGGL(batch_plan_kernel, dim3(nseq / 64 + 1), dim3(64), 0, s, start, offsets, ctr, nseq, each);
+  return hipGetLastError();
+}
+
+hipError_t dec_copy_pages(const DecPages& a, bool back, hipStream_t s) {
+  if (a.nseq < 1 || a.nseq > a.seqs || a.pg < 0 || a.pg >= a.per || a.rows < 0 || a.rows > a.page)
+    return hipErrorInvalidValue;
+  hipLaunchKernelGGL(copy_pages_kernel, dim3(a.layers * a.nseq * a.kv_heads), dim3(256), 0, s, a, back);
   return hipGetLastError();
 }
 

@@ -23,6 +23,7 @@
 
 #include <cmath>
 #include <string>
+#include <utility>
 #include <algorithm>
 #include <vector>
 
@@ -91,6 +92,8 @@ struct ane_decoder {
   int8_t *ke8 = nullptr, *ve8 = nullptr;
   int *table8 = nullptr, *start8 = nullptr, *off8 = nullptr;
   half_t* qkv8 = nullptr;  // [64][N1] rows of a step
+  uint8_t* kept8 = nullptr;  // each sequence's current page at the start of a call, kept to redo it
+  int8_t* kept_exp8 = nullptr;
   void* ws8 = nullptr;     // attention workspace
   size_t ws8_cap = 0;
   // controls on the logits, when set
@@ -129,6 +132,7 @@ struct ane_decoder {
   size_t tail_set_sz = 0;
   uint16_t *tok_d = nullptr, *hist_d = nullptr, *prefix_d = nullptr;
   uint16_t* tok_save = nullptr;  // a call's input tokens, kept to redo it after a failed chain wait
+  int fail_step = -1;            // the step of the next call from which the chain counts as failed (tests)
   int chain_latched = 0;         // 1 once a failed chain wait switched the decoder to one launch per GEMM
   int* ctr_d = nullptr;
   int TC = 0;
@@ -597,16 +601,28 @@ void latch_per_gemm(ane_decoder* d) {
   drop_graph(d);
 }
 
+// The page of the 8-bit cache that position pos0 goes to, and the rows it holds
+// before.
+DecPages pages8(const ane_decoder* d, int pos0) {
+  return {d->k8, d->v8, d->ke8, d->ve8, d->kept8, d->kept_exp8, d->L, d->B, d->nseq, d->seq_pages, d->NKV, d->page8,
+          pos0 / d->page8, pos0 % d->page8};
+}
+
 // The start of a step / generate call, kept so that the call can be redone:
 // the input tokens (the device copy the first step reads) and the position.
-int save_start(ane_decoder* d, const char* op) {
+// Cache rows from there on are rewritten by the redo before any read; but in
+// the 8-bit cache a louder row raises its page's exponent, and the rows before
+// are rounded again, so the page that position pos0 goes to is kept where it
+// holds any (64 sequences, 12 layers, 4 heads: 25 MB at most in pages of 64).
+int save_start(ane_decoder* d, const char* op, int pos0) {
+  if (d->page8 && pos0 % d->page8) DCHK(op, dec_copy_pages(pages8(d, pos0), false, d->stream));
   DCHK(op, hipMemcpyAsync(d->tok_save, d->tok_d, (size_t)d->nseq * 2, hipMemcpyDeviceToDevice, d->stream));
   return ANE_OK;
 }
 
-// Rewinds to a saved start: the tokens and the device counters of position
-// pos0 (cache rows from pos0 on are rewritten by the redo before any read).
+// Rewinds to a saved start.
 int restore_start(ane_decoder* d, const char* op, int pos0) {
+  if (d->page8 && pos0 % d->page8) DCHK(op, dec_copy_pages(pages8(d, pos0), true, d->stream));
   DCHK(op, hipMemcpyAsync(d->tok_d, d->tok_save, (size_t)d->nseq * 2, hipMemcpyDeviceToDevice, d->stream));
   DCHK(op, dec_set_ctr(d->ctr_d, pos0, 0, d->stream));
   return ANE_OK;
@@ -782,7 +798,8 @@ extern "C" int ane_decode_step(ane_decoder* d, const uint16_t* in_tok, uint16_t*
     if (int rc = room8(d, op, batch8(d, 0, d->nseq, d->nseq, d->C, 1))) return rc;
   if (in_tok) DCHK(op, hipMemcpyAsync(d->tok_d, in_tok, (size_t)d->nseq * 2, hipMemcpyHostToDevice, d->stream));
   const int pos0 = d->pos;
-  int rc = d->use_tail ? save_start(d, op) : ANE_OK;
+  int rc = d->use_tail ? save_start(d, op, pos0) : ANE_OK;
+  if (d->use_tail && std::exchange(d->fail_step, -1) == 0) DCHK(op, hipMemsetAsync(d->err_d, 1, 4, d->stream));
   if (rc == ANE_OK) rc = enqueue_step(d, logits ? d->logits_d : nullptr, nullptr);
   if (rc == ANE_OK) rc = copy_out(d, next_tok, logits);
   bool failed = false;
@@ -810,7 +827,7 @@ extern "C" int ane_decode_generate(ane_decoder* d, int32_t nsteps, uint16_t* out
   if (d->page8)
     if (int rc = room8(d, op, batch8(d, 0, d->nseq, d->nseq, d->C, 1))) return rc;
   const int pos0 = d->pos;
-  int rc = d->use_tail ? save_start(d, op) : ANE_OK;
+  int rc = d->use_tail ? save_start(d, op, pos0) : ANE_OK;
   if (rc == ANE_OK) rc = generate_run(d, op, nsteps, out_tok);
   bool failed = false;
   if (rc == ANE_OK) rc = tail_failed(d, op, &failed);
@@ -847,7 +864,11 @@ int generate_run(ane_decoder* d, const char* op, int nsteps, uint16_t* out_tok) 
   }
   DCHK(op, dec_set_ctr(d->ctr_d, d->pos, 0, st));  // history rows count from 0 for this call
   DCHK(op, hipEventRecord(d->ev0, st));
-  for (int i = 0; i < nsteps; i++) DCHK(op, hipGraphLaunch(d->gexec, st));
+  const int fail = d->use_tail ? std::exchange(d->fail_step, -1) : -1;
+  for (int i = 0; i < nsteps; i++) {
+    if (i == fail) DCHK(op, hipMemsetAsync(d->err_d, 1, 4, st));
+    DCHK(op, hipGraphLaunch(d->gexec, st));
+  }
   DCHK(op, hipEventRecord(d->ev1, st));
   if (out_tok)
     DCHK(op, hipMemcpyAsync(out_tok, d->hist_d, (size_t)nsteps * d->nseq * 2, hipMemcpyDeviceToHost, st));
@@ -892,6 +913,11 @@ int alloc8(ane_decoder* d, const char* op, int page) {
   DCHK(op, dalloc(d, &d->start8, (size_t)d->B + 1));
   DCHK(op, dalloc(d, &d->off8, (size_t)d->B + 1));
   DCHK(op, dalloc(d, &d->qkv8, (size_t)kDecRows * d->N1));
+  if (d->use_tail) {
+    const size_t kept = (size_t)2 * d->L * d->B * d->NKV;
+    DCHK(op, dalloc(d, &d->kept8, kept * page * 64));
+    DCHK(op, dalloc(d, &d->kept_exp8, kept));
+  }
   // each sequence's pages one after the other
   DCHK(op, dec_count_up(d->table8, d->B * per, d->stream));
   d->seq_pages = per;
@@ -901,6 +927,7 @@ int alloc8(ane_decoder* d, const char* op, int page) {
 void free8(ane_decoder* d) {
   drop(d, &d->k8); drop(d, &d->v8); drop(d, &d->ke8); drop(d, &d->ve8);
   drop(d, &d->table8); drop(d, &d->start8); drop(d, &d->off8); drop(d, &d->qkv8);
+  drop(d, &d->kept8); drop(d, &d->kept_exp8);
   d->page8 = d->seq_pages = 0;
 }
 int alloc16(ane_decoder* d, const char* op) {
@@ -1015,6 +1042,12 @@ extern "C" int ane_decode_set_controls(ane_decoder* d, const ane_decode_controls
   d->ctl = a;
   d->ctl_mask_rows = c->mask_rows;
   d->controls = true;
+  return ANE_OK;
+}
+
+extern "C" int ane_decode_debug_fail_chain(ane_decoder* d, int32_t step) {
+  if (!d || !d->stream) return ANE_ERR_STATE;
+  d->fail_step = step;
   return ANE_OK;
 }
 

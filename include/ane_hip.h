@@ -398,7 +398,9 @@ double ane_decode_last_ms(ane_decoder *d);
  * GPU can break both) the decoder switches to one launch per GEMM for good
  * and redoes the call from its start, as the reference disables a failing
  * accelerator piece and carries on (ane/engine.go:887-894,
- * ane/train_full.go:356-368).  If the redo itself fails, the active batch is
+ * ane/train_full.go:356-368).  What the attempt changed is taken back first,
+ * the exponents and rounding of the 8-bit cache's pages too, so the redo gives
+ * what a call without the chain gives.  If the redo itself fails, the active batch is
  * dropped: Step / Generate then refuse until the next Prefill. */
 int32_t ane_decode_fused_chain(ane_decoder *d);
 /* Which cache a decoder keeps (no reference counterpart): page_tokens = 0 the
@@ -430,6 +432,10 @@ int ane_decode_set_controls(ane_decoder *d, const ane_decode_controls *c);
  * with `byte` (0xFF: fp16 NaN everywhere), so a test can show that no
  * position is read before it is written. */
 int ane_decode_debug_fill_cache(ane_decoder *d, int byte);
+/* Test-only: the fused chain counts as failed from step `step` on of the next
+ * Generate call (0 also of a Step call), as after a wait that timed out there;
+ * the call is then redone with one launch per GEMM.  Below 0: not. */
+int ane_decode_debug_fail_chain(ane_decoder *d, int32_t step);
 
 /* ---- mixture-of-experts SwiGLU FFN layer ----------------------------------
  * No counterpart in the reference (its FFN is dense, ane/common.go:91-105
