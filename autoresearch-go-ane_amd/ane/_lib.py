@@ -192,6 +192,7 @@ SIGNATURES = {
     "ane_decode_set_controls": (C.c_int, [_eng, C.POINTER(DecodeControls)]),
     "ane_decode_debug_fill_cache": (C.c_int, [_eng, C.c_int]),
     "ane_decode_debug_fail_chain": (C.c_int, [_eng, C.c_int32]),
+    "ane_decode_debug_allocs": (C.c_int64, [C.c_int32, C.c_int32]),
     "ane_moe_open": (C.c_int, [C.POINTER(MoeCfg), C.POINTER(C.c_void_p)]),
     "ane_moe_destroy": (None, [_eng]),
     "ane_moe_last_error": (C.c_char_p, [_eng]),

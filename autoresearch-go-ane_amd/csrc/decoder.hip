@@ -160,15 +160,29 @@ int dfail(ane_decoder* d, int code, const char* fmt, ...) {
 
 #define DCHK(op, expr)                                                                                   \
   do {                                                                                                   \
-    hipError_t _h = (expr);                                                                              \
+    hipError_t _h = taken(expr);                                                                         \
     if (_h != hipSuccess)                                                                                \
       return dfail(d, ANE_ERR_HIP, "storiesane decode %s: %s: %s", op, #expr, hipGetErrorString(_h));    \
   } while (0)
 
+// What tests ask of this thread's allocations (ane_decode_debug_allocs).
+thread_local int64_t t_allocated = 0;
+thread_local int t_fail_first = 0, t_fail_count = 0;
+
+hipError_t device_malloc(void** p, size_t bytes) {
+  if (t_fail_count > 0 && t_fail_first-- <= 0) {
+    t_fail_count--;
+    return hipMalloc(p, (size_t)1 << 60);  // more than there is: the error as the runtime makes it
+  }
+  const hipError_t e = hipMalloc(p, bytes);
+  if (e == hipSuccess) t_allocated += (int64_t)bytes;
+  return e;
+}
+
 template <typename T>
 hipError_t dalloc(ane_decoder* d, T** p, size_t n) {
   void* q = nullptr;
-  hipError_t e = hipMalloc(&q, n * sizeof(T) > 0 ? n * sizeof(T) : 16);
+  hipError_t e = device_malloc(&q, n * sizeof(T) > 0 ? n * sizeof(T) : 16);
   if (e != hipSuccess) return e;
   d->allocs.push_back(q);
   *p = (T*)q;
@@ -392,7 +406,7 @@ int room8(ane_decoder* d, const char* op, const ane_kv8_batch& b) {
   if (d->ws8) (void)hipFree(d->ws8);
   d->ws8 = nullptr;
   d->ws8_cap = 0;
-  DCHK(op, hipMalloc(&d->ws8, (size_t)n));
+  DCHK(op, device_malloc(&d->ws8, (size_t)n));
   d->ws8_cap = (size_t)n;
   return ANE_OK;
 }
@@ -1043,6 +1057,12 @@ extern "C" int ane_decode_set_controls(ane_decoder* d, const ane_decode_controls
   d->ctl_mask_rows = c->mask_rows;
   d->controls = true;
   return ANE_OK;
+}
+
+extern "C" int64_t ane_decode_debug_allocs(int32_t first, int32_t count) {
+  t_fail_first = first;
+  t_fail_count = count;
+  return std::exchange(t_allocated, 0);
 }
 
 extern "C" int ane_decode_debug_fail_chain(ane_decoder* d, int32_t step) {

@@ -1082,7 +1082,7 @@ static int debug_fail(const char* what, hipError_t h) {
 
 #define DBGCHK(expr)                                  \
   do {                                                \
-    hipError_t _h = (expr);                           \
+    hipError_t _h = taken(expr);                      \
     if (_h != hipSuccess) { rc = debug_fail(#expr, _h); goto done; } \
   } while (0)
 

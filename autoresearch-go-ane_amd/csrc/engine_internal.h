@@ -275,7 +275,7 @@ int eng_fail(ane_engine* e, int code, const char* fmt, ...);
 
 #define HIPCHK(op, expr)                                                                             \
   do {                                                                                               \
-    hipError_t _h = (expr);                                                                          \
+    hipError_t _h = taken(expr);                                                                     \
     if (_h != hipSuccess) return eng_fail(e, ANE_ERR_HIP, "storiesane %s: %s: %s", op, #expr,        \
                                           hipGetErrorString(_h));                                    \
   } while (0)

@@ -111,7 +111,7 @@ extern "C" int ane_head_loss(const uint16_t* xn, const uint16_t* embed, const ui
   if (rc) return rc;
   const hipStream_t st = (hipStream_t)stream;
   void* ws = nullptr;
-  hipError_t h = hipMalloc(&ws, pl.bytes);
+  hipError_t h = taken(hipMalloc(&ws, pl.bytes));
   if (h != hipSuccess) return op_fail(ANE_ERR_NOMEM, "storiesane %s: hipMalloc(%zu): %s", op, pl.bytes,
                                       hipGetErrorString(h));
   h = head_run(pl, xn, embed, targets, ntok, dim, vocab, seq, softcap, loss_seq, lse, (char*)ws, st);

@@ -24,6 +24,14 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kWave = 64;
 
+// A status that the caller reports or copes with.  A failed HIP call also stays
+// the thread's last error, through calls that succeed, until something reads
+// it; left there it would be reported again by the next launch's check.
+inline hipError_t taken(hipError_t e) {
+  if (e != hipSuccess) (void)hipGetLastError();
+  return e;
+}
+
 __device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);

@@ -247,9 +247,9 @@ inline bool kv8_apart(int64_t rows, int64_t row, int64_t heads, int64_t head, in
 class DeviceScope {
  public:
   explicit DeviceScope(int device) {
-    status_ = hipGetDevice(&before_);
+    status_ = taken(hipGetDevice(&before_));
     if (status_ == hipSuccess && before_ != device) {
-      status_ = hipSetDevice(device);
+      status_ = taken(hipSetDevice(device));
       changed_ = status_ == hipSuccess;
     }
   }

@@ -300,7 +300,7 @@ int mfail(ane_moe* m, int code, const char* fmt, ...) {
 
 #define MCHK(op, expr)                                                                                \
   do {                                                                                                \
-    hipError_t _h = (expr);                                                                           \
+    hipError_t _h = taken(expr);                                                                      \
     if (_h != hipSuccess)                                                                             \
       return mfail(m, ANE_ERR_HIP, "storiesane moe %s: %s: %s", op, #expr, hipGetErrorString(_h));    \
   } while (0)
@@ -359,7 +359,7 @@ extern "C" int ane_moe_open(const ane_moe_cfg* cfg, ane_moe** out) {
   do {
     hipError_t h;
 #define OPEN_CHK(expr)                                                                                 \
-    if ((h = (expr)) != hipSuccess) {                                                                 \
+    if ((h = taken(expr)) != hipSuccess) {                                                            \
       rc = mfail(m, ANE_ERR_HIP, "storiesane moe %s: %s: %s", op, #expr, hipGetErrorString(h));       \
       break;                                                                                          \
     }

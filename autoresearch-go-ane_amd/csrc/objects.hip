@@ -43,7 +43,7 @@ int seam_fail(int code, const char* fmt, ...) {
 
 #define SEAMCHK(op, x)                                                                           \
   do {                                                                                           \
-    hipError_t e_ = (x);                                                                         \
+    hipError_t e_ = taken(x);                                                                    \
     if (e_ != hipSuccess) return seam_fail(ANE_ERR_HIP, "%s: %s", op, hipGetErrorString(e_)); \
   } while (0)
 

@@ -436,6 +436,10 @@ int ane_decode_debug_fill_cache(ane_decoder *d, int byte);
  * Generate call (0 also of a Step call), as after a wait that timed out there;
  * the call is then redone with one launch per GEMM.  Below 0: not. */
 int ane_decode_debug_fail_chain(ane_decoder *d, int32_t step);
+/* Test-only: of the device allocations that decoders make on this thread from
+ * here on, number first .. first + count - 1 (from 0) fail as they do when
+ * memory is out.  Returns the bytes allocated since the call before. */
+int64_t ane_decode_debug_allocs(int32_t first, int32_t count);
 
 /* ---- mixture-of-experts SwiGLU FFN layer ----------------------------------
  * No counterpart in the reference (its FFN is dense, ane/common.go:91-105
