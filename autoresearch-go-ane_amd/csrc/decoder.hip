@@ -104,7 +104,7 @@ struct ane_decoder {
   uint32_t* ctl_mask = nullptr;
   uint16_t* ctl_hist = nullptr;  // [B][max_ctx]
   int *ctl_len = nullptr, *ctl_prompt = nullptr, *ctl_tok = nullptr;
-  void* ctl_ws = nullptr;
+  uint8_t* ctl_ws = nullptr;
   int ctl_mask_rows = 0;
   float* x = nullptr;
   half_t *xn = nullptr, *att = nullptr, *gate = nullptr;
@@ -372,8 +372,8 @@ int generate_run(ane_decoder* d, const char* op, int nsteps, uint16_t* out_tok);
 // A serving operator's failure (its message is the thread's).
 #define SCHK(op, expr)                                                                              \
   do {                                                                                              \
-    const int _r = (int)(expr);                                                                     \
-    if (_r < 0) return dfail(d, _r, "storiesane decode %s: %s", op, ane_op_last_error());           \
+    const int64_t _r = (expr);                                                                      \
+    if (_r < 0) return dfail(d, (int)_r, "storiesane decode %s: %s", op, ane_op_last_error());           \
   } while (0)
 
 void drop_graph(ane_decoder* d) {
@@ -1003,29 +1003,24 @@ extern "C" int ane_decode_set_controls(ane_decoder* d, const ane_decode_controls
   if (d->V > 65535)
     return dfail(d, ANE_ERR_ARG, "storiesane decode set controls: vocab=%d exceeds 65535", d->V);
   DCHK(op, hipSetDevice(d->cfg.device));
-  if (!d->ctl_rows) {
-    float* rows = nullptr;
-    DCHK(op, dalloc(d, &d->ctl_bias, (size_t)d->V));
-    DCHK(op, dalloc(d, &d->ctl_mask, (size_t)B * W));
-    DCHK(op, dalloc(d, &d->ctl_hist, (size_t)B * d->C));
-    DCHK(op, dalloc(d, &d->ctl_len, (size_t)B));
-    DCHK(op, dalloc(d, &d->ctl_prompt, (size_t)B));
-    DCHK(op, dalloc(d, &d->ctl_tok, (size_t)B));
-    uint8_t* ws = nullptr;
-    const int64_t n = ane_control_logits_workspace(B, d->V);
-    SCHK(op, n);
-    DCHK(op, dalloc(d, &ws, (size_t)n));
-    d->ctl_ws = ws;
-    DCHK(op, dalloc(d, &rows, (size_t)3 * kDecRows));
-    d->ctl_rows = rows;  // last: all of them are there
-  }
+  const int64_t ws_bytes = ane_control_logits_workspace(B, d->V);
+  SCHK(op, ws_bytes);
+  // each the first time; what a call that failed got stays for the next
+  if (!d->ctl_rows) DCHK(op, dalloc(d, &d->ctl_rows, (size_t)3 * kDecRows));
+  if (!d->ctl_bias) DCHK(op, dalloc(d, &d->ctl_bias, (size_t)d->V));
+  if (!d->ctl_mask) DCHK(op, dalloc(d, &d->ctl_mask, (size_t)B * W));
+  if (!d->ctl_hist) DCHK(op, dalloc(d, &d->ctl_hist, (size_t)B * d->C));
+  if (!d->ctl_len) DCHK(op, dalloc(d, &d->ctl_len, (size_t)B));
+  if (!d->ctl_prompt) DCHK(op, dalloc(d, &d->ctl_prompt, (size_t)B));
+  if (!d->ctl_tok) DCHK(op, dalloc(d, &d->ctl_tok, (size_t)B));
+  if (!d->ctl_ws) DCHK(op, dalloc(d, &d->ctl_ws, (size_t)ws_bytes));
   ane_logits_args a{};
   a.logits = a.out = d->logits_d;
   a.logits_row = a.out_row = a.vocab = d->V;
   a.device = d->cfg.device;
   a.tokens = d->ctl_tok;
   a.ws = d->ctl_ws;
-  a.ws_bytes = ane_control_logits_workspace(B, d->V);
+  a.ws_bytes = ws_bytes;
   // copies behind whatever the stream still runs, done before the call returns
   HostCopy hc(&d->host_pool, d->cfg.device, d->stream);
   const float* given[3] = {c->repetition, c->frequency, c->presence};

@@ -107,3 +107,31 @@ def test_moe_layer_too_large_to_open():
         m.Run()
     finally:
         m.Close()
+
+
+@pytest.mark.parametrize("first", range(8))
+def test_controls_that_cannot_be_had_leave_nothing_behind(first, fail):
+    """However often setting them fails, what was allocated for them is used by
+    the call that succeeds."""
+    cfg = ane.tiny_decode(vocab=4096)
+    p, prefix, forced = setup(cfg, 2, 64, 1, 96)
+    bias = np.zeros(cfg.vocab, np.float32)
+    bias[77] = 1000
+    dec, other = (ane.Decoder(cfg, p, max_batch=2, max_ctx=128) for _ in range(2))
+    try:
+        fail(0, 0)
+        other.SetControls(bias=bias)
+        want = fail(0, 0)
+        got = 0
+        for _ in range(3):
+            fail(first, 1)
+            with pytest.raises(ane.EngineError, match="out of memory"):
+                dec.SetControls(bias=bias)
+            got += fail(0, 0)
+            first = 0
+        dec.SetControls(bias=bias)
+        assert got + fail(0, 0) == want
+        assert (dec.Prefill(prefix)[0] == 77).all()
+    finally:
+        dec.Close()
+        other.Close()
