@@ -178,6 +178,7 @@ SIGNATURES = {
                                         C.c_int32, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p]),
     "ane_op_last_error": (C.c_char_p, []),
     "ane_decode_open": (C.c_int, [C.POINTER(DecodeCfg), C.POINTER(C.c_void_p)]),
+    "ane_decode_open_cache": (C.c_int, [C.POINTER(DecodeCfg), C.c_int32, C.POINTER(C.c_void_p)]),
     "ane_decode_destroy": (None, [_eng]),
     "ane_decode_last_error": (C.c_char_p, [_eng]),
     "ane_decode_param_count": (C.c_int64, [C.POINTER(DecodeCfg)]),

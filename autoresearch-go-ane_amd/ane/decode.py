@@ -28,7 +28,8 @@ def _f(a):
 class Decoder:
     """Open(cfg, params, max_batch, max_ctx) -> Prefill -> Step / Generate.
 
-    page_tokens: 0 keeps the fp16 cache, 16..256 the paged 8-bit one (SetCache)."""
+    page_tokens: 0 keeps the fp16 cache, 16..256 the paged 8-bit one (SetCache),
+    without the fp16 one ever being allocated."""
 
     def __init__(self, cfg: Config, params, max_batch: int = 64, max_ctx: int = 1152, device: int = 0,
                  page_tokens: int = 0):
@@ -39,7 +40,7 @@ class Decoder:
         self._c = _lib.DecodeCfg(cfg.dim, cfg.hidden, cfg.heads, cfg.kv_heads, cfg.layers, cfg.vocab,
                                  int(max_batch), int(max_ctx), float(cfg.rope_theta), int(device))
         h = C.c_void_p()
-        rc = self._lib.ane_decode_open(C.byref(self._c), C.byref(h))
+        rc = self._lib.ane_decode_open_cache(C.byref(self._c), int(page_tokens), C.byref(h))
         if rc != _lib.ANE_OK:
             msg = self._lib.ane_decode_last_error(h) if h.value else b"storiesane decode open: failed"
             if h.value:
@@ -48,8 +49,6 @@ class Decoder:
         self._h = h
         self.nseq = 0
         try:
-            if page_tokens:
-                self.SetCache(page_tokens)
             self.SetParams(params)
         except Exception:
             self.Close()

@@ -233,7 +233,40 @@ int validate(const ane_decode_cfg& c, std::string* why) {
   return ANE_OK;
 }
 
-int open_impl(ane_decoder* d) {
+bool page_size(int page) { return page >= 16 && page <= 256 && !(page & (page - 1)); }
+
+// the 8-bit cache (use_tail is set by then)
+int alloc8(ane_decoder* d, const char* op, int page) {
+  const int per = (d->C + page - 1) / page;
+  const size_t pages = (size_t)d->L * d->B * per, codes = pages * d->NKV * page * 64;
+  DCHK(op, dalloc(d, &d->k8, codes));
+  DCHK(op, dalloc(d, &d->v8, codes));
+  DCHK(op, dalloc(d, &d->ke8, pages * d->NKV));
+  DCHK(op, dalloc(d, &d->ve8, pages * d->NKV));
+  DCHK(op, dalloc(d, &d->table8, (size_t)d->B * per));
+  DCHK(op, dalloc(d, &d->start8, (size_t)d->B + 1));
+  DCHK(op, dalloc(d, &d->off8, (size_t)d->B + 1));
+  DCHK(op, dalloc(d, &d->qkv8, (size_t)kDecRows * d->N1));
+  if (d->use_tail) {
+    const size_t kept = (size_t)2 * d->L * d->B * d->NKV;
+    DCHK(op, dalloc(d, &d->kept8, kept * page * 64));
+    DCHK(op, dalloc(d, &d->kept_exp8, kept));
+  }
+  // each sequence's pages one after the other
+  DCHK(op, dec_count_up(d->table8, d->B * per, d->stream));
+  d->seq_pages = per;
+  d->page8 = page;
+  return ANE_OK;
+}
+// the fp16 cache
+int alloc16(ane_decoder* d, const char* op) {
+  const size_t cache = (size_t)d->L * d->B * d->NKV * d->C * 64;
+  DCHK(op, dalloc(d, &d->kc, cache));
+  DCHK(op, dalloc(d, &d->vc, cache));
+  return ANE_OK;
+}
+
+int open_impl(ane_decoder* d, int page) {
   const char* op = "open";
   const ane_decode_cfg& c = d->cfg;
   d->D = c.dim; d->H = c.hidden; d->NH = c.heads; d->NKV = c.kv_heads; d->KVD = c.kv_heads * 64;
@@ -255,9 +288,6 @@ int open_impl(ane_decoder* d) {
   DCHK(op, dalloc(d, &d->fw13, (size_t)L * 2 * H * D));
   DCHK(op, dalloc(d, &d->fw2, (size_t)L * D * H));
   DCHK(op, dalloc(d, &d->fembed, (size_t)V * D));
-  const size_t cache = (size_t)L * B * d->NKV * C * 64;
-  DCHK(op, dalloc(d, &d->kc, cache));
-  DCHK(op, dalloc(d, &d->vc, cache));
   // RoPE tables (buildRoPETables, ane/train_util.go:183-202: f64 angle, fp32 cos/sin)
   {
     // to a whole page of any size: the paged cache's positions
@@ -354,6 +384,7 @@ int open_impl(ane_decoder* d) {
       }
     }
   }
+  if (int rc = page ? alloc8(d, op, page) : alloc16(d, op)) return rc;
   DCHK(op, hipDeviceSynchronize());
   return ANE_OK;
 }
@@ -666,6 +697,10 @@ extern "C" int64_t ane_decode_param_count(const ane_decode_cfg* cfg) {
 }
 
 extern "C" int ane_decode_open(const ane_decode_cfg* cfg, ane_decoder** out) {
+  return ane_decode_open_cache(cfg, 0, out);
+}
+
+extern "C" int ane_decode_open_cache(const ane_decode_cfg* cfg, int32_t page_tokens, ane_decoder** out) {
   if (!out) return ANE_ERR_ARG;
   *out = nullptr;
   ane_decoder* d = new ane_decoder();
@@ -674,7 +709,10 @@ extern "C" int ane_decode_open(const ane_decode_cfg* cfg, ane_decoder** out) {
   d->cfg = *cfg;
   std::string why;
   if (validate(*cfg, &why) != ANE_OK) return dfail(d, ANE_ERR_ARG, "storiesane decode open: %s", why.c_str());
-  int rc = open_impl(d);
+  if (page_tokens != 0 && !page_size(page_tokens))
+    return dfail(d, ANE_ERR_ARG, "storiesane decode open: page_tokens=%d must be 0, 16, 32, 64, 128 or 256",
+                 page_tokens);
+  int rc = open_impl(d, page_tokens);
   if (rc != ANE_OK) free_all(d);
   return rc;
 }
@@ -916,39 +954,11 @@ void drop(ane_decoder* d, T** p) {
   *p = nullptr;
 }
 
-int alloc8(ane_decoder* d, const char* op, int page) {
-  const int per = (d->C + page - 1) / page;
-  const size_t pages = (size_t)d->L * d->B * per, codes = pages * d->NKV * page * 64;
-  DCHK(op, dalloc(d, &d->k8, codes));
-  DCHK(op, dalloc(d, &d->v8, codes));
-  DCHK(op, dalloc(d, &d->ke8, pages * d->NKV));
-  DCHK(op, dalloc(d, &d->ve8, pages * d->NKV));
-  DCHK(op, dalloc(d, &d->table8, (size_t)d->B * per));
-  DCHK(op, dalloc(d, &d->start8, (size_t)d->B + 1));
-  DCHK(op, dalloc(d, &d->off8, (size_t)d->B + 1));
-  DCHK(op, dalloc(d, &d->qkv8, (size_t)kDecRows * d->N1));
-  if (d->use_tail) {
-    const size_t kept = (size_t)2 * d->L * d->B * d->NKV;
-    DCHK(op, dalloc(d, &d->kept8, kept * page * 64));
-    DCHK(op, dalloc(d, &d->kept_exp8, kept));
-  }
-  // each sequence's pages one after the other
-  DCHK(op, dec_count_up(d->table8, d->B * per, d->stream));
-  d->seq_pages = per;
-  d->page8 = page;
-  return ANE_OK;
-}
 void free8(ane_decoder* d) {
   drop(d, &d->k8); drop(d, &d->v8); drop(d, &d->ke8); drop(d, &d->ve8);
   drop(d, &d->table8); drop(d, &d->start8); drop(d, &d->off8); drop(d, &d->qkv8);
   drop(d, &d->kept8); drop(d, &d->kept_exp8);
   d->page8 = d->seq_pages = 0;
-}
-int alloc16(ane_decoder* d, const char* op) {
-  const size_t cache = (size_t)d->L * d->B * d->NKV * d->C * 64;
-  DCHK(op, dalloc(d, &d->kc, cache));
-  DCHK(op, dalloc(d, &d->vc, cache));
-  return ANE_OK;
 }
 
 }  // namespace
@@ -956,7 +966,7 @@ int alloc16(ane_decoder* d, const char* op) {
 extern "C" int ane_decode_set_cache(ane_decoder* d, int32_t page_tokens) {
   const char* op = "set cache";
   if (!d || !d->stream) return ANE_ERR_STATE;
-  if (page_tokens != 0 && (page_tokens < 16 || page_tokens > 256 || (page_tokens & (page_tokens - 1))))
+  if (page_tokens != 0 && !page_size(page_tokens))
     return dfail(d, ANE_ERR_ARG, "storiesane decode set cache: page_tokens=%d must be 0, 16, 32, 64, 128 or 256",
                  page_tokens);
   DCHK(op, hipSetDevice(d->cfg.device));

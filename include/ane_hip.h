@@ -370,6 +370,10 @@ typedef struct {
 typedef struct ane_decoder ane_decoder;
 
 int ane_decode_open(const ane_decode_cfg *cfg, ane_decoder **out);
+/* The same with the cache of ane_decode_set_cache's page_tokens from the start:
+ * the paged 8-bit cache without ever holding the fp16 one, for batches and
+ * lengths that fit in 8 bits alone (0: ane_decode_open). */
+int ane_decode_open_cache(const ane_decode_cfg *cfg, int32_t page_tokens, ane_decoder **out);
 void ane_decode_destroy(ane_decoder *d);
 const char *ane_decode_last_error(ane_decoder *d);
 int64_t ane_decode_param_count(const ane_decode_cfg *cfg);
@@ -407,8 +411,9 @@ int32_t ane_decode_fused_chain(ane_decoder *d);
  * fp16 one (as opened), 16..256 (a power of two) the paged 8-bit one of
  * ane_serve.h, half the memory and half the bytes an attention reads; codes of
  * e4m3 with an exponent for each page and head.  Frees the one cache and
- * allocates the other (on failure the old one is allocated again) and drops
- * the active batch: Prefill comes next. */
+ * allocates the other (on failure the old one is allocated again; where that
+ * fails too the decoder is closed) and drops the active batch: Prefill comes
+ * next. */
 int ane_decode_set_cache(ane_decoder *d, int32_t page_tokens);
 /* Controls on the logits before each next token is chosen (no reference
  * counterpart; formulas at ane_control_logits, ane_serve.h), for all later
