@@ -211,6 +211,7 @@ SIGNATURES = {
     "ane_control_logits": (C.c_int, [C.POINTER(LogitsArgs), C.c_void_p]),
     "ane_debug_kv8_item": (C.c_int, [C.POINTER(Kv8Cache), C.POINTER(Kv8Batch), C.c_int32, C.c_int32, C.c_int64,
                                      C.POINTER(C.c_int32)]),
+    "ane_debug_share_memory": (C.c_int, [C.POINTER(C.c_int64), C.POINTER(C.c_int64)]),
     # the per-object seam (include/ane_objects.h)
     "ane_seam_last_error": (C.c_char_p, []),
     "ane_layer_forward_open": (C.c_int, [C.c_int32] * 4 + [C.POINTER(LayerWeights), C.POINTER(C.c_void_p)]),

@@ -213,7 +213,7 @@ class KVCache8:
         """Causal attention of q (fp16 [rows, heads, head_dim], rotated) over
         the cache; the batch's tokens have been appended.  scale: default
         head_dim ** -0.5.  Returns out (new if None: rows of no sequence are
-        then undefined)."""
+        then undefined; may be q)."""
         op = "kv8 attend"
         self._batch(op, batch)
         qp, qr, qh = self._rows(op, "q", q, batch)

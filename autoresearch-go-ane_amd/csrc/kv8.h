@@ -242,6 +242,20 @@ inline bool kv8_apart(int64_t rows, int64_t row, int64_t heads, int64_t head, in
          ((rows == 1 || r >= dh) && (heads == 1 || h >= (rows - 1) * r + dh));
 }
 
+// A tensor of [rows][heads][width], for the question whether two of them share
+// memory.  All in bytes.
+struct Extent {
+  uintptr_t at;
+  int64_t rows, row, heads, head, width;
+};
+// Whether they do.  Rows that lie between another tensor's rows do not.  Exact,
+// but for tensors that lie through each other in different orders and are
+// large, which count as sharing.
+bool share_memory(Extent a, Extent b);
+inline Extent fp16_rows(const void* p, int64_t rows, int64_t row, int64_t heads, int64_t head, int64_t dh) {
+  return {(uintptr_t)p, rows, row * 2, heads, head * 2, dh * 2};
+}
+
 // Makes the cache's device current for a scope (launches go to the current
 // device; the caller's choice comes back).
 class DeviceScope {

@@ -16,6 +16,7 @@
 // before (one token 4.6 us, 64 of them 4.8 in a graph); the rows and their
 // angles are asked for while the page id is under way.
 #include <algorithm>
+#include <utility>
 
 #include "kv8_rows.h"
 #include "op_error.h"
@@ -209,6 +210,55 @@ bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 }  // namespace
 
+namespace {
+
+int64_t floor_div(int64_t x, int64_t y) { return x / y - (x % y < 0); }
+
+// Whether any [i sa, i sa + wa), i < na, meets any [d + j sb, d + j sb + wb), j < nb.
+bool meet(int64_t na, int64_t sa, int64_t wa, int64_t d, int64_t nb, int64_t sb, int64_t wb) {
+  for (int64_t i = 0; i < (sa ? na : 1); i++) {
+    const int64_t lo = i * sa - d - wb, hi = i * sa - d + wa;  // lo < j sb < hi
+    if (sb == 0 ? lo < 0 && hi > 0
+                : std::max<int64_t>(0, floor_div(lo, sb) + 1) <= std::min(nb - 1, -floor_div(-hi, sb) - 1))
+      return true;
+  }
+  return false;
+}
+
+}  // namespace
+
+bool share_memory(Extent a, Extent b) {
+  for (Extent* e : {&a, &b}) {
+    if (e->rows <= 0 || e->heads <= 0 || e->width <= 0) return false;
+    if (e->rows == 1) e->row = 0;
+    if (e->heads == 1) e->head = 0;
+    if (e->head > e->row) {  // the longer stride outside
+      std::swap(e->rows, e->heads);
+      std::swap(e->row, e->head);
+    }
+  }
+  const int64_t ea = (a.heads - 1) * a.head + a.width, eb = (b.heads - 1) * b.head + b.width;  // of a row
+  const int64_t d = (int64_t)(b.at - a.at);
+  if (d >= (a.rows - 1) * a.row + ea || -d >= (b.rows - 1) * b.row + eb) return false;
+  int64_t left = 1 << 20;  // comparisons
+  // rows j of b that reach over row i of a: lo < j b.row < hi; with equal strides they depend on j - i alone
+  const bool same = a.row == b.row && a.row > 0;
+  for (int64_t i = 0; i < (a.row && !same ? a.rows : 1); i++) {
+    const int64_t lo = i * a.row - d - eb, hi = i * a.row - d + ea;
+    int64_t j0 = same ? 1 - a.rows : 0, j1 = b.row ? b.rows - 1 : 0;
+    if (b.row) {
+      j0 = std::max(j0, floor_div(lo, b.row) + 1);
+      j1 = std::min(j1, -floor_div(-hi, b.row) - 1);
+    }
+    for (int64_t j = j0; j <= j1; j++) {
+      if ((left -= a.heads) < 0) return true;
+      if (meet(a.heads, a.head, a.width, d + j * b.row - i * a.row, b.heads, b.head, b.width)) return true;
+    }
+    if (--left < 0) return true;
+  }
+  return false;
+}
+
 int kv8_check(const char* op, const ane_kv8_cache* c, const ane_kv8_batch* b, Kv8Batch* out) {
   if (!c || !b) return op_fail(ANE_ERR_ARG, "storiesane %s: no cache or batch", op);
   if (!c->k || !c->v || !c->k_exp || !c->v_exp) return op_fail(ANE_ERR_ARG, "storiesane %s: null cache buffer", op);
@@ -278,6 +328,13 @@ int ane::kv8_append_check(const char* op, const ane_kv8_cache* cache, const ane_
     return op_fail(ANE_ERR_ARG, "storiesane %s: rows of q_out overlap", op);
   if (g.heads > 0 && g.q == g.q_out && (g.q_row != g.q_out_row || g.q_head != g.q_out_head))
     return op_fail(ANE_ERR_ARG, "storiesane %s: q_out is q with other strides", op);
+  if (g.heads > 0 && !from) {
+    const Extent out = fp16_rows(g.q_out, a.b.rows, g.q_out_row, g.heads, g.q_out_head, cache->head_dim);
+    if ((g.q != g.q_out && share_memory(out, fp16_rows(g.q, a.b.rows, g.q_row, g.heads, g.q_head, cache->head_dim))) ||
+        share_memory(out, fp16_rows(g.k, a.b.rows, g.k_row, a.b.NKV, g.k_head, cache->head_dim)) ||
+        share_memory(out, fp16_rows(g.v, a.b.rows, g.v_row, a.b.NKV, g.v_head, cache->head_dim)))
+      return op_fail(ANE_ERR_ARG, "storiesane %s: q_out overlaps q, k or v", op);
+  }
   a.k = (uint8_t*)cache->k; a.v = (uint8_t*)cache->v; a.k_exp = cache->k_exp; a.v_exp = cache->v_exp;
   a.xq = (const half_t*)g.q; a.xk = (const half_t*)g.k; a.xv = (const half_t*)g.v; a.q_out = (half_t*)g.q_out;
   a.cos = g.cos; a.sin = g.sin;
@@ -322,6 +379,10 @@ int ane::kv8_append(const ane_kv8_cache* cache, const ane_kv8_batch* batch, cons
   const hipError_t h = hipGetLastError();
   if (h != hipSuccess) return op_fail(ANE_ERR_HIP, "storiesane %s: %s", op, hipGetErrorString(h));
   return ANE_OK;
+}
+
+extern "C" int ane_debug_share_memory(const int64_t* a, const int64_t* b) {
+  return share_memory({(uintptr_t)a[0], a[1], a[2], a[3], a[4], a[5]}, {(uintptr_t)b[0], b[1], b[2], b[3], b[4], b[5]});
 }
 
 extern "C" int ane_debug_kv8_item(const ane_kv8_cache* cache, const ane_kv8_batch* batch, int32_t tile_tokens,

@@ -728,6 +728,10 @@ int attend(const ane_kv8_cache* cache, const ane_kv8_batch* batch, const ane_kv8
     return op_fail(ANE_ERR_ARG, "storiesane %s: rows=%d of fragments, want at most %d", op, a.b.rows, kDecRows);
   if (!frag && !kv8_apart(a.b.rows, g.out_row, g.heads, g.out_head, cache->head_dim))
     return op_fail(ANE_ERR_ARG, "storiesane %s: rows of out overlap", op);
+  const bool same = (const void*)g.q == g.out && g.q_row == g.out_row && g.q_head == g.out_head;
+  if (!frag && !same && share_memory(fp16_rows(g.q, a.b.rows, g.q_row, g.heads, g.q_head, cache->head_dim),
+                                     fp16_rows(g.out, a.b.rows, g.out_row, g.heads, g.out_head, cache->head_dim)))
+    return op_fail(ANE_ERR_ARG, "storiesane %s: out overlaps q with other strides, or in part", op);
   if (p.bytes > 0 && (!g.ws || g.ws_bytes < p.bytes))
     return op_fail(ANE_ERR_ARG, "storiesane %s: workspace of %lld bytes, want %lld", op,
                    (long long)(g.ws ? g.ws_bytes : 0), (long long)p.bytes);

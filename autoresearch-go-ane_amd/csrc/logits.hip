@@ -297,6 +297,10 @@ extern "C" int ane_control_logits(const ane_logits_args* args, void* stream) {
   if (g.out == g.logits && g.out_row != g.logits_row)
     return op_fail(ANE_ERR_ARG, "storiesane %s: in place, but out_row=%lld and logits_row=%lld", op,
                    (long long)g.out_row, (long long)g.logits_row);
+  if (g.out && g.out != g.logits &&
+      share_memory({(uintptr_t)g.out, g.rows, g.out_row * 4, 1, 0, g.vocab * 4},
+                   {(uintptr_t)g.logits, g.rows, g.logits_row * 4, 1, 0, g.vocab * 4}))
+    return op_fail(ANE_ERR_ARG, "storiesane %s: out overlaps logits in part", op);
   LogitsArgs a;
   a.chunks = chunks_of(g.rows, g.vocab);
   const int64_t need = a.chunks > 1 && g.tokens ? (int64_t)g.rows * a.chunks * 8 : 0;

@@ -84,7 +84,8 @@ typedef struct ane_kv8_batch {
  *
  * q, k, v, q_out: fp16, [rows][heads or kv_heads][head_dim] with element
  * strides between rows and heads; 16-byte aligned, strides multiples of 8.
- * q_out may be q itself (same strides).  heads = 0: keys and values only.
+ * q_out may be q itself (same strides), and shares no memory with q, k and v
+ * otherwise.  heads = 0: keys and values only.
  * cos, sin: fp32 [positions][head_dim / 2], 16-byte aligned, positions >=
  * table_pages * page_tokens. */
 typedef struct ane_kv8_append_args {
@@ -106,7 +107,8 @@ int ane_kv8_append(const ane_kv8_cache *cache, const ane_kv8_batch *batch, const
  * rows that attend to it and no other.
  *
  * q, out: fp16 [rows][heads][head_dim], 16-byte aligned, strides multiples of
- * 8; they do not overlap.  scale finite and > 0; heads / kv_heads at most 32.
+ * 8; out may be q itself (same strides), and shares no memory with it
+ * otherwise.  scale finite and > 0; heads / kv_heads at most 32.
  * ws: ane_kv8_attend_workspace() bytes of device memory, 16-byte aligned (NULL
  * when that is 0); its contents need not be set, and calls that may overlap
  * need one each. */
@@ -137,7 +139,8 @@ int ane_kv8_attend(const ane_kv8_cache *cache, const ane_kv8_batch *batch, const
  * chosen; ANE_NO_TOKEN where nothing is above -inf).
  *
  * logits, out: fp32 [rows][vocab] with row strides; out may be logits itself
- * (same stride) or NULL (tokens only).  history: uint16 [rows][history_row],
+ * (same stride) or NULL (tokens only), and shares no memory with it otherwise
+ * (rows of one may lie between the other's).  history: uint16 [rows][history_row],
  * ids from vocab on are passed over; lengths are taken within [0,
  * history_max], prompts within [0, lengths[r]] (NULL: 0).  repetition,
  * frequency, presence: fp32 [rows] or NULL (1, 0, 0); they need a history (NULL
@@ -174,6 +177,12 @@ int ane_control_logits(const ane_logits_args *args, void *stream);
  * No GPU is used. */
 int ane_debug_kv8_item(const ane_kv8_cache *cache, const ane_kv8_batch *batch, int32_t tile_tokens, int32_t pages,
                        int64_t item, int32_t *out);
+
+/* Whether two tensors [rows][heads][width] share memory, as the operators ask
+ * before they refuse an output that overlaps an input: each given as {address,
+ * rows, stride of rows, heads, stride of heads, width}, in bytes.  No GPU is
+ * used. */
+int ane_debug_share_memory(const int64_t *a, const int64_t *b);
 
 #ifdef __cplusplus
 }
