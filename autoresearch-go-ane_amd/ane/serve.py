@@ -226,8 +226,11 @@ class KVCache8:
         if n is None:
             n = batch._ws[key] = _check(self._lib, self._lib.ane_kv8_attend_workspace(self._c, batch._c, heads))
         ws = self._empty(n, dtype=self._u8, device=self.device) if n else None
-        a = _lib.pack_attend(qp, yp, qr, qh, yr, yh, heads, self.head_dim ** -0.5 if scale is None else scale,
-                             0 if ws is None else ws.data_ptr(), n)
+        try:
+            a = _lib.pack_attend(qp, yp, qr, qh, yr, yh, heads, self.head_dim ** -0.5 if scale is None else scale,
+                                 0 if ws is None else ws.data_ptr(), n)
+        except (OverflowError, _lib.struct.error):
+            _fail(op, f"scale={scale} is no fp32 number")
         rc = self._attend(self._at, batch._at, a, self._stream(self._index))
         if rc:
             _check(self._lib, rc)

@@ -719,8 +719,10 @@ int attend(const ane_kv8_cache* cache, const ane_kv8_batch* batch, const ane_kv8
       return op_fail(ANE_ERR_ARG, "storiesane %s: stride %lld must be a multiple of 8", op, (long long)s);
   if (!aligned16(g.q) || !aligned16(g.out) || !aligned16(g.ws))
     return op_fail(ANE_ERR_ARG, "storiesane %s: buffers must be 16-byte aligned", op);
-  if (!(g.scale > 0.f) || !std::isfinite(g.scale))
-    return op_fail(ANE_ERR_ARG, "storiesane %s: scale=%g must be positive and finite", op, (double)g.scale);
+  const float c = g.scale * 1.44269504088896340736f;  // log2(e)
+  if (!(g.scale > 0.f) || !std::isfinite(c))
+    return op_fail(ANE_ERR_ARG, "storiesane %s: scale=%g must be positive and finite, times log2(e) too", op,
+                   (double)g.scale);
   Plan p;
   rc = plan(op, a.b, *batch, cache->head_dim, g.heads, &p);
   if (rc) return rc;
@@ -743,7 +745,7 @@ int attend(const ane_kv8_cache* cache, const ane_kv8_batch* batch, const ane_kv8
   a.q_row = g.q_row; a.q_head = g.q_head; a.out_row = g.out_row; a.out_head = g.out_head;
   a.G = g.heads / a.b.NKV; a.tt = p.tt; a.tiles = (int)p.tiles; a.nsplit = p.nsplit; a.round = p.round;
   a.longest = p.longest;
-  a.c = g.scale * 1.44269504088896340736f;
+  a.c = c;
   a.part = (float*)g.ws;
   a.ml = (float2*)(a.part + (size_t)p.tiles * a.b.NKV * p.nsplit * p.tt * a.G * cache->head_dim);
   a.frag = frag;

@@ -108,7 +108,8 @@ int ane_kv8_append(const ane_kv8_cache *cache, const ane_kv8_batch *batch, const
  *
  * q, out: fp16 [rows][heads][head_dim], 16-byte aligned, strides multiples of
  * 8; out may be q itself (same strides), and shares no memory with it
- * otherwise.  scale finite and > 0; heads / kv_heads at most 32.
+ * otherwise.  scale > 0, and finite times log2(e) in fp32; heads / kv_heads at
+ * most 32.
  * ws: ane_kv8_attend_workspace() bytes of device memory, 16-byte aligned (NULL
  * when that is 0); its contents need not be set, and calls that may overlap
  * need one each. */
