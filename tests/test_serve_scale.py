@@ -1,5 +1,6 @@
 """Scales of the attention that cannot be used are refused in the operator's own
 manner, whatever kind of number they are."""
+import ctypes as C
 import types
 
 import pytest
@@ -36,7 +37,9 @@ def test_scale_that_is_no_fp32_number(scale):
     c = serve.KVCache8.__new__(serve.KVCache8)
     c._lib, c.device, c.kv_heads, c.page_tokens, c.head_dim = lib, "cuda:0", 2, 16, 64
     c._rows = lambda op, name, t, batch, heads=None: (t.data_ptr(), *t.stride()[:2])
-    b = types.SimpleNamespace(device="cuda:0", rows=5, _ws={(2, 16, 64, 4): 0}, _at=0)
+    held = cache(), batch()
+    c._at, c._attend, c._stream, c._index = C.addressof(held[0]), _lib.plain(lib, "ane_kv8_attend"), lambda i: None, 0
+    b = types.SimpleNamespace(device="cuda:0", rows=5, _ws={(2, 16, 64, 4): 0}, _at=C.addressof(held[1]))
     t = FakeTensor(5, 4, 64)
     with pytest.raises(ane.EngineError, match="scale="):
         c.Attend(b, t, t, scale)
