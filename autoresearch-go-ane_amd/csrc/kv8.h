@@ -212,7 +212,8 @@ __device__ __forceinline__ int kv8_exponent(uint32_t amax_bits) {
 int kv8_check(const char* op, const ane_kv8_cache* c, const ane_kv8_batch* b, Kv8Batch* out);
 
 // Rows q | k | v of the decoder's product as its fp32 sums [splits][kDecRows][n]
-// (added, times row_scale if there is one); a set *err: nothing is done.
+// (added, times row_scale if there is one).  A set *err: nothing is appended (a
+// step then attends over what is there; its outputs are redone).
 struct Kv8Sums {
   const float* part = nullptr;
   int splits = 0, n = 0;

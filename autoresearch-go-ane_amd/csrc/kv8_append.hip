@@ -13,7 +13,7 @@
 // prompts, 18,000 tokens, 12 / 4 heads of 64: 100 MB in 22.8 us, 4.4 TB/s).
 // Single tokens, which a wave per page and head takes: a chain of loads,
 // offsets, page id, rows, old exponent and codes, each waiting for the one
-// before (one token 4.6 us, 64 of them 4.8 in a graph); the rows and their
+// before (one token 4.3 us, 64 of them 4.5 in a graph); the rows and their
 // angles are asked for while the page id is under way.
 #include <algorithm>
 #include <utility>

@@ -20,9 +20,9 @@
 // sequences of up to 40,000 tokens, 2 heads of 128: 494 MB in 108 us, 4.6 TB/s,
 // where a large copy has 5.1).  Single tokens over short contexts: the chain
 // launch, offsets, page table, first loads, meeting (one sequence of 777 tokens
-// 6.5 us, 64 of 1100 10.1).  Prompts: the vector instructions around the
+// 6.7 us, 64 of 1100 10.1, in a graph).  Prompts: the vector instructions around the
 // products, about 150 for 32 keys and 48 rows where the products are 24 MFMAs,
-// with the vector units 78 % busy (one of 8192 tokens, 12 heads of 64: 121 us,
+// with the vector units 77 % busy (one of 8192 tokens, 12 heads of 64: 121 us,
 // 850 TFLOP/s).
 #include <algorithm>
 #include <type_traits>

@@ -36,8 +36,9 @@ extern "C" {
  *          and dimension d of a page at [s/16][s%16/4][d%16][d/16][s%4] (the
  *          order in which the matrix cores take it)
  *   k_exp, v_exp [pages][kv_heads]
- * page_tokens: 16, 32, 64, 128 or 256; head_dim: 64 or 128.  k and v are
- * 16-byte aligned. */
+ * page_tokens: 16, 32, 64, 128 or 256; head_dim: 64 or 128; kv_heads at most
+ * 1024.  k and v are 16-byte aligned.  Pages that no call has written may hold
+ * anything, exponents too. */
 typedef struct ane_kv8_cache {
   void *k, *v;
   int8_t *k_exp, *v_exp;
@@ -50,6 +51,7 @@ typedef struct ane_kv8_cache {
  * at position start[i] (the tokens it holds already); position p is row
  * p % page_tokens of page table[i][p / page_tokens].  All on the device.
  *
+ * At most 65536 sequences, 2^30 rows and 2^30 tokens of a table's row.
  * offsets rise from 0 to at most `rows`; a sequence may have no new rows.
  * What lies outside is not followed: offsets are taken within [0, rows],
  * positions from table_pages * page_tokens on are not taken (their rows belong
@@ -80,12 +82,13 @@ typedef struct ane_kv8_batch {
  * not this call's), the exponent is at least the old one, and if it rises, the
  * rows before are rounded again from their codes.  Codes are rounded to
  * nearest, ties to even; at exponent 8 they end at +-240, fp16's range.
- * A page may get rows of one sequence only in a call.
+ * A page may get rows of one sequence only in a call, from one place of its
+ * table.
  *
  * q, k, v, q_out: fp16, [rows][heads or kv_heads][head_dim] with element
  * strides between rows and heads; 16-byte aligned, strides multiples of 8.
  * q_out may be q itself (same strides), and shares no memory with q, k and v
- * otherwise.  heads = 0: keys and values only.
+ * otherwise.  heads = 0: keys and values only; at most 32768.
  * cos, sin: fp32 [positions][head_dim / 2], 16-byte aligned, positions >=
  * table_pages * page_tokens. */
 typedef struct ane_kv8_append_args {
@@ -148,7 +151,8 @@ int ane_kv8_attend(const ane_kv8_cache *cache, const ane_kv8_batch *batch, const
  * with lengths and history_max = 0: an empty one).  bias: fp32, row stride
  * bias_row (0: one row for all), or NULL.  mask: uint32 words, bit v % 32 of
  * word v / 32, row stride mask_row (0: one for all), or NULL.  tokens: int32
- * [rows] or NULL.  vocab 1..65535.  ws as above. */
+ * [rows] or NULL.  vocab 1..65535, rows at most 65535.  ws as
+ * above. */
 enum { ANE_NO_TOKEN = 65535 };
 typedef struct ane_logits_args {
   const float *logits;
