@@ -208,7 +208,7 @@ struct SeamBase {
   template <typename T>
   hipError_t alloc(T** p, size_t n) {
     void* q = nullptr;
-    hipError_t h = hipMalloc(&q, std::max<size_t>(n * sizeof(T), 256));
+    hipError_t h = taken(hipMalloc(&q, std::max<size_t>(n * sizeof(T), 256)));
     if (h != hipSuccess) return h;
     allocs.push_back(q);
     *p = (T*)q;
@@ -480,7 +480,7 @@ extern "C" int ane_layer_forward_open(int32_t dim, int32_t hidden, int32_t heads
   if (h == hipSuccess) h = f->alloc(&f->gate, HS);
   if (h == hipSuccess) h = f->alloc(&f->h1, HS);
   if (h == hipSuccess) h = stage_layer(f, &f->w, w, dim, hidden);
-  if (h != hipSuccess) {
+  if (taken(h) != hipSuccess) {
     f->release();
     delete f;
     return seam_fail(h == hipErrorOutOfMemory ? ANE_ERR_NOMEM : ANE_ERR_HIP, "%s: %s", op, hipGetErrorString(h));
@@ -578,7 +578,7 @@ extern "C" int ane_layer_backward_open(int32_t dim, int32_t hidden, int32_t head
   if (h == hipSuccess) h = b->alloc(&b->h1, HS);
   if (h == hipSuccess) h = b->alloc(&b->dh1, HS);
   if (h == hipSuccess) h = stage_layer(b, &b->w, w, dim, hidden);
-  if (h != hipSuccess) {
+  if (taken(h) != hipSuccess) {
     b->release();
     delete b;
     return seam_fail(h == hipErrorOutOfMemory ? ANE_ERR_NOMEM : ANE_ERR_HIP, "%s: %s", op, hipGetErrorString(h));
@@ -806,7 +806,7 @@ extern "C" int ane_offload_open(int32_t vocab, int32_t dim, int32_t seq, const f
     if (h == hipSuccess && o->bwd_splits > 1) h = o->alloc(&o->ws, (size_t)o->bwd_splits * DS);
     if (h == hipSuccess) h = stage_embed(o, embed);
   }
-  if (h != hipSuccess) {
+  if (taken(h) != hipSuccess) {
     o->release();
     delete o;
     return seam_fail(h == hipErrorOutOfMemory ? ANE_ERR_NOMEM : ANE_ERR_HIP, "%s: %s", op, hipGetErrorString(h));

@@ -135,3 +135,27 @@ def test_controls_that_cannot_be_had_leave_nothing_behind(first, fail):
     finally:
         dec.Close()
         other.Close()
+
+
+@pytest.mark.parametrize("which", ["forward", "backward", "offload"])
+def test_seam_object_too_large_to_open(which):
+    """Weights of 412 GB (dim 2^18) or an embedding of 4 TB: refused by
+    the allocator; a small object opens behind it."""
+    lib = _lib.load()
+    C = _lib.C
+
+    def open_(dim, hidden, heads, seq, vocab, w):
+        h = C.c_void_p()
+        p = w.ctypes.data_as(C.POINTER(C.c_float))
+        if which == "offload":
+            rc = lib.ane_offload_open(vocab, dim, seq, p, 0, C.byref(h))
+        else:
+            lw = _lib.LayerWeights(*[p] * 6)
+            rc = getattr(lib, f"ane_layer_{which}_open")(dim, hidden, heads, seq, C.byref(lw), C.byref(h))
+        return rc, h
+    w = np.zeros(1 << 16, np.float32)      # never read by the first call
+    rc, h = open_(1 << 18, 64, 1 << 12, 64, 1 << 23, w)
+    assert rc == _lib.ANE_ERR_NOMEM and not h.value, lib.ane_seam_last_error()
+    rc, h = open_(64, 64, 1, 64, 512, w)
+    assert rc == _lib.ANE_OK, lib.ane_seam_last_error()
+    getattr(lib, "ane_offload_destroy" if which == "offload" else f"ane_layer_{which}_destroy")(h)
