@@ -119,6 +119,50 @@ class LogitsArgs(C.Structure):
         ("ws", C.c_void_p), ("ws_bytes", C.c_int64)]
 
 
+class BeamArgs(C.Structure):
+    """ane_beam_args (include/ane_serve.h)."""
+    _fields_ = [(n, C.c_void_p) for n in ("logits", "scores", "weights", "finished", "tokens", "parents", "scores_out",
+                                          "finished_out", "history", "lengths")] + [
+        (n, C.c_int64) for n in ("logits_row", "history_row")] + [
+        (n, C.c_int32) for n in ("requests", "beams", "vocab", "eos", "history_max", "half", "device")] + [
+        ("ws", C.c_void_p), ("ws_bytes", C.c_int64)]
+
+
+class Kv8Bounds(C.Structure):
+    """ane_kv8_bounds (include/ane_serve.h)."""
+    _fields_ = [("box", C.c_void_p), ("unit", C.c_void_p)]
+
+
+class Kv8SelectArgs(C.Structure):
+    """ane_kv8_select_args (include/ane_serve.h)."""
+    _fields_ = [("q", C.c_void_p), ("blocks", C.c_void_p), ("q_row", C.c_int64), ("q_head", C.c_int64)] + [
+        (n, C.c_int32) for n in ("heads", "count", "first", "recent")] + [("ws", C.c_void_p), ("ws_bytes", C.c_int64)]
+
+
+class Kv8Pool(C.Structure):
+    """ane_kv8_pool (include/ane_serve.h)."""
+    _fields_ = [("layers", C.POINTER(Kv8Cache)), ("bounds", C.POINTER(Kv8Bounds)), ("refs", C.c_void_p),
+                ("nlayers", C.c_int32)]
+
+
+class Kv8ForkArgs(C.Structure):
+    """ane_kv8_fork_args (include/ane_serve.h)."""
+    _fields_ = [(n, C.c_void_p) for n in ("table", "start", "parents", "news", "missing")] + [
+        (n, C.c_int32) for n in ("table_stride", "table_pages", "nseq", "new_tokens")] + [
+        ("ws", C.c_void_p), ("ws_bytes", C.c_int64)]
+
+
+class Kv8CompactArgs(C.Structure):
+    """ane_kv8_compact_args (include/ane_serve.h)."""
+    _fields_ = [("table", C.c_void_p), ("moved", C.c_void_p)] + [
+        (n, C.c_int32) for n in ("table_stride", "table_pages", "nseq")] + [("ws", C.c_void_p), ("ws_bytes", C.c_int64)]
+
+
+class Kv8CopyArgs(C.Structure):
+    """ane_kv8_copy_args (include/ane_serve.h)."""
+    _fields_ = [("src", C.c_void_p), ("dst", C.c_void_p), ("tokens", C.c_void_p), ("n", C.c_int32)]
+
+
 class ProfEntry(C.Structure):
     _fields_ = [("launches", C.c_int64), ("ms", C.c_double), ("flops", C.c_double), ("bytes", C.c_double)]
 
@@ -209,6 +253,20 @@ SIGNATURES = {
     "ane_kv8_attend": (C.c_int, [C.POINTER(Kv8Cache), C.POINTER(Kv8Batch), C.POINTER(Kv8AttendArgs), C.c_void_p]),
     "ane_control_logits_workspace": (C.c_int64, [C.c_int32, C.c_int32]),
     "ane_control_logits": (C.c_int, [C.POINTER(LogitsArgs), C.c_void_p]),
+    "ane_beam_select_workspace": (C.c_int64, [C.c_int32] * 4),
+    "ane_beam_select": (C.c_int, [C.POINTER(BeamArgs), C.c_void_p]),
+    "ane_kv8_bound": (C.c_int, [C.POINTER(Kv8Cache), C.POINTER(Kv8Bounds), C.POINTER(Kv8Batch), C.c_void_p]),
+    "ane_kv8_select_workspace": (C.c_int64, [C.POINTER(Kv8Cache), C.POINTER(Kv8Batch), C.c_int32, C.c_int32]),
+    "ane_kv8_select": (C.c_int, [C.POINTER(Kv8Cache), C.POINTER(Kv8Bounds), C.POINTER(Kv8Batch),
+                                 C.POINTER(Kv8SelectArgs), C.c_void_p]),
+    "ane_kv8_attend_blocks_workspace": (C.c_int64, [C.POINTER(Kv8Cache), C.POINTER(Kv8Batch), C.c_int32, C.c_int32]),
+    "ane_kv8_attend_blocks": (C.c_int, [C.POINTER(Kv8Cache), C.POINTER(Kv8Batch), C.POINTER(Kv8AttendArgs),
+                                        C.c_void_p, C.c_int32, C.c_void_p]),
+    "ane_kv8_fork_workspace": (C.c_int64, [C.POINTER(Kv8Pool), C.c_int32, C.c_int32]),
+    "ane_kv8_fork": (C.c_int, [C.POINTER(Kv8Pool), C.POINTER(Kv8ForkArgs), C.c_void_p]),
+    "ane_kv8_compact_workspace": (C.c_int64, [C.POINTER(Kv8Pool)]),
+    "ane_kv8_compact": (C.c_int, [C.POINTER(Kv8Pool), C.POINTER(Kv8CompactArgs), C.c_void_p]),
+    "ane_kv8_copy": (C.c_int, [C.POINTER(Kv8Pool), C.POINTER(Kv8Pool), C.POINTER(Kv8CopyArgs), C.c_void_p]),
     "ane_debug_kv8_item": (C.c_int, [C.POINTER(Kv8Cache), C.POINTER(Kv8Batch), C.c_int32, C.c_int32, C.c_int64,
                                      C.POINTER(C.c_int32)]),
     "ane_debug_share_memory": (C.c_int, [C.POINTER(C.c_int64), C.POINTER(C.c_int64)]),
@@ -246,6 +304,11 @@ SIGNATURES = {
 pack_append = struct.Struct("6P8q2i").pack    # Kv8AppendArgs
 pack_attend = struct.Struct("2P4qifPq").pack  # Kv8AttendArgs
 pack_logits = struct.Struct("11P5q4iPq").pack  # LogitsArgs
+pack_beam = struct.Struct("10P2q7iPq").pack    # BeamArgs
+pack_select = struct.Struct("2P2q4iPq").pack   # Kv8SelectArgs
+pack_fork = struct.Struct("5P4iPq").pack       # Kv8ForkArgs
+pack_compact = struct.Struct("2P3iPq").pack    # Kv8CompactArgs
+pack_copy = struct.Struct("3Pi4x").pack        # Kv8CopyArgs
 
 
 def plain(lib, name):
@@ -253,7 +316,7 @@ def plain(lib, name):
     nothing to convert."""
     fn = lib[name]
     fn.restype, args = SIGNATURES[name]
-    fn.argtypes = [C.c_void_p] * len(args)
+    fn.argtypes = [t if t is C.c_int32 else C.c_void_p for t in args]
     return fn
 
 

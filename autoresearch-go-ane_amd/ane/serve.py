@@ -4,7 +4,9 @@
 batch's new queries and keys and writes its keys and values, ``Attend`` is the
 causal attention of its queries over the cache, for prompts, chunks of prompts
 and single tokens.  ``LogitControls`` changes logits by the requests'
-penalties, biases and masks and picks the next tokens.
+penalties, biases and masks and picks the next tokens.  ``BeamSearch`` picks
+them for several beams a request; the tables of the pages and the choice of
+pages in long contexts are in ``pages.py``.
 
 All tensors are torch tensors on one GPU.  Calls run on torch's current stream
 of that GPU, wait for nothing and can be captured into a graph.  What they need
@@ -140,7 +142,8 @@ class KVCache8:
         self._empty, self._u8, self._stream = torch.empty, torch.uint8, _stream_getter()
         self._c = _lib.Kv8Cache(kp, vp, ke, ve, pages, page, kvh, dh, dev.index)
         self._at = C.addressof(self._c)
-        self._append, self._attend = (_lib.plain(self._lib, "ane_kv8_" + n) for n in ("append", "attend"))
+        self._append, self._attend, self._attend_blocks = (_lib.plain(self._lib, "ane_kv8_" + n)
+                                                           for n in ("append", "attend", "attend_blocks"))
 
     @classmethod
     def Empty(cls, pages, kv_heads, head_dim=64, page_tokens=64, device="cuda"):
@@ -159,7 +162,7 @@ class KVCache8:
             r, h, d = t.shape
             sr, sh, sd = t.stride()
             if (t.dtype is self._half and t.get_device() == self._index and r == batch.rows and d == self.head_dim
-                    and sd == 1 and (heads is None or h == heads)):
+                    and (sd == 1 or r == 0) and (heads is None or h == heads)):
                 return t.data_ptr(), sr if r > 1 else 0, sh if h > 1 else 0
         except (AttributeError, ValueError):
             pass
@@ -209,11 +212,13 @@ class KVCache8:
             _check(self._lib, rc)
         return q_out
 
-    def Attend(self, batch, q, out=None, scale=None):
+    def Attend(self, batch, q, out=None, scale=None, blocks=None):
         """Causal attention of q (fp16 [rows, heads, head_dim], rotated) over
         the cache; the batch's tokens have been appended.  scale: default
-        head_dim ** -0.5.  Returns out (new if None: rows of no sequence are
-        then undefined; may be q)."""
+        head_dim ** -0.5.  blocks int32 [rows, kv_heads, count]: only the keys
+        of the pages at these places of each row's table (KVBounds.Select;
+        places that are none, -1 among them, take no part).  Returns out (new
+        if None: rows of no sequence are then undefined; may be q)."""
         op = "kv8 attend"
         self._batch(op, batch)
         qp, qr, qh = self._rows(op, "q", q, batch)
@@ -221,20 +226,37 @@ class KVCache8:
         if out is None:
             out = self._new(batch, heads)
         yp, yr, yh = self._rows(op, "out", out, batch, heads)
-        key = (self.kv_heads, self.page_tokens, self.head_dim, heads)
+        bp = count = 0
+        if blocks is not None:
+            bp, count = self._blocks(op, blocks, batch)
+        key = (self.kv_heads, self.page_tokens, self.head_dim, heads, count)
         n = batch._ws.get(key)
         if n is None:
-            n = batch._ws[key] = _check(self._lib, self._lib.ane_kv8_attend_workspace(self._c, batch._c, heads))
+            if blocks is None:
+                n = self._lib.ane_kv8_attend_workspace(self._c, batch._c, heads)
+            else:
+                n = self._lib.ane_kv8_attend_blocks_workspace(self._c, batch._c, heads, count)
+            batch._ws[key] = _check(self._lib, n)
         ws = self._empty(n, dtype=self._u8, device=self.device) if n else None
         try:
             a = _lib.pack_attend(qp, yp, qr, qh, yr, yh, heads, self.head_dim ** -0.5 if scale is None else scale,
                                  0 if ws is None else ws.data_ptr(), n)
         except (OverflowError, _lib.struct.error):
             _fail(op, f"scale={scale} is no fp32 number")
-        rc = self._attend(self._at, batch._at, a, self._stream(self._index))
+        if blocks is None:
+            rc = self._attend(self._at, batch._at, a, self._stream(self._index))
+        else:
+            rc = self._attend_blocks(self._at, batch._at, a, bp, count, self._stream(self._index))
         if rc:
             _check(self._lib, rc)
         return out
+
+    def _blocks(self, op, t, batch):
+        """(address, count) of int32 [rows, kv_heads, count]."""
+        _whole(op, "blocks", t, (_torch().int32,), self.device, dims=3)
+        if tuple(t.shape[:2]) != (batch.rows, self.kv_heads):
+            _fail(op, f"blocks has shape {tuple(t.shape)}, want ({batch.rows}, {self.kv_heads}, count)")
+        return t.data_ptr(), int(t.shape[2])
 
 
 class LogitControls:
@@ -354,3 +376,90 @@ class LogitControls:
         if t.dtype is self._i32[0] and t.get_device() == index and t.shape == (rows,) and t.is_contiguous():
             return t.data_ptr()
         return _whole(self._op, name, t, self._i32, _torch().device("cuda", index), shape=(rows,))
+
+
+class BeamSearch:
+    """Requests with ``beams`` beams each over ``vocab`` tokens; row r =
+    request * beams + beam.  eos: the token that finishes a beam (None: none
+    does)."""
+
+    def __init__(self, vocab, beams, eos=None):
+        torch = _torch()
+        self._op = "beam select"
+        self.vocab, self.beams, self.eos = int(vocab), int(beams), None if eos is None else int(eos)
+        self._lib = _lib.load()
+        _check(self._lib, self._lib.ane_beam_select_workspace(0, self.beams, self.vocab, 0))
+        if eos is not None and not 0 <= self.eos < self.vocab:
+            _fail(self._op, f"eos={eos} of vocab={vocab}")
+        self._empty, self._u8, self._stream = torch.empty, torch.uint8, _stream_getter()
+        self._types = {torch.float32: 0, torch.float16: 1}
+        self._f32, self._i32 = (torch.float32,), (torch.int32,)
+        self._flag, self._u16 = (torch.bool, torch.uint8), (torch.uint16, torch.int16)
+        self._bytes = {}  # of the workspace, by rows and type
+        self._select = _lib.plain(self._lib, "ane_beam_select")
+
+    def _vector(self, name, t, dtypes, dev, rows):
+        if t.dtype in dtypes and t.device == dev and t.dim() == 1 and t.shape[0] == rows and t.is_contiguous():
+            return t.data_ptr()
+        return _whole(self._op, name, t, dtypes, dev, shape=(rows,))
+
+    def Select(self, logits, scores, finished=None, weights=None, history=None, lengths=None, tokens=None,
+               parents=None, scores_out=None, finished_out=None):
+        """One step: logits fp32 or fp16 [requests * beams, vocab], scores fp32
+        [rows], the beams' sums of log probabilities (-inf: a beam that is
+        none) -> (tokens int32, parents int32, scores fp32), new if None;
+        scores_out may be scores.  finished bool or uint8 [rows], with eos:
+        beams that have only themselves to offer; their next state goes to
+        finished_out (may be finished, and is if None).  weights fp32 [rows],
+        above 0: what scores are multiplied by where they are compared (lengths
+        to some negative power).  history uint16 or int16 bits [rows, n] with
+        lengths int32 [rows]: reordered in place, and longer by the token.
+        Where a request has fewer candidates than beams, the last ones are
+        (NO_TOKEN, -1, -inf)."""
+        op = self._op
+        dev = _on_gpu(op, logits)
+        half = self._types.get(logits.dtype)
+        if half is None:
+            _fail(op, f"logits are {logits.dtype}, want torch.float32 or torch.float16")
+        lp = _tensor(op, "logits", logits, (logits.dtype,), dev, dims=2)
+        rows = int(logits.shape[0])
+        if logits.shape[1] != self.vocab or rows % self.beams:
+            _fail(op, f"logits have shape {tuple(logits.shape)}, want (requests * {self.beams}, {self.vocab})")
+        if (finished is None) != (self.eos is None):
+            _fail(op, "finished and eos go together")
+        if (history is None) != (lengths is None):
+            _fail(op, "history without lengths" if lengths is None else "lengths without a history")
+        new = self._empty
+        tokens = new(rows, dtype=self._i32[0], device=dev) if tokens is None else tokens
+        parents = new(rows, dtype=self._i32[0], device=dev) if parents is None else parents
+        scores_out = new(rows, dtype=self._f32[0], device=dev) if scores_out is None else scores_out
+        sp = self._vector("scores", scores, self._f32, dev, rows)
+        wp = 0 if weights is None else self._vector("weights", weights, self._f32, dev, rows)
+        fp = fo = hp = hr = most = np_ = 0
+        if finished is not None:
+            fp = self._vector("finished", finished, self._flag, dev, rows)
+            fo = fp if finished_out is None else self._vector("finished_out", finished_out, self._flag, dev, rows)
+        elif finished_out is not None:
+            _fail(op, "finished_out without finished")
+        if history is not None:
+            hp = _tensor(op, "history", history, self._u16, dev, dims=2)
+            if history.shape[0] != rows:
+                _fail(op, f"history has {history.shape[0]} rows, want {rows}")
+            most = int(history.shape[1])
+            hr = LogitControls._row(history)
+            np_ = self._vector("lengths", lengths, self._i32, dev, rows)
+        tp = self._vector("tokens", tokens, self._i32, dev, rows)
+        pp = self._vector("parents", parents, self._i32, dev, rows)
+        so = self._vector("scores_out", scores_out, self._f32, dev, rows)
+        n = self._bytes.get((rows, half))
+        if n is None:
+            n = self._bytes[rows, half] = _check(
+                self._lib, self._lib.ane_beam_select_workspace(rows // self.beams, self.beams, self.vocab, half))
+        ws = self._empty(n, dtype=self._u8, device=dev)
+        a = _lib.pack_beam(lp, sp, wp, fp, tp, pp, so, fo, hp, np_, LogitControls._row(logits), hr,
+                           rows // self.beams, self.beams, self.vocab, -1 if self.eos is None else self.eos, most,
+                           half, dev.index, ws.data_ptr(), n)
+        rc = self._select(a, self._stream(dev.index))
+        if rc:
+            _check(self._lib, rc)
+        return tokens, parents, scores_out

@@ -207,6 +207,10 @@ __device__ __forceinline__ int kv8_exponent(uint32_t amax_bits) {
   return clampi(e, kKvExpMin, kKvExpMax);
 }
 
+// Host: checks the cache of operator `op`; ANE_OK or ANE_ERR_ARG with the
+// message set.
+int kv8_cache_check(const char* op, const ane_kv8_cache* c);
+
 // Host: checks the cache and the batch of operator `op` and fills the
 // kernels' form; ANE_OK or ANE_ERR_ARG with the message set.
 int kv8_check(const char* op, const ane_kv8_cache* c, const ane_kv8_batch* b, Kv8Batch* out);
@@ -256,6 +260,21 @@ bool share_memory(Extent a, Extent b);
 inline Extent fp16_rows(const void* p, int64_t rows, int64_t row, int64_t heads, int64_t head, int64_t dh) {
   return {(uintptr_t)p, rows, row * 2, heads, head * 2, dh * 2};
 }
+
+// The buffers of a call, for the refusal of outputs that share memory with
+// another one.  Two with the same `pair` (not 0) may be one and the same.
+struct Buffer {
+  const char* name;
+  Extent at;
+  bool out;
+  int pair = 0;
+};
+inline Extent flat(const void* p, int64_t bytes) { return {(uintptr_t)p, 1, 0, 1, 0, bytes}; }
+inline Extent row_major(const void* p, int64_t rows, int64_t row, int64_t width) {
+  return {(uintptr_t)p, rows, row, 1, 0, width};
+}
+// ANE_OK, or ANE_ERR_ARG with the message set; null buffers share nothing.
+int check_apart(const char* op, const Buffer* b, int n);
 
 // Makes the cache's device current for a scope (launches go to the current
 // device; the caller's choice comes back).

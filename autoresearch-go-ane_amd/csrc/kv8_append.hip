@@ -259,8 +259,18 @@ bool share_memory(Extent a, Extent b) {
   return false;
 }
 
-int kv8_check(const char* op, const ane_kv8_cache* c, const ane_kv8_batch* b, Kv8Batch* out) {
-  if (!c || !b) return op_fail(ANE_ERR_ARG, "storiesane %s: no cache or batch", op);
+int check_apart(const char* op, const Buffer* b, int n) {
+  for (int i = 0; i < n; i++)
+    for (int j = 0; j < i; j++) {
+      const Buffer &x = b[i], &y = b[j];
+      if (!(x.out || y.out) || !x.at.at || !y.at.at) continue;
+      if (x.pair && x.pair == y.pair && x.at.at == y.at.at) continue;
+      if (share_memory(x.at, y.at)) return op_fail(ANE_ERR_ARG, "storiesane %s: %s overlaps %s", op, x.name, y.name);
+    }
+  return ANE_OK;
+}
+
+int kv8_cache_check(const char* op, const ane_kv8_cache* c) {
   if (!c->k || !c->v || !c->k_exp || !c->v_exp) return op_fail(ANE_ERR_ARG, "storiesane %s: null cache buffer", op);
   if (!aligned16(c->k) || !aligned16(c->v))
     return op_fail(ANE_ERR_ARG, "storiesane %s: k and v must be 16-byte aligned", op);
@@ -272,6 +282,14 @@ int kv8_check(const char* op, const ane_kv8_cache* c, const ane_kv8_batch* b, Kv
   if (c->pages < 1 || c->kv_heads < 1 || c->kv_heads > 1024)
     return op_fail(ANE_ERR_ARG, "storiesane %s: pages=%d kv_heads=%d (pages at least 1, kv_heads 1..1024)", op,
                    c->pages, c->kv_heads);
+  return ANE_OK;
+}
+
+int kv8_check(const char* op, const ane_kv8_cache* c, const ane_kv8_batch* b, Kv8Batch* out) {
+  if (!c || !b) return op_fail(ANE_ERR_ARG, "storiesane %s: no cache or batch", op);
+  const int rc = kv8_cache_check(op, c);
+  if (rc) return rc;
+  const int P = c->page_tokens;
   if (b->nseq < 0 || b->nseq > 65536 || b->rows < 0 || b->rows > (1 << 30))
     return op_fail(ANE_ERR_ARG, "storiesane %s: nseq=%d want 0..65536, rows=%d want 0..%d", op, b->nseq, b->rows,
                    1 << 30);

@@ -64,6 +64,26 @@ struct StepArgs : AttendArgs {
   Kv8AppendArgs in;
 };
 
+// over the pages that are named for each row and key/value head (tt = 1)
+struct ListArgs : AttendArgs {
+  const int* blocks;  // [rows][NKV][count] places in the table
+  int count;
+};
+__device__ __forceinline__ const int* list_of(const ListArgs& a, int row, int h) {
+  return a.blocks + ((size_t)row * a.b.NKV + h) * a.count;
+}
+// The list's keys, in its own order: those of its pages up to the last place
+// that is one (at least a page, so that a row without any gets its zeros).
+__device__ __forceinline__ int list_keys(const ListArgs& a, const int* list) {
+  int c = (a.count - 1) & ~63;
+  for (;; c -= 64) {
+    const int at = c + (int)(threadIdx.x & 63);
+    const uint64_t is = __ballot(at < a.count && (unsigned)list[min(at, a.count - 1)] < (unsigned)a.b.table_pages);
+    if (is) return (c + 64 - __clzll((long long)is)) << a.b.pshift;
+    if (c == 0) return 1 << a.b.pshift;
+  }
+}
+
 // where dimension d of a row's query head goes
 template <int DH>
 __device__ __forceinline__ half_t* out_at(const AttendArgs& a, int row, int head, int d) {
@@ -105,10 +125,11 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
 // A page that is not there reads the pool's first, which exists but may hold
 // anything; its scores are masked, its values cleared, and its exponents 0 (a
 // scale made of a stray one, -128, is NaN and makes NaN of cleared values too).
+// pos: of a list's pages, where the unit's tokens stand in the sequence.
 template <int DH>
 struct Step {
   u32x4 k[NU][DH / 64], v[NU][DH / 64];
-  int ex[NU];
+  int ex[NU], pos[NU];
 };
 constexpr int kThere = 1 << 16;
 __device__ __forceinline__ float k_scale(int ex) { return kv8_scale((int8_t)(ex & 0xff)); }
@@ -123,10 +144,12 @@ constexpr int waves_per_simd(int DH, int NT) {
 // takes, each by a wave of its own (KW = 1: the waves have nothing to do with
 // each other); ONE: a step's keys are of one page (pages of at least kStep
 // tokens).  Args is StepArgs: the sequences have a token each, and the block
-// first appends its key and value and rotates its queries.
+// first appends its key and value and rotates its queries.  ListArgs: the keys
+// are those of a list of pages, numbered in its order.
 template <int DH, int NT, int KW, int RW, bool ONE, typename Args>
 __global__ __launch_bounds__(64 * KW * RW, waves_per_simd(DH, NT)) void attend_kernel(Args a) {
   constexpr bool STEP = std::is_same_v<Args, StepArgs>;
+  constexpr bool LIST = std::is_same_v<Args, ListArgs>;
   static_assert(!STEP || (NT == 1 && KW == 4));
   static_assert(KW == 1 || RW == 1, "the waves of a block meet over one tile");
   constexpr int R = 16 * NT;    // rows of the tile
@@ -152,7 +175,10 @@ __global__ __launch_bounds__(64 * KW * RW, waves_per_simd(DH, NT)) void attend_k
   const Kv8Span span = NT > 1 && KW > 1 ? tile_span(a, tile) : kv8_tile_span(b, a.tt, tile);
   if (span.n == 0) return;
   const int rows = span.n * a.G;
-  const int kend = span.pos + span.n;  // keys of the tile's last token
+  const int* list = nullptr;
+  if constexpr (LIST) list = list_of(a, span.row, h);
+  int kend = span.pos + span.n;  // keys of the tile's last token
+  if constexpr (LIST) kend = list_keys(a, list);
   const int pk = part_keys(a, kend);
   const int k0 = sp * pk;
   if (k0 >= kend) return;
@@ -177,7 +203,7 @@ __global__ __launch_bounds__(64 * KW * RW, waves_per_simd(DH, NT)) void attend_k
   // 64 pages from wbase on, one per lane: where the head's rows begin, and
   // what Step says of the page.  wend: the first position behind them.
   const int* trow = b.table + (size_t)span.seq * b.table_stride;
-  int wbase = 0, wexp = 0;
+  int wbase = 0, wexp = 0, wpos = 0;
   int wend = 0;
   uint32_t wlo = 0, whi = 0;
   auto window = [&](int pg) {
@@ -185,7 +211,16 @@ __global__ __launch_bounds__(64 * KW * RW, waves_per_simd(DH, NT)) void attend_k
     wend = (pg + 64) << b.pshift;  // a table covers at most 2^30 tokens
     const int p = pg + lane;
     int id = -1;
-    if (p < b.table_pages && ((int64_t)p << b.pshift) < k1) {
+    if constexpr (LIST) {
+      if (p << b.pshift < k1) {  // and so within the list
+        const int place = list[p];
+        if ((unsigned)place < (unsigned)b.table_pages) {
+          id = trow[place];
+          wpos = place << b.pshift;
+        }
+      }
+      if ((unsigned)id >= (unsigned)b.pages) id = -1;
+    } else if (p < b.table_pages && ((int64_t)p << b.pshift) < k1) {
       id = trow[p];
       if ((unsigned)id >= (unsigned)b.pages) id = -1;
     }
@@ -211,9 +246,11 @@ __global__ __launch_bounds__(64 * KW * RW, waves_per_simd(DH, NT)) void attend_k
              (size_t)(uint32_t)__builtin_amdgcn_readlane((int)whi, w) << 32;
         s.ex[u] = __builtin_amdgcn_readlane(wexp, w);
         at += (ku & ((1 << b.pshift) - 1)) * DH;
+        if (LIST) s.pos[u] = __builtin_amdgcn_readlane(wpos, w) + (ku & ((1 << b.pshift) - 1));
       } else {
         s.ex[u] = s.ex[0];
         at += 16 * DH;
+        if (LIST) s.pos[u] = s.pos[0] + 16;
       }
       const uint8_t *kp = a.k + at, *vp = a.v + at;
 #pragma unroll
@@ -270,12 +307,20 @@ __global__ __launch_bounds__(64 * KW * RW, waves_per_simd(DH, NT)) void attend_k
     for (int d = 0; d < ND; d++) o[d][t] = floatx4{0.f, 0.f, 0.f, 0.f};
   }
 
+  // where the unit's first token stands
+  auto unit_pos = [&](const Step<DH>& s, int kb, int u) { return LIST ? s.pos[u] : kb + 16 * u; };
   // not 0: the step holds keys that some row does not attend to
   auto at_edge = [&](const Step<DH>& s, int kb) {
     int all = s.ex[0];
 #pragma unroll
     for (int u = 1; u < (ONE ? 1 : NU); u++) all &= s.ex[u];
-    return max(kb + kStep - 1 - span.pos, 0) | (~all & kThere);
+    int last = kb + kStep - 1;
+    if (LIST) {
+      last = s.pos[0] + 15;
+#pragma unroll
+      for (int u = 1; u < NU; u++) last = max(last, s.pos[u] + 15);
+    }
+    return max(last - span.pos, 0) | (~all & kThere);
   };
 
   half8 ones;
@@ -310,7 +355,7 @@ __global__ __launch_bounds__(64 * KW * RW, waves_per_simd(DH, NT)) void attend_k
         for (int t = 0; t < NT; t++)
 #pragma unroll
           for (int j = 0; j < 4; j++)
-            if (!(s.ex[u] & kThere) || kb + 16 * u + 4 * g + j > lim[t]) sc[u][t][j] = -INFINITY;
+            if (!(s.ex[u] & kThere) || unit_pos(s, kb, u) + 4 * g + j > lim[t]) sc[u][t][j] = -INFINITY;
     }
     float mx[NT];
     bool up = false;
@@ -366,8 +411,8 @@ __global__ __launch_bounds__(64 * KW * RW, waves_per_simd(DH, NT)) void attend_k
     if (edge) {
 #pragma unroll
       for (int u = 0; u < NU; u++) {
-        const int first = kb + 16 * u + 4 * g;  // the lane's four keys
-        const int n = s.ex[u] & kThere ? clampi(k1 - first, 0, 4) : 0;
+        const int first = unit_pos(s, kb, u) + 4 * g;  // the lane's four keys
+        const int n = s.ex[u] & kThere ? clampi((LIST ? span.pos + 1 : k1) - first, 0, 4) : 0;
         const uint32_t mine = n == 4 ? 0xffffffffu : (1u << (8 * n)) - 1;
 #pragma unroll
         for (int x = 0; x < DH / 64; x++)
@@ -422,7 +467,7 @@ __global__ __launch_bounds__(64 * KW * RW, waves_per_simd(DH, NT)) void attend_k
 #pragma unroll
           for (int j = 0; j < 8; j++) {
             const int u = 2 * y + (j >> 2);
-            sees[t][j] = (cur.ex[u] & kThere) && kb + 16 * u + 4 * g + (j & 3) <= lim[t] ? (half_t)1.f : (half_t)0.f;
+            sees[t][j] = (cur.ex[u] & kThere) && unit_pos(cur, kb, u) + 4 * g + (j & 3) <= lim[t] ? (half_t)1.f : (half_t)0.f;
           }
 #pragma unroll
         for (int d = 0; d < ND; d++) {
@@ -526,8 +571,8 @@ __global__ __launch_bounds__(64 * KW * RW, waves_per_simd(DH, NT)) void attend_k
 // s's maximum and sum (at most kMaxSplit parts), then every lane DH / 64
 // dimensions of all parts.
 constexpr int kMaxSplit = 64;
-template <int DH>
-__global__ __launch_bounds__(256) void join_kernel(AttendArgs a) {
+template <int DH, typename Args>
+__global__ __launch_bounds__(256) void join_kernel(Args a) {
   constexpr int W = DH / 64;
   const Kv8Batch& b = a.b;
   const int lane = threadIdx.x & 63;
@@ -535,7 +580,8 @@ __global__ __launch_bounds__(256) void join_kernel(AttendArgs a) {
   const Kv8Span span = tile_span(a, tile);
   const int r = blockIdx.y * 4 + (threadIdx.x >> 6);
   if (r >= span.n * a.G) return;
-  const int kend = span.pos + span.n;
+  int kend = span.pos + span.n;
+  if constexpr (std::is_same_v<Args, ListArgs>) kend = list_keys(a, list_of(a, span.row, h));
   const int pk = part_keys(a, kend);
   if (pk >= kend) return;  // one part: the output is written
   const int np = (kend + pk - 1) / pk;
@@ -579,14 +625,15 @@ struct Plan {
   int64_t bytes = 0;
 };
 
-int plan(const char* op, const Kv8Batch& b, const ane_kv8_batch& given, int DH, int heads, Plan* p) {
+// count: pages of a row's list (0: the whole context)
+int plan(const char* op, const Kv8Batch& b, const ane_kv8_batch& given, int DH, int heads, int count, Plan* p) {
   if (heads < 1 || heads % b.NKV || heads / b.NKV > kKvMaxGroup)
     return op_fail(ANE_ERR_ARG, "storiesane %s: heads=%d must be 1..%d times kv_heads=%d", op, heads, kKvMaxGroup,
                    b.NKV);
   const int G = heads / b.NKV;
   if (b.nseq == 0 || b.rows == 0) return ANE_OK;
   const int cap = b.table_pages << b.pshift;
-  const int len = given.max_len ? std::min(given.max_len, cap) : cap;
+  const int len = count ? count << b.pshift : given.max_len ? std::min(given.max_len, cap) : cap;
   // Tiles of 16 or 32 rows: the smallest that takes the longest sequence's rows
   // (the mean one's where that is not known), and at least a token's.  48 rows
   // use what a step converts a third better, in fewer and longer blocks: for
@@ -603,6 +650,10 @@ int plan(const char* op, const Kv8Batch& b, const ane_kv8_batch& given, int DH, 
       ((b.nseq == 1 && len >= 4096) || (int64_t)kv8_count(b.nseq, b.rows, kv8_tiles(48 / G)) * b.NKV >= 1536))
     p->nt = 3;
   p->tt = 16 * p->nt / G;
+  if (count) {  // a row is a tile
+    p->nt = G <= 16 ? 1 : 2;
+    p->tt = 1;
+  }
   p->tiles = kv8_count(b.nseq, b.rows, kv8_tiles(p->tt));
   const int64_t blocks = (int64_t)p->tiles * b.NKV;
   // Waves that share a tile's keys: four, and in larger tiles each wave a tile
@@ -612,7 +663,7 @@ int plan(const char* op, const Kv8Batch& b, const ane_kv8_batch& given, int DH, 
   // 2048 36 against 18; head dimension 128: 8 of 2048 206 against 248; but one
   // of 2048 46 against 37).
   const int wps = waves_per_simd(DH, p->nt);
-  p->kw = p->nt > 1 && 2 * blocks >= (int64_t)wps * len ? 1 : 4;
+  p->kw = p->nt > 1 && !count && 2 * blocks >= (int64_t)wps * len ? 1 : 4;
   p->round = p->kw * kStep;
   // The longest contexts first, so that the last blocks to end are short ones:
   // chunks of prompts at the lengths they come in (8 of 100 to 400 on up to
@@ -620,7 +671,7 @@ int plan(const char* op, const Kv8Batch& b, const ane_kv8_batch& given, int DH, 
   // up to 4000 33 against 38).  Finding them costs each block 1.2 us at 64
   // sequences (64 of 16 to 100, head dimension 128: 138 against 129), so up to
   // 32, and not where a CU has no second block.
-  p->longest = p->nt > 1 && p->kw == 4 && b.nseq > 1 && b.nseq <= 32 && blocks > 256;
+  p->longest = p->nt > 1 && p->kw == 4 && !count && b.nseq > 1 && b.nseq <= 32 && blocks > 256;
   // Parts of the keys, where there are few blocks.  What parts cost is the
   // join's launch, 3 us, and their sums in fp32: for tiles of 32 and 48 rows a
   // block has to save more than it writes (1500 tokens of a prompt, 600 blocks:
@@ -657,6 +708,11 @@ int plan(const char* op, const Kv8Batch& b, const ane_kv8_batch& given, int DH, 
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
+int check_count(const char* op, int count) {
+  if (count < 1 || count > 65536) return op_fail(ANE_ERR_ARG, "storiesane %s: count=%d want 1..65536", op, count);
+  return ANE_OK;
+}
+
 template <int DH, int NT, int KW, int RW, typename Args>
 void launch_form(const Args& a, hipStream_t st) {
   const dim3 grid(((uint32_t)a.tiles + RW - 1) / RW * a.b.NKV * a.nsplit), block(64 * KW * RW);
@@ -676,7 +732,17 @@ void launch(const AttendArgs& a, const Plan& p, hipStream_t st) {
     else launch_form<DH, 3, 1, 4>(a, st);
   }
   if (a.nsplit > 1)
-    hipLaunchKernelGGL(join_kernel<DH>, dim3((uint32_t)a.tiles * a.b.NKV, (a.tt * a.G + 3) / 4), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((join_kernel<DH, AttendArgs>), dim3((uint32_t)a.tiles * a.b.NKV, (a.tt * a.G + 3) / 4),
+                       dim3(256), 0, st, a);
+}
+
+template <int DH>
+void launch_list(const ListArgs& a, const Plan& p, hipStream_t st) {
+  if (p.nt == 1) launch_form<DH, 1, 4, 1>(a, st);
+  else launch_form<DH, 2, 4, 1>(a, st);
+  if (a.nsplit > 1)
+    hipLaunchKernelGGL((join_kernel<DH, ListArgs>), dim3((uint32_t)a.tiles * a.b.NKV, (a.G + 3) / 4), dim3(256), 0, st,
+                       a);
 }
 
 }  // namespace
@@ -691,7 +757,19 @@ extern "C" int64_t ane_kv8_attend_workspace(const ane_kv8_cache* cache, const an
   int rc = kv8_check(op, cache, batch, &b);
   if (rc) return rc;
   Plan p;
-  rc = plan(op, b, *batch, cache->head_dim, heads, &p);
+  rc = plan(op, b, *batch, cache->head_dim, heads, 0, &p);
+  return rc ? rc : p.bytes;
+}
+
+extern "C" int64_t ane_kv8_attend_blocks_workspace(const ane_kv8_cache* cache, const ane_kv8_batch* batch,
+                                                   int32_t heads, int32_t count) {
+  const char* op = "kv8 attend workspace";
+  Kv8Batch b;
+  int rc = kv8_check(op, cache, batch, &b);
+  if (!rc) rc = check_count(op, count);
+  if (rc) return rc;
+  Plan p;
+  rc = plan(op, b, *batch, cache->head_dim, heads, count, &p);
   return rc ? rc : p.bytes;
 }
 
@@ -702,17 +780,25 @@ extern "C" int ane_kv8_attend(const ane_kv8_cache* cache, const ane_kv8_batch* b
 
 namespace {
 
-// in: the append that the launch takes with it, where the plan lets it
+struct List {
+  const int* blocks = nullptr;
+  int count = 0;
+};
+
+// in: the append that the launch takes with it, where the plan lets it; list:
+// the pages that the rows attend to, if not all
 int attend(const ane_kv8_cache* cache, const ane_kv8_batch* batch, const ane_kv8_attend_args* args, bool frag,
-           const Kv8AppendArgs* in, void* stream) {
+           const Kv8AppendArgs* in, const List* list, void* stream) {
   const char* op = "kv8 attend";
   StepArgs step;
   AttendArgs& a = step;
   int rc = kv8_check(op, cache, batch, &a.b);
+  if (!rc && list) rc = check_count(op, list->count);
   if (rc) return rc;
   if (!args) return op_fail(ANE_ERR_ARG, "storiesane %s: null arguments", op);
   if (a.b.nseq == 0 || a.b.rows == 0) return ANE_OK;  // an empty tensor may have no address
-  if (!args->q || !args->out) return op_fail(ANE_ERR_ARG, "storiesane %s: null buffer", op);
+  if (!args->q || !args->out || (list && !list->blocks))
+    return op_fail(ANE_ERR_ARG, "storiesane %s: null buffer", op);
   const ane_kv8_attend_args& g = *args;
   for (const int64_t s : {g.q_row, g.q_head, g.out_row, g.out_head})
     if (s < 0 || s % 8)
@@ -724,7 +810,7 @@ int attend(const ane_kv8_cache* cache, const ane_kv8_batch* batch, const ane_kv8
     return op_fail(ANE_ERR_ARG, "storiesane %s: scale=%g must be positive and finite, times log2(e) too", op,
                    (double)g.scale);
   Plan p;
-  rc = plan(op, a.b, *batch, cache->head_dim, g.heads, &p);
+  rc = plan(op, a.b, *batch, cache->head_dim, g.heads, list ? list->count : 0, &p);
   if (rc) return rc;
   if (frag && a.b.rows > kDecRows)
     return op_fail(ANE_ERR_ARG, "storiesane %s: rows=%d of fragments, want at most %d", op, a.b.rows, kDecRows);
@@ -734,6 +820,12 @@ int attend(const ane_kv8_cache* cache, const ane_kv8_batch* batch, const ane_kv8
   if (!frag && !same && share_memory(fp16_rows(g.q, a.b.rows, g.q_row, g.heads, g.q_head, cache->head_dim),
                                      fp16_rows(g.out, a.b.rows, g.out_row, g.heads, g.out_head, cache->head_dim)))
     return op_fail(ANE_ERR_ARG, "storiesane %s: out overlaps q with other strides, or in part", op);
+  if (list) {
+    const Buffer buffers[] = {{"blocks", flat(list->blocks, (int64_t)a.b.rows * a.b.NKV * list->count * 4), false},
+                              {"out", fp16_rows(g.out, a.b.rows, g.out_row, g.heads, g.out_head, cache->head_dim), true}};
+    rc = check_apart(op, buffers, 2);
+    if (rc) return rc;
+  }
   if (p.bytes > 0 && (!g.ws || g.ws_bytes < p.bytes))
     return op_fail(ANE_ERR_ARG, "storiesane %s: workspace of %lld bytes, want %lld", op,
                    (long long)(g.ws ? g.ws_bytes : 0), (long long)p.bytes);
@@ -752,6 +844,13 @@ int attend(const ane_kv8_cache* cache, const ane_kv8_batch* batch, const ane_kv8
   if (in) {
     step.in = *in;
     launch_form<64, 1, 4, 1>(step, (hipStream_t)stream);
+  } else if (list) {
+    ListArgs l;
+    static_cast<AttendArgs&>(l) = a;
+    l.blocks = list->blocks;
+    l.count = list->count;
+    if (cache->head_dim == 64) launch_list<64>(l, p, (hipStream_t)stream);
+    else launch_list<128>(l, p, (hipStream_t)stream);
   } else if (cache->head_dim == 64) launch<64>(a, p, (hipStream_t)stream);
   else launch<128>(a, p, (hipStream_t)stream);
   const hipError_t h = hipGetLastError();
@@ -763,7 +862,14 @@ int attend(const ane_kv8_cache* cache, const ane_kv8_batch* batch, const ane_kv8
 
 int ane::kv8_attend(const ane_kv8_cache* cache, const ane_kv8_batch* batch, const ane_kv8_attend_args* args, bool frag,
                     void* stream) {
-  return attend(cache, batch, args, frag, nullptr, stream);
+  return attend(cache, batch, args, frag, nullptr, nullptr, stream);
+}
+
+extern "C" int ane_kv8_attend_blocks(const ane_kv8_cache* cache, const ane_kv8_batch* batch,
+                                     const ane_kv8_attend_args* args, const int32_t* blocks, int32_t count,
+                                     void* stream) {
+  const List list = {blocks, count};
+  return attend(cache, batch, args, false, nullptr, &list, stream);
 }
 
 int ane::kv8_step(const ane_kv8_cache* cache, const ane_kv8_batch* batch, const ane_kv8_append_args* append,
@@ -772,12 +878,12 @@ int ane::kv8_step(const ane_kv8_cache* cache, const ane_kv8_batch* batch, const 
   int rc = kv8_append_check("kv8 append", cache, batch, append, from, &in);
   if (rc || in.b.nseq == 0 || in.b.rows == 0) return rc;
   Plan p;
-  rc = plan("kv8 attend", in.b, *batch, cache->head_dim, append->heads, &p);
+  rc = plan("kv8 attend", in.b, *batch, cache->head_dim, append->heads, 0, &p);
   if (rc) return rc;
   // The decoder's step of 64 sequences and 1024 tokens, 12 layers: 0.504 ms in
   // one launch a layer, 0.534 in two; of 3 sequences 0.330 and 0.346.
   const bool one = from && batch->max_new == 1 && in.b.rows <= in.b.nseq && p.nt == 1 && p.nsplit == 1;
-  if (one) return attend(cache, batch, args, frag, &in, stream);
+  if (one) return attend(cache, batch, args, frag, &in, nullptr, stream);
   rc = kv8_append(cache, batch, append, from, stream);
-  return rc ? rc : attend(cache, batch, args, frag, nullptr, stream);
+  return rc ? rc : attend(cache, batch, args, frag, nullptr, nullptr, stream);
 }

@@ -1,0 +1,610 @@
+// The tables of the 8-bit cache's pages: forking with copy on write, reserving
+// and freeing (ane_kv8_fork), compacting (ane_kv8_compact) and copying
+// (ane_kv8_copy); include/ane_serve.h says what each does.
+//
+// Everything is whole numbers, so results do not depend on the order in which
+// blocks run: reference counts change by atomic additions, and the pages that
+// are handed out are ranked (by sequence and position), as are the free ones
+// (by id).
+#include <algorithm>
+
+#include "kv8.h"
+#include "op_error.h"
+
+namespace ane {
+
+namespace {
+
+constexpr int kMaxLayers = 32;  // of a launch
+constexpr int kTh = 1024;       // threads of the blocks that rank
+constexpr int kChunk = 4 * kTh; // pages such a block ranks at a time
+
+// The layers' pages as the copies take them: k, v, exponents, and the bounds or
+// null.
+struct Layers {
+  uint8_t *k[kMaxLayers], *v[kMaxLayers];
+  int8_t *ke[kMaxLayers], *ve[kMaxLayers];
+  int8_t *box[kMaxLayers], *unit[kMaxLayers];
+};
+struct Pool {
+  int pages, pshift, NKV, dshift;  // page_tokens = 1 << pshift, head_dim = 1 << dshift
+};
+
+__device__ __forceinline__ int load_ref(const int* p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// One side (K or V) of page `from` of a layer to page `to`, its first `units`
+// units of 16 tokens, by a block of TH threads.  A unit of a head is 16 *
+// head_dim bytes in a row, on both sides.
+template <int TH>
+__device__ __forceinline__ void copy_side(const Pool& p, const Layers& x, const Layers& y, int layer, bool values,
+                                          int from, int to, int units) {
+  const int tid = threadIdx.x;
+  const uint32_t whole = 1u << (p.pshift - 4 + p.dshift), used = (uint32_t)units << p.dshift;  // 16-byte words of a head
+  const size_t at = (size_t)p.NKV * whole;
+  const u32x4* s = reinterpret_cast<const u32x4*>(values ? x.v[layer] : x.k[layer]) + from * at;
+  u32x4* d = reinterpret_cast<u32x4*>(values ? y.v[layer] : y.k[layer]) + to * at;
+  const uint32_t n = p.NKV * used;
+  constexpr int U = 4;
+  for (uint32_t t0 = tid; t0 < n; t0 += TH * U) {
+    u32x4 w[U];
+    uint32_t o[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const uint32_t t = min(t0 + u * TH, n - 1), h = used == whole ? 0 : t / used;
+      o[u] = h * whole + (t - h * used);
+      w[u] = s[o[u]];
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++)
+      if (t0 + u * TH < n) d[o[u]] = w[u];
+  }
+  const size_t ef = (size_t)from * p.NKV, et = (size_t)to * p.NKV;
+  const int8_t* se = values ? x.ve[layer] : x.ke[layer];
+  int8_t* de = values ? y.ve[layer] : y.ke[layer];
+  for (int h = tid; h < p.NKV; h += TH) de[et + h] = se[ef + h];
+  if (!values && x.box[layer] && y.box[layer]) {
+    const int m = p.NKV << (p.dshift - 3);  // 16-byte words of a page's boxes
+    const u32x4* sb = reinterpret_cast<const u32x4*>(x.box[layer]) + (size_t)from * m;
+    u32x4* db = reinterpret_cast<u32x4*>(y.box[layer]) + (size_t)to * m;
+    for (int t = tid; t < m; t += TH) db[t] = sb[t];
+    for (int h = tid; h < p.NKV; h += TH) y.unit[layer][et + h] = x.unit[layer][ef + h];
+  }
+}
+
+__device__ __forceinline__ int units_of(const Pool& p, int tokens) {
+  return (clampi(tokens, 0, 1 << p.pshift) + 15) >> 4;
+}
+
+// ---- fork ----------------------------------------------------------------------
+
+// What becomes of a sequence: it holds st tokens and will hold `end`; its new
+// pages have the ranks from `base` on, the first of them for a copy of page
+// `src` (-1: none).
+struct Next {
+  int st, end, base, src;
+};
+
+struct ForkArgs {
+  Pool p;
+  int *table, *start, *refs, *missing;
+  const int *parents, *news;
+  int stride, width, nseq, new_tokens;
+  int* mid;    // [nseq][width]: the parents' rows (unused where there are no parents)
+  Next* next;  // [nseq]
+  int* free;   // [pages]: free pages by rank
+  int* found;  // how many of them there are, of those that are wanted
+};
+
+__device__ __forceinline__ int there(int id, int pages) { return (unsigned)id < (unsigned)pages ? id : -1; }
+__device__ __forceinline__ int held_of(const ForkArgs& a, int i) {
+  const int from = a.parents ? a.parents[i] : i;
+  return (unsigned)from < (unsigned)a.nseq ? clampi(a.start[from], 0, a.width << a.p.pshift) : 0;
+}
+__device__ __forceinline__ int pages_for(const ForkArgs& a, int tokens) {
+  return (tokens + (1 << a.p.pshift) - 1) >> a.p.pshift;
+}
+
+// The parents' rows, cut to what they hold; reference counts follow.  A thread
+// an entry.
+__global__ __launch_bounds__(256) void rows_kernel(ForkArgs a) {
+  const int blocks = (a.width + 255) / 256, i = blockIdx.x / blocks;
+  const int j = (blockIdx.x - i * blocks) * 256 + threadIdx.x;
+  if (j >= a.width) return;
+  const int from = a.parents ? a.parents[i] : i;
+  const bool holds = j < pages_for(a, held_of(a, i));
+  int* mine = a.table + (size_t)i * a.stride + j;
+  const int raw = *mine, old = there(raw, a.p.pages);
+  const int mid = !holds ? -1 : from == i ? old : there(a.table[(size_t)from * a.stride + j], a.p.pages);
+  if (old != mid) {
+    if (old >= 0) atomicSub(a.refs + old, 1);
+    if (mid >= 0) atomicAdd(a.refs + mid, 1);
+  }
+  if (a.parents) a.mid[(size_t)i * a.width + j] = mid;
+  else if (raw != mid) *mine = mid;
+}
+
+// the sum over the threads before this one, and over all
+__device__ __forceinline__ int block_scan(int x, int (&sums)[kTh / 64], int& total) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  int s = x;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int y = __shfl_up(s, o, 64);
+    if (lane >= o) s += y;
+  }
+  __syncthreads();
+  if (lane == 63) sums[w] = s;
+  __syncthreads();
+  int before = 0;
+  total = 0;
+#pragma unroll
+  for (int k = 0; k < kTh / 64; k++) {
+    const int y = sums[k];
+    before += k < w ? y : 0;
+    total += y;
+  }
+  return before + s - x;
+}
+
+// One block: who copies, how many pages each sequence gets, and which are free.
+__global__ __launch_bounds__(kTh) void plan_kernel(ForkArgs a) {
+  __shared__ int sums[kTh / 64];
+  __shared__ int lost_all;
+  const int tid = threadIdx.x, P = 1 << a.p.pshift, cap = a.width << a.p.pshift;
+  if (tid == 0) lost_all = 0;
+  // the page that the sequence's first new token goes to, where it holds
+  // tokens already; -2: no such token
+  struct Seq {
+    int st, end, page;
+  };
+  const auto seq_of = [&](int i) {
+    Seq s;
+    s.st = held_of(a, i);
+    s.end = s.st + clampi(a.news ? a.news[i] : a.new_tokens, 0, cap - s.st);
+    s.page = -2;
+    if (s.end > s.st && (s.st & (P - 1))) {
+      const int j = s.st >> a.p.pshift;
+      s.page = a.parents ? a.mid[(size_t)i * a.width + j] : there(a.table[(size_t)i * a.stride + j], a.p.pages);
+    }
+    return s;
+  };
+  // A page whose count falls to 0 when its writers leave it is held by writers
+  // alone, and the lowest of them keeps it: the count then holds its number,
+  // as a negative one, until it becomes 1 again.
+  constexpr int kMark = -(1 << 30);
+  for (int i = tid; i < a.nseq; i += kTh) {
+    const int p = seq_of(i).page;
+    if (p >= 0) atomicSub(a.refs + p, 1);
+  }
+  __syncthreads();
+  for (int i = tid; i < a.nseq; i += kTh) {
+    const int p = seq_of(i).page;
+    if (p >= 0 && load_ref(a.refs + p) <= 0) atomicMin(a.refs + p, kMark + i);
+  }
+  __syncthreads();
+  for (int i = tid; i < a.nseq; i += kTh) {
+    const Seq s = seq_of(i);
+    const bool keeps = s.page >= 0 && load_ref(a.refs + s.page) == kMark + i;
+    a.next[i] = {s.st, s.end, keeps, keeps || s.page < 0 ? -1 : s.page};
+  }
+  __syncthreads();
+  int want = 0, lost = 0;
+  for (int i0 = 0; i0 < a.nseq; i0 += kTh) {
+    const int i = i0 + tid;
+    int need = 0;
+    if (i < a.nseq) {
+      const Next n = a.next[i];
+      need = (n.src >= 0) + pages_for(a, n.end) - pages_for(a, n.st);
+      if (n.end > n.st && (n.st & (P - 1)) && n.src < 0) {
+        const int p = seq_of(i).page;
+        if (n.base) __hip_atomic_store(a.refs + p, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        else lost++;
+      }
+    }
+    int all;
+    const int before = block_scan(need, sums, all);
+    if (i < a.nseq) a.next[i].base = want + before;
+    want += all;
+  }
+  if (lost) atomicAdd(&lost_all, lost);
+  __syncthreads();
+  int found = 0;
+  for (int p0 = 0; p0 < a.p.pages && found < want; p0 += kChunk) {
+    int is[4], n = 0;
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+      const int p = p0 + tid * 4 + u;
+      is[u] = p < a.p.pages && load_ref(a.refs + min(p, a.p.pages - 1)) <= 0;
+      n += is[u];
+    }
+    int all;
+    int rank = found + block_scan(n, sums, all);
+#pragma unroll
+    for (int u = 0; u < 4; u++)
+      if (is[u]) {
+        if (rank < want) a.free[rank] = p0 + tid * 4 + u;
+        rank++;
+      }
+    found += all;
+  }
+  if (tid == 0) {
+    found = min(found, want);
+    *a.found = found;
+    *a.missing = want - found + lost_all;
+  }
+}
+
+// The tables' entries and starts, a thread an entry; behind those blocks the
+// copies, a block for each sequence, layer and side.
+__global__ __launch_bounds__(256) void finish_kernel(ForkArgs a, Layers x, int nlayers, int table_blocks) {
+  const int P = 1 << a.p.pshift, found = *a.found;
+  if ((int)blockIdx.x < table_blocks) {
+    const int blocks = (a.width + 255) / 256, i = blockIdx.x / blocks;
+    const int j = (blockIdx.x - i * blocks) * 256 + threadIdx.x;
+    if (j >= a.width) return;
+    const Next n = a.next[i];
+    const int copies = n.src >= 0, held = pages_for(a, n.st);
+    int rank = -1;
+    if (copies && j == n.st >> a.p.pshift) rank = n.base;
+    else if (j >= held && j < pages_for(a, n.end)) rank = n.base + copies + (j - held);
+    int id = a.parents ? a.mid[(size_t)i * a.width + j] : -1;
+    if (rank >= 0) {
+      id = rank < found ? a.free[rank] : -1;
+      if (id >= 0) a.refs[id] = 1;
+    }
+    if (a.parents || rank >= 0) a.table[(size_t)i * a.stride + j] = id;
+    if (j == 0) a.start[i] = n.st;
+    return;
+  }
+  const int b = blockIdx.x - table_blocks, i = b / (2 * nlayers), ls = b - i * 2 * nlayers;
+  const Next n = a.next[i];
+  if (n.src < 0 || n.base >= found) return;
+  copy_side<256>(a.p, x, x, ls >> 1, ls & 1, n.src, a.free[n.base], units_of(a.p, n.st & (P - 1)));
+}
+
+// ---- compact -------------------------------------------------------------------
+
+struct CompactArgs {
+  Pool p;
+  int *table, *refs, *moved;
+  int stride, width, nseq;
+  int chunks;
+  int* counts;          // [chunks]: pages held in each
+  int* total;           // [1]: pages that go
+  int* code;            // [pages]: where a page is then; -1 free; -2 - k: it is the k-th that goes
+  int *holes, *movers;  // [pages / 2 + 1]
+};
+
+__global__ __launch_bounds__(kTh) void count_kernel(CompactArgs a) {
+  __shared__ int sums[kTh / 64];
+  int n = 0;
+#pragma unroll
+  for (int u = 0; u < 4; u++) {
+    const int64_t p = (int64_t)blockIdx.x * kChunk + u * kTh + threadIdx.x;
+    n += p < a.p.pages && a.refs[p] > 0;
+  }
+  int all;
+  block_scan(n, sums, all);
+  if (threadIdx.x == 0) a.counts[blockIdx.x] = all;
+}
+
+// Ranks: a block a chunk, which adds up the counts of all.
+__global__ __launch_bounds__(kTh) void rank_kernel(CompactArgs a) {
+  __shared__ int sums[kTh / 64];
+  const int tid = threadIdx.x;
+  int n = 0, m = 0, held, before, low;
+  for (int b = tid; b < a.chunks; b += kTh) {
+    const int c = a.counts[b];
+    n += c;
+    m += b < (int)blockIdx.x ? c : 0;
+  }
+  block_scan(n, sums, held);    // U: the pages held
+  block_scan(m, sums, before);  // those before this chunk
+  // those below U: whole chunks, and the one that U lies in
+  const int cu = held / kChunk;
+  n = 0;
+  for (int b = tid; b < cu; b += kTh) n += a.counts[b];
+  for (int p = cu * kChunk + tid; p < held; p += kTh) n += a.refs[p] > 0;
+  block_scan(n, sums, low);
+  if (blockIdx.x == 0 && tid == 0) *a.total = held - low;
+  const int64_t p0 = (int64_t)blockIdx.x * kChunk + tid * 4;
+  int is[4];
+  n = 0;
+#pragma unroll
+  for (int u = 0; u < 4; u++) {
+    is[u] = p0 + u < a.p.pages && a.refs[p0 + u] > 0;
+    n += is[u];
+  }
+  int all;
+  int rank = before + block_scan(n, sums, all);  // pages held before the thread's
+#pragma unroll
+  for (int u = 0; u < 4; u++) {
+    if (p0 + u >= a.p.pages) break;
+    const int p = (int)p0 + u;
+    int code = -1;
+    if (is[u]) {
+      code = p;
+      if (p >= held) {
+        const int k = rank - low;
+        code = -2 - k;
+        a.movers[k] = p;
+      }
+      rank++;
+    } else if (p < held) {
+      a.holes[p - rank] = p;
+    }
+    a.code[p] = code;
+  }
+}
+
+__global__ __launch_bounds__(256) void move_kernel(CompactArgs a, Layers x, int nlayers, int book_blocks) {
+  if ((int)blockIdx.x < book_blocks) {
+    // a thread a page or an entry of the table
+    const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (t < a.p.pages) {
+      const int p = (int)t, c = a.code[p];
+      int to = c;
+      if (c <= -2) {
+        to = a.holes[-2 - c];
+        a.refs[to] = a.refs[p];
+        a.refs[p] = 0;
+      }
+      a.moved[p] = to;
+    } else if (t - a.p.pages < (int64_t)a.nseq * a.width) {
+      const int64_t e = t - a.p.pages;
+      const int i = (int)(e / a.width), j = (int)(e - (int64_t)i * a.width);
+      int* at = a.table + (size_t)i * a.stride + j;
+      const int id = *at;
+      if ((unsigned)id < (unsigned)a.p.pages) {
+        const int c = a.code[id];
+        *at = c <= -2 ? a.holes[-2 - c] : c;
+      }
+    }
+    return;
+  }
+  const int b = blockIdx.x - book_blocks, ls = b % (2 * nlayers);
+  const int total = *a.total, step = (gridDim.x - book_blocks) / (2 * nlayers);
+  for (int k = b / (2 * nlayers); k < total; k += step)
+    copy_side<256>(a.p, x, x, ls >> 1, ls & 1, a.movers[k], a.holes[k], 1 << (a.p.pshift - 4));
+}
+
+// ---- copy ----------------------------------------------------------------------
+
+__global__ __launch_bounds__(256) void copy_kernel(Pool p, int into_pages, Layers x, Layers y, int nlayers,
+                                                   const int* src, const int* dst, const int* tokens) {
+  const int i = blockIdx.x / (2 * nlayers), ls = blockIdx.x - i * 2 * nlayers;
+  const int from = src[i], to = dst[i];
+  if ((unsigned)from >= (unsigned)p.pages || (unsigned)to >= (unsigned)into_pages) return;
+  const int units = tokens ? units_of(p, tokens[i]) : 1 << (p.pshift - 4);
+  if (units > 0) copy_side<256>(p, x, y, ls >> 1, ls & 1, from, to, units);
+}
+
+// ---- host ----------------------------------------------------------------------
+
+int check_pool(const char* op, const ane_kv8_pool* pool, bool refs, Pool* out) {
+  if (!pool || !pool->layers || pool->nlayers < 1 || pool->nlayers > 1024)
+    return op_fail(ANE_ERR_ARG, "storiesane %s: no pool, or %d layers, want 1..1024", op, pool ? pool->nlayers : 0);
+  if (refs && !pool->refs) return op_fail(ANE_ERR_ARG, "storiesane %s: null refs", op);
+  const ane_kv8_cache& c = pool->layers[0];
+  for (int l = 0; l < pool->nlayers; l++) {
+    const ane_kv8_cache& x = pool->layers[l];
+    const int rc = kv8_cache_check(op, &x);
+    if (rc) return rc;
+    if (x.pages != c.pages || x.page_tokens != c.page_tokens || x.kv_heads != c.kv_heads || x.head_dim != c.head_dim ||
+        x.device != c.device)
+      return op_fail(ANE_ERR_ARG, "storiesane %s: layer %d differs from layer 0 in its sizes or its device", op, l);
+    if (pool->bounds) {
+      const ane_kv8_bounds& b = pool->bounds[l];
+      if (!b.box != !b.unit || ((uintptr_t)b.box & 15))
+        return op_fail(ANE_ERR_ARG, "storiesane %s: bounds of layer %d: box without unit, or not 16-byte aligned", op, l);
+    }
+  }
+  *out = {c.pages, 0, c.kv_heads, c.head_dim == 64 ? 6 : 7};
+  while (1 << out->pshift < c.page_tokens) out->pshift++;
+  return ANE_OK;
+}
+
+// the layers from l0 on that a launch takes
+int layers_of(const ane_kv8_pool& pool, int l0, Layers* x) {
+  const int n = std::min(kMaxLayers, pool.nlayers - l0);
+  for (int i = 0; i < n; i++) {
+    const ane_kv8_cache& c = pool.layers[l0 + i];
+    x->k[i] = (uint8_t*)c.k; x->v[i] = (uint8_t*)c.v; x->ke[i] = c.k_exp; x->ve[i] = c.v_exp;
+    x->box[i] = pool.bounds ? pool.bounds[l0 + i].box : nullptr;
+    x->unit[i] = pool.bounds ? pool.bounds[l0 + i].unit : nullptr;
+  }
+  return n;
+}
+
+int check_table(const char* op, const int* table, int stride, int width, int nseq, int pshift) {
+  if (nseq < 0 || nseq > 65536) return op_fail(ANE_ERR_ARG, "storiesane %s: nseq=%d want 0..65536", op, nseq);
+  if (nseq == 0) return ANE_OK;
+  if (!table) return op_fail(ANE_ERR_ARG, "storiesane %s: null table", op);
+  if (width < 1 || stride < width || ((int64_t)width << pshift) > 1 << 30)
+    return op_fail(ANE_ERR_ARG, "storiesane %s: table_pages=%d (at least 1, at most its stride %d and %d tokens)", op,
+                   width, stride, 1 << 30);
+  if ((int64_t)nseq * width > 1 << 30)
+    return op_fail(ANE_ERR_ARG, "storiesane %s: a table of %d x %d entries, want at most %d", op, nseq, width, 1 << 30);
+  return ANE_OK;
+}
+
+int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }
+
+struct ForkPlan {
+  int64_t next, mid, free, bytes;  // offsets; found comes first
+};
+ForkPlan fork_plan(const Pool& p, int nseq, int width) {
+  ForkPlan w;
+  w.next = 16;
+  w.mid = w.next + (int64_t)nseq * sizeof(Next);
+  w.free = w.mid + up16((int64_t)nseq * width * 4);
+  w.bytes = w.free + up16((int64_t)p.pages * 4);
+  return w;
+}
+struct CompactPlan {
+  int chunks;
+  int64_t counts, code, holes, movers, bytes;  // offsets; total comes first
+};
+CompactPlan compact_plan(const Pool& p) {
+  CompactPlan w;
+  w.chunks = (int)(((int64_t)p.pages + kChunk - 1) / kChunk);
+  w.counts = 16;
+  w.code = w.counts + up16((int64_t)w.chunks * 4);
+  w.holes = w.code + up16((int64_t)p.pages * 4);
+  w.movers = w.holes + up16(((int64_t)p.pages / 2 + 1) * 4);
+  w.bytes = w.movers + up16(((int64_t)p.pages / 2 + 1) * 4);
+  return w;
+}
+
+int check_ws(const char* op, const void* ws, int64_t given, int64_t need) {
+  if (!ws || ((uintptr_t)ws & 15) || given < need)
+    return op_fail(ANE_ERR_ARG, "storiesane %s: workspace of %lld bytes, want %lld, 16-byte aligned", op,
+                   (long long)(ws ? given : 0), (long long)need);
+  return ANE_OK;
+}
+int launched(const char* op) {
+  const hipError_t h = hipGetLastError();
+  return h == hipSuccess ? ANE_OK : op_fail(ANE_ERR_HIP, "storiesane %s: %s", op, hipGetErrorString(h));
+}
+int device_error(const char* op, int device, hipError_t h) {
+  return op_fail(ANE_ERR_HIP, "storiesane %s: device %d: %s", op, device, hipGetErrorString(h));
+}
+
+}  // namespace
+
+}  // namespace ane
+
+using namespace ane;
+
+extern "C" int64_t ane_kv8_fork_workspace(const ane_kv8_pool* pool, int32_t nseq, int32_t table_pages) {
+  const char* op = "kv8 fork workspace";
+  Pool p;
+  int rc = check_pool(op, pool, false, &p);
+  if (!rc) rc = check_table(op, &table_pages, table_pages, table_pages, nseq, p.pshift);
+  return rc ? rc : fork_plan(p, nseq, table_pages).bytes;
+}
+
+extern "C" int ane_kv8_fork(const ane_kv8_pool* pool, const ane_kv8_fork_args* args, void* stream) {
+  const char* op = "kv8 fork";
+  ForkArgs a;
+  int rc = check_pool(op, pool, true, &a.p);
+  if (rc) return rc;
+  if (!args) return op_fail(ANE_ERR_ARG, "storiesane %s: null arguments", op);
+  const ane_kv8_fork_args& g = *args;
+  rc = check_table(op, g.table, g.table_stride, g.table_pages, g.nseq, a.p.pshift);
+  if (rc) return rc;
+  if (!g.missing || (g.nseq > 0 && !g.start)) return op_fail(ANE_ERR_ARG, "storiesane %s: null buffer", op);
+  if (!g.news && g.new_tokens < 0) return op_fail(ANE_ERR_ARG, "storiesane %s: new_tokens=%d", op, g.new_tokens);
+  const Buffer buffers[] = {{"table", row_major(g.table, g.nseq, g.table_stride * 4ll, g.table_pages * 4ll), true},
+                            {"start", flat(g.start, g.nseq * 4ll), true},
+                            {"parents", flat(g.parents, g.nseq * 4ll), false},
+                            {"news", flat(g.news, g.nseq * 4ll), false},
+                            {"missing", flat(g.missing, 4), true},
+                            {"refs", flat(pool->refs, a.p.pages * 4ll), true}};
+  rc = check_apart(op, buffers, sizeof buffers / sizeof *buffers);
+  if (rc) return rc;
+  const ForkPlan w = fork_plan(a.p, g.nseq, g.table_pages);
+  rc = check_ws(op, g.ws, g.ws_bytes, w.bytes);
+  if (rc) return rc;
+  const int device = pool->layers[0].device;
+  DeviceScope dev(device);
+  if (dev.status() != hipSuccess) return device_error(op, device, dev.status());
+  a.table = g.table; a.start = g.start; a.refs = pool->refs; a.missing = g.missing;
+  a.parents = g.parents; a.news = g.news;
+  a.stride = g.table_stride; a.width = g.table_pages; a.nseq = g.nseq; a.new_tokens = g.new_tokens;
+  char* ws = (char*)g.ws;
+  a.found = (int*)ws;
+  a.next = (Next*)(ws + w.next);
+  a.mid = (int*)(ws + w.mid);
+  a.free = (int*)(ws + w.free);
+  const hipStream_t st = (hipStream_t)stream;
+  const int table_blocks = a.nseq * ((a.width + 255) / 256);
+  if (table_blocks > 0) hipLaunchKernelGGL(rows_kernel, dim3(table_blocks), dim3(256), 0, st, a);
+  hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(kTh), 0, st, a);
+  for (int l0 = 0; l0 < pool->nlayers && a.nseq > 0; l0 += kMaxLayers) {
+    Layers x;
+    const int n = layers_of(*pool, l0, &x);
+    const int tb = l0 == 0 ? table_blocks : 0;
+    hipLaunchKernelGGL(finish_kernel, dim3(tb + a.nseq * 2 * n), dim3(256), 0, st, a, x, n, tb);
+  }
+  return launched(op);
+}
+
+extern "C" int64_t ane_kv8_compact_workspace(const ane_kv8_pool* pool) {
+  Pool p;
+  const int rc = check_pool("kv8 compact workspace", pool, false, &p);
+  return rc ? rc : compact_plan(p).bytes;
+}
+
+extern "C" int ane_kv8_compact(const ane_kv8_pool* pool, const ane_kv8_compact_args* args, void* stream) {
+  const char* op = "kv8 compact";
+  CompactArgs a;
+  int rc = check_pool(op, pool, true, &a.p);
+  if (rc) return rc;
+  if (!args || !args->moved) return op_fail(ANE_ERR_ARG, "storiesane %s: null arguments", op);
+  const ane_kv8_compact_args& g = *args;
+  rc = check_table(op, g.table, g.table_stride, g.table_pages, g.nseq, a.p.pshift);
+  if (rc) return rc;
+  const Buffer buffers[] = {{"table", row_major(g.table, g.nseq, g.table_stride * 4ll, g.table_pages * 4ll), true},
+                            {"moved", flat(g.moved, a.p.pages * 4ll), true},
+                            {"refs", flat(pool->refs, a.p.pages * 4ll), true}};
+  rc = check_apart(op, buffers, sizeof buffers / sizeof *buffers);
+  if (rc) return rc;
+  const CompactPlan w = compact_plan(a.p);
+  rc = check_ws(op, g.ws, g.ws_bytes, w.bytes);
+  if (rc) return rc;
+  const int device = pool->layers[0].device;
+  DeviceScope dev(device);
+  if (dev.status() != hipSuccess) return device_error(op, device, dev.status());
+  a.table = g.table; a.refs = pool->refs; a.moved = g.moved;
+  a.stride = g.table_stride; a.width = g.nseq > 0 ? g.table_pages : 0; a.nseq = g.nseq;
+  a.chunks = w.chunks;
+  char* ws = (char*)g.ws;
+  a.total = (int*)ws;
+  a.counts = (int*)(ws + w.counts);
+  a.code = (int*)(ws + w.code);
+  a.holes = (int*)(ws + w.holes);
+  a.movers = (int*)(ws + w.movers);
+  const hipStream_t st = (hipStream_t)stream;
+  hipLaunchKernelGGL(count_kernel, dim3(a.chunks), dim3(kTh), 0, st, a);
+  hipLaunchKernelGGL(rank_kernel, dim3(a.chunks), dim3(kTh), 0, st, a);
+  const int book = (int)(((int64_t)a.p.pages + (int64_t)a.nseq * a.width + 255) / 256);
+  for (int l0 = 0; l0 < pool->nlayers; l0 += kMaxLayers) {
+    Layers x;
+    const int n = layers_of(*pool, l0, &x);
+    const int bb = l0 == 0 ? book : 0;
+    const int items = std::min(std::max(a.p.pages / 2, 1), 1024);
+    hipLaunchKernelGGL(move_kernel, dim3(bb + items * 2 * n), dim3(256), 0, st, a, x, n, bb);
+  }
+  return launched(op);
+}
+
+extern "C" int ane_kv8_copy(const ane_kv8_pool* from, const ane_kv8_pool* into, const ane_kv8_copy_args* args,
+                            void* stream) {
+  const char* op = "kv8 copy";
+  Pool p, q;
+  int rc = check_pool(op, from, false, &p);
+  if (!rc) rc = check_pool(op, into, false, &q);
+  if (rc) return rc;
+  if (from->nlayers != into->nlayers || p.pshift != q.pshift || p.NKV != q.NKV || p.dshift != q.dshift ||
+      from->layers[0].device != into->layers[0].device)
+    return op_fail(ANE_ERR_ARG, "storiesane %s: the pools differ in layers, page_tokens, kv_heads, head_dim or device", op);
+  if (!args) return op_fail(ANE_ERR_ARG, "storiesane %s: null arguments", op);
+  const ane_kv8_copy_args& g = *args;
+  if (g.n < 0 || g.n > 1 << 24) return op_fail(ANE_ERR_ARG, "storiesane %s: n=%d want 0..%d", op, g.n, 1 << 24);
+  if (g.n == 0) return ANE_OK;  // an empty tensor may have no address
+  if (!g.src || !g.dst) return op_fail(ANE_ERR_ARG, "storiesane %s: null buffer", op);
+  const int device = from->layers[0].device;
+  DeviceScope dev(device);
+  if (dev.status() != hipSuccess) return device_error(op, device, dev.status());
+  const hipStream_t st = (hipStream_t)stream;
+  for (int l0 = 0; l0 < from->nlayers; l0 += kMaxLayers) {
+    Layers x, y;
+    const int n = layers_of(*from, l0, &x);
+    layers_of(*into, l0, &y);
+    hipLaunchKernelGGL(copy_kernel, dim3(g.n * 2 * n), dim3(256), 0, st, p, q.pages, x, y, n, g.src, g.dst, g.tokens);
+  }
+  return launched(op);
+}

@@ -1,7 +1,8 @@
 /*
  * ane_serve.h -- serving operators of libane_hip.so on caller-owned device
- * memory: a paged key/value cache held in 8 bits (append, attention), and the
- * controls on logits before the next token is chosen.  No counterpart in the
+ * memory: a paged key/value cache held in 8 bits (append, attention, whole or
+ * over selected pages, and the tables of its pages), the controls on logits
+ * before the next token is chosen, and beam search.  No counterpart in the
  * reference, which evaluates whole windows only (ane/engine.go:954-1038); the
  * model they serve is that of ane_hip.h's decoder, built from the reference's
  * RoPE (ane/train_util.go:183-224) and causal softmax attention
@@ -170,6 +171,178 @@ typedef struct ane_logits_args {
 
 int64_t ane_control_logits_workspace(int32_t rows, int32_t vocab);
 int ane_control_logits(const ane_logits_args *args, void *stream);
+
+/* ---- beam search ---------------------------------------------------------------
+ * One step of `requests` searches with `beams` beams each; row r = request *
+ * beams + beam.  With x = logits (fp32, or fp16 where half is set) and NaN as
+ * -inf, sums in 64 bits:
+ *   lse[r] = log sum_v exp(x[r][v])
+ *   s(r, v) = scores[r] + (x[r][v] - lse[r]),  key(r, v) = weights[r] * s(r, v)
+ * and the request's `beams` candidates of the largest key become its next
+ * beams, the best first, equal keys in the order of beam, then token.  A beam
+ * that is finished has one candidate, itself: (r, eos) with s = scores[r].  No
+ * candidate: keys that are -inf or NaN, rows with scores -inf or NaN, weights
+ * that are not above 0, or +inf among their logits.
+ *   tokens, parents   the candidate's v and r (the row in the call, not within
+ *                     the request); ANE_NO_TOKEN and -1 where there are not
+ *                     enough candidates
+ *   scores_out        s, rounded to fp32 (-inf); may be scores
+ *   finished_out      1 where the parent was finished or the token is eos, else
+ *                     0 (also where there is no candidate); may be finished
+ *   history, lengths  move with their beams, in place: a row gets its parent's
+ *                     first lengths[parent] ids, and behind them the token if
+ *                     the parent was not finished and there is room; ids from
+ *                     the new length on stay as they are.  No candidate: length
+ *                     0, ids as they are.  Lengths are taken within [0,
+ *                     history_max].
+ * weights NULL: 1.  finished NULL with finished_out NULL and eos -1: beams do
+ * not finish.  history and lengths NULL: no histories
+ * (history NULL, history_max 0, with lengths: empty ones).
+ * beams 1..32, vocab 1..65535, at most 65535 rows.  logits: row stride
+ * logits_row; history: uint16, row stride history_row.  Outputs share no memory
+ * with each other or with inputs but where said.  ws as above. */
+typedef struct ane_beam_args {
+  const void *logits;
+  const float *scores, *weights;
+  const uint8_t *finished;
+  int32_t *tokens, *parents;
+  float *scores_out;
+  uint8_t *finished_out;
+  uint16_t *history;
+  int32_t *lengths;
+  int64_t logits_row, history_row;
+  int32_t requests, beams, vocab, eos, history_max, half, device;
+  void *ws;
+  int64_t ws_bytes;
+} ane_beam_args;
+
+int64_t ane_beam_select_workspace(int32_t requests, int32_t beams, int32_t vocab, int32_t half);
+int ane_beam_select(const ane_beam_args *args, void *stream);
+
+/* ---- bounds on the keys of a page ------------------------------------------------
+ * For each page and key/value head, of the keys it holds: unit, the smallest
+ * exponent e >= -30 at which every |k| <= 127 * 2^e, and box [2][head_dim], the
+ * largest (first) and smallest key of each dimension in that unit, rounded
+ * outwards.  NaN does not count; a dimension without a number has 0 and 0. */
+typedef struct ane_kv8_bounds {
+  int8_t *box;  /* [pages][kv_heads][2][head_dim], 16-byte aligned */
+  int8_t *unit; /* [pages][kv_heads] */
+} ane_kv8_bounds;
+
+/* The bounds of the pages that the batch's new tokens went to (append comes
+ * first), of all the sequence's tokens in them. */
+int ane_kv8_bound(const ane_kv8_cache *cache, const ane_kv8_bounds *bounds, const ane_kv8_batch *batch, void *stream);
+
+/* For each row of the batch and key/value head, the `count` pages of the row's
+ * sequence that its queries may match best.  A query becomes whole numbers z of
+ * a power of two 2^f, the smallest f >= -30 with |q| <= 127 * 2^f (to nearest,
+ * ties to even; infinities as 65504, NaN as 0); with the page's box and unit
+ *   score(page) = max over the group's query heads of
+ *                 2^(f + unit) * sum_d z_d * (z_d > 0 ? largest_d : smallest_d)
+ * which is exact in fp32, and no smaller than q . k of any key of the page but
+ * for the rounding of q.  The first `first` pages and the last `recent` ones up
+ * to the row's own position are always taken, then the largest scores, equal
+ * ones from the lower page.  Pages that are not there are not taken.
+ *
+ * blocks: int32 [rows][kv_heads][count], the pages' places in the sequence's
+ * table, rising, then -1.  Rows of no sequence are left as they are.
+ * q as in ane_kv8_attend.  count 1..65536, first and recent >= 0 and together
+ * at most count.  ws as above. */
+typedef struct ane_kv8_select_args {
+  const uint16_t *q;
+  int32_t *blocks;
+  int64_t q_row, q_head;
+  int32_t heads, count, first, recent;
+  void *ws;
+  int64_t ws_bytes;
+} ane_kv8_select_args;
+
+int64_t ane_kv8_select_workspace(const ane_kv8_cache *cache, const ane_kv8_batch *batch, int32_t heads, int32_t count);
+int ane_kv8_select(const ane_kv8_cache *cache, const ane_kv8_bounds *bounds, const ane_kv8_batch *batch,
+                   const ane_kv8_select_args *args, void *stream);
+
+/* ane_kv8_attend over the pages that `blocks` (as above) names for each row and
+ * key/value head, alone: the row at position p attends to the keys at positions
+ * 0..p in them.  Places outside [0, table_pages) and pages that are not there
+ * take no part; the order of the places does not matter, and a page named twice
+ * counts twice. */
+int64_t ane_kv8_attend_blocks_workspace(const ane_kv8_cache *cache, const ane_kv8_batch *batch, int32_t heads,
+                                        int32_t count);
+int ane_kv8_attend_blocks(const ane_kv8_cache *cache, const ane_kv8_batch *batch, const ane_kv8_attend_args *args,
+                          const int32_t *blocks, int32_t count, void *stream);
+
+/* ---- the tables of the pages -----------------------------------------------------
+ * A pool of pages that the caches of all layers share: page id i is page i of
+ * every layer (equal sizes, one device).  refs[i]: how many entries of tables
+ * name it; not above 0: free.  bounds: NULL, or one per layer, which then move
+ * with their pages (pointers NULL: that layer has none). */
+typedef struct ane_kv8_pool {
+  const ane_kv8_cache *layers;
+  const ane_kv8_bounds *bounds;
+  int32_t *refs; /* [pages] */
+  int32_t nlayers; /* 1..1024 */
+} ane_kv8_pool;
+
+/* Brings the table of nseq sequences to their next step, with `new` tokens each
+ * to come (news[i], or new_tokens where news is NULL; taken within [0, table's
+ * room]):
+ *  1. sequence i goes on from parents[i] (NULL: itself; outside [0, nseq): it
+ *     ends): start[i] = start[parents[i]] (0), taken within [0, table's room],
+ *     and its row is the parent's up to the page of its last token, -1 behind.
+ *     Smaller starts so cut sequences off, and 0 frees them.  refs follow.
+ *  2. A sequence with new tokens writes into the page of its last one, if that
+ *     is not full.  Where others hold that page too, it gets a page of its own,
+ *     with the tokens held so far (in all layers); the lowest sequence keeps the
+ *     page itself if all that hold it (by refs) are such sequences of this call.
+ *     A page that is not there stays so.
+ *  3. Positions of the new tokens without a page get one.
+ * The pages for 2 and 3 are the lowest free ones, in the order of sequence and
+ * position.  Where none is left, the entry is -1 (nothing is written there, and
+ * its tokens take no part in attention); *missing = the entries that have no
+ * page for such tokens, those of 2 that stay without one included.
+ *
+ * Copies take whole 16-token units; what a page holds behind them stays.
+ * A table names a page at most once per sequence. */
+typedef struct ane_kv8_fork_args {
+  int32_t *table, *start;
+  const int32_t *parents, *news;
+  int32_t *missing; /* 1 */
+  int32_t table_stride, table_pages, nseq, new_tokens;
+  void *ws;
+  int64_t ws_bytes;
+} ane_kv8_fork_args;
+
+int64_t ane_kv8_fork_workspace(const ane_kv8_pool *pool, int32_t nseq, int32_t table_pages);
+int ane_kv8_fork(const ane_kv8_pool *pool, const ane_kv8_fork_args *args, void *stream);
+
+/* Brings the U pages that are held (refs above 0) to the ids 0..U-1: those at U
+ * and beyond go, in order, to the free ones below U, in order.  moved[i] = where
+ * page i is now, -1 if it was free; refs follow, and so do the entries of the
+ * table (others outside [0, pages) stay; ones that name a free page become -1).
+ * nseq = 0: no table; further tables are the caller's, by `moved`. */
+typedef struct ane_kv8_compact_args {
+  int32_t *table;
+  int32_t *moved; /* [pages] */
+  int32_t table_stride, table_pages, nseq;
+  void *ws;
+  int64_t ws_bytes;
+} ane_kv8_compact_args;
+
+int64_t ane_kv8_compact_workspace(const ane_kv8_pool *pool);
+int ane_kv8_compact(const ane_kv8_pool *pool, const ane_kv8_compact_args *args, void *stream);
+
+/* Copies the pages src[i] of `from` to the pages dst[i] of `into` (the same pool
+ * or another of the same layers, page_tokens, kv_heads and head_dim; pages may
+ * differ), i < n: the 16-token units that hold their first tokens[i] tokens
+ * (NULL: all; taken within [0, page_tokens]; 0: nothing), exponents and, where
+ * both have them, bounds.  Ids outside the pools are passed over.  A page that
+ * is written twice, or read and written, holds either; refs are not looked at. */
+typedef struct ane_kv8_copy_args {
+  const int32_t *src, *dst, *tokens;
+  int32_t n;
+} ane_kv8_copy_args;
+
+int ane_kv8_copy(const ane_kv8_pool *from, const ane_kv8_pool *into, const ane_kv8_copy_args *args, void *stream);
 
 /* ---- for tests -----------------------------------------------------------------
  * The rows, positions and pages that a work item of the cache kernels takes,
