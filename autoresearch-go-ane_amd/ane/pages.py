@@ -123,8 +123,8 @@ class KVPages:
         self._empty, self._u8, self._stream = torch.empty, torch.uint8, _stream_getter()
         self._fork, self._compact, self._copy = (_lib.plain(self._lib, "ane_kv8_" + n)
                                                  for n in ("fork", "compact", "copy"))
-        self._bytes = {}  # of the workspaces, by sizes
-        _check(self._lib, self._lib.ane_kv8_compact_workspace(self._c))
+        self._bytes = {}  # of a fork's workspace, by the table's size
+        self._compact_bytes = _check(self._lib, self._lib.ane_kv8_compact_workspace(self._c))
 
     @classmethod
     def Empty(cls, caches, bounds=None):
@@ -136,6 +136,13 @@ class KVPages:
 
     def _table(self, op, t):
         """(address, stride, pages, sequences)."""
+        try:
+            n, w = t.shape
+            sn, sw = t.stride()
+            if t.dtype in self._i32 and t.get_device() == self._index and (sw == 1 or w == 1) and 0 < w <= sn < 1 << 31:
+                return t.data_ptr(), sn, w, n
+        except (AttributeError, ValueError):
+            pass
         p = _tensor(op, "table", t, self._i32, self.device, dims=2)
         n, w = (int(x) for x in t.shape)
         if w < 1:
@@ -145,11 +152,13 @@ class KVPages:
             _fail(op, f"table's rows are {stride} apart")
         return p, stride, w, n
 
-    def _work(self, key, size):
-        n = self._bytes.get(key)
-        if n is None:
-            n = self._bytes[key] = _check(self._lib, size())
-        return self._empty(n, dtype=self._u8, device=self.device), n
+    def _vector(self, op, name, t, n):
+        try:
+            if t.dtype in self._i32 and t.get_device() == self._index and t.shape == (n,) and t.is_contiguous():
+                return t.data_ptr()
+        except AttributeError:
+            pass
+        return _whole(op, name, t, self._i32, self.device, shape=(n,))
 
     def Fork(self, table, start, parents=None, new=1, missing=None):
         """Takes table int32 [nseq, pages] and start int32 [nseq] (the tokens
@@ -162,19 +171,22 @@ class KVPages:
         page, which are -1."""
         op = "kv8 fork"
         tp, stride, width, nseq = self._table(op, table)
-        sp = _whole(op, "start", start, self._i32, self.device, shape=(nseq,))
-        pp = 0 if parents is None else _whole(op, "parents", parents, self._i32, self.device, shape=(nseq,))
+        sp = self._vector(op, "start", start, nseq)
+        pp = 0 if parents is None else self._vector(op, "parents", parents, nseq)
         each = np_ = 0
         if hasattr(new, "data_ptr"):
-            np_ = _whole(op, "new", new, self._i32, self.device, shape=(nseq,))
+            np_ = self._vector(op, "new", new, nseq)
         else:
             each = int(new)
             if not 0 <= each < 1 << 31:
                 _fail(op, f"new={new}")
         if missing is None:
             missing = self._empty(1, dtype=self._i32[0], device=self.device)
-        mp = _whole(op, "missing", missing, self._i32, self.device, shape=(1,))
-        ws, n = self._work((nseq, width), lambda: self._lib.ane_kv8_fork_workspace(self._c, nseq, width))
+        mp = self._vector(op, "missing", missing, 1)
+        n = self._bytes.get((nseq, width))
+        if n is None:
+            n = self._bytes[nseq, width] = _check(self._lib, self._lib.ane_kv8_fork_workspace(self._c, nseq, width))
+        ws = self._empty(n, dtype=self._u8, device=self.device)
         a = _lib.pack_fork(tp, sp, pp, np_, mp, stride, width, nseq, each, ws.data_ptr(), n)
         rc = self._fork(self._at, a, self._stream(self._index))
         if rc:
@@ -192,8 +204,9 @@ class KVPages:
             tp, stride, width, nseq = self._table(op, table)
         if moved is None:
             moved = self._empty(self.pages, dtype=self._i32[0], device=self.device)
-        mp = _whole(op, "moved", moved, self._i32, self.device, shape=(self.pages,))
-        ws, n = self._work((), lambda: self._lib.ane_kv8_compact_workspace(self._c))
+        mp = self._vector(op, "moved", moved, self.pages)
+        n = self._compact_bytes
+        ws = self._empty(n, dtype=self._u8, device=self.device)
         a = _lib.pack_compact(tp, mp, stride, width, nseq, ws.data_ptr(), n)
         rc = self._compact(self._at, a, self._stream(self._index))
         if rc:
@@ -208,9 +221,9 @@ class KVPages:
         op = "kv8 copy"
         to = self if into is None else into
         n = int(src.shape[0]) if hasattr(src, "shape") and src.dim() == 1 else 0
-        sp = _whole(op, "src", src, self._i32, self.device, dims=1)
-        dp = _whole(op, "dst", dst, self._i32, self.device, shape=(n,))
-        kp = 0 if tokens is None else _whole(op, "tokens", tokens, self._i32, self.device, shape=(n,))
+        sp = self._vector(op, "src", src, n)
+        dp = self._vector(op, "dst", dst, n)
+        kp = 0 if tokens is None else self._vector(op, "tokens", tokens, n)
         rc = self._copy(self._at, to._at, _lib.pack_copy(sp, dp, kp, n), self._stream(self._index))
         if rc:
             _check(self._lib, rc)

@@ -62,6 +62,20 @@ def _whole(op, name, t, dtypes, device, dims=None, shape=None):
     return p
 
 
+def _matrix(op, name, t, dtypes, index):
+    """(address, stride of rows, rows, columns); one row has no stride that
+    matters."""
+    try:
+        n, w = t.shape
+        sn, sw = t.stride()
+        if t.dtype in dtypes and t.get_device() == index and (sw == 1 or w <= 1 or n == 0):
+            return t.data_ptr(), sn if n > 1 else max(sn, w), n, w
+    except (AttributeError, ValueError):
+        pass
+    _tensor(op, name, t, dtypes, _torch().device("cuda", index), dims=2)  # says what is wrong with it
+    _fail(op, f"{name} is not a matrix of rows")
+
+
 def _on_gpu(op, t):
     if not hasattr(t, "device") or t.device.type != "cuda":
         _fail(op, "tensors must be on a GPU")
@@ -137,7 +151,7 @@ class KVCache8:
         self.k, self.v, self.k_exp, self.v_exp = k, v, k_exp, v_exp
         self.device, self.kv_heads, self.head_dim = dev, kvh, dh
         self.pages, self.page_tokens = pages, page
-        self._half, self._f32 = torch.float16, (torch.float32,)
+        self._half, self._f32, self._i32 = torch.float16, (torch.float32,), torch.int32
         self._index = dev.index
         self._empty, self._u8, self._stream = torch.empty, torch.uint8, _stream_getter()
         self._c = _lib.Kv8Cache(kp, vp, ke, ve, pages, page, kvh, dh, dev.index)
@@ -253,7 +267,14 @@ class KVCache8:
 
     def _blocks(self, op, t, batch):
         """(address, count) of int32 [rows, kv_heads, count]."""
-        _whole(op, "blocks", t, (_torch().int32,), self.device, dims=3)
+        try:
+            r, h, n = t.shape
+            if (t.dtype is self._i32 and t.get_device() == self._index and r == batch.rows and h == self.kv_heads
+                    and t.is_contiguous()):
+                return t.data_ptr(), n
+        except (AttributeError, ValueError):
+            pass
+        _whole(op, "blocks", t, (self._i32,), self.device, dims=3)
         if tuple(t.shape[:2]) != (batch.rows, self.kv_heads):
             _fail(op, f"blocks has shape {tuple(t.shape)}, want ({batch.rows}, {self.kv_heads}, count)")
         return t.data_ptr(), int(t.shape[2])
@@ -323,12 +344,12 @@ class LogitControls:
             _on_gpu(op, logits)
         if self._index is not None and index != self._index:
             _fail(op, f"logits are on {logits.device}, the controls on {self.device}")
-        lp, lr, rows, vocab = self._matrix("logits", logits, self._f32, index)
+        lp, lr, rows, vocab = _matrix(op, "logits", logits, self._f32, index)
         if vocab != self.vocab or (self.rows is not None and rows != self.rows):
             _fail(op, f"logits have shape {tuple(logits.shape)}, want ({self.rows or 'rows'}, {self.vocab})")
         if out is None:
             out = self._empty((rows, vocab), dtype=logits.dtype, device=logits.device)
-        yp, yr, yn, yv = self._matrix("out", out, self._f32, index)
+        yp, yr, yn, yv = _matrix(op, "out", out, self._f32, index)
         if yn != rows or yv != vocab:
             _fail(op, f"out has shape {tuple(out.shape)}, want ({rows}, {vocab})")
         if tokens is None:
@@ -336,7 +357,7 @@ class LogitControls:
         tp = self._vector("tokens", tokens, index, rows)
         hp = hr = np_ = pp = most = 0
         if history is not None:
-            hp, hr, hn, most = self._matrix("history", history, self._u16, index)
+            hp, hr, hn, most = _matrix(op, "history", history, self._u16, index)
             if hn != rows:
                 _fail(op, f"history has {hn} rows, want {rows}")
             if lengths is None:
@@ -360,18 +381,6 @@ class LogitControls:
             _check(self._lib, rc)
         return out, tokens
 
-    def _matrix(self, name, t, dtypes, index):
-        """(address, stride of rows, rows, columns)."""
-        try:
-            n, w = t.shape
-            sn, sw = t.stride()
-            if t.dtype in dtypes and t.get_device() == index and (sw == 1 or w <= 1 or n == 0):
-                return t.data_ptr(), sn if n > 1 else max(sn, w), n, w
-        except (AttributeError, ValueError):
-            pass
-        _tensor(self._op, name, t, dtypes, _torch().device("cuda", index), dims=2)  # says what is wrong with it
-        _fail(self._op, f"{name} is not a matrix of rows")
-
     def _vector(self, name, t, index, rows):
         if t.dtype is self._i32[0] and t.get_device() == index and t.shape == (rows,) and t.is_contiguous():
             return t.data_ptr()
@@ -387,6 +396,7 @@ class BeamSearch:
         torch = _torch()
         self._op = "beam select"
         self.vocab, self.beams, self.eos = int(vocab), int(beams), None if eos is None else int(eos)
+        self._eos = -1 if eos is None else self.eos
         self._lib = _lib.load()
         _check(self._lib, self._lib.ane_beam_select_workspace(0, self.beams, self.vocab, 0))
         if eos is not None and not 0 <= self.eos < self.vocab:
@@ -398,10 +408,13 @@ class BeamSearch:
         self._bytes = {}  # of the workspace, by rows and type
         self._select = _lib.plain(self._lib, "ane_beam_select")
 
-    def _vector(self, name, t, dtypes, dev, rows):
-        if t.dtype in dtypes and t.device == dev and t.dim() == 1 and t.shape[0] == rows and t.is_contiguous():
-            return t.data_ptr()
-        return _whole(self._op, name, t, dtypes, dev, shape=(rows,))
+    def _vector(self, name, t, dtypes, index, rows):
+        try:
+            if t.dtype in dtypes and t.get_device() == index and t.shape == (rows,) and t.is_contiguous():
+                return t.data_ptr()
+        except AttributeError:
+            pass
+        return _whole(self._op, name, t, dtypes, _torch().device("cuda", index), shape=(rows,))
 
     def Select(self, logits, scores, finished=None, weights=None, history=None, lengths=None, tokens=None,
                parents=None, scores_out=None, finished_out=None):
@@ -417,49 +430,45 @@ class BeamSearch:
         Where a request has fewer candidates than beams, the last ones are
         (NO_TOKEN, -1, -inf)."""
         op = self._op
-        dev = _on_gpu(op, logits)
-        half = self._types.get(logits.dtype)
-        if half is None:
-            _fail(op, f"logits are {logits.dtype}, want torch.float32 or torch.float16")
-        lp = _tensor(op, "logits", logits, (logits.dtype,), dev, dims=2)
-        rows = int(logits.shape[0])
-        if logits.shape[1] != self.vocab or rows % self.beams:
+        index = logits.get_device() if hasattr(logits, "get_device") else -1
+        if index < 0:
+            _on_gpu(op, logits)
+        lp, lr, rows, vocab = _matrix(op, "logits", logits, self._types, index)
+        half = self._types[logits.dtype]
+        if vocab != self.vocab or rows % self.beams:
             _fail(op, f"logits have shape {tuple(logits.shape)}, want (requests * {self.beams}, {self.vocab})")
         if (finished is None) != (self.eos is None):
             _fail(op, "finished and eos go together")
         if (history is None) != (lengths is None):
             _fail(op, "history without lengths" if lengths is None else "lengths without a history")
-        new = self._empty
+        new, dev, vector = self._empty, logits.device, self._vector
         tokens = new(rows, dtype=self._i32[0], device=dev) if tokens is None else tokens
         parents = new(rows, dtype=self._i32[0], device=dev) if parents is None else parents
         scores_out = new(rows, dtype=self._f32[0], device=dev) if scores_out is None else scores_out
-        sp = self._vector("scores", scores, self._f32, dev, rows)
-        wp = 0 if weights is None else self._vector("weights", weights, self._f32, dev, rows)
+        sp = vector("scores", scores, self._f32, index, rows)
+        wp = 0 if weights is None else vector("weights", weights, self._f32, index, rows)
         fp = fo = hp = hr = most = np_ = 0
         if finished is not None:
-            fp = self._vector("finished", finished, self._flag, dev, rows)
-            fo = fp if finished_out is None else self._vector("finished_out", finished_out, self._flag, dev, rows)
+            fp = vector("finished", finished, self._flag, index, rows)
+            fo = fp if finished_out is None else vector("finished_out", finished_out, self._flag, index, rows)
         elif finished_out is not None:
             _fail(op, "finished_out without finished")
         if history is not None:
-            hp = _tensor(op, "history", history, self._u16, dev, dims=2)
-            if history.shape[0] != rows:
-                _fail(op, f"history has {history.shape[0]} rows, want {rows}")
-            most = int(history.shape[1])
-            hr = LogitControls._row(history)
-            np_ = self._vector("lengths", lengths, self._i32, dev, rows)
-        tp = self._vector("tokens", tokens, self._i32, dev, rows)
-        pp = self._vector("parents", parents, self._i32, dev, rows)
-        so = self._vector("scores_out", scores_out, self._f32, dev, rows)
+            hp, hr, hn, most = _matrix(op, "history", history, self._u16, index)
+            if hn != rows:
+                _fail(op, f"history has {hn} rows, want {rows}")
+            np_ = vector("lengths", lengths, self._i32, index, rows)
+        tp = vector("tokens", tokens, self._i32, index, rows)
+        pp = vector("parents", parents, self._i32, index, rows)
+        so = vector("scores_out", scores_out, self._f32, index, rows)
         n = self._bytes.get((rows, half))
         if n is None:
             n = self._bytes[rows, half] = _check(
                 self._lib, self._lib.ane_beam_select_workspace(rows // self.beams, self.beams, self.vocab, half))
         ws = self._empty(n, dtype=self._u8, device=dev)
-        a = _lib.pack_beam(lp, sp, wp, fp, tp, pp, so, fo, hp, np_, LogitControls._row(logits), hr,
-                           rows // self.beams, self.beams, self.vocab, -1 if self.eos is None else self.eos, most,
-                           half, dev.index, ws.data_ptr(), n)
-        rc = self._select(a, self._stream(dev.index))
+        a = _lib.pack_beam(lp, sp, wp, fp, tp, pp, so, fo, hp, np_, lr, hr, rows // self.beams, self.beams, vocab,
+                           self._eos, most, half, index, ws.data_ptr(), n)
+        rc = self._select(a, self._stream(index))
         if rc:
             _check(self._lib, rc)
         return tokens, parents, scores_out

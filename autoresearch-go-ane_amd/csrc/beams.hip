@@ -25,15 +25,24 @@ namespace {
 
 constexpr int kSeg = 256;       // entries of a segment
 constexpr int kMaxBeams = 32;   // of a request
-constexpr int kTh = 1024;       // threads of the second launch
-constexpr int kPer = 8;         // items a thread of it holds
-static_assert(kMaxBeams * (65536 / kSeg) <= kTh * kPer && kMaxBeams * kSeg <= kTh * kPer, "");
+constexpr int kPer = 8;         // items a thread of the second launch holds
+constexpr int kFew = 8;         // beams for which 256 threads of it are enough
+constexpr int kMaxParts = 128;  // of a row
+constexpr int kWords = 1024;    // of 8 ids: the histories of a request that a block holds
+static_assert(kMaxBeams * (65536 / kSeg) <= 1024 * kPer && kMaxBeams * kSeg <= 1024 * kPer, "");
+static_assert(kFew * (65536 / kSeg) <= 256 * kPer && kFew * kSeg <= 256 * kPer, "");
 
 // a wave's part of a row's log sum
 struct Part {
   double sum;  // of exp(x - max)
   float max;
   int pad;
+};
+
+// where a row's history comes from (-1: nowhere), how long that is, and the
+// token behind it (-1: none)
+struct Move {
+  int from, len, token;
 };
 
 struct BeamArgs {
@@ -47,7 +56,10 @@ struct BeamArgs {
   int* lengths;
   int64_t logits_row, history_row;
   int beams, vocab, eos, history_max;
-  int segs, parts;  // of a row
+  int segs, parts;     // of a row
+  int words, stretch;  // of 8 ids: of a history; of one that a block moves at a time
+  uint32_t words_magic;
+  Move* moves;         // [rows], where histories have a launch of their own
   float* seg_max;   // [rows][segs]
   Part* part;       // [rows][parts]
 };
@@ -55,6 +67,26 @@ struct BeamArgs {
 typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));
 typedef _Float16 half8u __attribute__((ext_vector_type(8), aligned(2)));
 typedef uint16_t ushort8u __attribute__((ext_vector_type(8), aligned(2)));
+
+// ids c .. c + 7 of a history of n > c (behind the last: anything)
+__device__ __forceinline__ ushort8u get_ids(const uint16_t* h, int c, int n) {
+  if (c + 8 <= n) return *reinterpret_cast<const ushort8u*>(h + c);
+  ushort8u v;
+#pragma unroll
+  for (int j = 0; j < 8; j++) v[j] = h[min(c + j, n - 1)];
+  return v;
+}
+__device__ __forceinline__ void put_ids(uint16_t* h, int c, int n, ushort8u v) {
+  if (c + 8 <= n) {
+    *reinterpret_cast<ushort8u*>(h + c) = v;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; j++)
+      if (c + j < n) h[c + j] = v[j];
+  }
+}
+// t / n for t below 2^16; magic = ceil(2^32 / n)
+__device__ __forceinline__ int quotient(int t, int n, uint32_t magic) { return n == 1 ? t : (int)__umulhi(t, magic); }
 
 // a beam that has continuations: alive, and not finished
 __device__ __forceinline__ bool proposes(const BeamArgs& a, int r) {
@@ -82,6 +114,43 @@ __device__ __forceinline__ void load_row(const T* row, int c, int vocab, float (
   for (int j = 0; j < N; j++) x[j] = x[j] == x[j] ? x[j] : -INFINITY;
 }
 
+// the value of the lane N further on in the row of 16
+template <int N>
+__device__ __forceinline__ int row_ror(int v) {
+  return __builtin_amdgcn_update_dpp(0, v, 0x120 + N, 0xf, 0xf, false);
+}
+template <int N>
+__device__ __forceinline__ double row_ror(double v) {
+  return __hiloint2double(row_ror<N>(__double2hiint(v)), row_ror<N>(__double2loint(v)));
+}
+template <int N>
+__device__ __forceinline__ float row_ror(float v) {
+  return __int_as_float(row_ror<N>(__float_as_int(v)));
+}
+// in every lane: the largest, and the sum (the same order of additions in all)
+__device__ __forceinline__ float wave_top(float v) {
+  v = fmaxf(v, row_ror<1>(v));
+  v = fmaxf(v, row_ror<2>(v));
+  v = fmaxf(v, row_ror<4>(v));
+  v = fmaxf(v, row_ror<8>(v));
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ double wave_total(double v) {
+  v += row_ror<1>(v);
+  v += row_ror<2>(v);
+  v += row_ror<4>(v);
+  v += row_ror<8>(v);
+  double s = 0.0;
+#pragma unroll
+  for (int r = 0; r < 4; r++)
+    s += __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(v), 16 * r),
+                          __builtin_amdgcn_readlane(__double2loint(v), 16 * r));
+  return s;
+}
+
 // A wave takes U loads of 64 N entries of a row.
 template <typename T, int U>
 __global__ __launch_bounds__(256) void part_kernel(BeamArgs a) {
@@ -100,11 +169,17 @@ __global__ __launch_bounds__(256) void part_kernel(BeamArgs a) {
     top[u] = x[u][0];
 #pragma unroll
     for (int j = 1; j < N; j++) top[u] = fmaxf(top[u], x[u][j]);
-#pragma unroll
-    for (int o = LS / 2; o > 0; o >>= 1) top[u] = fmaxf(top[u], __shfl_xor(top[u], o, 64));
-    m = fmaxf(m, top[u]);
+    top[u] = fmaxf(top[u], row_ror<1>(top[u]));
+    top[u] = fmaxf(top[u], row_ror<2>(top[u]));
+    top[u] = fmaxf(top[u], row_ror<4>(top[u]));
+    top[u] = fmaxf(top[u], row_ror<8>(top[u]));
+    const auto x16 = __builtin_amdgcn_permlane16_swap(__float_as_uint(top[u]), __float_as_uint(top[u]), false, false);
+    top[u] = fmaxf(__uint_as_float(x16[0]), __uint_as_float(x16[1]));
+    const auto x32 = __builtin_amdgcn_permlane32_swap(__float_as_uint(top[u]), __float_as_uint(top[u]), false, false);
+    const float both = fmaxf(__uint_as_float(x32[0]), __uint_as_float(x32[1]));
+    if (SPW == 1) top[u] = both;
+    m = fmaxf(m, both);
   }
-  if (SPW == 2) m = fmaxf(m, __shfl_xor(m, 32, 64));
   float s = 0.f;
   if (m > -INFINITY) {  // +inf: NaN, a row without candidates
 #pragma unroll
@@ -112,7 +187,7 @@ __global__ __launch_bounds__(256) void part_kernel(BeamArgs a) {
 #pragma unroll
       for (int j = 0; j < N; j++) s += __builtin_amdgcn_exp2f((x[u][j] - m) * 1.44269504088896340736f);
   }
-  const double sum = wave_sum_d((double)s);
+  const double sum = wave_total((double)s);
   float* seg = a.seg_max + (size_t)r * a.segs;
 #pragma unroll
   for (int u = 0; u < U; u++) {
@@ -128,177 +203,250 @@ constexpr int kNone = 1 << 30;
 struct Item {
   double key;
   int at;
+  float x;  // the logit behind it
 };
-__device__ __forceinline__ bool before(const Item& a, const Item& b) {
-  return a.key > b.key || (a.key == b.key && a.at < b.at);
+__device__ __forceinline__ bool before(double ak, int aa, double bk, int ba) {
+  return (ak > bk) | ((ak == bk) & (aa < ba));
 }
 
+template <int TH>
 struct Pick {
-  double key[kMaxBeams * 16 * kPer];  // those that may be among the best
-  int at[kMaxBeams * 16 * kPer];
-  double gkey[64];
-  int gat[64], grank[64];
-  int rank[64];
+  static constexpr int kBeams = TH == 256 ? kFew : kMaxBeams, kGroups = TH / 16;
+  double key[kBeams * 16 * kPer];  // those that may be among the best
+  int at[kBeams * 16 * kPer];
+  float x[kBeams * 16 * kPer];
+  double gkey[kGroups];
+  int gat[kGroups];
   int count;
-  Item bar;
+  double bar_key;
+  int bar_at;
 };
 
-// The `want` best of the block's items (kPer a thread, n of them used, keys
-// above -inf count), best(rank, item) called for each by some thread.
+template <int N>
+__device__ __forceinline__ void row_best(double& key, int& at) {
+  const double k = row_ror<N>(key);
+  const int i = row_ror<N>(at);
+  const bool b = before(k, i, key, at);
+  key = b ? k : key;
+  at = b ? i : at;
+}
+
+// The `want` best of the block's items (`per` a thread, keys above -inf count),
+// best(rank, item) called for each by one thread.
 //
-// The want-th best of 64 groups' best items is a bar that at least `want`
-// items reach and few others do; ranks are counted among those.  At most the
-// items of `want` groups reach it.
-template <typename F>
-__device__ __forceinline__ void pick(const Item (&x)[kPer], int per, int want, Pick& p, F best) {
-  const int tid = threadIdx.x, lane = tid & 63;
-  Item t = x[0];
+// The want-th best of the best items of groups of 16 threads is a bar that at
+// least `want` items reach and few others do; ranks are counted among those, a wave an item,
+// its lanes the others.  At most the items of `want` groups reach the bar.
+template <int TH, typename F>
+__device__ __forceinline__ void pick(const Item (&x)[kPer], int per, int want, Pick<TH>& p, F best) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  double key = x[0].key;
+  int at = x[0].at;
 #pragma unroll
-  for (int j = 1; j < kPer; j++)
-    if (j < per && before(x[j], t)) t = x[j];
-#pragma unroll
-  for (int o = 8; o > 0; o >>= 1) {
-    const Item y = {__shfl_xor(t.key, o, 64), __shfl_xor(t.at, o, 64)};
-    if (before(y, t)) t = y;
+  for (int j = 1; j < kPer; j++) {
+    if (j >= per) break;
+    const bool b = before(x[j].key, x[j].at, key, at);
+    key = b ? x[j].key : key;
+    at = b ? x[j].at : at;
   }
+  row_best<8>(key, at);
+  row_best<4>(key, at);
+  row_best<2>(key, at);
+  row_best<1>(key, at);
   if ((tid & 15) == 0) {
-    p.gkey[tid >> 4] = t.key;
-    p.gat[tid >> 4] = t.at;
-    p.grank[tid >> 4] = 0;
-    p.rank[tid >> 4] = 0;
+    p.gkey[tid >> 4] = key;
+    p.gat[tid >> 4] = at;
   }
   if (tid == 0) p.count = 0;
   __syncthreads();
-  const Item mine = {p.gkey[lane], p.gat[lane]};
-  int above = 0;
+  constexpr int GR = Pick<TH>::kGroups;
+  key = p.gkey[lane % GR];
+  at = p.gat[lane % GR];
 #pragma unroll
-  for (int j = 0; j < 4; j++) {
-    const int b = (tid >> 6) * 4 + j;
-    above += before({p.gkey[b], p.gat[b]}, mine);
+  for (int j = 0; j < 4; j++) {  // the groups have different items: one of them has this rank
+    const int b = wave * 4 + j;
+    const double bk = p.gkey[b];
+    const int ba = p.gat[b];
+    if (__popcll(__ballot(lane < GR && before(key, at, bk, ba))) == want - 1 && lane == 0) {
+      p.bar_key = bk;
+      p.bar_at = ba;
+    }
   }
-  if (above) atomicAdd(&p.grank[lane], above);
   __syncthreads();
-  if (tid < 64 && p.grank[tid] == want - 1) p.bar = mine;  // groups have different items: one has this rank
-  __syncthreads();
-  const Item bar = p.bar;
+  key = p.bar_key;
+  at = p.bar_at;
 #pragma unroll
-  for (int j = 0; j < kPer; j++)
-    if (j < per && x[j].key > -INFINITY && !before(bar, x[j])) {
+  for (int j = 0; j < kPer; j++) {
+    if (j >= per) break;
+    if ((x[j].key > -INFINITY) & !before(key, at, x[j].key, x[j].at)) {
       const int k = atomicAdd(&p.count, 1);
       p.key[k] = x[j].key;
       p.at[k] = x[j].at;
+      p.x[k] = x[j].x;
     }
+  }
   __syncthreads();
   const int n = p.count;
   if (n <= 64) {
-    if (lane < n) {
-      const Item me = {p.key[lane], p.at[lane]};
-      above = 0;
-      for (int b = tid >> 6; b < n; b += kTh / 64) above += before({p.key[b], p.at[b]}, me);
-      if (above) atomicAdd(&p.rank[lane], above);
+    key = p.key[min(lane, n)];
+    at = p.at[min(lane, n)];
+    for (int b = wave; b < n; b += TH / 64) {
+      const double bk = p.key[b];
+      const int ba = p.at[b];
+      const int rank = __popcll(__ballot(lane < n && before(key, at, bk, ba)));
+      if (rank < want && lane == 0) best(rank, Item{bk, ba, p.x[b]});
     }
-    __syncthreads();
-    if (tid < n && p.rank[tid] < want) best(p.rank[tid], Item{p.key[tid], p.at[tid]});
   } else {
-    for (int k = tid; k < n; k += kTh) {
-      const Item me = {p.key[k], p.at[k]};
-      above = 0;
-      for (int b = 0; b < n && above < want; b++) above += before({p.key[b], p.at[b]}, me);
-      if (above < want) best(above, me);
+    for (int k = tid; k < n; k += TH) {
+      key = p.key[k];
+      at = p.at[k];
+      int above = 0;
+      for (int b = 0; b < n && above < want; b++) above += before(p.key[b], p.at[b], key, at);
+      if (above < want) best(above, Item{key, at, p.x[k]});
     }
   }
   __syncthreads();
 }
 
-// A block per request.
-template <typename T>
-__global__ __launch_bounds__(kTh) void choose_kernel(BeamArgs a) {
-  __shared__ Pick pick_;
-  __shared__ double score[kMaxBeams], lse[kMaxBeams], weight[kMaxBeams];
-  __shared__ int state[kMaxBeams], length[kMaxBeams];  // 0: proposes nothing, 1: continuations, 2: itself
-  __shared__ int seg_of[kMaxBeams], parent[kMaxBeams], token[kMaxBeams];
-  __shared__ double score_of[kMaxBeams];
-  const int tid = threadIdx.x, lane = tid & 63, W = a.beams;
+// A block per request.  What bounds it is the chain of its memory accesses:
+// everything that does not depend on a choice is on its way first.
+template <typename T, int TH>
+__global__ __launch_bounds__(TH) void choose_kernel(BeamArgs a) {
+  constexpr int NW = TH / 64, MB = Pick<TH>::kBeams;
+  constexpr int BW = MB / NW, PL = kMaxParts / 64, HQ = kWords / TH;  // beams of a wave, parts and words of a lane
+  __shared__ Pick<TH> pick_;
+  // a beam's s(v) = score + (x - lse); one that is finished has lse 0 and the
+  // candidate x = 0, and one that proposes nothing has no number
+  __shared__ double score[MB], lse[MB], weight[MB], score_of[MB];
+  __shared__ int ended[MB], length[MB];
+  __shared__ int seg_of[MB], parent[MB], token[MB];  // seg_of: beam << 16 | segment, -1: none
+  __shared__ ushort8u hist[kWords];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), W = a.beams;
   const int row0 = blockIdx.x * W;
   const T* logits = static_cast<const T*>(a.logits);
-  for (int w = tid >> 6; w < W; w += kTh / 64) {
-    const int r = row0 + w;
-    const bool done = a.finished && a.finished[r];
-    const float sc = a.scores[r], wt = a.weights ? a.weights[r] : 1.f;
-    const bool live = sc > -INFINITY && wt > 0.f;
-    double sum = 0.0;
-    float m = -INFINITY;
-    if (live && !done) {
-      const Part* p = a.part + (size_t)r * a.parts;
-      for (int k = lane; k < a.parts; k += 64) {
-        const Part q = p[k];
-        if (q.max > -INFINITY) {
-          const float hi = fmaxf(m, q.max);
-          // the larger one's factor is 1 (infinities: NaN, as they should be)
-          sum = (m == hi ? sum : sum * exp((double)m - hi)) + (q.max == hi ? q.sum : q.sum * exp((double)q.max - hi));
-          m = hi;
-        }
-      }
+
+  // segments: 64 of a beam are a wave's at a time
+  const int runs = (a.segs + 63) >> 6;
+  int per = (W * runs + NW - 1) / NW;
+  Item x[kPer];
+#pragma unroll
+  for (int j = 0; j < kPer; j++) {
+    x[j] = {-INFINITY, kNone + j * TH + tid, -INFINITY};
+    if (j >= per) continue;
+    const int u = j * NW + wave, w = u / runs, seg = (u - w * runs) * 64 + lane;
+    if (w < W && seg < a.segs) {
+      x[j].x = a.seg_max[(size_t)(row0 + w) * a.segs + seg];
+      x[j].at = w << 16 | seg;
     }
-    const float top = wave_max(m);
-    sum = wave_sum_d(m > -INFINITY && m != top ? sum * exp((double)m - top) : sum);
-    if (lane == 0) {
-      score[w] = sc;
-      weight[w] = wt;
-      lse[w] = top + log(sum);
-      state[w] = !live ? 0 : done ? 2 : 1;
-      length[w] = a.lengths ? clampi(a.lengths[r], 0, a.history_max) : 0;
+  }
+  Part q[BW][PL];
+  float sc[BW], wt[BW];
+  int done[BW], len[BW];
+#pragma unroll
+  for (int i = 0; i < BW; i++) {
+    const int w = min(wave + i * NW, W - 1), r = row0 + w;
+    sc[i] = a.scores[r];
+    wt[i] = a.weights ? a.weights[r] : 1.f;
+    done[i] = a.finished ? a.finished[r] : 0;
+    len[i] = a.lengths ? a.lengths[r] : 0;
+#pragma unroll
+    for (int k = 0; k < PL; k++) {
+      q[i][k] = a.part[(size_t)r * a.parts + min(lane + 64 * k, a.parts - 1)];
+      if (lane + 64 * k >= a.parts) q[i][k] = {0.0, -INFINITY, 0};
+    }
+  }
+  ushort8u ids[HQ];
+  const int words = a.lengths && !a.moves ? W * a.words : 0;
+#pragma unroll
+  for (int k = 0; k < HQ; k++) {
+    const int t = k * TH + tid;
+    if (t < words) {
+      const int w = quotient(t, a.words, a.words_magic);
+      ids[k] = get_ids(a.history + (row0 + w) * a.history_row, (t - w * a.words) * 8, a.history_max);
+    }
+  }
+  double sum = 0.0, top = 0.0;
+#pragma unroll
+  for (int i = 0; i < BW; i++) {
+    float m = q[i][0].max;
+#pragma unroll
+    for (int k = 1; k < PL; k++) m = fmaxf(m, q[i][k].max);
+    m = wave_top(m);
+    // Factors of the parts in fp32: off by what a part's own exponentials are.
+    // An infinite maximum makes NaN, as it should.
+    double s = 0.0;
+#pragma unroll
+    for (int k = 0; k < PL; k++) {
+      const float f = __builtin_amdgcn_exp2f((q[i][k].max - m) * 1.44269504088896340736f);
+      s += q[i][k].max > -INFINITY ? q[i][k].sum * f : 0.0;
+    }
+    s = wave_total(s);
+    sum = lane == i ? s : sum;
+    top = lane == i ? (double)m : top;
+  }
+  const double l = top + log(sum);
+#pragma unroll
+  for (int i = 0; i < BW; i++) {
+    const int w = wave + i * NW;
+    if (lane == i && w < W) {
+      const bool live = sc[i] > -INFINITY && wt[i] > 0.f;
+      score[w] = sc[i];
+      weight[w] = wt[i];
+      lse[w] = !live ? (double)NAN : done[i] ? 0.0 : l;
+      ended[w] = done[i];
+      length[w] = clampi(len[i], 0, a.history_max);
       seg_of[w] = -1;
       parent[w] = -1;
       token[w] = ANE_NO_TOKEN;
       score_of[w] = -INFINITY;
     }
   }
+#pragma unroll
+  for (int k = 0; k < HQ; k++)
+    if (k * TH + tid < words) hist[k * TH + tid] = ids[k];
   __syncthreads();
-  const auto score_at = [&](int w, float x) { return score[w] + ((double)x - lse[w]); };
-  const auto key_of = [&](int w, double s) {
-    const double k = s * weight[w];
+  const auto key_of = [&](int w, float x) {
+    const double k = weight[w] * (score[w] + ((double)x - lse[w]));
     return k == k ? k : (double)-INFINITY;
   };
 
   // the best W segments
-  Item x[kPer];
-  int n = W * a.segs;
 #pragma unroll
   for (int j = 0; j < kPer; j++) {
-    const int t = j * kTh + tid;
-    x[j] = {-INFINITY, kNone + t};
-    if (t < n) {
-      x[j].at = t;
-      const int w = t / a.segs, g = t - w * a.segs;
-      if (state[w] == 1) x[j].key = key_of(w, score_at(w, a.seg_max[(size_t)(row0 + w) * a.segs + g]));
-      else if (state[w] == 2 && g == 0) x[j].key = key_of(w, score[w]);
-    }
+    if (j >= per) break;
+    const int w = min((j * NW + wave) / runs, W - 1);
+    if (ended[w]) x[j].x = (x[j].at & 0xffff) == 0 ? 0.f : -INFINITY;
+    if (x[j].at < kNone) x[j].key = key_of(w, x[j].x);
   }
-  pick(x, (n + kTh - 1) / kTh, W, pick_, [&](int rank, const Item& t) { seg_of[rank] = t.at; });
+  pick<TH>(x, per, W, pick_, [&](int rank, const Item& t) { seg_of[rank] = t.at; });
 
-  // the best W candidates in them
-  n = W * kSeg;
+  // the best W candidates in them, 64 of a segment a wave's at a time; an index
+  // is the beam and the token
+  per = (W * (kSeg / 64) + NW - 1) / NW;
 #pragma unroll
   for (int j = 0; j < kPer; j++) {
-    const int t = j * kTh + tid;
-    x[j] = {-INFINITY, kNone + t};
-    if (t < n && seg_of[t / kSeg] >= 0) {
-      const int w = seg_of[t / kSeg] / a.segs, v = (seg_of[t / kSeg] - w * a.segs) * kSeg + t % kSeg;
-      if (state[w] == 2) {
-        if (t % kSeg == 0) x[j] = {key_of(w, score[w]), w * a.vocab + a.eos};
-      } else if (v < a.vocab) {
-        x[j].at = w * a.vocab + v;
-        const float y = (float)logits[(row0 + w) * a.logits_row + v];
-        if (y == y) x[j].key = key_of(w, score_at(w, y));
-      }
+    x[j] = {-INFINITY, kNone + j * TH + tid, -INFINITY};
+    if (j >= per) continue;
+    const int u = j * NW + wave, seg = __builtin_amdgcn_readfirstlane(seg_of[min(u / (kSeg / 64), W - 1)]);
+    const int w = seg >> 16, i = u % (kSeg / 64) * 64 + lane, v = (seg & 0xffff) * kSeg + i;
+    if (seg < 0 || u >= W * (kSeg / 64)) continue;
+    if (ended[w]) {
+      if (i == 0) x[j] = {-INFINITY, w << 16 | a.eos, 0.f};
+    } else if (v < a.vocab) {
+      x[j].x = (float)logits[(row0 + w) * a.logits_row + v];
+      x[j].at = w << 16 | v;
     }
   }
-  pick(x, (n + kTh - 1) / kTh, W, pick_, [&](int rank, const Item& t) {
-    const int w = t.at / a.vocab, v = t.at - w * a.vocab;
+#pragma unroll
+  for (int j = 0; j < kPer; j++) {
+    if (j >= per) break;
+    if (x[j].at < kNone) x[j].key = key_of(x[j].at >> 16, x[j].x);
+  }
+  pick<TH>(x, per, W, pick_, [&](int rank, const Item& t) {
+    const int w = t.at >> 16;
     parent[rank] = w;
-    token[rank] = v;
-    score_of[rank] = state[w] == 2 ? score[w] : score_at(w, (float)logits[(row0 + w) * a.logits_row + v]);
+    token[rank] = t.at & 0xffff;
+    score_of[rank] = score[w] + ((double)t.x - lse[w]);
   });
 
   if (tid < W) {
@@ -306,57 +454,58 @@ __global__ __launch_bounds__(kTh) void choose_kernel(BeamArgs a) {
     a.tokens[r] = token[tid];
     a.parents[r] = w < 0 ? -1 : row0 + w;
     a.scores_out[r] = (float)score_of[tid];
-    if (a.finished_out) a.finished_out[r] = w >= 0 && (state[w] == 2 || token[tid] == a.eos);
+    if (a.finished_out) a.finished_out[r] = w >= 0 && (ended[w] || token[tid] == a.eos);
   }
   if (!a.lengths) return;
-
-  // The histories move with their beams: a stretch of columns at a time is read
-  // by the block before any of it is written.
-  int most = 0;
-  for (int w = 0; w < W; w++) most = max(most, parent[w] >= 0 && parent[w] != w ? length[parent[w]] : 0);
-  constexpr int Q = 4;
-  const int wide = kTh * Q / W;  // stretches of 8 ids
-  for (int c0 = 0; c0 * 8 < most; c0 += wide) {
-    ushort8u v[Q];
-    int c[Q], to[Q];
-#pragma unroll
-    for (int q = 0; q < Q; q++) {
-      const int t = q * kTh + tid, w = t / wide;
-      c[q] = (c0 + t - w * wide) * 8;
-      to[q] = -1;
-      if (w < W && parent[w] >= 0 && parent[w] != w && c[q] < length[parent[w]]) {
-        to[q] = w;
-        const uint16_t* h = a.history + (row0 + parent[w]) * a.history_row;
-        if (c[q] + 8 <= length[parent[w]]) {
-          v[q] = *reinterpret_cast<const ushort8u*>(h + c[q]);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; j++) v[q][j] = c[q] + j < length[parent[w]] ? h[c[q] + j] : 0;
-        }
-      }
+  if (a.moves) {  // in a launch of their own
+    if (tid < W) {
+      const int r = row0 + tid, w = parent[tid], len = w < 0 ? 0 : length[w];
+      const bool grows = w >= 0 && !ended[w] && len < a.history_max;
+      a.moves[r] = {w < 0 ? -1 : row0 + w, len, grows ? token[tid] : -1};
+      a.lengths[r] = len + grows;
     }
-    __syncthreads();
-#pragma unroll
-    for (int q = 0; q < Q; q++)
-      if (to[q] >= 0) {
-        uint16_t* h = a.history + (row0 + to[q]) * a.history_row;
-        const int len = length[parent[to[q]]];
-        if (c[q] + 8 <= len) {
-          *reinterpret_cast<ushort8u*>(h + c[q]) = v[q];
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; j++)
-            if (c[q] + j < len) h[c[q] + j] = v[q][j];
-        }
-      }
+    return;
   }
-  __syncthreads();
+  // the histories are in LDS
+#pragma unroll 1
+  for (int t = tid; t < words; t += TH) {
+    const int w = quotient(t, a.words, a.words_magic), c = t - w * a.words, from = parent[w];
+    if (from >= 0 && from != w) put_ids(a.history + (row0 + w) * a.history_row, c * 8, length[from], hist[from * a.words + c]);
+  }
   if (tid < W) {
     const int r = row0 + tid, w = parent[tid];
     int len = w < 0 ? 0 : length[w];
-    if (w >= 0 && state[w] == 1 && len < a.history_max) a.history[r * a.history_row + len++] = (uint16_t)token[tid];
+    if (w >= 0 && !ended[w] && len < a.history_max) a.history[r * a.history_row + len++] = (uint16_t)token[tid];
     a.lengths[r] = len;
   }
+}
+
+// The histories, where they are long: a block takes a stretch of columns of a
+// request's rows, all of which it reads before it writes any.
+__global__ __launch_bounds__(256) void move_kernel(BeamArgs a) {
+  __shared__ Move move[kMaxBeams];
+  const int tid = threadIdx.x, W = a.beams, row0 = blockIdx.y * W, c0 = blockIdx.x * a.stretch;
+  constexpr int Q = kWords / 256;
+  if (tid < W) move[tid] = a.moves[row0 + tid];
+  __syncthreads();
+  ushort8u v[Q];
+  int c[Q], to[Q];
+#pragma unroll
+  for (int q = 0; q < Q; q++) {
+    const int t = q * 256 + tid, w = t / a.stretch;
+    c[q] = (c0 + t - w * a.stretch) * 8;
+    to[q] = -1;
+    if (w < W && move[w].from >= 0 && move[w].from != row0 + w && c[q] < move[w].len) {
+      to[q] = w;
+      v[q] = get_ids(a.history + move[w].from * a.history_row, c[q], move[w].len);
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int q = 0; q < Q; q++)
+    if (to[q] >= 0) put_ids(a.history + (row0 + to[q]) * a.history_row, c[q], move[to[q]].len, v[q]);
+  if (tid < W && move[tid].token >= 0 && move[tid].len / 8 >= c0 && move[tid].len / 8 < c0 + a.stretch)
+    a.history[(row0 + tid) * a.history_row + move[tid].len] = (uint16_t)move[tid].token;
 }
 
 // Loads of a wave in the first launch.
@@ -364,7 +513,7 @@ int loads_of(int64_t rows, int vocab, bool half) { return 2; }
 
 struct Plan {
   int loads, segs, parts;
-  int64_t seg_bytes, bytes;
+  int64_t seg_bytes, move_bytes, bytes;
 };
 int plan(const char* op, int requests, int beams, int vocab, bool half, Plan* p) {
   if (requests < 0 || beams < 1 || beams > kMaxBeams || vocab < 1 || vocab > 65535 || (int64_t)requests * beams > 65535)
@@ -377,8 +526,17 @@ int plan(const char* op, int requests, int beams, int vocab, bool half, Plan* p)
   p->segs = (vocab + kSeg - 1) / kSeg;
   p->parts = (vocab + width - 1) / width;
   p->seg_bytes = (rows * p->segs * 4 + 15) / 16 * 16;
-  p->bytes = p->seg_bytes + rows * p->parts * (int64_t)sizeof(Part);
+  p->move_bytes = (rows * (int64_t)sizeof(Move) + 15) / 16 * 16;
+  p->bytes = p->seg_bytes + p->move_bytes + rows * p->parts * (int64_t)sizeof(Part);
   return ANE_OK;
+}
+
+uint32_t magic(int n) { return (uint32_t)(((1ull << 32) + n - 1) / n); }
+
+template <typename T>
+void launch_choose(const BeamArgs& a, int requests, hipStream_t st) {
+  if (a.beams <= kFew) hipLaunchKernelGGL((choose_kernel<T, 256>), dim3(requests), dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((choose_kernel<T, 1024>), dim3(requests), dim3(1024), 0, st, a);
 }
 
 }  // namespace
@@ -439,16 +597,22 @@ extern "C" int ane_beam_select(const ane_beam_args* args, void* stream) {
   a.beams = g.beams; a.vocab = g.vocab; a.eos = g.eos; a.history_max = g.history_max;
   a.segs = p.segs; a.parts = p.parts;
   a.seg_max = (float*)g.ws;
-  a.part = (Part*)((char*)g.ws + p.seg_bytes);
+  a.words = (g.history_max + 7) / 8;
+  a.words_magic = a.words ? magic(a.words) : 0;
+  a.stretch = kWords / g.beams;
+  a.moves = g.beams * a.words > kWords ? (Move*)((char*)g.ws + p.seg_bytes) : nullptr;
+  a.part = (Part*)((char*)g.ws + p.seg_bytes + p.move_bytes);
   const hipStream_t st = (hipStream_t)stream;
   const dim3 grid((p.parts + 3) / 4, (uint32_t)rows);
   if (g.half) {
     hipLaunchKernelGGL((part_kernel<half_t, 2>), grid, dim3(256), 0, st, a);
-    hipLaunchKernelGGL(choose_kernel<half_t>, dim3(g.requests), dim3(kTh), 0, st, a);
+    launch_choose<half_t>(a, g.requests, st);
   } else {
     hipLaunchKernelGGL((part_kernel<float, 2>), grid, dim3(256), 0, st, a);
-    hipLaunchKernelGGL(choose_kernel<float>, dim3(g.requests), dim3(kTh), 0, st, a);
+    launch_choose<float>(a, g.requests, st);
   }
+  if (a.moves)
+    hipLaunchKernelGGL(move_kernel, dim3((a.words + a.stretch - 1) / a.stretch, g.requests), dim3(256), 0, st, a);
   const hipError_t h = hipGetLastError();
   if (h != hipSuccess) return op_fail(ANE_ERR_HIP, "storiesane %s: %s", op, hipGetErrorString(h));
   return ANE_OK;

@@ -260,10 +260,14 @@ bool share_memory(Extent a, Extent b) {
 }
 
 int check_apart(const char* op, const Buffer* b, int n) {
-  for (int i = 0; i < n; i++)
+  const auto end = [](const Extent& e) {
+    return e.at + (e.rows > 1 ? (e.rows - 1) * e.row : 0) + (e.heads > 1 ? (e.heads - 1) * e.head : 0) + e.width;
+  };
+  for (int i = 1; i < n; i++)
     for (int j = 0; j < i; j++) {
       const Buffer &x = b[i], &y = b[j];
       if (!(x.out || y.out) || !x.at.at || !y.at.at) continue;
+      if (x.at.at >= end(y.at) || y.at.at >= end(x.at)) continue;
       if (x.pair && x.pair == y.pair && x.at.at == y.at.at) continue;
       if (share_memory(x.at, y.at)) return op_fail(ANE_ERR_ARG, "storiesane %s: %s overlaps %s", op, x.name, y.name);
     }

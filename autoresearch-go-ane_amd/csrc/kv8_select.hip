@@ -19,7 +19,9 @@ namespace {
 
 typedef int intx4 __attribute__((ext_vector_type(4)));
 
-constexpr int kUnitMin = -30;
+// Units of bounds that an update has written are in between (keys are at most
+// 448 * 2^8); of others they are taken so, and scores stay finite.
+constexpr int kUnitMin = -30, kUnitMax = 40;
 
 // the smallest exponent from kUnitMin on at which amax <= 127 * 2^e; amax finite, >= 0
 __device__ __forceinline__ int unit_of(float amax) {
@@ -127,41 +129,127 @@ struct SelectArgs {
   int* blocks;
   int64_t q_row, q_head;
   int G, count, first, recent;
+  int room;  // scores that LDS holds
 };
 
-// A page's place in the order of the choice: fp32 scores as whole numbers that
-// rise with them.
-constexpr uint32_t kNever = 0, kAlways = 0xffffffffu;
-__device__ __forceinline__ uint32_t key_of(float x) {
-  const uint32_t b = __float_as_uint(x);
-  return b >> 31 ? ~b : b | 0x80000000u;
+// Reductions over a wave, and over what its lanes hold NW-periodically.
+template <int N>
+__device__ __forceinline__ int row_ror(int v) {
+  return __builtin_amdgcn_update_dpp(0, v, 0x120 + N, 0xf, 0xf, false);
+}
+template <int N>
+__device__ __forceinline__ float row_ror(float v) {
+  return __int_as_float(row_ror<N>(__float_as_int(v)));
+}
+struct Max {
+  template <typename T>
+  __device__ T operator()(T a, T b) const { return a > b ? a : b; }
+};
+struct Sum {
+  __device__ int operator()(int a, int b) const { return a + b; }
+};
+template <typename T>
+__device__ __forceinline__ void swap16(T& a, T& b) {  // a's odd rows of 16 with b's even ones
+  const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b), false, false);
+  const uint32_t x = r[0], y = r[1];
+  a = __builtin_bit_cast(T, x);
+  b = __builtin_bit_cast(T, y);
+}
+template <typename T>
+__device__ __forceinline__ void swap32(T& a, T& b) {  // a's upper half with b's lower half
+  const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b), false, false);
+  const uint32_t x = r[0], y = r[1];
+  a = __builtin_bit_cast(T, x);
+  b = __builtin_bit_cast(T, y);
+}
+template <int N, typename T, typename Op>
+__device__ __forceinline__ T lanes(T v, Op op) {
+  if (N >= 2) v = op(v, row_ror<1>(v));
+  if (N >= 4) v = op(v, row_ror<2>(v));
+  if (N >= 8) v = op(v, row_ror<4>(v));
+  if (N >= 16) v = op(v, row_ror<8>(v));
+  if (N >= 32) {
+    T w = v;
+    swap16(v, w);
+    v = op(v, w);
+  }
+  if (N >= 64) {
+    T w = v;
+    swap32(v, w);
+    v = op(v, w);
+  }
+  return v;
+}
+// the sum over the lanes up to this one: within rows of 16, then the last lane
+// of a row to the row behind it, and of the lower half to the upper one
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int shifted(int v) {
+  return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ int sum_up_to(int v) {
+  v += shifted<0x111, 0xf>(v);
+  v += shifted<0x112, 0xf>(v);
+  v += shifted<0x114, 0xf>(v);
+  v += shifted<0x118, 0xf>(v);
+  v += shifted<0x142, 0xa>(v);
+  v += shifted<0x143, 0xc>(v);
+  return v;
 }
 
-constexpr int kKeys = 4096;  // pages whose keys are held at a time
+constexpr int kBins = 256;
+constexpr int kHeld = 1024;  // pages of a token whose scores its waves hold in registers
+constexpr int kFar = 32768;  // scores that LDS holds at most
 
-// NW waves a row and key/value head.  The keys of kKeys pages at a time lie in
-// LDS: all of a context that is no longer, otherwise each pass over the keys
-// computes them again.
-template <int DH, int NT, int NW>
+// A block takes up to 4, 2 or 1 tokens of a sequence (as their query heads, up
+// to 4, 8 or 16, or 32 with NT = 2, fill the 16 rows of a product) and a
+// key/value head.
+//
+// First its NW waves score the context's pages for all the tokens: 64 pages a
+// wave at a time, their ids with one load, their boxes in four products of 16.
+// Row 4 g + j of a product is token j / (4 / TOK) and head g + 4 (j % (4 / TOK)),
+// so that a token's heads are registers of a lane and rows of lanes.  Then each
+// token is CW waves' own: one's, which needs no barrier, or where there is one
+// token, all waves'.  Contexts that LDS does not hold are scored again, by those
+// waves, in each pass over the scores.
+//
+// The choice.  The score of the last page to be taken is narrowed down by
+// histograms between the lowest and the highest score in question, in steps of
+// equal width (a step's number rises with the score whatever the rounding),
+// until at most 64 pages are left, or ones that are all equal; then ranks are
+// counted.  The bin that the last page lies in has neither all of them nor
+// none, so every histogram leaves fewer.
+template <int DH, int NT, int TOK, int NW, int CW>
 __global__ __launch_bounds__(64 * NW) void select_kernel(SelectArgs a) {
   constexpr int NM = DH / 32;  // products of 64 terms
-  __shared__ uint32_t keys[kKeys];
-  __shared__ int sums[2][NW];
+  constexpr int HJ = 4 / TOK;  // registers of a token
+  static_assert(CW == 1 || CW == NW);
+  constexpr int CH = NW / CW, CT = 64 * CW, R = kHeld / CT;
+  extern __shared__ float scores[];  // [TOK][stride], room of them in all
+  __shared__ int bins_of[CH][kBins];
+  __shared__ float few_of[CH][64];
+  __shared__ int fews, sums[2][CW];
   const Kv8Batch& b = a.b;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, g = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  for (int i = tid; i < CH * kBins; i += 64 * NW) bins_of[0][i] = 0;
   const int h = blockIdx.x % b.NKV;
-  const Kv8Span span = kv8_tile_span(b, 1, blockIdx.x / b.NKV);
+  const Kv8Span span = kv8_tile_span(b, TOK, blockIdx.x / b.NKV);
   if (span.n == 0) return;
-  const int np = (span.pos >> b.pshift) + 1;  // pages of the context
+  const int np = ((span.pos + span.n - 1) >> b.pshift) + 1;  // pages of the last token's context
   const int* trow = b.table + (size_t)span.seq * b.table_stride;
+  const auto id_of = [&](int page) {
+    const int id = trow[min(page, np - 1)];
+    return page < np && (unsigned)id < (unsigned)b.pages ? id : -1;
+  };
+  int id = id_of(tid);
 
-  // the queries, rows 16 t + col of the product: largest's factors, then smallest's
+  // the queries: largest's factors, then smallest's
   intx4 z[NT][NM];
   float up[NT][4], off[NT][4];  // what the lane's rows of the result are scaled by; rows of no head: -inf
 #pragma unroll
   for (int t = 0; t < NT; t++) {
-    const int head = min(16 * t + col, a.G - 1);
-    const half_t* p = a.q + (int64_t)span.row * a.q_row + (h * a.G + head) * a.q_head;
+    const int tok = min((col & 3) / HJ, span.n - 1), head = 16 * t + (col >> 2) + 4 * ((col & 3) % HJ);
+    const half_t* p = a.q + (int64_t)(span.row + tok) * a.q_row + (h * a.G + min(head, a.G - 1)) * a.q_head;
     // the lane's 16 dimensions of each 64; its row's other 48 lie with lanes col + 16 i
     float x[DH / 64][16];
     float amax = 0.f;
@@ -178,8 +266,12 @@ __global__ __launch_bounds__(64 * NW) void select_kernel(SelectArgs a) {
           amax = fmaxf(amax, fabsf(w));
         }
       }
-    amax = fmaxf(amax, __shfl_xor(amax, 16, 64));
-    amax = fmaxf(amax, __shfl_xor(amax, 32, 64));
+    float other = amax;
+    swap16(amax, other);
+    amax = fmaxf(amax, other);
+    other = amax;
+    swap32(amax, other);
+    amax = fmaxf(amax, other);
     const int e = unit_of(amax);
     const float inv = kv8_scale(-e);
 #pragma unroll
@@ -198,129 +290,303 @@ __global__ __launch_bounds__(64 * NW) void select_kernel(SelectArgs a) {
       }
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-      const int row = 4 * g + j;
-      const int er = __shfl(e, row, 64);
-      up[t][j] = 16 * t + row < a.G ? kv8_scale(er) : 0.f;
-      off[t][j] = 16 * t + row < a.G ? 0.f : -INFINITY;
+      const int er = __shfl(e, 4 * g + j, 64);
+      const bool is = 16 * t + g + 4 * (j % HJ) < a.G;
+      up[t][j] = is ? kv8_scale(er) : 0.f;
+      off[t][j] = is ? 0.f : -INFINITY;
     }
   }
 
-  // keys of pages p0 .. p1 - 1 to LDS, 16 a wave at a time
-  const auto fill = [&](int p0, int p1) {
-    for (int c = p0 + wave * 16; c < p1; c += NW * 16) {
-      const int page = c + col;
-      const int id = page < np ? trow[page] : -1;
-      const bool there = (unsigned)id < (unsigned)b.pages;
-      const size_t ph = (size_t)(there ? id : 0) * b.NKV + h;
-      const int8_t* box = a.box + ph * (2 * DH) + 16 * g;
-      const int unit = a.unit[ph];
-      intx4 w[NM];
+  // the boxes of 64 neighbours (id: of the lane's page, or -1), and what the
+  // lane's page's scores are scaled by (-1: it is not there)
+  struct Boxes {
+    intx4 w[4][NM];
+    float scale;
+  };
+  const auto load = [&](int id) {
+    Boxes x;
+    const int unit = a.unit[(size_t)max(id, 0) * b.NKV + h];
 #pragma unroll
-      for (int m = 0; m < NM; m++) w[m] = *reinterpret_cast<const intx4*>(box + 64 * m);
-      float best = -INFINITY;
+    for (int c = 0; c < 4; c++) {
+      const int i = __shfl(id, 16 * c + col, 64);
+      const int8_t* box = a.box + ((size_t)max(i, 0) * b.NKV + h) * (2 * DH) + 16 * g;
+#pragma unroll
+      for (int m = 0; m < NM; m++) x.w[c][m] = *reinterpret_cast<const intx4*>(box + 64 * m);
+    }
+    x.scale = id < 0 ? -1.f : kv8_scale(clampi(unit, kUnitMin, kUnitMax));
+    return x;
+  };
+  // Scores before that scale: of the values i = c TOK + token, for 16 pages c
+  // and a token, row g of the lanes ends with those of i = 4 k + g in v[k].
+  struct Raw {
+    float v[TOK];
+  };
+  const auto raw_of = [&](const Boxes& x) {
+    float best[4 * TOK];
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
+#pragma unroll
+      for (int i = 0; i < TOK; i++) best[c * TOK + i] = -INFINITY;
 #pragma unroll
       for (int t = 0; t < NT; t++) {
         intx4 s = {0, 0, 0, 0};
 #pragma unroll
-        for (int m = 0; m < NM; m++) s = __builtin_amdgcn_mfma_i32_16x16x64_i8(z[t][m], w[m], s, 0, 0, 0);
+        for (int m = 0; m < NM; m++) s = __builtin_amdgcn_mfma_i32_16x16x64_i8(z[t][m], x.w[c][m], s, 0, 0, 0);
 #pragma unroll
-        for (int j = 0; j < 4; j++) best = fmaxf(best, __builtin_fmaf((float)s[j], up[t][j], off[t][j]));
-      }
-      best = fmaxf(best, __shfl_xor(best, 16, 64));
-      best = fmaxf(best, __shfl_xor(best, 32, 64));
-      if (g == 0 && page < p1) {
-        uint32_t key = key_of(best * kv8_scale(max(unit, kUnitMin)));
-        if (page < a.first || page >= np - a.recent) key = kAlways;
-        keys[page - p0] = there ? key : kNever;
+        for (int j = 0; j < 4; j++) {
+          float& y = best[c * TOK + j / HJ];
+          y = fmaxf(y, __builtin_fmaf((float)s[j], up[t][j], off[t][j]));
+        }
       }
     }
-  };
-  const bool once = np <= kKeys;
-  // f(page, key, whether it is one) over the pages, in order, all threads at a time
-  const auto each = [&](bool filled, auto f) {
-    for (int p0 = 0; p0 < np; p0 += kKeys) {
-      const int p1 = min(np, p0 + kKeys);
-      if (!once || !filled) {
-        __syncthreads();
-        fill(p0, p1);
-        __syncthreads();
-      }
-      for (int c = p0; c < p1; c += 64 * NW) f(c + tid, c + tid < p1 ? keys[c + tid - p0] : kNever, c + tid < p1);
-    }
-  };
-  // the sum of x over the waves (x the same in a wave's lanes)
-  int turn = 0;
-  const auto total = [&](int x) {
-    if (NW == 1) return x;
-    if (lane == 0) sums[turn][wave] = x;
-    __syncthreads();
-    int s = 0;
+    Raw r;
 #pragma unroll
-    for (int w = 0; w < NW; w++) s += sums[turn][w];
-    turn ^= 1;
-    return s;
+    for (int k = 0; k < TOK; k++) {
+      float* y = best + 4 * k;
+      swap32(y[0], y[2]);
+      swap32(y[1], y[3]);
+      y[0] = fmaxf(y[0], y[2]);
+      y[1] = fmaxf(y[1], y[3]);
+      swap16(y[0], y[1]);
+      r.v[k] = fmaxf(y[0], y[1]);
+    }
+    return r;
   };
-  const auto count_from = [&](bool filled, uint32_t bar) {
-    int n = 0;
-    each(filled, [&](int, uint32_t key, bool is) { n += __popcll(__ballot(is && key >= bar)); });
-    return total(n);
+  const auto pages_of = [&](int tok) { return ((span.pos + tok) >> b.pshift) + 1; };
+  // a token's score of a page: inf where it is always taken, -inf where it never is
+  const auto score = [&](float raw, float scale, int page, int n) {
+    const float x = page < a.first || page >= n - a.recent ? INFINITY : raw * scale;
+    return scale < 0.f || page >= n ? -INFINITY : x;
   };
 
-  // The lowest key of the choice, from the top bit down: the largest bar that
-  // `count` pages reach.  Where exactly that many do, it is found.
-  uint32_t bar = 1;
-  int reach = count_from(false, bar);
-  if (reach > a.count) {
-    bar = 0;
-    for (uint32_t bit = 0x80000000u; bit; bit >>= 1) {
-      const int n = count_from(true, bar | bit);
-      if (n >= a.count) {
-        bar |= bit;
-        reach = n;
-        if (n == a.count) break;
+  const int stride = (np + 63) & ~63;
+  const bool near = span.n * stride <= a.room;
+  if (near) {
+    // a wave's boxes are on their way while it works on those before
+    int p = wave * 64;
+    Boxes now;
+    if (p < np) now = load(id);
+    for (; p < np; p += 64 * NW) {
+      Boxes then = now;
+      if (p + 64 * NW < np) then = load(id_of(p + 64 * NW + lane));
+      const Raw r = raw_of(now);
+#pragma unroll
+      for (int k = 0; k < TOK; k++) {
+        const int i = 4 * k + g, at = i / TOK * 16 + col, tok = i % TOK;
+        const float scale = __shfl(now.scale, at, 64);
+        if (tok < span.n) scores[tok * stride + p + at] = score(r.v[k], scale, p + at, pages_of(tok));
       }
+      now = then;
     }
+    if (NW > 1) __syncthreads();
   }
-  // pages above the bar, and as many at the bar, from the lowest, as are left
-  int at_bar = 0x7fffffff;  // how many of those with the bar's own key
-  if (reach > a.count) at_bar = a.count - (bar == kAlways ? 0 : count_from(true, bar + 1));
-  int* out = a.blocks + ((size_t)span.row * b.NKV + h) * a.count;
-  int taken = 0, equal = 0;  // before this stretch of pages
-  each(true, [&](int page, uint32_t key, bool is) {
-    const uint64_t eq = __ballot(is && key == bar);
-    const uint64_t below = (1ull << lane) - 1;
-    int eq_before = equal, n = __popcll(eq);
-    if (NW > 1) {
-      if (lane == 0) sums[turn][wave] = n;
+
+  // of the waves of a token
+  const auto meet = [] {
+    if constexpr (CW > 1) {
       __syncthreads();
-      n = 0;
-#pragma unroll
-      for (int w = 0; w < NW; w++) {
-        eq_before += w < wave ? sums[turn][w] : 0;
-        n += sums[turn][w];
-      }
+    } else {  // LDS accesses of a wave stay in order; this keeps the compiler to it
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    }
+  };
+  // over them, of values that are the same in a wave's lanes; and the sum over
+  // those before
+  int turn = 0;
+  const auto over = [&](auto x, auto op) {
+    if constexpr (CW > 1) {
+      using T = decltype(x);
+      if (lane == 0) sums[turn][wave] = __builtin_bit_cast(int, x);
+      __syncthreads();
+      x = lanes<CW>(__builtin_bit_cast(T, sums[turn][lane % CW]), op);
       turn ^= 1;
     }
-    equal += n;
-    const bool take = is && (key > bar || (key == bar && eq_before + __popcll(eq & below) < at_bar));
-    const uint64_t tk = __ballot(take);
-    int before = taken;
-    n = __popcll(tk);
-    if (NW > 1) {
-      if (lane == 0) sums[turn][wave] = n;
+    return x;
+  };
+  const auto ranked = [&](int x, int& before) {
+    before = 0;
+    if constexpr (CW > 1) {
+      if (lane == 0) sums[turn][wave] = x;
       __syncthreads();
-      n = 0;
-#pragma unroll
-      for (int w = 0; w < NW; w++) {
-        before += w < wave ? sums[turn][w] : 0;
-        n += sums[turn][w];
-      }
+      const int y = sums[turn][lane % CW];
       turn ^= 1;
+      x = 0;
+#pragma unroll
+      for (int w = 0; w < CW; w++) {
+        const int k = __builtin_amdgcn_readlane(y, w);
+        before += w < wave ? k : 0;
+        x += k;
+      }
     }
-    taken += n;
-    if (take) out[before + __popcll(tk & below)] = page;
-  });
-  for (int c = taken + tid; c < a.count; c += 64 * NW) out[c] = -1;
+    return x;
+  };
+  const auto widest = [&](float x) { return over(lanes<64>(x, Max()), Max()); };
+  int* bins = bins_of[wave / CW];
+  float* few = few_of[wave / CW];
+  const int ct = tid % CT, cw = wave % CW;
+  const uint64_t below = (1ull << lane) - 1;
+  for (int tok = wave / CW; tok < span.n; tok += CH) {
+    const int n = pages_of(tok);
+    if (tok >= CH) {
+      meet();
+      for (int i = ct; i < kBins; i += CT) bins[i] = 0;
+    }
+    if (CW > 1 && tid == 0) fews = 0;  // behind barriers before it counts
+    const bool held = near && n <= kHeld;
+    float mine[R];
+    if (held) {
+#pragma unroll
+      for (int r = 0; r < R; r++) {
+        mine[r] = -INFINITY;
+        if (r * CT + cw * 64 < n) mine[r] = scores[tok * stride + r * CT + ct];
+      }
+    }
+    // f(page, score) over the pages, in order, a thread a page (-inf behind the last)
+    const auto each = [&](auto f) {
+      if (held) {
+#pragma unroll
+        for (int r = 0; r < R; r++)
+          if (r * CT < n) f(r * CT + ct, mine[r]);
+      } else if (near) {
+        for (int p = 0; p < n; p += CT)
+          f(p + ct, p + cw * 64 < n ? scores[tok * stride + p + ct] : -INFINITY);
+      } else {
+        for (int p = 0; p < n; p += CT) {
+          const Boxes x = load(id_of(p + ct));
+          const Raw r = raw_of(x);
+          const int i = g * TOK + tok;
+          float y = 0.f;
+#pragma unroll
+          for (int k = 0; k < TOK; k++) {
+            const float v = __shfl(r.v[k], (i & 3) * 16 + col, 64);
+            y = k == i >> 2 ? v : y;
+          }
+          f(p + ct, score(y, x.scale, p + ct, n));
+        }
+      }
+    };
+
+    int all = 0, always = 0;
+    float hi = -INFINITY, lo = -INFINITY;  // of the scores in question; the lowest one negated until it is known
+    each([&](int, float x) {
+      all += __popcll(__ballot(x > -INFINITY));
+      always += __popcll(__ballot(x == INFINITY));
+      if (fabsf(x) < INFINITY) {
+        hi = fmaxf(hi, x);
+        lo = fmaxf(lo, -x);
+      }
+    });
+    all = over(all, Sum());
+    // what is taken: scores above the bar, and of those at the bar the first
+    // `ties`, or all of them (-1)
+    float bar = -INFINITY;
+    int ties = 0;
+    if (all > a.count) {
+      always = over(always, Sum());
+      int need = a.count - always, in = all - always;  // pages to be taken, of those in question
+      bar = INFINITY;
+      if (need > 0) {
+        int bin = -1;
+        float step = 0.f;
+        const auto bin_of = [&](float x) {
+          return x >= lo && x <= hi ? min((int)((x - lo) * step), kBins - 1) : -1;
+        };
+        if (in > 64) {
+          hi = widest(hi);
+          lo = -widest(lo);
+          while (lo < hi) {
+            step = (float)kBins / (hi - lo);
+            each([&](int, float x) {
+              const int k = bin_of(x);
+              if (k >= 0) atomicAdd(&bins[k], 1);
+            });
+            meet();
+            // pages in the bins above the lane's four, and in them
+            int c[4], sum = 0;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+              c[i] = bins[kBins - 1 - (lane * 4 + i)];
+              sum += c[i];
+            }
+            int above = sum_up_to(sum) - sum, it = -1, left = 0, size = 0;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+              if (above < need && need <= above + c[i]) {
+                it = kBins - 1 - (lane * 4 + i);
+                left = need - above;
+                size = c[i];
+              }
+              above += c[i];
+            }
+            const int who = __ffsll((unsigned long long)__ballot(it >= 0)) - 1;
+            bin = __builtin_amdgcn_readlane(it, who);
+            need = __builtin_amdgcn_readlane(left, who);
+            in = __builtin_amdgcn_readlane(size, who);
+            if (in <= 64) break;
+            float x1 = -INFINITY, x0 = -INFINITY;
+            each([&](int, float x) {
+              if (bin_of(x) == bin) {
+                x1 = fmaxf(x1, x);
+                x0 = fmaxf(x0, -x);
+              }
+            });
+            hi = widest(x1);  // behind its barrier no wave reads the bins
+            lo = -widest(x0);
+            bin = -1;
+            for (int i = ct; i < kBins; i += CT) bins[i] = 0;
+            meet();
+          }
+        }
+        if (in <= 64) {
+          // the ones that are left, in any order
+          int at = 0;
+          each([&](int, float x) {
+            const bool is = bin < 0 ? fabsf(x) < INFINITY : bin_of(x) == bin;
+            const uint64_t who = __ballot(is);
+            if (CW > 1 && who) {
+              if (lane == 0) at = atomicAdd(&fews, __popcll(who));
+              at = __builtin_amdgcn_readfirstlane(at);
+            }
+            if (is) few[at + __popcll(who & below)] = x;
+            at += __popcll(who);
+          });
+          meet();
+          const float x = few[min(lane, in - 1)];
+          int above = 0, from = 0;
+          for (int k = 0; k < in; k++) {
+            const float y = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), k));
+            above += y > x;
+            from += y >= x;
+          }
+          const int who = __ffsll((unsigned long long)__ballot(lane < in && above < need && need <= from)) - 1;
+          bar = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), who));
+          above = __builtin_amdgcn_readlane(above, who);
+          from = __builtin_amdgcn_readlane(from, who);
+          ties = need == from ? -1 : need - above;
+        } else {  // all equal
+          bar = lo;
+          ties = need;
+        }
+      }
+    }
+    int* out = a.blocks + ((size_t)(span.row + tok) * b.NKV + h) * a.count;
+    int taken = 0, equal = 0;  // before these 64 pages
+    each([&](int page, float x) {
+      bool take = x > bar || x == INFINITY || (ties < 0 && x == bar);
+      int before;
+      if (ties > 0) {
+        const uint64_t eq = __ballot(x == bar);
+        const int all_eq = ranked(__popcll(eq), before);
+        take = take || (x == bar && equal + before + __popcll(eq & below) < ties);
+        equal += all_eq;
+      }
+      const uint64_t tk = __ballot(take);
+      const int all_tk = ranked(__popcll(tk), before);
+      if (take) out[taken + before + __popcll(tk & below)] = page;
+      taken += all_tk;
+    });
+    for (int c = taken + ct; c < a.count; c += CT) out[c] = -1;
+  }
 }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
@@ -341,11 +607,35 @@ int check_sizes(const char* op, const Kv8Batch& b, int heads, int count) {
   return ANE_OK;
 }
 
+template <int DH, int NT, int TOK, int NW, int CW>
+int launch_form(const char* op, SelectArgs a, int pages, hipStream_t st) {
+  auto* const kernel = select_kernel<DH, NT, TOK, NW, CW>;
+  a.room = std::min(TOK * ((pages + 63) & ~63), kFar);
+  const int lds = a.room * 4;
+  if (lds > 32768) {
+    const hipError_t e = taken(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+    if (e != hipSuccess) return op_fail(ANE_ERR_HIP, "storiesane %s: %s", op, hipGetErrorString(e));
+  }
+  const dim3 grid(kv8_count(a.b.nseq, a.b.rows, kv8_tiles(TOK)) * a.b.NKV);
+  hipLaunchKernelGGL(kernel, grid, dim3(64 * NW), lds, st, a);
+  return ANE_OK;
+}
+
+template <int DH, int NT, int TOK>
+int launch_tokens(const char* op, const SelectArgs& a, int pages, int most, hipStream_t st) {
+  if (TOK > 1 && most > 1) return launch_form<DH, NT, TOK, 4, 1>(op, a, pages, st);
+  return launch_form<DH, NT, TOK, 8, 8>(op, a, pages, st);
+}
+
 template <int DH>
-void launch(const SelectArgs& a, hipStream_t st) {
-  const dim3 grid(kv8_count(a.b.nseq, a.b.rows, kv8_tiles(1)) * a.b.NKV);
-  if (a.G <= 16) hipLaunchKernelGGL((select_kernel<DH, 1, 4>), grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((select_kernel<DH, 2, 4>), grid, dim3(256), 0, st, a);
+int launch(const char* op, const SelectArgs& a, const ane_kv8_batch& batch, hipStream_t st) {
+  const int cap = a.b.table_pages << a.b.pshift;
+  const int pages = (((batch.max_len ? std::min(batch.max_len, cap) : cap) - 1) >> a.b.pshift) + 1;
+  const int most = batch.max_new ? batch.max_new : (a.b.rows + a.b.nseq - 1) / a.b.nseq;
+  if (a.G <= 4) return launch_tokens<DH, 1, 4>(op, a, pages, most, st);
+  if (a.G <= 8) return launch_tokens<DH, 1, 2>(op, a, pages, most, st);
+  if (a.G <= 16) return launch_tokens<DH, 1, 1>(op, a, pages, most, st);
+  return launch_tokens<DH, 2, 1>(op, a, pages, most, st);
 }
 
 }  // namespace
@@ -412,8 +702,9 @@ extern "C" int ane_kv8_select(const ane_kv8_cache* cache, const ane_kv8_bounds* 
   a.q = (const half_t*)g.q; a.box = bounds->box; a.unit = bounds->unit; a.blocks = g.blocks;
   a.q_row = g.q_row; a.q_head = g.q_head;
   a.G = g.heads / a.b.NKV; a.count = g.count; a.first = g.first; a.recent = g.recent;
-  if (cache->head_dim == 64) launch<64>(a, (hipStream_t)stream);
-  else launch<128>(a, (hipStream_t)stream);
+  rc = cache->head_dim == 64 ? launch<64>(op, a, *batch, (hipStream_t)stream)
+                             : launch<128>(op, a, *batch, (hipStream_t)stream);
+  if (rc) return rc;
   const hipError_t h = hipGetLastError();
   if (h != hipSuccess) return op_fail(ANE_ERR_HIP, "storiesane %s: %s", op, hipGetErrorString(h));
   return ANE_OK;
