@@ -18,6 +18,7 @@
 
 #include "kv8.h"
 #include "op_error.h"
+#include "wave_ops.h"
 
 namespace ane {
 
@@ -114,43 +115,6 @@ __device__ __forceinline__ void load_row(const T* row, int c, int vocab, float (
   for (int j = 0; j < N; j++) x[j] = x[j] == x[j] ? x[j] : -INFINITY;
 }
 
-// the value of the lane N further on in the row of 16
-template <int N>
-__device__ __forceinline__ int row_ror(int v) {
-  return __builtin_amdgcn_update_dpp(0, v, 0x120 + N, 0xf, 0xf, false);
-}
-template <int N>
-__device__ __forceinline__ double row_ror(double v) {
-  return __hiloint2double(row_ror<N>(__double2hiint(v)), row_ror<N>(__double2loint(v)));
-}
-template <int N>
-__device__ __forceinline__ float row_ror(float v) {
-  return __int_as_float(row_ror<N>(__float_as_int(v)));
-}
-// in every lane: the largest, and the sum (the same order of additions in all)
-__device__ __forceinline__ float wave_top(float v) {
-  v = fmaxf(v, row_ror<1>(v));
-  v = fmaxf(v, row_ror<2>(v));
-  v = fmaxf(v, row_ror<4>(v));
-  v = fmaxf(v, row_ror<8>(v));
-  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
-}
-__device__ __forceinline__ double wave_total(double v) {
-  v += row_ror<1>(v);
-  v += row_ror<2>(v);
-  v += row_ror<4>(v);
-  v += row_ror<8>(v);
-  double s = 0.0;
-#pragma unroll
-  for (int r = 0; r < 4; r++)
-    s += __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(v), 16 * r),
-                          __builtin_amdgcn_readlane(__double2loint(v), 16 * r));
-  return s;
-}
-
 // A wave takes U loads of 64 N entries of a row.
 template <typename T, int U>
 __global__ __launch_bounds__(256) void part_kernel(BeamArgs a) {
@@ -169,14 +133,8 @@ __global__ __launch_bounds__(256) void part_kernel(BeamArgs a) {
     top[u] = x[u][0];
 #pragma unroll
     for (int j = 1; j < N; j++) top[u] = fmaxf(top[u], x[u][j]);
-    top[u] = fmaxf(top[u], row_ror<1>(top[u]));
-    top[u] = fmaxf(top[u], row_ror<2>(top[u]));
-    top[u] = fmaxf(top[u], row_ror<4>(top[u]));
-    top[u] = fmaxf(top[u], row_ror<8>(top[u]));
-    const auto x16 = __builtin_amdgcn_permlane16_swap(__float_as_uint(top[u]), __float_as_uint(top[u]), false, false);
-    top[u] = fmaxf(__uint_as_float(x16[0]), __uint_as_float(x16[1]));
-    const auto x32 = __builtin_amdgcn_permlane32_swap(__float_as_uint(top[u]), __float_as_uint(top[u]), false, false);
-    const float both = fmaxf(__uint_as_float(x32[0]), __uint_as_float(x32[1]));
+    top[u] = over_lanes<32>(top[u], Max());
+    const float both = fmaxf(top[u], xor32_f(top[u]));
     if (SPW == 1) top[u] = both;
     m = fmaxf(m, both);
   }
@@ -187,7 +145,7 @@ __global__ __launch_bounds__(256) void part_kernel(BeamArgs a) {
 #pragma unroll
       for (int j = 0; j < N; j++) s += __builtin_amdgcn_exp2f((x[u][j] - m) * 1.44269504088896340736f);
   }
-  const double sum = wave_total((double)s);
+  const double sum = sum_over_lanes((double)s);
   float* seg = a.seg_max + (size_t)r * a.segs;
 #pragma unroll
   for (int u = 0; u < U; u++) {
@@ -371,7 +329,7 @@ __global__ __launch_bounds__(TH) void choose_kernel(BeamArgs a) {
     float m = q[i][0].max;
 #pragma unroll
     for (int k = 1; k < PL; k++) m = fmaxf(m, q[i][k].max);
-    m = wave_top(m);
+    m = over_lanes<64>(m, Max());
     // Factors of the parts in fp32: off by what a part's own exponentials are.
     // An infinite maximum makes NaN, as it should.
     double s = 0.0;
@@ -380,7 +338,7 @@ __global__ __launch_bounds__(TH) void choose_kernel(BeamArgs a) {
       const float f = __builtin_amdgcn_exp2f((q[i][k].max - m) * 1.44269504088896340736f);
       s += q[i][k].max > -INFINITY ? q[i][k].sum * f : 0.0;
     }
-    s = wave_total(s);
+    s = sum_over_lanes(s);
     sum = lane == i ? s : sum;
     top = lane == i ? (double)m : top;
   }

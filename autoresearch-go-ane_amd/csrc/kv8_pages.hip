@@ -10,6 +10,7 @@
 
 #include "kv8.h"
 #include "op_error.h"
+#include "wave_ops.h"
 
 namespace ane {
 
@@ -34,43 +35,94 @@ __device__ __forceinline__ int load_ref(const int* p) {
   return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-// One side (K or V) of page `from` of a layer to page `to`, its first `units`
-// units of 16 tokens, by a block of TH threads.  A unit of a head is 16 *
-// head_dim bytes in a row, on both sides.
+// A barrier behind which the block's atomics and stores to global memory so far
+// have arrived.
+__device__ __forceinline__ void settle() {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+}
+
+// Of page `from` to page `to`, `sides` sides from side0 on (side 2 l is layer
+// l's keys, 2 l + 1 its values), their first `units` units of 16 tokens, by a
+// block of TH threads.  A unit of a head is 16 * head_dim bytes in a row on both
+// sides.  Four loads a thread are under way at once: of one side, or of four
+// where sides are small and come several to a block.
 template <int TH>
-__device__ __forceinline__ void copy_side(const Pool& p, const Layers& x, const Layers& y, int layer, bool values,
-                                          int from, int to, int units) {
+__device__ __forceinline__ void copy_sides(const Pool& p, const Layers& x, const Layers& y, int side0, int sides,
+                                           int from, int to, int units) {
   const int tid = threadIdx.x;
   const uint32_t whole = 1u << (p.pshift - 4 + p.dshift), used = (uint32_t)units << p.dshift;  // 16-byte words of a head
-  const size_t at = (size_t)p.NKV * whole;
-  const u32x4* s = reinterpret_cast<const u32x4*>(values ? x.v[layer] : x.k[layer]) + from * at;
-  u32x4* d = reinterpret_cast<u32x4*>(values ? y.v[layer] : y.k[layer]) + to * at;
   const uint32_t n = p.NKV * used;
+  const size_t at = (size_t)p.NKV * whole;
+  const auto place = [&](uint32_t t) {
+    const uint32_t h = used == whole ? 0 : t / used;
+    return h * whole + (t - h * used);
+  };
   constexpr int U = 4;
-  for (uint32_t t0 = tid; t0 < n; t0 += TH * U) {
-    u32x4 w[U];
-    uint32_t o[U];
+  if (sides == 1) {
+    const int l = side0 >> 1;
+    const u32x4* s = reinterpret_cast<const u32x4*>(side0 & 1 ? x.v[l] : x.k[l]) + from * at;
+    u32x4* d = reinterpret_cast<u32x4*>(side0 & 1 ? y.v[l] : y.k[l]) + to * at;
+    for (uint32_t t0 = tid; t0 < n; t0 += TH * U) {
+      u32x4 w[U];
+      uint32_t o[U];
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-      const uint32_t t = min(t0 + u * TH, n - 1), h = used == whole ? 0 : t / used;
-      o[u] = h * whole + (t - h * used);
-      w[u] = s[o[u]];
+      for (int u = 0; u < U; u++) {
+        o[u] = place(min(t0 + u * TH, n - 1));
+        w[u] = s[o[u]];
+      }
+#pragma unroll
+      for (int u = 0; u < U; u++)
+        if (t0 + u * TH < n) d[o[u]] = w[u];
     }
+  } else {
+    for (int i = 0; i < sides; i += U) {
+      const u32x4* s[U];
+      u32x4* d[U];
 #pragma unroll
-    for (int u = 0; u < U; u++)
-      if (t0 + u * TH < n) d[o[u]] = w[u];
+      for (int u = 0; u < U; u++) {
+        const int c = side0 + min(i + u, sides - 1), l = c >> 1;
+        s[u] = reinterpret_cast<const u32x4*>(c & 1 ? x.v[l] : x.k[l]) + from * at;
+        d[u] = reinterpret_cast<u32x4*>(c & 1 ? y.v[l] : y.k[l]) + to * at;
+      }
+      for (uint32_t t = tid; t < n; t += TH) {
+        const uint32_t o = place(t);
+        u32x4 w[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) w[u] = s[u][o];
+#pragma unroll
+        for (int u = 0; u < U; u++)
+          if (i + u < sides) d[u][o] = w[u];
+      }
+    }
   }
   const size_t ef = (size_t)from * p.NKV, et = (size_t)to * p.NKV;
-  const int8_t* se = values ? x.ve[layer] : x.ke[layer];
-  int8_t* de = values ? y.ve[layer] : y.ke[layer];
-  for (int h = tid; h < p.NKV; h += TH) de[et + h] = se[ef + h];
-  if (!values && x.box[layer] && y.box[layer]) {
-    const int m = p.NKV << (p.dshift - 3);  // 16-byte words of a page's boxes
-    const u32x4* sb = reinterpret_cast<const u32x4*>(x.box[layer]) + (size_t)from * m;
-    u32x4* db = reinterpret_cast<u32x4*>(y.box[layer]) + (size_t)to * m;
-    for (int t = tid; t < m; t += TH) db[t] = sb[t];
-    for (int h = tid; h < p.NKV; h += TH) y.unit[layer][et + h] = x.unit[layer][ef + h];
+  for (int c = side0; c < side0 + sides; c++) {
+    const int l = c >> 1;
+    const int8_t* se = c & 1 ? x.ve[l] : x.ke[l];
+    int8_t* de = c & 1 ? y.ve[l] : y.ke[l];
+    for (int h = tid; h < p.NKV; h += TH) de[et + h] = se[ef + h];
+    if (!(c & 1) && x.box[l] && y.box[l]) {
+      const int m = p.NKV << (p.dshift - 3);  // 16-byte words of a page's boxes
+      const u32x4* sb = reinterpret_cast<const u32x4*>(x.box[l]) + (size_t)from * m;
+      u32x4* db = reinterpret_cast<u32x4*>(y.box[l]) + (size_t)to * m;
+      for (int t = tid; t < m; t += TH) db[t] = sb[t];
+      for (int h = tid; h < p.NKV; h += TH) y.unit[l][et + h] = x.unit[l][ef + h];
+    }
   }
+}
+// The sides of an item (a page's copy in all layers of a launch) that a block
+// takes, `group` at a time.
+struct Sides {
+  int item, first, count;
+};
+__device__ __forceinline__ Sides sides_of(uint32_t block, int nlayers, int group) {
+  const int per = (2 * nlayers + group - 1) / group;
+  Sides s;
+  s.item = block / per;
+  s.first = (block - s.item * per) * group;
+  s.count = min(group, 2 * nlayers - s.first);
+  return s;
 }
 
 __device__ __forceinline__ int units_of(const Pool& p, int tokens) {
@@ -97,13 +149,43 @@ struct ForkArgs {
   int* found;  // how many of them there are, of those that are wanted
 };
 
+// One block does the tables by itself where they are small: their entries are
+// in LDS.
+constexpr int kSmall = 8192;
+bool small_table(int64_t nseq, int64_t width) { return nseq <= kTh && nseq * width <= kSmall; }
+
 __device__ __forceinline__ int there(int id, int pages) { return (unsigned)id < (unsigned)pages ? id : -1; }
 __device__ __forceinline__ int held_of(const ForkArgs& a, int i) {
   const int from = a.parents ? a.parents[i] : i;
   return (unsigned)from < (unsigned)a.nseq ? clampi(a.start[from], 0, a.width << a.p.pshift) : 0;
 }
+__device__ __forceinline__ int end_of(const ForkArgs& a, int i, int st) {
+  return st + clampi(a.news ? a.news[i] : a.new_tokens, 0, (a.width << a.p.pshift) - st);
+}
 __device__ __forceinline__ int pages_for(const ForkArgs& a, int tokens) {
   return (tokens + (1 << a.p.pshift) - 1) >> a.p.pshift;
+}
+// whether tokens that come go to a page that holds some already
+__device__ __forceinline__ bool goes_on(const ForkArgs& a, int st, int end) {
+  return end > st && (st & ((1 << a.p.pshift) - 1));
+}
+__device__ __forceinline__ void recount(const ForkArgs& a, int old, int mid) {
+  if (old == mid) return;
+  if (old >= 0) atomicSub(a.refs + old, 1);
+  if (mid >= 0) atomicAdd(a.refs + mid, 1);
+}
+// What entry j of a sequence's row becomes: a new page by its rank, which then
+// has one holder, or what the parent has there.
+__device__ __forceinline__ int entry_of(const ForkArgs& a, const Next& n, int j, int mid, int found, bool& fresh) {
+  const int copies = n.src >= 0, held = pages_for(a, n.st);
+  int rank = -1;
+  if (copies && j == n.st >> a.p.pshift) rank = n.base;
+  else if (j >= held && j < pages_for(a, n.end)) rank = n.base + copies + (j - held);
+  fresh = rank >= 0;
+  if (!fresh) return mid;
+  const int id = rank < found ? a.free[rank] : -1;
+  if (id >= 0) a.refs[id] = 1;
+  return id;
 }
 
 // The parents' rows, cut to what they hold; reference counts follow.  A thread
@@ -117,10 +199,7 @@ __global__ __launch_bounds__(256) void rows_kernel(ForkArgs a) {
   int* mine = a.table + (size_t)i * a.stride + j;
   const int raw = *mine, old = there(raw, a.p.pages);
   const int mid = !holds ? -1 : from == i ? old : there(a.table[(size_t)from * a.stride + j], a.p.pages);
-  if (old != mid) {
-    if (old >= 0) atomicSub(a.refs + old, 1);
-    if (mid >= 0) atomicAdd(a.refs + mid, 1);
-  }
+  recount(a, old, mid);
   if (a.parents) a.mid[(size_t)i * a.width + j] = mid;
   else if (raw != mid) *mine = mid;
 }
@@ -128,95 +207,88 @@ __global__ __launch_bounds__(256) void rows_kernel(ForkArgs a) {
 // the sum over the threads before this one, and over all
 __device__ __forceinline__ int block_scan(int x, int (&sums)[kTh / 64], int& total) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  int s = x;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int y = __shfl_up(s, o, 64);
-    if (lane >= o) s += y;
-  }
+  const int s = sum_up_to(x);
   __syncthreads();
   if (lane == 63) sums[w] = s;
   __syncthreads();
-  int before = 0;
-  total = 0;
-#pragma unroll
-  for (int k = 0; k < kTh / 64; k++) {
-    const int y = sums[k];
-    before += k < w ? y : 0;
-    total += y;
-  }
-  return before + s - x;
+  const int y = sum_up_to(sums[lane % (kTh / 64)]);  // lane k: the waves up to k
+  total = __builtin_amdgcn_readlane(y, kTh / 64 - 1);
+  const int upto = __shfl(y, w, 64);
+  return upto - __builtin_amdgcn_readlane(s, 63) + s - x;
 }
 
-// One block: who copies, how many pages each sequence gets, and which are free.
-__global__ __launch_bounds__(kTh) void plan_kernel(ForkArgs a) {
-  __shared__ int sums[kTh / 64];
-  __shared__ int lost_all;
-  const int tid = threadIdx.x, P = 1 << a.p.pshift, cap = a.width << a.p.pshift;
-  if (tid == 0) lost_all = 0;
-  // the page that the sequence's first new token goes to, where it holds
-  // tokens already; -2: no such token
-  struct Seq {
-    int st, end, page;
-  };
-  const auto seq_of = [&](int i) {
-    Seq s;
-    s.st = held_of(a, i);
-    s.end = s.st + clampi(a.news ? a.news[i] : a.new_tokens, 0, cap - s.st);
-    s.page = -2;
-    if (s.end > s.st && (s.st & (P - 1))) {
-      const int j = s.st >> a.p.pshift;
-      s.page = a.parents ? a.mid[(size_t)i * a.width + j] : there(a.table[(size_t)i * a.stride + j], a.p.pages);
+// Sequences that write into a page they hold (`page`, of threads up to nseq <=
+// kTh; below 0: none): whether this one copies it first.  Counts become those
+// without the sequences that do.  The writers of a page meet in a table of
+// twice as many places as there can be pages: a page's place is the first free
+// one, or its own, from where its id's hash points on.
+constexpr int kPlaces = 2 * kTh;
+struct Writers {
+  int page[kPlaces], count[kPlaces], lowest[kPlaces];
+};
+__device__ __forceinline__ bool copies_few(const ForkArgs& a, int page, Writers& t) {
+  const int tid = threadIdx.x;
+  const int held = page >= 0 ? load_ref(a.refs + page) : 0;  // behind a barrier after the rows' counts
+  for (int k = tid; k < kPlaces; k += kTh) {
+    t.page[k] = -1;
+    t.count[k] = 0;
+    t.lowest[k] = kTh;
+  }
+  __syncthreads();
+  int at = 0;
+  if (page >= 0) {
+    at = (uint32_t)page * 2654435769u >> 21;  // 2^32 / golden ratio; 11 bits
+    for (;;) {
+      const int was = atomicCAS(&t.page[at], -1, page);
+      if (was == -1 || was == page) break;
+      at = (at + 1) % kPlaces;
     }
-    return s;
-  };
-  // A page whose count falls to 0 when its writers leave it is held by writers
-  // alone, and the lowest of them keeps it: the count then holds its number,
-  // as a negative one, until it becomes 1 again.
+    atomicAdd(&t.count[at], 1);
+    atomicMin(&t.lowest[at], tid);
+  }
+  __syncthreads();
+  if (page < 0) return false;
+  const int writers = t.count[at];
+  const bool first = t.lowest[at] == tid;
+  if (first)
+    __hip_atomic_store(a.refs + page, held <= writers ? 1 : held - writers, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  return !(first && held <= writers);
+}
+
+// The same of any number of sequences, whose pages stand in next[].base; those
+// that copy have them in next[].src then.  A page whose count falls to 0 when
+// its writers leave it is held by writers alone, and the lowest of them keeps
+// it: the count holds its number, as a negative one, until it becomes 1 again.
+__device__ __forceinline__ void copies_many(const ForkArgs& a) {
   constexpr int kMark = -(1 << 30);
+  const int tid = threadIdx.x;
+  for (int i = tid; i < a.nseq; i += kTh)
+    if (const int p = a.next[i].base; p >= 0) atomicSub(a.refs + p, 1);
+  settle();
+  for (int i = tid; i < a.nseq; i += kTh)
+    if (const int p = a.next[i].base; p >= 0 && load_ref(a.refs + p) <= 0) atomicMin(a.refs + p, kMark + i);
+  settle();
   for (int i = tid; i < a.nseq; i += kTh) {
-    const int p = seq_of(i).page;
-    if (p >= 0) atomicSub(a.refs + p, 1);
+    const int p = a.next[i].base;
+    if (p >= 0 && load_ref(a.refs + p) != kMark + i) a.next[i].src = p;
   }
-  __syncthreads();
+  settle();
   for (int i = tid; i < a.nseq; i += kTh) {
-    const int p = seq_of(i).page;
-    if (p >= 0 && load_ref(a.refs + p) <= 0) atomicMin(a.refs + p, kMark + i);
+    const Next n = a.next[i];
+    if (n.base >= 0 && n.src < 0) __hip_atomic_store(a.refs + n.base, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
-  __syncthreads();
-  for (int i = tid; i < a.nseq; i += kTh) {
-    const Seq s = seq_of(i);
-    const bool keeps = s.page >= 0 && load_ref(a.refs + s.page) == kMark + i;
-    a.next[i] = {s.st, s.end, keeps, keeps || s.page < 0 ? -1 : s.page};
-  }
-  __syncthreads();
-  int want = 0, lost = 0;
-  for (int i0 = 0; i0 < a.nseq; i0 += kTh) {
-    const int i = i0 + tid;
-    int need = 0;
-    if (i < a.nseq) {
-      const Next n = a.next[i];
-      need = (n.src >= 0) + pages_for(a, n.end) - pages_for(a, n.st);
-      if (n.end > n.st && (n.st & (P - 1)) && n.src < 0) {
-        const int p = seq_of(i).page;
-        if (n.base) __hip_atomic_store(a.refs + p, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        else lost++;
-      }
-    }
-    int all;
-    const int before = block_scan(need, sums, all);
-    if (i < a.nseq) a.next[i].base = want + before;
-    want += all;
-  }
-  if (lost) atomicAdd(&lost_all, lost);
-  __syncthreads();
+}
+
+// The lowest `want` free pages, by rank; how many of them there are.
+__device__ __forceinline__ int find_free(const ForkArgs& a, int want, int (&sums)[kTh / 64]) {
   int found = 0;
-  for (int p0 = 0; p0 < a.p.pages && found < want; p0 += kChunk) {
+  const uint32_t pages = a.p.pages;
+  for (uint32_t p0 = 0; p0 < pages && found < want; p0 += kChunk) {
     int is[4], n = 0;
 #pragma unroll
     for (int u = 0; u < 4; u++) {
-      const int p = p0 + tid * 4 + u;
-      is[u] = p < a.p.pages && load_ref(a.refs + min(p, a.p.pages - 1)) <= 0;
+      const uint32_t p = p0 + threadIdx.x * 4 + u;
+      is[u] = p < pages && load_ref(a.refs + min(p, pages - 1)) <= 0;
       n += is[u];
     }
     int all;
@@ -224,44 +296,135 @@ __global__ __launch_bounds__(kTh) void plan_kernel(ForkArgs a) {
 #pragma unroll
     for (int u = 0; u < 4; u++)
       if (is[u]) {
-        if (rank < want) a.free[rank] = p0 + tid * 4 + u;
+        if (rank < want) a.free[rank] = (int)(p0 + threadIdx.x * 4 + u);
         rank++;
       }
     found += all;
   }
+  return min(found, want);
+}
+
+// One block: who copies, how many pages each sequence gets, and which are free.
+// SMALL: also the rows before that, and the table behind it.
+template <bool SMALL>
+__global__ __launch_bounds__(kTh) void plan_kernel(ForkArgs a) {
+  __shared__ int sums[kTh / 64];
+  __shared__ Writers writers;
+  __shared__ int lost_all;
+  __shared__ int mids[SMALL ? kSmall : 1], source[SMALL ? kTh : 1], holds[SMALL ? kTh : 1];
+  __shared__ Next nexts[SMALL ? kTh : 1];
+  constexpr int E = SMALL ? kSmall / kTh : 1;  // entries a thread
+  const int tid = threadIdx.x;
+  if (tid == 0) lost_all = 0;
+  int raw[E];
+  int st = 0, end = 0;
+  if constexpr (SMALL) {
+    if (tid < a.nseq) {
+      source[tid] = a.parents ? a.parents[tid] : tid;
+      st = held_of(a, tid);
+      end = end_of(a, tid, st);
+      holds[tid] = pages_for(a, st);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < E; k++) {
+      const int e = k * kTh + tid;
+      if (e >= a.nseq * a.width) break;
+      const int i = e / a.width, j = e - i * a.width;
+      raw[k] = a.table[(size_t)i * a.stride + j];
+      mids[e] = j < holds[i] ? there(a.table[(size_t)source[i] * a.stride + j], a.p.pages) : -1;
+      recount(a, there(raw[k], a.p.pages), mids[e]);
+    }
+    settle();
+  }
+  int want = 0, lost = 0;
+  if (SMALL || a.nseq <= kTh) {
+    int page = -2;  // -1: it is not there
+    if (tid < a.nseq) {
+      if (!SMALL) {
+        st = held_of(a, tid);
+        end = end_of(a, tid, st);
+      }
+      if (goes_on(a, st, end)) {
+        const int j = st >> a.p.pshift;
+        if (SMALL) page = mids[tid * a.width + j];
+        else if (a.parents) page = a.mid[(size_t)tid * a.width + j];
+        else page = there(a.table[(size_t)tid * a.stride + j], a.p.pages);
+      }
+    }
+    lost = page == -1;
+    const bool copies = copies_few(a, page, writers);
+    const int before = block_scan(copies + pages_for(a, end) - pages_for(a, st), sums, want);
+    if (tid < a.nseq) {
+      const Next n = {st, end, before, copies ? page : -1};
+      a.next[tid] = n;
+      if (SMALL) nexts[tid] = n;
+    }
+  } else {
+    for (int i = tid; i < a.nseq; i += kTh) {
+      st = held_of(a, i);
+      end = end_of(a, i, st);
+      int page = -2;
+      if (goes_on(a, st, end)) {
+        const int j = st >> a.p.pshift;
+        page = a.parents ? a.mid[(size_t)i * a.width + j] : there(a.table[(size_t)i * a.stride + j], a.p.pages);
+        lost += page < 0;
+      }
+      a.next[i] = {st, end, page, -1};
+    }
+    copies_many(a);
+    for (int i0 = 0; i0 < a.nseq; i0 += kTh) {
+      const int i = i0 + tid;
+      Next n = {0, 0, 0, -1};
+      if (i < a.nseq) n = a.next[i];
+      int all;
+      n.base = want + block_scan((n.src >= 0) + pages_for(a, n.end) - pages_for(a, n.st), sums, all);
+      if (i < a.nseq) a.next[i] = n;
+      want += all;
+    }
+  }
+  if (lost) atomicAdd(&lost_all, lost);
+  settle();
+  const int found = find_free(a, want, sums);
   if (tid == 0) {
-    found = min(found, want);
     *a.found = found;
     *a.missing = want - found + lost_all;
   }
+  if constexpr (SMALL) {
+    settle();  // the free pages are written
+#pragma unroll
+    for (int k = 0; k < E; k++) {
+      const int e = k * kTh + tid;
+      if (e >= a.nseq * a.width) break;
+      const int i = e / a.width, j = e - i * a.width;
+      bool fresh;
+      const int id = entry_of(a, nexts[i], j, mids[e], found, fresh);
+      if (id != raw[k]) a.table[(size_t)i * a.stride + j] = id;
+    }
+    if (tid < a.nseq) a.start[tid] = st;
+  }
 }
 
-// The tables' entries and starts, a thread an entry; behind those blocks the
-// copies, a block for each sequence, layer and side.
-__global__ __launch_bounds__(256) void finish_kernel(ForkArgs a, Layers x, int nlayers, int table_blocks) {
-  const int P = 1 << a.p.pshift, found = *a.found;
+// The tables' entries and starts, a thread an entry (table_blocks of them);
+// behind those blocks the copies, blocks for each sequence.
+__global__ __launch_bounds__(256) void finish_kernel(ForkArgs a, Layers x, int nlayers, int group, int table_blocks) {
+  const int found = *a.found;
   if ((int)blockIdx.x < table_blocks) {
     const int blocks = (a.width + 255) / 256, i = blockIdx.x / blocks;
     const int j = (blockIdx.x - i * blocks) * 256 + threadIdx.x;
     if (j >= a.width) return;
     const Next n = a.next[i];
-    const int copies = n.src >= 0, held = pages_for(a, n.st);
-    int rank = -1;
-    if (copies && j == n.st >> a.p.pshift) rank = n.base;
-    else if (j >= held && j < pages_for(a, n.end)) rank = n.base + copies + (j - held);
-    int id = a.parents ? a.mid[(size_t)i * a.width + j] : -1;
-    if (rank >= 0) {
-      id = rank < found ? a.free[rank] : -1;
-      if (id >= 0) a.refs[id] = 1;
-    }
-    if (a.parents || rank >= 0) a.table[(size_t)i * a.stride + j] = id;
+    bool fresh;
+    const int id = entry_of(a, n, j, a.parents ? a.mid[(size_t)i * a.width + j] : -1, found, fresh);
+    if (a.parents || fresh) a.table[(size_t)i * a.stride + j] = id;
     if (j == 0) a.start[i] = n.st;
     return;
   }
-  const int b = blockIdx.x - table_blocks, i = b / (2 * nlayers), ls = b - i * 2 * nlayers;
-  const Next n = a.next[i];
+  const Sides s = sides_of(blockIdx.x - table_blocks, nlayers, group);
+  const Next n = a.next[s.item];
   if (n.src < 0 || n.base >= found) return;
-  copy_side<256>(a.p, x, x, ls >> 1, ls & 1, n.src, a.free[n.base], units_of(a.p, n.st & (P - 1)));
+  copy_sides<256>(a.p, x, x, s.first, s.count, n.src, a.free[n.base],
+                  units_of(a.p, n.st & ((1 << a.p.pshift) - 1)));
 }
 
 // ---- compact -------------------------------------------------------------------
@@ -290,35 +453,42 @@ __global__ __launch_bounds__(kTh) void count_kernel(CompactArgs a) {
   if (threadIdx.x == 0) a.counts[blockIdx.x] = all;
 }
 
-// Ranks: a block a chunk, which adds up the counts of all.
+// Ranks: a block a chunk, which adds up the counts of all (of one chunk, its
+// own).
 __global__ __launch_bounds__(kTh) void rank_kernel(CompactArgs a) {
   __shared__ int sums[kTh / 64];
   const int tid = threadIdx.x;
-  int n = 0, m = 0, held, before, low;
-  for (int b = tid; b < a.chunks; b += kTh) {
-    const int c = a.counts[b];
-    n += c;
-    m += b < (int)blockIdx.x ? c : 0;
-  }
-  block_scan(n, sums, held);    // U: the pages held
-  block_scan(m, sums, before);  // those before this chunk
-  // those below U: whole chunks, and the one that U lies in
-  const int cu = held / kChunk;
-  n = 0;
-  for (int b = tid; b < cu; b += kTh) n += a.counts[b];
-  for (int p = cu * kChunk + tid; p < held; p += kTh) n += a.refs[p] > 0;
-  block_scan(n, sums, low);
-  if (blockIdx.x == 0 && tid == 0) *a.total = held - low;
   const int64_t p0 = (int64_t)blockIdx.x * kChunk + tid * 4;
-  int is[4];
-  n = 0;
+  int is[4], n = 0, m = 0, held, before = 0, low;
 #pragma unroll
   for (int u = 0; u < 4; u++) {
     is[u] = p0 + u < a.p.pages && a.refs[p0 + u] > 0;
     n += is[u];
   }
-  int all;
-  int rank = before + block_scan(n, sums, all);  // pages held before the thread's
+  int rank = block_scan(n, sums, held);  // pages held before the thread's
+  if (a.chunks > 1) {
+    n = 0;
+    for (int b = tid; b < a.chunks; b += kTh) {
+      const int c = a.counts[b];
+      n += c;
+      m += b < (int)blockIdx.x ? c : 0;
+    }
+    block_scan(n, sums, held);    // U: the pages held
+    block_scan(m, sums, before);  // those before this chunk
+    rank += before;
+  }
+  // those below U: whole chunks, and the one that U lies in
+  const int cu = held / kChunk;
+  n = 0;
+  if (a.chunks > 1) {
+    for (int b = tid; b < cu; b += kTh) n += a.counts[b];
+    for (int p = cu * kChunk + tid; p < held; p += kTh) n += a.refs[p] > 0;
+  } else {
+#pragma unroll
+    for (int u = 0; u < 4; u++) n += is[u] && p0 + u < held;
+  }
+  block_scan(n, sums, low);
+  if (blockIdx.x == 0 && tid == 0) *a.total = held - low;
 #pragma unroll
   for (int u = 0; u < 4; u++) {
     if (p0 + u >= a.p.pages) break;
@@ -339,7 +509,7 @@ __global__ __launch_bounds__(kTh) void rank_kernel(CompactArgs a) {
   }
 }
 
-__global__ __launch_bounds__(256) void move_kernel(CompactArgs a, Layers x, int nlayers, int book_blocks) {
+__global__ __launch_bounds__(256) void move_kernel(CompactArgs a, Layers x, int nlayers, int group, int items, int book_blocks) {
   if ((int)blockIdx.x < book_blocks) {
     // a thread a page or an entry of the table
     const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -364,21 +534,21 @@ __global__ __launch_bounds__(256) void move_kernel(CompactArgs a, Layers x, int 
     }
     return;
   }
-  const int b = blockIdx.x - book_blocks, ls = b % (2 * nlayers);
-  const int total = *a.total, step = (gridDim.x - book_blocks) / (2 * nlayers);
-  for (int k = b / (2 * nlayers); k < total; k += step)
-    copy_side<256>(a.p, x, x, ls >> 1, ls & 1, a.movers[k], a.holes[k], 1 << (a.p.pshift - 4));
+  const Sides s = sides_of(blockIdx.x - book_blocks, nlayers, group);
+  const int total = *a.total;
+  for (int k = s.item; k < total; k += items)
+    copy_sides<256>(a.p, x, x, s.first, s.count, a.movers[k], a.holes[k], 1 << (a.p.pshift - 4));
 }
 
 // ---- copy ----------------------------------------------------------------------
 
 __global__ __launch_bounds__(256) void copy_kernel(Pool p, int into_pages, Layers x, Layers y, int nlayers,
-                                                   const int* src, const int* dst, const int* tokens) {
-  const int i = blockIdx.x / (2 * nlayers), ls = blockIdx.x - i * 2 * nlayers;
-  const int from = src[i], to = dst[i];
+                                                   int group, const int* src, const int* dst, const int* tokens) {
+  const Sides s = sides_of(blockIdx.x, nlayers, group);
+  const int from = src[s.item], to = dst[s.item];
   if ((unsigned)from >= (unsigned)p.pages || (unsigned)to >= (unsigned)into_pages) return;
-  const int units = tokens ? units_of(p, tokens[i]) : 1 << (p.pshift - 4);
-  if (units > 0) copy_side<256>(p, x, y, ls >> 1, ls & 1, from, to, units);
+  const int units = tokens ? units_of(p, tokens[s.item]) : 1 << (p.pshift - 4);
+  if (units > 0) copy_sides<256>(p, x, y, s.first, s.count, from, to, units);
 }
 
 // ---- host ----------------------------------------------------------------------
@@ -417,6 +587,16 @@ int layers_of(const ane_kv8_pool& pool, int l0, Layers* x) {
   }
   return n;
 }
+
+// Sides a block copies: one where there are few, and of small pages as many as
+// make 16 KB, which is what a block's threads load at a time.
+int group_of(const Pool& p, int64_t items, int nlayers) {
+  const int side = p.NKV << (p.pshift + p.dshift);  // bytes
+  int g = std::max(1, std::min(2 * nlayers, 16384 / side));
+  while (g > 1 && items * ((2 * nlayers + g - 1) / g) < 2048) g /= 2;
+  return g;
+}
+int blocks_of(int64_t items, int nlayers, int group) { return (int)(items * ((2 * nlayers + group - 1) / group)); }
 
 int check_table(const char* op, const int* table, int stride, int width, int nseq, int pshift) {
   if (nseq < 0 || nseq > 65536) return op_fail(ANE_ERR_ARG, "storiesane %s: nseq=%d want 0..65536", op, nseq);
@@ -521,13 +701,19 @@ extern "C" int ane_kv8_fork(const ane_kv8_pool* pool, const ane_kv8_fork_args* a
   a.free = (int*)(ws + w.free);
   const hipStream_t st = (hipStream_t)stream;
   const int table_blocks = a.nseq * ((a.width + 255) / 256);
-  if (table_blocks > 0) hipLaunchKernelGGL(rows_kernel, dim3(table_blocks), dim3(256), 0, st, a);
-  hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(kTh), 0, st, a);
+  const bool small = small_table(a.nseq, a.width);
+  if (small) {
+    hipLaunchKernelGGL(plan_kernel<true>, dim3(1), dim3(kTh), 0, st, a);
+  } else {
+    hipLaunchKernelGGL(rows_kernel, dim3(table_blocks), dim3(256), 0, st, a);
+    hipLaunchKernelGGL(plan_kernel<false>, dim3(1), dim3(kTh), 0, st, a);
+  }
   for (int l0 = 0; l0 < pool->nlayers && a.nseq > 0; l0 += kMaxLayers) {
     Layers x;
     const int n = layers_of(*pool, l0, &x);
-    const int tb = l0 == 0 ? table_blocks : 0;
-    hipLaunchKernelGGL(finish_kernel, dim3(tb + a.nseq * 2 * n), dim3(256), 0, st, a, x, n, tb);
+    const int tb = l0 == 0 && !small ? table_blocks : 0;
+    const int group = group_of(a.p, a.nseq, n);
+    hipLaunchKernelGGL(finish_kernel, dim3(tb + blocks_of(a.nseq, n, group)), dim3(256), 0, st, a, x, n, group, tb);
   }
   return launched(op);
 }
@@ -568,7 +754,7 @@ extern "C" int ane_kv8_compact(const ane_kv8_pool* pool, const ane_kv8_compact_a
   a.holes = (int*)(ws + w.holes);
   a.movers = (int*)(ws + w.movers);
   const hipStream_t st = (hipStream_t)stream;
-  hipLaunchKernelGGL(count_kernel, dim3(a.chunks), dim3(kTh), 0, st, a);
+  if (a.chunks > 1) hipLaunchKernelGGL(count_kernel, dim3(a.chunks), dim3(kTh), 0, st, a);
   hipLaunchKernelGGL(rank_kernel, dim3(a.chunks), dim3(kTh), 0, st, a);
   const int book = (int)(((int64_t)a.p.pages + (int64_t)a.nseq * a.width + 255) / 256);
   for (int l0 = 0; l0 < pool->nlayers; l0 += kMaxLayers) {
@@ -576,7 +762,8 @@ extern "C" int ane_kv8_compact(const ane_kv8_pool* pool, const ane_kv8_compact_a
     const int n = layers_of(*pool, l0, &x);
     const int bb = l0 == 0 ? book : 0;
     const int items = std::min(std::max(a.p.pages / 2, 1), 1024);
-    hipLaunchKernelGGL(move_kernel, dim3(bb + items * 2 * n), dim3(256), 0, st, a, x, n, bb);
+    const int group = group_of(a.p, items, n);
+    hipLaunchKernelGGL(move_kernel, dim3(bb + blocks_of(items, n, group)), dim3(256), 0, st, a, x, n, group, items, bb);
   }
   return launched(op);
 }
@@ -604,7 +791,9 @@ extern "C" int ane_kv8_copy(const ane_kv8_pool* from, const ane_kv8_pool* into, 
     Layers x, y;
     const int n = layers_of(*from, l0, &x);
     layers_of(*into, l0, &y);
-    hipLaunchKernelGGL(copy_kernel, dim3(g.n * 2 * n), dim3(256), 0, st, p, q.pages, x, y, n, g.src, g.dst, g.tokens);
+    const int group = group_of(p, g.n, n);
+    hipLaunchKernelGGL(copy_kernel, dim3(blocks_of(g.n, n, group)), dim3(256), 0, st, p, q.pages, x, y, n, group, g.src,
+                       g.dst, g.tokens);
   }
   return launched(op);
 }

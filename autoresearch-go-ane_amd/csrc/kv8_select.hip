@@ -12,6 +12,7 @@
 
 #include "kv8.h"
 #include "op_error.h"
+#include "wave_ops.h"
 
 namespace ane {
 
@@ -132,70 +133,6 @@ struct SelectArgs {
   int room;  // scores that LDS holds
 };
 
-// Reductions over a wave, and over what its lanes hold NW-periodically.
-template <int N>
-__device__ __forceinline__ int row_ror(int v) {
-  return __builtin_amdgcn_update_dpp(0, v, 0x120 + N, 0xf, 0xf, false);
-}
-template <int N>
-__device__ __forceinline__ float row_ror(float v) {
-  return __int_as_float(row_ror<N>(__float_as_int(v)));
-}
-struct Max {
-  template <typename T>
-  __device__ T operator()(T a, T b) const { return a > b ? a : b; }
-};
-struct Sum {
-  __device__ int operator()(int a, int b) const { return a + b; }
-};
-template <typename T>
-__device__ __forceinline__ void swap16(T& a, T& b) {  // a's odd rows of 16 with b's even ones
-  const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b), false, false);
-  const uint32_t x = r[0], y = r[1];
-  a = __builtin_bit_cast(T, x);
-  b = __builtin_bit_cast(T, y);
-}
-template <typename T>
-__device__ __forceinline__ void swap32(T& a, T& b) {  // a's upper half with b's lower half
-  const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b), false, false);
-  const uint32_t x = r[0], y = r[1];
-  a = __builtin_bit_cast(T, x);
-  b = __builtin_bit_cast(T, y);
-}
-template <int N, typename T, typename Op>
-__device__ __forceinline__ T lanes(T v, Op op) {
-  if (N >= 2) v = op(v, row_ror<1>(v));
-  if (N >= 4) v = op(v, row_ror<2>(v));
-  if (N >= 8) v = op(v, row_ror<4>(v));
-  if (N >= 16) v = op(v, row_ror<8>(v));
-  if (N >= 32) {
-    T w = v;
-    swap16(v, w);
-    v = op(v, w);
-  }
-  if (N >= 64) {
-    T w = v;
-    swap32(v, w);
-    v = op(v, w);
-  }
-  return v;
-}
-// the sum over the lanes up to this one: within rows of 16, then the last lane
-// of a row to the row behind it, and of the lower half to the upper one
-template <int CTRL, int ROWS>
-__device__ __forceinline__ int shifted(int v) {
-  return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
-}
-__device__ __forceinline__ int sum_up_to(int v) {
-  v += shifted<0x111, 0xf>(v);
-  v += shifted<0x112, 0xf>(v);
-  v += shifted<0x114, 0xf>(v);
-  v += shifted<0x118, 0xf>(v);
-  v += shifted<0x142, 0xa>(v);
-  v += shifted<0x143, 0xc>(v);
-  return v;
-}
-
 constexpr int kBins = 256;
 constexpr int kHeld = 1024;  // pages of a token whose scores its waves hold in registers
 constexpr int kFar = 32768;  // scores that LDS holds at most
@@ -266,7 +203,7 @@ __global__ __launch_bounds__(64 * NW) void select_kernel(SelectArgs a) {
           amax = fmaxf(amax, fabsf(w));
         }
       }
-    float other = amax;
+    float other = amax;  // the row's other dimensions lie in the other rows of lanes
     swap16(amax, other);
     amax = fmaxf(amax, other);
     other = amax;
@@ -398,7 +335,7 @@ __global__ __launch_bounds__(64 * NW) void select_kernel(SelectArgs a) {
       using T = decltype(x);
       if (lane == 0) sums[turn][wave] = __builtin_bit_cast(int, x);
       __syncthreads();
-      x = lanes<CW>(__builtin_bit_cast(T, sums[turn][lane % CW]), op);
+      x = over_lanes<CW>(__builtin_bit_cast(T, sums[turn][lane % CW]), op);
       turn ^= 1;
     }
     return x;
@@ -420,7 +357,7 @@ __global__ __launch_bounds__(64 * NW) void select_kernel(SelectArgs a) {
     }
     return x;
   };
-  const auto widest = [&](float x) { return over(lanes<64>(x, Max()), Max()); };
+  const auto widest = [&](float x) { return over(over_lanes<64>(x, Max()), Max()); };
   int* bins = bins_of[wave / CW];
   float* few = few_of[wave / CW];
   const int ct = tid % CT, cw = wave % CW;
