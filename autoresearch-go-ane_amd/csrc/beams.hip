@@ -27,11 +27,12 @@ namespace {
 constexpr int kSeg = 256;       // entries of a segment
 constexpr int kMaxBeams = 32;   // of a request
 constexpr int kPer = 8;         // items a thread of the second launch holds
-constexpr int kFew = 8;         // beams for which 256 threads of it are enough
 constexpr int kMaxParts = 128;  // of a row
-constexpr int kWords = 1024;    // of 8 ids: the histories of a request that a block holds
-static_assert(kMaxBeams * (65536 / kSeg) <= 1024 * kPer && kMaxBeams * kSeg <= 1024 * kPer, "");
-static_assert(kFew * (65536 / kSeg) <= 256 * kPer && kFew * kSeg <= 256 * kPer, "");
+constexpr int kWords = 1024;    // of 8 ids: the histories of a request that the second launch reads ahead
+constexpr int kMoved = 8;       // words a thread of it moves
+// It has 32 threads a beam, or more: enough for the segments of a beam, and for
+// one segment.
+static_assert(65536 / kSeg <= 32 * kPer && kSeg <= 32 * kPer, "");
 
 // a wave's part of a row's log sum
 struct Part {
@@ -65,8 +66,6 @@ struct BeamArgs {
   Part* part;       // [rows][parts]
 };
 
-typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));
-typedef _Float16 half8u __attribute__((ext_vector_type(8), aligned(2)));
 typedef uint16_t ushort8u __attribute__((ext_vector_type(8), aligned(2)));
 
 // ids c .. c + 7 of a history of n > c (behind the last: anything)
@@ -94,58 +93,75 @@ __device__ __forceinline__ bool proposes(const BeamArgs& a, int r) {
   return !(a.finished && a.finished[r]) && a.scores[r] > -INFINITY && (!a.weights || a.weights[r] > 0.f);
 }
 
-// N neighbours from entry c on, NaN and what lies behind the vocabulary as -inf
-template <typename T, int N>
-__device__ __forceinline__ void load_row(const T* row, int c, int vocab, float (&x)[N]) {
-  if (c + N <= vocab) {
-    if constexpr (sizeof(T) == 4) {
-      const float4u v = *reinterpret_cast<const float4u*>(row + c);
-#pragma unroll
-      for (int j = 0; j < N; j++) x[j] = v[j];
-    } else {
-      const half8u v = *reinterpret_cast<const half8u*>(row + c);
-#pragma unroll
-      for (int j = 0; j < N; j++) x[j] = (float)v[j];
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < N; j++) x[j] = c + j < vocab ? (float)row[c + j] : -INFINITY;
-  }
-#pragma unroll
-  for (int j = 0; j < N; j++) x[j] = x[j] == x[j] ? x[j] : -INFINITY;
-}
-
-// A wave takes U loads of 64 N entries of a row.
+// A wave takes U loads of 64 N entries of a row.  A lane whose N reach past the
+// row's end takes the row's last N instead, and of those its own; rows of fewer
+// than N are read one by one.
 template <typename T, int U>
 __global__ __launch_bounds__(256) void part_kernel(BeamArgs a) {
   constexpr int N = 16 / sizeof(T), LS = kSeg / N, SPW = 64 / LS;  // lanes of a segment, segments of a load
+  typedef T Words __attribute__((ext_vector_type(N), aligned(sizeof(T))));
   const int lane = threadIdx.x & 63, r = blockIdx.y;
   const int p = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (p >= a.parts || !proposes(a, r)) return;
+  if (p >= a.parts) return;
+  if (!proposes(a, r)) return;
   const T* row = static_cast<const T*>(a.logits) + r * a.logits_row;
   const int c0 = p * (U * 64 * N) + lane * N;
-  float x[U][N], top[U];
+  Words w[U];
 #pragma unroll
-  for (int u = 0; u < U; u++) load_row<T, N>(row, c0 + u * 64 * N, a.vocab, x[u]);
+  for (int u = 0; u < U; u++) {
+    const int c = min(c0 + u * 64 * N, a.vocab - N);
+    if (a.vocab >= N) {
+      w[u] = *reinterpret_cast<const Words*>(row + c);
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; j++) w[u][j] = row[min(j, a.vocab - 1)];
+    }
+  }
+  Words none;  // -inf; the larger of it and NaN is it
+#pragma unroll
+  for (int j = 0; j < N; j++) none[j] = (T)-INFINITY;
+#pragma unroll
+  for (int u = 0; u < U; u++) w[u] = __builtin_elementwise_max(w[u], none);
+  if ((p + 1) * (U * 64 * N) > a.vocab) {  // the row's last wave
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const int c = c0 + u * 64 * N, at = a.vocab >= N ? min(c, a.vocab - N) : 0;
+#pragma unroll
+      for (int j = 0; j < N; j++) w[u][j] = at + j >= c && at + j < a.vocab ? w[u][j] : (T)-INFINITY;
+    }
+  }
+  float top[U];
   float m = -INFINITY;
 #pragma unroll
   for (int u = 0; u < U; u++) {
-    top[u] = x[u][0];
+    Words t = w[u];
 #pragma unroll
-    for (int j = 1; j < N; j++) top[u] = fmaxf(top[u], x[u][j]);
-    top[u] = over_lanes<32>(top[u], Max());
+    for (int n = N / 2; n > 0; n /= 2)  // of pairs while there are any
+#pragma unroll
+      for (int j = 0; j < n; j++) t[j] = __builtin_elementwise_max(t[j], t[j + n]);
+    top[u] = over_lanes<32>((float)t[0], Max());
     const float both = fmaxf(top[u], xor32_f(top[u]));
     if (SPW == 1) top[u] = both;
     m = fmaxf(m, both);
   }
+  // 2^((x - m) log2 e).  Of fp16 logits in one multiply-add, x log2 e less m
+  // log2 e as rounded; the sum makes up for that rounding.  An infinite m makes
+  // NaN: a row without candidates.
+  constexpr float kLog2e = 1.44269504088896340736f;
   float s = 0.f;
-  if (m > -INFINITY) {  // +inf: NaN, a row without candidates
+  double more = 1.0;
+  if (m > -INFINITY) {
+    const float ml = m * kLog2e;
+    if (sizeof(T) == 2) more = 1.0 - (double)__builtin_fmaf(m, kLog2e, -ml) * 0.69314718055994531;
 #pragma unroll
     for (int u = 0; u < U; u++)
 #pragma unroll
-      for (int j = 0; j < N; j++) s += __builtin_amdgcn_exp2f((x[u][j] - m) * 1.44269504088896340736f);
+      for (int j = 0; j < N; j++) {
+        const float x = (float)w[u][j];
+        s += __builtin_amdgcn_exp2f(sizeof(T) == 2 ? __builtin_fmaf(x, kLog2e, -ml) : (x - m) * kLog2e);
+      }
   }
-  const double sum = sum_over_lanes((double)s);
+  const double sum = sum_over_lanes((double)s) * more;
   float* seg = a.seg_max + (size_t)r * a.segs;
 #pragma unroll
   for (int u = 0; u < U; u++) {
@@ -169,7 +185,7 @@ __device__ __forceinline__ bool before(double ak, int aa, double bk, int ba) {
 
 template <int TH>
 struct Pick {
-  static constexpr int kBeams = TH == 256 ? kFew : kMaxBeams, kGroups = TH / 16;
+  static constexpr int kBeams = TH / 32, kGroups = TH / 16;
   double key[kBeams * 16 * kPer];  // those that may be among the best
   int at[kBeams * 16 * kPer];
   float x[kBeams * 16 * kPer];
@@ -193,77 +209,105 @@ __device__ __forceinline__ void row_best(double& key, int& at) {
 // best(rank, item) called for each by one thread.
 //
 // The want-th best of the best items of groups of 16 threads is a bar that at
-// least `want` items reach and few others do; ranks are counted among those, a wave an item,
-// its lanes the others.  At most the items of `want` groups reach the bar.
+// least `want` items reach and few others do; ranks are counted among those, a
+// wave an item, its lanes the others.  Where the groups were uneven and more
+// than a wave's lanes reach the bar, they are dealt out again, one to each group
+// in turn: at most the items of `want` groups, half of them, reach the next bar.
 template <int TH, typename F>
-__device__ __forceinline__ void pick(const Item (&x)[kPer], int per, int want, Pick<TH>& p, F best) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  double key = x[0].key;
-  int at = x[0].at;
-#pragma unroll
-  for (int j = 1; j < kPer; j++) {
-    if (j >= per) break;
-    const bool b = before(x[j].key, x[j].at, key, at);
-    key = b ? x[j].key : key;
-    at = b ? x[j].at : at;
-  }
-  row_best<8>(key, at);
-  row_best<4>(key, at);
-  row_best<2>(key, at);
-  row_best<1>(key, at);
-  if ((tid & 15) == 0) {
-    p.gkey[tid >> 4] = key;
-    p.gat[tid >> 4] = at;
-  }
-  if (tid == 0) p.count = 0;
-  __syncthreads();
+__device__ __forceinline__ void pick(Item (&x)[kPer], int per, int want, Pick<TH>& p, F best) {
   constexpr int GR = Pick<TH>::kGroups;
-  key = p.gkey[lane % GR];
-  at = p.gat[lane % GR];
+  static_assert(2 * Pick<TH>::kBeams <= GR, "");
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  for (;;) {
+    double key = x[0].key;
+    int at = x[0].at;
 #pragma unroll
-  for (int j = 0; j < 4; j++) {  // the groups have different items: one of them has this rank
-    const int b = wave * 4 + j;
-    const double bk = p.gkey[b];
-    const int ba = p.gat[b];
-    if (__popcll(__ballot(lane < GR && before(key, at, bk, ba))) == want - 1 && lane == 0) {
-      p.bar_key = bk;
-      p.bar_at = ba;
+    for (int j = 1; j < kPer; j++) {
+      if (j >= per) break;
+      const bool b = before(x[j].key, x[j].at, key, at);
+      key = b ? x[j].key : key;
+      at = b ? x[j].at : at;
     }
-  }
-  __syncthreads();
-  key = p.bar_key;
-  at = p.bar_at;
+    row_best<8>(key, at);
+    row_best<4>(key, at);
+    row_best<2>(key, at);
+    row_best<1>(key, at);
+    if ((tid & 15) == 0) {
+      p.gkey[tid >> 4] = key;
+      p.gat[tid >> 4] = at;
+    }
+    if (tid == 0) p.count = 0;
+    __syncthreads();
+    key = p.gkey[lane % GR];
+    at = p.gat[lane % GR];
 #pragma unroll
-  for (int j = 0; j < kPer; j++) {
-    if (j >= per) break;
-    if ((x[j].key > -INFINITY) & !before(key, at, x[j].key, x[j].at)) {
-      const int k = atomicAdd(&p.count, 1);
-      p.key[k] = x[j].key;
-      p.at[k] = x[j].at;
-      p.x[k] = x[j].x;
+    for (int j = 0; j < 4; j++) {  // the groups have different items: one of them has this rank
+      const int b = wave * 4 + j;
+      const double bk = p.gkey[b];
+      const int ba = p.gat[b];
+      if (__popcll(__ballot(lane < GR && before(key, at, bk, ba))) == want - 1 && lane == 0) {
+        p.bar_key = bk;
+        p.bar_at = ba;
+      }
     }
+    __syncthreads();
+    key = p.bar_key;
+    at = p.bar_at;
+#pragma unroll
+    for (int j = 0; j < kPer; j++) {
+      if (j >= per) break;
+      if ((x[j].key > -INFINITY) & !before(key, at, x[j].key, x[j].at)) {
+        const int k = atomicAdd(&p.count, 1);
+        p.key[k] = x[j].key;
+        p.at[k] = x[j].at;
+        p.x[k] = x[j].x;
+      }
+    }
+    __syncthreads();
+    const int n = p.count;
+    if (n <= 64) {
+      key = p.key[min(lane, n)];
+      at = p.at[min(lane, n)];
+      for (int b = wave; b < n; b += TH / 64) {
+        const double bk = p.key[b];
+        const int ba = p.at[b];
+        const int rank = __popcll(__ballot(lane < n && before(key, at, bk, ba)));
+        if (rank < want && lane == 0) best(rank, Item{bk, ba, p.x[b]});
+      }
+      break;
+    }
+    per = (n + TH - 1) / TH;
+#pragma unroll
+    for (int j = 0; j < kPer; j++) {
+      if (j >= per) break;
+      const int k = j * TH + (tid & 15) * GR + (tid >> 4);
+      x[j] = {-INFINITY, kNone + k, 0.f};
+      if (k < n) x[j] = {p.key[k], p.at[k], p.x[k]};
+    }
+    __syncthreads();
   }
   __syncthreads();
-  const int n = p.count;
-  if (n <= 64) {
-    key = p.key[min(lane, n)];
-    at = p.at[min(lane, n)];
-    for (int b = wave; b < n; b += TH / 64) {
-      const double bk = p.key[b];
-      const int ba = p.at[b];
-      const int rank = __popcll(__ballot(lane < n && before(key, at, bk, ba)));
-      if (rank < want && lane == 0) best(rank, Item{bk, ba, p.x[b]});
-    }
-  } else {
-    for (int k = tid; k < n; k += TH) {
-      key = p.key[k];
-      at = p.at[k];
-      int above = 0;
-      for (int b = 0; b < n && above < want; b++) above += before(p.key[b], p.at[b], key, at);
-      if (above < want) best(above, Item{key, at, p.x[k]});
-    }
+}
+
+// The natural logarithm of a positive number, to 1e-11: of m 2^e with m about 1,
+// 2 atanh((m - 1) / (m + 1)) as its series.  The library's, to the last bit,
+// takes three times the instructions, in all 16 waves.
+__device__ __forceinline__ double log_of(double x) {
+  int e = __builtin_amdgcn_frexp_exp(x);
+  double m = __builtin_amdgcn_frexp_mant(x);  // 0.5 .. 1
+  if (m < 0.70710678118654752) {
+    m *= 2.0;
+    e -= 1;
   }
-  __syncthreads();
+  const double s = (m - 1.0) / (m + 1.0), q = s * s;  // q < 0.0295, whose 7th power over 15 is 1e-12
+  double y = 1.0 / 13;
+  y = __builtin_fma(y, q, 1.0 / 11);
+  y = __builtin_fma(y, q, 1.0 / 9);
+  y = __builtin_fma(y, q, 1.0 / 7);
+  y = __builtin_fma(y, q, 1.0 / 5);
+  y = __builtin_fma(y, q, 1.0 / 3);
+  y = __builtin_fma(y, q, 1.0);
+  return __builtin_fma((double)e, 0.69314718055994531, 2.0 * s * y);
 }
 
 // A block per request.  What bounds it is the chain of its memory accesses:
@@ -292,10 +336,8 @@ __global__ __launch_bounds__(TH) void choose_kernel(BeamArgs a) {
     x[j] = {-INFINITY, kNone + j * TH + tid, -INFINITY};
     if (j >= per) continue;
     const int u = j * NW + wave, w = u / runs, seg = (u - w * runs) * 64 + lane;
-    if (w < W && seg < a.segs) {
-      x[j].x = a.seg_max[(size_t)(row0 + w) * a.segs + seg];
-      x[j].at = w << 16 | seg;
-    }
+    x[j].x = a.seg_max[(size_t)(row0 + min(w, W - 1)) * a.segs + min(seg, a.segs - 1)];
+    if (w < W && seg < a.segs) x[j].at = w << 16 | seg;
   }
   Part q[BW][PL];
   float sc[BW], wt[BW];
@@ -318,7 +360,7 @@ __global__ __launch_bounds__(TH) void choose_kernel(BeamArgs a) {
 #pragma unroll
   for (int k = 0; k < HQ; k++) {
     const int t = k * TH + tid;
-    if (t < words) {
+    if (t < words && words <= kWords) {
       const int w = quotient(t, a.words, a.words_magic);
       ids[k] = get_ids(a.history + (row0 + w) * a.history_row, (t - w * a.words) * 8, a.history_max);
     }
@@ -342,7 +384,7 @@ __global__ __launch_bounds__(TH) void choose_kernel(BeamArgs a) {
     sum = lane == i ? s : sum;
     top = lane == i ? (double)m : top;
   }
-  const double l = top + log(sum);
+  const double l = top + log_of(sum);
 #pragma unroll
   for (int i = 0; i < BW; i++) {
     const int w = wave + i * NW;
@@ -361,7 +403,7 @@ __global__ __launch_bounds__(TH) void choose_kernel(BeamArgs a) {
   }
 #pragma unroll
   for (int k = 0; k < HQ; k++)
-    if (k * TH + tid < words) hist[k * TH + tid] = ids[k];
+    if (k * TH + tid < words && words <= kWords) hist[k * TH + tid] = ids[k];
   __syncthreads();
   const auto key_of = [&](int w, float x) {
     const double k = weight[w] * (score[w] + ((double)x - lse[w]));
@@ -381,24 +423,27 @@ __global__ __launch_bounds__(TH) void choose_kernel(BeamArgs a) {
   // the best W candidates in them, 64 of a segment a wave's at a time; an index
   // is the beam and the token
   per = (W * (kSeg / 64) + NW - 1) / NW;
+  T y[kPer];
 #pragma unroll
-  for (int j = 0; j < kPer; j++) {
-    x[j] = {-INFINITY, kNone + j * TH + tid, -INFINITY};
+  for (int j = 0; j < kPer; j++) {  // all on their way
+    x[j] = {-INFINITY, kNone + j * TH + tid, 0.f};
     if (j >= per) continue;
-    const int u = j * NW + wave, seg = __builtin_amdgcn_readfirstlane(seg_of[min(u / (kSeg / 64), W - 1)]);
-    const int w = seg >> 16, i = u % (kSeg / 64) * 64 + lane, v = (seg & 0xffff) * kSeg + i;
-    if (seg < 0 || u >= W * (kSeg / 64)) continue;
-    if (ended[w]) {
-      if (i == 0) x[j] = {-INFINITY, w << 16 | a.eos, 0.f};
-    } else if (v < a.vocab) {
-      x[j].x = (float)logits[(row0 + w) * a.logits_row + v];
-      x[j].at = w << 16 | v;
+    const int u = j * NW + wave, k = u / (kSeg / 64), seg = __builtin_amdgcn_readfirstlane(seg_of[min(k, W - 1)]);
+    const int w = max(seg, 0) >> 16, i = u % (kSeg / 64) * 64 + lane, v = (seg & 0xffff) * kSeg + i;
+    y[j] = logits[(row0 + w) * a.logits_row + min(v, a.vocab - 1)];
+    if (seg >= 0 && k < W) {
+      if (ended[w]) x[j].at = i == 0 ? w << 16 | a.eos : x[j].at;
+      else if (v < a.vocab) x[j].at = w << 16 | v;
     }
   }
 #pragma unroll
   for (int j = 0; j < kPer; j++) {
     if (j >= per) break;
-    if (x[j].at < kNone) x[j].key = key_of(x[j].at >> 16, x[j].x);
+    if (x[j].at < kNone) {
+      const int w = x[j].at >> 16;
+      x[j].x = ended[w] ? 0.f : (float)y[j];
+      x[j].key = key_of(w, x[j].x);
+    }
   }
   pick<TH>(x, per, W, pick_, [&](int rank, const Item& t) {
     const int w = t.at >> 16;
@@ -424,9 +469,27 @@ __global__ __launch_bounds__(TH) void choose_kernel(BeamArgs a) {
     }
     return;
   }
-  // the histories are in LDS
+  if (words > kWords) {
+    // the ones that move: all are read before any is written
+    ushort8u v[kMoved];
+#pragma unroll
+    for (int k = 0; k < kMoved; k++) {
+      const int t = k * TH + tid, w = quotient(min(t, words - 1), a.words, a.words_magic), c = (t - w * a.words) * 8;
+      const int from = parent[w];
+      if (t < words && from >= 0 && from != w && c < length[from])
+        v[k] = get_ids(a.history + (row0 + from) * a.history_row, c, length[from]);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kMoved; k++) {
+      const int t = k * TH + tid, w = quotient(min(t, words - 1), a.words, a.words_magic), c = (t - w * a.words) * 8;
+      const int from = parent[w];
+      if (t < words && from >= 0 && from != w) put_ids(a.history + (row0 + w) * a.history_row, c, length[from], v[k]);
+    }
+  }
+  // the ones that are in LDS
 #pragma unroll 1
-  for (int t = tid; t < words; t += TH) {
+  for (int t = tid; t < words && words <= kWords; t += TH) {
     const int w = quotient(t, a.words, a.words_magic), c = t - w * a.words, from = parent[w];
     if (from >= 0 && from != w) put_ids(a.history + (row0 + w) * a.history_row, c * 8, length[from], hist[from * a.words + c]);
   }
@@ -466,8 +529,11 @@ __global__ __launch_bounds__(256) void move_kernel(BeamArgs a) {
     a.history[(row0 + tid) * a.history_row + move[tid].len] = (uint16_t)move[tid].token;
 }
 
-// Loads of a wave in the first launch.
-int loads_of(int64_t rows, int vocab, bool half) { return 2; }
+// Loads of a wave in the first launch.  Of fp32 logits four, where that leaves
+// enough waves (512 rows of 32000: 21.2 us a step, with two 22.4; 64 rows 12.8
+// and 12.6); of fp16, which take as many instructions for half the bytes, two
+// (640 rows of 60011: 32.7 us, with four 33.5).
+int loads_of(int64_t rows, int vocab, bool half) { return !half && rows * (vocab / 512) >= 16384 ? 4 : 2; }
 
 struct Plan {
   int loads, segs, parts;
@@ -493,7 +559,7 @@ uint32_t magic(int n) { return (uint32_t)(((1ull << 32) + n - 1) / n); }
 
 template <typename T>
 void launch_choose(const BeamArgs& a, int requests, hipStream_t st) {
-  if (a.beams <= kFew) hipLaunchKernelGGL((choose_kernel<T, 256>), dim3(requests), dim3(256), 0, st, a);
+  if (a.beams <= 8) hipLaunchKernelGGL((choose_kernel<T, 256>), dim3(requests), dim3(256), 0, st, a);
   else hipLaunchKernelGGL((choose_kernel<T, 1024>), dim3(requests), dim3(1024), 0, st, a);
 }
 
@@ -558,7 +624,10 @@ extern "C" int ane_beam_select(const ane_beam_args* args, void* stream) {
   a.words = (g.history_max + 7) / 8;
   a.words_magic = a.words ? magic(a.words) : 0;
   a.stretch = kWords / g.beams;
-  a.moves = g.beams * a.words > kWords ? (Move*)((char*)g.ws + p.seg_bytes) : nullptr;
+  // Histories of up to 8 words a thread move in the second launch (40 requests of
+  // 16 beams and 2564 ids: 35.6 us a step, in a launch of their own 37.8).
+  const int threads = g.beams <= 8 ? 256 : 1024;
+  a.moves = g.beams * a.words > kMoved * threads ? (Move*)((char*)g.ws + p.seg_bytes) : nullptr;
   a.part = (Part*)((char*)g.ws + p.seg_bytes + p.move_bytes);
   const hipStream_t st = (hipStream_t)stream;
   const dim3 grid((p.parts + 3) / 4, (uint32_t)rows);
@@ -566,7 +635,8 @@ extern "C" int ane_beam_select(const ane_beam_args* args, void* stream) {
     hipLaunchKernelGGL((part_kernel<half_t, 2>), grid, dim3(256), 0, st, a);
     launch_choose<half_t>(a, g.requests, st);
   } else {
-    hipLaunchKernelGGL((part_kernel<float, 2>), grid, dim3(256), 0, st, a);
+    if (p.loads == 4) hipLaunchKernelGGL((part_kernel<float, 4>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((part_kernel<float, 2>), grid, dim3(256), 0, st, a);
     launch_choose<float>(a, g.requests, st);
   }
   if (a.moves)

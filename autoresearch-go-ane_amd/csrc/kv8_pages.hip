@@ -46,8 +46,9 @@ __device__ __forceinline__ void settle() {
 // l's keys, 2 l + 1 its values), their first `units` units of 16 tokens, by a
 // block of TH threads.  A unit of a head is 16 * head_dim bytes in a row on both
 // sides.  Four loads a thread are under way at once: of one side, or of four
-// where sides are small and come several to a block.
-template <int TH>
+// where sides are small and come several to a block.  FAR: pages that the caches
+// do not hold until somebody reads them go past them.
+template <int TH, bool FAR>
 __device__ __forceinline__ void copy_sides(const Pool& p, const Layers& x, const Layers& y, int side0, int sides,
                                            int from, int to, int units) {
   const int tid = threadIdx.x;
@@ -57,6 +58,11 @@ __device__ __forceinline__ void copy_sides(const Pool& p, const Layers& x, const
   const auto place = [&](uint32_t t) {
     const uint32_t h = used == whole ? 0 : t / used;
     return h * whole + (t - h * used);
+  };
+  const auto load = [](const u32x4* p) { return FAR ? __builtin_nontemporal_load(p) : *p; };
+  const auto store = [](u32x4* p, u32x4 w) {
+    if (FAR) __builtin_nontemporal_store(w, p);
+    else *p = w;
   };
   constexpr int U = 4;
   if (sides == 1) {
@@ -69,11 +75,11 @@ __device__ __forceinline__ void copy_sides(const Pool& p, const Layers& x, const
 #pragma unroll
       for (int u = 0; u < U; u++) {
         o[u] = place(min(t0 + u * TH, n - 1));
-        w[u] = s[o[u]];
+        w[u] = load(s + o[u]);
       }
 #pragma unroll
       for (int u = 0; u < U; u++)
-        if (t0 + u * TH < n) d[o[u]] = w[u];
+        if (t0 + u * TH < n) store(d + o[u], w[u]);
     }
   } else {
     for (int i = 0; i < sides; i += U) {
@@ -89,10 +95,10 @@ __device__ __forceinline__ void copy_sides(const Pool& p, const Layers& x, const
         const uint32_t o = place(t);
         u32x4 w[U];
 #pragma unroll
-        for (int u = 0; u < U; u++) w[u] = s[u][o];
+        for (int u = 0; u < U; u++) w[u] = load(s[u] + o);
 #pragma unroll
         for (int u = 0; u < U; u++)
-          if (i + u < sides) d[u][o] = w[u];
+          if (i + u < sides) store(d[u] + o, w[u]);
       }
     }
   }
@@ -423,8 +429,8 @@ __global__ __launch_bounds__(256) void finish_kernel(ForkArgs a, Layers x, int n
   const Sides s = sides_of(blockIdx.x - table_blocks, nlayers, group);
   const Next n = a.next[s.item];
   if (n.src < 0 || n.base >= found) return;
-  copy_sides<256>(a.p, x, x, s.first, s.count, n.src, a.free[n.base],
-                  units_of(a.p, n.st & ((1 << a.p.pshift) - 1)));
+  copy_sides<256, false>(a.p, x, x, s.first, s.count, n.src, a.free[n.base],
+                         units_of(a.p, n.st & ((1 << a.p.pshift) - 1)));
 }
 
 // ---- compact -------------------------------------------------------------------
@@ -537,18 +543,19 @@ __global__ __launch_bounds__(256) void move_kernel(CompactArgs a, Layers x, int 
   const Sides s = sides_of(blockIdx.x - book_blocks, nlayers, group);
   const int total = *a.total;
   for (int k = s.item; k < total; k += items)
-    copy_sides<256>(a.p, x, x, s.first, s.count, a.movers[k], a.holes[k], 1 << (a.p.pshift - 4));
+    copy_sides<256, true>(a.p, x, x, s.first, s.count, a.movers[k], a.holes[k], 1 << (a.p.pshift - 4));
 }
 
 // ---- copy ----------------------------------------------------------------------
 
+template <bool FAR>
 __global__ __launch_bounds__(256) void copy_kernel(Pool p, int into_pages, Layers x, Layers y, int nlayers,
                                                    int group, const int* src, const int* dst, const int* tokens) {
   const Sides s = sides_of(blockIdx.x, nlayers, group);
   const int from = src[s.item], to = dst[s.item];
   if ((unsigned)from >= (unsigned)p.pages || (unsigned)to >= (unsigned)into_pages) return;
   const int units = tokens ? units_of(p, tokens[s.item]) : 1 << (p.pshift - 4);
-  if (units > 0) copy_sides<256>(p, x, y, s.first, s.count, from, to, units);
+  if (units > 0) copy_sides<256, FAR>(p, x, y, s.first, s.count, from, to, units);
 }
 
 // ---- host ----------------------------------------------------------------------
@@ -792,8 +799,11 @@ extern "C" int ane_kv8_copy(const ane_kv8_pool* from, const ane_kv8_pool* into, 
     const int n = layers_of(*from, l0, &x);
     layers_of(*into, l0, &y);
     const int group = group_of(p, g.n, n);
-    hipLaunchKernelGGL(copy_kernel, dim3(blocks_of(g.n, n, group)), dim3(256), 0, st, p, q.pages, x, y, n, group, g.src,
-                       g.dst, g.tokens);
+    // past the caches from what the L2s hold on: 3700 pages in 8 layers (490 MB)
+    // 98 us, through them 105
+    const bool far = (int64_t)g.n * 2 * n * (p.NKV << (p.pshift + p.dshift)) >= 32 << 20;
+    hipLaunchKernelGGL(far ? copy_kernel<true> : copy_kernel<false>, dim3(blocks_of(g.n, n, group)), dim3(256), 0, st, p,
+                       q.pages, x, y, n, group, g.src, g.dst, g.tokens);
   }
   return launched(op);
 }
