@@ -664,6 +664,13 @@ int plan(const char* op, const Kv8Batch& b, const ane_kv8_batch& given, int DH, 
   // of 2048 46 against 37).
   const int wps = waves_per_simd(DH, p->nt);
   p->kw = p->nt > 1 && !count && 2 * blocks >= (int64_t)wps * len ? 1 : 4;
+  // Lists of up to 2048 keys in up to 128 blocks: eight waves, and whole (with
+  // update and choice of pages, 4 blocks of 1024 keys 17.5 us, with four waves
+  // 18.1; of 2048 19.3, in parts 19.5; 64 blocks of 2048 20.3 and 21.4, 128 22.8
+  // and 23.9; but 256 28.1 and 27.1, 4 of 4096 23.0 and 20.1, and at head
+  // dimension 128 26.4 and 22.0).
+  const bool eight = count && p->nt == 1 && DH == 64 && blocks <= 128 && len <= 2048;
+  if (eight) p->kw = 8;
   p->round = p->kw * kStep;
   // The longest contexts first, so that the last blocks to end are short ones:
   // chunks of prompts at the lengths they come in (8 of 100 to 400 on up to
@@ -690,7 +697,9 @@ int plan(const char* op, const Kv8Batch& b, const ane_kv8_batch& given, int DH, 
   // outlast the rest (64 of 8 heads and up to 30,000 keys 206 us, whole 232;
   // 80 blocks of up to 40,000 108 us, of 4096 keys 113).
   int64_t ns = 1;
-  if (p->nt == 1) {
+  if (eight) {
+    ns = 1;
+  } else if (p->nt == 1) {
     if (len > (blocks >= 128 ? std::min<int64_t>(32 * blocks, 8192) : DH == 64 ? 1280 : 768))
       ns = std::max<int64_t>(std::min<int64_t>((511 + blocks) / blocks, (len + 255) / 256), (len + 2047) / 2048);
   } else if (p->kw == 4) {
@@ -738,8 +747,11 @@ void launch(const AttendArgs& a, const Plan& p, hipStream_t st) {
 
 template <int DH>
 void launch_list(const ListArgs& a, const Plan& p, hipStream_t st) {
-  if (p.nt == 1) launch_form<DH, 1, 4, 1>(a, st);
-  else launch_form<DH, 2, 4, 1>(a, st);
+  if constexpr (DH == 64) {
+    if (p.kw == 8) launch_form<DH, 1, 8, 1>(a, st);
+  }
+  if (p.kw == 4 && p.nt == 1) launch_form<DH, 1, 4, 1>(a, st);
+  else if (p.kw == 4) launch_form<DH, 2, 4, 1>(a, st);
   if (a.nsplit > 1)
     hipLaunchKernelGGL((join_kernel<DH, ListArgs>), dim3((uint32_t)a.tiles * a.b.NKV, (a.G + 3) / 4), dim3(256), 0, st,
                        a);

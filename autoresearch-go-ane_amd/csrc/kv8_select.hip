@@ -41,8 +41,17 @@ struct BoundArgs {
 
 __device__ __forceinline__ half2v min2(half2v a, half2v b) { return __builtin_elementwise_min(a, b); }
 __device__ __forceinline__ half2v max2(half2v a, half2v b) { return __builtin_elementwise_max(a, b); }
-__device__ __forceinline__ half2v shfl2(half2v x, int o) {
-  return __builtin_bit_cast(half2v, __shfl_xor(__builtin_bit_cast(int, x), o, 64));
+// over the lanes that are N apart, N = 4 or 8
+template <int N, typename Op>
+__device__ __forceinline__ half2v over_rows(half2v v, Op op) {
+  if constexpr (N == 4) v = op(v, __builtin_bit_cast(half2v, row_ror<4>(__builtin_bit_cast(int, v))));
+  v = op(v, __builtin_bit_cast(half2v, row_ror<8>(__builtin_bit_cast(int, v))));
+  half2v w = v;
+  swap16(v, w);
+  v = op(v, w);
+  w = v;
+  swap32(v, w);
+  return op(v, w);
 }
 
 // A wave per page that got rows and key/value head.  A lane takes 16
@@ -85,11 +94,8 @@ __global__ __launch_bounds__(64) void bound_kernel(BoundArgs a) {
   float l[16], u[16];
 #pragma unroll
   for (int j = 0; j < 8; j++) {
-#pragma unroll
-    for (int o = 32; o >= LR; o >>= 1) {
-      lo[j] = min2(lo[j], shfl2(lo[j], o));
-      hi[j] = max2(hi[j], shfl2(hi[j], o));
-    }
+    lo[j] = over_rows<LR>(lo[j], [](half2v a, half2v b) { return min2(a, b); });
+    hi[j] = over_rows<LR>(hi[j], [](half2v a, half2v b) { return max2(a, b); });
 #pragma unroll
     for (int e = 0; e < 2; e++) {
       // no number: lo = inf, hi = -inf (or both NaN)
