@@ -240,10 +240,10 @@ class KVCache8:
         if out is None:
             out = self._new(batch, heads)
         yp, yr, yh = self._rows(op, "out", out, batch, heads)
-        bp = count = 0
+        key = (self.kv_heads, self.page_tokens, self.head_dim, heads)
         if blocks is not None:
             bp, count = self._blocks(op, blocks, batch)
-        key = (self.kv_heads, self.page_tokens, self.head_dim, heads, count)
+            key += (count,)
         n = batch._ws.get(key)
         if n is None:
             if blocks is None:

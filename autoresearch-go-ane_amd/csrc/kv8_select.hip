@@ -169,7 +169,7 @@ __global__ __launch_bounds__(64 * NW) void select_kernel(SelectArgs a) {
   constexpr int CH = NW / CW, CT = 64 * CW, R = kHeld / CT;
   extern __shared__ float scores[];  // [TOK][stride], room of them in all
   __shared__ int bins_of[CH][kBins];
-  __shared__ float few_of[CH][64];
+  __shared__ __attribute__((aligned(16))) float few_of[CH][64];
   __shared__ int fews, sums[2][CW];
   const Kv8Batch& b = a.b;
   const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, g = lane >> 4;
@@ -493,13 +493,18 @@ __global__ __launch_bounds__(64 * NW) void select_kernel(SelectArgs a) {
             if (is) few[at + __popcll(who & below)] = x;
             at += __popcll(who);
           });
+          if (ct < 4 && in + ct < 64) few[in + ct] = -INFINITY;  // behind them, to whole words
           meet();
           const float x = few[min(lane, in - 1)];
           int above = 0, from = 0;
-          for (int k = 0; k < in; k++) {
-            const float y = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), k));
-            above += y > x;
-            from += y >= x;
+#pragma unroll 2
+          for (int k = 0; k < in; k += 4) {
+            const floatx4 y = *reinterpret_cast<const floatx4*>(few + k);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+              above += y[j] > x;
+              from += y[j] >= x;
+            }
           }
           const int who = __ffsll((unsigned long long)__ballot(lane < in && above < need && need <= from)) - 1;
           bar = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), who));

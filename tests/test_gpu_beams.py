@@ -302,3 +302,44 @@ def test_two_calls_at_once():
         np.testing.assert_array_equal(g[0].cpu().numpy(), want["tokens"])
         np.testing.assert_array_equal(g[1].cpu().numpy(), want["parents"])
         np.testing.assert_array_equal(h.cpu().numpy().view(np.uint16), want["history"])
+
+
+@pytest.mark.parametrize("beams, hist", [(4, 2040), (4, 2056), (4, 4096), (4, 4104), (8, 1023), (8, 2050), (16, 500),
+                                         (16, 513), (16, 4095), (16, 4097), (32, 256), (32, 2049), (9, 7000)])
+def test_histories_in_every_form(beams, hist):
+    """Read ahead, moved by the second launch, and by one of their own."""
+    r = np.random.default_rng(beams * 10000 + hist)
+    c = Case(r, 2, beams, 64, hist=hist, eos=1, wide=beams % 3)
+    c.lengths[:] = np.maximum(hist - r.integers(0, 20, 2 * beams), 0)
+    c.lengths[0], c.lengths[-1] = hist, 0
+    c.check(offset=beams % 2)
+
+
+@pytest.mark.parametrize("beams", [8, 9, 16, 32])
+@pytest.mark.parametrize("vocab", [64, 300, 5000, 20000])
+def test_uneven_groups(beams, vocab):
+    """Sorted logits and few segments: far more than a wave's lanes reach the
+    first bar."""
+    r = np.random.default_rng(vocab)
+    for order in (1, -1):
+        c = Case(r, 2, beams, vocab, hist=None, weights=False)
+        c.logits[:] = np.sort(r.standard_normal((2 * beams, vocab)).astype(np.float32))[:, ::order]
+        c.scores[:] = -5 - 1e-3 * np.arange(2 * beams)
+        c.check()
+
+
+def test_scores_far_from_each_other():
+    c = Case(np.random.default_rng(12), 2, 6, 500, weights=False)
+    c.scores[:] = [0, -1e4, -1e30, 1e30, 3e38, -3e38] * 2
+    c.logits[3, 7] = 60000
+    c.check()
+
+
+@pytest.mark.parametrize("half", [False, True])
+def test_logits_of_large_magnitude(half):
+    r = np.random.default_rng(13)
+    c = Case(r, 2, 4, 700, half, weights=False)
+    top = 60000.0 if half else 3e38
+    c.logits[:4] = (r.uniform(-1, 1, (4, 700)) * top).astype(c.logits.dtype)
+    c.logits[4:] = (top - r.integers(0, 3, (4, 700)) * (32 if half else 1e33)).astype(c.logits.dtype)
+    c.check()

@@ -351,3 +351,29 @@ def test_captured_forks():
         np.testing.assert_array_equal(to.cpu().numpy(), wm)
         assert int(missing) == m
         pool.check()
+
+
+@pytest.mark.parametrize("nseq, width", [(1024, 8), (1025, 8), (1024, 9), (3000, 4)])
+def test_every_size_of_table(nseq, width):
+    """By one block, and by many; writers of shared pages by hashing and by
+    marks."""
+    r = np.random.default_rng(nseq + width)
+    P, pages = 16, nseq * 3 + 100
+    pool = Pool(r, pages, 1, 1)
+    table = np.full((nseq, width), -1, np.int32)
+    ids = r.permutation(pages)
+    table[:, 0], table[:, 1] = ids[:nseq], ids[nseq + r.integers(0, nseq // 2, nseq)]   # second pages shared
+    start = r.integers(17, 31, nseq).astype(np.int32)
+    refs = np.bincount(table[table >= 0], minlength=pages).astype(np.int32)
+    refs[table[::7, 1]] += 1
+    run_fork(pool, table, start, refs, r.integers(0, nseq, nseq), r.integers(0, 20, nseq))
+
+
+def test_copies_of_many_small_pages():
+    """Four sides a block, more layers than make whole fours, and past the
+    caches."""
+    r = np.random.default_rng(10)
+    for layers, kvh, P, n in ((5, 1, 16, 600), (3, 2, 16, 900), (7, 4, 16, 2100)):
+        a, b = Pool(r, n + 5, layers, kvh, P), Pool(r, n + 9, layers, kvh, P, bounds=True)
+        copy_pages(a, b, r.permutation(n + 5)[:n], r.permutation(n + 9)[:n], r.integers(0, P + 1, n))
+        copy_pages(a, b, r.permutation(n + 5)[:n], r.permutation(n + 9)[:n], None)

@@ -318,3 +318,96 @@ def test_captured():
         step()
         torch.cuda.synchronize()
         assert torch.equal(gb[:2], b[:2]) and torch.equal(got[:2], out[:2])
+
+
+@pytest.mark.parametrize("heads, kvh, dh", [(2, 2, 64), (6, 1, 128), (12, 1, 64), (20, 1, 64), (3, 1, 128)])
+def test_long_chunks_and_wrong_hints(heads, kvh, dh):
+    """Contexts of more pages than a token's waves hold, with scores in LDS, and
+    (hints of a shorter one) without."""
+    r = np.random.default_rng(heads)
+    for hints in (dict(max_new=3), dict(max_new=3, max_len=100), dict(max_new=1, max_len=100), {}):
+        x = Run(r, [(16 * 1100 + 3, 3), (70, 2)], heads, kvh, dh, 16, **hints).go()
+        lo = np.minimum(x.box[:, :, 0], x.box[:, :, 1])
+        x.box[:, :, 0], x.box[:, :, 1] = np.maximum(x.box[:, :, 0], x.box[:, :, 1]), lo
+        x.bounds.box.copy_(dev(x.box))
+        x.select(33, 1, 2)
+
+
+def test_most_scores_in_lds_under_capture():
+    r = np.random.default_rng(14)
+    x = Run(r, [(16 * 12000 + 3, 1)], 2, 1, 64, 16, max_len=16 * 12001, max_new=1).go()
+    q, b = dev(x.q), torch.zeros((x.rows, 1, 50), dtype=torch.int32, device=DEV)
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            x.bounds.Select(x.batch, q, 50, blocks=b)
+    for _ in range(3):
+        b.fill_(77)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        want = x.select(50)
+        np.testing.assert_array_equal(b.cpu().numpy()[:1], want[:1])
+
+
+def test_scores_far_apart():
+    """Outliers, so that the first histograms leave nearly all pages in a bin."""
+    r = np.random.default_rng(15)
+    x = Run(r, [(16 * 700 + 5, 1), (16 * 300, 2)], 4, 2, 64, 16)
+    x.box[:] = r.integers(-3, 4, x.box.shape)
+    x.unit[:] = r.choice([-30, -20, -8, 0, 9], x.unit.shape, p=[0.5, 0.3, 0.1, 0.09, 0.01])
+    x.go()
+    for count in (5, 64, 100, 300):
+        x.select(count, 0, 0)
+    x.box[:] = 0
+    x.bounds.box.zero_()
+    x.select(9, 0, 0)
+
+
+def test_units_that_no_update_wrote_stay_in_range():
+    r = np.random.default_rng(16)
+    x = Run(r, [(16 * 200 + 5, 1)], 4, 2, 64, 16)
+    x.unit[:] = r.choice([-128, -31, 41, 127], x.unit.shape)
+    x.go()
+    b = x.bounds.Select(x.batch, dev(x.q), 7).cpu().numpy()[0]
+    assert ((b >= 0) & (b <= 200)).all() and (np.diff(b, axis=1) > 0).all() and (b[:, 0] == 0).all() and (b[:, -1] == 200).all()
+
+
+@pytest.mark.parametrize("P, heads, kvh, dh", [(16, 4, 2, 64), (64, 12, 1, 128), (32, 20, 1, 64)])
+def test_nan_in_keys_and_values(P, heads, kvh, dh):
+    r = np.random.default_rng(17)
+    x = Run(r, [(P * 9 + 5, 3), (P * 3, 1), (2, 2)], heads, kvh, dh, P, nan=0.001).go()
+    b = np.sort(r.integers(-2, 10, (x.rows, kvh, 4)).astype(np.int32))
+    x.attend(b)
+
+
+@pytest.mark.parametrize("heads, kvh, dh", [(4, 4, 64), (12, 4, 64), (16, 2, 128), (40, 2, 64)])
+def test_many_parts(heads, kvh, dh):
+    """Lists long enough to be cut, some of them short."""
+    r = np.random.default_rng(18)
+    x = Run(r, [(64 * 90 + 3, 1), (64 * 3, 1), (7, 1)], heads, kvh, dh, 64).go()
+    b = np.full((x.rows, kvh, 80), -1, np.int32)
+    b[0] = np.sort(np.stack([r.permutation(91)[:80] for _ in range(kvh)]))
+    b[0, 0, 60:] = -1
+    b[1, :, :4], b[2, :, 0] = np.arange(4), 0
+    x.attend(b)
+
+
+def test_two_streams_at_once():
+    r = np.random.default_rng(19)
+    runs = [Run(r, [(64 * 40 + i, 1), (64 * 30, 2)], 4, 2, 64, 64).go() for i in range(2)]
+    qs = [dev(x.q) for x in runs]
+    torch.cuda.synchronize()
+    got = []
+    for x, q in zip(runs, qs):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            x.bounds.Update(x.batch)
+            b = x.bounds.Select(x.batch, q, 40)
+            got.append((b, x.pool.cache.Attend(x.batch, q, blocks=b)))
+    torch.cuda.synchronize()
+    for x, q, (b, o) in zip(runs, qs, got):
+        n = int(x.offsets[-1])
+        w = x.bounds.Select(x.batch, q, 40)
+        y = x.pool.cache.Attend(x.batch, q, blocks=w)
+        assert torch.equal(b[:n], w[:n]) and torch.equal(o[:n], y[:n])
