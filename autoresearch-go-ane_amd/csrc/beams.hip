@@ -11,9 +11,10 @@
 // that only W segments are read again and no launch sorts or keeps more.
 //
 // Keys are 64-bit sums of 32-bit logits and scores and of log sums whose
-// exponentials are fp32 and whose additions are 64-bit: two candidates' order
-// is in doubt only where they differ by 1e-8 or so; equal ones go to the lower
-// beam, then the lower token.
+// exponentials are fp32 (off by 2e-7 at most) and whose additions are 64-bit:
+// the order of two beams' candidates is in doubt only where they differ by
+// less, and of one beam's where 64 bits make their keys equal; equal ones go to
+// the lower beam, then the lower token.
 #include <algorithm>
 
 #include "kv8.h"
@@ -145,14 +146,18 @@ __global__ __launch_bounds__(256) void part_kernel(BeamArgs a) {
     m = fmaxf(m, both);
   }
   // 2^((x - m) log2 e).  Of fp16 logits in one multiply-add, x log2 e less m
-  // log2 e as rounded; the sum makes up for that rounding.  An infinite m makes
-  // NaN: a row without candidates.
+  // log2 e as rounded; the sum makes up for that rounding, d (below 0.003 for any
+  // fp16 m), to its third power.  An infinite m makes NaN: a row without
+  // candidates.
   constexpr float kLog2e = 1.44269504088896340736f;
   float s = 0.f;
   double more = 1.0;
   if (m > -INFINITY) {
     const float ml = m * kLog2e;
-    if (sizeof(T) == 2) more = 1.0 - (double)__builtin_fmaf(m, kLog2e, -ml) * 0.69314718055994531;
+    if (sizeof(T) == 2) {
+      const double d = (double)__builtin_fmaf(m, kLog2e, -ml) * 0.69314718055994531;
+      more = 1.0 - d * (1.0 - 0.5 * d);
+    }
 #pragma unroll
     for (int u = 0; u < U; u++)
 #pragma unroll

@@ -343,3 +343,13 @@ def test_logits_of_large_magnitude(half):
     c.logits[:4] = (r.uniform(-1, 1, (4, 700)) * top).astype(c.logits.dtype)
     c.logits[4:] = (top - r.integers(0, 3, (4, 700)) * (32 if half else 1e33)).astype(c.logits.dtype)
     c.check()
+
+
+@pytest.mark.parametrize("x", [49984.0, 58592.0, 63872.0, -63872.0])
+def test_large_fp16_maximum(x):
+    """Where the maximum times log2(e) is furthest from what 32 bits hold of
+    it."""
+    c = Case(np.random.default_rng(10), 1, 2, 1000, half=True, weights=False)
+    c.scores[:] = [0.0, -0.5]
+    c.logits[:] = x
+    c.check()
