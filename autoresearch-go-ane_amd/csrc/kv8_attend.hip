@@ -709,7 +709,7 @@ int plan(const char* op, const Kv8Batch& b, const ane_kv8_batch& given, int DH, 
   ns = std::min<int64_t>(ns, (len + p->round - 1) / p->round);
   ns = std::max<int64_t>(1, std::min<int64_t>(ns, kMaxSplit));
   p->nsplit = (int)ns;
-  if (blocks * ns > 0x7fffffff)
+  if (blocks * ns * 64 * p->kw > 0xffffffffll)  // threads (kw 1: a wave a tile)
     return op_fail(ANE_ERR_ARG, "storiesane %s: rows=%d nseq=%d are too many for one launch", op, b.rows, b.nseq);
   p->bytes = ns > 1 ? blocks * ns * p->tt * G * (DH + 2) * 4 : 0;
   return ANE_OK;

@@ -802,8 +802,11 @@ extern "C" int ane_kv8_copy(const ane_kv8_pool* from, const ane_kv8_pool* into, 
     // past the caches from what the L2s hold on: 3700 pages in 8 layers (490 MB)
     // 98 us, through them 105
     const bool far = (int64_t)g.n * 2 * n * (p.NKV << (p.pshift + p.dshift)) >= 32 << 20;
-    hipLaunchKernelGGL(far ? copy_kernel<true> : copy_kernel<false>, dim3(blocks_of(g.n, n, group)), dim3(256), 0, st, p,
-                       q.pages, x, y, n, group, g.src, g.dst, g.tokens);
+    const int most = (1 << 23) / blocks_of(1, n, group);  // pages of a launch, which has fewer than 2^32 threads
+    for (int i = 0; i < g.n; i += most)
+      hipLaunchKernelGGL(far ? copy_kernel<true> : copy_kernel<false>,
+                         dim3(blocks_of(std::min(most, g.n - i), n, group)), dim3(256), 0, st, p, q.pages, x, y, n,
+                         group, g.src + i, g.dst + i, g.tokens ? g.tokens + i : nullptr);
   }
   return launched(op);
 }

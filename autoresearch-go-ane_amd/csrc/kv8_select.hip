@@ -545,12 +545,29 @@ int check_bounds(const char* op, const ane_kv8_bounds* x) {
   return ANE_OK;
 }
 
-int check_sizes(const char* op, const Kv8Batch& b, int heads, int count) {
+// Rows of the queries' tile (16 or, of more heads, 32), tokens that it takes, and
+// the waves of a block: four, each a token's own, where a sequence may have
+// several tokens for them (11 chunks of up to 300 tokens 61 us a pass with the
+// update and the attention, with all waves at each token 64 to 69); eight that share
+// one where it has one (64 single tokens over 32,000 keys 31.4 us, with four
+// 32.0, with one of them choosing 33.5).
+struct Form {
+  int nt, tok, waves;
+};
+Form form_of(const ane_kv8_batch& batch, int G) {
+  const int most = batch.max_new ? batch.max_new : (batch.rows + batch.nseq - 1) / std::max(batch.nseq, 1);
+  Form f = {G <= 16 ? 1 : 2, G <= 4 ? 4 : G <= 8 ? 2 : 1, 8};
+  if (f.tok > 1 && most > 1) f.waves = 4;
+  return f;
+}
+
+int check_sizes(const char* op, const Kv8Batch& b, const ane_kv8_batch& batch, int heads, int count) {
   if (heads < 1 || heads % b.NKV || heads / b.NKV > kKvMaxGroup)
     return op_fail(ANE_ERR_ARG, "storiesane %s: heads=%d must be 1..%d times kv_heads=%d", op, heads, kKvMaxGroup,
                    b.NKV);
   if (count < 1 || count > 65536) return op_fail(ANE_ERR_ARG, "storiesane %s: count=%d want 1..65536", op, count);
-  if ((int64_t)kv8_count(b.nseq, b.rows, kv8_tiles(1)) * b.NKV > 0x7fffffff)
+  const Form f = form_of(batch, heads / b.NKV);
+  if ((int64_t)kv8_count(b.nseq, b.rows, kv8_tiles(f.tok)) * b.NKV * 64 * f.waves > 0xffffffffll)  // threads
     return op_fail(ANE_ERR_ARG, "storiesane %s: rows=%d are too many for one launch", op, b.rows);
   return ANE_OK;
 }
@@ -570,8 +587,9 @@ int launch_form(const char* op, SelectArgs a, int pages, hipStream_t st) {
 }
 
 template <int DH, int NT, int TOK>
-int launch_tokens(const char* op, const SelectArgs& a, int pages, int most, hipStream_t st) {
-  if (TOK > 1 && most > 1) return launch_form<DH, NT, TOK, 4, 1>(op, a, pages, st);
+int launch_tokens(const char* op, const SelectArgs& a, int pages, int waves, hipStream_t st) {
+  if constexpr (TOK > 1)
+    if (waves == 4) return launch_form<DH, NT, TOK, 4, 1>(op, a, pages, st);
   return launch_form<DH, NT, TOK, 8, 8>(op, a, pages, st);
 }
 
@@ -579,11 +597,11 @@ template <int DH>
 int launch(const char* op, const SelectArgs& a, const ane_kv8_batch& batch, hipStream_t st) {
   const int cap = a.b.table_pages << a.b.pshift;
   const int pages = (((batch.max_len ? std::min(batch.max_len, cap) : cap) - 1) >> a.b.pshift) + 1;
-  const int most = batch.max_new ? batch.max_new : (a.b.rows + a.b.nseq - 1) / a.b.nseq;
-  if (a.G <= 4) return launch_tokens<DH, 1, 4>(op, a, pages, most, st);
-  if (a.G <= 8) return launch_tokens<DH, 1, 2>(op, a, pages, most, st);
-  if (a.G <= 16) return launch_tokens<DH, 1, 1>(op, a, pages, most, st);
-  return launch_tokens<DH, 2, 1>(op, a, pages, most, st);
+  const Form f = form_of(batch, a.G);
+  if (f.nt == 2) return launch_tokens<DH, 2, 1>(op, a, pages, f.waves, st);
+  if (f.tok == 4) return launch_tokens<DH, 1, 4>(op, a, pages, f.waves, st);
+  if (f.tok == 2) return launch_tokens<DH, 1, 2>(op, a, pages, f.waves, st);
+  return launch_tokens<DH, 1, 1>(op, a, pages, f.waves, st);
 }
 
 }  // namespace
@@ -599,11 +617,13 @@ extern "C" int ane_kv8_bound(const ane_kv8_cache* cache, const ane_kv8_bounds* b
   int rc = kv8_check(op, cache, batch, &a.b);
   if (!rc) rc = check_bounds(op, bounds);
   if (rc || a.b.nseq == 0 || a.b.rows == 0) return rc;
+  const dim3 grid(kv8_count(a.b.nseq, a.b.rows, kv8_pages(1 << a.b.pshift)), a.b.NKV);
+  if (grid.x * 64ll > 0xffffffffll)  // threads
+    return op_fail(ANE_ERR_ARG, "storiesane %s: rows=%d are too many for one launch", op, a.b.rows);
   DeviceScope dev(cache->device);
   if (dev.status() != hipSuccess)
     return op_fail(ANE_ERR_HIP, "storiesane %s: device %d: %s", op, cache->device, hipGetErrorString(dev.status()));
   a.k = (const uint8_t*)cache->k; a.k_exp = cache->k_exp; a.box = bounds->box; a.unit = bounds->unit;
-  const dim3 grid(kv8_count(a.b.nseq, a.b.rows, kv8_pages(1 << a.b.pshift)), a.b.NKV);
   const hipStream_t st = (hipStream_t)stream;
   if (cache->head_dim == 64) hipLaunchKernelGGL(bound_kernel<64>, grid, dim3(64), 0, st, a);
   else hipLaunchKernelGGL(bound_kernel<128>, grid, dim3(64), 0, st, a);
@@ -617,7 +637,7 @@ extern "C" int64_t ane_kv8_select_workspace(const ane_kv8_cache* cache, const an
   const char* op = "kv8 select workspace";
   Kv8Batch b;
   int rc = kv8_check(op, cache, batch, &b);
-  if (!rc) rc = check_sizes(op, b, heads, count);
+  if (!rc) rc = check_sizes(op, b, *batch, heads, count);
   return rc ? rc : 0;
 }
 
@@ -630,7 +650,7 @@ extern "C" int ane_kv8_select(const ane_kv8_cache* cache, const ane_kv8_bounds* 
   if (rc) return rc;
   if (!args) return op_fail(ANE_ERR_ARG, "storiesane %s: null arguments", op);
   const ane_kv8_select_args& g = *args;
-  rc = check_sizes(op, a.b, g.heads, g.count);
+  rc = check_sizes(op, a.b, *batch, g.heads, g.count);
   if (rc) return rc;
   if (g.first < 0 || g.recent < 0 || (int64_t)g.first + g.recent > g.count)
     return op_fail(ANE_ERR_ARG, "storiesane %s: first=%d recent=%d want 0 or more, together at most count=%d", op,

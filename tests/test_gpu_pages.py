@@ -377,3 +377,16 @@ def test_copies_of_many_small_pages():
         a, b = Pool(r, n + 5, layers, kvh, P), Pool(r, n + 9, layers, kvh, P, bounds=True)
         copy_pages(a, b, r.permutation(n + 5)[:n], r.permutation(n + 9)[:n], r.integers(0, P + 1, n))
         copy_pages(a, b, r.permutation(n + 5)[:n], r.permutation(n + 9)[:n], None)
+
+
+def test_copies_of_more_pages_than_a_launch_takes():
+    r = np.random.default_rng(11)
+    a, b = Pool(r, 6, 32, 1), Pool(r, 5, 32, 1)
+    n = 1 << 22
+    src = np.full(n, -1)
+    at = [0, n // 2 - 1, n // 2, n - 1]
+    src[at] = [5, 2, 0, 3]
+    dst = np.full(n, 4)
+    dst[at] = [1, 3, 2, 0]
+    copy_pages(a, b, src, dst, None)
+    copy_pages(b, a, src, dst, r.integers(0, 17, n))
