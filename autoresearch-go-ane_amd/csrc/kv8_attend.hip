@@ -24,6 +24,13 @@
 // products, about 150 for 32 keys and 48 rows where the products are 24 MFMAs,
 // with the vector units 77 % busy (one of 8192 tokens, 12 heads of 64: 121 us,
 // 850 TFLOP/s).
+//
+// Lists of pages (ane_kv8_attend_blocks) go the same ways, their keys numbered in
+// the list's order.  Single tokens: the chain again, the list's loads before the
+// page table's (one row of 12 heads and 32 pages of 64 5.6 us; 64 rows of 16
+// heads of 128 and 48 pages of 32 12.4 us, 47 MB).  Chunks: the vector
+// instructions, so the tokens of a tile share what they name (5 chunks, 957 rows
+// of 12 heads, 24 pages of 64 each out of up to 190: 25 us, a tile a row 48).
 #include <algorithm>
 #include <type_traits>
 
@@ -69,6 +76,10 @@ struct ListArgs : AttendArgs {
   const int* blocks;  // [rows][NKV][count] places in the table
   int count;
 };
+// the same for tiles of several tokens, over the pages that any of them names
+struct UnionArgs : ListArgs {
+  int room;  // places that LDS has masks of
+};
 __device__ __forceinline__ const int* list_of(const ListArgs& a, int row, int h) {
   return a.blocks + ((size_t)row * a.b.NKV + h) * a.count;
 }
@@ -82,6 +93,81 @@ __device__ __forceinline__ int list_keys(const ListArgs& a, const int* list) {
     if (is) return (c + 64 - __clzll((long long)is)) << a.b.pshift;
     if (c == 0) return 1 << a.b.pshift;
   }
+}
+
+// The pages that the tokens of a tile name: their places, and which tokens name
+// each.  Rising places, each once; but where a token names one twice, or there
+// are more places than LDS has masks of, all lists one behind the other.  The
+// order does not depend on that of any atomics.
+struct Named {
+  int* place;      // [tt * count]
+  uint16_t* mask;  // [tt * count]
+};
+extern __shared__ uint32_t union_lds[];  // masks of all places in halves of words, then the two above
+__device__ __forceinline__ Named named_of(const UnionArgs& a) {
+  int* place = reinterpret_cast<int*>(union_lds + (a.room + 1) / 2);
+  return {place, reinterpret_cast<uint16_t*>(place + a.tt * a.count)};
+}
+template <int KW>
+__device__ __forceinline__ int name_pages(const UnionArgs& a, const Kv8Span& span, int h, Named out) {
+  __shared__ int twice, counts[KW];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // places behind the tile's last token have no key for it
+  const int np = min(((span.pos + span.n - 1) >> a.b.pshift) + 1, a.b.table_pages), all = span.n * a.count;
+  const auto place_of = [&](int e, int tok) {
+    const int at = list_of(a, span.row + tok, h)[e - tok * a.count];
+    return (unsigned)at < (unsigned)np ? at : -1;
+  };
+  bool apart = np > a.room;
+  if (!apart) {
+    for (int i = tid; i < (np + 1) / 2; i += 64 * KW) union_lds[i] = 0;
+    if (tid == 0) twice = 0;
+    __syncthreads();
+    for (int e = tid; e < all; e += 64 * KW) {
+      const int tok = e / a.count, at = place_of(e, tok);
+      if (at >= 0) {
+        const uint32_t bit = 1u << (tok + 16 * (at & 1));
+        if (atomicOr(union_lds + (at >> 1), bit) & bit) twice = 1;
+      }
+    }
+    __syncthreads();
+    apart = twice;
+  }
+  if (apart) {
+    for (int e = tid; e < all; e += 64 * KW) {
+      const int tok = e / a.count;
+      out.place[e] = place_of(e, tok);
+      out.mask[e] = (uint16_t)(1 << tok);
+    }
+    __syncthreads();
+    return all;
+  }
+  // a wave a run of places
+  const int run = (np + 64 * KW - 1) / (64 * KW) * 64, p0 = wave * run, p1 = min(p0 + run, np);
+  const auto mask_of = [&](int p) { return p < p1 ? union_lds[p >> 1] >> (16 * (p & 1)) & 0xffff : 0u; };
+  int n = 0;
+  for (int p = p0; p < p1; p += 64) n += __popcll(__ballot(mask_of(p + lane) != 0));
+  if (lane == 0) counts[wave] = n;
+  __syncthreads();
+  int at = 0;
+  n = 0;
+#pragma unroll
+  for (int w = 0; w < KW; w++) {
+    at += w < wave ? counts[w] : 0;
+    n += counts[w];
+  }
+  for (int p = p0; p < p1; p += 64) {
+    const uint32_t mask = mask_of(p + lane);
+    const uint64_t is = __ballot(mask != 0);
+    if (mask) {
+      const int i = at + __popcll(is & ((1ull << lane) - 1));
+      out.place[i] = p + lane;
+      out.mask[i] = (uint16_t)mask;
+    }
+    at += __popcll(is);
+  }
+  __syncthreads();
+  return n;
 }
 
 // where dimension d of a row's query head goes
@@ -125,11 +211,12 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
 // A page that is not there reads the pool's first, which exists but may hold
 // anything; its scores are masked, its values cleared, and its exponents 0 (a
 // scale made of a stray one, -128, is NaN and makes NaN of cleared values too).
-// pos: of a list's pages, where the unit's tokens stand in the sequence.
+// pos: of a list's pages, where the unit's tokens stand in the sequence; by:
+// which of the tile's tokens name the page.
 template <int DH>
 struct Step {
   u32x4 k[NU][DH / 64], v[NU][DH / 64];
-  int ex[NU], pos[NU];
+  int ex[NU], pos[NU], by[NU];
 };
 constexpr int kThere = 1 << 16;
 __device__ __forceinline__ float k_scale(int ex) { return kv8_scale((int8_t)(ex & 0xff)); }
@@ -145,11 +232,12 @@ constexpr int waves_per_simd(int DH, int NT) {
 // each other); ONE: a step's keys are of one page (pages of at least kStep
 // tokens).  Args is StepArgs: the sequences have a token each, and the block
 // first appends its key and value and rotates its queries.  ListArgs: the keys
-// are those of a list of pages, numbered in its order.
+// are those of a list of pages, numbered in its order.  UnionArgs: and each page
+// is for some of the tile's tokens.
 template <int DH, int NT, int KW, int RW, bool ONE, typename Args>
 __global__ __launch_bounds__(64 * KW * RW, waves_per_simd(DH, NT)) void attend_kernel(Args a) {
   constexpr bool STEP = std::is_same_v<Args, StepArgs>;
-  constexpr bool LIST = std::is_same_v<Args, ListArgs>;
+  constexpr bool UNION = std::is_same_v<Args, UnionArgs>, LIST = UNION || std::is_same_v<Args, ListArgs>;
   static_assert(!STEP || (NT == 1 && KW == 4));
   static_assert(KW == 1 || RW == 1, "the waves of a block meet over one tile");
   constexpr int R = 16 * NT;    // rows of the tile
@@ -176,9 +264,17 @@ __global__ __launch_bounds__(64 * KW * RW, waves_per_simd(DH, NT)) void attend_k
   if (span.n == 0) return;
   const int rows = span.n * a.G;
   const int* list = nullptr;
-  if constexpr (LIST) list = list_of(a, span.row, h);
+  Named named = {};
+  int npages = 0;
   int kend = span.pos + span.n;  // keys of the tile's last token
-  if constexpr (LIST) kend = list_keys(a, list);
+  if constexpr (UNION) {
+    named = named_of(a);
+    npages = name_pages<KW>(a, span, h, named);
+    kend = max(npages, 1) << b.pshift;
+  } else if constexpr (LIST) {
+    list = list_of(a, span.row, h);
+    kend = list_keys(a, list);
+  }
   const int pk = part_keys(a, kend);
   const int k0 = sp * pk;
   if (k0 >= kend) return;
@@ -203,7 +299,7 @@ __global__ __launch_bounds__(64 * KW * RW, waves_per_simd(DH, NT)) void attend_k
   // 64 pages from wbase on, one per lane: where the head's rows begin, and
   // what Step says of the page.  wend: the first position behind them.
   const int* trow = b.table + (size_t)span.seq * b.table_stride;
-  int wbase = 0, wexp = 0, wpos = 0;
+  int wbase = 0, wexp = 0, wpos = 0, wby = 0;
   int wend = 0;
   uint32_t wlo = 0, whi = 0;
   auto window = [&](int pg) {
@@ -213,7 +309,13 @@ __global__ __launch_bounds__(64 * KW * RW, waves_per_simd(DH, NT)) void attend_k
     int id = -1;
     if constexpr (LIST) {
       if (p << b.pshift < k1) {  // and so within the list
-        const int place = list[p];
+        int place;
+        if constexpr (UNION) {
+          place = npages ? named.place[p] : -1;
+          wby = npages ? named.mask[p] : 0;
+        } else {
+          place = list[p];
+        }
         if ((unsigned)place < (unsigned)b.table_pages) {
           id = trow[place];
           wpos = place << b.pshift;
@@ -247,10 +349,12 @@ __global__ __launch_bounds__(64 * KW * RW, waves_per_simd(DH, NT)) void attend_k
         s.ex[u] = __builtin_amdgcn_readlane(wexp, w);
         at += (ku & ((1 << b.pshift) - 1)) * DH;
         if (LIST) s.pos[u] = __builtin_amdgcn_readlane(wpos, w) + (ku & ((1 << b.pshift) - 1));
+        if (UNION) s.by[u] = __builtin_amdgcn_readlane(wby, w);
       } else {
         s.ex[u] = s.ex[0];
         at += 16 * DH;
         if (LIST) s.pos[u] = s.pos[0] + 16;
+        if (UNION) s.by[u] = s.by[0];
       }
       const uint8_t *kp = a.k + at, *vp = a.v + at;
 #pragma unroll
@@ -264,11 +368,13 @@ __global__ __launch_bounds__(64 * KW * RW, waves_per_simd(DH, NT)) void attend_k
   // Q: row r = 16 t + col, dimensions 64 (m / 2) + 16 g + 8 (m % 2) + j
   half8 q[NT][NM];
   int lim[NT];  // the last key of the lane's row
+  int me[NT];   // its token's bit
 #pragma unroll
   for (int t = 0; t < NT; t++) {
     const int r = min(16 * t + col, rows - 1);
     const int tok = r / a.G, hg = r - tok * a.G;
     lim[t] = span.pos + tok;
+    me[t] = 1 << tok;
     const half_t* p = a.q + (span.row + tok) * a.q_row + (h * a.G + hg) * a.q_head + 16 * g;
 #pragma unroll
     for (int m = 0; m < NM; m++)
@@ -328,8 +434,9 @@ __global__ __launch_bounds__(64 * KW * RW, waves_per_simd(DH, NT)) void attend_k
   for (int j = 0; j < 8; j++) ones[j] = (half_t)1.f;
   asm volatile("" : "+v"(ones));  // in vector registers: scalar ones are spilled and read back in every step
   uint32_t nan = 0;
+  int careful = 0;
   auto step = [&](Step<DH>& s, int kb) {
-    const int edge = at_edge(s, kb);
+    const int edge = at_edge(s, kb) | careful;
     floatx4 sc[NU][NT];
 #pragma unroll
     for (int u = 0; u < NU; u++) {
@@ -356,6 +463,16 @@ __global__ __launch_bounds__(64 * KW * RW, waves_per_simd(DH, NT)) void attend_k
 #pragma unroll
           for (int j = 0; j < 4; j++)
             if (!(s.ex[u] & kThere) || unit_pos(s, kb, u) + 4 * g + j > lim[t]) sc[u][t][j] = -INFINITY;
+    }
+    if constexpr (UNION) {
+#pragma unroll
+      for (int u = 0; u < NU; u++)
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+          const bool is = s.by[u] & me[t];
+#pragma unroll
+          for (int j = 0; j < 4; j++) sc[u][t][j] = is ? sc[u][t][j] : -INFINITY;
+        }
     }
     float mx[NT];
     bool up = false;
@@ -412,7 +529,7 @@ __global__ __launch_bounds__(64 * KW * RW, waves_per_simd(DH, NT)) void attend_k
 #pragma unroll
       for (int u = 0; u < NU; u++) {
         const int first = unit_pos(s, kb, u) + 4 * g;  // the lane's four keys
-        const int n = s.ex[u] & kThere ? clampi((LIST ? span.pos + 1 : k1) - first, 0, 4) : 0;
+        const int n = s.ex[u] & kThere ? clampi((LIST ? span.pos + span.n : k1) - first, 0, 4) : 0;
         const uint32_t mine = n == 4 ? 0xffffffffu : (1u << (8 * n)) - 1;
 #pragma unroll
         for (int x = 0; x < DH / 64; x++)
@@ -447,10 +564,37 @@ __global__ __launch_bounds__(64 * KW * RW, waves_per_simd(DH, NT)) void attend_k
     kb = kn;
     return kn < k1;
   };
-  if (kb < k1) {
-    Step<DH> nxt;
-    while (turn(cur, nxt) && turn(nxt, cur)) {
+  for (;;) {
+    if (kb < k1) {
+      Step<DH> nxt;
+      while (turn(cur, nxt) && turn(nxt, cur)) {
+      }
     }
+    if constexpr (!UNION) break;
+    // NaN among values that some row's page holds and another's does not: rare,
+    // and all over again, with them taken out in every step
+    if (careful) break;
+    float sum = 0.f;
+#pragma unroll
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+      for (int d = 0; d < ND; d++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) sum = __builtin_fmaf(o[d][t][j], 0.f, sum);
+    if (!__any(sum != sum)) break;
+    careful = 1;
+    nan = 0;
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+      m[t] = 0.f;
+      bar[t] = -INFINITY;
+      l[t] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int d = 0; d < ND; d++) o[d][t] = floatx4{0.f, 0.f, 0.f, 0.f};
+    }
+    wend = 0;
+    kb = k0 + wave * kStep;
+    fetch(cur, kb, kb < k1);
   }
   if (__any(nan != 0)) {
     // rare: how many NaN of each dimension a row attends to, as a product of
@@ -458,7 +602,7 @@ __global__ __launch_bounds__(64 * KW * RW, waves_per_simd(DH, NT)) void attend_k
     wend = 0;
     for (kb = k0 + wave * kStep; kb < k1; kb += kStep * KW) {
       fetch(cur, kb, true);
-      if (!at_edge(cur, kb)) continue;
+      if (!at_edge(cur, kb) && !careful) continue;
 #pragma unroll
       for (int y = 0; y < NU / 2; y++) {
         half8 sees[NT];
@@ -467,7 +611,10 @@ __global__ __launch_bounds__(64 * KW * RW, waves_per_simd(DH, NT)) void attend_k
 #pragma unroll
           for (int j = 0; j < 8; j++) {
             const int u = 2 * y + (j >> 2);
-            sees[t][j] = (cur.ex[u] & kThere) && unit_pos(cur, kb, u) + 4 * g + (j & 3) <= lim[t] ? (half_t)1.f : (half_t)0.f;
+            sees[t][j] = (cur.ex[u] & kThere) && unit_pos(cur, kb, u) + 4 * g + (j & 3) <= lim[t] &&
+                                 (!UNION || (cur.by[u] & me[t]))
+                             ? (half_t)1.f
+                             : (half_t)0.f;
           }
 #pragma unroll
         for (int d = 0; d < ND; d++) {
@@ -623,6 +770,7 @@ struct Plan {
   int nt = 0, tt = 0, nsplit = 0, kw = 4, round = 0, longest = 0;
   uint32_t tiles = 0;
   int64_t bytes = 0;
+  int room = 0;  // of UnionArgs
 };
 
 // count: pages of a row's list (0: the whole context)
@@ -653,6 +801,21 @@ int plan(const char* op, const Kv8Batch& b, const ane_kv8_batch& given, int DH, 
   if (count) {  // a row is a tile
     p->nt = G <= 16 ? 1 : 2;
     p->tt = 1;
+    // Chunks: tiles of several tokens (UnionArgs), which read and convert a page
+    // once for all that name it.  They cost the joining of the lists, 3 us, and
+    // blocks, so where there is enough to do (update, choice and attention, pages
+    // named at random out of 125: 5 x 300 rows of 4 heads and 1536 keys 59 us, a
+    // row a tile 100; 2 x 100 rows 22.9 and 27.2; 2 x 50 23.1 and 21.7; 4 x 200
+    // of 256 keys 34 and 40, 4 x 50 24 and 20; head dimension 128, 4 x 100 of 2
+    // heads 31 and 47, 4 x 30 30 and 24), and for up to 4 heads a token (of 8, two
+    // tokens a tile: 2 x 100 rows 38 and 36).
+    const int pages = ((given.max_len ? std::min(given.max_len, cap) : cap) + (1 << b.pshift) - 1) >> b.pshift;
+    const int most = given.max_new ? given.max_new : (b.rows + b.nseq - 1) / b.nseq;
+    const int64_t lists = (int64_t)b.rows * b.NKV;
+    if (G <= 4 && most > 1 && pages <= 8192 && 16 / G * count <= 2048 && lists >= 640 && lists * len * DH >= 48 << 20) {
+      p->tt = 16 / G;
+      p->room = pages;
+    }
   }
   p->tiles = kv8_count(b.nseq, b.rows, kv8_tiles(p->tt));
   const int64_t blocks = (int64_t)p->tiles * b.NKV;
@@ -669,7 +832,10 @@ int plan(const char* op, const Kv8Batch& b, const ane_kv8_batch& given, int DH, 
   // 18.1; of 2048 19.3, in parts 19.5; 64 blocks of 2048 20.3 and 21.4, 128 22.8
   // and 23.9; but 256 28.1 and 27.1, 4 of 4096 23.0 and 20.1, and at head
   // dimension 128 26.4 and 22.0).
-  const bool eight = count && p->nt == 1 && DH == 64 && blocks <= 128 && len <= 2048;
+  // Tiles of several tokens up to 320: eight (5 x 100 rows, 400 tiles 32.0 us,
+  // with four 32.0; 3 x 100, 240 tiles 24.5 and 26.9; head dimension 128, 140
+  // tiles 29.7 and 29.1).
+  const bool eight = count && DH == 64 && p->nt == 1 && (p->room ? blocks <= 320 : blocks <= 128 && len <= 2048);
   if (eight) p->kw = 8;
   p->round = p->kw * kStep;
   // The longest contexts first, so that the last blocks to end are short ones:
@@ -697,7 +863,7 @@ int plan(const char* op, const Kv8Batch& b, const ane_kv8_batch& given, int DH, 
   // outlast the rest (64 of 8 heads and up to 30,000 keys 206 us, whole 232;
   // 80 blocks of up to 40,000 108 us, of 4096 keys 113).
   int64_t ns = 1;
-  if (eight) {
+  if (eight || p->room) {
     ns = 1;
   } else if (p->nt == 1) {
     if (len > (blocks >= 128 ? std::min<int64_t>(32 * blocks, 8192) : DH == 64 ? 1280 : 768))
@@ -723,12 +889,12 @@ int check_count(const char* op, int count) {
 }
 
 template <int DH, int NT, int KW, int RW, typename Args>
-void launch_form(const Args& a, hipStream_t st) {
+void launch_form(const Args& a, hipStream_t st, int lds = 0) {
   const dim3 grid(((uint32_t)a.tiles + RW - 1) / RW * a.b.NKV * a.nsplit), block(64 * KW * RW);
   if (kStep <= 1 << a.b.pshift)
-    hipLaunchKernelGGL((attend_kernel<DH, NT, KW, RW, true, Args>), grid, block, 0, st, a);
+    hipLaunchKernelGGL((attend_kernel<DH, NT, KW, RW, true, Args>), grid, block, lds, st, a);
   else
-    hipLaunchKernelGGL((attend_kernel<DH, NT, KW, RW, false, Args>), grid, block, 0, st, a);
+    hipLaunchKernelGGL((attend_kernel<DH, NT, KW, RW, false, Args>), grid, block, lds, st, a);
 }
 
 template <int DH>
@@ -746,12 +912,15 @@ void launch(const AttendArgs& a, const Plan& p, hipStream_t st) {
 }
 
 template <int DH>
-void launch_list(const ListArgs& a, const Plan& p, hipStream_t st) {
-  if constexpr (DH == 64) {
-    if (p.kw == 8) launch_form<DH, 1, 8, 1>(a, st);
+void launch_list(const UnionArgs& a, const Plan& p, hipStream_t st) {
+  const int lds = (a.room + 1) / 2 * 4 + a.tt * a.count * 6;
+  if constexpr (DH == 64) {  // which alone has eight waves
+    if (p.kw == 8 && p.room) return launch_form<DH, 1, 8, 1>(a, st, lds);
+    if (p.kw == 8) launch_form<DH, 1, 8, 1, ListArgs>(a, st);
   }
-  if (p.kw == 4 && p.nt == 1) launch_form<DH, 1, 4, 1>(a, st);
-  else if (p.kw == 4) launch_form<DH, 2, 4, 1>(a, st);
+  if (p.room) return launch_form<DH, 1, 4, 1>(a, st, lds);
+  if (p.kw == 4 && p.nt == 1) launch_form<DH, 1, 4, 1, ListArgs>(a, st);
+  else if (p.kw == 4) launch_form<DH, 2, 4, 1, ListArgs>(a, st);
   if (a.nsplit > 1)
     hipLaunchKernelGGL((join_kernel<DH, ListArgs>), dim3((uint32_t)a.tiles * a.b.NKV, (a.G + 3) / 4), dim3(256), 0, st,
                        a);
@@ -857,10 +1026,11 @@ int attend(const ane_kv8_cache* cache, const ane_kv8_batch* batch, const ane_kv8
     step.in = *in;
     launch_form<64, 1, 4, 1>(step, (hipStream_t)stream);
   } else if (list) {
-    ListArgs l;
+    UnionArgs l;
     static_cast<AttendArgs&>(l) = a;
     l.blocks = list->blocks;
     l.count = list->count;
+    l.room = p.room;
     if (cache->head_dim == 64) launch_list<64>(l, p, (hipStream_t)stream);
     else launch_list<128>(l, p, (hipStream_t)stream);
   } else if (cache->head_dim == 64) launch<64>(a, p, (hipStream_t)stream);

@@ -548,8 +548,8 @@ int check_bounds(const char* op, const ane_kv8_bounds* x) {
 // Rows of the queries' tile (16 or, of more heads, 32), tokens that it takes, and
 // the waves of a block: four, each a token's own, where a sequence may have
 // several tokens for them (11 chunks of up to 300 tokens 61 us a pass with the
-// update and the attention, with all waves at each token 64 to 69); eight that share
-// one where it has one (64 single tokens over 32,000 keys 31.4 us, with four
+// update and the attention, with all waves at each token 64 to 69); eight that
+// share one where it has one (64 single tokens over 32,000 keys 31.4 us, with four
 // 32.0, with one of them choosing 33.5).
 struct Form {
   int nt, tok, waves;

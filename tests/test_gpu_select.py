@@ -411,3 +411,94 @@ def test_two_streams_at_once():
         w = x.bounds.Select(x.batch, q, 40)
         y = x.pool.cache.Attend(x.batch, q, blocks=w)
         assert torch.equal(b[:n], w[:n]) and torch.equal(o[:n], y[:n])
+
+
+def lists(r, x, count, twice=False, none=0.1):
+    """`count` places a row and head, rising, some behind the position, some no
+    place at all."""
+    b = np.empty((x.rows, x.kvh, count), np.int32)
+    width = x.table.shape[1]
+    for i in range(x.rows):
+        for h in range(x.kvh):
+            b[i, h] = np.sort(r.choice(width, count, replace=twice or count > width))
+    b[r.random(b.shape) < none] = -1
+    return b
+
+
+@pytest.mark.parametrize("heads, kvh, dh, P, count, lens", [
+    (8, 8, 64, 128, 8, [(128 * 20, 70), (5, 31)]),               # 16 tokens a tile, the last ones of few
+    (16, 8, 64, 16, 64, [(16 * 70 + 3, 50), (0, 1), (900, 52)]),
+    (24, 8, 128, 32, 16, [(32 * 40, 97)]),
+    (32, 8, 64, 256, 4, [(256 * 9 + 200, 61), (1, 40)]),
+    (16, 4, 64, 64, 20, [(2000, 161), (2100, 3), (77, 170)]),    # four waves a tile
+    (9, 3, 128, 16, 50, [(3000, 220)]),
+])
+def test_chunks_whose_tokens_share_pages(heads, kvh, dh, P, count, lens):
+    r = np.random.default_rng(heads + P)
+    x = Run(r, lens, heads, kvh, dh, P).go()
+    b = lists(r, x, count)
+    b[x.rows // 2] = -1                   # a row that names nothing
+    b[:20, 1] = -1                        # tiles that name nothing
+    x.attend(b)
+
+
+def test_chunks_that_name_pages_twice_or_further_than_the_hint():
+    r = np.random.default_rng(23)
+    lens = [(128 * 18 + 5, 60), (9, 45)]
+    x = Run(r, lens, 16, 8, 64, 128).go()
+    b = lists(r, x, 8)
+    b[0, 0, :2], b[70, 5, 3:] = 4, 0      # twice in some tiles
+    x.attend(b)
+    x.attend(r.permuted(lists(r, x, 8, twice=True), axis=2))
+    y = Run(r, lens, 16, 8, 64, 128, max_len=300, max_new=7).go()
+    y.attend(lists(r, y, 8))
+
+
+@pytest.mark.parametrize("dh, heads", [(64, 24), (128, 8)])
+def test_chunks_with_nan_in_pages_of_others(dh, heads):
+    r = np.random.default_rng(24)
+    x = Run(r, [(128 * 20 + 7, 90)], heads, 8, dh, 128, nan=2e-6).go()
+    x.attend(lists(r, x, 8))
+    x = Run(r, [(128 * 20 + 7, 90)], heads, 8, dh, 128, nan=1e-3).go()
+    x.attend(lists(r, x, 8))
+
+
+def test_chunks_captured_and_in_place():
+    """Lists, starts and queries change between replays."""
+    r = np.random.default_rng(25)
+    x = Run(r, [(128 * 20, 70), (128 * 12, 40)], 16, 8, 64, 128).go()
+    q, b = dev(x.q), dev(lists(r, x, 8))
+    work = torch.empty_like(q)
+
+    def step():
+        work.copy_(q)
+        x.pool.cache.Attend(x.batch, work, work, blocks=b)
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        step()
+        stream.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            step()
+    start = x.batch._keep[1]
+    for i in range(4):
+        q.copy_(dev(r.standard_normal(x.q.shape).astype(np.float16)))
+        b.copy_(dev(lists(r, x, 8, twice=i == 2)))
+        start.copy_(dev(np.array([128 * (20 - 3 * i) + i, 128 * 12 - 50 * i], np.int32)))
+        torch.cuda.synchronize()
+        work.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = work.clone()
+        out = torch.zeros_like(q)
+        x.pool.cache.Attend(x.batch, q, out, blocks=b)
+        torch.cuda.synchronize()
+        assert torch.equal(got[:110], out[:110])
+        assert torch.equal(got[110:], q[110:])
+
+
+def test_chunks_with_as_many_places_and_lists_as_lds_holds():
+    r = np.random.default_rng(26)
+    x = Run(r, [(16 * 8130 + 3, 640)], 1, 1, 64, 16, spare=0).go()
+    assert 8160 < x.table.shape[1] <= 8192
+    x.attend(lists(r, x, 128, none=0.01))
