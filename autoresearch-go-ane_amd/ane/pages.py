@@ -71,9 +71,11 @@ class KVBounds:
             _fail(op, f"count={count} first={first} recent={recent}")
         if blocks is None:
             blocks = self._empty((batch.rows, c.kv_heads, count), dtype=self._i32, device=c.device)
-        bp, n = c._blocks(op, blocks, batch)
-        if n != count:
-            _fail(op, f"blocks has shape {tuple(blocks.shape)}, want ({batch.rows}, {c.kv_heads}, {count})")
+            bp = blocks.data_ptr()
+        else:
+            bp, n = c._blocks(op, blocks, batch)
+            if n != count:
+                _fail(op, f"blocks has shape {tuple(blocks.shape)}, want ({batch.rows}, {c.kv_heads}, {count})")
         key = ("select", c.kv_heads, c.page_tokens, c.head_dim, heads, count)
         n = batch._ws.get(key)
         if n is None:
@@ -182,7 +184,9 @@ class KVPages:
                 _fail(op, f"new={new}")
         if missing is None:
             missing = self._empty(1, dtype=self._i32[0], device=self.device)
-        mp = self._vector(op, "missing", missing, 1)
+            mp = missing.data_ptr()
+        else:
+            mp = self._vector(op, "missing", missing, 1)
         n = self._bytes.get((nseq, width))
         if n is None:
             n = self._bytes[nseq, width] = _check(self._lib, self._lib.ane_kv8_fork_workspace(self._c, nseq, width))
@@ -204,7 +208,9 @@ class KVPages:
             tp, stride, width, nseq = self._table(op, table)
         if moved is None:
             moved = self._empty(self.pages, dtype=self._i32[0], device=self.device)
-        mp = self._vector(op, "moved", moved, self.pages)
+            mp = moved.data_ptr()
+        else:
+            mp = self._vector(op, "moved", moved, self.pages)
         n = self._compact_bytes
         ws = self._empty(n, dtype=self._u8, device=self.device)
         a = _lib.pack_compact(tp, mp, stride, width, nseq, ws.data_ptr(), n)

@@ -442,9 +442,13 @@ class BeamSearch:
         if (history is None) != (lengths is None):
             _fail(op, "history without lengths" if lengths is None else "lengths without a history")
         new, dev, vector = self._empty, logits.device, self._vector
-        tokens = new(rows, dtype=self._i32[0], device=dev) if tokens is None else tokens
-        parents = new(rows, dtype=self._i32[0], device=dev) if parents is None else parents
-        scores_out = new(rows, dtype=self._f32[0], device=dev) if scores_out is None else scores_out
+        given = tokens, parents, scores_out
+        if tokens is None:
+            tokens = new(rows, dtype=self._i32[0], device=dev)
+        if parents is None:
+            parents = new(rows, dtype=self._i32[0], device=dev)
+        if scores_out is None:
+            scores_out = new(rows, dtype=self._f32[0], device=dev)
         sp = vector("scores", scores, self._f32, index, rows)
         wp = 0 if weights is None else vector("weights", weights, self._f32, index, rows)
         fp = fo = hp = hr = most = np_ = 0
@@ -458,9 +462,9 @@ class BeamSearch:
             if hn != rows:
                 _fail(op, f"history has {hn} rows, want {rows}")
             np_ = vector("lengths", lengths, self._i32, index, rows)
-        tp = vector("tokens", tokens, self._i32, index, rows)
-        pp = vector("parents", parents, self._i32, index, rows)
-        so = vector("scores_out", scores_out, self._f32, index, rows)
+        tp = tokens.data_ptr() if given[0] is None else vector("tokens", tokens, self._i32, index, rows)
+        pp = parents.data_ptr() if given[1] is None else vector("parents", parents, self._i32, index, rows)
+        so = scores_out.data_ptr() if given[2] is None else vector("scores_out", scores_out, self._f32, index, rows)
         n = self._bytes.get((rows, half))
         if n is None:
             n = self._bytes[rows, half] = _check(

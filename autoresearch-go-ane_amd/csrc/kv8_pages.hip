@@ -6,6 +6,12 @@
 // blocks run: reference counts change by atomic additions, and the pages that
 // are handed out are ranked (by sequence and position), as are the free ones
 // (by id).
+//
+// What bounds it.  Copies: HBM, once pages fill it (compacting, 558 MB read and
+// written, 106 us, 5.3 TB/s; 3700 pages in 8 layers, 490 MB, 98 us, 5.0 TB/s).
+// Tables: chains of dependent accesses, and launches (a fork of 4 sequences 5.1 us
+// for the table and 3.5 for its copies; of 384 sequences of up to 8000 tokens 3.7
+// for the rows, 5.0 for the plan and 8.5 for the table and 63 MB of copies).
 #include <algorithm>
 
 #include "kv8.h"
@@ -117,6 +123,14 @@ __device__ __forceinline__ void copy_sides(const Pool& p, const Layers& x, const
     }
   }
 }
+// Copies of so many bytes go past the caches, which hold twice that no more
+// (compacting, 372 MB read and written 75 us either way, 466 MB 94 past them and
+// 101 through them, 279 MB 58 and 49).
+constexpr int64_t kFar = 180 << 20;
+__host__ __device__ __forceinline__ int64_t bytes_of(const Pool& p, int nlayers) {
+  return (int64_t)2 * nlayers * (p.NKV << (p.pshift + p.dshift));
+}
+
 // The sides of an item (a page's copy in all layers of a launch) that a block
 // takes, `group` at a time.
 struct Sides {
@@ -156,8 +170,9 @@ struct ForkArgs {
 };
 
 // One block does the tables by itself where they are small: their entries are
-// in LDS.
-constexpr int kSmall = 8192;
+// in LDS (8 rows of 31 a fork 7.8 us, with launches for the rows and the table
+// 9.9; 32 of 59 9.1 and 9.8; but 64 of 59 11.9 and 10.8).
+constexpr int kSmall = 2048;
 bool small_table(int64_t nseq, int64_t width) { return nseq <= kTh && nseq * width <= kSmall; }
 
 __device__ __forceinline__ int there(int id, int pages) { return (unsigned)id < (unsigned)pages ? id : -1; }
@@ -311,7 +326,9 @@ __device__ __forceinline__ int find_free(const ForkArgs& a, int want, int (&sums
 }
 
 // One block: who copies, how many pages each sequence gets, and which are free.
-// SMALL: also the rows before that, and the table behind it.
+// A block ranks all of them without another launch (384 sequences in 5.0 us,
+// most of it waits for loads and atomics).  SMALL: also the rows before that, and
+// the table behind it, in one launch in place of two.
 template <bool SMALL>
 __global__ __launch_bounds__(kTh) void plan_kernel(ForkArgs a) {
   __shared__ int sums[kTh / 64];
@@ -541,9 +558,14 @@ __global__ __launch_bounds__(256) void move_kernel(CompactArgs a, Layers x, int 
     return;
   }
   const Sides s = sides_of(blockIdx.x - book_blocks, nlayers, group);
-  const int total = *a.total;
-  for (int k = s.item; k < total; k += items)
-    copy_sides<256, true>(a.p, x, x, s.first, s.count, a.movers[k], a.holes[k], 1 << (a.p.pshift - 4));
+  const int total = *a.total, units = 1 << (a.p.pshift - 4);
+  if (total * bytes_of(a.p, nlayers) >= kFar) {
+    for (int k = s.item; k < total; k += items)
+      copy_sides<256, true>(a.p, x, x, s.first, s.count, a.movers[k], a.holes[k], units);
+  } else {
+    for (int k = s.item; k < total; k += items)
+      copy_sides<256, false>(a.p, x, x, s.first, s.count, a.movers[k], a.holes[k], units);
+  }
 }
 
 // ---- copy ----------------------------------------------------------------------
@@ -596,7 +618,9 @@ int layers_of(const ane_kv8_pool& pool, int l0, Layers* x) {
 }
 
 // Sides a block copies: one where there are few, and of small pages as many as
-// make 16 KB, which is what a block's threads load at a time.
+// make 16 KB, which is what a block's threads load at a time (pages of 1 KB a side
+// 30 us, one a block 66; of 4 KB 98 and 101; 64 KB for pages of 16 KB 126 and
+// 112).
 int group_of(const Pool& p, int64_t items, int nlayers) {
   const int side = p.NKV << (p.pshift + p.dshift);  // bytes
   int g = std::max(1, std::min(2 * nlayers, 16384 / side));
@@ -799,9 +823,7 @@ extern "C" int ane_kv8_copy(const ane_kv8_pool* from, const ane_kv8_pool* into, 
     const int n = layers_of(*from, l0, &x);
     layers_of(*into, l0, &y);
     const int group = group_of(p, g.n, n);
-    // past the caches from what the L2s hold on: 3700 pages in 8 layers (490 MB)
-    // 98 us, through them 105
-    const bool far = (int64_t)g.n * 2 * n * (p.NKV << (p.pshift + p.dshift)) >= 32 << 20;
+    const bool far = g.n * bytes_of(p, n) >= kFar;
     const int most = (1 << 23) / blocks_of(1, n, group);  // pages of a launch, which has fewer than 2^32 threads
     for (int i = 0; i < g.n; i += most)
       hipLaunchKernelGGL(far ? copy_kernel<true> : copy_kernel<false>,
