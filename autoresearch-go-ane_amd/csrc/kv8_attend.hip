@@ -260,7 +260,7 @@ __global__ __launch_bounds__(64 * KW * RW, waves_per_simd(DH, NT)) void attend_k
   // the longest rows of a prompt first
   const int tile = a.tiles - 1 - rest / a.nsplit * RW - (RW > 1 ? __builtin_amdgcn_readfirstlane(tid >> 6) : 0);
   if (RW > 1 && tile < 0) return;
-  const Kv8Span span = NT > 1 && KW > 1 ? tile_span(a, tile) : kv8_tile_span(b, a.tt, tile);
+  const Kv8Span span = UNION || (NT > 1 && KW > 1) ? tile_span(a, tile) : kv8_tile_span(b, a.tt, tile);
   if (span.n == 0) return;
   const int rows = span.n * a.G;
   const int* list = nullptr;
@@ -843,8 +843,10 @@ int plan(const char* op, const Kv8Batch& b, const ane_kv8_batch& given, int DH, 
   // 8000, three draws: 73, 101, 57 us against 100, 105, 60; 32 of 10 to 128 on
   // up to 4000 33 against 38).  Finding them costs each block 1.2 us at 64
   // sequences (64 of 16 to 100, head dimension 128: 138 against 129), so up to
-  // 32, and not where a CU has no second block.
-  p->longest = p->nt > 1 && p->kw == 4 && !count && b.nseq > 1 && b.nseq <= 32 && blocks > 256;
+  // 32, and not where a CU has no second block.  Tiles over lists likewise (update,
+  // choice and attention, 5 chunks of 50 to 333 on up to 12,000 38.7 us, in the
+  // batch's order 41.5; 6 on up to 30,000 54 and 56, of 10 to 200 44.0 and 43.9).
+  p->longest = (count ? p->room > 0 : p->nt > 1 && p->kw == 4) && b.nseq > 1 && b.nseq <= 32 && blocks > 256;
   // Parts of the keys, where there are few blocks.  What parts cost is the
   // join's launch, 3 us, and their sums in fp32: for tiles of 32 and 48 rows a
   // block has to save more than it writes (1500 tokens of a prompt, 600 blocks:

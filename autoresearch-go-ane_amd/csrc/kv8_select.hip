@@ -167,7 +167,7 @@ constexpr int kFar = 32768;  // scores that LDS holds at most
 // What bounds it: the chain of ids, boxes and scores, then the narrowing's steps,
 // each an LDS round trip and a barrier (1 token of 20,000 keys, 4 heads, 313
 // pages: 7.2 us; 64 tokens of 3500 to 24,000, 2 heads of 128, pages of 32: 13 us
-// for 14 MB of boxes; 841 tokens of 4 heads in 5 chunks 11.8 us).  Narrowing by
+// for 14 MB of boxes; 841 tokens of 4 heads in 5 chunks 9.9 us).  Narrowing by
 // halves, of bits or values, takes more such steps (21.6 us for the first with
 // update and attention, by histograms 19.2).
 template <int DH, int NT, int TOK, int NW, int CW>
@@ -195,13 +195,42 @@ __global__ __launch_bounds__(64 * NW) void select_kernel(SelectArgs a) {
   };
   int id = id_of(tid);
 
-  // the queries: largest's factors, then smallest's
-  intx4 z[NT][NM];
-  float up[NT][4], off[NT][4];  // what the lane's rows of the result are scaled by; rows of no head: -inf
+  // the boxes of 64 neighbours (id: of the lane's page, or -1), and what the
+  // lane's page's scores are scaled by (-1: it is not there)
+  struct Boxes {
+    intx4 w[4][NM];
+    float scale;
+  };
+  const auto load = [&](int id) {
+    Boxes x;
+    const int unit = a.unit[(size_t)max(id, 0) * b.NKV + h];
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
+      const int i = __shfl(id, 16 * c + col, 64);
+      const int8_t* box = a.box + ((size_t)max(i, 0) * b.NKV + h) * (2 * DH) + 16 * g;
+#pragma unroll
+      for (int m = 0; m < NM; m++) x.w[c][m] = *reinterpret_cast<const intx4*>(box + 64 * m);
+    }
+    x.scale = id < 0 ? -1.f : kv8_scale(clampi(unit, kUnitMin, kUnitMax));
+    return x;
+  };
+  // the queries: largest's factors, then smallest's; on their way with the wave's
+  // first boxes
+  half8 qs[NT][DH / 64][2];
 #pragma unroll
   for (int t = 0; t < NT; t++) {
     const int tok = min((col & 3) / HJ, span.n - 1), head = 16 * t + (col >> 2) + 4 * ((col & 3) % HJ);
     const half_t* p = a.q + (int64_t)(span.row + tok) * a.q_row + (h * a.G + min(head, a.G - 1)) * a.q_head;
+#pragma unroll
+    for (int m = 0; m < DH / 64; m++)
+#pragma unroll
+      for (int v = 0; v < 2; v++) qs[t][m][v] = ld_h8(p + 64 * m + 16 * g + 8 * v);
+  }
+  Boxes now = load(id);
+  intx4 z[NT][NM];
+  float up[NT][4], off[NT][4];  // what the lane's rows of the result are scaled by; rows of no head: -inf
+#pragma unroll
+  for (int t = 0; t < NT; t++) {
     // the lane's 16 dimensions of each 64; its row's other 48 lie with lanes col + 16 i
     float x[DH / 64][16];
     float amax = 0.f;
@@ -209,7 +238,7 @@ __global__ __launch_bounds__(64 * NW) void select_kernel(SelectArgs a) {
     for (int m = 0; m < DH / 64; m++)
 #pragma unroll
       for (int v = 0; v < 2; v++) {
-        const half8 y = ld_h8(p + 64 * m + 16 * g + 8 * v);
+        const half8 y = qs[t][m][v];
 #pragma unroll
         for (int j = 0; j < 8; j++) {
           float w = (float)y[j];
@@ -249,25 +278,6 @@ __global__ __launch_bounds__(64 * NW) void select_kernel(SelectArgs a) {
     }
   }
 
-  // the boxes of 64 neighbours (id: of the lane's page, or -1), and what the
-  // lane's page's scores are scaled by (-1: it is not there)
-  struct Boxes {
-    intx4 w[4][NM];
-    float scale;
-  };
-  const auto load = [&](int id) {
-    Boxes x;
-    const int unit = a.unit[(size_t)max(id, 0) * b.NKV + h];
-#pragma unroll
-    for (int c = 0; c < 4; c++) {
-      const int i = __shfl(id, 16 * c + col, 64);
-      const int8_t* box = a.box + ((size_t)max(i, 0) * b.NKV + h) * (2 * DH) + 16 * g;
-#pragma unroll
-      for (int m = 0; m < NM; m++) x.w[c][m] = *reinterpret_cast<const intx4*>(box + 64 * m);
-    }
-    x.scale = id < 0 ? -1.f : kv8_scale(clampi(unit, kUnitMin, kUnitMax));
-    return x;
-  };
   // Scores before that scale: of the values i = c TOK + token, for 16 pages c
   // and a token, row g of the lanes ends with those of i = 4 k + g in v[k].
   struct Raw {
@@ -315,10 +325,7 @@ __global__ __launch_bounds__(64 * NW) void select_kernel(SelectArgs a) {
   const bool near = span.n * stride <= a.room;
   if (near) {
     // a wave's boxes are on their way while it works on those before
-    int p = wave * 64;
-    Boxes now;
-    if (p < np) now = load(id);
-    for (; p < np; p += 64 * NW) {
+    for (int p = wave * 64; p < np; p += 64 * NW) {
       Boxes then = now;
       if (p + 64 * NW < np) then = load(id_of(p + 64 * NW + lane));
       const Raw r = raw_of(now);
