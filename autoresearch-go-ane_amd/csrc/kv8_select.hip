@@ -145,9 +145,9 @@ constexpr int kBins = 256;
 constexpr int kHeld = 1024;  // pages of a token whose scores its waves hold in registers
 constexpr int kFar = 32768;  // scores that LDS holds at most
 
-// A block takes up to 4, 2 or 1 tokens of a sequence (as their query heads, up
-// to 4, 8 or 16, or 32 with NT = 2, fill the 16 rows of a product) and a
-// key/value head.
+// A block takes up to 4, 2 or 1 tokens of a sequence (whose query heads, up to 4,
+// 8 or 16, or 32 with NT = 2, go into the 16 rows of a product) and a key/value
+// head.
 //
 // First its NW waves score the context's pages for all the tokens: 64 pages a
 // wave at a time, their ids with one load, their boxes in four products of 16.
@@ -321,6 +321,16 @@ __global__ __launch_bounds__(64 * NW) void select_kernel(SelectArgs a) {
     return scale < 0.f || page >= n ? -INFINITY : x;
   };
 
+  // of the waves of a token
+  const auto meet = [] {
+    if constexpr (CW > 1) {
+      __syncthreads();
+    } else {  // LDS accesses of a wave stay in order; this keeps the compiler to it
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    }
+  };
+
   const int stride = (np + 63) & ~63;
   const bool near = span.n * stride <= a.room;
   if (near) {
@@ -337,18 +347,10 @@ __global__ __launch_bounds__(64 * NW) void select_kernel(SelectArgs a) {
       }
       now = then;
     }
-    if (NW > 1) __syncthreads();
+    if constexpr (NW > 1) __syncthreads();
+    else meet();
   }
 
-  // of the waves of a token
-  const auto meet = [] {
-    if constexpr (CW > 1) {
-      __syncthreads();
-    } else {  // LDS accesses of a wave stay in order; this keeps the compiler to it
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-    }
-  };
   // over them, of values that are the same in a wave's lanes; and the sum over
   // those before
   int turn = 0;
@@ -561,20 +563,36 @@ int check_bounds(const char* op, const ane_kv8_bounds* x) {
   return ANE_OK;
 }
 
-// Rows of the queries' tile (16 or, of more heads, 32), tokens that it takes, and
-// the waves of a block: four, each a token's own, where a sequence may have
-// several tokens for them (11 chunks of up to 300 tokens 61 us a pass with the
-// update and the attention, with all waves at each token 64 to 69); eight that
-// share one where it has one (64 single tokens over 32,000 keys 31.4 us, with four
-// 32.0, with one of them choosing 33.5).
+// How a batch's tokens are dealt to blocks: nt tiles of 16 query rows, tok tokens
+// a block, its waves (which choose for a token together, or where it has several
+// each for its own).
+//
+// Tokens of chunks share their context's boxes, 4 to a block (of up to 4 heads)
+// or 2 (of up to 8), where there are more than 512 lists to make (800 of 3 heads
+// and 250 pages 7.4 us, a token a block 8.7 to 15.5 by its waves; 2000 pages 27
+// and 41; but 480 lists 26.6 and 25.2).  Otherwise a token has a block: of one
+// wave up to 64 pages (256 lists of 60 pages 5.2 us, of four waves 5.6, of eight
+// 6.1; 5600 13, 34 and 64), or 256 and 512 where there are more than 512 and 1024
+// lists (800 of 120 pages 7.3 us, of four 8.7; 512 of 250 8.3 and 7.8; 1600 of 250
+// 16.4 and 18.9); of four up to 512 pages (256
+// lists of 250 pages 6.4 us, eight 6.8); of eight beyond (900 pages 10.1 us, four
+// 10.7; 2000 pages, 4 lists, 15.5 and 17.9).
 struct Form {
   int nt, tok, waves;
 };
-Form form_of(const ane_kv8_batch& batch, int G) {
+// pages of the longest context, as far as the host knows
+int pages_of(const Kv8Batch& b, const ane_kv8_batch& batch) {
+  const int cap = b.table_pages << b.pshift;
+  return (((batch.max_len ? std::min(batch.max_len, cap) : cap) - 1) >> b.pshift) + 1;
+}
+Form form_of(const Kv8Batch& b, const ane_kv8_batch& batch, int G) {
+  const int pages = pages_of(b, batch);
   const int most = batch.max_new ? batch.max_new : (batch.rows + batch.nseq - 1) / std::max(batch.nseq, 1);
-  Form f = {G <= 16 ? 1 : 2, G <= 4 ? 4 : G <= 8 ? 2 : 1, 8};
-  if (f.tok > 1 && most > 1) f.waves = 4;
-  return f;
+  const int64_t lists = (int64_t)b.rows * b.NKV;
+  const int nt = G <= 16 ? 1 : 2;
+  if (most > 1 && lists > 512 && (G <= 4 || (G <= 8 && pages > 64))) return {nt, G <= 4 ? 4 : 2, 4};
+  if (pages <= (lists > 1024 ? 512 : lists > 512 ? 256 : 64)) return {nt, 1, 1};
+  return {nt, 1, pages <= 512 ? 4 : 8};
 }
 
 int check_sizes(const char* op, const Kv8Batch& b, const ane_kv8_batch& batch, int heads, int count) {
@@ -582,7 +600,7 @@ int check_sizes(const char* op, const Kv8Batch& b, const ane_kv8_batch& batch, i
     return op_fail(ANE_ERR_ARG, "storiesane %s: heads=%d must be 1..%d times kv_heads=%d", op, heads, kKvMaxGroup,
                    b.NKV);
   if (count < 1 || count > 65536) return op_fail(ANE_ERR_ARG, "storiesane %s: count=%d want 1..65536", op, count);
-  const Form f = form_of(batch, heads / b.NKV);
+  const Form f = form_of(b, batch, heads / b.NKV);
   if ((int64_t)kv8_count(b.nseq, b.rows, kv8_tiles(f.tok)) * b.NKV * 64 * f.waves > 0xffffffffll)  // threads
     return op_fail(ANE_ERR_ARG, "storiesane %s: rows=%d are too many for one launch", op, b.rows);
   return ANE_OK;
@@ -602,22 +620,20 @@ int launch_form(const char* op, SelectArgs a, int pages, hipStream_t st) {
   return ANE_OK;
 }
 
-template <int DH, int NT, int TOK>
-int launch_tokens(const char* op, const SelectArgs& a, int pages, int waves, hipStream_t st) {
-  if constexpr (TOK > 1)
-    if (waves == 4) return launch_form<DH, NT, TOK, 4, 1>(op, a, pages, st);
-  return launch_form<DH, NT, TOK, 8, 8>(op, a, pages, st);
+template <int DH, int NT>
+int launch_token(const char* op, const SelectArgs& a, int pages, const Form& f, hipStream_t st) {
+  if (f.waves == 1) return launch_form<DH, NT, 1, 1, 1>(op, a, pages, st);
+  if (f.waves == 4) return launch_form<DH, NT, 1, 4, 4>(op, a, pages, st);
+  return launch_form<DH, NT, 1, 8, 8>(op, a, pages, st);
 }
 
 template <int DH>
 int launch(const char* op, const SelectArgs& a, const ane_kv8_batch& batch, hipStream_t st) {
-  const int cap = a.b.table_pages << a.b.pshift;
-  const int pages = (((batch.max_len ? std::min(batch.max_len, cap) : cap) - 1) >> a.b.pshift) + 1;
-  const Form f = form_of(batch, a.G);
-  if (f.nt == 2) return launch_tokens<DH, 2, 1>(op, a, pages, f.waves, st);
-  if (f.tok == 4) return launch_tokens<DH, 1, 4>(op, a, pages, f.waves, st);
-  if (f.tok == 2) return launch_tokens<DH, 1, 2>(op, a, pages, f.waves, st);
-  return launch_tokens<DH, 1, 1>(op, a, pages, f.waves, st);
+  const int pages = pages_of(a.b, batch);
+  const Form f = form_of(a.b, batch, a.G);
+  if (f.tok == 4) return launch_form<DH, 1, 4, 4, 1>(op, a, pages, st);
+  if (f.tok == 2) return launch_form<DH, 1, 2, 4, 1>(op, a, pages, st);
+  return f.nt == 1 ? launch_token<DH, 1>(op, a, pages, f, st) : launch_token<DH, 2>(op, a, pages, f, st);
 }
 
 }  // namespace

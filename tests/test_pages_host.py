@@ -130,14 +130,14 @@ def test_select_of_nothing_and_attend_blocks_refuse():
 def test_more_rows_than_a_launch_takes():
     big = cache(kv_heads=1024)
     wide = dict(q_row=16 * 1024 * 64, heads=1024 * 16, blocks=1 << 50)
-    many = batch(rows=1 << 13)
-    refused(lib.ane_kv8_select(big, bounds(), many, select_args(**wide), None), "rows=8192 are too many")
-    refused(lib.ane_kv8_select_workspace(big, many, 1024 * 16, 7), "rows=8192 are too many")
-    assert lib.ane_kv8_select_workspace(big, many, 1024 * 4, 7) == 0    # four tokens a block
+    many = batch(rows=1 << 16)
+    refused(lib.ane_kv8_select(big, bounds(), many, select_args(**wide), None), "rows=65536 are too many")
+    refused(lib.ane_kv8_select_workspace(big, many, 1024 * 16, 7), "rows=65536 are too many")
+    assert lib.ane_kv8_select_workspace(big, batch(rows=1 << 15), 1024 * 16, 7) == 0
     a = _lib.Kv8AttendArgs(q=P16, out=1 << 50, q_row=16 * 1024 * 64, q_head=64, out_row=16 * 1024 * 64, out_head=64,
                            heads=1024 * 16, scale=0.125, ws=P16, ws_bytes=1 << 60)
     refused(lib.ane_kv8_attend_blocks(big, batch(rows=1 << 14), a, P16, 3, None), "rows=16384 nseq=2 are too many")
-    assert lib.ane_kv8_attend_blocks_workspace(big, many, 1024 * 16, 3) == 0
+    assert lib.ane_kv8_attend_blocks_workspace(big, batch(rows=1 << 13), 1024 * 16, 3) == 0
     refused(lib.ane_kv8_bound(cache(page_tokens=16), bounds(), batch(nseq=65536, rows=1 << 30), None),
             "rows=1073741824 are too many")
 
