@@ -837,6 +837,10 @@ int plan(const char* op, const Kv8Batch& b, const ane_kv8_batch& given, int DH, 
   // tiles 29.7 and 29.1).
   const bool eight = count && DH == 64 && p->nt == 1 && (p->room ? blocks <= 320 : blocks <= 128 && len <= 2048);
   if (eight) p->kw = 8;
+  // Many short lists: a wave a tile, four to a block (1200 of 64 keys, 16 heads, 6.3
+  // us, with four waves a tile 8.1; of 256 11.4 and 11.9, of 1024 29.8 and 28.4; 400
+  // of 128 6.6 and 5.9; of 32 heads 1200 of 512 20.3 and 24.7).
+  if (count && !p->room && blocks >= 768 && len <= 256 * p->nt) p->kw = 1;
   p->round = p->kw * kStep;
   // The longest contexts first, so that the last blocks to end are short ones:
   // chunks of prompts at the lengths they come in (8 of 100 to 400 on up to
@@ -921,6 +925,8 @@ void launch_list(const UnionArgs& a, const Plan& p, hipStream_t st) {
     if (p.kw == 8) launch_form<DH, 1, 8, 1, ListArgs>(a, st);
   }
   if (p.room) return launch_form<DH, 1, 4, 1>(a, st, lds);
+  if (p.kw == 1 && p.nt == 1) launch_form<DH, 1, 1, 4, ListArgs>(a, st);
+  else if (p.kw == 1) launch_form<DH, 2, 1, 4, ListArgs>(a, st);
   if (p.kw == 4 && p.nt == 1) launch_form<DH, 1, 4, 1, ListArgs>(a, st);
   else if (p.kw == 4) launch_form<DH, 2, 4, 1, ListArgs>(a, st);
   if (a.nsplit > 1)

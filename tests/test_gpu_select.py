@@ -502,3 +502,17 @@ def test_chunks_with_as_many_places_and_lists_as_lds_holds():
     x = Run(r, [(16 * 8130 + 3, 640)], 1, 1, 64, 16, spare=0).go()
     assert 8160 < x.table.shape[1] <= 8192
     x.attend(lists(r, x, 128, none=0.01))
+
+
+@pytest.mark.parametrize("heads, kvh, dh, P, count, lens", [
+    (12, 4, 64, 16, 7, [(700, 1)] * 201),
+    (16, 8, 128, 64, 2, [(130, 1), (0, 1), (63, 3)] * 34),
+    (40, 2, 64, 32, 13, [(900, 60), (3, 170), (0, 191)]),
+    (24, 1, 128, 16, 30, [(500, 801)]),
+])
+def test_many_short_lists(heads, kvh, dh, P, count, lens):
+    r = np.random.default_rng(heads + count)
+    x = Run(r, lens, heads, kvh, dh, P, nan=1e-5, max_new=max(n for _, n in lens)).go()
+    b = lists(r, x, count, twice=True, none=0.3)
+    b[5:9] = -1
+    x.attend(b)
