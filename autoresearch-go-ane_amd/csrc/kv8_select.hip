@@ -138,12 +138,199 @@ struct SelectArgs {
   int* blocks;
   int64_t q_row, q_head;
   int G, count, first, recent;
-  int room;  // scores that LDS holds
+  int room;       // scores that LDS holds
+  float* scores;  // [rows][NKV][table_pages], where the choice has a launch of its own
 };
 
 constexpr int kBins = 256;
 constexpr int kHeld = 1024;  // pages of a token whose scores its waves hold in registers
 constexpr int kFar = 32768;  // scores that LDS holds at most
+
+// LDS accesses of a wave stay in order; this keeps the compiler to it.
+__device__ __forceinline__ void in_order() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// What the CW waves of a token choose with.
+template <int CW>
+struct Choice {
+  int bins[kBins];
+  __attribute__((aligned(16))) float few[64];
+  int fews, sums[2][CW];
+};
+
+// The choice among scores that each(f) gives as f(page, score), a thread a page,
+// in order (-inf behind the last), by CW waves: of one, without a barrier.
+template <int CW, typename Each>
+__device__ __forceinline__ void choose(Choice<CW>& c, const Each& each, int count, int* out) {
+  constexpr int CT = 64 * CW;
+  const int lane = threadIdx.x & 63, ct = threadIdx.x % CT;
+  const int cw = __builtin_amdgcn_readfirstlane(ct >> 6);
+  for (int i = ct; i < kBins; i += CT) c.bins[i] = 0;
+  if (ct == 0) c.fews = 0;  // behind barriers before they count
+  if constexpr (CW == 1) in_order();
+  const auto meet = [] {
+    if constexpr (CW > 1) __syncthreads();
+    else in_order();
+  };
+  // over the waves, of values that are the same in a wave's lanes; and the sum
+  // over those before
+  int turn = 0;
+  const auto over = [&](auto x, auto op) {
+    if constexpr (CW > 1) {
+      using T = decltype(x);
+      if (lane == 0) c.sums[turn][cw] = __builtin_bit_cast(int, x);
+      __syncthreads();
+      x = over_lanes<CW>(__builtin_bit_cast(T, c.sums[turn][lane % CW]), op);
+      turn ^= 1;
+    }
+    return x;
+  };
+  const auto ranked = [&](int x, int& before) {
+    before = 0;
+    if constexpr (CW > 1) {
+      if (lane == 0) c.sums[turn][cw] = x;
+      __syncthreads();
+      const int y = c.sums[turn][lane % CW];
+      turn ^= 1;
+      x = 0;
+#pragma unroll
+      for (int w = 0; w < CW; w++) {
+        const int k = __builtin_amdgcn_readlane(y, w);
+        before += w < cw ? k : 0;
+        x += k;
+      }
+    }
+    return x;
+  };
+  const auto widest = [&](float x) { return over(over_lanes<64>(x, Max()), Max()); };
+  const uint64_t below = (1ull << lane) - 1;
+  int all = 0, always = 0;
+  float hi = -INFINITY, lo = -INFINITY;  // of the scores in question; the lowest one negated until it is known
+  each([&](int, float x) {
+    all += __popcll(__ballot(x > -INFINITY));
+    always += __popcll(__ballot(x == INFINITY));
+    if (fabsf(x) < INFINITY) {
+      hi = fmaxf(hi, x);
+      lo = fmaxf(lo, -x);
+    }
+  });
+  all = over(all, Sum());
+  // what is taken: scores above the bar, and of those at the bar the first
+  // `ties`, or all of them (-1)
+  float bar = -INFINITY;
+  int ties = 0;
+  if (all > count) {
+    always = over(always, Sum());
+    int need = count - always, in = all - always;  // pages to be taken, of those in question
+    bar = INFINITY;
+    if (need > 0) {
+      int bin = -1;
+      float step = 0.f;
+      const auto bin_of = [&](float x) {
+        return x >= lo && x <= hi ? min((int)((x - lo) * step), kBins - 1) : -1;
+      };
+      if (in > 64) {
+        hi = widest(hi);
+        lo = -widest(lo);
+        while (lo < hi) {
+          step = (float)kBins / (hi - lo);
+          each([&](int, float x) {
+            const int k = bin_of(x);
+            if (k >= 0) atomicAdd(&c.bins[k], 1);
+          });
+          meet();
+          // pages in the bins above the lane's four, and in them
+          int in_bin[4], sum = 0;
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            in_bin[i] = c.bins[kBins - 1 - (lane * 4 + i)];
+            sum += in_bin[i];
+          }
+          int above = sum_up_to(sum) - sum, it = -1, left = 0, size = 0;
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            if (above < need && need <= above + in_bin[i]) {
+              it = kBins - 1 - (lane * 4 + i);
+              left = need - above;
+              size = in_bin[i];
+            }
+            above += in_bin[i];
+          }
+          const int who = __ffsll((unsigned long long)__ballot(it >= 0)) - 1;
+          bin = __builtin_amdgcn_readlane(it, who);
+          need = __builtin_amdgcn_readlane(left, who);
+          in = __builtin_amdgcn_readlane(size, who);
+          if (in <= 64) break;
+          float x1 = -INFINITY, x0 = -INFINITY;
+          each([&](int, float x) {
+            if (bin_of(x) == bin) {
+              x1 = fmaxf(x1, x);
+              x0 = fmaxf(x0, -x);
+            }
+          });
+          hi = widest(x1);  // behind its barrier no wave reads the bins
+          lo = -widest(x0);
+          bin = -1;
+          for (int i = ct; i < kBins; i += CT) c.bins[i] = 0;
+          meet();
+        }
+      }
+      if (in <= 64) {
+        // the ones that are left, in any order
+        int at = 0;
+        each([&](int, float x) {
+          const bool is = bin < 0 ? fabsf(x) < INFINITY : bin_of(x) == bin;
+          const uint64_t who = __ballot(is);
+          if (CW > 1 && who) {
+            if (lane == 0) at = atomicAdd(&c.fews, __popcll(who));
+            at = __builtin_amdgcn_readfirstlane(at);
+          }
+          if (is) c.few[at + __popcll(who & below)] = x;
+          at += __popcll(who);
+        });
+        if (ct < 4 && in + ct < 64) c.few[in + ct] = -INFINITY;  // behind them, to whole words
+        meet();
+        const float x = c.few[min(lane, in - 1)];
+        int above = 0, from = 0;
+#pragma unroll 2
+        for (int k = 0; k < in; k += 4) {
+          const floatx4 y = *reinterpret_cast<const floatx4*>(c.few + k);
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            above += y[j] > x;
+            from += y[j] >= x;
+          }
+        }
+        const int who = __ffsll((unsigned long long)__ballot(lane < in && above < need && need <= from)) - 1;
+        bar = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), who));
+        above = __builtin_amdgcn_readlane(above, who);
+        from = __builtin_amdgcn_readlane(from, who);
+        ties = need == from ? -1 : need - above;
+      } else {  // all equal
+        bar = lo;
+        ties = need;
+      }
+    }
+  }
+  int taken = 0, equal = 0;  // before these 64 pages
+  each([&](int page, float x) {
+    bool take = x > bar || x == INFINITY || (ties < 0 && x == bar);
+    int before;
+    if (ties > 0) {
+      const uint64_t eq = __ballot(x == bar);
+      const int all_eq = ranked(__popcll(eq), before);
+      take = take || (x == bar && equal + before + __popcll(eq & below) < ties);
+      equal += all_eq;
+    }
+    const uint64_t tk = __ballot(take);
+    const int all_tk = ranked(__popcll(tk), before);
+    if (take) out[taken + before + __popcll(tk & below)] = page;
+    taken += all_tk;
+  });
+  for (int i = taken + ct; i < count; i += CT) out[i] = -1;
+}
 
 // A block takes up to 4, 2 or 1 tokens of a sequence (whose query heads, up to 4,
 // 8 or 16, or 32 with NT = 2, go into the 16 rows of a product) and a key/value
@@ -170,20 +357,21 @@ constexpr int kFar = 32768;  // scores that LDS holds at most
 // for 14 MB of boxes; 841 tokens of 4 heads in 5 chunks 9.9 us).  Narrowing by
 // halves, of bits or values, takes more such steps (21.6 us for the first with
 // update and attention, by histograms 19.2).
-template <int DH, int NT, int TOK, int NW, int CW>
+//
+// PART: a block leaves the scores of 64 NW pages of a token (and of those as many
+// blocks on) to choose_kernel.
+template <int DH, int NT, int TOK, int NW, int CW, bool PART>
 __global__ __launch_bounds__(64 * NW) void select_kernel(SelectArgs a) {
+  static_assert(!PART || TOK == 1);
   constexpr int NM = DH / 32;  // products of 64 terms
   constexpr int HJ = 4 / TOK;  // registers of a token
   static_assert(CW == 1 || CW == NW);
   constexpr int CH = NW / CW, CT = 64 * CW, R = kHeld / CT;
   extern __shared__ float scores[];  // [TOK][stride], room of them in all
-  __shared__ int bins_of[CH][kBins];
-  __shared__ __attribute__((aligned(16))) float few_of[CH][64];
-  __shared__ int fews, sums[2][CW];
+  __shared__ Choice<CW> choices[PART ? 1 : CH];
   const Kv8Batch& b = a.b;
   const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  for (int i = tid; i < CH * kBins; i += 64 * NW) bins_of[0][i] = 0;
   const int h = blockIdx.x % b.NKV;
   const Kv8Span span = kv8_tile_span(b, TOK, blockIdx.x / b.NKV);
   if (span.n == 0) return;
@@ -193,7 +381,9 @@ __global__ __launch_bounds__(64 * NW) void select_kernel(SelectArgs a) {
     const int id = trow[min(page, np - 1)];
     return page < np && (unsigned)id < (unsigned)b.pages ? id : -1;
   };
-  int id = id_of(tid);
+  const int base = PART ? blockIdx.y * (64 * NW) : 0, on = 64 * NW * (PART ? gridDim.y : 1);
+  if (base >= np) return;
+  int id = id_of(base + tid);
 
   // the boxes of 64 neighbours (id: of the lane's page, or -1), and what the
   // lane's page's scores are scaled by (-1: it is not there)
@@ -321,78 +511,35 @@ __global__ __launch_bounds__(64 * NW) void select_kernel(SelectArgs a) {
     return scale < 0.f || page >= n ? -INFINITY : x;
   };
 
-  // of the waves of a token
-  const auto meet = [] {
-    if constexpr (CW > 1) {
-      __syncthreads();
-    } else {  // LDS accesses of a wave stay in order; this keeps the compiler to it
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-    }
-  };
-
   const int stride = (np + 63) & ~63;
-  const bool near = span.n * stride <= a.room;
+  const bool near = PART || span.n * stride <= a.room;
   if (near) {
     // a wave's boxes are on their way while it works on those before
-    for (int p = wave * 64; p < np; p += 64 * NW) {
+    for (int p = base + wave * 64; p < np; p += on) {
       Boxes then = now;
-      if (p + 64 * NW < np) then = load(id_of(p + 64 * NW + lane));
+      if (p + on < np) then = load(id_of(p + on + lane));
       const Raw r = raw_of(now);
 #pragma unroll
       for (int k = 0; k < TOK; k++) {
         const int i = 4 * k + g, at = i / TOK * 16 + col, tok = i % TOK;
         const float scale = __shfl(now.scale, at, 64);
-        if (tok < span.n) scores[tok * stride + p + at] = score(r.v[k], scale, p + at, pages_of(tok));
+        const float x = score(r.v[k], scale, p + at, pages_of(tok));
+        if constexpr (PART) {
+          if (p + at < np) a.scores[((size_t)span.row * b.NKV + h) * b.table_pages + p + at] = x;
+        } else if (tok < span.n) {
+          scores[tok * stride + p + at] = x;
+        }
       }
       now = then;
     }
+    if constexpr (PART) return;
     if constexpr (NW > 1) __syncthreads();
-    else meet();
+    else in_order();
   }
 
-  // over them, of values that are the same in a wave's lanes; and the sum over
-  // those before
-  int turn = 0;
-  const auto over = [&](auto x, auto op) {
-    if constexpr (CW > 1) {
-      using T = decltype(x);
-      if (lane == 0) sums[turn][wave] = __builtin_bit_cast(int, x);
-      __syncthreads();
-      x = over_lanes<CW>(__builtin_bit_cast(T, sums[turn][lane % CW]), op);
-      turn ^= 1;
-    }
-    return x;
-  };
-  const auto ranked = [&](int x, int& before) {
-    before = 0;
-    if constexpr (CW > 1) {
-      if (lane == 0) sums[turn][wave] = x;
-      __syncthreads();
-      const int y = sums[turn][lane % CW];
-      turn ^= 1;
-      x = 0;
-#pragma unroll
-      for (int w = 0; w < CW; w++) {
-        const int k = __builtin_amdgcn_readlane(y, w);
-        before += w < wave ? k : 0;
-        x += k;
-      }
-    }
-    return x;
-  };
-  const auto widest = [&](float x) { return over(over_lanes<64>(x, Max()), Max()); };
-  int* bins = bins_of[wave / CW];
-  float* few = few_of[wave / CW];
   const int ct = tid % CT, cw = wave % CW;
-  const uint64_t below = (1ull << lane) - 1;
   for (int tok = wave / CW; tok < span.n; tok += CH) {
     const int n = pages_of(tok);
-    if (tok >= CH) {
-      meet();
-      for (int i = ct; i < kBins; i += CT) bins[i] = 0;
-    }
-    if (CW > 1 && tid == 0) fews = 0;  // behind barriers before it counts
     const bool held = near && n <= kHeld;
     float mine[R];
     if (held) {
@@ -427,133 +574,43 @@ __global__ __launch_bounds__(64 * NW) void select_kernel(SelectArgs a) {
       }
     };
 
-    int all = 0, always = 0;
-    float hi = -INFINITY, lo = -INFINITY;  // of the scores in question; the lowest one negated until it is known
-    each([&](int, float x) {
-      all += __popcll(__ballot(x > -INFINITY));
-      always += __popcll(__ballot(x == INFINITY));
-      if (fabsf(x) < INFINITY) {
-        hi = fmaxf(hi, x);
-        lo = fmaxf(lo, -x);
-      }
-    });
-    all = over(all, Sum());
-    // what is taken: scores above the bar, and of those at the bar the first
-    // `ties`, or all of them (-1)
-    float bar = -INFINITY;
-    int ties = 0;
-    if (all > a.count) {
-      always = over(always, Sum());
-      int need = a.count - always, in = all - always;  // pages to be taken, of those in question
-      bar = INFINITY;
-      if (need > 0) {
-        int bin = -1;
-        float step = 0.f;
-        const auto bin_of = [&](float x) {
-          return x >= lo && x <= hi ? min((int)((x - lo) * step), kBins - 1) : -1;
-        };
-        if (in > 64) {
-          hi = widest(hi);
-          lo = -widest(lo);
-          while (lo < hi) {
-            step = (float)kBins / (hi - lo);
-            each([&](int, float x) {
-              const int k = bin_of(x);
-              if (k >= 0) atomicAdd(&bins[k], 1);
-            });
-            meet();
-            // pages in the bins above the lane's four, and in them
-            int c[4], sum = 0;
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-              c[i] = bins[kBins - 1 - (lane * 4 + i)];
-              sum += c[i];
-            }
-            int above = sum_up_to(sum) - sum, it = -1, left = 0, size = 0;
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-              if (above < need && need <= above + c[i]) {
-                it = kBins - 1 - (lane * 4 + i);
-                left = need - above;
-                size = c[i];
-              }
-              above += c[i];
-            }
-            const int who = __ffsll((unsigned long long)__ballot(it >= 0)) - 1;
-            bin = __builtin_amdgcn_readlane(it, who);
-            need = __builtin_amdgcn_readlane(left, who);
-            in = __builtin_amdgcn_readlane(size, who);
-            if (in <= 64) break;
-            float x1 = -INFINITY, x0 = -INFINITY;
-            each([&](int, float x) {
-              if (bin_of(x) == bin) {
-                x1 = fmaxf(x1, x);
-                x0 = fmaxf(x0, -x);
-              }
-            });
-            hi = widest(x1);  // behind its barrier no wave reads the bins
-            lo = -widest(x0);
-            bin = -1;
-            for (int i = ct; i < kBins; i += CT) bins[i] = 0;
-            meet();
-          }
-        }
-        if (in <= 64) {
-          // the ones that are left, in any order
-          int at = 0;
-          each([&](int, float x) {
-            const bool is = bin < 0 ? fabsf(x) < INFINITY : bin_of(x) == bin;
-            const uint64_t who = __ballot(is);
-            if (CW > 1 && who) {
-              if (lane == 0) at = atomicAdd(&fews, __popcll(who));
-              at = __builtin_amdgcn_readfirstlane(at);
-            }
-            if (is) few[at + __popcll(who & below)] = x;
-            at += __popcll(who);
-          });
-          if (ct < 4 && in + ct < 64) few[in + ct] = -INFINITY;  // behind them, to whole words
-          meet();
-          const float x = few[min(lane, in - 1)];
-          int above = 0, from = 0;
-#pragma unroll 2
-          for (int k = 0; k < in; k += 4) {
-            const floatx4 y = *reinterpret_cast<const floatx4*>(few + k);
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-              above += y[j] > x;
-              from += y[j] >= x;
-            }
-          }
-          const int who = __ffsll((unsigned long long)__ballot(lane < in && above < need && need <= from)) - 1;
-          bar = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), who));
-          above = __builtin_amdgcn_readlane(above, who);
-          from = __builtin_amdgcn_readlane(from, who);
-          ties = need == from ? -1 : need - above;
-        } else {  // all equal
-          bar = lo;
-          ties = need;
-        }
-      }
-    }
-    int* out = a.blocks + ((size_t)(span.row + tok) * b.NKV + h) * a.count;
-    int taken = 0, equal = 0;  // before these 64 pages
-    each([&](int page, float x) {
-      bool take = x > bar || x == INFINITY || (ties < 0 && x == bar);
-      int before;
-      if (ties > 0) {
-        const uint64_t eq = __ballot(x == bar);
-        const int all_eq = ranked(__popcll(eq), before);
-        take = take || (x == bar && equal + before + __popcll(eq & below) < ties);
-        equal += all_eq;
-      }
-      const uint64_t tk = __ballot(take);
-      const int all_tk = ranked(__popcll(tk), before);
-      if (take) out[taken + before + __popcll(tk & below)] = page;
-      taken += all_tk;
-    });
-    for (int c = taken + ct; c < a.count; c += CT) out[c] = -1;
+    choose<CW>(choices[wave / CW], each, a.count, a.blocks + ((size_t)(span.row + tok) * b.NKV + h) * a.count);
   }
 }
+
+// The choice among scores that another launch left: a block a token and key/value
+// head (4 of 2000 pages 10 us with the scores' launch, 5 of them this one's).
+constexpr int kHeldFar = 16384;  // of them, those that registers hold; more are read in every pass
+__global__ __launch_bounds__(512) void choose_kernel(SelectArgs a) {
+  constexpr int CW = 8, CT = 64 * CW, R = kHeldFar / CT;
+  __shared__ Choice<CW> c;
+  const Kv8Batch& b = a.b;
+  const int tid = threadIdx.x, h = blockIdx.x % b.NKV;
+  const Kv8Span span = kv8_tile_span(b, 1, blockIdx.x / b.NKV);
+  if (span.n == 0) return;
+  const int n = (span.pos >> b.pshift) + 1;
+  const size_t list = (size_t)span.row * b.NKV + h;
+  const float* s = a.scores + list * b.table_pages;
+  float mine[R];
+#pragma unroll
+  for (int r = 0; r < R; r++) {
+    mine[r] = -INFINITY;
+    if (r * CT < n && n <= kHeldFar) mine[r] = r * CT + tid < n ? s[r * CT + tid] : -INFINITY;
+  }
+  const auto each = [&](auto f) {
+    if (n <= kHeldFar) {
+#pragma unroll
+      for (int r = 0; r < R; r++)
+        if (r * CT < n) f(r * CT + tid, mine[r]);
+    } else {
+      for (int p = 0; p < n; p += CT) f(p + tid, p + tid < n ? s[p + tid] : -INFINITY);
+    }
+  };
+  choose<CW>(c, each, a.count, a.blocks + list * a.count);
+}
+
+// of the workspace of a choice in parts
+int64_t scores_bytes(const Kv8Batch& b) { return (int64_t)b.rows * b.NKV * b.table_pages * 4; }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
@@ -577,38 +634,55 @@ int check_bounds(const char* op, const ane_kv8_bounds* x) {
 // 16.4 and 18.9); of four up to 512 pages (256
 // lists of 250 pages 6.4 us, eight 6.8); of eight beyond (900 pages 10.1 us, four
 // 10.7; 2000 pages, 4 lists, 15.5 and 17.9).
+//
+// Up to 128 lists of long contexts: the scores by two waves for every 128 pages,
+// the choice behind a launch (4 lists of head dimension 64 and 1000 pages 9.0 us,
+// in one launch 10.0; of 2000 10.1 and 15.5, 8000 16.4 and 44; of 750 9.1 and 9.0;
+// 128 of 2000 17.1 and 18.4, 256 22.9 and 20.2; head dimension 128, 8 of 500 9.5
+// and 9.8, 8000 18 and 73).
 struct Form {
   int nt, tok, waves;
+  bool parts = false;
 };
 // pages of the longest context, as far as the host knows
 int pages_of(const Kv8Batch& b, const ane_kv8_batch& batch) {
   const int cap = b.table_pages << b.pshift;
   return (((batch.max_len ? std::min(batch.max_len, cap) : cap) - 1) >> b.pshift) + 1;
 }
-Form form_of(const Kv8Batch& b, const ane_kv8_batch& batch, int G) {
+Form form_of(const Kv8Batch& b, const ane_kv8_batch& batch, int dh, int G) {
   const int pages = pages_of(b, batch);
   const int most = batch.max_new ? batch.max_new : (batch.rows + batch.nseq - 1) / std::max(batch.nseq, 1);
   const int64_t lists = (int64_t)b.rows * b.NKV;
   const int nt = G <= 16 ? 1 : 2;
   if (most > 1 && lists > 512 && (G <= 4 || (G <= 8 && pages > 64))) return {nt, G <= 4 ? 4 : 2, 4};
   if (pages <= (lists > 1024 ? 512 : lists > 512 ? 256 : 64)) return {nt, 1, 1};
+  if (lists <= 128 && pages * dh >= 65536 && lists * b.table_pages <= 1 << 22) return {nt, 1, 2, true};
   return {nt, 1, pages <= 512 ? 4 : 8};
 }
 
-int check_sizes(const char* op, const Kv8Batch& b, const ane_kv8_batch& batch, int heads, int count) {
+int check_sizes(const char* op, const Kv8Batch& b, const ane_kv8_batch& batch, int dh, int heads, int count) {
   if (heads < 1 || heads % b.NKV || heads / b.NKV > kKvMaxGroup)
     return op_fail(ANE_ERR_ARG, "storiesane %s: heads=%d must be 1..%d times kv_heads=%d", op, heads, kKvMaxGroup,
                    b.NKV);
   if (count < 1 || count > 65536) return op_fail(ANE_ERR_ARG, "storiesane %s: count=%d want 1..65536", op, count);
-  const Form f = form_of(b, batch, heads / b.NKV);
+  const Form f = form_of(b, batch, dh, heads / b.NKV);
   if ((int64_t)kv8_count(b.nseq, b.rows, kv8_tiles(f.tok)) * b.NKV * 64 * f.waves > 0xffffffffll)  // threads
     return op_fail(ANE_ERR_ARG, "storiesane %s: rows=%d are too many for one launch", op, b.rows);
   return ANE_OK;
 }
 
+template <int DH, int NT>
+void launch_parts(const SelectArgs& a, int pages, hipStream_t st) {
+  const uint32_t lists = kv8_count(a.b.nseq, a.b.rows, kv8_tiles(1)) * a.b.NKV;
+  // blocks for what the longest context may have, but no more than fill the card many times
+  const uint32_t parts = std::min<uint32_t>((pages + 127) / 128, std::max(1u, 16384 / lists));
+  hipLaunchKernelGGL((select_kernel<DH, NT, 1, 2, 1, true>), dim3(lists, parts), dim3(128), 0, st, a);
+  hipLaunchKernelGGL(choose_kernel, dim3(lists), dim3(512), 0, st, a);
+}
+
 template <int DH, int NT, int TOK, int NW, int CW>
 int launch_form(const char* op, SelectArgs a, int pages, hipStream_t st) {
-  auto* const kernel = select_kernel<DH, NT, TOK, NW, CW>;
+  auto* const kernel = select_kernel<DH, NT, TOK, NW, CW, false>;
   a.room = std::min(TOK * ((pages + 63) & ~63), kFar);
   const int lds = a.room * 4;
   if (lds > 32768) {
@@ -630,7 +704,12 @@ int launch_token(const char* op, const SelectArgs& a, int pages, const Form& f, 
 template <int DH>
 int launch(const char* op, const SelectArgs& a, const ane_kv8_batch& batch, hipStream_t st) {
   const int pages = pages_of(a.b, batch);
-  const Form f = form_of(a.b, batch, a.G);
+  const Form f = form_of(a.b, batch, DH, a.G);
+  if (f.parts) {
+    if (f.nt == 1) launch_parts<DH, 1>(a, pages, st);
+    else launch_parts<DH, 2>(a, pages, st);
+    return ANE_OK;
+  }
   if (f.tok == 4) return launch_form<DH, 1, 4, 4, 1>(op, a, pages, st);
   if (f.tok == 2) return launch_form<DH, 1, 2, 4, 1>(op, a, pages, st);
   return f.nt == 1 ? launch_token<DH, 1>(op, a, pages, f, st) : launch_token<DH, 2>(op, a, pages, f, st);
@@ -669,8 +748,8 @@ extern "C" int64_t ane_kv8_select_workspace(const ane_kv8_cache* cache, const an
   const char* op = "kv8 select workspace";
   Kv8Batch b;
   int rc = kv8_check(op, cache, batch, &b);
-  if (!rc) rc = check_sizes(op, b, *batch, heads, count);
-  return rc ? rc : 0;
+  if (!rc) rc = check_sizes(op, b, *batch, cache->head_dim, heads, count);
+  return rc ? rc : form_of(b, *batch, cache->head_dim, heads / b.NKV).parts ? scores_bytes(b) : 0;
 }
 
 extern "C" int ane_kv8_select(const ane_kv8_cache* cache, const ane_kv8_bounds* bounds, const ane_kv8_batch* batch,
@@ -682,7 +761,7 @@ extern "C" int ane_kv8_select(const ane_kv8_cache* cache, const ane_kv8_bounds* 
   if (rc) return rc;
   if (!args) return op_fail(ANE_ERR_ARG, "storiesane %s: null arguments", op);
   const ane_kv8_select_args& g = *args;
-  rc = check_sizes(op, a.b, *batch, g.heads, g.count);
+  rc = check_sizes(op, a.b, *batch, cache->head_dim, g.heads, g.count);
   if (rc) return rc;
   if (g.first < 0 || g.recent < 0 || (int64_t)g.first + g.recent > g.count)
     return op_fail(ANE_ERR_ARG, "storiesane %s: first=%d recent=%d want 0 or more, together at most count=%d", op,
@@ -696,11 +775,16 @@ extern "C" int ane_kv8_select(const ane_kv8_cache* cache, const ane_kv8_bounds* 
                             {"blocks", flat(g.blocks, (int64_t)a.b.rows * a.b.NKV * g.count * 4), true}};
   rc = check_apart(op, buffers, 2);
   if (rc) return rc;
+  if (form_of(a.b, *batch, cache->head_dim, g.heads / a.b.NKV).parts &&
+      (!g.ws || !aligned16(g.ws) || g.ws_bytes < scores_bytes(a.b)))
+    return op_fail(ANE_ERR_ARG, "storiesane %s: workspace of %lld bytes, want %lld, 16-byte aligned", op,
+                   (long long)(g.ws ? g.ws_bytes : 0), (long long)scores_bytes(a.b));
   DeviceScope dev(cache->device);
   if (dev.status() != hipSuccess)
     return op_fail(ANE_ERR_HIP, "storiesane %s: device %d: %s", op, cache->device, hipGetErrorString(dev.status()));
   a.q = (const half_t*)g.q; a.box = bounds->box; a.unit = bounds->unit; a.blocks = g.blocks;
   a.q_row = g.q_row; a.q_head = g.q_head;
+  a.scores = (float*)g.ws;
   a.G = g.heads / a.b.NKV; a.count = g.count; a.first = g.first; a.recent = g.recent;
   rc = cache->head_dim == 64 ? launch<64>(op, a, *batch, (hipStream_t)stream)
                              : launch<128>(op, a, *batch, (hipStream_t)stream);

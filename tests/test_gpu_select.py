@@ -516,3 +516,54 @@ def test_many_short_lists(heads, kvh, dh, P, count, lens):
     b = lists(r, x, count, twice=True, none=0.3)
     b[5:9] = -1
     x.attend(b)
+
+
+@pytest.mark.parametrize("n, count", [(1024, 7), (1500, 100), (16383, 40), (16384, 40), (16385, 40), (17500, 3000)])
+@pytest.mark.parametrize("heads, kvh, dh", [(3, 1, 64), (34, 2, 128)])
+def test_long_contexts_in_parts(n, count, heads, kvh, dh):
+    """Scores and choice in launches of their own, next to short contexts, and
+    with hints of shorter ones."""
+    r = np.random.default_rng(n + heads)
+    for hints in ({}, dict(max_len=16 * 1100)):
+        x = Run(r, [(16 * (n - 1) + 3, 1), (40, 2), (0, 1)], heads, kvh, dh, 16, **hints).go()
+        x.box[:, :, 0], x.box[:, :, 1] = np.maximum(x.box[:, :, 0], x.box[:, :, 1]), np.minimum(x.box[:, :, 0],
+                                                                                              x.box[:, :, 1])
+        x.table[0, r.integers(0, n, 9)] = -1
+        x.batch = batch_of(x.table, x.start, x.offsets, x.rows, **hints)
+        x.bounds.box.copy_(dev(x.box))
+        x.select(count, 1, 2)
+
+
+@pytest.mark.parametrize("n", [1100, 9000])
+def test_long_contexts_of_wide_tables(n):
+    """In one launch, as the scores of all places would be too many."""
+    r = np.random.default_rng(n)
+    x = Run(r, [(16 * (n - 1) + 3, 1), (40, 1)], 3, 1, 64, 16, spare=1 << 21, rows_behind=0, max_len=16 * n).go()
+    x.select(50, 1, 2)
+
+
+def test_long_contexts_in_parts_captured():
+    r = np.random.default_rng(29)
+    x = Run(r, [(16 * 1500, 1), (16 * 1200, 1)], 4, 2, 64, 16).go()
+    q = dev(x.q)
+    b = torch.zeros((x.rows, 2, 33), dtype=torch.int32, device=DEV)
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        x.bounds.Select(x.batch, q, 33, blocks=b)
+        stream.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            x.bounds.Select(x.batch, q, 33, blocks=b)
+    start = x.batch._keep[1]
+    for i in range(4):
+        q.copy_(dev(r.standard_normal(x.q.shape).astype(np.float16)))
+        start.copy_(dev(np.array([16 * (1500 - 300 * i) + i, 16 * 1200 - 999 * i], np.int32)))
+        torch.cuda.synchronize()
+        b.fill_(-7)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = b.clone()
+        b.fill_(-7)
+        x.bounds.Select(x.batch, q, 33, blocks=b)
+        torch.cuda.synchronize()
+        assert torch.equal(got, b) and (b[:2] >= -1).all() and (b[2:] == -7).all()

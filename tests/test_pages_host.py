@@ -127,6 +127,14 @@ def test_select_of_nothing_and_attend_blocks_refuse():
     assert lib.ane_kv8_attend_blocks(cache(), batch(nseq=0, rows=0), a, None, 3, None) == _lib.ANE_OK
 
 
+def test_select_of_long_contexts_wants_a_workspace():
+    long = batch(table_pages=1024, table_stride=1024)
+    assert lib.ane_kv8_select_workspace(cache(), long, 4, 3) == 5 * 2 * 1024 * 4
+    assert lib.ane_kv8_select_workspace(cache(), batch(table_pages=1023, table_stride=1023), 4, 3) == 0
+    for ws, n in ((None, 1 << 20), (P16, 5 * 2 * 1024 * 4 - 1), (P16 + 8, 1 << 20)):
+        refused(lib.ane_kv8_select(cache(), bounds(), long, select_args(ws=ws, ws_bytes=n), None), "workspace of")
+
+
 def test_more_rows_than_a_launch_takes():
     big = cache(kv_heads=1024)
     wide = dict(q_row=16 * 1024 * 64, heads=1024 * 16, blocks=1 << 50)
@@ -136,7 +144,7 @@ def test_more_rows_than_a_launch_takes():
     assert lib.ane_kv8_select_workspace(big, batch(rows=1 << 15), 1024 * 16, 7) == 0
     a = _lib.Kv8AttendArgs(q=P16, out=1 << 50, q_row=16 * 1024 * 64, q_head=64, out_row=16 * 1024 * 64, out_head=64,
                            heads=1024 * 16, scale=0.125, ws=P16, ws_bytes=1 << 60)
-    refused(lib.ane_kv8_attend_blocks(big, batch(rows=1 << 14), a, P16, 3, None), "rows=16384 nseq=2 are too many")
+    refused(lib.ane_kv8_attend_blocks(big, batch(rows=1 << 14), a, P16, 30, None), "rows=16384 nseq=2 are too many")
     assert lib.ane_kv8_attend_blocks_workspace(big, batch(rows=1 << 13), 1024 * 16, 3) == 0
     refused(lib.ane_kv8_bound(cache(page_tokens=16), bounds(), batch(nseq=65536, rows=1 << 30), None),
             "rows=1073741824 are too many")
