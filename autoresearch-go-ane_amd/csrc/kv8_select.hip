@@ -631,15 +631,17 @@ int check_bounds(const char* op, const ane_kv8_bounds* x) {
 // wave up to 64 pages (256 lists of 60 pages 5.2 us, of four waves 5.6, of eight
 // 6.1; 5600 13, 34 and 64), or 256 and 512 where there are more than 512 and 1024
 // lists (800 of 120 pages 7.3 us, of four 8.7; 512 of 250 8.3 and 7.8; 1600 of 250
-// 16.4 and 18.9); of four up to 512 pages (256
-// lists of 250 pages 6.4 us, eight 6.8); of eight beyond (900 pages 10.1 us, four
-// 10.7; 2000 pages, 4 lists, 15.5 and 17.9).
+// 16.4 and 18.9); of four up to 512 pages (256 lists of 250 pages 6.4 us, eight
+// 6.8); of eight beyond (900 pages 10.1 us, four 10.7; 2000 pages, 4 lists, 15.5
+// and 17.9).
 //
 // Up to 128 lists of long contexts: the scores by two waves for every 128 pages,
 // the choice behind a launch (4 lists of head dimension 64 and 1000 pages 9.0 us,
 // in one launch 10.0; of 2000 10.1 and 15.5, 8000 16.4 and 44; of 750 9.1 and 9.0;
-// 128 of 2000 17.1 and 18.4, 256 22.9 and 20.2; head dimension 128, 8 of 500 9.5
-// and 9.8, 8000 18 and 73).
+// head dimension 128, 8 of 500 9.5 and 9.8, 8000 18 and 73).  Of more than 32 they
+// have to be twice as long (64 of 1500 11.7 and 13.9, of 1000 10.1 and 10.2; 128 of
+// head dimension 128, 1500 18.5 and 21.0, of up to 750 13.4 and 12.4), and 256 gain
+// nothing (of 2000 22.9 and 20.2).
 struct Form {
   int nt, tok, waves;
   bool parts = false;
@@ -656,7 +658,8 @@ Form form_of(const Kv8Batch& b, const ane_kv8_batch& batch, int dh, int G) {
   const int nt = G <= 16 ? 1 : 2;
   if (most > 1 && lists > 512 && (G <= 4 || (G <= 8 && pages > 64))) return {nt, G <= 4 ? 4 : 2, 4};
   if (pages <= (lists > 1024 ? 512 : lists > 512 ? 256 : 64)) return {nt, 1, 1};
-  if (lists <= 128 && pages * dh >= 65536 && lists * b.table_pages <= 1 << 22) return {nt, 1, 2, true};
+  if (lists <= 128 && (int64_t)pages * dh >= (lists <= 32 ? 65536 : 131072) && lists * b.table_pages <= 1 << 22)
+    return {nt, 1, 2, true};
   return {nt, 1, pages <= 512 ? 4 : 8};
 }
 
