@@ -67,7 +67,7 @@ struct BeamArgs {
   int beams, vocab, eos, history_max;
   int segs, parts;     // of a row
   int words, stretch;  // of 8 ids: of a history; of one that a block moves at a time
-  uint32_t words_magic;
+  uint32_t words_magic, segs_magic;
   Move* moves;         // [rows], where histories have a launch of their own
   float* seg_max;   // [rows][segs]
   Part* part;       // [rows][parts]
@@ -343,15 +343,18 @@ __global__ __launch_bounds__(TH) void choose_kernel(BeamArgs a) {
   const int row0 = blockIdx.x * W;
   const T* logits = static_cast<const T*>(a.logits);
 
-  // segments: 64 of a beam are a wave's at a time
-  const int runs = (a.segs + 63) >> 6;
-  int per = (W * runs + NW - 1) / NW;
+  // segments: one a thread, dealt to the groups in turn, or 64 of a beam a wave's at
+  // a time
+  const int runs = (a.segs + 63) >> 6, dealt = (tid & 15) * Pick<TH>::kGroups + (tid >> 4);
+  const bool few = W * a.segs <= TH;
+  int per = few ? 1 : (W * runs + NW - 1) / NW;
   Item x[kPer];
 #pragma unroll
   for (int j = 0; j < kPer; j++) {
     x[j] = {-INFINITY, kNone + j * TH + tid, -INFINITY};
     if (j >= per) continue;
-    const int u = j * NW + wave, w = u / runs, seg = (u - w * runs) * 64 + lane;
+    const int u = j * NW + wave, w = few ? quotient(dealt, a.segs, a.segs_magic) : u / runs;
+    const int seg = few ? dealt - w * a.segs : (u - w * runs) * 64 + lane;
     x[j].x = a.seg_max[(size_t)(row0 + min(w, W - 1)) * a.segs + min(seg, a.segs - 1)];
     if (w < W && seg < a.segs) x[j].at = w << 16 | seg;
   }
@@ -430,7 +433,7 @@ __global__ __launch_bounds__(TH) void choose_kernel(BeamArgs a) {
 #pragma unroll
   for (int j = 0; j < kPer; j++) {
     if (j >= per) break;
-    const int w = min((j * NW + wave) / runs, W - 1);
+    const int w = x[j].at < kNone ? x[j].at >> 16 : 0;
     if (ended[w]) x[j].x = (x[j].at & 0xffff) == 0 ? 0.f : -INFINITY;
     if (x[j].at < kNone) x[j].key = key_of(w, x[j].x);
   }
@@ -642,6 +645,7 @@ extern "C" int ane_beam_select(const ane_beam_args* args, void* stream) {
   a.seg_max = (float*)g.ws;
   a.words = (g.history_max + 7) / 8;
   a.words_magic = a.words ? magic(a.words) : 0;
+  a.segs_magic = magic(a.segs);
   a.stretch = kWords / g.beams;
   // Histories of up to 8 words a thread move in the second launch (40 requests of
   // 16 beams and 2564 ids: 35.6 us a step, in a launch of their own 37.8).
