@@ -199,12 +199,13 @@ __device__ __forceinline__ bool before(double ak, int aa, double bk, int ba) {
 template <int TH>
 struct Pick {
   static constexpr int kBeams = TH / 32, kGroups = TH / 16;
-  double key[kBeams * 16 * kPer];  // those that may be among the best
-  int at[kBeams * 16 * kPer];
-  float x[kBeams * 16 * kPer];
+  static constexpr int kMost = kBeams * 16 * kPer;
+  double key[kMost];  // those that may be among the best
+  int at[kMost];
+  float x[kMost];
   double gkey[kGroups];
   int gat[kGroups];
-  int count;
+  int count[2];  // of the first pick and of the second
   double bar_key;
   int bar_at;
 };
@@ -226,58 +227,66 @@ __device__ __forceinline__ void row_best(double& key, int& at) {
 // wave an item, its lanes the others.  Where the groups were uneven and more
 // than a wave's lanes reach the bar, they are dealt out again, one to each group
 // in turn: at most the items of `want` groups, half of them, reach the next bar.
-template <int TH, typename F>
-__device__ __forceinline__ void pick(Item (&x)[kPer], int per, int want, Pick<TH>& p, F best) {
+// BAR: a key that at least `want` items reach, if there are as many, is known, and
+// `count` is 0; it does in place of the first bar where those that reach it have
+// room.
+template <int TH, bool BAR, typename F>
+__device__ __forceinline__ void pick(Item (&x)[kPer], int per, int want, Pick<TH>& p, int& count, double known, F best) {
   constexpr int GR = Pick<TH>::kGroups;
   static_assert(2 * Pick<TH>::kBeams <= GR, "");
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  for (;;) {
-    double key = x[0].key;
-    int at = x[0].at;
+  for (bool first = BAR;; first = false) {
+    double key = known;
+    int at = 0x7fffffff;  // behind every index
+    if (!first) {
+      key = x[0].key;
+      at = x[0].at;
 #pragma unroll
-    for (int j = 1; j < kPer; j++) {
-      if (j >= per) break;
-      const bool b = before(x[j].key, x[j].at, key, at);
-      key = b ? x[j].key : key;
-      at = b ? x[j].at : at;
-    }
-    row_best<8>(key, at);
-    row_best<4>(key, at);
-    row_best<2>(key, at);
-    row_best<1>(key, at);
-    if ((tid & 15) == 0) {
-      p.gkey[tid >> 4] = key;
-      p.gat[tid >> 4] = at;
-    }
-    if (tid == 0) p.count = 0;
-    __syncthreads();
-    key = p.gkey[lane % GR];
-    at = p.gat[lane % GR];
-#pragma unroll
-    for (int j = 0; j < 4; j++) {  // the groups have different items: one of them has this rank
-      const int b = wave * 4 + j;
-      const double bk = p.gkey[b];
-      const int ba = p.gat[b];
-      if (__popcll(__ballot(lane < GR && before(key, at, bk, ba))) == want - 1 && lane == 0) {
-        p.bar_key = bk;
-        p.bar_at = ba;
+      for (int j = 1; j < kPer; j++) {
+        if (j >= per) break;
+        const bool b = before(x[j].key, x[j].at, key, at);
+        key = b ? x[j].key : key;
+        at = b ? x[j].at : at;
       }
+      row_best<8>(key, at);
+      row_best<4>(key, at);
+      row_best<2>(key, at);
+      row_best<1>(key, at);
+      if ((tid & 15) == 0) {
+        p.gkey[tid >> 4] = key;
+        p.gat[tid >> 4] = at;
+      }
+      if (tid == 0) count = 0;
+      __syncthreads();
+      key = p.gkey[lane % GR];
+      at = p.gat[lane % GR];
+#pragma unroll
+      for (int j = 0; j < 4; j++) {  // the groups have different items: one of them has this rank
+        const int b = wave * 4 + j;
+        const double bk = p.gkey[b];
+        const int ba = p.gat[b];
+        if (__popcll(__ballot(lane < GR && before(key, at, bk, ba))) == want - 1 && lane == 0) {
+          p.bar_key = bk;
+          p.bar_at = ba;
+        }
+      }
+      __syncthreads();
+      key = p.bar_key;
+      at = p.bar_at;
     }
-    __syncthreads();
-    key = p.bar_key;
-    at = p.bar_at;
 #pragma unroll
     for (int j = 0; j < kPer; j++) {
       if (j >= per) break;
       if ((x[j].key > -INFINITY) & !before(key, at, x[j].key, x[j].at)) {
-        const int k = atomicAdd(&p.count, 1);
+        const int k = atomicAdd(&count, 1);
+        if (first && k >= Pick<TH>::kMost) continue;
         p.key[k] = x[j].key;
         p.at[k] = x[j].at;
         p.x[k] = x[j].x;
       }
     }
     __syncthreads();
-    const int n = p.count;
+    const int n = count;
     if (n <= 64) {
       key = p.key[min(lane, n)];
       at = p.at[min(lane, n)];
@@ -289,13 +298,15 @@ __device__ __forceinline__ void pick(Item (&x)[kPer], int per, int want, Pick<TH
       }
       break;
     }
-    per = (n + TH - 1) / TH;
+    if (n <= Pick<TH>::kMost) {
+      per = (n + TH - 1) / TH;
 #pragma unroll
-    for (int j = 0; j < kPer; j++) {
-      if (j >= per) break;
-      const int k = j * TH + (tid & 15) * GR + (tid >> 4);
-      x[j] = {-INFINITY, kNone + k, 0.f};
-      if (k < n) x[j] = {p.key[k], p.at[k], p.x[k]};
+      for (int j = 0; j < kPer; j++) {
+        if (j >= per) break;
+        const int k = j * TH + (tid & 15) * GR + (tid >> 4);
+        x[j] = {-INFINITY, kNone + k, 0.f};
+        if (k < n) x[j] = {p.key[k], p.at[k], p.x[k]};
+      }
     }
     __syncthreads();
   }
@@ -333,6 +344,7 @@ __global__ __launch_bounds__(TH) void choose_kernel(BeamArgs a) {
   constexpr int NW = TH / 64, MB = Pick<TH>::kBeams;
   constexpr int BW = MB / NW, PL = kMaxParts / 64, HQ = kWords / TH;  // beams of a wave, parts and words of a lane
   __shared__ Pick<TH> pick_;
+  __shared__ double bar;  // the key of the last of the best segments
   // a beam's s(v) = score + (x - lse); one that is finished has lse 0 and the
   // candidate x = 0, and one that proposes nothing has no number
   __shared__ double score[MB], lse[MB], weight[MB], score_of[MB];
@@ -437,7 +449,14 @@ __global__ __launch_bounds__(TH) void choose_kernel(BeamArgs a) {
     if (ended[w]) x[j].x = (x[j].at & 0xffff) == 0 ? 0.f : -INFINITY;
     if (x[j].at < kNone) x[j].key = key_of(w, x[j].x);
   }
-  pick<TH>(x, per, W, pick_, [&](int rank, const Item& t) { seg_of[rank] = t.at; });
+  if (tid == 0) {
+    bar = -INFINITY;
+    pick_.count[1] = 0;
+  }
+  pick<TH, false>(x, per, W, pick_, pick_.count[0], 0.0, [&](int rank, const Item& t) {
+    seg_of[rank] = t.at;
+    if (rank == W - 1) bar = t.key;
+  });
 
   // the best W candidates in them, 64 of a segment a wave's at a time; an index
   // is the beam and the token
@@ -464,7 +483,7 @@ __global__ __launch_bounds__(TH) void choose_kernel(BeamArgs a) {
       x[j].key = key_of(w, x[j].x);
     }
   }
-  pick<TH>(x, per, W, pick_, [&](int rank, const Item& t) {
+  pick<TH, true>(x, per, W, pick_, pick_.count[1], bar, [&](int rank, const Item& t) {
     const int w = t.at >> 16;
     parent[rank] = w;
     token[rank] = t.at & 0xffff;

@@ -353,3 +353,22 @@ def test_large_fp16_maximum(x):
     c.scores[:] = [0.0, -0.5]
     c.logits[:] = x
     c.check()
+
+
+@pytest.mark.parametrize("half", [False, True])
+def test_more_candidates_at_the_bar_than_there_is_room_for(half):
+    """All of the best segments' candidates equal; and fewer segments than
+    beams."""
+    r = np.random.default_rng(12)
+    c = Case(r, 2, 32, 20000, half, weights=False)
+    c.logits[:] = 1.5
+    c.scores[:] = -3
+    got = c.check()
+    assert got["tokens"].tolist() == list(range(32)) * 2
+    for beams, vocab in ((32, 7000), (32, 4097), (32, 900), (5, 900), (16, 3000)):
+        c = Case(r, 2, beams, vocab, half)
+        c.scores[:] = -np.inf
+        c.scores[[1, beams + 2]] = -1
+        c.check()
+        c.logits[:] = np.round(c.logits)      # many equal ones
+        c.check()
