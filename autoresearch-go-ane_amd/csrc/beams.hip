@@ -18,9 +18,9 @@
 //
 // What bounds it.  Much to read: the first launch, HBM (640 rows of 60011 fp16
 // logits, 77 MB, in 18.6 us, 4.1 TB/s) and then the second one's chain of
-// accesses and barriers, 17 us for 16 beams (of them 4 for histories of 2564
-// ids).  Little: the two launches' chains (4 rows of 32000 fp32 logits 3.3 and 6.7
-// us, 64 rows 4.0 and 8.0).
+// accesses and barriers, 15.8 us for 16 beams (of them 4 for histories of 2564
+// ids).  Little: the two launches' chains (4 rows of 32000 fp32 logits 3.3 and 6.0
+// us, 64 rows 4.0 and 7.7).
 #include <algorithm>
 
 #include "kv8.h"
@@ -335,10 +335,10 @@ __device__ __forceinline__ double log_of(double x) {
 }
 
 // A block per request.  What bounds it is the chain of its memory accesses:
-// everything that does not depend on a choice is on its way first.  Of 6.3 us for
-// 4 beams of 32000 (16 of 60011: 14.4) the loads take 1.3 (1.4), log sums 0.8
-// (1.9), segments' keys 0.3 (0.7), their choice 1.2 (2.3), candidates 0.7 (2.2),
-// their choice 1.3 (2.4), outputs and histories 0.7 (3.5).
+// everything that does not depend on a choice is on its way first.  Of 5.5 us for
+// 4 beams of 32000 (16 of 60011: 13.3) the loads take 1.2 (1.3), log sums 0.8
+// (1.9), segments' keys 0.2 (0.6), their choice 1.2 (2.0), candidates 0.7 (2.2),
+// their choice 0.7 (1.5), outputs and histories 0.7 (3.8).
 template <typename T, int TH>
 __global__ __launch_bounds__(TH) void choose_kernel(BeamArgs a) {
   constexpr int NW = TH / 64, MB = Pick<TH>::kBeams;
@@ -595,9 +595,10 @@ int plan(const char* op, int requests, int beams, int vocab, bool half, Plan* p)
 
 uint32_t magic(int n) { return (uint32_t)(((1ull << 32) + n - 1) / n); }
 
-// 512 threads for up to 8 beams, 1024 for more (4 beams of 32000, 16 requests, 11.4
-// us a step, with 256 threads 12.4, with 1024 12.3; 8 of 60011 14.9, 18.1 and 14.7;
-// 12 of 32000 17.9 with 512, 17.1 with 1024).
+// 512 threads for up to 8 beams, 1024 for more (before the second choice knew its
+// bar: 4 beams of 32000, 16 requests, 11.4 us a step, with 256 threads 12.4, with
+// 1024 12.3; 8 of 60011 14.9, 18.1 and 14.7; 12 of 32000 17.9 with 512, 17.1 with
+// 1024).
 template <typename T>
 void launch_choose(const BeamArgs& a, int requests, hipStream_t st) {
   if (a.beams <= 8) hipLaunchKernelGGL((choose_kernel<T, 512>), dim3(requests), dim3(512), 0, st, a);
