@@ -165,8 +165,11 @@ struct ForkArgs {
   int stride, width, nseq, new_tokens;
   int* mid;    // [nseq][width]: the parents' rows (unused where there are no parents)
   Next* next;  // [nseq]
-  int* free;   // [pages]: free pages by rank
-  int* found;  // how many of them there are, of those that are wanted
+  int* free;    // [pages]: free pages by rank
+  int* found;   // how many of them there are, of those that are wanted
+  int* want;    // of a large pool: how many are
+  int* counts;  // and how many each chunk has
+  int chunks;
 };
 
 // One block does the tables by itself where they are small: their entries are
@@ -329,7 +332,8 @@ __device__ __forceinline__ int find_free(const ForkArgs& a, int want, int (&sums
 // A block ranks all of them without another launch (384 sequences in 5.0 us,
 // most of it waits for loads and atomics).  SMALL: also the rows before that, and
 // the table behind it, in one launch in place of two.
-template <bool SMALL>
+// FIND: and the free pages; otherwise the launches behind it do.
+template <bool SMALL, bool FIND>
 __global__ __launch_bounds__(kTh) void plan_kernel(ForkArgs a) {
   __shared__ int sums[kTh / 64];
   __shared__ Writers writers;
@@ -408,6 +412,13 @@ __global__ __launch_bounds__(kTh) void plan_kernel(ForkArgs a) {
   }
   if (lost) atomicAdd(&lost_all, lost);
   settle();
+  if constexpr (!FIND) {
+    if (tid == 0) {
+      *a.want = want;
+      *a.missing = lost_all;
+    }
+    return;
+  }
   const int found = find_free(a, want, sums);
   if (tid == 0) {
     *a.found = found;
@@ -426,6 +437,57 @@ __global__ __launch_bounds__(kTh) void plan_kernel(ForkArgs a) {
     }
     if (tid < a.nseq) a.start[tid] = st;
   }
+}
+
+// The free (or held) pages of each chunk, a block a chunk.
+__global__ __launch_bounds__(kTh) void count_kernel(const int* refs, int pages, bool held, int* counts) {
+  __shared__ int sums[kTh / 64];
+  int n = 0;
+#pragma unroll
+  for (int u = 0; u < 4; u++) {
+    const int64_t p = (int64_t)blockIdx.x * kChunk + u * kTh + threadIdx.x;
+    n += p < pages && (refs[p] > 0) == held;
+  }
+  int all;
+  block_scan(n, sums, all);
+  if (threadIdx.x == 0) counts[blockIdx.x] = all;
+}
+
+// What find_free does, of a large pool: a block a chunk, which adds up the counts
+// of all.
+__global__ __launch_bounds__(kTh) void list_kernel(ForkArgs a) {
+  __shared__ int sums[kTh / 64];
+  const int tid = threadIdx.x, want = *a.want;
+  int n = 0, m = 0, all, before;
+  for (int b = tid; b < a.chunks; b += kTh) {
+    const int c = a.counts[b];
+    n += c;
+    m += b < (int)blockIdx.x ? c : 0;
+  }
+  block_scan(m, sums, before);
+  if (blockIdx.x == 0) {
+    block_scan(n, sums, all);
+    if (tid == 0) {
+      *a.found = min(all, want);
+      *a.missing += want - min(all, want);
+    }
+  }
+  if (before >= want) return;
+  const int64_t p0 = (int64_t)blockIdx.x * kChunk + tid * 4;
+  int is[4];
+  n = 0;
+#pragma unroll
+  for (int u = 0; u < 4; u++) {
+    is[u] = p0 + u < a.p.pages && a.refs[p0 + u] <= 0;
+    n += is[u];
+  }
+  int rank = before + block_scan(n, sums, all);
+#pragma unroll
+  for (int u = 0; u < 4; u++)
+    if (is[u]) {
+      if (rank < want) a.free[rank] = (int)(p0 + u);
+      rank++;
+    }
 }
 
 // The tables' entries and starts, a thread an entry (table_blocks of them);
@@ -462,19 +524,6 @@ struct CompactArgs {
   int* code;            // [pages]: where a page is then; -1 free; -2 - k: it is the k-th that goes
   int *holes, *movers;  // [pages / 2 + 1]
 };
-
-__global__ __launch_bounds__(kTh) void count_kernel(CompactArgs a) {
-  __shared__ int sums[kTh / 64];
-  int n = 0;
-#pragma unroll
-  for (int u = 0; u < 4; u++) {
-    const int64_t p = (int64_t)blockIdx.x * kChunk + u * kTh + threadIdx.x;
-    n += p < a.p.pages && a.refs[p] > 0;
-  }
-  int all;
-  block_scan(n, sums, all);
-  if (threadIdx.x == 0) a.counts[blockIdx.x] = all;
-}
 
 // Ranks: a block a chunk, which adds up the counts of all (of one chunk, its
 // own).
@@ -643,15 +692,22 @@ int check_table(const char* op, const int* table, int stride, int width, int nse
 
 int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }
 
+// Of larger pools the free pages are found by a block a chunk (100,000 pages, nine
+// tenths held, 12 us a fork, by the block of the plan 34; 20,000 12 and 11.7).
+constexpr int kLarge = 20480;
+
 struct ForkPlan {
-  int64_t next, mid, free, bytes;  // offsets; found comes first
+  int chunks;
+  int64_t next, mid, free, counts, bytes;  // offsets; found and want come first
 };
 ForkPlan fork_plan(const Pool& p, int nseq, int width) {
   ForkPlan w;
   w.next = 16;
   w.mid = w.next + (int64_t)nseq * sizeof(Next);
   w.free = w.mid + up16((int64_t)nseq * width * 4);
-  w.bytes = w.free + up16((int64_t)p.pages * 4);
+  w.chunks = p.pages > kLarge ? (int)(((int64_t)p.pages + kChunk - 1) / kChunk) : 0;
+  w.counts = w.free + up16((int64_t)p.pages * 4);
+  w.bytes = w.counts + up16((int64_t)w.chunks * 4);
   return w;
 }
 struct CompactPlan {
@@ -727,17 +783,24 @@ extern "C" int ane_kv8_fork(const ane_kv8_pool* pool, const ane_kv8_fork_args* a
   a.stride = g.table_stride; a.width = g.table_pages; a.nseq = g.nseq; a.new_tokens = g.new_tokens;
   char* ws = (char*)g.ws;
   a.found = (int*)ws;
+  a.want = a.found + 1;
+  a.counts = (int*)(ws + w.counts);
+  a.chunks = w.chunks;
   a.next = (Next*)(ws + w.next);
   a.mid = (int*)(ws + w.mid);
   a.free = (int*)(ws + w.free);
   const hipStream_t st = (hipStream_t)stream;
   const int table_blocks = a.nseq * ((a.width + 255) / 256);
-  const bool small = small_table(a.nseq, a.width);
+  const bool large = a.chunks > 0 && a.nseq > 0, small = !large && small_table(a.nseq, a.width);
   if (small) {
-    hipLaunchKernelGGL(plan_kernel<true>, dim3(1), dim3(kTh), 0, st, a);
+    hipLaunchKernelGGL((plan_kernel<true, true>), dim3(1), dim3(kTh), 0, st, a);
   } else {
     hipLaunchKernelGGL(rows_kernel, dim3(table_blocks), dim3(256), 0, st, a);
-    hipLaunchKernelGGL(plan_kernel<false>, dim3(1), dim3(kTh), 0, st, a);
+    hipLaunchKernelGGL((large ? plan_kernel<false, false> : plan_kernel<false, true>), dim3(1), dim3(kTh), 0, st, a);
+  }
+  if (large) {
+    hipLaunchKernelGGL(count_kernel, dim3(a.chunks), dim3(kTh), 0, st, a.refs, a.p.pages, false, a.counts);
+    hipLaunchKernelGGL(list_kernel, dim3(a.chunks), dim3(kTh), 0, st, a);
   }
   for (int l0 = 0; l0 < pool->nlayers && a.nseq > 0; l0 += kMaxLayers) {
     Layers x;
@@ -785,7 +848,7 @@ extern "C" int ane_kv8_compact(const ane_kv8_pool* pool, const ane_kv8_compact_a
   a.holes = (int*)(ws + w.holes);
   a.movers = (int*)(ws + w.movers);
   const hipStream_t st = (hipStream_t)stream;
-  if (a.chunks > 1) hipLaunchKernelGGL(count_kernel, dim3(a.chunks), dim3(kTh), 0, st, a);
+  if (a.chunks > 1) hipLaunchKernelGGL(count_kernel, dim3(a.chunks), dim3(kTh), 0, st, a.refs, a.p.pages, true, a.counts);
   hipLaunchKernelGGL(rank_kernel, dim3(a.chunks), dim3(kTh), 0, st, a);
   const int book = (int)(((int64_t)a.p.pages + (int64_t)a.nseq * a.width + 255) / 256);
   for (int l0 = 0; l0 < pool->nlayers; l0 += kMaxLayers) {

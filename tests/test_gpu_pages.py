@@ -390,3 +390,23 @@ def test_copies_of_more_pages_than_a_launch_takes():
     dst[at] = [1, 3, 2, 0]
     copy_pages(a, b, src, dst, None)
     copy_pages(b, a, src, dst, r.integers(0, 17, n))
+
+
+@pytest.mark.parametrize("pages", [20480, 20481, 24576, 41000])
+def test_large_pools(pages):
+    """Hardly any page is free, and those lie far apart, or at the end; then none
+    is; fewer and more sequences than a block has threads."""
+    r = np.random.default_rng(pages)
+    pool = Pool(r, pages, 1, 1)
+    for requests, each, width, free in ((4, 3, 6, 40), (4, 3, 6, 5), (300, 4, 4, 4000), (300, 4, 4, 300)):
+        lens = r.integers(1, 3 * 16, requests)
+        table, start, refs = beams(r, 16, requests, width, lens, each, pages)
+        others = np.ones(pages, int)
+        others[r.permutation(pages)[:free] if free != 300 else slice(-free, None)] = 0
+        refs = refs + others
+        n = len(start)
+        for parents in (None, np.repeat(np.arange(requests) * each, each)):
+            new = r.integers(0, 40, n)
+            table, start, refs, missing, _ = run_fork(pool, table, start, refs, parents, new)
+            start = np.minimum(start + new, width * 16).astype(np.int32)
+        assert (missing > 0) == (free in (5, 300))
