@@ -807,12 +807,16 @@ int plan(const char* op, const Kv8Batch& b, const ane_kv8_batch& given, int DH, 
     // named at random out of 125: 5 x 300 rows of 4 heads and 1536 keys 59 us, a
     // row a tile 100; 2 x 100 rows 22.9 and 27.2; 2 x 50 23.1 and 21.7; 4 x 200
     // of 256 keys 34 and 40, 4 x 50 24 and 20; head dimension 128, 4 x 100 of 2
-    // heads 31 and 47, 4 x 30 30 and 24), and for up to 4 heads a token (of 8, two
-    // tokens a tile: 2 x 100 rows 38 and 36).
+    // heads 31 and 47, 4 x 30 30 and 24).  Of 5 to 8 heads, two or three tokens a
+    // tile, from 1024 keys on (the attention of 5 x 200 rows of 8 heads and 1536 keys
+    // 41 us, a row a tile 52; of head dimension 128 86 and 120; named out of 470
+    // pages, which few tokens share, 2 x 100 rows 39 and 36; 31 x 38 rows of 640 keys
+    // 42 and 39).
     const int pages = ((given.max_len ? std::min(given.max_len, cap) : cap) + (1 << b.pshift) - 1) >> b.pshift;
     const int most = given.max_new ? given.max_new : (b.rows + b.nseq - 1) / b.nseq;
     const int64_t lists = (int64_t)b.rows * b.NKV;
-    if (G <= 4 && most > 1 && pages <= 8192 && 16 / G * count <= 2048 && lists >= 640 && lists * len * DH >= 48 << 20) {
+    if (G <= (len < 1024 ? 4 : 8) && most > 1 && pages <= 8192 && 16 / G * count <= 2048 && lists >= 640 &&
+        lists * len * DH >= 48 << 20) {
       p->tt = 16 / G;
       p->room = pages;
     }

@@ -567,3 +567,18 @@ def test_long_contexts_in_parts_captured():
         x.bounds.Select(x.batch, q, 33, blocks=b)
         torch.cuda.synchronize()
         assert torch.equal(got, b) and (b[:2] >= -1).all() and (b[2:] == -7).all()
+
+
+@pytest.mark.parametrize("heads, kvh, dh, P, count, lens", [
+    (40, 8, 64, 128, 8, [(128 * 20, 70), (5, 31)]),             # three tokens a tile
+    (48, 8, 128, 64, 16, [(64 * 40 + 3, 50), (0, 1), (900, 52)]),
+    (32, 4, 64, 256, 6, [(256 * 9 + 200, 161), (1, 40)]),
+])
+def test_chunks_of_wide_groups_share_pages(heads, kvh, dh, P, count, lens):
+    r = np.random.default_rng(heads + P)
+    x = Run(r, lens, heads, kvh, dh, P, nan=3e-6).go()
+    b = lists(r, x, count)
+    b[x.rows // 2] = -1
+    b[:20, 1] = -1
+    b[5, 0, :2] = 1                       # twice
+    x.attend(b)
