@@ -100,9 +100,9 @@ __device__ __forceinline__ bool proposes(const BeamArgs& a, int r) {
   return !(a.finished && a.finished[r]) && a.scores[r] > -INFINITY && (!a.weights || a.weights[r] > 0.f);
 }
 
-// A wave takes U loads of 64 N entries of a row, all under way at once: a wave
-// that took more would have fewer beside it, and a row's waves need not meet.  A
-// lane whose N reach past the
+// A wave takes U loads of 64 N entries of a row, all under way at once: waves that
+// take several such turns, the next one's loads under way, are no faster (33.3 to
+// 39.0 us a step for 640 rows of 60011, one turn 32.0).  A lane whose N reach past the
 // row's end takes the row's last N instead, and of those its own; rows of fewer
 // than N are read one by one.
 template <typename T, int U>
