@@ -410,3 +410,36 @@ def test_large_pools(pages):
             table, start, refs, missing, _ = run_fork(pool, table, start, refs, parents, new)
             start = np.minimum(start + new, width * 16).astype(np.int32)
         assert (missing > 0) == (free in (5, 300))
+
+
+def test_captured_forks_in_a_large_pool():
+    r = np.random.default_rng(31)
+    pages, P, width = 20500, 16, 5
+    c = Pool(r, pages, 1, 1)
+    refs, table, start = (torch.zeros(n, dtype=torch.int32, device=DEV) for n in (pages, (24, width), 24))
+    parents, missing = torch.zeros(24, dtype=torch.int32, device=DEV), torch.zeros(1, dtype=torch.int32, device=DEV)
+    p = ane.KVPages(c.caches, refs)
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        p.Fork(table, start, parents=parents, new=20, missing=missing)
+        stream.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            p.Fork(table, start, parents=parents, new=20, missing=missing)
+    for i in range(4):
+        t, s, f = beams(r, P, 6, width, r.integers(1, 3 * P, 6), 4, pages)
+        others = (r.random(pages) < (0.99, 1.0, 0.9, 0.999)[i]).astype(int)
+        f = f + others
+        q = np.repeat(np.arange(6) * 4, 4) + r.integers(0, 4, 24)
+        for x, y in ((table, t), (start, s), (refs, f), (parents, q)):
+            x.copy_(dev(y, np.int32))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        wt, ws, wr, wm, _ = ref.fork(t, s, f, P, q, [20] * 24)
+        np.testing.assert_array_equal(table.cpu().numpy(), wt)
+        np.testing.assert_array_equal(start.cpu().numpy(), ws)
+        np.testing.assert_array_equal(refs.cpu().numpy(), wr)
+        assert int(missing) == wm and (wm > 0) == (i in (1, 3))
+        p.Fork(table, start, parents=parents, new=1)      # eager between the replays
+        torch.cuda.synchronize()
