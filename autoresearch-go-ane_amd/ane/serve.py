@@ -461,6 +461,8 @@ class BeamSearch:
             hp, hr, hn, most = _matrix(op, "history", history, self._u16, index)
             if hn != rows:
                 _fail(op, f"history has {hn} rows, want {rows}")
+            if most > 1 << 30:
+                _fail(op, f"history has {most} places a row, want at most {1 << 30}")
             np_ = vector("lengths", lengths, self._i32, index, rows)
         tp = tokens.data_ptr() if given[0] is None else vector("tokens", tokens, self._i32, index, rows)
         pp = parents.data_ptr() if given[1] is None else vector("parents", parents, self._i32, index, rows)

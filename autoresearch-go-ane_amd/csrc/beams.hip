@@ -40,6 +40,9 @@ constexpr int kMoved = 8;       // words a thread of it moves
 // It has 32 threads a beam, or more: enough for the segments of a beam, and for
 // one segment.
 static_assert(65536 / kSeg <= 32 * kPer && kSeg <= 32 * kPer, "");
+// Ids of a history: places in it, and those that the last words and stretches
+// reach to behind its end, are 32-bit numbers.
+constexpr int kMaxHistory = 1 << 30;
 
 // a wave's part of a row's log sum
 struct Part {
@@ -633,6 +636,8 @@ extern "C" int ane_beam_select(const ane_beam_args* args, void* stream) {
   if ((g.history && !g.lengths) || g.history_max < 0 || (g.history ? g.history_row < g.history_max : g.history_max > 0))
     return op_fail(ANE_ERR_ARG, "storiesane %s: history without lengths, or not of history_max=%d within its stride %lld",
                    op, g.history_max, (long long)g.history_row);
+  if (g.history_max > kMaxHistory)
+    return op_fail(ANE_ERR_ARG, "storiesane %s: history_max=%d want at most %d", op, g.history_max, kMaxHistory);
   if (g.logits_row < g.vocab)
     return op_fail(ANE_ERR_ARG, "storiesane %s: logits_row=%lld is shorter than vocab=%d", op, (long long)g.logits_row,
                    g.vocab);
@@ -649,7 +654,7 @@ extern "C" int ane_beam_select(const ane_beam_args* args, void* stream) {
                             {"parents", flat(g.parents, rows * 4), true},
                             {"scores_out", flat(g.scores_out, rows * 4), true, 1},
                             {"finished_out", flat(g.finished_out, rows), true, 2},
-                            {"history", row_major(g.history, rows, g.history_row * 2, g.history_max * 2), true},
+                            {"history", row_major(g.history, rows, g.history_row * 2, g.history_max * 2ll), true},
                             {"lengths", flat(g.lengths, rows * 4), true}};
   rc = check_apart(op, buffers, sizeof buffers / sizeof *buffers);
   if (rc) return rc;
@@ -670,7 +675,7 @@ extern "C" int ane_beam_select(const ane_beam_args* args, void* stream) {
   // Histories of up to 8 words a thread move in the second launch (40 requests of
   // 16 beams and 2564 ids: 35.6 us a step, in a launch of their own 37.8).
   const int threads = g.beams <= 8 ? 512 : 1024;
-  a.moves = g.beams * a.words > kMoved * threads ? (Move*)((char*)g.ws + p.seg_bytes) : nullptr;
+  a.moves = (int64_t)g.beams * a.words > kMoved * threads ? (Move*)((char*)g.ws + p.seg_bytes) : nullptr;
   a.part = (Part*)((char*)g.ws + p.seg_bytes + p.move_bytes);
   const hipStream_t st = (hipStream_t)stream;
   const dim3 grid((p.parts + 3) / 4, (uint32_t)rows);

@@ -197,7 +197,7 @@ int ane_control_logits(const ane_logits_args *args, void *stream);
  *                     history_max].
  * weights NULL: 1.  finished NULL with finished_out NULL and eos -1: beams do
  * not finish.  history and lengths NULL: no histories
- * (history NULL, history_max 0, with lengths: empty ones).
+ * (history NULL, history_max 0, with lengths: empty ones); history_max at most 2^30.
  * beams 1..32, vocab 1..65535, at most 65535 rows.  logits: row stride
  * logits_row; history: uint16, row stride history_row.  Outputs share no memory
  * with each other or with inputs but where said.  ws as above. */
