@@ -101,21 +101,23 @@ __device__ __forceinline__ ushort8u first_ids(const LogitsArgs& a, const Row& w)
     if (j + u < a.history_max) h[u] = w.hist[j + u];
   return h;
 }
-// count(j, id) for the row's ids
+// count(j, id) for the row's ids; a step behind the last one of the longest
+// history passes 2^31
 template <int TH, typename F>
 __device__ __forceinline__ void for_history(const Row& w, const ushort8u& first, F count) {
-  int j = threadIdx.x * 8;
+  const uint32_t len = w.len;
+  uint32_t j = threadIdx.x * 8;
 #pragma unroll
   for (int u = 0; u < 8; u++)
-    if (j + u < w.len) count(j + u, first[u]);
-  for (j += TH * 8; j < w.len; j += TH * 8) {
-    if (j + 7 < w.len) {
+    if (j + u < len) count(j + u, first[u]);
+  for (j += TH * 8; j < len; j += TH * 8) {
+    if (j + 7 < len) {
       const ushort8u h = *reinterpret_cast<const ushort8u*>(w.hist + j);
 #pragma unroll
       for (int u = 0; u < 8; u++) count(j + u, h[u]);
     } else {
       for (int u = 0; u < 7; u++)
-        if (j + u < w.len) count(j + u, w.hist[j + u]);
+        if (j + u < len) count(j + u, w.hist[j + u]);
     }
   }
 }
