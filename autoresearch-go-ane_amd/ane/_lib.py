@@ -270,6 +270,11 @@ SIGNATURES = {
     "ane_debug_kv8_item": (C.c_int, [C.POINTER(Kv8Cache), C.POINTER(Kv8Batch), C.c_int32, C.c_int32, C.c_int64,
                                      C.POINTER(C.c_int32)]),
     "ane_debug_share_memory": (C.c_int, [C.POINTER(C.c_int64), C.POINTER(C.c_int64)]),
+    "ane_debug_kv8_select_form": (C.c_int, [C.POINTER(Kv8Cache), C.POINTER(Kv8Batch), C.c_int32, C.POINTER(C.c_int32)]),
+    "ane_debug_kv8_attend_form": (C.c_int, [C.POINTER(Kv8Cache), C.POINTER(Kv8Batch), C.c_int32, C.c_int32,
+                                            C.POINTER(C.c_int32)]),
+    "ane_debug_kv8_copy_form": (C.c_int, [C.POINTER(Kv8Pool), C.c_int32, C.POINTER(C.c_int32)]),
+    "ane_debug_beam_form": (C.c_int, [C.c_int32] * 5 + [C.POINTER(C.c_int32)]),
     # the per-object seam (include/ane_objects.h)
     "ane_seam_last_error": (C.c_char_p, []),
     "ane_layer_forward_open": (C.c_int, [C.c_int32] * 4 + [C.POINTER(LayerWeights), C.POINTER(C.c_void_p)]),

@@ -602,9 +602,14 @@ uint32_t magic(int n) { return (uint32_t)(((1ull << 32) + n - 1) / n); }
 // bar: 4 beams of 32000, 16 requests, 11.4 us a step, with 256 threads 12.4, with
 // 1024 12.3; 8 of 60011 14.9, 18.1 and 14.7; 12 of 32000 17.9 with 512, 17.1 with
 // 1024).
+int threads_of(int beams) { return beams <= 8 ? 512 : 1024; }
+// Histories of up to 8 words a thread move in the second launch (40 requests of
+// 16 beams and 2564 ids: 35.6 us a step, in a launch of their own 37.8).
+bool moves_apart(int beams, int words) { return (int64_t)beams * words > kMoved * threads_of(beams); }
+
 template <typename T>
 void launch_choose(const BeamArgs& a, int requests, hipStream_t st) {
-  if (a.beams <= 8) hipLaunchKernelGGL((choose_kernel<T, 512>), dim3(requests), dim3(512), 0, st, a);
+  if (threads_of(a.beams) == 512) hipLaunchKernelGGL((choose_kernel<T, 512>), dim3(requests), dim3(512), 0, st, a);
   else hipLaunchKernelGGL((choose_kernel<T, 1024>), dim3(requests), dim3(1024), 0, st, a);
 }
 
@@ -672,10 +677,7 @@ extern "C" int ane_beam_select(const ane_beam_args* args, void* stream) {
   a.words_magic = a.words ? magic(a.words) : 0;
   a.segs_magic = magic(a.segs);
   a.stretch = kWords / g.beams;
-  // Histories of up to 8 words a thread move in the second launch (40 requests of
-  // 16 beams and 2564 ids: 35.6 us a step, in a launch of their own 37.8).
-  const int threads = g.beams <= 8 ? 512 : 1024;
-  a.moves = (int64_t)g.beams * a.words > kMoved * threads ? (Move*)((char*)g.ws + p.seg_bytes) : nullptr;
+  a.moves = moves_apart(g.beams, a.words) ? (Move*)((char*)g.ws + p.seg_bytes) : nullptr;
   a.part = (Part*)((char*)g.ws + p.seg_bytes + p.move_bytes);
   const hipStream_t st = (hipStream_t)stream;
   const dim3 grid((p.parts + 3) / 4, (uint32_t)rows);
@@ -691,5 +693,19 @@ extern "C" int ane_beam_select(const ane_beam_args* args, void* stream) {
     hipLaunchKernelGGL(move_kernel, dim3((a.words + a.stretch - 1) / a.stretch, g.requests), dim3(256), 0, st, a);
   const hipError_t h = hipGetLastError();
   if (h != hipSuccess) return op_fail(ANE_ERR_HIP, "storiesane %s: %s", op, hipGetErrorString(h));
+  return ANE_OK;
+}
+
+extern "C" int ane_debug_beam_form(int32_t requests, int32_t beams, int32_t vocab, int32_t half, int32_t history_max,
+                                   int32_t* out) {
+  const char* op = "debug beam form";
+  Plan p;
+  const int rc = plan(op, requests, beams, vocab, half != 0, &p);
+  if (rc) return rc;
+  if (!out || history_max < 0 || history_max > kMaxHistory)
+    return op_fail(ANE_ERR_ARG, "storiesane %s: null buffer, or history_max=%d", op, history_max);
+  out[0] = p.loads;
+  out[1] = threads_of(beams);
+  out[2] = moves_apart(beams, (history_max + 7) / 8);
   return ANE_OK;
 }

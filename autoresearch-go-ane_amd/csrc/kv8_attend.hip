@@ -1081,3 +1081,22 @@ int ane::kv8_step(const ane_kv8_cache* cache, const ane_kv8_batch* batch, const 
   rc = kv8_append(cache, batch, append, from, stream);
   return rc ? rc : attend(cache, batch, args, frag, nullptr, nullptr, stream);
 }
+
+extern "C" int ane_debug_kv8_attend_form(const ane_kv8_cache* cache, const ane_kv8_batch* batch, int32_t heads,
+                                         int32_t count, int32_t* out) {
+  const char* op = "debug kv8 attend form";
+  Kv8Batch b;
+  int rc = kv8_check(op, cache, batch, &b);
+  if (!rc && count) rc = check_count(op, count);
+  Plan p;
+  if (!rc) rc = plan(op, b, *batch, cache->head_dim, heads, count, &p);
+  if (rc) return rc;
+  if (!out) return op_fail(ANE_ERR_ARG, "storiesane %s: null buffer", op);
+  out[0] = p.nt;
+  out[1] = p.tt;
+  out[2] = p.kw;
+  out[3] = p.nsplit;
+  out[4] = p.longest;
+  out[5] = p.room;
+  return ANE_OK;
+}

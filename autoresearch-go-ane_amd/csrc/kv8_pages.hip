@@ -899,3 +899,15 @@ extern "C" int ane_kv8_copy(const ane_kv8_pool* from, const ane_kv8_pool* into, 
   }
   return launched(op);
 }
+
+extern "C" int ane_debug_kv8_copy_form(const ane_kv8_pool* pool, int32_t pages, int32_t* out) {
+  const char* op = "debug kv8 copy form";
+  Pool p;
+  const int rc = check_pool(op, pool, false, &p);
+  if (rc) return rc;
+  if (!out || pages < 0 || pages > 1 << 24) return op_fail(ANE_ERR_ARG, "storiesane %s: null buffer, or pages=%d", op, pages);
+  const int n = std::min(kMaxLayers, pool->nlayers);
+  out[0] = pages * bytes_of(p, n) >= kFar;
+  out[1] = group_of(p, pages, n);
+  return ANE_OK;
+}

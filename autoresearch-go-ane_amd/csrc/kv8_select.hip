@@ -674,6 +674,9 @@ int check_sizes(const char* op, const Kv8Batch& b, const ane_kv8_batch& batch, i
   return ANE_OK;
 }
 
+// scores that a block's LDS holds, of contexts as long as the host knows
+int room_of(int tok, int pages) { return std::min(tok * ((pages + 63) & ~63), kFar); }
+
 template <int DH, int NT>
 void launch_parts(const SelectArgs& a, int pages, hipStream_t st) {
   const uint32_t lists = kv8_count(a.b.nseq, a.b.rows, kv8_tiles(1)) * a.b.NKV;
@@ -686,7 +689,7 @@ void launch_parts(const SelectArgs& a, int pages, hipStream_t st) {
 template <int DH, int NT, int TOK, int NW, int CW>
 int launch_form(const char* op, SelectArgs a, int pages, hipStream_t st) {
   auto* const kernel = select_kernel<DH, NT, TOK, NW, CW, false>;
-  a.room = std::min(TOK * ((pages + 63) & ~63), kFar);
+  a.room = room_of(TOK, pages);
   const int lds = a.room * 4;
   if (lds > 32768) {
     const hipError_t e = taken(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
@@ -794,5 +797,22 @@ extern "C" int ane_kv8_select(const ane_kv8_cache* cache, const ane_kv8_bounds* 
   if (rc) return rc;
   const hipError_t h = hipGetLastError();
   if (h != hipSuccess) return op_fail(ANE_ERR_HIP, "storiesane %s: %s", op, hipGetErrorString(h));
+  return ANE_OK;
+}
+
+extern "C" int ane_debug_kv8_select_form(const ane_kv8_cache* cache, const ane_kv8_batch* batch, int32_t heads,
+                                         int32_t* out) {
+  const char* op = "debug kv8 select form";
+  Kv8Batch b;
+  int rc = kv8_check(op, cache, batch, &b);
+  if (!rc) rc = check_sizes(op, b, *batch, cache->head_dim, heads, 1);
+  if (rc) return rc;
+  if (!out) return op_fail(ANE_ERR_ARG, "storiesane %s: null buffer", op);
+  const Form f = form_of(b, *batch, cache->head_dim, heads / b.NKV);
+  out[0] = f.nt;
+  out[1] = f.tok;
+  out[2] = f.waves;
+  out[3] = f.parts;
+  out[4] = f.parts ? 0 : room_of(f.tok, pages_of(b, *batch));
   return ANE_OK;
 }

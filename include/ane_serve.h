@@ -362,6 +362,27 @@ int ane_debug_kv8_item(const ane_kv8_cache *cache, const ane_kv8_batch *batch, i
  * used. */
 int ane_debug_share_memory(const int64_t *a, const int64_t *b);
 
+/* The form that a call of these sizes takes, by the operators' own rules, so that
+ * a test that is to reach a form can ask for it.  No GPU is used, no address
+ * followed; ANE_OK, or what the call itself would refuse.
+ * select: {tiles of 16 query rows, tokens a block, waves a block, 1: the choice
+ *   has a launch of its own, scores that LDS holds}
+ * attend, count 0: all pages, else a list of so many: {tiles of 16 rows, tokens
+ *   a tile, waves that share its keys, parts of the keys at most, 1: the longest
+ *   contexts first, places that a union of lists has masks of (0: a list a
+ *   tile)}
+ * copy, also of so many pages that a compaction moves: {1: past the caches;
+ *   sides (keys or values of a layer) a block of ane_kv8_copy takes}; of the
+ *   first 32 layers
+ * beam: {loads of a wave of the first launch, threads of the second one, 1:
+ *   histories have a launch of their own} */
+int ane_debug_kv8_select_form(const ane_kv8_cache *cache, const ane_kv8_batch *batch, int32_t heads, int32_t *out);
+int ane_debug_kv8_attend_form(const ane_kv8_cache *cache, const ane_kv8_batch *batch, int32_t heads, int32_t count,
+                              int32_t *out);
+int ane_debug_kv8_copy_form(const ane_kv8_pool *pool, int32_t pages, int32_t *out);
+int ane_debug_beam_form(int32_t requests, int32_t beams, int32_t vocab, int32_t half, int32_t history_max,
+                        int32_t *out);
+
 #ifdef __cplusplus
 }
 #endif

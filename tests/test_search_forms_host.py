@@ -1,9 +1,12 @@
 """Limits of beam search and of the pages' operators at their largest sizes, and
 the forms that calls take, without a GPU."""
+import ctypes as C
+
 import pytest
 
+import search_forms as forms
 from ane import _lib
-from test_pages_host import beam, refused
+from test_pages_host import batch, beam, cache, pool, refused
 
 lib = _lib.load()
 
@@ -23,3 +26,27 @@ def test_long_histories_that_overlap_an_input():
     for other in ("logits", "scores", "weights"):
         refused(beam(history_max=most, history_row=most, requests=1, beams=1, history=at, **{other: at + 2 * most - 400}),
                 "overlaps")
+
+
+@pytest.mark.parametrize("case", forms.SELECT, ids=forms.name_of)
+def test_shapes_take_the_forms_of_the_choice_that_they_are_for(case):
+    shape, want, scores = case
+    got = forms.select_form(**shape)
+    assert got[:4] == want
+    assert forms.where_scores_are(shape, got) == scores
+
+
+def test_forms_refuse_what_the_calls_refuse():
+    out = (C.c_int32 * 6)()
+    refused(lib.ane_debug_kv8_select_form(cache(), batch(), 3, out), "heads=3")
+    refused(lib.ane_debug_kv8_select_form(cache(page_tokens=48), batch(), 4, out), "page_tokens=48")
+    refused(lib.ane_debug_kv8_select_form(cache(), batch(), 4, None), "null")
+    refused(lib.ane_debug_kv8_attend_form(cache(), batch(), 5, 7, out), "heads=5")
+    refused(lib.ane_debug_kv8_attend_form(cache(), batch(), 4, 70000, out), "count=70000")
+    refused(lib.ane_debug_kv8_attend_form(cache(), batch(), 4, 7, None), "null")
+    refused(lib.ane_debug_kv8_copy_form(pool([cache(), cache(pages=5)]), 4, out), "layer 1 differs")
+    refused(lib.ane_debug_kv8_copy_form(pool(), -1, out), "pages=-1")
+    refused(lib.ane_debug_kv8_copy_form(pool(), 4, None), "null")
+    refused(lib.ane_debug_beam_form(1, 33, 100, 0, 5, out), "beams=33")
+    refused(lib.ane_debug_beam_form(1, 3, 100, 0, (1 << 30) + 1, out), "history_max")
+    refused(lib.ane_debug_beam_form(1, 3, 100, 0, 5, None), "null")
