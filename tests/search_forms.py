@@ -96,3 +96,43 @@ def where_scores_are(shape, form):
 def name_of(case):
     shape, form, *rest = case
     return "-".join([f"{shape['heads']}-{shape['kvh']}-{shape['dh']}", *(str(x) for x in form), *(str(x) for x in rest)])
+
+
+def attend_form(lens, heads, kvh, dh, P, count, spare=1, rows_behind=2, **hints):
+    """(tiles of 16 rows, tokens a tile, waves on its keys, parts, longest first, places with masks)"""
+    return _form(6, lib.ane_debug_kv8_attend_form, _cache(kvh, dh, P),
+                 _batch(lens, width_of(lens, P, spare), rows_behind, **hints), heads, count)
+
+
+# Attention over lists of `count` pages: the form as (tiles of 16 rows, whether tokens share a tile, waves, whether
+# its keys are cut, longest contexts first).
+ATTEND = [
+    # a wave a list, pages of at least a step's 32 keys and smaller ones
+    (dict(lens=[(700, 1)] * 201, heads=12, kvh=4, dh=64, P=32, count=7, max_new=1), (1, False, 1, False, 0)),
+    (dict(lens=[(400, 1)] * 101, heads=16, kvh=8, dh=128, P=16, count=10, max_new=1), (1, False, 1, False, 0)),
+    (dict(lens=[(500, 781)], heads=24, kvh=1, dh=128, P=64, count=5), (2, False, 1, False, 0)),
+    (dict(lens=[(900, 60), (3, 170), (0, 191)], heads=40, kvh=2, dh=64, P=16, count=13), (2, False, 1, False, 0)),
+    # lists that are cut, pages smaller than a step
+    (dict(lens=[(16 * 100, 1), (40, 2)], heads=16, kvh=2, dh=128, P=16, count=80), (1, False, 4, True, 0)),
+    (dict(lens=[(16 * 140, 1), (40, 2)], heads=40, kvh=2, dh=64, P=16, count=120), (2, False, 4, True, 0)),
+    (dict(lens=[(16 * 140, 1), (40, 2)], heads=40, kvh=2, dh=128, P=16, count=120), (2, False, 4, True, 0)),
+    # tiles over lists by four waves, in the batch's order and with the longest contexts first
+    (dict(lens=[(16 * 60 + 3, 200)], heads=32, kvh=8, dh=64, P=16, count=32), (1, True, 4, False, 0)),
+    (dict(lens=[(16 * 60 + 3, 90), (5, 60), (300, 50)], heads=32, kvh=8, dh=64, P=16, count=32), (1, True, 4, False, 1)),
+    (dict(lens=[(64 * 20 + 3, 220)], heads=32, kvh=8, dh=64, P=64, count=8), (1, True, 4, False, 0)),
+    (dict(lens=[(16 * 60 + 3, 90), (5, 60), (300, 50)], heads=32, kvh=8, dh=128, P=16, count=16), (1, True, 4, False, 1)),
+    (dict(lens=[(64 * 20 + 3, 90), (5, 60)], heads=40, kvh=8, dh=128, P=64, count=16), (1, True, 4, False, 1)),
+    # by eight
+    (dict(lens=[(16 * 60 + 3, 200)], heads=16, kvh=8, dh=64, P=16, count=32), (1, True, 8, False, 0)),
+    (dict(lens=[(64 * 20 + 3, 90), (5, 50), (300, 42)], heads=24, kvh=8, dh=64, P=64, count=9), (1, True, 8, False, 1)),
+    # a list a block, by eight and by four waves
+    (dict(lens=[(64 * 20 + 3, 1), (5, 2)], heads=12, kvh=4, dh=64, P=64, count=9), (1, False, 8, False, 0)),
+    (dict(lens=[(16 * 40 + 3, 5)], heads=6, kvh=2, dh=64, P=16, count=9), (1, False, 8, False, 0)),
+    (dict(lens=[(64 * 20 + 3, 1), (5, 2)], heads=12, kvh=4, dh=128, P=64, count=9), (1, False, 4, False, 0)),
+    (dict(lens=[(64 * 20 + 3, 1), (5, 2)], heads=40, kvh=2, dh=64, P=64, count=9), (2, False, 4, False, 0)),
+    (dict(lens=[(64 * 60 + 3, 1), (5, 2)], heads=4, kvh=4, dh=64, P=64, count=50), (1, False, 4, True, 0)),
+]
+
+
+def attend_kind(form):
+    return form[0], form[1] > 1, form[2], form[3] > 1, form[4]

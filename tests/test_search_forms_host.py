@@ -50,3 +50,9 @@ def test_forms_refuse_what_the_calls_refuse():
     refused(lib.ane_debug_beam_form(1, 33, 100, 0, 5, out), "beams=33")
     refused(lib.ane_debug_beam_form(1, 3, 100, 0, (1 << 30) + 1, out), "history_max")
     refused(lib.ane_debug_beam_form(1, 3, 100, 0, 5, None), "null")
+
+
+@pytest.mark.parametrize("case", forms.ATTEND, ids=forms.name_of)
+def test_shapes_take_the_forms_of_attention_that_they_are_for(case):
+    shape, want = case
+    assert forms.attend_kind(forms.attend_form(**shape)) == want
