@@ -136,3 +136,22 @@ ATTEND = [
 
 def attend_kind(form):
     return form[0], form[1] > 1, form[2], form[3] > 1, form[4]
+
+
+def copy_form(pages, layers, kvh, dh, P):
+    """(past the caches, sides a block) of a copy of so many pages"""
+    cache = _cache(kvh, dh, P)
+    pool = _lib.Kv8Pool((_lib.Kv8Cache * layers)(*[cache] * layers), None, AT, layers)
+    return _form(2, lib.ane_debug_kv8_copy_form, pool, pages)
+
+
+# Copies of so many pages, and whether they go past the caches: sides of 16 KB and more one a block, smaller ones
+# several.
+COPY = [
+    (dict(pages=3500, layers=2, kvh=4, dh=64, P=64), (1, 1)),
+    (dict(pages=400, layers=3, kvh=4, dh=128, P=256), (1, 1)),
+    (dict(pages=5000, layers=5, kvh=2, dh=64, P=32), (1, 4)),
+    (dict(pages=34000, layers=3, kvh=1, dh=64, P=16), (1, 6)),
+    (dict(pages=2000, layers=2, kvh=4, dh=64, P=64), (0, 1)),
+    (dict(pages=9000, layers=3, kvh=1, dh=64, P=16), (0, 6)),
+]

@@ -56,3 +56,9 @@ def test_forms_refuse_what_the_calls_refuse():
 def test_shapes_take_the_forms_of_attention_that_they_are_for(case):
     shape, want = case
     assert forms.attend_kind(forms.attend_form(**shape)) == want
+
+
+@pytest.mark.parametrize("case", forms.COPY, ids=str)
+def test_sizes_take_the_forms_of_copies_that_they_are_for(case):
+    size, want = case
+    assert forms.copy_form(**size) == want
