@@ -155,3 +155,29 @@ COPY = [
     (dict(pages=2000, layers=2, kvh=4, dh=64, P=64), (0, 1)),
     (dict(pages=9000, layers=3, kvh=1, dh=64, P=16), (0, 6)),
 ]
+
+
+def beam_form(requests, beams, vocab, half, hist, **_):
+    """(loads of a wave, threads of the second launch, histories in a launch of their own)"""
+    return _form(3, lib.ane_debug_beam_form, requests, beams, vocab, int(half), hist or 0)
+
+
+BEAMS = [
+    # four loads a wave: many fp32 logits, rows that end in a turn's first, second and third entry and elsewhere
+    (dict(requests=34, beams=8, vocab=32003, half=False, hist=40, eos=32002, masked=0.5), (4, 512, 0)),
+    (dict(requests=17, beams=16, vocab=32769, half=False, hist=None), (4, 1024, 0)),
+    (dict(requests=1025, beams=4, vocab=2049, half=False, hist=9, eos=2048), (4, 512, 0)),
+    (dict(requests=257, beams=16, vocab=2050, half=False, hist=600, eos=2049, masked=0.9), (4, 1024, 0)),
+    (dict(requests=5461, beams=1, vocab=2051, half=False, hist=3, eos=0), (4, 512, 0)),
+    (dict(requests=129, beams=32, vocab=2560, half=False, hist=5, eos=1), (4, 1024, 0)),
+    (dict(requests=2049, beams=8, vocab=513, half=False, hist=17), (4, 512, 0)),
+    (dict(requests=256, beams=2, vocab=16700, half=False, hist=4200, eos=3, wide=5), (4, 512, 0)),
+    # below that line
+    (dict(requests=1, beams=4, vocab=32000, half=False, hist=300, eos=2), (2, 512, 0)),
+    # fp16: histories read ahead, moved by the second launch, in one of their own
+    (dict(requests=34, beams=8, vocab=32003, half=True, hist=40, eos=32002), (2, 512, 0)),
+    (dict(requests=3, beams=4, vocab=700, half=True, hist=2600, eos=3), (2, 512, 0)),
+    (dict(requests=3, beams=16, vocab=700, half=True, hist=600, eos=3), (2, 1024, 0)),
+    (dict(requests=2, beams=16, vocab=700, half=True, hist=4300, eos=3, wide=3), (2, 1024, 1)),
+    (dict(requests=2, beams=5, vocab=700, half=True, hist=9000, wide=3), (2, 512, 1)),
+]

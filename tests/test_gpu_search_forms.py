@@ -1,12 +1,15 @@
-"""Forms of beam search, of the pages' copies and of the choice of pages that
-large batches take, against plain implementations."""
+"""Forms of beam search's step that large batches and long histories take, against
+a plain 64-bit implementation."""
 import numpy as np
 import pytest
+
+import search_forms as forms
 
 torch = pytest.importorskip("torch")
 pytestmark = [pytest.mark.gpu, pytest.mark.filterwarnings("ignore:overflow encountered", "ignore:invalid value")]
 
 import ane  # noqa: E402
+from test_gpu_beams import Case  # noqa: E402
 
 DEV = "cuda"
 
@@ -45,3 +48,15 @@ def test_longer_histories_are_refused(most):
     with pytest.raises(ane.EngineError, match="at most 1073741824"):
         ane.BeamSearch(50, 1).Select(torch.zeros((1, 50), device=DEV), torch.zeros(1, device=DEV), history=history,
                                      lengths=lengths)
+
+
+@pytest.mark.parametrize("case", forms.BEAMS, ids=str)
+def test_beam_step(case):
+    size, form = case
+    assert forms.beam_form(**size) == form
+    c = Case(np.random.default_rng(size["vocab"]), **size)
+    c.check(offset=1 if size.get("wide") else 0)
+    if size["hist"] is None:     # the last entries of a row, behind its last whole turn, are the best
+        c.logits[:, -1] = c.logits.max(1) + 2
+        got = c.check()
+        assert (got["tokens"] == size["vocab"] - 1).any()

@@ -62,3 +62,9 @@ def test_shapes_take_the_forms_of_attention_that_they_are_for(case):
 def test_sizes_take_the_forms_of_copies_that_they_are_for(case):
     size, want = case
     assert forms.copy_form(**size) == want
+
+
+@pytest.mark.parametrize("case", forms.BEAMS, ids=str)
+def test_sizes_take_the_forms_of_the_beam_step_that_they_are_for(case):
+    size, want = case
+    assert forms.beam_form(**size) == want
