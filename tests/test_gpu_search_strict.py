@@ -1,0 +1,50 @@
+"""What other tests of the search ask only in part: the entries of a sequence
+whose last page is not there, and every step of a search within one bound."""
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = [pytest.mark.gpu, pytest.mark.filterwarnings("ignore:overflow encountered", "ignore:invalid value")]
+
+import ane  # noqa: E402
+import test_gpu_search_run as run  # noqa: E402
+
+DEV = "cuda"
+
+
+def ids(x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+@pytest.mark.parametrize("other, pages", [(0, 12), (3, 21000)])   # by one block, and in a large pool
+def test_page_that_is_not_there_stays_so(other, pages):
+    """Its tokens are lost and count as missing; the ones behind them get a
+    page."""
+    cache = ane.KVCache8.Empty(pages, 1, 64, 16)
+    pool = ane.KVPages(([cache]), torch.zeros(pages, dtype=torch.int32, device=DEV))
+    pool.refs[4] = 1
+    pool.refs[:other] = 1
+    table, start = ids([[4, -1, -1]]), ids([20])
+    missing = pool.Fork(table, start, new=30)
+    assert missing.tolist() == [1]
+    assert table.tolist() == [[4, -1, other]]
+    assert start.tolist() == [20]
+    want = torch.zeros(pages, dtype=torch.int32, device=DEV)
+    want[4] = want[other] = 1
+    want[:other] = 1
+    assert torch.equal(pool.refs, want)
+
+
+@pytest.mark.parametrize("seed, beams, compact", [(0, 4, False), (1, 3, True), (2, 6, True)])
+def test_no_error_adds_up_over_a_search(monkeypatch, seed, beams, compact):
+    """Each step of the plain search starts from the scores and sequences of the
+    GPU's, so the first step's bound holds for all."""
+    real, steps = np.testing.assert_allclose, []
+
+    def close(a, b, atol):
+        steps.append(np.nanmax(np.abs(np.where(np.isfinite(b), a - b, 0))))
+        real(a, b, atol=min(atol, 2e-2))
+    monkeypatch.setattr(run.np.testing, "assert_allclose", close)
+    run.test_search(seed, beams, compact)
+    print("largest differences of a step:", " ".join(f"{x:.1e}" for x in steps))
+    assert len(steps) == 12
