@@ -175,7 +175,7 @@ int ane_control_logits(const ane_logits_args *args, void *stream);
 /* ---- beam search ---------------------------------------------------------------
  * One step of `requests` searches with `beams` beams each; row r = request *
  * beams + beam.  With x = logits (fp32, or fp16 where half is set) and NaN as
- * -inf, sums in 64 bits:
+ * -inf:
  *   lse[r] = log sum_v exp(x[r][v])
  *   s(r, v) = scores[r] + (x[r][v] - lse[r]),  key(r, v) = weights[r] * s(r, v)
  * and the request's `beams` candidates of the largest key become its next
@@ -183,6 +183,10 @@ int ane_control_logits(const ane_logits_args *args, void *stream);
  * that is finished has one candidate, itself: (r, eos) with s = scores[r].  No
  * candidate: keys that are -inf or NaN, rows with scores -inf or NaN, weights
  * that are not above 0, or +inf among their logits.
+ * s and keys are 64-bit; lse is the sum of fp32 exponentials, a row's off by at
+ * most (19 + 3 sum_v p(v) (max x - x(v))) 2^-24 with p = softmax(x), 2e-6 for
+ * logits of normal distribution.  Candidates of two beams whose keys lie closer
+ * together than that (times their weights) may change places.
  *   tokens, parents   the candidate's v and r (the row in the call, not within
  *                     the request); ANE_NO_TOKEN and -1 where there are not
  *                     enough candidates

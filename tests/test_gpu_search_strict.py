@@ -48,3 +48,25 @@ def test_no_error_adds_up_over_a_search(monkeypatch, seed, beams, compact):
     run.test_search(seed, beams, compact)
     print("largest differences of a step:", " ".join(f"{x:.1e}" for x in steps))
     assert len(steps) == 12
+
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("rows, vocab", [(256, 1000), (64, 32000), (300, 32000), (40, 60011), (3, 17)])
+def test_log_sums(rows, vocab, half):
+    """Scores that leave only the log sum's error, of rows of one beam each: s = scores + (max - lse) is about 0,
+    and what fp32 then rounds away is 2^-24 of it.
+
+    The bound, in half steps of fp32 (2^-24): the exponent is off by its difference's rounding, the constant's and the
+    product's, 3 |x - max|; each of two powers of two (a part's, and its factor) by 2; 15 additions of a lane."""
+    g = torch.Generator(device=DEV).manual_seed(vocab)
+    for scale in (0.3, 1.0, 3.0, 10.0):
+        x = torch.randn((rows, vocab), device=DEV, generator=g) * scale
+        x = x.half() if half else x
+        y = x.double()
+        top, lse = y.amax(1), torch.logsumexp(y, 1)
+        scores = (lse - top).float()
+        _, _, out = ane.BeamSearch(vocab, 1).Select(x, scores)
+        want = scores.double() + (top - lse)
+        p = torch.exp(y - lse[:, None])
+        bound = (19 + 3 * (p * (top[:, None] - y)).sum(1)) * 2.0 ** -24
+        assert ((out.double() - want).abs() <= bound + want.abs() * 2.0 ** -24).all()
