@@ -61,7 +61,9 @@ class KVBounds:
         key/value head the ``count`` pages of its sequence whose keys can match
         it best, the first ``first`` and the last ``recent`` pages always among
         them: blocks int32 [rows, kv_heads, count] (new if None: rows of no
-        sequence are then undefined), places in the table, rising, then -1."""
+        sequence are then undefined), places in the table, rising, then -1.
+        Bounds of a row's own page are of later tokens of the batch too: with
+        recent 0 a chunk may choose otherwise than token by token."""
         op = "kv8 select"
         c = self.cache
         c._batch(op, batch)
@@ -223,7 +225,8 @@ class KVPages:
         """Copies the pages src[i] to the pages dst[i] (int32 [n]) of ``into``
         (another pool of like layers; None: this one), in all layers: the
         16-token units of their first tokens[i] tokens (None: all).  Ids
-        outside the pools are passed over; refs stay as they are."""
+        outside the pools are passed over; refs stay as they are.  n is at
+        most 2**24."""
         op = "kv8 copy"
         to = self if into is None else into
         n = int(src.shape[0]) if hasattr(src, "shape") and src.dim() == 1 else 0

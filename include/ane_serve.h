@@ -227,7 +227,10 @@ int ane_beam_select(const ane_beam_args *args, void *stream);
  * For each page and key/value head, of the keys it holds: unit, the smallest
  * exponent e >= -30 at which every |k| <= 127 * 2^e, and box [2][head_dim], the
  * largest (first) and smallest key of each dimension in that unit, rounded
- * outwards.  NaN does not count; a dimension without a number has 0 and 0. */
+ * outwards.  NaN does not count; a dimension without a number has 0 and 0.
+ * They are as the last update left them: a fork that cuts a sequence off, or
+ * copies a part of a page, leaves those of all the keys that the page (the one
+ * copied from) held, no smaller than its own keys', until a token comes to it. */
 typedef struct ane_kv8_bounds {
   int8_t *box;  /* [pages][kv_heads][2][head_dim], 16-byte aligned */
   int8_t *unit; /* [pages][kv_heads] */
@@ -247,6 +250,10 @@ int ane_kv8_bound(const ane_kv8_cache *cache, const ane_kv8_bounds *bounds, cons
  * for the rounding of q.  The first `first` pages and the last `recent` ones up
  * to the row's own position are always taken, then the largest scores, equal
  * ones from the lower page.  Pages that are not there are not taken.
+ * A row's own page has bounds of all the call's tokens in it, later ones than the
+ * row's too.  With recent >= 1 it is taken whatever they are, and a chunk's rows
+ * choose as they would token by token over the same codes; with recent 0 they may
+ * choose their own page for the sake of keys that they do not attend to.
  *
  * blocks: int32 [rows][kv_heads][count], the pages' places in the sequence's
  * table, rising, then -1.  Rows of no sequence are left as they are.
@@ -287,7 +294,8 @@ typedef struct ane_kv8_pool {
   int32_t nlayers; /* 1..1024 */
 } ane_kv8_pool;
 
-/* Brings the table of nseq sequences to their next step, with `new` tokens each
+/* Brings the table of nseq sequences (at most 65536, and 2^30 entries and 2^30
+ * tokens of a row, here and below) to their next step, with `new` tokens each
  * to come (news[i], or new_tokens where news is NULL; taken within [0, table's
  * room]):
  *  1. sequence i goes on from parents[i] (NULL: itself; outside [0, nseq): it
@@ -339,8 +347,9 @@ int ane_kv8_compact(const ane_kv8_pool *pool, const ane_kv8_compact_args *args, 
  * or another of the same layers, page_tokens, kv_heads and head_dim; pages may
  * differ), i < n: the 16-token units that hold their first tokens[i] tokens
  * (NULL: all; taken within [0, page_tokens]; 0: nothing), exponents and, where
- * both have them, bounds.  Ids outside the pools are passed over.  A page that
- * is written twice, or read and written, holds either; refs are not looked at. */
+ * both have them, bounds.  n at most 2^24.  Ids outside the pools are passed
+ * over.  A page that is written twice, or read and written, holds either; refs
+ * are not looked at. */
 typedef struct ane_kv8_copy_args {
   const int32_t *src, *dst, *tokens;
   int32_t n;

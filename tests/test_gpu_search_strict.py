@@ -70,3 +70,44 @@ def test_log_sums(rows, vocab, half):
         p = torch.exp(y - lse[:, None])
         bound = (19 + 3 * (p * (top[:, None] - y)).sum(1)) * 2.0 ** -24
         assert ((out.double() - want).abs() <= bound + want.abs() * 2.0 ** -24).all()
+
+
+def choices_of_a_chunk(recent, count=3):
+    """Of 90 tokens on 200, in one batch and token by token, over the same codes."""
+    P, held, new = 16, 200, 90
+    g = torch.Generator(device=DEV).manual_seed(recent)
+    cache = ane.KVCache8.Empty(30, 2, 64, P)
+    cache.k.view(torch.uint8).copy_(torch.randint(0, 0x70, cache.k.shape, dtype=torch.uint8, device=DEV, generator=g)
+                                    + 128 * torch.randint(0, 2, cache.k.shape, dtype=torch.uint8, device=DEV, generator=g))
+    cache.k_exp.fill_(-6)
+    table = torch.randperm(30, device=DEV, generator=g)[None, :20].int()
+    q = torch.randn((new, 4, 64), device=DEV, generator=g).half()
+    out = []
+    for whole in (True, False):
+        bounds = ane.KVBounds.Empty(cache)
+        bounds.Update(ane.KVBatch(table, ids([0]), ids([0, held]), held))
+        rows = []
+        for t in [0] if whole else range(new):
+            n = new if whole else 1
+            batch = ane.KVBatch(table, ids([held + t]), ids([0, n]), n)
+            bounds.Update(batch)
+            rows.append(bounds.Select(batch, q[t:t + n], count, first=0, recent=recent))
+        out.append(torch.cat(rows))
+    return out
+
+
+@pytest.mark.parametrize("recent", [1, 2])
+def test_rows_of_a_chunk_choose_as_token_by_token(recent):
+    whole, single = choices_of_a_chunk(recent)
+    assert torch.equal(whole, single)
+
+
+def test_rows_of_a_chunk_without_recent_pages_differ_by_their_own_page():
+    """Its bounds are of the chunk's later tokens too; of the other pages nothing
+    differs but what takes its place."""
+    whole, single = choices_of_a_chunk(0, count=1)
+    own = (200 + torch.arange(90, device=DEV))[:, None, None] // 16
+    differ = whole != single
+    assert differ.any()
+    # bounds that hold more keys promise no less: where the choices differ, the chunk's is the own page
+    assert (whole == own)[differ].all()
