@@ -24,10 +24,11 @@
 // to the lower beam, then the lower token.
 //
 // What bounds it.  Much to read: the first launch, HBM (640 rows of 60011 fp16
-// logits, 77 MB, in 18.6 us, 4.1 TB/s) and then the second one's chain of
-// accesses and barriers, 15.8 us for 16 beams (of them 4 for histories of 2564
-// ids).  Little: the two launches' chains (4 rows of 32000 fp32 logits 3.3 and 6.0
-// us, 64 rows 4.0 and 7.7).
+// logits, 77 MB, in 18.6 us, 4.1 TB/s; 512 rows of 32000 fp32, 66 MB, in 13.2, 5.0
+// TB/s) and then the second one's chain of accesses and barriers, 15.9 us for 16
+// beams (of them 4 for histories of 2564 ids), 9.5 for 8.  Little: the two
+// launches' chains (4 rows of 32000 fp32 logits 3.2 and 6.2 us, 64 rows 4.0 and
+// 7.6).
 #include <algorithm>
 
 #include "kv8.h"
@@ -578,9 +579,10 @@ __global__ __launch_bounds__(256) void move_kernel(BeamArgs a) {
 }
 
 // Loads of a wave in the first launch.  Of fp32 logits four, where that leaves
-// enough waves (512 rows of 32000: 21.2 us a step, with two 22.4; 64 rows 12.8
-// and 12.6); of fp16, which take as many instructions for half the bytes, two
-// (640 rows of 60011: 32.7 us, with four 33.5).
+// enough waves (512 rows of 32000: 20.3 us a step, with two 21.2; 272 rows 15.7
+// and 15.9, 256 15.7 and 15.6, 64 10.9 and 10.8; 4100 rows of 2049 24.5 and 26.4);
+// of fp16, which take as many instructions for half the bytes, two (640 rows of
+// 60011: 33.1 us, with four 33.8; 512 of 32000 18.4 and 18.8).
 int loads_of(int64_t rows, int vocab, bool half) { return !half && rows * (vocab / 512) >= 16384 ? 4 : 2; }
 
 struct Plan {
@@ -605,13 +607,16 @@ int plan(const char* op, int requests, int beams, int vocab, bool half, Plan* p)
 
 uint32_t magic(int n) { return (uint32_t)(((1ull << 32) + n - 1) / n); }
 
-// 512 threads for up to 8 beams, 1024 for more (before the second choice knew its
-// bar: 4 beams of 32000, 16 requests, 11.4 us a step, with 256 threads 12.4, with
-// 1024 12.3; 8 of 60011 14.9, 18.1 and 14.7; 12 of 32000 17.9 with 512, 17.1 with
-// 1024).
+// 512 threads for up to 8 beams, 1024 for more (4 beams of 32000, 16 requests, 10.9
+// us a step, with 256 threads 12.3, with 1024 11.3; one request 9.0, 10.1 and 10.1;
+// 2 of 2000, 64 requests, 9.5, 9.7 and 10.6; 8 of 60011, 8 requests, 15.3, 19.1 and
+// 14.6; 8 of 32000, one request, 11.1, 13.7 and 11.0; 9 of 32000 12.6 with 512 and
+// with 1024, 12 of 32000, 16 requests, 16.6 and 15.6, 16 of 60011, 40 requests, 38.1
+// and 33.1).
 int threads_of(int beams) { return beams <= 8 ? 512 : 1024; }
 // Histories of up to 8 words a thread move in the second launch (40 requests of
-// 16 beams and 2564 ids: 35.6 us a step, in a launch of their own 37.8).
+// 16 beams and 2564 ids: 32.9 us a step, in a launch of their own 35.4; 16 of 4 and
+// 4064 ids 11.9 and 13.6).
 bool moves_apart(int beams, int words) { return (int64_t)beams * words > kMoved * threads_of(beams); }
 
 template <typename T>

@@ -27,10 +27,11 @@
 //
 // Lists of pages (ane_kv8_attend_blocks) go the same ways, their keys numbered in
 // the list's order.  Single tokens: the chain again, the list's loads before the
-// page table's (one row of 12 heads and 32 pages of 64 5.6 us; 64 rows of 16
-// heads of 128 and 48 pages of 32 12.4 us, 47 MB).  Chunks: the vector
-// instructions, so the tokens of a tile share what they name (5 chunks, 841 rows
-// of 12 heads, 24 pages of 64 each out of up to 190: 25 us, a tile a row 48).
+// page table's (in a captured graph, one row of 12 heads and 32 pages of 64 8.4
+// us; 64 rows of 16 heads of 128 and 48 pages of 32 13.2 us, 47 MB).  Chunks: the
+// vector instructions, so the tokens of a tile share what they name (5 chunks, 841
+// rows of 12 heads, 24 pages of 64 each out of up to 190: 21.5 us, a tile a row
+// 48).
 #include <algorithm>
 #include <type_traits>
 

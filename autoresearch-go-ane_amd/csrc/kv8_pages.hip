@@ -8,10 +8,10 @@
 // (by id).
 //
 // What bounds it.  Copies: HBM, once pages fill it (compacting, 558 MB read and
-// written, 106 us, 5.3 TB/s; 3700 pages in 8 layers, 490 MB, 98 us, 5.0 TB/s).
-// Tables: chains of dependent accesses, and launches (a fork of 4 sequences 5.1 us
-// for the table and 3.5 for its copies; of 384 sequences of up to 8000 tokens 3.7
-// for the rows, 5.0 for the plan and 8.5 for the table and 63 MB of copies).
+// written, 105 us, 5.3 TB/s; 3700 pages in 8 layers, 490 MB, 98 us, 5.0 TB/s).
+// Tables: chains of dependent accesses, and launches (a fork of 4 sequences 4.6 us
+// for the table and 3.8 for its copies; of 384 sequences of up to 8000 tokens 3.6
+// for the rows, 5.0 for the plan and 8.4 for the table and 63 MB of copies).
 #include <algorithm>
 
 #include "kv8.h"
@@ -692,8 +692,12 @@ int check_table(const char* op, const int* table, int stride, int width, int nse
 
 int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }
 
-// Of larger pools the free pages are found by a block a chunk (100,000 pages, nine
-// tenths held, 12 us a fork, by the block of the plan 34; 20,000 12 and 11.7).
+// Of larger pools the free pages are found by a block a chunk: 13 us a fork (32
+// sequences of 8 pages) wherever they lie.  The block of the plan goes from chunk
+// to chunk until it has enough: 6 us where they lie all over the pool, but where
+// the lowest nine tenths are held 12 of 20,000 pages, 18 of 40,000, 37 of 100,000,
+// 100 of 300,000.  The host does not know which, so the line is where the worst is
+// equal.
 constexpr int kLarge = 20480;
 
 struct ForkPlan {

@@ -352,11 +352,11 @@ __device__ __forceinline__ void choose(Choice<CW>& c, const Each& each, int coun
 // none, so every histogram leaves fewer.
 //
 // What bounds it: the chain of ids, boxes and scores, then the narrowing's steps,
-// each an LDS round trip and a barrier (1 token of 20,000 keys, 4 heads, 313
-// pages: 7.2 us; 64 tokens of 3500 to 24,000, 2 heads of 128, pages of 32: 13 us
-// for 14 MB of boxes; 841 tokens of 4 heads in 5 chunks 9.9 us).  Narrowing by
-// halves, of bits or values, takes more such steps (21.6 us for the first with
-// update and attention, by histograms 19.2).
+// each an LDS round trip and a barrier (in a captured graph, 1 token of 20,000
+// keys, 4 heads, 313 pages: 7.0 us; 64 tokens of 3500 to 24,000, 2 heads of 128,
+// pages of 32: 12.1 us for 14 MB of boxes; 841 tokens of 4 heads in 5 chunks 9.8
+// us).  Narrowing by halves, of bits or values, takes more such steps (21.6 us for
+// the first with update and attention, by histograms 19.2).
 //
 // PART: a block leaves the scores of 64 NW pages of a token (and of those as many
 // blocks on) to choose_kernel.
