@@ -360,6 +360,8 @@ class LogitControls:
             hp, hr, hn, most = _matrix(op, "history", history, self._u16, index)
             if hn != rows:
                 _fail(op, f"history has {hn} rows, want {rows}")
+            if most >= 1 << 31:
+                _fail(op, f"history has {most} places a row, want at most {(1 << 31) - 1}")
             if lengths is None:
                 _fail(op, "history without lengths")
             np_ = self._vector("lengths", lengths, index, rows)

@@ -29,3 +29,10 @@ def test_history_of_nearly_2_to_the_31_ids(held):
     want[3] = 4.0 - 2 * 0.25 - 0.5
     assert torch.equal(out[0].cpu(), want)
     assert int(tokens) == 0
+
+
+def test_longer_history_is_refused():
+    history = torch.empty((1, 1 << 31), dtype=torch.int16, device=DEV)
+    controls = ane.LogitControls(100, repetition=torch.ones(1, device=DEV))
+    with pytest.raises(ane.EngineError, match="2147483648 places"):
+        controls.Apply(torch.zeros((1, 100), device=DEV), history, torch.zeros(1, dtype=torch.int32, device=DEV))
